@@ -1,0 +1,299 @@
+// Writing a step's new tokens into a 4-bit cache (bias, per-head norm and rotation on the way), and reading pages back.
+//
+// Formulas: x += bias; q and k are multiplied by rsqrt(mean(x^2) + eps) and their scales, head by head, then turned: with a, b the
+// partners of a pair, a' = a c - b s, b' = b c + a s, c and s from the row of the token's position in the tables (which carry any
+// scaling of the frequencies or multiplier), the pairs being (i, i + D / 2) or (2 i, 2 i + 1) of the first D channels; the others
+// pass.  All of it in float32; the queries are rounded once, at their store.  A group of 32 channels of a key or value is stored as
+//   offset = min(x) rounded down to bfloat16,  step = (max(x) - offset) / 15 rounded up to bfloat16,
+//   code = (x - offset) / step to the nearest whole number (ties to even), 0 where the step is 0,
+// so every value of the group lies between the first and the last code's value and is at most half a step from its own (the
+// roundings are directed for that).  A group that holds a value that is not finite reads back as NaN.
+//
+// A lane owns four consecutive channels, eight lanes a group, HD / 4 lanes a head.
+#include "packed.cuh"
+
+namespace zb {
+
+constexpr int PKW_WARPS = 4;
+
+struct PackedWriteArgs {
+  void* q_out;               // [T, nh * HD]
+  const void* qkv;           // [T, qkv_stride]
+  long long qkv_stride;
+  const float* bias;         // null, or [(nh + 2 nkv) HD]
+  const void* q_norm_w;      // null, or [HD]
+  const void* k_norm_w;
+  int norm_w_dtype;
+  float eps;
+  const float* cos_table;    // null, or [max_positions, half]
+  const float* sin_table;
+  int half, max_positions, pairs;
+  const int* positions;      // [T]
+  const int* token_row;      // [T]
+  unsigned char* packed;     // null: queries alone
+  const int* block_table;    // [num_rows, max_blocks]
+  int max_blocks, page_shift, num_pages, num_rows, tokens, nh, nkv;
+  int* status;
+};
+
+__device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void load_four(const __nv_bfloat16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = pk_low(v.x); x[1] = pk_high(v.x); x[2] = pk_low(v.y); x[3] = pk_high(v.y);
+}
+__device__ __forceinline__ void store_four(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void store_four(__nv_bfloat16* p, const float (&x)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+template <int HD, typename TI, typename TO>
+__global__ void __launch_bounds__(PKW_WARPS * 32)
+qk_norm_rope_packed_kernel(const PackedWriteArgs a) {
+  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, NG = HD / 32;      // (24 lanes: one head a warp)
+  wait_for_prior_grids();
+  let_dependents_launch();
+  const int lane = threadIdx.x & 31, sub = HEADS > 1 ? lane % LANES : lane;
+  const int t = blockIdx.x;
+  const int heads = a.packed != nullptr ? a.nh + 2 * a.nkv : a.nh;
+  const int head = (blockIdx.y * PKW_WARPS + (threadIdx.x >> 5)) * HEADS + (HEADS > 1 ? lane / LANES : 0);
+  const bool active = head < heads && sub < LANES;
+  const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + a.nkv, turns = (is_q || is_k) && a.cos_table != nullptr;
+  const int d = 4 * sub, pos = a.positions[t];
+  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (active) {
+    load_four(static_cast<const TI*>(a.qkv) + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(head) * HD + d, x);
+    if (a.bias != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += a.bias[head * HD + d + e];
+    }
+  }
+  const void* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
+  float ss = fmaf(x[0], x[0], fmaf(x[1], x[1], fmaf(x[2], x[2], x[3] * x[3])));
+#pragma unroll
+  for (int o = 1; o < (HEADS > 1 ? LANES : 32); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (active && w != nullptr) {
+    const float inv = rsqrtf(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] *= inv * load_scale(w, a.norm_w_dtype, d + e);
+  }
+  const bool pos_ok = pos >= 0 && (a.cos_table == nullptr || pos < a.max_positions);
+  if (!pos_ok && lane == 0) report(a.status, STATUS_POSITION_OUT_OF_RANGE, pos, t);
+  if (!pos_ok) return;                         // (the same for the whole CTA)
+  if (a.cos_table != nullptr) {
+    const float* c = a.cos_table + static_cast<size_t>(pos) * a.half;
+    const float* s = a.sin_table + static_cast<size_t>(pos) * a.half;
+    if (a.pairs) {
+      if (active && turns) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const int i = (d + e) / 2;
+          if (i < a.half) {
+            const float u = x[e], v = x[e + 1];
+            x[e] = u * c[i] - v * s[i];
+            x[e + 1] = v * c[i] + u * s[i];
+          }
+        }
+      }
+    } else {
+      // The partner's four channels: half a rotated part further, or back.
+      const bool first = d < a.half, mine = d < 2 * a.half;
+      const int from = lane + (!mine ? 0 : first ? a.half / 4 : -(a.half / 4));
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from);
+      if (active && turns && mine) {
+        float cs[4], sn[4];
+        load_four(c + (first ? d : d - a.half), cs);
+        load_four(s + (first ? d : d - a.half), sn);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = first ? x[e] * cs[e] - y[e] * sn[e] : x[e] * cs[e] + y[e] * sn[e];
+      }
+    }
+  }
+  if (active && is_q) {
+    store_four(static_cast<TO*>(a.q_out) + (static_cast<size_t>(t) * a.nh + head) * HD + d, x);
+  }
+  if (a.packed == nullptr) return;
+
+  // The group's least and largest value, and whether all are finite (eight lanes).
+  float low = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bad = bad || !(fabsf(x[e]) <= 3.402823466e38f);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  }
+  const unsigned any_bad = __ballot_sync(0xffffffffu, bad) >> (lane & 24) & 0xffu;
+  __nv_bfloat16 offset = __float2bfloat16_rd(low);
+  const float base = __bfloat162float(offset);
+  __nv_bfloat16 step = __float2bfloat16_ru(__fdiv_rn(high - base, 15.0f));
+  const float width = __bfloat162float(step);
+  unsigned codes = 0;
+  if (any_bad || !(width <= 3.0e38f)) {
+    offset = __ushort_as_bfloat16(0x7fc0);
+    step = __ushort_as_bfloat16(0);
+  } else if (width > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float code = fminf(rintf(__fdiv_rn(x[e] - base, width)), 15.0f);       // (never below 0: the offset is rounded down)
+      codes |= static_cast<unsigned>(code) << (4 * e);
+    }
+  }
+  const unsigned beside = __shfl_xor_sync(0xffffffffu, codes, 1);
+  if (!active || is_q) return;
+
+  const int row = a.token_row[t], kvh = is_k ? head - a.nh : head - a.nh - a.nkv;
+  const int block = pos >> a.page_shift;
+  if (row < 0 || row >= a.num_rows || block >= a.max_blocks) {
+    if (sub == 0) report(a.status, STATUS_ROW_OUT_OF_RANGE, row, t);
+    return;
+  }
+  const int page = a.block_table[static_cast<size_t>(row) * a.max_blocks + block];
+  if (page <= 0 || page >= a.num_pages) {      // page 0 is the null page and is never written
+    if (sub == 0) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, t);
+    return;
+  }
+  const int in_page = pos & ((1 << a.page_shift) - 1), p = in_page & (PK_BLOCK - 1);
+  unsigned char* dst = a.packed + (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + (in_page >> 4)) * pk_block_bytes(HD);
+  const int g = sub & 7, m = sub >> 3;          // the lane's place in its group, and the group
+  if (is_k) {
+    if ((g & 1) == 0) *reinterpret_cast<unsigned*>(dst + pk_key_word<HD>(p, g >> 1, m)) = codes | (beside << 16);
+    if (g == 0) {
+      *reinterpret_cast<__nv_bfloat16*>(dst + pk_key_step<HD>(p, m)) = step;
+      *reinterpret_cast<__nv_bfloat16*>(dst + pk_key_step<HD>(p, m) + 2 * NG) = offset;
+    }
+  } else {
+    *reinterpret_cast<unsigned short*>(dst + pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m) + 2 * (p & 1)) = static_cast<unsigned short>(codes);
+    if (g == 0) {
+      *reinterpret_cast<__nv_bfloat16*>(dst + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1)) = step;
+      *reinterpret_cast<__nv_bfloat16*>(dst + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1) + 4 * NG) = offset;
+    }
+  }
+}
+
+template <int HD, typename TI, typename TO>
+int packed_write_launch(const PackedWriteArgs& a, cudaStream_t stream) {
+  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1;
+  const int heads = a.packed != nullptr ? a.nh + 2 * a.nkv : a.nh;
+  const int per_block = PKW_WARPS * HEADS, across = (heads + per_block - 1) / per_block;
+  if (across > 65535) return ERR_UNSUPPORTED;
+  return launch_dependent(qk_norm_rope_packed_kernel<HD, TI, TO>, dim3(a.tokens, across), dim3(PKW_WARPS * 32), 0, stream, false, a);
+}
+template <int HD>
+int packed_write_types(const PackedWriteArgs& a, int in_dtype, int out_dtype, cudaStream_t stream) {
+  if (in_dtype == DTYPE_BF16 && out_dtype == DTYPE_BF16) return packed_write_launch<HD, __nv_bfloat16, __nv_bfloat16>(a, stream);
+  if (in_dtype == DTYPE_F32 && out_dtype == DTYPE_BF16) return packed_write_launch<HD, float, __nv_bfloat16>(a, stream);
+  if (in_dtype == DTYPE_F32 && out_dtype == DTYPE_F32) return packed_write_launch<HD, float, float>(a, stream);
+  return ERR_UNSUPPORTED;
+}
+
+// Page pages[i] -> out[i] ([2][nkv][page_size][HD], rows in their natural order): a thread eight channels of a position.
+template <int HD, typename T>
+__global__ void __launch_bounds__(256)
+unpack_pages_kernel(T* out, const unsigned char* packed, const int* pages, int n_pages, int num_pages, int nkv, int page_shift, int* status) {
+  constexpr int NG = HD / 32, PIECES = HD / 8;
+  wait_for_prior_grids();
+  let_dependents_launch();
+  const int page_size = 1 << page_shift;
+  const long long per_page = 2LL * nkv * page_size * PIECES;
+  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= per_page * n_pages) return;
+  const int n = static_cast<int>(i / per_page);
+  int rest = static_cast<int>(i - n * per_page);
+  const int c = rest % PIECES;
+  rest /= PIECES;
+  const int in_page = rest & (page_size - 1);
+  rest >>= page_shift;
+  const int kvh = rest % nkv, kind = rest / nkv;
+  const int page = pages[n];
+  if (page < 0 || page >= num_pages) {
+    if (i == n * per_page) report(status, STATUS_PAGE_OUT_OF_RANGE, page, n);
+    return;
+  }
+  const int p = in_page & (PK_BLOCK - 1), j = c >> 2;           // the channels 8 c .. 8 c + 7 lie in group j
+  const unsigned char* block = packed + (((static_cast<long long>(page) * nkv + kvh) << (page_shift - 4)) + (in_page >> 4)) * pk_block_bytes(HD);
+  unsigned word;
+  float step, offset;
+  if (kind == 0) {
+    word = *reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, j));
+    step = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(block + pk_key_step<HD>(p, j)));
+    offset = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(block + pk_key_step<HD>(p, j) + 2 * NG));
+  } else {
+    const int g = 2 * (c & 3), at = 2 * (p & 1);
+    const unsigned lo = *reinterpret_cast<const unsigned short*>(block + pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, j) + at);
+    const unsigned hi = *reinterpret_cast<const unsigned short*>(block + pk_value_word<HD>(p >> 3, g + 1, (p & 7) >> 1, j) + at);
+    word = lo | (hi << 16);
+    step = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(block + pk_value_step<HD>(p >> 1, j) + at));
+    offset = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(block + pk_value_step<HD>(p >> 1, j) + at + 4 * NG));
+  }
+  float x[2][4];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = fmaf(step, static_cast<float>(word >> (4 * e) & 15u), offset);
+  store_four(out + i * 8, x[0]);
+  store_four(out + i * 8 + 4, x[1]);
+}
+
+template <int HD>
+int unpack_launch(void* out, const unsigned char* packed, const int* pages, int n_pages, int num_pages, int nkv, int page_shift, int dtype,
+                  int* status, cudaStream_t stream) {
+  const long long per_page = 2LL * nkv * (HD / 8) << page_shift, blocks = (per_page * n_pages + 255) / 256;
+  if (per_page >= (1LL << 31) || blocks >= (1LL << 31)) return ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (dtype == DTYPE_BF16)
+    return launch_dependent(unpack_pages_kernel<HD, __nv_bfloat16>, grid, dim3(256), 0, stream, false, static_cast<__nv_bfloat16*>(out), packed,
+                            pages, n_pages, num_pages, nkv, page_shift, status);
+  return launch_dependent(unpack_pages_kernel<HD, float>, grid, dim3(256), 0, stream, false, static_cast<float*>(out), packed, pages, n_pages,
+                          num_pages, nkv, page_shift, status);
+}
+
+}  // namespace zb
+
+using namespace zb;
+
+// Bytes of a block of 16 positions of one head; 0 for a head size that the packed cache does not take.
+ZB_API int zb_packed_block_bytes(int hd) { return pk_head_dim_ok(hd) ? pk_block_bytes(hd) : 0; }
+
+// `packed` null: the queries alone (qkv then holds nh heads).  `pairs`: adjacent channels are partners, else halves of the rotated part.
+ZB_API int zb_qk_norm_rope_packed(void* q_out, const void* qkv, long long qkv_stride, const float* bias, const void* q_norm_w,
+                                  const void* k_norm_w, int norm_w_dtype, float eps, const float* cos_table, const float* sin_table, int half,
+                                  int max_positions, int pairs, const int* positions, const int* token_row, void* packed,
+                                  const int* block_table, int max_blocks, int page_size, int num_pages, int num_rows, int tokens, int nh,
+                                  int nkv, int hd, int in_dtype, int out_dtype, int* status, void* stream) {
+  const int page_shift = packed != nullptr ? pk_page_shift(page_size) : 4;
+  if (tokens < 0 || nh <= 0 || nkv <= 0 || page_shift < 0 || half < 0 || 2 * half > hd || (cos_table != nullptr && half == 0) ||
+      (!pairs && half % 4 != 0) || qkv_stride % 4 != 0)
+    return ERR_BAD_ARGUMENT;
+  if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
+  if (tokens == 0) return OK;
+  const PackedWriteArgs a = {q_out, qkv, qkv_stride, bias, q_norm_w, k_norm_w, norm_w_dtype, eps, cos_table, sin_table, half, max_positions,
+                             pairs, positions, token_row, static_cast<unsigned char*>(packed), block_table, max_blocks, page_shift, num_pages,
+                             num_rows, tokens, nh, nkv, status};
+  const auto s = static_cast<cudaStream_t>(stream);
+  switch (hd) {
+    case 32: return packed_write_types<32>(a, in_dtype, out_dtype, s);
+    case 64: return packed_write_types<64>(a, in_dtype, out_dtype, s);
+    case 96: return packed_write_types<96>(a, in_dtype, out_dtype, s);
+    default: return packed_write_types<128>(a, in_dtype, out_dtype, s);
+  }
+}
+
+ZB_API int zb_unpack_pages(void* out, const void* packed, const int* pages, int n_pages, int num_pages, int nkv, int page_size, int hd,
+                           int dtype, int* status, void* stream) {
+  const int page_shift = pk_page_shift(page_size);
+  if (n_pages < 0 || nkv <= 0 || page_shift < 0) return ERR_BAD_ARGUMENT;
+  if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
+  if (n_pages == 0) return OK;
+  const auto* from = static_cast<const unsigned char*>(packed);
+  const auto s = static_cast<cudaStream_t>(stream);
+  switch (hd) {
+    case 32: return unpack_launch<32>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
+    case 64: return unpack_launch<64>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
+    case 96: return unpack_launch<96>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
+    default: return unpack_launch<128>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
+  }
+}

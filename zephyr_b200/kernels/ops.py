@@ -115,6 +115,14 @@ _SIGNATURES = {
     "zb_qkv_halves": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int, c_float,
                       c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                       c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "zb_packed_block_bytes": [c_int],
+    "zb_qk_norm_rope_packed": [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_int,
+                               c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                               c_int, c_int, c_int, c_void_p, c_void_p],
+    "zb_unpack_pages": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "zb_paged_decode_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                               c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_int, c_void_p, c_void_p,
+                               c_void_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
                        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_head_mix": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -260,6 +268,8 @@ def library() -> ctypes.CDLL:
             lib.zb_paged_decode_scratch_floats.restype = c_longlong
             lib.zb_paged_decode_balanced_scratch_floats.argtypes = [c_int, c_int, c_int]
             lib.zb_paged_decode_balanced_scratch_floats.restype = c_longlong
+            lib.zb_paged_decode_packed_scratch_floats.argtypes = [c_int, c_int, c_int]
+            lib.zb_paged_decode_packed_scratch_floats.restype = c_longlong
             if os.environ.get("ZEPHYR_B200_DEPENDENT_LAUNCH", "1") == "0":
                 lib.zb_set_dependent_launch(0)
             _lib = lib
@@ -1320,6 +1330,177 @@ def qkv_halves(qkv: torch.Tensor, nh: int, nkv: int, kd: int, vd: int, norm: str
         _ptr(block_table), block_table.shape[1], page_size, pages, block_table.shape[0], T, nh, nkv, kd, vd,
         DTYPE_CODE[qkv.dtype], DTYPE_CODE[dtype], _ptr(status), _stream()), "qkv_halves")
     return q_out
+
+
+# ------------------------------------------------------------------------ the 4-bit cache
+PACKED_HEAD_DIMS = (32, 64, 96, 128)
+PACKED_BLOCK = 16           # positions per block
+
+
+def packed_block_bytes(hd: int) -> int:
+    """Bytes of a block of 16 positions' keys and values of one head in a 4-bit cache: a code of 4 bits a value, a step and an offset in
+    bfloat16 for every 32 channels of a key or value.  The layout is in csrc/packed.cuh."""
+    _require(hd in PACKED_HEAD_DIMS, f"a 4-bit cache takes head sizes {PACKED_HEAD_DIMS}, not {hd}")
+    return 20 * hd
+
+
+def packed_page_size_ok(page_size: int) -> bool:
+    return page_size >= PACKED_BLOCK and page_size & (page_size - 1) == 0
+
+
+def packed_cache_shape(pages: int, nkv: int, page_size: int, hd: int) -> tuple[int, int, int, int]:
+    """The shape of a 4-bit cache, a uint8 tensor (zeros are an empty cache)."""
+    _require(packed_page_size_ok(page_size), "the pages of a 4-bit cache hold a power of two of positions, 16 or more")
+    return pages, nkv, page_size // PACKED_BLOCK, packed_block_bytes(hd)
+
+
+def _check_packed(packed: torch.Tensor, nkv: int, hd: int) -> tuple[int, int]:
+    block = packed_block_bytes(hd)
+    _require(packed.dtype == torch.uint8 and packed.dim() == 4 and packed.is_contiguous() and packed.shape[1] == nkv
+             and packed.shape[3] == block, f"a 4-bit cache must be a contiguous uint8 [pages, kv_heads, page_size / 16, {block}] tensor")
+    page_size = packed.shape[2] * PACKED_BLOCK
+    _require(packed_page_size_ok(page_size), "the pages of a 4-bit cache hold a power of two of positions, 16 or more")
+    _require(packed.data_ptr() % 16 == 0, "a 4-bit cache must start on a 16-byte boundary")
+    return packed.shape[0], page_size
+
+
+def _same_device(*tensors: torch.Tensor | None) -> None:
+    """Kernels are launched on the current device's current stream: all they are given lies there."""
+    _cuda(*tensors)
+    current = torch.cuda.current_device()
+    for t in tensors:
+        _require(t is None or t.device.index == current, f"tensors of one call lie on the current device, cuda:{current}")
+
+
+def _check_status_word(status: torch.Tensor) -> None:
+    _require(status.dtype == torch.int32 and status.is_contiguous() and status.numel() >= 3, "status must be an int32 status word (new_status)")
+
+
+def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w: torch.Tensor | None, k_norm_w: torch.Tensor | None,
+                        eps: float, cos: torch.Tensor | None, sin: torch.Tensor | None, positions: torch.Tensor,
+                        token_row: torch.Tensor, packed: torch.Tensor | None, block_table: torch.Tensor, status: torch.Tensor,
+                        dtype: torch.dtype | None = None, layout: str = "halves", bias: torch.Tensor | None = None,
+                        q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``qk_norm_rope_cache`` into a 4-bit cache: bias, per-head norm of q and k, rotation, and the write of keys and values as codes of
+    4 bits with a step and an offset for every 32 channels.  Returns q as [T, nh*hd] in ``dtype`` (None: that of ``qkv``).
+
+    ``qkv`` [T, >= (nh + 2 nkv) hd], bfloat16 or float32 (``dtype`` may be bfloat16 for either, float32 for float32), rows on 16-byte
+    (float32) or 8-byte boundaries; without ``packed`` only the queries are made, from the first nh*hd columns.  ``cos`` / ``sin``:
+    float32 [positions, D / 2]; the first D channels of a head turn, in pairs (i, i + D / 2) with ``layout`` "halves" (D a multiple
+    of 8), (2i, 2i + 1) with "pairs"; any scaling of frequencies and any multiplier is in the tables.  ``bias``: float32, one value a
+    column.  A (row, position) comes once in a call."""
+    _i32(positions, token_row, block_table)
+    _check_status_word(status)
+    T = qkv.shape[0]
+    dtype = dtype or qkv.dtype
+    _require(hd in PACKED_HEAD_DIMS, f"a 4-bit cache takes head sizes {PACKED_HEAD_DIMS}, not {hd}")
+    _require(nh > 0 and nkv > 0, "head counts must be positive")
+    width = (nh + 2 * nkv) * hd if packed is not None else nh * hd
+    _require(qkv.dim() == 2 and qkv.shape[1] >= width and qkv.stride(1) == 1 and qkv.dtype in DTYPE_CODE,
+             "qkv must be [T, (heads + 2*kv_heads)*head_dim] with unit inner stride")
+    _require(T <= 1 or qkv.stride(0) >= width, "rows of qkv must not overlap")
+    _require(qkv.data_ptr() % (4 * qkv.element_size()) == 0 and qkv.stride(0) % 4 == 0,
+             "rows of qkv must start on boundaries of four values")
+    _require(dtype == torch.bfloat16 or (dtype == torch.float32 and qkv.dtype == torch.float32),
+             "the queries are bfloat16, or float32 where qkv is")
+    _require(positions.numel() == T and token_row.numel() == T and block_table.dim() == 2, "one position and row per token")
+    w_code = 0
+    if q_norm_w is not None or k_norm_w is not None:
+        _require(q_norm_w is not None and k_norm_w is not None and q_norm_w.dtype == k_norm_w.dtype,
+                 "q and k norm scales come together and share a type")
+        w_code = _scale_code(q_norm_w, hd)
+        _scale_code(k_norm_w, hd)
+    _require(layout in ("halves", "pairs"), "layout is 'halves' or 'pairs'")
+    half, max_positions = 0, 0
+    _require((cos is None) == (sin is None), "cos and sin come together")
+    if cos is not None:
+        _require(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2
+                 and cos.is_contiguous() and sin.is_contiguous(), "cos/sin must be contiguous float32 [positions, rotated / 2]")
+        max_positions, half = cos.shape
+        _require(0 < 2 * half <= hd and (layout == "pairs" or half % 4 == 0),
+                 "the rotated channels are part of the head, in halves a multiple of 8 of them")
+        _require(layout == "pairs" or (cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0), "cos/sin must start on 16-byte boundaries")
+    _require(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == width), f"bias: {width} float32 values")
+    pages, page_size = _check_packed(packed, nkv, hd) if packed is not None else (0, PACKED_BLOCK)
+    _same_device(qkv, positions, token_row, block_table, status, packed, q_norm_w, k_norm_w, cos, sin, bias, q_out)
+    if q_out is None:
+        q_out = torch.empty((T, nh * hd), dtype=dtype, device=qkv.device)
+    _require(q_out.shape == (T, nh * hd) and q_out.is_contiguous() and q_out.dtype == dtype and q_out.data_ptr() % 16 == 0, "q_out shape")
+    _check(library().zb_qk_norm_rope_packed(
+        _ptr(q_out), _ptr(qkv), qkv.stride(0) if T > 1 else width, _ptr(bias), _ptr(q_norm_w), _ptr(k_norm_w), w_code, float(eps), _ptr(cos), _ptr(sin),
+        half, max_positions, int(layout == "pairs"), _ptr(positions), _ptr(token_row), _ptr(packed), _ptr(block_table),
+        block_table.shape[1], page_size, pages, block_table.shape[0], T, nh, nkv, hd, DTYPE_CODE[qkv.dtype], DTYPE_CODE[dtype],
+        _ptr(status), _stream()), "qk_norm_rope_packed")
+    return q_out
+
+
+def unpack_pages(packed: torch.Tensor, pages: torch.Tensor, dtype: torch.dtype, status: torch.Tensor | None = None) -> torch.Tensor:
+    """What the given pages (int32) of a 4-bit cache stand for: [pages, 2 (keys, values), kv_heads, page_size, head_dim] in ``dtype``,
+    channels in their natural order.  A page outside the cache is reported, and its part of the result is not written."""
+    _i32(pages)
+    _require(dtype in DTYPE_CODE, "values are bfloat16 or float32")
+    _require(packed.dim() == 4 and packed.shape[3] % 20 == 0, "a 4-bit cache must be [pages, kv_heads, page_size / 16, 20 * head_dim]")
+    nkv, hd = packed.shape[1], packed.shape[3] // 20
+    num_pages, page_size = _check_packed(packed, nkv, hd)
+    if status is not None:
+        _check_status_word(status)
+    _same_device(packed, pages, status)
+    out = torch.empty((pages.numel(), 2, nkv, page_size, hd), dtype=dtype, device=packed.device)
+    _check(library().zb_unpack_pages(_ptr(out), _ptr(packed), _ptr(pages), pages.numel(), num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
+                                     _ptr(status) if status is not None else _device_status_pointer(packed.device), _stream()),
+           "unpack_pages")
+    return out
+
+
+def _packed_attention_args(q, packed, block_table, status, out, nh, nkv, hd, window, chunk, softcap, sinks) -> tuple[int, int]:
+    _check_status_word(status)
+    _require(nh > 0 and nkv > 0 and nh % nkv == 0, "head counts must be positive, heads divisible by kv_heads")
+    _require(q.dim() == 2 and q.is_contiguous() and q.shape[1] == nh * hd and q.dtype in DTYPE_CODE and q.data_ptr() % 16 == 0,
+             "q must be contiguous [T, heads*head_dim], bfloat16 or float32, on a 16-byte boundary")
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must match q")
+    _require(block_table.dim() == 2 and window >= 0 and chunk >= 0 and softcap >= 0.0,
+             "block_table is [rows, blocks]; window, chunk and softcap are not negative")
+    _require(sinks is None or (sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.numel() == nh),
+             "one float32 sink per query head")
+    return _check_packed(packed, nkv, hd)
+
+
+def packed_decode_plan(n_rows: int, nh: int, nkv: int, max_context: int) -> tuple[int, int]:
+    """How ``paged_decode_packed`` cuts its rows' contexts: (CTAs a (row, key/value head) pair, 0), or (0, CTAs) for balanced shares."""
+    pairs = n_rows * nkv * -(-nh // nkv // 8)
+    slots = 2 * _sm_count()
+    if pairs > slots:
+        return 0, slots
+    ranks = 1
+    while ranks < 8 and 2 * ranks * pairs <= slots and max_context > 256 * ranks:
+        ranks *= 2
+    return ranks, 0
+
+
+def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, row_q_start: torch.Tensor,
+                        row_ctx: torch.Tensor, max_context: int, nh: int, nkv: int, hd: int, window: int, scale: float,
+                        status: torch.Tensor, out: torch.Tensor, chunk: int = 0, sinks: torch.Tensor | None = None,
+                        softcap: float = 0.0, plan: tuple[int, int] | None = None) -> torch.Tensor:
+    """``paged_decode`` over a 4-bit cache: attention of rows with one new token each, whose key and value the cache holds already;
+    writes those tokens' rows of ``out``.  bfloat16; ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  ``max_context`` is at
+    least the longest context of the rows, the new token included.  ``plan``: as ``packed_decode_plan`` gives it (None: chosen by
+    that).  The scratch of a launch is the call's own."""
+    _i32(block_table, rows, row_q_start, row_ctx)
+    pages, page_size = _packed_attention_args(q, packed, block_table, status, out, nh, nkv, hd, window, chunk, softcap, sinks)
+    _require(q.dtype == torch.bfloat16, "the 4-bit decode attention takes bfloat16 queries")
+    _require(row_q_start.numel() >= block_table.shape[0] and row_ctx.numel() >= block_table.shape[0], "one start and context per row")
+    _same_device(q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
+    n_rows = rows.numel()
+    ranks, grid = plan or packed_decode_plan(n_rows, nh, nkv, min([max_context] + [n for n in (window, chunk) if n > 0]))
+    scratch = None
+    if ranks == 0 and n_rows > 0:
+        pairs = n_rows * nkv * -(-nh // nkv // 8)
+        scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(grid, pairs, hd)), dtype=torch.float32, device=q.device)
+    _check(library().zb_paged_decode_packed(
+        _ptr(out), _ptr(q), _ptr(packed), _ptr(block_table), block_table.shape[1], page_size, pages, block_table.shape[0], _ptr(rows),
+        n_rows, _ptr(row_q_start), _ptr(row_ctx), int(max_context), nh, nkv, hd, int(window), int(chunk), float(scale), float(softcap),
+        _ptr(sinks), ranks, grid, _ptr(scratch), _ptr(status), _stream()), "paged_decode_packed", 2 if ranks == 0 else 1)
+    return out
 
 
 def pool_blocks(kv_cache: torch.Tensor, block_table: torch.Tensor, pool_cache: torch.Tensor, pool_table: torch.Tensor,
