@@ -74,22 +74,28 @@ def pack(k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
     return blocks
 
 
-def attention(q, k, v, steps, pos, scale, window=0, chunk=0, sinks=None, softcap=0.0, rounded_keys=False):
-    """One row: q [tokens, nh, hd] at positions ``pos``, keys and values [positions, nkv, hd] (what the codes stand for), ``steps`` the keys'.
+def attention(q, keys, vals, pos, scale, window=0, chunk=0, sinks=None, softcap=0.0, rounded=False):
+    """One row: q [tokens, nh, hd] at positions ``pos``; keys and values as (codes, steps, offsets), [positions, nkv, hd] each.
     Returns the result [tokens, nh, hd] in float64, and how far a kernel may be from it.
 
-    The bound, with u = 2^-8 the most that a rounding to bfloat16 moves a value: values and probabilities are rounded once each,
-    2 u sum p |v|; the result is rounded, u |o|; a score may be off by d, which moves every weight by a factor of at most e^(2 d), 2 d
-    (1 + d) sum p |v| more.  d: the products of a group of 32 channels are sums of terms of up to 143 |q| in units of the step, added
-    up in float32 (34 additions and roundings, 2^-23 each for sums that are cut off), times step and scale; a kernel that rounds keys
-    to bfloat16 (``rounded_keys``) is off by scale sum u |q k| instead.  A bound on the scores does not stretch d."""
-    group = q.shape[1] // k.shape[1]
-    k, v, steps = (x.repeat_interleave(group, dim=1) for x in (k, v, steps))
+    The bound, with u = 2^-8 the most that a rounding to bfloat16 moves a value: the result is rounded, u |o|.  The single tokens'
+    kernel rounds a group's weights step p for codes that count from 8, and weights p for offset + 8 step: u sum p (|code - 8| step +
+    |offset + 8 step|).  A kernel with ``rounded`` operands rounds p and the values: 2 u sum p |v|.  A score that is off by d moves
+    every weight by a factor of at most e^(2 d): 2 d (1 + d) sum p |v| more.  d, with ``rounded`` operands: the keys are rounded,
+    scale u sum |q k|.  Else: a query channel is off by at most 2^-17 of the head's largest (two parts of 4 bits of a value scaled
+    to 128 .. 256, the second on a grid of 2^-9), which a code multiplies by up to 15 steps, and sums of up to 32 terms and of
+    groups are added up in float32, 40 roundings of at most 2^-23 of what is summed, codes and offsets apart."""
+    group = q.shape[1] // keys[0].shape[1]
+    (kc, ks, ko), (vc, vs, vo) = ([x.to(F64).repeat_interleave(group, dim=1) for x in part] for part in (keys, vals))
+    k, v = ko + ks * kc, vo + vs * vc
     s = torch.einsum("thd,khd->htk", q, k) * scale
-    if rounded_keys:
-        d = torch.einsum("thd,khd->htk", q.abs(), k.abs()) * scale * 2.0 ** -8
+    if rounded:
+        d = torch.einsum("thd,khd->htk", q.abs(), k.abs()) * scale * (2.0 ** -8 + 40 * 2.0 ** -23)
+        weight = 2 * v.abs()
     else:
-        d = torch.einsum("thd,khd->htk", q.abs(), steps) * scale * 143 * 34 * 2.0 ** -23
+        d = torch.einsum("thd,khd->htk", q.abs(), ks * kc + ko.abs()) * 40 * 2.0 ** -23
+        d = scale * (d + 15 * 2.0 ** -17 * q.abs().amax(-1).T.unsqueeze(-1) * ks.sum(-1).T.unsqueeze(1))
+        weight = (vc - 8).abs() * vs + (vo + 8 * vs).abs()
     d = d + 2.0 ** -20 * (1 + s.abs())
     if softcap:
         s = softcap * torch.tanh(s / softcap)
@@ -102,13 +108,12 @@ def attention(q, k, v, steps, pos, scale, window=0, chunk=0, sinks=None, softcap
     if chunk:
         hidden |= key < pos // chunk * chunk
     s = s.masked_fill(hidden, -math.inf)
-    d = d.masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+    d = d.masked_fill(hidden, 0.0).amax(-1, keepdim=True).permute(1, 0, 2)
     if sinks is not None:
         sink = sinks.to(F64).view(-1, 1, 1).expand(-1, s.shape[1], 1)
         p = torch.softmax(torch.cat([s, sink], -1), -1)[..., :-1]
     else:
         p = torch.softmax(s, -1)
     o = torch.einsum("htk,khd->thd", p, v)
-    spread = torch.einsum("htk,khd->thd", p, v.abs())
-    u, d = 2.0 ** -8, d.permute(1, 0, 2)
-    return o, (2 * u + 2 * d * (1 + d)) * spread + u * o.abs() + 1e-6
+    u = 2.0 ** -8
+    return o, u * torch.einsum("htk,khd->thd", p, weight) + 2 * d * (1 + d) * torch.einsum("htk,khd->thd", p, v.abs()) + u * o.abs() + 1e-6

@@ -19,7 +19,7 @@ def ops():
 
 
 def paged_case(device, nkv, hd, page, totals, seed, poison=True):
-    """A 4-bit cache with ``totals[r]`` positions of row r, its table, and what its keys and values stand for, row by row.  Positions
+    """A 4-bit cache with ``totals[r]`` positions of row r, its table, and its keys and values (codes, steps, offsets), row by row.  Positions
     behind a row's last, and unused pages, hold parameters that are NaN."""
     g = torch.Generator().manual_seed(seed)
     blocks = [-(-n // page) for n in totals]
@@ -37,9 +37,7 @@ def paged_case(device, nkv, hd, page, totals, seed, poison=True):
     rows = []
     for r, n in enumerate(totals):
         own = packed[table[r, :blocks[r]].long()]
-        k, v = ([x.permute(0, 2, 3, 1, 4).reshape(-1, nkv, hd)[:n] for x in plain.values(own)])
-        steps = plain.read(own)[0][1].permute(0, 2, 3, 1, 4).reshape(-1, nkv, hd)[:n]
-        rows.append((k, v, steps))
+        rows.append([[x.permute(0, 2, 3, 1, 4).reshape(-1, nkv, hd)[:n] for x in part] for part in plain.read(own)])
     if poison:
         for r, n in enumerate(totals):
             for pos in range(n, blocks[r] * page):
@@ -244,7 +242,7 @@ DECODES = [
 ]
 
 
-@pytest.mark.parametrize("plan", [None, (1, 0), (2, 0), (8, 0), (0, 3), (0, 296)])
+@pytest.mark.parametrize("plan", [None, (0, 1), (0, 2), (0, 8), (1, 3), (1, 296), (2, 1), (2, 148)])
 @pytest.mark.parametrize("nh,nkv,hd,page,ctx,masks", DECODES)
 def test_single_tokens(ops, cuda_device, nh, nkv, hd, page, ctx, masks, plan):
     n = len(ctx)
@@ -274,7 +272,7 @@ def test_many_rows(ops, cuda_device):
     packed, table, rows = paged_case(cuda_device, nkv, hd, 16, [c + 1 for c in ctx], 37)
     q = (torch.randn((n, nh * hd), generator=torch.Generator().manual_seed(41)) * 1.5).to(torch.bfloat16)
     outs = []
-    for plan in (None, (1, 0), (0, 17)):
+    for plan in (None, (0, 1), (1, 17), (2, 17)):
         status = ops.new_status(cuda_device)
         outs.append(ops.paged_decode_packed(q.to(cuda_device), packed, table, torch.arange(n, dtype=torch.int32, device=cuda_device), i32(cuda_device, list(range(n))),
                                             i32(cuda_device, ctx), max(ctx) + 1, nh, nkv, hd, 0, 0.125, status,
@@ -286,7 +284,7 @@ def test_many_rows(ops, cuda_device):
             assert ((out[r].cpu().double().view(1, nh, hd) - expected).abs() <= bound).all(), r
 
 
-@pytest.mark.parametrize("plan", [(1, 0), (4, 0), (0, 5)])
+@pytest.mark.parametrize("plan", [(0, 1), (0, 4), (1, 5), (2, 5)])
 def test_bad_rows_and_pages_are_reported(ops, cuda_device, plan):
     nh, nkv, hd, ctx = 4, 2, 64, [40, 90]
     packed, table, rows = paged_case(cuda_device, nkv, hd, 16, [c + 1 for c in ctx], 43)
@@ -317,7 +315,7 @@ def test_captured_and_on_a_side_stream(ops, cuda_device):
     outs = [torch.zeros_like(q) for q in qs]
     def call(i, out):
         return ops.paged_decode_packed(qs[i], packed, table, rows, starts, contexts, 701, nh, nkv, hd, 0, 0.09, status, out)
-    assert ops.packed_decode_plan(n, nh, nkv, 701)[0] == 0
+    assert ops.packed_decode_plan(n, nh, nkv, 701)[0] != ops.PACKED_CLUSTERS
     graphs = []
     for i in range(2):
         graph = torch.cuda.CUDAGraph()

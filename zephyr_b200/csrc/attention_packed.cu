@@ -1,34 +1,45 @@
 // Attention of single decoded tokens over the 4-bit cache, float32 scores, softmax and accumulation, bfloat16 queries.
 //
 // A step's cost is the bytes of its contexts, 20 HD for 16 positions of a head where bfloat16 pages have 64 HD, and what it takes to
-// turn their codes into operands.  So the layout (packed.cuh) is the operands': a warp takes 32 positions at a time, reads words from
-// shared memory that are fragments but for shifts and masks, and multiplies with m16n8k16, positions on the 16 rows and up to eight
-// query heads of the group on the 8 columns:
-//   scores   S[p, h] = sum_j step_pj (sum_{d in j} (128 + code_pd) q_hd) + (offset_pj - 128 step_pj) sum_{d in j} q_hd,
-//            the inner sums by the tensor cores from codes as they come out of the words, a group of 32 channels a sum of its own;
-//            steps and offsets join in float32, so that keys are not rounded again
-//   results  O[d, h] = sum_p v_pd P[p, h], values as offset + step * code in bfloat16 (one rounding), probabilities in bfloat16, as
-//            the other attention kernels have them
-// A warp copies its own tiles (two blocks of 16 positions, one bulk copy each, into a ring of its own, completion counted on an
-// mbarrier a tile), so no warp waits for another until the CTA's results meet.
+// turn their codes into operands: to keep up with the memory an SM has some ten instructions' room for every 100 bytes.  So the
+// layout (packed.cuh) is the operands', codes become numbers by masks alone, and steps and offsets join where there is little:
+//   codes    The low four bits of a bfloat16's low byte are, as a number, code * 2^-133, the next four 16 times that: bfloat16's
+//            subnormals and its first binade are one line.  A word of eight codes is four operand registers after four masks and a
+//            shift.  What multiplies them carries a power of two (2^60 in weights, a head's own in queries) that keeps products and
+//            sums far from float32's ends; all of it is exact.
+//   keys     S[h, p] = sum_j step_pj c_j[h, p] + sum_j offset_pj (sum_{d in j} q_hd), c_j being the product over the codes of a group
+//            of 32 channels.  The first sum in float32; the second a product of the position's parameters as they lie and the query
+//            sums as two bfloat16 parts.
+//   values   O[d, h] = sum_p code_pd (step_p P[p, h]), a group of channels at a time, its weights step_p P rounded to bfloat16 (the only
+//            rounding, 2^-9 of a weight; the weights of other attention kernels here have it too).  The offsets' part is sum_p (offset_p
+//            + 8 step_p) P - 8 sum_p (step_p P rounded): codes then count from 8, so that what the roundings of step_p P and of P do
+//            not share is small.
+// (Measured against it: values dequantised to bfloat16, 400 instructions for 16 positions of a head of 128, half again as far from
+// the exact result; products of e4m3 values, which this GPU turns into half-precision ones with conversions, 430.)
+// A warp copies its own tiles (two blocks of 16 positions) into a ring of its own, so no warp waits for another until the CTA's
+// results meet.  By 16-byte asynchronous copies: a bulk copy of a block from a lane of its own takes some 25 instructions, five such
+// copies a lane take ten.
 //
 // How contexts are cut: a cluster of CTAs takes a (row, key/value head) pair, its CTAs equal shares of the context, and they merge
-// over distributed shared memory; or, for many rows, CTAs take equal shares of all pairs' tiles laid end to end, and a second kernel
-// merges the pairs that were cut.  More than eight query heads a key/value head run as several pairs.
-//
-// Every wait is bounded and reports instead of hanging.
+// over distributed shared memory; or CTAs, or for many pairs the warps of the CTAs, each for itself, take equal shares of all pairs'
+// tiles laid end to end, and a second kernel merges the pairs that were cut.  More than eight query heads a key/value head run as
+// several pairs.
+#include <type_traits>
+
 #include "packed.cuh"
 #include "tcgen05.cuh"
 
 namespace zb {
 
 constexpr int PD_WARPS = 8;
-constexpr int PD_STAGES = 2;
+constexpr int PD_STAGES = 2;              // a power of two
 constexpr int PD_TILE = 32;              // positions per tile: a warp's unit of work
 constexpr int PD_HEADS = 8;              // query heads on the products' columns
-constexpr int PD_WAIT_LIMIT = 1 << 20;
 constexpr int PD_MERGE_WARPS = PD_WARPS / 2;
+constexpr float PD_LIFT = 60.0f;         // weights carry 2^60, results 2^(60 - 133)
 constexpr float PD_RESCALE = 8.0f;       // a running maximum (in powers of two) may be passed by this before sums are rescaled
+
+enum { PD_CLUSTERS, PD_CTA_SHARES, PD_WARP_SHARES };      // how contexts are cut
 
 struct PackedDecodeArgs {
   const __nv_bfloat16* q;        // [T, nh * hd]
@@ -38,8 +49,8 @@ struct PackedDecodeArgs {
   const int* rows;               // [n_rows] request rows that decode one token
   const int* row_q_start;        // [num_rows]
   const int* row_ctx;            // [num_rows] the new token's position
-  float* part_o;                 // [2 grid][8][hd]: partial results of pairs that are cut
-  float* part_ml;                // [2 grid][8][2]: their maxima and sums
+  float* part_o;                 // [2 shares][8][hd]: partial results of pairs that are cut
+  float* part_ml;                // [2 shares][8][2]: their maxima and sums
   int4* cuts;                    // [pairs]: first range, ranges, first tile, tiles per range
   int max_blocks, page_shift, num_pages, num_rows, n_rows;
   int nh, nkv, subs, window, chunk;
@@ -49,6 +60,51 @@ struct PackedDecodeArgs {
   float scale_over_cap;          // scale / softcap
   int* status;
 };
+
+__device__ __forceinline__ void cp_async_16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(smem)), "l"(gmem));
+}
+// The four operand registers of a word of eight codes (packed.cuh), as said above: nibbles 0 and 4, 1 and 5 (16 times), 2 and 6, 3 and 7
+// (16 times), the lower one in the lower half.
+__device__ __forceinline__ void pd_codes(unsigned word, unsigned (&r)[4]) {
+  const unsigned high = word >> 8;
+  r[0] = word & 0x000f000fu;
+  r[1] = word & 0x00f000f0u;
+  r[2] = high & 0x000f000fu;
+  r[3] = high & 0x00f000f0u;
+}
+// m16n8k8: an operand register for rows 0 .. 7 and one for rows 8 .. 15.
+__device__ __forceinline__ void mma_bf16_1688(float (&d)[4], const unsigned (&a)[2], unsigned b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(b));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The product of which rows 0 .. 7 alone are wanted (d[0], d[1]): the operand's other rows are whatever the registers hold.
+__device__ __forceinline__ void mma_rows8(float (&d)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
+  unsigned any, other;
+  asm("" : "=r"(any), "=r"(other));
+  const unsigned a[4] = {a0, any, a2, other};
+  mma_bf16(d, a, b0, b1);
+}
+// The same with nothing to add to.
+__device__ __forceinline__ void mma_bf16_1688_first(float (&d)[4], const unsigned (&a)[2], unsigned b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(b), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_bf16_16816_first(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// An 8 x 8 matrix of bfloat16 pairs (a lane has two neighbours of a row) with rows and columns exchanged.
+__device__ __forceinline__ unsigned turned(unsigned pair) {
+  unsigned r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(pair));
+  return r;
+}
 
 // A run of tiles of one pair.
 struct PdSegment {
@@ -71,33 +127,31 @@ __device__ __forceinline__ void pd_pair(const PackedDecodeArgs& a, int pair, int
 // The scratch slot of a pair's part in range `range`: a range has one for a pair that began before it, and one for a pair that begins in it.
 __device__ __forceinline__ int pd_slot(int pair_first, int range, int per_range) { return 2 * range + (pair_first < range * per_range ? 0 : 1); }
 
-template <int HD, bool BALANCED>
+template <int HD, int MODE>
 __global__ void __launch_bounds__(PD_WARPS * 32, 2)
 paged_decode_packed_kernel(const PackedDecodeArgs a) {
+  constexpr bool BALANCED = MODE != PD_CLUSTERS, WARPWISE = MODE == PD_WARP_SHARES;
+  constexpr int STRIDE = WARPWISE ? 1 : PD_WARPS;          // a segment's tiles are one warp's, or all warps' in turn
   constexpr int NG = HD / 32, BLOCK_BYTES = pk_block_bytes(HD), TILE_BYTES = 2 * BLOCK_BYTES;
   constexpr int OROW = HD + 4;             // padded: four heads' pieces of 16 bytes fall into different banks
   extern __shared__ __align__(128) unsigned char smem[];
   unsigned char* const rings = smem;                                                       // [warps][stages][2][20 HD]
   float* const merge_o = reinterpret_cast<float*>(rings + PD_WARPS * PD_STAGES * TILE_BYTES);    // [merge warps][8][OROW]
-  float* const merge_ml = merge_o + PD_MERGE_WARPS * PD_HEADS * OROW;                       // [warps][8][2]
-  float* const result_ml = merge_ml + PD_WARPS * PD_HEADS * 2;                              // [8][2]
-  int* const prefix = reinterpret_cast<int*>(result_ml + PD_HEADS * 2);                     // balanced: every row's first tile, n_rows + 1
-  __shared__ unsigned long long full_bars[PD_WARPS * PD_STAGES];
+  float* const merge_ml = merge_o + (WARPWISE ? 0 : PD_MERGE_WARPS * PD_HEADS * OROW);      // [warps][8][2]
+  float* const result_ml = merge_ml + (WARPWISE ? 0 : PD_WARPS * PD_HEADS * 2);             // [8][2]
+  int* const prefix = reinterpret_cast<int*>(result_ml + (WARPWISE ? 0 : PD_HEADS * 2));    // balanced: every row's first tile, n_rows + 1
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = a.nh / a.nkv, pairs_a_row = a.nkv * a.subs;
-  unsigned long long* const full = full_bars + warp * PD_STAGES;
+  const unsigned minus_even = g & 1 ? 0u : 0xbf80bf80u, minus_odd = g & 1 ? 0xbf80bf80u : 0u;      // -1 in the columns that count
+  const unsigned my_half = g & 1 ? 0x3244u : 0x1044u;        // a bfloat16 of a pair as float32 (__byte_perm)
   unsigned char* const ring = rings + warp * PD_STAGES * TILE_BYTES;
-  if (lane == 0) {
-    for (int s = 0; s < PD_STAGES; ++s) mbar_init(&full[s], 1);
-    fence_barrier_init();
-  }
   wait_for_prior_grids();          // queries, cache and the step's description: all of it earlier kernels' work
   let_dependents_launch();
-  __syncwarp();
 
   // ------------------------------------------------------------------ which tiles are this CTA's
   const unsigned ranks = BALANCED ? 1u : gridDim.x / (a.n_rows * pairs_a_row), rank = BALANCED ? 0u : blockIdx.x % ranks;
+  const int range = WARPWISE ? static_cast<int>(blockIdx.x) * PD_WARPS + warp : static_cast<int>(blockIdx.x);
   int per_range = 0, range_first = 0, range_end = 0;
   PdSegment whole;                 // not balanced: the only segment
   whole.count = 0;
@@ -129,8 +183,9 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     }
     __syncthreads();
     const int all = prefix[a.n_rows];
-    per_range = max(1, static_cast<int>((static_cast<long long>(all) + gridDim.x - 1) / gridDim.x));
-    const long long begin = static_cast<long long>(blockIdx.x) * per_range;
+    const int ranges = static_cast<int>(gridDim.x) * (WARPWISE ? PD_WARPS : 1);
+    per_range = max(1, static_cast<int>((static_cast<long long>(all) + ranges - 1) / ranges));
+    const long long begin = static_cast<long long>(range) * per_range;
     range_first = static_cast<int>(min(begin, static_cast<long long>(all)));
     range_end = static_cast<int>(min(begin + per_range, static_cast<long long>(all)));
   } else {
@@ -146,7 +201,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     whole.count = static_cast<int>(static_cast<long long>(count) * (rank + 1) / ranks) - from;
     whole.row = ok ? row : -1;
   }
-  // The segment that holds tile `at` of the CTA's range (balanced), and the tile behind it.
+  // The segment that holds tile `at` of the range (balanced), and the tile behind it.
   auto segment_at = [&](int at, PdSegment& s, int& pair_first, int& pair_tiles, int& pair) -> int {
     int lo = 0, hi = a.n_rows - 1;                       // the last row whose first tile is not behind `at`
     while (lo < hi) {
@@ -168,55 +223,58 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
   };
 
   // ------------------------------------------------------------------ the copies, which run ahead of the products
-  bool failed = false;
   PdSegment ahead;                // the segment the copies are in
-  int ahead_next = range_first, ahead_tile = warp;
+  int ahead_next = range_first, ahead_tile = WARPWISE ? 0 : warp, ahead_left = 0;
   ahead.count = 0;
-  bool more = true;
   if (!BALANCED) ahead = whole;
-  // To the warp's next tile; false behind the last.
-  auto next_tile = [&]() -> bool {
+  // Where the next 16 of the warp's tiles lie: lane 2 i + b has block b of the i-th, as a number of blocks from the cache's start.
+  // (A block of which nothing is seen is block 0, whose bytes nobody looks at.)
+  int my_block = 0;
+  bool more = true;
+  auto look_up = [&]() {
     while (ahead_tile >= ahead.count) {
-      if (!BALANCED || ahead_next >= range_end) return false;
+      if (!BALANCED || ahead_next >= range_end) {
+        more = false;
+        return;
+      }
       int x, y, z;
       ahead_next = segment_at(ahead_next, ahead, x, y, z);
-      ahead_tile = warp;
+      ahead_tile = WARPWISE ? 0 : warp;
     }
-    return true;
+    ahead_left = 16;
+    const int tile = ahead_tile + (lane >> 1) * STRIDE, pos = (ahead.first + tile) * PD_TILE + (lane & 1) * PK_BLOCK;
+    my_block = 0;
+    if (tile < ahead.count && pos < ahead.hi && pos + PK_BLOCK > ahead.lo) {
+      const int entry = pos >> a.page_shift;
+      const int page = entry < a.max_blocks ? a.block_table[static_cast<size_t>(ahead.row) * a.max_blocks + entry] : 0;
+      if (page <= 0 || page >= a.num_pages) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, ahead.row);
+      else my_block = ((page * a.nkv + ahead.kvh) << (a.page_shift - 4)) + ((pos & ((1 << a.page_shift) - 1)) >> 4);
+    }
   };
-  // The page of this lane's block (lanes 0 and 1 have one each) of the tile the copies are at, asked for a tile early.
-  int page = -1;
-  auto look_up = [&]() {
-    const int pos = (ahead.first + ahead_tile) * PD_TILE + lane * PK_BLOCK, block = pos >> a.page_shift;
-    page = -1;
-    if (lane < 2 && pos < ahead.hi && pos + PK_BLOCK > ahead.lo)
-      page = block < a.max_blocks ? a.block_table[static_cast<size_t>(ahead.row) * a.max_blocks + block] : 0;
-  };
+  const unsigned char* const from_lane = a.packed + lane * 16;
+  unsigned char* const to_lane = ring + lane * 16;
   int issued = 0;
   auto issue = [&]() {
-    const int stage = issued % PD_STAGES;
-    const bool copies = page >= 0;
-    const unsigned blocks = __popc(__ballot_sync(0xffffffffu, copies));
-    if (lane == 0) mbar_arrive_expect_tx(&full[stage], blocks * BLOCK_BYTES);
-    __syncwarp();
-    if (copies) {
-      if (page == 0 || page >= a.num_pages) {
-        report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, ahead.row);
-        page = 0;                    // the bytes must arrive all the same
+    if (more) {
+      unsigned char* const dst = to_lane + (issued & (PD_STAGES - 1)) * TILE_BYTES;
+      const int pair = 2 * (16 - ahead_left);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const unsigned char* const src = from_lane + static_cast<long long>(__shfl_sync(0xffffffffu, my_block, pair + b)) * BLOCK_BYTES;
+#pragma unroll
+        for (int c = 0; c < (BLOCK_BYTES + 511) / 512; ++c)
+          if ((c + 1) * 512 <= BLOCK_BYTES || lane * 16 + c * 512 < BLOCK_BYTES)
+            cp_async_16(dst + b * BLOCK_BYTES + c * 512, src + c * 512);
       }
-      const int pos = (ahead.first + ahead_tile) * PD_TILE + lane * PK_BLOCK, in_page = pos & ((1 << a.page_shift) - 1);
-      const long long block = ((static_cast<long long>(page) * a.nkv + ahead.kvh) << (a.page_shift - 4)) + (in_page >> 4);
-      bulk_copy_g2s(ring + stage * TILE_BYTES + lane * BLOCK_BYTES, a.packed + block * BLOCK_BYTES, BLOCK_BYTES, &full[stage]);
+      ++issued;
+      ahead_tile += STRIDE;
+      if (--ahead_left == 0 || ahead_tile >= ahead.count) look_up();
     }
-    ++issued;
-    ahead_tile += PD_WARPS;
-    more = next_tile();
-    if (more) look_up();
+    cp_async_commit();               // a group a tile, empty ones behind the last
   };
-  more = next_tile();
-  if (more) look_up();
+  look_up();
 #pragma unroll 1
-  for (int s = 0; s < PD_STAGES && more; ++s) issue();
+  for (int s = 0; s < PD_STAGES; ++s) issue();
 
   // ------------------------------------------------------------------ the segments
   int taken = 0, at = range_first;
@@ -233,85 +291,140 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     }
     const int heads = min(PD_HEADS, group - seg.sub * PD_HEADS), head0 = seg.kvh * group + seg.sub * PD_HEADS;
     const size_t token = seg.row >= 0 ? static_cast<size_t>(a.row_q_start[seg.row]) : 0;
-    // The queries as operands: lane (g, t) holds head g's channels 8 t .. 8 t + 7 of every group, in the order in which the words'
-    // nibbles come out (0 4, 1 5, 2 6, 3 7); and their sums over a group for heads 2 t, 2 t + 1.
-    unsigned qb[NG][4];
-    float2 q_sum[NG];
+    // The queries as operands, heads on the columns.  Lane (g, t) holds head g's channels 8 t .. 8 t + 7 of every group, in the order
+    // in which a key's word gives them, those that meet 16 times the code divided by that.
+    unsigned qb[NG][4], sums_b[2] = {0u, 0u};
+    float scale_c[2];                // what heads 2 t and 2 t + 1 multiply their first sums by: the power of two back, and the scale
+    const float scale_d = a.softcap_log2 > 0.0f ? 1.0f : a.scale_log2;
+    {
+      float x[NG][8], q_sum[NG], largest = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (g < heads && seg.row >= 0) v = *reinterpret_cast<const uint4*>(a.q + (token * a.nh + head0 + g) * HD + 32 * j + 8 * t);
-      qb[j][0] = __byte_perm(v.x, v.z, 0x5410); qb[j][1] = __byte_perm(v.x, v.z, 0x7632);
-      qb[j][2] = __byte_perm(v.y, v.w, 0x5410); qb[j][3] = __byte_perm(v.y, v.w, 0x7632);
-      const unsigned ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      mma_bf16_16816(c, ones, qb[j][0], qb[j][1]);
-      mma_bf16_16816(c, ones, qb[j][2], qb[j][3]);
-      q_sum[j] = make_float2(c[0], c[1]);
+      for (int j = 0; j < NG; ++j) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (g < heads && seg.row >= 0) v = *reinterpret_cast<const uint4*>(a.q + (token * a.nh + head0 + g) * HD + 32 * j + 8 * t);
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+        q_sum[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[j][i] = i & 1 ? pk_high(w[i >> 1]) : pk_low(w[i >> 1]);
+          q_sum[j] += x[j][i];
+          largest = fmaxf(largest, fabsf(x[j][i]));
+        }
+        q_sum[j] += __shfl_xor_sync(0xffffffffu, q_sum[j], 1);
+        q_sum[j] += __shfl_xor_sync(0xffffffffu, q_sum[j], 2);
+      }
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      // The largest query value to 2^119, or as near as a factor of 2^126 takes it.
+      const int shift = min(126, 246 - static_cast<int>(__float_as_uint(largest) >> 23));
+      const float up = __uint_as_float(static_cast<unsigned>(127 + shift) << 23);
+      const float back = largest <= 3.402823466e38f ? __uint_as_float(static_cast<unsigned>(127 - shift) << 23) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        qb[j][0] = pack_bf16(x[j][0] * up, x[j][4] * up);
+        qb[j][1] = pack_bf16(x[j][1] * up * 0.0625f, x[j][5] * up * 0.0625f);
+        qb[j][2] = pack_bf16(x[j][2] * up, x[j][6] * up);
+        qb[j][3] = pack_bf16(x[j][3] * up * 0.0625f, x[j][7] * up * 0.0625f);
+      }
+      // A position's parameters are the NG steps and NG offsets of a row; the offsets' columns get the sums, scaled.
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float rest = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) rest = 2 * t + u == NG + j ? q_sum[j] * scale_d : rest;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const __nv_bfloat16 part = __float2bfloat16_rn(rest);
+          sums_b[i] |= static_cast<unsigned>(__bfloat16_as_ushort(part)) << (16 * u);
+          rest -= __bfloat162float(part);
+        }
+      }
+      // (2^120 and 2^13: a code is read as code * 2^-133.)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) scale_c[h] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * h) * 1.329227995784916e36f * (8192.0f * scale_d);
     }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-    float o[2 * NG][4];
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};      // heads 2 t and 2 t + 1; the sums over this lane's positions
+    float o[2 * NG][4], rest_c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, weights_c[(NG + 1) / 2][4];
+#pragma unroll
+    for (int n = 0; n < (NG + 1) / 2; ++n) weights_c[n][0] = weights_c[n][1] = weights_c[n][2] = weights_c[n][3] = 0.0f;
 #pragma unroll
     for (int n = 0; n < 2 * NG; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
 #pragma unroll 1
-    for (int j0 = warp; j0 < seg.count; j0 += PD_WARPS) {
-      const int stage = taken % PD_STAGES;
-      if (!failed && !__all_sync(0xffffffffu, mbar_wait(&full[stage], (taken / PD_STAGES) & 1, PD_WAIT_LIMIT))) {
-        if (lane == 0) report(a.status, STATUS_COPY_TIMEOUT, j0, seg.row);
-        failed = true;
-      }
+    for (int j0 = WARPWISE ? 0 : warp; j0 < seg.count; j0 += STRIDE) {
+      const int stage = taken & (PD_STAGES - 1);
       ++taken;
-      if (failed) continue;
+      cp_async_wait<PD_STAGES - 1>();
+      __syncwarp();                // every lane's part of the tile is there
       const unsigned char* const tile = ring + stage * TILE_BYTES;
       const int pos0 = (seg.first + j0) * PD_TILE;
-      const bool edge = pos0 < seg.lo || pos0 + PD_TILE > seg.hi;
+      auto work = [&](auto at_edge) {
+      constexpr bool edge = decltype(at_edge)::value;
 
-      // Scores: s[b][c] of positions 16 b + g (+ 8 for c >= 2), heads 2 t + (c & 1).
+      // Scores in powers of two: s[b][c] of position 16 b + g (+ 8 for c >= 2) and head 2 t + (c & 1).
       float s[2][4];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const unsigned char* const block = tile + b * BLOCK_BYTES;
-        unsigned w0[NG], w1[NG];
+        unsigned w0[NG], w1[NG], steps[2][(NG + 1) / 2];
         pk_load_words(w0, block + pk_key_word<HD>(g, t, 0));
         pk_load_words(w1, block + pk_key_word<HD>(g + 8, t, 0));
-        unsigned params[2][NG];              // steps 0 .. NG - 1, offsets 0 .. NG - 1 of the two positions, in pairs
-        pk_load_words(params[0], block + pk_key_step<HD>(g, 0));
-        pk_load_words(params[1], block + pk_key_step<HD>(g + 8, 0));
-        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const unsigned char* const from = block + pk_key_step<HD>(g + 8 * u, 0);
+          if constexpr (NG == 3) {           // (rows of 12 bytes: no boundary for two words at once)
+            steps[u][0] = *reinterpret_cast<const unsigned*>(from);
+            steps[u][1] = *reinterpret_cast<const unsigned*>(from + 4);
+          } else {
+            pk_load_words(steps[u], from);
+          }
+        }
+        unsigned params[2] = {0u, 0u};
+        if (NG == 4 || t < NG) {
+          params[0] = *reinterpret_cast<const unsigned*>(block + pk_key_step<HD>(g, 0) + 4 * t);
+          params[1] = *reinterpret_cast<const unsigned*>(block + pk_key_step<HD>(g + 8, 0) + 4 * t);
+        }
+        float d[4], sum[4];
+        mma_bf16_1688_first(d, params, sums_b[1]);
+        mma_bf16_1688(d, params, sums_b[0]);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const unsigned k0[4] = {pk_biased_codes<0>(w0[j]), pk_biased_codes<0>(w1[j]), pk_biased_codes<1>(w0[j]), pk_biased_codes<1>(w1[j])};
-          const unsigned k1[4] = {pk_biased_codes<2>(w0[j]), pk_biased_codes<2>(w1[j]), pk_biased_codes<3>(w0[j]), pk_biased_codes<3>(w1[j])};
-          mma_bf16_16816(c, k0, qb[j][0], qb[j][1]);
-          mma_bf16_16816(c, k1, qb[j][2], qb[j][3]);
+          float c[4];
+          unsigned k0[4], k1[4];
+          pd_codes(w0[j], k0);
+          pd_codes(w1[j], k1);
+          const unsigned a0[4] = {k0[0], k1[0], k0[1], k1[1]}, a1[4] = {k0[2], k1[2], k0[3], k1[3]};
+          mma_bf16_16816_first(c, a0, qb[j][0], qb[j][1]);
+          mma_bf16(c, a1, qb[j][2], qb[j][3]);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            auto param = [&](int i) { return i & 1 ? pk_high(params[u][i >> 1]) : pk_low(params[u][i >> 1]); };
-            const float step = param(j), offset = param(NG + j);
-            const float base = fmaf(-128.0f, step, offset);
-            sum[u] = fma_pair(make_float2(step, step), make_float2(c[2 * u], c[2 * u + 1]), sum[u]);
-            sum[u] = fma_pair(make_float2(base, base), q_sum[j], sum[u]);
+          for (int i = 0; i < 4; ++i) {
+            const unsigned pair = steps[i >> 1][j >> 1];
+            const float step = j & 1 ? pk_high(pair) : pk_low(pair);
+            sum[i] = j == 0 ? step * c[i] : fmaf(step, c[i], sum[i]);
           }
         }
-        s[b][0] = sum[0].x; s[b][1] = sum[0].y; s[b][2] = sum[1].x; s[b][3] = sum[1].y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b][i] = fmaf(sum[i], scale_c[i & 1], d[i]);
       }
-      float top[2] = {-INFINITY, -INFINITY};
+      if (a.softcap_log2 > 0.0f) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v = a.softcap_log2 > 0.0f ? a.softcap_log2 * tanhf(s[b][c] * a.scale_over_cap) : s[b][c] * a.scale_log2;
-          if (edge) {
+          for (int c = 0; c < 4; ++c) s[b][c] = a.softcap_log2 * tanhf(s[b][c] * a.scale_over_cap);
+      }
+      if constexpr (edge) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
             const int pos = pos0 + 16 * b + g + 4 * (c & 2);
-            if (pos < seg.lo || pos >= seg.hi) v = -INFINITY;
+            if (pos < seg.lo || pos >= seg.hi) s[b][c] = -INFINITY;
           }
-          s[b][c] = v;
-          top[c & 1] = fmaxf(top[c & 1], v);
-        }
       }
       // The shift follows the maximum only where some position passes it by much: no shuffles in most tiles.
+      float top[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
       if (__any_sync(0xffffffffu, top[0] > m_run[0] + PD_RESCALE || top[1] > m_run[1] + PD_RESCALE)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -325,9 +438,19 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
             o[n][h] *= factor;
             o[n][2 + h] *= factor;
           }
+          // Those two have a head a row.
+          const float other = __shfl_sync(0xffffffffu, factor, g >> 1);
+          if ((g & 1) == h) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              rest_c[c] *= other;
+#pragma unroll
+              for (int n = 0; n < (NG + 1) / 2; ++n) weights_c[n][c] *= other;
+            }
+          }
         }
       }
-      const float shift[2] = {m_run[0] == -INFINITY ? 0.0f : m_run[0], m_run[1] == -INFINITY ? 0.0f : m_run[1]};
+      const float shift[2] = {m_run[0] == -INFINITY ? 0.0f : m_run[0] - PD_LIFT, m_run[1] == -INFINITY ? 0.0f : m_run[1] - PD_LIFT};
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const unsigned char* const block = tile + b * BLOCK_BYTES;
@@ -337,55 +460,122 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(p[c]) : "f"(s[b][c] - shift[c & 1]));
           l_run[c & 1] += p[c];
         }
-        // P's rows are positions, the product wants them on its inner dimension: 8 x 8 pieces change sides.
-        unsigned p0 = pack_bf16(p[0], p[1]), p1 = pack_bf16(p[2], p[3]);
-        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;\n" : "+r"(p0));
-        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;\n" : "+r"(p1));
-        unsigned v0[NG], v1[NG], steps0[NG], steps1[NG], offsets0[NG], offsets1[NG];
+        // This lane's positions' steps: words of the pairs g / 2 and g / 2 + 4, the half that g says.
+        unsigned v0[NG], v1[NG], steps0[NG], steps1[NG];
         pk_load_words(v0, block + pk_value_word<HD>(0, g, t, 0));
         pk_load_words(v1, block + pk_value_word<HD>(1, g, t, 0));
-        pk_load_words(steps0, block + pk_value_step<HD>(t, 0));
-        pk_load_words(offsets0, block + pk_value_step<HD>(t, 0) + 4 * NG);
-        pk_load_words(steps1, block + pk_value_step<HD>(t + 4, 0));
-        pk_load_words(offsets1, block + pk_value_step<HD>(t + 4, 0) + 4 * NG);
-        if (edge) {
-          // Positions outside hold what was there before, a NaN maybe: their values become zeros.
-          auto keep = [&](int pos) {
-            return (pos >= seg.lo && pos < seg.hi ? 0x0000ffffu : 0u) | (pos + 1 >= seg.lo && pos + 1 < seg.hi ? 0xffff0000u : 0u);
-          };
-          const unsigned keep0 = keep(pos0 + 16 * b + 2 * t), keep1 = keep(pos0 + 16 * b + 8 + 2 * t);
+        pk_load_words(steps0, block + pk_value_step<HD>(g >> 1, 0));
+        pk_load_words(steps1, block + pk_value_step<HD>((g >> 1) + 4, 0));
+        // Columns 0 .. NG - 1: steps, NG .. 2 NG - 1: offsets.
+        unsigned params[2] = {0u, 0u};
+        if (NG == 4 || g < 2 * NG) {
+          params[0] = *reinterpret_cast<const unsigned*>(block + pk_value_step<HD>(t, 0) + 4 * g);
+          params[1] = *reinterpret_cast<const unsigned*>(block + pk_value_step<HD>(t + 4, 0) + 4 * g);
+        }
+        if constexpr (edge) {
+          // Positions outside hold what was there before, a NaN maybe: their parameters become zeros.
+          auto seen = [&](int pos) { return pos >= seg.lo && pos < seg.hi; };
+          auto keep = [&](int pos) { return (seen(pos) ? 0x0000ffffu : 0u) | (seen(pos + 1) ? 0xffff0000u : 0u); };
+          const unsigned keep0 = seen(pos0 + 16 * b + g) ? 0xffffffffu : 0u, keep1 = seen(pos0 + 16 * b + 8 + g) ? 0xffffffffu : 0u;
 #pragma unroll
           for (int m = 0; m < NG; ++m) {
-            steps0[m] &= keep0; offsets0[m] &= keep0;
-            steps1[m] &= keep1; offsets1[m] &= keep1;
+            steps0[m] &= keep0;
+            steps1[m] &= keep1;
           }
+          params[0] &= keep(pos0 + 16 * b + 2 * t);
+          params[1] &= keep(pos0 + 16 * b + 8 + 2 * t);
         }
+        // Weights have positions on rows, the products want them on their inner dimension: 8 x 8 pieces change sides.
+        mma_rows8(rest_c, turned(pack_bf16(p[0], p[1])), turned(pack_bf16(p[2], p[3])), params[0], params[1]);
+        unsigned w[NG + (NG & 1)][2];
+        if constexpr (NG & 1) w[NG][0] = w[NG][1] = 0u;
 #pragma unroll
         for (int m = 0; m < NG; ++m) {
-          const unsigned a0[4] = {pk_values<0>(v0[m], steps0[m], offsets0[m]), pk_values<1>(v0[m], steps0[m], offsets0[m]),
-                                  pk_values<0>(v1[m], steps1[m], offsets1[m]), pk_values<1>(v1[m], steps1[m], offsets1[m])};
-          const unsigned a1[4] = {pk_values<2>(v0[m], steps0[m], offsets0[m]), pk_values<3>(v0[m], steps0[m], offsets0[m]),
-                                  pk_values<2>(v1[m], steps1[m], offsets1[m]), pk_values<3>(v1[m], steps1[m], offsets1[m])};
-          mma_bf16_16816(o[2 * m], a0, p0, p1);
-          mma_bf16_16816(o[2 * m + 1], a1, p0, p1);
+          const float step0 = __uint_as_float(__byte_perm(steps0[m], 0u, my_half)), step1 = __uint_as_float(__byte_perm(steps1[m], 0u, my_half));
+          w[m][0] = turned(pack_bf16(p[0] * step0, p[1] * step0));
+          w[m][1] = turned(pack_bf16(p[2] * step1, p[3] * step1));
+          // Channels 32 m + 4 g (rows g) and + 1 (rows g + 8, 16 times the code), then + 2 and + 3.
+          unsigned c0[4], c1[4];
+          pd_codes(v0[m], c0);
+          pd_codes(v1[m], c1);
+          const unsigned a0[4] = {c0[0], c0[1], c1[0], c1[1]}, a1[4] = {c0[2], c0[3], c1[2], c1[3]};
+          mma_bf16(o[2 * m], a0, w[m][0], w[m][1]);
+          mma_bf16(o[2 * m + 1], a1, w[m][0], w[m][1]);
+        }
+        // The sums of the rounded weights, two groups of channels a product: positions 0 .. 7 on rows 0 .. 7 and 8 .. 15 on the
+        // others, one group on the inner dimension's first half and on even columns, the other on the second and on odd ones.
+#pragma unroll
+        for (int m = 0; m < NG; m += 2) {
+          const unsigned both[4] = {w[m][0], w[m][1], w[m + 1][0], w[m + 1][1]};
+          mma_bf16(weights_c[m / 2], both, minus_even, minus_odd);
         }
       }
+      };
+      if (pos0 < seg.lo || pos0 + PD_TILE > seg.hi) work(std::true_type{});
+      else work(std::false_type{});
       __syncwarp();                // every lane has read the tile: its place may be filled again
-      if (more) issue();
+      issue();
     }
-
-    // ---------------------------------------------------------------- the warps' results meet
+    // The weights' power of two out, and the offsets' part in.  Lane (g, t): rest_c has sum step P and sum offset P of head g, columns
+    // 2 t and 2 t + 1 of the parameters; weights_c -1 times the sums of the rounded weights of head g, a half of the positions each.
+    constexpr float DOWN = 8.673617379884035e-19f, CODE_UP = 9.44473296573929e21f;        // 2^-60, 2^73
+    l_run[0] *= DOWN;
+    l_run[1] *= DOWN;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int m = 0; m < NG; ++m) {
+      const float weights = weights_c[m / 2][m & 1] + weights_c[m / 2][2 + (m & 1)];
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-      if (g == 0) {
-        merge_ml[(warp * PD_HEADS + 2 * t + h) * 2] = m_run[h];
-        merge_ml[(warp * PD_HEADS + 2 * t + h) * 2 + 1] = l_run[h];
+      for (int h = 0; h < 2; ++h) {
+        const int row = 4 * (2 * t + h);          // the lanes of head 2 t + h
+        const float steps = __shfl_sync(0xffffffffu, rest_c[m & 1], row + m / 2);
+        const float offsets = __shfl_sync(0xffffffffu, rest_c[(NG + m) & 1], row + (NG + m) / 2);
+        const float extra = DOWN * fmaf(8.0f, steps + __shfl_sync(0xffffffffu, weights, row), offsets);
+#pragma unroll
+        for (int n = 2 * m; n < 2 * m + 2; ++n) {
+          o[n][h] = fmaf(o[n][h], CODE_UP, extra);
+          o[n][2 + h] = fmaf(o[n][2 + h], CODE_UP / 16.0f, extra);
+        }
       }
     }
+
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
+    const bool cut = BALANCED ? seg.count < pair_tiles : ranks > 1;
+    if (BALANCED && at0 == pair_first && (WARPWISE ? lane : threadIdx.x) == 0) {
+      const int first = pair_first / per_range, last = (pair_first + pair_tiles - 1) / per_range;
+      a.cuts[pair] = make_int4(first, last - first + 1, pair_first, per_range);
+    }
+    if constexpr (WARPWISE) {
+      // The warp's own result, or its part of one: four channels of a group lie in a lane's two products.
+      const size_t slot = static_cast<size_t>(pd_slot(pair_first, range, per_range)) * PD_HEADS;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int head = 2 * t + h;
+        if (head >= heads) continue;
+        if (cut) {
+          if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (slot + head) * 2) = make_float2(m_run[h], l_run[h]);
+#pragma unroll
+          for (int m = 0; m < NG; ++m)
+            *reinterpret_cast<float4*>(a.part_o + (slot + head) * HD + 32 * m + 4 * g) =
+                make_float4(o[2 * m][h], o[2 * m][2 + h], o[2 * m + 1][h], o[2 * m + 1][2 + h]);
+        } else {
+          const float sum = l_run[h] + (a.sinks != nullptr ? exp2f(a.sinks[head0 + head] * 1.4426950408889634f - m_run[h]) : 0.0f);
+          const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+          for (int m = 0; m < NG; ++m)
+            *reinterpret_cast<uint2*>(a.out + (token * a.nh + head0 + head) * HD + 32 * m + 4 * g) =
+                make_uint2(pack_bf16(o[2 * m][h] * inv, o[2 * m][2 + h] * inv), pack_bf16(o[2 * m + 1][h] * inv, o[2 * m + 1][2 + h] * inv));
+        }
+      }
+    } else {
+    // ---------------------------------------------------------------- the warps' results meet
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * PD_HEADS + 2 * t + h) * 2) = make_float2(m_run[h], l_run[h]);
     __syncthreads();
-    float factor[2];
+    float factor[2];                 // of heads 2 t, 2 t + 1
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float all = -INFINITY;
@@ -418,7 +608,6 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     }
     __syncthreads();
     // Four values of a head a thread: the sum of the four warps' sums, the pair's maximum and sum of exponentials.
-    const bool cut = BALANCED ? seg.count < pair_tiles : ranks > 1;
     for (int e = threadIdx.x; e < PD_HEADS * HD / 4; e += PD_WARPS * 32) {
       const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
       float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -443,7 +632,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
               make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
         }
       } else if (BALANCED) {
-        const int slot = pd_slot(pair_first, blockIdx.x, per_range);
+        const int slot = pd_slot(pair_first, range, per_range);
         *reinterpret_cast<float4*>(a.part_o + (static_cast<size_t>(slot) * PD_HEADS + h) * HD + d) = x;
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (static_cast<size_t>(slot) * PD_HEADS + h) * 2) = make_float2(top, sum);
       } else {
@@ -454,10 +643,6 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           result_ml[2 * h + 1] = sum;
         }
       }
-    }
-    if (BALANCED && at0 == pair_first && threadIdx.x == 0) {
-      const int first = pair_first / per_range, last = (pair_first + pair_tiles - 1) / per_range;
-      a.cuts[pair] = make_int4(first, last - first + 1, pair_first, per_range);
     }
     if (BALANCED) __syncthreads();           // the next segment writes where these sums lay
     if (!BALANCED && ranks > 1) {
@@ -495,48 +680,69 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
       __syncwarp();
       cluster_sync_all();                    // nobody leaves while its memory is read
     }
+    }
   }
-  if (failed) let_copies_land();
 }
 
-// The pairs whose tiles lie in several ranges: their parts meet.  A CTA a pair, a thread four values of a head.
+// The pairs whose tiles lie in several ranges: their parts meet.  A CTA a pair and head; threads are columns of four channels times
+// groups that share the parts.
 template <int HD>
-__global__ void __launch_bounds__(PD_HEADS * HD / 4)
+__global__ void __launch_bounds__(256)
 paged_decode_packed_merge_kernel(const PackedDecodeArgs a) {
+  constexpr int COLUMNS = HD / 4, GROUPS = 256 / COLUMNS;
+  __shared__ float4 sums[GROUPS][COLUMNS];
+  __shared__ float of_warp[8], totals[GROUPS];
   wait_for_prior_grids();
   let_dependents_launch();
-  const int pair = blockIdx.x, pairs_a_row = a.nkv * a.subs, group = a.nh / a.nkv;
+  const int pair = blockIdx.x, h = blockIdx.y, pairs_a_row = a.nkv * a.subs, group = a.nh / a.nkv;
   const int4 cut = a.cuts[pair];
-  if (cut.y <= 1) return;
-  const int row = a.rows[pair / pairs_a_row], p = pair % pairs_a_row, sub = p % a.subs, kvh = p / a.subs;
-  const int heads = min(PD_HEADS, group - sub * PD_HEADS), head0 = kvh * group + sub * PD_HEADS;
-  const int h = threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
-  if (h >= heads) return;
-  float top = -INFINITY, sum = 0.0f;
-  for (int i = 0; i < cut.y; ++i)
-    top = fmaxf(top, a.part_ml[(static_cast<size_t>(pd_slot(cut.z, cut.x + i, cut.w)) * PD_HEADS + h) * 2]);
-  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int p = pair % pairs_a_row, sub = p % a.subs, kvh = p / a.subs;
+  if (cut.y <= 1 || h >= min(PD_HEADS, group - sub * PD_HEADS)) return;
+  auto at = [&](int i) { return static_cast<size_t>(pd_slot(cut.z, cut.x + i, cut.w)) * PD_HEADS + h; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < cut.y; i += 256) top = fmaxf(top, a.part_ml[at(i) * 2]);
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, of_warp[w]);
+  const int column = threadIdx.x % COLUMNS, own = threadIdx.x / COLUMNS;
+  if (own < GROUPS) {
+    float sum = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int i = 0; i < cut.y; ++i) {
-    const size_t at = static_cast<size_t>(pd_slot(cut.z, cut.x + i, cut.w)) * PD_HEADS + h;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-    const float4 y = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
-    const float f = ml.x > -INFINITY ? exp2f(ml.x - top) : 0.0f;
-    sum += ml.y * f;
-    x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
+    for (int i = own; i < cut.y; i += GROUPS) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(i) * 2);
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + at(i) * HD + 4 * column);
+      const float f = ml.x > -INFINITY ? exp2f(ml.x - top) : 0.0f;
+      sum += ml.y * f;
+      x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
+    }
+    sums[own][column] = x;
+    if (column == 0) totals[own] = sum;
   }
-  if (a.sinks != nullptr) sum += exp2f(a.sinks[head0 + h] * 1.4426950408889634f - top);
+  __syncthreads();
+  if (threadIdx.x >= COLUMNS) return;
+  const int row = a.rows[pair / pairs_a_row], head = kvh * group + sub * PD_HEADS + h;
+  float sum = a.sinks != nullptr ? exp2f(a.sinks[head] * 1.4426950408889634f - top) : 0.0f;
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float4 y = sums[i][threadIdx.x];
+    sum += totals[i];
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  *reinterpret_cast<uint2*>(a.out + (static_cast<size_t>(a.row_q_start[row]) * a.nh + head0 + h) * HD + d) =
+  *reinterpret_cast<uint2*>(a.out + (static_cast<size_t>(a.row_q_start[row]) * a.nh + head) * HD + 4 * threadIdx.x) =
       make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
-template <int HD, bool BALANCED>
+template <int HD, int MODE>
 int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(PD_WARPS) * PD_STAGES * 2 * pk_block_bytes(HD) +
-                      (static_cast<size_t>(PD_MERGE_WARPS) * PD_HEADS * (HD + 4) + PD_WARPS * PD_HEADS * 2 + PD_HEADS * 2) * sizeof(float) +
-                      (BALANCED ? (a.n_rows + 1) * sizeof(int) : 0);
-  auto kernel = paged_decode_packed_kernel<HD, BALANCED>;
+  const size_t merge = MODE == PD_WARP_SHARES ? 0 : PD_MERGE_WARPS * PD_HEADS * (HD + 4) + PD_WARPS * PD_HEADS * 2 + PD_HEADS * 2;
+  const size_t smem = static_cast<size_t>(PD_WARPS) * PD_STAGES * 2 * pk_block_bytes(HD) + merge * sizeof(float) +
+                      (MODE == PD_CLUSTERS ? 0 : (a.n_rows + 1) * sizeof(int));
+  auto kernel = paged_decode_packed_kernel<HD, MODE>;
   if (smem > 227 * 1024) return ERR_UNSUPPORTED;
   if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
   cudaLaunchConfig_t config = {};
@@ -562,49 +768,52 @@ int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStr
 }
 
 template <int HD>
-int packed_decode_run(const PackedDecodeArgs& a, int ranks, int grid, cudaStream_t stream) {
+int packed_decode_run(const PackedDecodeArgs& a, int mode, int ctas, cudaStream_t stream) {
   const int pairs = a.n_rows * a.nkv * a.subs;
-  if (ranks > 0) return packed_decode_launch<HD, false>(a, pairs * ranks, ranks, stream);
-  const int rc = packed_decode_launch<HD, true>(a, grid, 1, stream);
+  if (mode == PD_CLUSTERS) return packed_decode_launch<HD, PD_CLUSTERS>(a, pairs * ctas, ctas, stream);
+  const int rc = mode == PD_CTA_SHARES ? packed_decode_launch<HD, PD_CTA_SHARES>(a, ctas, 1, stream)
+                                       : packed_decode_launch<HD, PD_WARP_SHARES>(a, ctas, 1, stream);
   if (rc != OK) return rc;
-  return launch_dependent(paged_decode_packed_merge_kernel<HD>, dim3(pairs), dim3(PD_HEADS * HD / 4), 0, stream, false, a);
+  const int group = a.nh / a.nkv;
+  return launch_dependent(paged_decode_packed_merge_kernel<HD>, dim3(pairs, group < PD_HEADS ? group : PD_HEADS), dim3(256), 0, stream, false, a);
 }
 
 }  // namespace zb
 
 using namespace zb;
 
-// Floats of scratch that zb_paged_decode_packed needs with `grid` CTAs for balanced shares of `pairs` pairs.
-ZB_API long long zb_paged_decode_packed_scratch_floats(int grid, int pairs, int hd) {
-  return 2LL * grid * PD_HEADS * (hd + 2) + 4LL * pairs;
+// Floats of scratch that zb_paged_decode_packed needs with `ctas` CTAs for equal shares of `pairs` pairs, a CTA's or (by_warp) a warp's.
+ZB_API long long zb_paged_decode_packed_scratch_floats(int ctas, int by_warp, int pairs, int hd) {
+  return 2LL * ctas * (by_warp ? PD_WARPS : 1) * PD_HEADS * (hd + 2) + 4LL * pairs;
 }
 
-// Attention of one new token a row over its context in the 4-bit cache.  `ranks` > 0: a cluster of that many CTAs (1, 2, 4 or 8) a
-// (row, key/value head) pair; 0: `grid` CTAs with equal shares of all pairs' tiles and a second kernel, with `scratch`
-// (zb_paged_decode_packed_scratch_floats, 16-byte aligned, any contents).
+// Attention of one new token a row over its context in the 4-bit cache.  `mode` 0: a cluster of `ctas` CTAs (1, 2, 4 or 8) a (row,
+// key/value head) pair; 1 and 2: `ctas` CTAs, each or each of whose warps has an equal share of all pairs' tiles, and a second kernel,
+// with `scratch` (zb_paged_decode_packed_scratch_floats, 16-byte aligned, any contents).
 ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
                                   int num_pages, int num_rows, const int* rows, int n_rows, const int* row_q_start, const int* row_ctx,
                                   long long max_context, int nh, int nkv, int hd, int window, int chunk, float scale, float softcap,
-                                  const float* sinks, int ranks, int grid, float* scratch, int* status, void* stream) {
+                                  const float* sinks, int mode, int ctas, float* scratch, int* status, void* stream) {
   const int page_shift = pk_page_shift(page_size);
   if (n_rows < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || max_context < 0 ||
-      !(ranks == 0 || ranks == 1 || ranks == 2 || ranks == 4 || ranks == 8) || (ranks == 0 && (grid <= 0 || scratch == nullptr)))
+      mode < PD_CLUSTERS || mode > PD_WARP_SHARES || ctas <= 0 || (mode == PD_CLUSTERS && ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) ||
+      (mode != PD_CLUSTERS && scratch == nullptr))
     return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
   if (n_rows == 0) return OK;
   const int subs = (nh / nkv + PD_HEADS - 1) / PD_HEADS;
   const long long pairs = static_cast<long long>(n_rows) * nkv * subs;
-  // (Tiles are counted in 32 bits.)
-  if (pairs * 8 >= (1LL << 31) || pairs * (max_context / PD_TILE + 1) >= (1LL << 31)) return ERR_UNSUPPORTED;
+  // (Blocks and tiles are counted in 32 bits.)
+  if (static_cast<long long>(num_pages) * nkv * (page_size / PK_BLOCK) >= (1LL << 31) || pairs * 8 >= (1LL << 31) || pairs * (max_context / PD_TILE + 1) >= (1LL << 31)) return ERR_UNSUPPORTED;
   PackedDecodeArgs a = {};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.packed = static_cast<const unsigned char*>(packed);
   a.block_table = block_table; a.rows = rows; a.row_q_start = row_q_start; a.row_ctx = row_ctx;
-  if (ranks == 0) {
+  if (mode != PD_CLUSTERS) {
     a.cuts = reinterpret_cast<int4*>(scratch);
     a.part_o = scratch + 4 * pairs;
-    a.part_ml = a.part_o + 2LL * grid * PD_HEADS * hd;
+    a.part_ml = a.part_o + 2LL * ctas * (mode == PD_WARP_SHARES ? PD_WARPS : 1) * PD_HEADS * hd;
   }
   a.max_blocks = max_blocks; a.page_shift = page_shift; a.num_pages = num_pages; a.num_rows = num_rows; a.n_rows = n_rows;
   a.nh = nh; a.nkv = nkv; a.subs = subs; a.window = window; a.chunk = chunk; a.sinks = sinks;
@@ -614,9 +823,9 @@ ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, 
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);
   switch (hd) {
-    case 32: return packed_decode_run<32>(a, ranks, grid, s);
-    case 64: return packed_decode_run<64>(a, ranks, grid, s);
-    case 96: return packed_decode_run<96>(a, ranks, grid, s);
-    default: return packed_decode_run<128>(a, ranks, grid, s);
+    case 32: return packed_decode_run<32>(a, mode, ctas, s);
+    case 64: return packed_decode_run<64>(a, mode, ctas, s);
+    case 96: return packed_decode_run<96>(a, mode, ctas, s);
+    default: return packed_decode_run<128>(a, mode, ctas, s);
   }
 }

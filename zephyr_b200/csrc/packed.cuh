@@ -69,7 +69,7 @@ __device__ __forceinline__ unsigned pk_values(unsigned word, unsigned steps, uns
   return pk_fma_bf16x2(pk_sub_bf16x2(pk_biased_codes<I>(word), 0x43004300u), steps, offsets);
 }
 
-// N words that lie side by side in shared memory, 16 bytes at a time where they are a multiple of that.
+// N words that lie side by side in shared memory.  Two, and four, must lie on a boundary of their size.
 template <int N>
 __device__ __forceinline__ void pk_load_words(unsigned (&w)[N], const unsigned char* from) {
   if constexpr (N == 4) {

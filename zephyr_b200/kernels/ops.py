@@ -268,7 +268,7 @@ def library() -> ctypes.CDLL:
             lib.zb_paged_decode_scratch_floats.restype = c_longlong
             lib.zb_paged_decode_balanced_scratch_floats.argtypes = [c_int, c_int, c_int]
             lib.zb_paged_decode_balanced_scratch_floats.restype = c_longlong
-            lib.zb_paged_decode_packed_scratch_floats.argtypes = [c_int, c_int, c_int]
+            lib.zb_paged_decode_packed_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
             lib.zb_paged_decode_packed_scratch_floats.restype = c_longlong
             if os.environ.get("ZEPHYR_B200_DEPENDENT_LAUNCH", "1") == "0":
                 lib.zb_set_dependent_launch(0)
@@ -1465,16 +1465,20 @@ def _packed_attention_args(q, packed, block_table, status, out, nh, nkv, hd, win
     return _check_packed(packed, nkv, hd)
 
 
+PACKED_CLUSTERS, PACKED_CTA_SHARES, PACKED_WARP_SHARES = 0, 1, 2
+
+
 def packed_decode_plan(n_rows: int, nh: int, nkv: int, max_context: int) -> tuple[int, int]:
-    """How ``paged_decode_packed`` cuts its rows' contexts: (CTAs a (row, key/value head) pair, 0), or (0, CTAs) for balanced shares."""
+    """How ``paged_decode_packed`` cuts its rows' contexts: a cluster of n CTAs a (row, key/value head) pair, or shares for n CTAs or
+    their warps."""
     pairs = n_rows * nkv * -(-nh // nkv // 8)
     slots = 2 * _sm_count()
     if pairs > slots:
-        return 0, slots
+        return PACKED_WARP_SHARES, slots
     ranks = 1
     while ranks < 8 and 2 * ranks * pairs <= slots and max_context > 256 * ranks:
         ranks *= 2
-    return ranks, 0
+    return PACKED_CLUSTERS, ranks
 
 
 def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, row_q_start: torch.Tensor,
@@ -1491,15 +1495,16 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
     _require(row_q_start.numel() >= block_table.shape[0] and row_ctx.numel() >= block_table.shape[0], "one start and context per row")
     _same_device(q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
     n_rows = rows.numel()
-    ranks, grid = plan or packed_decode_plan(n_rows, nh, nkv, min([max_context] + [n for n in (window, chunk) if n > 0]))
+    mode, ctas = plan or packed_decode_plan(n_rows, nh, nkv, min([max_context] + [n for n in (window, chunk) if n > 0]))
     scratch = None
-    if ranks == 0 and n_rows > 0:
+    if mode != PACKED_CLUSTERS and n_rows > 0:
         pairs = n_rows * nkv * -(-nh // nkv // 8)
-        scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(grid, pairs, hd)), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(ctas, int(mode == PACKED_WARP_SHARES), pairs, hd)),
+                              dtype=torch.float32, device=q.device)
     _check(library().zb_paged_decode_packed(
         _ptr(out), _ptr(q), _ptr(packed), _ptr(block_table), block_table.shape[1], page_size, pages, block_table.shape[0], _ptr(rows),
         n_rows, _ptr(row_q_start), _ptr(row_ctx), int(max_context), nh, nkv, hd, int(window), int(chunk), float(scale), float(softcap),
-        _ptr(sinks), ranks, grid, _ptr(scratch), _ptr(status), _stream()), "paged_decode_packed", 2 if ranks == 0 else 1)
+        _ptr(sinks), mode, ctas, _ptr(scratch), _ptr(status), _stream()), "paged_decode_packed", 1 if mode == PACKED_CLUSTERS else 2)
     return out
 
 
