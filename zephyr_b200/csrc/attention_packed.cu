@@ -35,7 +35,6 @@ constexpr int PD_WARPS = 8;
 constexpr int PD_STAGES = 2;              // a power of two
 constexpr int PD_TILE = 32;              // positions per tile: a warp's unit of work
 constexpr int PD_HEADS = 8;              // query heads on the products' columns
-constexpr int PD_MERGE_WARPS = PD_WARPS / 2;
 constexpr float PD_LIFT = 60.0f;         // weights carry 2^60, results 2^(60 - 133)
 constexpr float PD_RESCALE = 8.0f;       // a running maximum (in powers of two) may be passed by this before sums are rescaled
 
@@ -51,7 +50,8 @@ struct PackedDecodeArgs {
   const int* row_ctx;            // [num_rows] the new token's position
   float* part_o;                 // [2 shares][8][hd]: partial results of pairs that are cut
   float* part_ml;                // [2 shares][8][2]: their maxima and sums
-  int4* cuts;                    // [pairs]: first range, ranges, first tile, tiles per range
+  int4* cuts;                    // [pairs]: first range, ranges, the first tile's place, places per range
+  long long q_values;            // of q
   int max_blocks, page_shift, num_pages, num_rows, n_rows;
   int nh, nkv, subs, window, chunk;
   const float* sinks;            // null, or [nh]: exp(sinks[h]) joins the softmax's denominator of head h
@@ -89,10 +89,10 @@ __device__ __forceinline__ void mma_rows8(float (&d)[4], unsigned a0, unsigned a
   const unsigned a[4] = {a0, any, a2, other};
   mma_bf16(d, a, b0, b1);
 }
-// The same with nothing to add to.
-__device__ __forceinline__ void mma_bf16_1688_first(float (&d)[4], const unsigned (&a)[2], unsigned b) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(b), "f"(0.0f));
+// On top of one value a column; and on top of nothing.
+__device__ __forceinline__ void mma_bf16_1688_on(float (&d)[4], const unsigned (&a)[2], unsigned b, float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%7,%8};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(b), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void mma_bf16_16816_first(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
@@ -124,22 +124,27 @@ __device__ __forceinline__ void pd_pair(const PackedDecodeArgs& a, int pair, int
   s.lo = pd_first_seen(a, total);
   s.hi = total;
 }
-// The scratch slot of a pair's part in range `range`: a range has one for a pair that began before it, and one for a pair that begins in it.
-__device__ __forceinline__ int pd_slot(int pair_first, int range, int per_range) { return 2 * range + (pair_first < range * per_range ? 0 : 1); }
+// The scratch slot of a pair's part in range `range`: a range has one for a pair whose first tile is before it, and one for a pair whose
+// first tile is in it.
+__device__ __forceinline__ int pd_slot(int first_place, int range, int per_range) { return 2 * range + (first_place < range * per_range ? 0 : 1); }
 
 template <int HD, int MODE>
 __global__ void __launch_bounds__(PD_WARPS * 32, 2)
 paged_decode_packed_kernel(const PackedDecodeArgs a) {
   constexpr bool BALANCED = MODE != PD_CLUSTERS, WARPWISE = MODE == PD_WARP_SHARES;
   constexpr int STRIDE = WARPWISE ? 1 : PD_WARPS;          // a segment's tiles are one warp's, or all warps' in turn
+  // What a pair costs whoever has it beyond its tiles, in tiles: its queries, its first tile's way, its end.  (48 rows of 60 to 6001
+  // positions, warps' shares: 69 us without it, the warps with the shortest rows' pairs end last.)
+  constexpr int PAIR_COST = WARPWISE ? 3 : 12;
   constexpr int NG = HD / 32, BLOCK_BYTES = pk_block_bytes(HD), TILE_BYTES = 2 * BLOCK_BYTES;
   constexpr int OROW = HD + 4;             // padded: four heads' pieces of 16 bytes fall into different banks
   extern __shared__ __align__(128) unsigned char smem[];
   unsigned char* const rings = smem;                                                       // [warps][stages][2][20 HD]
-  float* const merge_o = reinterpret_cast<float*>(rings + PD_WARPS * PD_STAGES * TILE_BYTES);    // [merge warps][8][OROW]
-  float* const merge_ml = merge_o + (WARPWISE ? 0 : PD_MERGE_WARPS * PD_HEADS * OROW);      // [warps][8][2]
-  float* const result_ml = merge_ml + (WARPWISE ? 0 : PD_WARPS * PD_HEADS * 2);             // [8][2]
-  int* const prefix = reinterpret_cast<int*>(result_ml + (WARPWISE ? 0 : PD_HEADS * 2));    // balanced: every row's first tile, n_rows + 1
+  float* const merge_ml = reinterpret_cast<float*>(rings + PD_WARPS * PD_STAGES * TILE_BYTES);     // [warps][8][2]
+  int* const prefix = reinterpret_cast<int*>(merge_ml + PD_WARPS * PD_HEADS * 2);           // balanced: every row's first tile, n_rows + 1
+  float* const parts_ml = merge_ml + PD_WARPS * PD_HEADS * 2;                               // clusters: the CTAs' [8][8][2]
+  float* const parts_o = parts_ml + 8 * PD_HEADS * 2;                                       // and their parts of this CTA's share
+  static_assert(PD_HEADS * OROW * 4 <= PD_STAGES * TILE_BYTES, "a warp's results fit where its tiles lay");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = a.nh / a.nkv, pairs_a_row = a.nkv * a.subs;
@@ -149,8 +154,20 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
   wait_for_prior_grids();          // queries, cache and the step's description: all of it earlier kernels' work
   let_dependents_launch();
 
+  // In a step of decoding requests only, row r is request r: what hangs on its number is asked for together with it.
+  auto ask = [](const void* p) { asm volatile("prefetch.global.L1 [%0];\n" ::"l"(p)); };
+  const int guess = BALANCED ? static_cast<int>(threadIdx.x) : static_cast<int>(blockIdx.x / (gridDim.x / a.n_rows));
+  if (guess < min(a.n_rows, a.num_rows) && (BALANCED || threadIdx.x == 0)) {
+    ask(a.row_ctx + guess);
+    ask(a.row_q_start + guess);
+  }
+  if (!BALANCED && guess < a.num_rows && threadIdx.x * 32 < min(a.max_blocks, 2048))
+    ask(a.block_table + static_cast<size_t>(guess) * a.max_blocks + threadIdx.x * 32);
+
   // ------------------------------------------------------------------ which tiles are this CTA's
   const unsigned ranks = BALANCED ? 1u : gridDim.x / (a.n_rows * pairs_a_row), rank = BALANCED ? 0u : blockIdx.x % ranks;
+  __syncwarp();
+  if (!BALANCED && ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   const int range = WARPWISE ? static_cast<int>(blockIdx.x) * PD_WARPS + warp : static_cast<int>(blockIdx.x);
   int per_range = 0, range_first = 0, range_end = 0;
   PdSegment whole;                 // not balanced: the only segment
@@ -164,7 +181,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
         for (int p = 0; p < pairs_a_row; ++p) a.cuts[r * pairs_a_row + p] = make_int4(0, 0, 0, 1);
       }
       const int total = ok ? a.row_ctx[row] + 1 : 0;
-      prefix[r + 1] = ok ? ((total + PD_TILE - 1) / PD_TILE - pd_first_seen(a, total) / PD_TILE) * pairs_a_row : 0;
+      prefix[r + 1] = ok ? (PAIR_COST + (total + PD_TILE - 1) / PD_TILE - pd_first_seen(a, total) / PD_TILE) * pairs_a_row : 0;
     }
     __syncthreads();
     if (warp == 0) {
@@ -201,46 +218,49 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     whole.count = static_cast<int>(static_cast<long long>(count) * (rank + 1) / ranks) - from;
     whole.row = ok ? row : -1;
   }
-  // The segment that holds tile `at` of the range (balanced), and the tile behind it.
-  auto segment_at = [&](int at, PdSegment& s, int& pair_first, int& pair_tiles, int& pair) -> int {
-    int lo = 0, hi = a.n_rows - 1;                       // the last row whose first tile is not behind `at`
+  // The segment that begins at place `at` of the range (balanced; maybe one without tiles), and the place behind it.
+  auto segment_at = [&](int at, PdSegment& s, int& first_place, int& pair_tiles, int& pair) -> int {
+    int lo = 0, hi = a.n_rows - 1;                       // the last row whose first place is not behind `at`
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (prefix[mid] <= at) lo = mid;
       else hi = mid - 1;
     }
-    const int r = lo;
-    pair_tiles = (prefix[r + 1] - prefix[r]) / pairs_a_row;
-    const int p = (at - prefix[r]) / pair_tiles;
-    pair_first = prefix[r] + p * pair_tiles;
+    const int r = lo, places = (prefix[r + 1] - prefix[r]) / pairs_a_row, p = (at - prefix[r]) / places;
+    const int end = min(range_end, prefix[r] + (p + 1) * places);
+    first_place = prefix[r] + p * places + PAIR_COST;       // the place of the pair's first tile
+    pair_tiles = places - PAIR_COST;
     pair = r * pairs_a_row + p;
     s.row = a.rows[r];
     pd_pair(a, p, a.row_ctx[s.row] + 1, s);
-    const int end = min(range_end, pair_first + pair_tiles);
-    s.first = s.lo / PD_TILE + (at - pair_first);
-    s.count = end - at;
+    const int from = max(at - first_place, 0);
+    s.first = s.lo / PD_TILE + from;
+    s.count = max(end - first_place, 0) - from;
     return end;
   };
 
   // ------------------------------------------------------------------ the copies, which run ahead of the products
   PdSegment ahead;                // the segment the copies are in
-  int ahead_next = range_first, ahead_tile = WARPWISE ? 0 : warp, ahead_left = 0;
+  int ahead_next = range_first, ahead_tile = 0, ahead_left = 0;
   ahead.count = 0;
-  if (!BALANCED) ahead = whole;
   // Where the next 16 of the warp's tiles lie: lane 2 i + b has block b of the i-th, as a number of blocks from the cache's start.
   // (A block of which nothing is seen is block 0, whose bytes nobody looks at.)
   int my_block = 0;
-  bool more = true;
+  bool more = false;
   auto look_up = [&]() {
     while (ahead_tile >= ahead.count) {
-      if (!BALANCED || ahead_next >= range_end) {
+      if (!WARPWISE || ahead_next >= range_end) {
         more = false;
         return;
       }
       int x, y, z;
       ahead_next = segment_at(ahead_next, ahead, x, y, z);
-      ahead_tile = WARPWISE ? 0 : warp;
+      ahead_tile = 0;
+      if (ahead.count > 0 && lane < PD_HEADS * HD / 64)      // its queries: 128 bytes a lane
+        ask(a.q + min((static_cast<size_t>(a.row_q_start[ahead.row]) * a.nh + ahead.kvh * group + ahead.sub * PD_HEADS) * HD + lane * 64,
+                      static_cast<size_t>(a.q_values - 1)));
     }
+    more = true;
     ahead_left = 16;
     const int tile = ahead_tile + (lane >> 1) * STRIDE, pos = (ahead.first + tile) * PD_TILE + (lane & 1) * PK_BLOCK;
     my_block = 0;
@@ -272,9 +292,16 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     }
     cp_async_commit();               // a group a tile, empty ones behind the last
   };
-  look_up();
+  // The first tiles' copies: every warp's first before any warp's second, so that all can begin when half of it is there.
+  auto begin = [&]() {
+    look_up();
 #pragma unroll 1
-  for (int s = 0; s < PD_STAGES; ++s) issue();
+    for (int s = 0; s < PD_STAGES; ++s) {
+      if (s > 0) __syncthreads();
+      issue();
+    }
+  };
+  if (WARPWISE) begin();
 
   // ------------------------------------------------------------------ the segments
   int taken = 0, at = range_first;
@@ -282,12 +309,21 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
 #pragma unroll 1
   while (BALANCED ? at < range_end : once) {
     PdSegment seg;
-    int pair_first = 0, pair_tiles = 0, pair = 0, at0 = at;
+    int first_place = 0, pair_tiles = 0, pair = 0;
+    bool begins = false;
     if (BALANCED) {
-      at = segment_at(at, seg, pair_first, pair_tiles, pair);
+      const int from = at;
+      at = segment_at(at, seg, first_place, pair_tiles, pair);
+      if (seg.count == 0) continue;
+      begins = from <= first_place;
     } else {
       seg = whole;
       once = false;
+    }
+    if (!WARPWISE) {
+      ahead = seg;
+      ahead_tile = warp;
+      begin();
     }
     const int heads = min(PD_HEADS, group - seg.sub * PD_HEADS), head0 = seg.kvh * group + seg.sub * PD_HEADS;
     const size_t token = seg.row >= 0 ? static_cast<size_t>(a.row_q_start[seg.row]) : 0;
@@ -343,7 +379,9 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) scale_c[h] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * h) * 1.329227995784916e36f * (8192.0f * scale_d);
     }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};      // heads 2 t and 2 t + 1; the sums over this lane's positions
+    // Heads 2 t and 2 t + 1: the maximum, what is added to scores so that it becomes 2^60's exponent, from where on it has to move; and
+    // the sums over this lane's positions.
+    float m_run[2] = {-INFINITY, -INFINITY}, lift[2] = {0.0f, 0.0f}, limit[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
     float o[2 * NG][4], rest_c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, weights_c[(NG + 1) / 2][4];
 #pragma unroll
     for (int n = 0; n < (NG + 1) / 2; ++n) weights_c[n][0] = weights_c[n][1] = weights_c[n][2] = weights_c[n][3] = 0.0f;
@@ -361,7 +399,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
       auto work = [&](auto at_edge) {
       constexpr bool edge = decltype(at_edge)::value;
 
-      // Scores in powers of two: s[b][c] of position 16 b + g (+ 8 for c >= 2) and head 2 t + (c & 1).
+      // Scores in powers of two, lifted: s[b][c] of position 16 b + g (+ 8 for c >= 2) and head 2 t + (c & 1).
       float s[2][4];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -385,7 +423,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           params[1] = *reinterpret_cast<const unsigned*>(block + pk_key_step<HD>(g + 8, 0) + 4 * t);
         }
         float d[4], sum[4];
-        mma_bf16_1688_first(d, params, sums_b[1]);
+        mma_bf16_1688_on(d, params, sums_b[1], lift[0], lift[1]);
         mma_bf16_1688(d, params, sums_b[0]);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
@@ -410,7 +448,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[b][c] = a.softcap_log2 * tanhf(s[b][c] * a.scale_over_cap);
+          for (int c = 0; c < 4; ++c) s[b][c] = fmaf(a.softcap_log2, tanhf((s[b][c] - lift[c & 1]) * a.scale_over_cap), lift[c & 1]);
       }
       if constexpr (edge) {
 #pragma unroll
@@ -425,12 +463,22 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
       float top[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
-      if (__any_sync(0xffffffffu, top[0] > m_run[0] + PD_RESCALE || top[1] > m_run[1] + PD_RESCALE)) {
+      if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1])) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
-          const float now = fmaxf(m_run[h], top[h]), factor = m_run[h] == -INFINITY ? 0.0f : exp2f(m_run[h] - now);
+          const float now = fmaxf(m_run[h], top[h] - lift[h]), factor = m_run[h] == -INFINITY ? 0.0f : exp2f(m_run[h] - now);
+          if (now > -INFINITY) {
+            const float to = PD_LIFT - now, by = to - lift[h];
+            lift[h] = to;
+            limit[h] = PD_LIFT + PD_RESCALE;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              s[b][h] += by;
+              s[b][2 + h] += by;
+            }
+          }
           m_run[h] = now;
           l_run[h] *= factor;
 #pragma unroll
@@ -450,14 +498,13 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           }
         }
       }
-      const float shift[2] = {m_run[0] == -INFINITY ? 0.0f : m_run[0] - PD_LIFT, m_run[1] == -INFINITY ? 0.0f : m_run[1] - PD_LIFT};
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const unsigned char* const block = tile + b * BLOCK_BYTES;
         float p[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(p[c]) : "f"(s[b][c] - shift[c & 1]));
+          asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(p[c]) : "f"(s[b][c]));
           l_run[c & 1] += p[c];
         }
         // This lane's positions' steps: words of the pairs g / 2 and g / 2 + 4, the half that g says.
@@ -543,13 +590,13 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
     const bool cut = BALANCED ? seg.count < pair_tiles : ranks > 1;
-    if (BALANCED && at0 == pair_first && (WARPWISE ? lane : threadIdx.x) == 0) {
-      const int first = pair_first / per_range, last = (pair_first + pair_tiles - 1) / per_range;
-      a.cuts[pair] = make_int4(first, last - first + 1, pair_first, per_range);
+    if (BALANCED && begins && (WARPWISE ? lane : threadIdx.x) == 0) {
+      const int first = first_place / per_range, last = (first_place + pair_tiles - 1) / per_range;
+      a.cuts[pair] = make_int4(first, last - first + 1, first_place, per_range);
     }
     if constexpr (WARPWISE) {
       // The warp's own result, or its part of one: four channels of a group lie in a lane's two products.
-      const size_t slot = static_cast<size_t>(pd_slot(pair_first, range, per_range)) * PD_HEADS;
+      const size_t slot = static_cast<size_t>(pd_slot(first_place, range, per_range)) * PD_HEADS;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int head = 2 * t + h;
@@ -570,59 +617,36 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
         }
       }
     } else {
-    // ---------------------------------------------------------------- the warps' results meet
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * PD_HEADS + 2 * t + h) * 2) = make_float2(m_run[h], l_run[h]);
-    __syncthreads();
-    float factor[2];                 // of heads 2 t, 2 t + 1
+    // ---------------------------------------------------------------- the warps' results meet, each where its tiles lay
+    float* const own_o = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float all = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) all = fmaxf(all, merge_ml[(w * PD_HEADS + 2 * t + h) * 2]);
-      factor[h] = m_run[h] == -INFINITY ? 0.0f : exp2f(m_run[h] - all);
-    }
-    // Four channels of a group lie in a lane's two products: heads 2 t and 2 t + 1, channels 32 m + 4 g ..
-    auto mine = [&](int m, int h) {
-      return make_float4(o[2 * m][h] * factor[h], o[2 * m][2 + h] * factor[h], o[2 * m + 1][h] * factor[h], o[2 * m + 1][2 + h] * factor[h]);
-    };
-    auto place = [&](int w, int m, int h) { return reinterpret_cast<float4*>(merge_o + (w * PD_HEADS + 2 * t + h) * OROW + 32 * m + 4 * g); };
-    if (warp >= PD_MERGE_WARPS) {
+      if (g == 0) *reinterpret_cast<float2*>(merge_ml + (warp * PD_HEADS + 2 * t + h) * 2) = make_float2(m_run[h], l_run[h]);
+      // Four channels of a group lie in a lane's two products: heads 2 t and 2 t + 1, channels 32 m + 4 g ..
 #pragma unroll
       for (int m = 0; m < NG; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) *place(warp - PD_MERGE_WARPS, m, h) = mine(m, h);
+        *reinterpret_cast<float4*>(own_o + (2 * t + h) * OROW + 32 * m + 4 * g) =
+            make_float4(o[2 * m][h], o[2 * m][2 + h], o[2 * m + 1][h], o[2 * m + 1][2 + h]);
     }
     __syncthreads();
-    if (warp < PD_MERGE_WARPS) {
-#pragma unroll
-      for (int m = 0; m < NG; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 x = mine(m, h);
-          float4 y = *place(warp, m, h);
-          y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
-          *place(warp, m, h) = y;
-        }
-    }
-    __syncthreads();
-    // Four values of a head a thread: the sum of the four warps' sums, the pair's maximum and sum of exponentials.
+    if (!BALANCED && ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // all of the cluster's CTAs run
+    // Four values of a head a thread.
     for (int e = threadIdx.x; e < PD_HEADS * HD / 4; e += PD_WARPS * 32) {
       const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
-      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < PD_MERGE_WARPS; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(merge_o + (w * PD_HEADS + h) * OROW + d);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
+      float2 ml[PD_WARPS];
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, merge_ml[(w * PD_HEADS + h) * 2]);
+      for (int w = 0; w < PD_WARPS; ++w) {
+        ml[w] = *reinterpret_cast<const float2*>(merge_ml + (w * PD_HEADS + h) * 2);
+        top = fmaxf(top, ml[w].x);
+      }
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < PD_WARPS; ++w) {
-        const float m = merge_ml[(w * PD_HEADS + h) * 2];
-        if (m > -INFINITY) sum += merge_ml[(w * PD_HEADS + h) * 2 + 1] * exp2f(m - top);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rings + w * PD_STAGES * TILE_BYTES) + h * OROW + d);
+        const float f = ml[w].x > -INFINITY ? exp2f(ml[w].x - top) : 0.0f;
+        sum += ml[w].y * f;
+        x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
       }
       if (!cut) {
         if (h < heads && seg.row >= 0) {
@@ -632,44 +656,43 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
               make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
         }
       } else if (BALANCED) {
-        const int slot = pd_slot(pair_first, range, per_range);
+        const int slot = pd_slot(first_place, range, per_range);
         *reinterpret_cast<float4*>(a.part_o + (static_cast<size_t>(slot) * PD_HEADS + h) * HD + d) = x;
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (static_cast<size_t>(slot) * PD_HEADS + h) * 2) = make_float2(top, sum);
       } else {
-        // (Read by this thread alone; the first warp's sums are the CTA's from here on.)
-        *reinterpret_cast<float4*>(merge_o + h * OROW + d) = x;
-        if (d == 0) {
-          result_ml[2 * h] = top;
-          result_ml[2 * h + 1] = sum;
-        }
+        // To the CTA whose share of the results it is; maxima and sums to all.
+        const int per_rank = PD_HEADS * HD / 4 / static_cast<int>(ranks), target = e / per_rank;
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n"
+                     ::"r"(in_cta_of_rank(smem_u32(parts_o + (static_cast<int>(rank) * per_rank + e - target * per_rank) * 4), target)),
+                       "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
+        if (d / 4 < static_cast<int>(ranks))
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};\n"
+                       ::"r"(in_cta_of_rank(smem_u32(parts_ml + (static_cast<int>(rank) * PD_HEADS + h) * 2), d / 4)), "f"(top), "f"(sum) : "memory");
       }
     }
-    if (BALANCED) __syncthreads();           // the next segment writes where these sums lay
+    if (BALANCED) __syncthreads();           // the next segment's tiles come where these results lie
     if (!BALANCED && ranks > 1) {
-      // The cluster's CTAs each join a share of the results, read from all of them.
+      // Every CTA of the cluster has been handed the parts of its share of the results, and joins them.
       __syncwarp();
       cluster_sync_all();
-      const int per_rank = (PD_HEADS * HD / 4 + static_cast<int>(ranks) - 1) / static_cast<int>(ranks);
+      const int per_rank = PD_HEADS * HD / 4 / static_cast<int>(ranks);
       for (int i = threadIdx.x; i < per_rank; i += PD_WARPS * 32) {
         const int e = static_cast<int>(rank) * per_rank + i, h = e / (HD / 4), d = 4 * (e % (HD / 4));
-        if (e >= PD_HEADS * HD / 4 || h >= heads || seg.row < 0) continue;
-        auto in_rank = [&](const float* p, unsigned r) { return in_cta_of_rank(smem_u32(p), r); };
+        if (h >= heads || seg.row < 0) continue;
+        float2 ml[8];
         float top = -INFINITY, sum = 0.0f;
-        for (unsigned r = 0; r < ranks; ++r) {
-          float m;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(m) : "r"(in_rank(result_ml + 2 * h, r)));
-          top = fmaxf(top, m);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          ml[r] = r < static_cast<int>(ranks) ? *reinterpret_cast<const float2*>(parts_ml + (r * PD_HEADS + h) * 2) : make_float2(-INFINITY, 0.0f);
+          top = fmaxf(top, ml[r].x);
         }
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (unsigned r = 0; r < ranks; ++r) {
-          float m, l;
-          float4 y;
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(m), "=f"(l) : "r"(in_rank(result_ml + 2 * h, r)));
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
-                       : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(in_rank(merge_o + h * OROW + d, r)));
-          if (m == -INFINITY) continue;
-          const float f = exp2f(m - top);
-          sum += l * f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r >= static_cast<int>(ranks)) continue;
+          const float4 y = *reinterpret_cast<const float4*>(parts_o + (r * per_rank + i) * 4);
+          const float f = ml[r].x > -INFINITY ? exp2f(ml[r].x - top) : 0.0f;
+          sum += ml[r].y * f;
           x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
         }
         if (a.sinks != nullptr) sum += exp2f(a.sinks[head0 + h] * 1.4426950408889634f - top);
@@ -677,71 +700,80 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
         *reinterpret_cast<uint2*>(a.out + (token * a.nh + head0 + h) * HD + d) =
             make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
       }
-      __syncwarp();
-      cluster_sync_all();                    // nobody leaves while its memory is read
     }
     }
   }
 }
 
-// The pairs whose tiles lie in several ranges: their parts meet.  A CTA a pair and head; threads are columns of four channels times
-// groups that share the parts.
+// The pairs whose tiles lie in several ranges: their parts meet.  A CTA a pair, or a head of one (grid y): a thread four channels of a
+// head, and where that leaves threads idle, groups of threads share the parts.  Parts come eight at a time, all asked for before the first is used.
 template <int HD>
 __global__ void __launch_bounds__(256)
 paged_decode_packed_merge_kernel(const PackedDecodeArgs a) {
-  constexpr int COLUMNS = HD / 4, GROUPS = 256 / COLUMNS;
-  __shared__ float4 sums[GROUPS][COLUMNS];
-  __shared__ float of_warp[8], totals[GROUPS];
+  constexpr int COLUMNS = HD / 4, BATCH = 8;
+  __shared__ float4 sums[256];
+  __shared__ float2 mls[256];
   wait_for_prior_grids();
   let_dependents_launch();
-  const int pair = blockIdx.x, h = blockIdx.y, pairs_a_row = a.nkv * a.subs, group = a.nh / a.nkv;
+  const int pair = blockIdx.x, pairs_a_row = a.nkv * a.subs, group = a.nh / a.nkv;
   const int4 cut = a.cuts[pair];
+  if (cut.y <= 1) return;
   const int p = pair % pairs_a_row, sub = p % a.subs, kvh = p / a.subs;
-  if (cut.y <= 1 || h >= min(PD_HEADS, group - sub * PD_HEADS)) return;
-  auto at = [&](int i) { return static_cast<size_t>(pd_slot(cut.z, cut.x + i, cut.w)) * PD_HEADS + h; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < cut.y; i += 256) top = fmaxf(top, a.part_ml[at(i) * 2]);
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, of_warp[w]);
-  const int column = threadIdx.x % COLUMNS, own = threadIdx.x / COLUMNS;
-  if (own < GROUPS) {
-    float sum = 0.0f;
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = own; i < cut.y; i += GROUPS) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(i) * 2);
-      const float4 y = *reinterpret_cast<const float4*>(a.part_o + at(i) * HD + 4 * column);
-      const float f = ml.x > -INFINITY ? exp2f(ml.x - top) : 0.0f;
-      sum += ml.y * f;
-      x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
-    }
-    sums[own][column] = x;
-    if (column == 0) totals[own] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x >= COLUMNS) return;
+  const int heads = min(PD_HEADS, group - sub * PD_HEADS);
+  if (static_cast<int>(blockIdx.y) >= heads) return;
+  const int wanted = (gridDim.y > 1 ? 1 : heads) * COLUMNS, groups = 256 / wanted;
+  const int own = threadIdx.x / wanted, e = threadIdx.x - own * wanted, h = blockIdx.y + e / COLUMNS, d = 4 * (e % COLUMNS);
   const int row = a.rows[pair / pairs_a_row], head = kvh * group + sub * PD_HEADS + h;
-  float sum = a.sinks != nullptr ? exp2f(a.sinks[head] * 1.4426950408889634f - top) : 0.0f;
+  const size_t token = a.row_q_start[row];
+  float top = -INFINITY, sum = 0.0f;
   float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto join = [&](float m, float l, float4 y) {      // one part on the shift `top`, which is not below m
+    const float scale = m > -INFINITY ? exp2f(m - top) : 0.0f;
+    sum = fmaf(l, scale, sum);
+    x.x = fmaf(y.x, scale, x.x); x.y = fmaf(y.y, scale, x.y); x.z = fmaf(y.z, scale, x.z); x.w = fmaf(y.w, scale, x.w);
+  };
+  for (int i0 = own; own < groups && i0 < cut.y; i0 += BATCH * groups) {
+    float2 ml[BATCH];
+    float4 y[BATCH];
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const float4 y = sums[i][threadIdx.x];
-    sum += totals[i];
-    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * groups;
+      ml[u] = make_float2(-INFINITY, 0.0f);
+      y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i >= cut.y) continue;
+      const size_t at = static_cast<size_t>(pd_slot(cut.z, cut.x + i, cut.w)) * PD_HEADS + h;
+      ml[u] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+      y[u] = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+    }
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) now = fmaxf(now, ml[u].x);
+    const float f = top > -INFINITY ? exp2f(top - now) : 0.0f;
+    top = now;
+    sum *= f;
+    x.x *= f; x.y *= f; x.z *= f; x.w *= f;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) join(ml[u].x, ml[u].y, y[u]);
   }
+  sums[threadIdx.x] = x;
+  mls[threadIdx.x] = make_float2(top, sum);
+  __syncthreads();
+  if (own > 0) return;
+  for (int i = 1; i < groups; ++i) top = fmaxf(top, mls[i * wanted + e].x);
+  const float f = mls[e].x > -INFINITY ? exp2f(mls[e].x - top) : 0.0f;
+  sum *= f;
+  x.x *= f; x.y *= f; x.z *= f; x.w *= f;
+  for (int i = 1; i < groups; ++i) join(mls[i * wanted + e].x, mls[i * wanted + e].y, sums[i * wanted + e]);
+  if (a.sinks != nullptr) sum += exp2f(a.sinks[head] * 1.4426950408889634f - top);
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  *reinterpret_cast<uint2*>(a.out + (static_cast<size_t>(a.row_q_start[row]) * a.nh + head) * HD + 4 * threadIdx.x) =
+  *reinterpret_cast<uint2*>(a.out + (token * a.nh + head) * HD + d) =
       make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
 template <int HD, int MODE>
 int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStream_t stream) {
-  const size_t merge = MODE == PD_WARP_SHARES ? 0 : PD_MERGE_WARPS * PD_HEADS * (HD + 4) + PD_WARPS * PD_HEADS * 2 + PD_HEADS * 2;
-  const size_t smem = static_cast<size_t>(PD_WARPS) * PD_STAGES * 2 * pk_block_bytes(HD) + merge * sizeof(float) +
-                      (MODE == PD_CLUSTERS ? 0 : (a.n_rows + 1) * sizeof(int));
+  const size_t smem = static_cast<size_t>(PD_WARPS) * PD_STAGES * 2 * pk_block_bytes(HD) + PD_WARPS * PD_HEADS * 2 * sizeof(float) +
+                      (MODE != PD_CLUSTERS ? (a.n_rows + 1) * sizeof(int) : ranks > 1 ? (8 * 2 + HD) * PD_HEADS * sizeof(float) : 0);
   auto kernel = paged_decode_packed_kernel<HD, MODE>;
   if (smem > 227 * 1024) return ERR_UNSUPPORTED;
   if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
@@ -774,8 +806,8 @@ int packed_decode_run(const PackedDecodeArgs& a, int mode, int ctas, cudaStream_
   const int rc = mode == PD_CTA_SHARES ? packed_decode_launch<HD, PD_CTA_SHARES>(a, ctas, 1, stream)
                                        : packed_decode_launch<HD, PD_WARP_SHARES>(a, ctas, 1, stream);
   if (rc != OK) return rc;
-  const int group = a.nh / a.nkv;
-  return launch_dependent(paged_decode_packed_merge_kernel<HD>, dim3(pairs, group < PD_HEADS ? group : PD_HEADS), dim3(256), 0, stream, false, a);
+  const int group = a.nh / a.nkv, across = pairs <= 128 ? (group < PD_HEADS ? group : PD_HEADS) : 1;      // few pairs: a head a CTA
+  return launch_dependent(paged_decode_packed_merge_kernel<HD>, dim3(pairs, across), dim3(256), 0, stream, false, a);
 }
 
 }  // namespace zb
@@ -792,7 +824,7 @@ ZB_API long long zb_paged_decode_packed_scratch_floats(int ctas, int by_warp, in
 // with `scratch` (zb_paged_decode_packed_scratch_floats, 16-byte aligned, any contents).
 ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
                                   int num_pages, int num_rows, const int* rows, int n_rows, const int* row_q_start, const int* row_ctx,
-                                  long long max_context, int nh, int nkv, int hd, int window, int chunk, float scale, float softcap,
+                                  long long max_context, long long tokens, int nh, int nkv, int hd, int window, int chunk, float scale, float softcap,
                                   const float* sinks, int mode, int ctas, float* scratch, int* status, void* stream) {
   const int page_shift = pk_page_shift(page_size);
   if (n_rows < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || max_context < 0 ||
@@ -804,7 +836,7 @@ ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, 
   const int subs = (nh / nkv + PD_HEADS - 1) / PD_HEADS;
   const long long pairs = static_cast<long long>(n_rows) * nkv * subs;
   // (Blocks and tiles are counted in 32 bits.)
-  if (static_cast<long long>(num_pages) * nkv * (page_size / PK_BLOCK) >= (1LL << 31) || pairs * 8 >= (1LL << 31) || pairs * (max_context / PD_TILE + 1) >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (static_cast<long long>(num_pages) * nkv * (page_size / PK_BLOCK) >= (1LL << 31) || pairs * 8 >= (1LL << 31) || pairs * (max_context / PD_TILE + 16) >= (1LL << 30)) return ERR_UNSUPPORTED;
   PackedDecodeArgs a = {};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
@@ -815,6 +847,7 @@ ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, 
     a.part_o = scratch + 4 * pairs;
     a.part_ml = a.part_o + 2LL * ctas * (mode == PD_WARP_SHARES ? PD_WARPS : 1) * PD_HEADS * hd;
   }
+  a.q_values = tokens * nh * hd;
   a.max_blocks = max_blocks; a.page_shift = page_shift; a.num_pages = num_pages; a.num_rows = num_rows; a.n_rows = n_rows;
   a.nh = nh; a.nkv = nkv; a.subs = subs; a.window = window; a.chunk = chunk; a.sinks = sinks;
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -121,8 +121,8 @@ _SIGNATURES = {
                                c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_unpack_pages": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_paged_decode_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                               c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_int, c_void_p, c_void_p,
-                               c_void_p],
+                               c_longlong, c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_int, c_void_p,
+                               c_void_p, c_void_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
                        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_head_mix": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -1503,7 +1503,7 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
                               dtype=torch.float32, device=q.device)
     _check(library().zb_paged_decode_packed(
         _ptr(out), _ptr(q), _ptr(packed), _ptr(block_table), block_table.shape[1], page_size, pages, block_table.shape[0], _ptr(rows),
-        n_rows, _ptr(row_q_start), _ptr(row_ctx), int(max_context), nh, nkv, hd, int(window), int(chunk), float(scale), float(softcap),
+        n_rows, _ptr(row_q_start), _ptr(row_ctx), int(max_context), q.shape[0], nh, nkv, hd, int(window), int(chunk), float(scale), float(softcap),
         _ptr(sinks), mode, ctas, _ptr(scratch), _ptr(status), _stream()), "paged_decode_packed", 1 if mode == PACKED_CLUSTERS else 2)
     return out
 
