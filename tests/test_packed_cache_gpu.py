@@ -303,7 +303,8 @@ def test_bad_rows_and_pages_are_reported(ops, cuda_device, plan):
         assert torch.equal(got[0], good[0])
 
 
-def test_captured_and_on_a_side_stream(ops, cuda_device):
+@pytest.mark.parametrize("plan", [(0, 2), (1, 296), (2, 148)])
+def test_captured_and_on_a_side_stream(ops, cuda_device, plan):
     """Two captured graphs, replayed at the same time on two streams, with contexts that change between replays."""
     nh, nkv, hd, n = 16, 8, 128, 40
     ctx = [(53 * r) % 700 for r in range(n)]
@@ -314,8 +315,7 @@ def test_captured_and_on_a_side_stream(ops, cuda_device):
     qs = [(torch.randn((n, nh * hd), generator=g) * 1.5).to(torch.bfloat16).to(cuda_device) for _ in range(2)]
     outs = [torch.zeros_like(q) for q in qs]
     def call(i, out):
-        return ops.paged_decode_packed(qs[i], packed, table, rows, starts, contexts, 701, nh, nkv, hd, 0, 0.09, status, out)
-    assert ops.packed_decode_plan(n, nh, nkv, 701)[0] != ops.PACKED_CLUSTERS
+        return ops.paged_decode_packed(qs[i], packed, table, rows, starts, contexts, 701, nh, nkv, hd, 0, 0.09, status, out, plan=plan)
     graphs = []
     for i in range(2):
         graph = torch.cuda.CUDAGraph()

@@ -24,6 +24,7 @@
 // over distributed shared memory; or CTAs, or for many pairs the warps of the CTAs, each for itself, take equal shares of all pairs'
 // tiles laid end to end, and a second kernel merges the pairs that were cut.  More than eight query heads a key/value head run as
 // several pairs.
+#include <atomic>
 #include <type_traits>
 
 #include "packed.cuh"
@@ -776,7 +777,14 @@ int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStr
                       (MODE != PD_CLUSTERS ? (a.n_rows + 1) * sizeof(int) : ranks > 1 ? (8 * 2 + HD) * PD_HEADS * sizeof(float) : 0);
   auto kernel = paged_decode_packed_kernel<HD, MODE>;
   if (smem > 227 * 1024) return ERR_UNSUPPORTED;
-  if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
+  static std::atomic<unsigned long long> raised{0};          // devices on which the kernel may have all it can ever ask for
+  int device = 0;
+  if (cuda_failed(cudaGetDevice(&device))) return ERR_CUDA;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+  if ((raised.load(std::memory_order_relaxed) & bit) == 0) {
+    if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024))) return ERR_CUDA;
+    raised.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(grid);
   config.blockDim = dim3(PD_WARPS * 32);

@@ -10,6 +10,8 @@
 // roundings are directed for that).  A group that holds a value that is not finite reads back as NaN.
 //
 // A lane owns four consecutive channels, eight lanes a group, HD / 4 lanes a head.
+#include <type_traits>
+
 #include "packed.cuh"
 
 namespace zb {
@@ -33,6 +35,7 @@ struct PackedWriteArgs {
   unsigned char* packed;     // null: queries alone
   const int* block_table;    // [num_rows, max_blocks]
   int max_blocks, page_shift, num_pages, num_rows, tokens, nh, nkv;
+  int shared;                // warps of a CTA that share a token
   int* status;
 };
 
@@ -49,143 +52,208 @@ __device__ __forceinline__ void store_four(__nv_bfloat16* p, const float (&x)[4]
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
 }
 
-template <int HD, typename TI, typename TO>
-__global__ void __launch_bounds__(PKW_WARPS * 32)
-qk_norm_rope_packed_kernel(const PackedWriteArgs a) {
-  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, NG = HD / 32;      // (24 lanes: one head a warp)
-  wait_for_prior_grids();
-  let_dependents_launch();
-  const int lane = threadIdx.x & 31, sub = HEADS > 1 ? lane % LANES : lane;
-  const int t = blockIdx.x;
-  const int heads = a.packed != nullptr ? a.nh + 2 * a.nkv : a.nh;
-  const int head = (blockIdx.y * PKW_WARPS + (threadIdx.x >> 5)) * HEADS + (HEADS > 1 ? lane / LANES : 0);
-  const bool active = head < heads && sub < LANES;
-  const bool is_q = head < a.nh, is_k = !is_q && head < a.nh + a.nkv, turns = (is_q || is_k) && a.cos_table != nullptr;
-  const int d = 4 * sub, pos = a.positions[t];
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (active) {
-    load_four(static_cast<const TI*>(a.qkv) + static_cast<size_t>(t) * a.qkv_stride + static_cast<size_t>(head) * HD + d, x);
-    if (a.bias != nullptr) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += a.bias[head * HD + d + e];
-    }
-  }
-  const void* w = is_q ? a.q_norm_w : is_k ? a.k_norm_w : nullptr;
-  float ss = fmaf(x[0], x[0], fmaf(x[1], x[1], fmaf(x[2], x[2], x[3] * x[3])));
-#pragma unroll
-  for (int o = 1; o < (HEADS > 1 ? LANES : 32); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (active && w != nullptr) {
-    const float inv = rsqrtf(ss / static_cast<float>(HD) + a.eps);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] *= inv * load_scale(w, a.norm_w_dtype, d + e);
-  }
-  const bool pos_ok = pos >= 0 && (a.cos_table == nullptr || pos < a.max_positions);
-  if (!pos_ok && lane == 0) report(a.status, STATUS_POSITION_OUT_OF_RANGE, pos, t);
-  if (!pos_ok) return;                         // (the same for the whole CTA)
-  if (a.cos_table != nullptr) {
-    const float* c = a.cos_table + static_cast<size_t>(pos) * a.half;
-    const float* s = a.sin_table + static_cast<size_t>(pos) * a.half;
-    if (a.pairs) {
-      if (active && turns) {
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const int i = (d + e) / 2;
-          if (i < a.half) {
-            const float u = x[e], v = x[e + 1];
-            x[e] = u * c[i] - v * s[i];
-            x[e + 1] = v * c[i] + u * s[i];
-          }
-        }
-      }
-    } else {
-      // The partner's four channels: half a rotated part further, or back.
-      const bool first = d < a.half, mine = d < 2 * a.half;
-      const int from = lane + (!mine ? 0 : first ? a.half / 4 : -(a.half / 4));
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from);
-      if (active && turns && mine) {
-        float cs[4], sn[4];
-        load_four(c + (first ? d : d - a.half), cs);
-        load_four(s + (first ? d : d - a.half), sn);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = first ? x[e] * cs[e] - y[e] * sn[e] : x[e] * cs[e] + y[e] * sn[e];
-      }
-    }
-  }
-  if (active && is_q) {
-    store_four(static_cast<TO*>(a.q_out) + (static_cast<size_t>(t) * a.nh + head) * HD + d, x);
-  }
-  if (a.packed == nullptr) return;
-
-  // The group's least and largest value, and whether all are finite (eight lanes).
+// Codes of a lane's four values, nibble i for value i, and its group's step and offset (eight lanes); all lanes call.
+__device__ __forceinline__ unsigned pk_quantise(const float (&x)[4], __nv_bfloat16& step, __nv_bfloat16& offset) {
   float low = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) bad = bad || !(fabsf(x[e]) <= 3.402823466e38f);
+  // (A product of a value that is not finite with zero is a NaN.)
+  const float zero = fmaf(x[0], 0.0f, fmaf(x[1], 0.0f, fmaf(x[2], 0.0f, x[3] * 0.0f)));
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
   }
-  const unsigned any_bad = __ballot_sync(0xffffffffu, bad) >> (lane & 24) & 0xffu;
-  __nv_bfloat16 offset = __float2bfloat16_rd(low);
+  const unsigned any_bad = __ballot_sync(0xffffffffu, !(zero == 0.0f)) >> (threadIdx.x & 24) & 0xffu;
+  offset = __float2bfloat16_rd(low);
   const float base = __bfloat162float(offset);
-  __nv_bfloat16 step = __float2bfloat16_ru(__fdiv_rn(high - base, 15.0f));
+  step = __float2bfloat16_ru(__fdiv_rn(high - base, 15.0f));
   const float width = __bfloat162float(step);
   unsigned codes = 0;
   if (any_bad || !(width <= 3.0e38f)) {
     offset = __ushort_as_bfloat16(0x7fc0);
     step = __ushort_as_bfloat16(0);
-  } else if (width > 0.0f) {
+  } else if (width >= 1.0e-30f) {
+    // The quotient from a reciprocal is off by some 2^-22: the whole number next to it is right, or off by one where the quotient is
+    // half way between two.  What is left over (exact in float32: a code of 4 bits times a step of 8) says so: it may be half a step,
+    // or with an odd code less than that, so that ties go to the even one.  (No code is below 0 or above 15: the offset is rounded
+    // down, the step up.)
+    constexpr float MAGIC = 12582912.0f;         // 1.5 * 2^23: a sum with it is rounded to whole numbers, ties to even, in its last bits
+    const float inv = __fdiv_rn(1.0f, width), half = 0.5f * width;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float code = fminf(rintf(__fdiv_rn(x[e] - base, width)), 15.0f);       // (never below 0: the offset is rounded down)
-      codes |= static_cast<unsigned>(code) << (4 * e);
+      const float y = x[e] - base, t = fmaf(y, inv, MAGIC), left = fmaf(MAGIC - t, width, y);
+      unsigned code = __float_as_uint(t) & 15u;
+      const float most = __uint_as_float(__float_as_uint(half) - (code & 1u));
+      if (left > most) ++code;
+      if (left < -most) --code;
+      codes |= code << (4 * e);
     }
+  } else if (width > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) codes |= static_cast<unsigned>(rintf(__fdiv_rn(x[e] - base, width))) << (4 * e);
   }
-  const unsigned beside = __shfl_xor_sync(0xffffffffu, codes, 1);
-  if (!active || is_q) return;
-
-  const int row = a.token_row[t], kvh = is_k ? head - a.nh : head - a.nh - a.nkv;
-  const int block = pos >> a.page_shift;
-  if (row < 0 || row >= a.num_rows || block >= a.max_blocks) {
-    if (sub == 0) report(a.status, STATUS_ROW_OUT_OF_RANGE, row, t);
-    return;
-  }
-  const int page = a.block_table[static_cast<size_t>(row) * a.max_blocks + block];
-  if (page <= 0 || page >= a.num_pages) {      // page 0 is the null page and is never written
-    if (sub == 0) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, t);
-    return;
-  }
-  const int in_page = pos & ((1 << a.page_shift) - 1), p = in_page & (PK_BLOCK - 1);
-  unsigned char* dst = a.packed + (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + (in_page >> 4)) * pk_block_bytes(HD);
-  const int g = sub & 7, m = sub >> 3;          // the lane's place in its group, and the group
-  if (is_k) {
-    if ((g & 1) == 0) *reinterpret_cast<unsigned*>(dst + pk_key_word<HD>(p, g >> 1, m)) = codes | (beside << 16);
-    if (g == 0) {
-      *reinterpret_cast<__nv_bfloat16*>(dst + pk_key_step<HD>(p, m)) = step;
-      *reinterpret_cast<__nv_bfloat16*>(dst + pk_key_step<HD>(p, m) + 2 * NG) = offset;
-    }
-  } else {
-    *reinterpret_cast<unsigned short*>(dst + pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m) + 2 * (p & 1)) = static_cast<unsigned short>(codes);
-    if (g == 0) {
-      *reinterpret_cast<__nv_bfloat16*>(dst + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1)) = step;
-      *reinterpret_cast<__nv_bfloat16*>(dst + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1) + 4 * NG) = offset;
-    }
-  }
+  return codes;
 }
 
+__device__ __forceinline__ void load_scales(const void* w, int w_dtype, int d, float (&s)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = load_scale(w, w_dtype, d + e);
+}
+
+// A warp takes every so many'th run of query, key and value heads of one token (a run: as many heads as have lanes in a warp), UNITS of
+// them at a time, whose values are all asked for before the first is used; the token's place, its angles and the scales serve all.
+// (Eight channels a lane take as many instructions and more registers: 2048 tokens of 32 / 8 heads 24 to 30 us.)
+template <int HD, int UNITS, typename TI, typename TO>
+__global__ void __launch_bounds__(PKW_WARPS * 32)
+qk_norm_rope_packed_kernel(const PackedWriteArgs a) {
+  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, NG = HD / 32;      // (24 lanes: one head a warp)
+  wait_for_prior_grids();
+  let_dependents_launch();
+  const int lane = threadIdx.x & 31, sub = HEADS > 1 ? lane % LANES : lane, among = HEADS > 1 ? lane / LANES : 0;
+  const bool lane_ok = sub < LANES;
+  // A token has `shared` warps of the CTA, and as many of every CTA beside it (grid y).
+  const int warp = threadIdx.x >> 5, t = blockIdx.x * (PKW_WARPS / a.shared) + warp / a.shared;
+  if (t >= a.tokens) return;
+  const int d = lane_ok ? 4 * sub : 0, pos = a.positions[t];
+  const int stride = gridDim.y * a.shared, own = blockIdx.y * a.shared + warp % a.shared;
+  const TI* const from = static_cast<const TI*>(a.qkv) + static_cast<size_t>(t) * a.qkv_stride + d;
+  const bool pos_ok = pos >= 0 && (a.cos_table == nullptr || pos < a.max_positions);
+  if (!pos_ok) {                               // (the same for all of the token's warps)
+    if (lane == 0) report(a.status, STATUS_POSITION_OUT_OF_RANGE, pos, t);
+    return;
+  }
+  // Where the token's keys and values go: its block in the first head's part of the page.
+  const int in_page = pos & ((1 << a.page_shift) - 1), p = in_page & (PK_BLOCK - 1);
+  unsigned char* to = nullptr;
+  if (a.packed != nullptr) {
+    const int row = a.token_row[t], entry = pos >> a.page_shift;
+    if (row < 0 || row >= a.num_rows || entry >= a.max_blocks) {
+      if (own == 0 && lane == 0) report(a.status, STATUS_ROW_OUT_OF_RANGE, row, t);
+    } else {
+      const int page = a.block_table[static_cast<size_t>(row) * a.max_blocks + entry];
+      if (page <= 0 || page >= a.num_pages) {  // page 0 is the null page and is never written
+        if (own == 0 && lane == 0) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, t);
+      } else {
+        to = a.packed + ((static_cast<long long>(page) * a.nkv << (a.page_shift - 4)) + (in_page >> 4)) * pk_block_bytes(HD);
+      }
+    }
+  }
+  // This lane's angles: of pairs (d, d + 1), (d + 2, d + 3); or of d .. d + 3 and their partners, half a rotated part further or back.
+  const bool turned = a.cos_table != nullptr, normed = a.q_norm_w != nullptr, mine = turned && d < 2 * a.half && lane_ok, front = d < a.half;
+  float cs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (mine) {
+    const float* c = a.cos_table + static_cast<size_t>(pos) * a.half;
+    const float* s = a.sin_table + static_cast<size_t>(pos) * a.half;
+    if (a.pairs) {
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const int i = (d + e) / 2;
+        if (i < a.half) {
+          cs[e] = cs[e + 1] = c[i];
+          sn[e] = -s[i];
+          sn[e + 1] = s[i];
+        }
+      }
+    } else {
+      load_four(c + (front ? d : d - a.half), cs);
+      load_four(s + (front ? d : d - a.half), sn);
+      if (front) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sn[e] = -sn[e];
+      }
+    }
+  }
+  const int partner = !mine ? lane : front ? lane + a.half / 4 : lane - a.half / 4;
+  const int g = sub & 7, m = sub >> 3;          // the lane's place in its group of channels, and the group
+
+  // The heads of one kind: 0 queries, 1 keys, 2 values.
+  // (Runs of all kinds are counted through, so that every warp has as many.)
+  auto work = [&](auto which, int head0, int heads, int passed, const void* norm_w) {
+    constexpr int KIND = decltype(which)::value;
+    const int start = (own - passed % stride + stride) % stride;
+    if (start * HEADS >= heads) return;
+    float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (KIND < 2 && normed) load_scales(norm_w, a.norm_w_dtype, d, scale);
+    // A codes' place: of the keys' word that two lanes share, or of the values' half word.
+    unsigned char* const codes_to = KIND == 1 ? to + pk_key_word<HD>(p, g >> 1, m) : to + pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m) + 2 * (p & 1);
+    unsigned char* const steps_to = KIND == 1 ? to + pk_key_step<HD>(p, m) : to + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1);
+    for (int first = start * HEADS; first < heads; first += UNITS * stride * HEADS) {
+      float x[UNITS][4];
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int head = first + u * stride * HEADS + among;
+        x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+        if (head < heads && lane_ok) load_four(from + static_cast<size_t>(head0 + head) * HD, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        if (first + u * stride * HEADS >= heads) break;               // (the same for the warp)
+        const int head = first + u * stride * HEADS + among;
+        const bool active = head < heads && lane_ok;
+        float (&v)[4] = x[u];
+        if (a.bias != nullptr && active) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += a.bias[(head0 + head) * HD + d + e];
+        }
+        if (KIND < 2 && normed) {
+          float ss = fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3])));
+#pragma unroll
+          for (int o = 1; o < (HEADS > 1 ? LANES : 32); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * (1.0f / static_cast<float>(HD)) + a.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= inv * scale[e];
+        }
+        if (KIND < 2 && turned) {
+          float y[4];
+          if (a.pairs) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = v[e ^ 1];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, v[e], partner);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], sn[e], v[e] * cs[e]);      // (times 0 and 1 where nothing turns)
+        }
+        if (KIND == 0) {
+          if (active) store_four(static_cast<TO*>(a.q_out) + (static_cast<size_t>(t) * a.nh + head) * HD + d, v);
+          continue;
+        }
+        __nv_bfloat16 step, offset;
+        unsigned codes = pk_quantise(v, step, offset);
+        if (KIND == 1) codes |= __shfl_xor_sync(0xffffffffu, codes, 1) << 16;
+        if (!active || to == nullptr) continue;
+        const long long at = (static_cast<long long>(head) << (a.page_shift - 4)) * pk_block_bytes(HD);
+        if (KIND == 1 && (g & 1) == 0) *reinterpret_cast<unsigned*>(codes_to + at) = codes;
+        if (KIND == 2) *reinterpret_cast<unsigned short*>(codes_to + at) = static_cast<unsigned short>(codes);
+        if (g == 0) {
+          *reinterpret_cast<__nv_bfloat16*>(steps_to + at) = step;
+          *reinterpret_cast<__nv_bfloat16*>(steps_to + at + (KIND == 1 ? 2 : 4) * NG) = offset;
+        }
+      }
+    }
+  };
+  const int q_runs = (a.nh + HEADS - 1) / HEADS, k_runs = (a.nkv + HEADS - 1) / HEADS;
+  work(std::integral_constant<int, 0>{}, 0, a.nh, 0, a.q_norm_w);
+  if (a.packed == nullptr) return;
+  work(std::integral_constant<int, 1>{}, a.nh, a.nkv, q_runs, a.k_norm_w);
+  work(std::integral_constant<int, 2>{}, a.nh + a.nkv, a.nkv, q_runs + k_runs, nullptr);
+}
+
+// Many tokens: SHARED warps a token, four runs of heads at a time.  Few: a run a warp.
 template <int HD, typename TI, typename TO>
-int packed_write_launch(const PackedWriteArgs& a, cudaStream_t stream) {
-  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1;
-  const int heads = a.packed != nullptr ? a.nh + 2 * a.nkv : a.nh;
-  const int per_block = PKW_WARPS * HEADS, across = (heads + per_block - 1) / per_block;
-  if (across > 65535) return ERR_UNSUPPORTED;
-  return launch_dependent(qk_norm_rope_packed_kernel<HD, TI, TO>, dim3(a.tokens, across), dim3(PKW_WARPS * 32), 0, stream, false, a);
+int packed_write_launch(PackedWriteArgs& a, cudaStream_t stream) {
+  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, SHARED = 2;
+  const dim3 threads(PKW_WARPS * 32);
+  if (a.tokens > 64) {
+    a.shared = SHARED;
+    const int tokens = PKW_WARPS / SHARED;
+    return launch_dependent(qk_norm_rope_packed_kernel<HD, 4, TI, TO>, dim3((a.tokens + tokens - 1) / tokens), threads, 0, stream, false, a);
+  }
+  const int runs = (a.nh + HEADS - 1) / HEADS + (a.packed != nullptr ? 2 * ((a.nkv + HEADS - 1) / HEADS) : 0), across = (runs + PKW_WARPS - 1) / PKW_WARPS;
+  return launch_dependent(qk_norm_rope_packed_kernel<HD, 1, TI, TO>, dim3(a.tokens, across > 65535 ? 65535 : across), threads, 0, stream, false, a);
 }
 template <int HD>
-int packed_write_types(const PackedWriteArgs& a, int in_dtype, int out_dtype, cudaStream_t stream) {
+int packed_write_types(PackedWriteArgs& a, int in_dtype, int out_dtype, cudaStream_t stream) {
   if (in_dtype == DTYPE_BF16 && out_dtype == DTYPE_BF16) return packed_write_launch<HD, __nv_bfloat16, __nv_bfloat16>(a, stream);
   if (in_dtype == DTYPE_F32 && out_dtype == DTYPE_BF16) return packed_write_launch<HD, float, __nv_bfloat16>(a, stream);
   if (in_dtype == DTYPE_F32 && out_dtype == DTYPE_F32) return packed_write_launch<HD, float, float>(a, stream);
@@ -270,9 +338,9 @@ ZB_API int zb_qk_norm_rope_packed(void* q_out, const void* qkv, long long qkv_st
     return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
   if (tokens == 0) return OK;
-  const PackedWriteArgs a = {q_out, qkv, qkv_stride, bias, q_norm_w, k_norm_w, norm_w_dtype, eps, cos_table, sin_table, half, max_positions,
+  PackedWriteArgs a = {q_out, qkv, qkv_stride, bias, q_norm_w, k_norm_w, norm_w_dtype, eps, cos_table, sin_table, half, max_positions,
                              pairs, positions, token_row, static_cast<unsigned char*>(packed), block_table, max_blocks, page_shift, num_pages,
-                             num_rows, tokens, nh, nkv, status};
+                             num_rows, tokens, nh, nkv, PKW_WARPS, status};
   const auto s = static_cast<cudaStream_t>(stream);
   switch (hd) {
     case 32: return packed_write_types<32>(a, in_dtype, out_dtype, s);

@@ -1340,7 +1340,8 @@ PACKED_BLOCK = 16           # positions per block
 def packed_block_bytes(hd: int) -> int:
     """Bytes of a block of 16 positions' keys and values of one head in a 4-bit cache: a code of 4 bits a value, a step and an offset in
     bfloat16 for every 32 channels of a key or value.  The layout is in csrc/packed.cuh."""
-    _require(hd in PACKED_HEAD_DIMS, f"a 4-bit cache takes head sizes {PACKED_HEAD_DIMS}, not {hd}")
+    if hd not in PACKED_HEAD_DIMS:
+        raise InvalidArgumentError(f"a 4-bit cache takes head sizes {PACKED_HEAD_DIMS}, not {hd}")
     return 20 * hd
 
 
@@ -1354,26 +1355,31 @@ def packed_cache_shape(pages: int, nkv: int, page_size: int, hd: int) -> tuple[i
     return pages, nkv, page_size // PACKED_BLOCK, packed_block_bytes(hd)
 
 
+# (The calls below are made for every layer of a step: their checks make a message only where one fails.)
 def _check_packed(packed: torch.Tensor, nkv: int, hd: int) -> tuple[int, int]:
-    block = packed_block_bytes(hd)
-    _require(packed.dtype == torch.uint8 and packed.dim() == 4 and packed.is_contiguous() and packed.shape[1] == nkv
-             and packed.shape[3] == block, f"a 4-bit cache must be a contiguous uint8 [pages, kv_heads, page_size / 16, {block}] tensor")
-    page_size = packed.shape[2] * PACKED_BLOCK
-    _require(packed_page_size_ok(page_size), "the pages of a 4-bit cache hold a power of two of positions, 16 or more")
-    _require(packed.data_ptr() % 16 == 0, "a 4-bit cache must start on a 16-byte boundary")
-    return packed.shape[0], page_size
+    block, shape = packed_block_bytes(hd), packed.shape
+    if len(shape) != 4 or shape[1] != nkv or shape[3] != block or packed.dtype != torch.uint8 or not packed.is_contiguous():
+        raise InvalidArgumentError(f"a 4-bit cache must be a contiguous uint8 [pages, {nkv}, page_size / 16, {block}] tensor")
+    page_size = shape[2] * PACKED_BLOCK
+    if not packed_page_size_ok(page_size):
+        raise InvalidArgumentError("the pages of a 4-bit cache hold a power of two of positions, 16 or more")
+    if packed.data_ptr() % 16 != 0:
+        raise InvalidArgumentError("a 4-bit cache must start on a 16-byte boundary")
+    return shape[0], page_size
 
 
 def _same_device(*tensors: torch.Tensor | None) -> None:
     """Kernels are launched on the current device's current stream: all they are given lies there."""
-    _cuda(*tensors)
-    current = torch.cuda.current_device()
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
     for t in tensors:
-        _require(t is None or t.device.index == current, f"tensors of one call lie on the current device, cuda:{current}")
+        if t is not None and t.get_device() != current:       # (-1: a tensor on the CPU)
+            _cuda(t)
+            raise InvalidArgumentError(f"tensors of one call lie on the current device, cuda:{current}, not on {t.device}")
 
 
 def _check_status_word(status: torch.Tensor) -> None:
-    _require(status.dtype == torch.int32 and status.is_contiguous() and status.numel() >= 3, "status must be an int32 status word (new_status)")
+    if status.dtype != torch.int32 or status.numel() < 3 or not status.is_contiguous():
+        raise InvalidArgumentError("status must be an int32 status word (new_status)")
 
 
 def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w: torch.Tensor | None, k_norm_w: torch.Tensor | None,
@@ -1391,46 +1397,50 @@ def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w:
     column.  A (row, position) comes once in a call."""
     _i32(positions, token_row, block_table)
     _check_status_word(status)
-    T = qkv.shape[0]
-    dtype = dtype or qkv.dtype
-    _require(hd in PACKED_HEAD_DIMS, f"a 4-bit cache takes head sizes {PACKED_HEAD_DIMS}, not {hd}")
-    _require(nh > 0 and nkv > 0, "head counts must be positive")
+    T, in_dtype = qkv.shape[0], qkv.dtype
+    dtype = dtype or in_dtype
+    if hd not in PACKED_HEAD_DIMS or nh <= 0 or nkv <= 0:
+        raise InvalidArgumentError(f"a 4-bit cache takes positive head counts and head sizes {PACKED_HEAD_DIMS}, not {nh}, {nkv}, {hd}")
     width = (nh + 2 * nkv) * hd if packed is not None else nh * hd
-    _require(qkv.dim() == 2 and qkv.shape[1] >= width and qkv.stride(1) == 1 and qkv.dtype in DTYPE_CODE,
-             "qkv must be [T, (heads + 2*kv_heads)*head_dim] with unit inner stride")
-    _require(T <= 1 or qkv.stride(0) >= width, "rows of qkv must not overlap")
-    _require(qkv.data_ptr() % (4 * qkv.element_size()) == 0 and qkv.stride(0) % 4 == 0,
-             "rows of qkv must start on boundaries of four values")
-    _require(dtype == torch.bfloat16 or (dtype == torch.float32 and qkv.dtype == torch.float32),
-             "the queries are bfloat16, or float32 where qkv is")
-    _require(positions.numel() == T and token_row.numel() == T and block_table.dim() == 2, "one position and row per token")
+    if qkv.dim() != 2 or qkv.shape[1] < width or qkv.stride(1) != 1 or in_dtype not in DTYPE_CODE:
+        raise InvalidArgumentError("qkv must be [T, (heads + 2*kv_heads)*head_dim] with unit inner stride")
+    stride = qkv.stride(0) if T > 1 else width
+    if stride < width or stride % 4 != 0 or qkv.data_ptr() % (16 if in_dtype == torch.float32 else 8) != 0:
+        raise InvalidArgumentError("rows of qkv must not overlap and must start on boundaries of four values")
+    if dtype != torch.bfloat16 and not (dtype == in_dtype == torch.float32):
+        raise InvalidArgumentError("the queries are bfloat16, or float32 where qkv is")
+    if positions.numel() != T or token_row.numel() != T or block_table.dim() != 2:
+        raise InvalidArgumentError("one position and row per token, and a block_table [rows, blocks]")
     w_code = 0
     if q_norm_w is not None or k_norm_w is not None:
-        _require(q_norm_w is not None and k_norm_w is not None and q_norm_w.dtype == k_norm_w.dtype,
-                 "q and k norm scales come together and share a type")
+        if q_norm_w is None or k_norm_w is None or q_norm_w.dtype != k_norm_w.dtype:
+            raise InvalidArgumentError("q and k norm scales come together and share a type")
         w_code = _scale_code(q_norm_w, hd)
         _scale_code(k_norm_w, hd)
-    _require(layout in ("halves", "pairs"), "layout is 'halves' or 'pairs'")
+    if layout not in ("halves", "pairs") or (cos is None) != (sin is None):
+        raise InvalidArgumentError("layout is 'halves' or 'pairs', and cos and sin come together")
     half, max_positions = 0, 0
-    _require((cos is None) == (sin is None), "cos and sin come together")
     if cos is not None:
-        _require(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2
-                 and cos.is_contiguous() and sin.is_contiguous(), "cos/sin must be contiguous float32 [positions, rotated / 2]")
+        if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                or not cos.is_contiguous() or not sin.is_contiguous()):
+            raise InvalidArgumentError("cos/sin must be contiguous float32 [positions, rotated / 2]")
         max_positions, half = cos.shape
-        _require(0 < 2 * half <= hd and (layout == "pairs" or half % 4 == 0),
-                 "the rotated channels are part of the head, in halves a multiple of 8 of them")
-        _require(layout == "pairs" or (cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0), "cos/sin must start on 16-byte boundaries")
-    _require(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == width), f"bias: {width} float32 values")
+        if not 0 < 2 * half <= hd or (layout == "halves" and (half % 4 != 0 or cos.data_ptr() % 16 != 0 or sin.data_ptr() % 16 != 0)):
+            raise InvalidArgumentError("the rotated channels are part of the head, in halves a multiple of 8 of them with cos/sin on "
+                                       "16-byte boundaries")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != width or not bias.is_contiguous()):
+        raise InvalidArgumentError(f"bias: {width} float32 values")
     pages, page_size = _check_packed(packed, nkv, hd) if packed is not None else (0, PACKED_BLOCK)
     _same_device(qkv, positions, token_row, block_table, status, packed, q_norm_w, k_norm_w, cos, sin, bias, q_out)
     if q_out is None:
         q_out = torch.empty((T, nh * hd), dtype=dtype, device=qkv.device)
-    _require(q_out.shape == (T, nh * hd) and q_out.is_contiguous() and q_out.dtype == dtype and q_out.data_ptr() % 16 == 0, "q_out shape")
+    elif q_out.shape != (T, nh * hd) or q_out.dtype != dtype or not q_out.is_contiguous() or q_out.data_ptr() % 16 != 0:
+        raise InvalidArgumentError("q_out must be contiguous [T, heads*head_dim] on a 16-byte boundary")
     _check(library().zb_qk_norm_rope_packed(
-        _ptr(q_out), _ptr(qkv), qkv.stride(0) if T > 1 else width, _ptr(bias), _ptr(q_norm_w), _ptr(k_norm_w), w_code, float(eps), _ptr(cos), _ptr(sin),
-        half, max_positions, int(layout == "pairs"), _ptr(positions), _ptr(token_row), _ptr(packed), _ptr(block_table),
-        block_table.shape[1], page_size, pages, block_table.shape[0], T, nh, nkv, hd, DTYPE_CODE[qkv.dtype], DTYPE_CODE[dtype],
-        _ptr(status), _stream()), "qk_norm_rope_packed")
+        q_out.data_ptr(), qkv.data_ptr(), stride, _ptr(bias), _ptr(q_norm_w), _ptr(k_norm_w), w_code, eps, _ptr(cos), _ptr(sin), half,
+        max_positions, layout == "pairs", positions.data_ptr(), token_row.data_ptr(), _ptr(packed), block_table.data_ptr(),
+        block_table.shape[1], page_size, pages, block_table.shape[0], T, nh, nkv, hd, DTYPE_CODE[in_dtype], DTYPE_CODE[dtype],
+        status.data_ptr(), _stream()), "qk_norm_rope_packed")
     return q_out
 
 
@@ -1438,47 +1448,67 @@ def unpack_pages(packed: torch.Tensor, pages: torch.Tensor, dtype: torch.dtype, 
     """What the given pages (int32) of a 4-bit cache stand for: [pages, 2 (keys, values), kv_heads, page_size, head_dim] in ``dtype``,
     channels in their natural order.  A page outside the cache is reported, and its part of the result is not written."""
     _i32(pages)
-    _require(dtype in DTYPE_CODE, "values are bfloat16 or float32")
-    _require(packed.dim() == 4 and packed.shape[3] % 20 == 0, "a 4-bit cache must be [pages, kv_heads, page_size / 16, 20 * head_dim]")
+    if dtype not in DTYPE_CODE:
+        raise InvalidArgumentError("values are bfloat16 or float32")
+    if packed.dim() != 4 or packed.shape[3] % 20 != 0:
+        raise InvalidArgumentError("a 4-bit cache must be [pages, kv_heads, page_size / 16, 20 * head_dim]")
     nkv, hd = packed.shape[1], packed.shape[3] // 20
     num_pages, page_size = _check_packed(packed, nkv, hd)
     if status is not None:
         _check_status_word(status)
     _same_device(packed, pages, status)
     out = torch.empty((pages.numel(), 2, nkv, page_size, hd), dtype=dtype, device=packed.device)
-    _check(library().zb_unpack_pages(_ptr(out), _ptr(packed), _ptr(pages), pages.numel(), num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
-                                     _ptr(status) if status is not None else _device_status_pointer(packed.device), _stream()),
-           "unpack_pages")
+    _check(library().zb_unpack_pages(
+        out.data_ptr(), packed.data_ptr(), pages.data_ptr(), pages.numel(), num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
+        status.data_ptr() if status is not None else _device_status_pointer(packed.device), _stream()), "unpack_pages")
     return out
 
 
-def _packed_attention_args(q, packed, block_table, status, out, nh, nkv, hd, window, chunk, softcap, sinks) -> tuple[int, int]:
+def _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk, softcap,
+                           sinks) -> tuple[int, int]:
+    """(pages, page size), once everything that the two kinds of attention over a 4-bit cache share is found right."""
     _check_status_word(status)
-    _require(nh > 0 and nkv > 0 and nh % nkv == 0, "head counts must be positive, heads divisible by kv_heads")
-    _require(q.dim() == 2 and q.is_contiguous() and q.shape[1] == nh * hd and q.dtype in DTYPE_CODE and q.data_ptr() % 16 == 0,
-             "q must be contiguous [T, heads*head_dim], bfloat16 or float32, on a 16-byte boundary")
-    _require(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must match q")
-    _require(block_table.dim() == 2 and window >= 0 and chunk >= 0 and softcap >= 0.0,
-             "block_table is [rows, blocks]; window, chunk and softcap are not negative")
-    _require(sinks is None or (sinks.dtype == torch.float32 and sinks.is_contiguous() and sinks.numel() == nh),
-             "one float32 sink per query head")
+    if nh <= 0 or nkv <= 0 or nh % nkv != 0:
+        raise InvalidArgumentError("head counts must be positive, heads divisible by kv_heads")
+    if q.dim() != 2 or q.shape[1] != nh * hd or q.dtype != torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16 != 0:
+        raise InvalidArgumentError("q must be contiguous bfloat16 [T, heads*head_dim] on a 16-byte boundary")
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16 != 0:
+        raise InvalidArgumentError("out must match q")
+    if block_table.dim() != 2 or row_q_start.numel() < block_table.shape[0] or row_ctx.numel() < block_table.shape[0]:
+        raise InvalidArgumentError("block_table is [rows, blocks], with one start and context per row")
+    if window < 0 or chunk < 0 or not softcap >= 0.0:
+        raise InvalidArgumentError("window, chunk and softcap are not negative")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nh or not sinks.is_contiguous()):
+        raise InvalidArgumentError("one float32 sink per query head")
     return _check_packed(packed, nkv, hd)
 
 
 PACKED_CLUSTERS, PACKED_CTA_SHARES, PACKED_WARP_SHARES = 0, 1, 2
 
 
-def packed_decode_plan(n_rows: int, nh: int, nkv: int, max_context: int) -> tuple[int, int]:
-    """How ``paged_decode_packed`` cuts its rows' contexts: a cluster of n CTAs a (row, key/value head) pair, or shares for n CTAs or
-    their warps."""
+def packed_decode_plan(n_rows: int, nh: int, nkv: int, visible: int) -> tuple[int, int]:
+    """How ``paged_decode_packed`` cuts contexts of which up to ``visible`` positions are seen: a cluster of n CTAs a (row, key/value
+    head) pair, or equal shares of all pairs for n CTAs or their warps, whose parts a second kernel merges (some 9 us more).
+
+    Two CTAs an SM.  A cluster doubles while its shares stay above 128 positions and every CTA has an SM, and on to two an SM while
+    shares stay above 2048 (us: 4 rows of 600, 8 key/value heads, 1 / 2 / 4 / 8 CTAs 8.4 / 8.3 / 7.7 / 9.0; 12 of 1000, 1 / 2 10.2 /
+    11.5; 8 of 4096, 2 / 4 18.2 / 18.4; 4 of 16384, 4 / 8 33 / 26).  A warp takes 1.2 us for 32 positions while few
+    SMs read, 2 with two CTAs on every SM; so long contexts of few pairs are cheaper in shares (1 row of 40000 in clusters of 8 / shares 32 / 24, 2 rows 46 /
+    33; 1 of 4096 8.9 / 10.2), and more pairs than CTAs in warps' shares, which also even out rows of unequal lengths (64 rows of 4096
+    in whole contexts / shares 74 / 74, of 1 to 4096 56 / 47, 256 of 64 41 / 16), unless they are not many and short (64 of 300 17.5 /
+    20.5, of 1000 31 / 33)."""
     pairs = n_rows * nkv * -(-nh // nkv // 8)
-    slots = 2 * _sm_count()
-    if pairs > slots:
-        return PACKED_WARP_SHARES, slots
-    ranks = 1
-    while ranks < 8 and 2 * ranks * pairs <= slots and max_context > 256 * ranks:
-        ranks *= 2
-    return PACKED_CLUSTERS, ranks
+    sms = _sm_count()
+    if pairs > 2 * sms:
+        return (PACKED_CLUSTERS, 1) if pairs <= 4 * sms and visible <= 1024 else (PACKED_WARP_SHARES, 2 * sms)
+    ctas = 1
+    while ctas < 8 and visible > 256 * ctas and (2 * ctas * pairs <= sms or (2 * ctas * pairs <= 2 * sms and visible >= 4096 * ctas)):
+        ctas *= 2
+    tiles = -(-visible // 32)
+    us = 1.2 if 2 * pairs * ctas <= sms else (1.6 if pairs * ctas <= sms else 2.0)
+    if tiles / (8 * ctas) * us <= pairs * tiles / (8 * sms) + 9.0:
+        return PACKED_CLUSTERS, ctas
+    return PACKED_CTA_SHARES, (1 if pairs * tiles < 8192 else 2) * sms
 
 
 def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, row_q_start: torch.Tensor,
@@ -1490,21 +1520,24 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
     least the longest context of the rows, the new token included.  ``plan``: as ``packed_decode_plan`` gives it (None: chosen by
     that).  The scratch of a launch is the call's own."""
     _i32(block_table, rows, row_q_start, row_ctx)
-    pages, page_size = _packed_attention_args(q, packed, block_table, status, out, nh, nkv, hd, window, chunk, softcap, sinks)
-    _require(q.dtype == torch.bfloat16, "the 4-bit decode attention takes bfloat16 queries")
-    _require(row_q_start.numel() >= block_table.shape[0] and row_ctx.numel() >= block_table.shape[0], "one start and context per row")
+    pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk,
+                                              softcap, sinks)
     _same_device(q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
     n_rows = rows.numel()
-    mode, ctas = plan or packed_decode_plan(n_rows, nh, nkv, min([max_context] + [n for n in (window, chunk) if n > 0]))
+    if plan is None:
+        visible = min(max_context, window) if window else max_context
+        plan = packed_decode_plan(n_rows, nh, nkv, min(visible, chunk) if chunk else visible)
+    mode, ctas = plan
     scratch = None
     if mode != PACKED_CLUSTERS and n_rows > 0:
         pairs = n_rows * nkv * -(-nh // nkv // 8)
         scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(ctas, int(mode == PACKED_WARP_SHARES), pairs, hd)),
                               dtype=torch.float32, device=q.device)
     _check(library().zb_paged_decode_packed(
-        _ptr(out), _ptr(q), _ptr(packed), _ptr(block_table), block_table.shape[1], page_size, pages, block_table.shape[0], _ptr(rows),
-        n_rows, _ptr(row_q_start), _ptr(row_ctx), int(max_context), q.shape[0], nh, nkv, hd, int(window), int(chunk), float(scale), float(softcap),
-        _ptr(sinks), mode, ctas, _ptr(scratch), _ptr(status), _stream()), "paged_decode_packed", 1 if mode == PACKED_CLUSTERS else 2)
+        out.data_ptr(), q.data_ptr(), packed.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, pages,
+        block_table.shape[0], rows.data_ptr(), n_rows, row_q_start.data_ptr(), row_ctx.data_ptr(), max_context, q.shape[0], nh, nkv, hd,
+        window, chunk, scale, softcap, _ptr(sinks), mode, ctas, _ptr(scratch), status.data_ptr(), _stream()), "paged_decode_packed",
+        1 if mode == PACKED_CLUSTERS else 2)
     return out
 
 
