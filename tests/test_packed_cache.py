@@ -68,6 +68,25 @@ def test_decode_refuses(what):
         ops.paged_decode_packed(**decode_args(**DECODE_REFUSALS[what]))
 
 
+def prompt_args(**change):
+    a = decode_args()
+    for name in ("rows", "max_context"):
+        del a[name]
+    a.update(tile_row=torch.arange(2, dtype=torch.int32), tile_q0=torch.zeros(2, dtype=torch.int32), row_q_len=torch.ones(2, dtype=torch.int32))
+    a.update(change)
+    return a
+
+
+PROMPT_REFUSALS = {**{k: v for k, v in DECODE_REFUSALS.items()}, "tiles": dict(tile_q0=torch.zeros(3, dtype=torch.int32)),
+                   "lengths": dict(row_q_len=torch.ones(1, dtype=torch.int32)), "lengths' type": dict(row_q_len=torch.ones(2))}
+
+
+@pytest.mark.parametrize("what", PROMPT_REFUSALS)
+def test_prompts_refuse(what):
+    with pytest.raises(InvalidArgumentError):
+        ops.paged_prefill_packed(**prompt_args(**PROMPT_REFUSALS[what]))
+
+
 def write_args(**change):
     nh, nkv, hd = 8, 2, 64
     a = dict(qkv=torch.zeros((2, (nh + 2 * nkv) * hd), dtype=torch.bfloat16), nh=nh, nkv=nkv, hd=hd, q_norm_w=torch.ones(hd), k_norm_w=torch.ones(hd),
@@ -115,6 +134,8 @@ def test_sizes_are_refused():
 def test_there_is_no_cpu_path():
     with pytest.raises(KernelError):
         ops.paged_decode_packed(**decode_args())
+    with pytest.raises(KernelError):
+        ops.paged_prefill_packed(**prompt_args())
     with pytest.raises(KernelError):
         ops.qk_norm_rope_packed(**write_args())
     with pytest.raises(KernelError):

@@ -303,6 +303,69 @@ def test_bad_rows_and_pages_are_reported(ops, cuda_device, plan):
         assert torch.equal(got[0], good[0])
 
 
+# -------------------------------------------------------------------------------------------- prompts
+PROMPTS = [
+    # nh, nkv, hd, page, new tokens, cached, masks
+    (16, 8, 128, 16, [2], [0], {}),
+    (8, 2, 128, 16, [129, 1, 128, 63], [0, 5, 127, 700], {}),
+    (8, 4, 128, 32, [300], [1000], {}),
+    (6, 2, 128, 64, [200, 17], [64, 0], dict(window=90, sinks=True, softcap=15.0)),
+    (4, 4, 128, 16, [260, 50], [33, 250], dict(chunk=100)),
+    (3, 3, 128, 16, [40], [129], dict(window=1)),
+    (20, 2, 128, 16, [140], [0], dict(sinks=True)),
+    (12, 4, 64, 16, [333, 90, 2], [100, 0, 61], {}),
+    (5, 5, 96, 32, [70, 130], [31, 0], dict(chunk=64, sinks=True)),
+    (6, 3, 32, 64, [65, 64], [0, 300], dict(window=100, softcap=10.0)),
+    (2, 1, 64, 16, [16], [15], dict(window=17)),
+]
+
+
+@pytest.mark.parametrize("tensor_memory", [True, False])
+@pytest.mark.parametrize("nh,nkv,hd,page,new,cached,masks", PROMPTS)
+def test_prompts(ops, cuda_device, nh, nkv, hd, page, new, cached, masks, tensor_memory):
+    if hd != 128 and tensor_memory:
+        pytest.skip("this head size has one kernel")
+    packed, table, rows = paged_case(cuda_device, nkv, hd, page, [c + n for n, c in zip(new, cached)], 59)
+    g = torch.Generator().manual_seed(61)
+    T, starts = sum(new), [sum(new[:r]) for r in range(len(new))]
+    q = (torch.randn((T, nh * hd), generator=g) * 1.5).to(torch.bfloat16)
+    masks = dict(masks)
+    sinks = torch.randn(nh, generator=g) if masks.pop("sinks", False) else None
+    scale, status = 1 / math.sqrt(hd), ops.new_status(cuda_device)
+    tile = ops.paged_prefill_tile_tokens()
+    tiles = sorted((cached[r] + q0, r, q0) for r, n in enumerate(new) for q0 in range(0, n, tile))
+    out = torch.full((T, nh * hd), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+    ops.paged_prefill_packed(q.to(cuda_device), packed, table, i32(cuda_device, [t[1] for t in tiles]), i32(cuda_device, [t[2] for t in tiles]),
+                             i32(cuda_device, starts), i32(cuda_device, new), i32(cuda_device, cached), nh, nkv, hd, masks.get("window", 0), scale,
+                             status, out, chunk=masks.get("chunk", 0), softcap=masks.get("softcap", 0.0),
+                             sinks=None if sinks is None else sinks.to(cuda_device), tensor_memory=tensor_memory)
+    ops.check_status(status)
+    for r, n in enumerate(new):
+        mine = slice(starts[r], starts[r] + n)
+        expected, bound = plain.attention(q[mine].double().view(n, nh, hd), *rows[r], cached[r] + torch.arange(n), scale, sinks=sinks, rounded=True, **masks)
+        assert ((out[mine].cpu().double().view(n, nh, hd) - expected).abs() <= bound).all(), r
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompts_report_bad_pages_and_rows(ops, cuda_device, hd):
+    nh, nkv, new, cached = 4, 2, [150, 140], [40, 20]
+    packed, table, _ = paged_case(cuda_device, nkv, hd, 16, [c + n for n, c in zip(new, cached)], 67)
+    q = torch.randn((290, nh * hd), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda_device)
+    def call(table, tile_row, status):
+        return ops.paged_prefill_packed(q, packed, table, i32(cuda_device, tile_row), i32(cuda_device, [0, 0, 128, 128]), i32(cuda_device, [0, 150]),
+                                        i32(cuda_device, new), i32(cuda_device, cached), nh, nkv, hd, 0, 0.1, status, torch.zeros_like(q))
+    good = call(table, [0, 1, 0, 1], ops.new_status(cuda_device))
+    for page, tile_row, code in ((10 ** 6, [0, 1, 0, 1], 3), (0, [0, 1, 0, 1], 3), (-5, [0, 1, 0, 1], 3), (None, [0, 1, 0, 9], 4)):
+        status, bad = ops.new_status(cuda_device), table.clone()
+        if page is not None:
+            bad[1, 3] = page
+        got = call(bad, tile_row, status)
+        with pytest.raises(ops.KernelError, match=ops.STATUS_TEXT[code].split("(")[0]):
+            ops.check_status(status)
+        assert torch.equal(got[:150], good[:150])
+
+
+# --------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("plan", [(0, 2), (1, 296), (2, 148)])
 def test_captured_and_on_a_side_stream(ops, cuda_device, plan):
     """Two captured graphs, replayed at the same time on two streams, with contexts that change between replays."""

@@ -34,6 +34,7 @@
 // kernel does not take the cached row's width.
 #include "common.cuh"
 #include "mma.cuh"
+#include "packed.cuh"
 
 namespace zb {
 
@@ -75,7 +76,9 @@ struct PrefillArgs {
 // NS: stages of the ring of key/value tiles.  Two leave room for two CTAs an SM; three and four were measured
 // for tiles of one token (a decode step of 8 requests: 2.63 against 2.59 ms) and are not used.
 // DISTANT: with the distance bias (a form of its own, so that the others keep their registers).
-template <int HD, bool DEC, int NS, bool DISTANT>
+// PACKED: over a 4-bit cache (packed.cuh): a tile's blocks are copied as they are one tile ahead, and become bfloat16 rows in shared
+// memory between two barriers; without pooled blocks and kept tokens.
+template <int HD, bool DEC, int NS, bool DISTANT, bool PACKED = false>
 __global__ void __launch_bounds__(PRE_WARPS * 32, 1)
 paged_prefill_kernel(const PrefillArgs a) {
   static_assert(HD % 32 == 0 && HD <= 256, "head sizes that are multiples of 32, up to 256");
@@ -127,6 +130,58 @@ paged_prefill_kernel(const PrefillArgs a) {
                             : static_cast<size_t>(tok0 + (ok ? j : 0)) * a.nh + head;
     cp_async_16(q_s + j * KROW + c, a.q + from * HD + c, ok);
   }
+  // PACKED: two tiles' blocks behind the ring's one stage, and whether a block's page was found.
+  constexpr int RAW_BLOCKS = PRE_BN / PK_BLOCK, RAW_BYTES = RAW_BLOCKS * pk_block_bytes(HD);
+  unsigned char* const raw = reinterpret_cast<unsigned char*>(ring + STAGE);
+  __shared__ int raw_ok[2][RAW_BLOCKS];
+  auto load_packed = [&](int t) {
+    constexpr int PIECES = pk_block_bytes(HD) / 16;
+    const unsigned char* const source = reinterpret_cast<const unsigned char*>(a.kv_cache);
+    for (int e = threadIdx.x; e < RAW_BLOCKS * PIECES; e += PRE_WARPS * 32) {
+      const int b = e / PIECES, c = e - b * PIECES, pos = first_tile + t * PRE_BN + b * PK_BLOCK;
+      bool ok = pos < hi && pos + PK_BLOCK > lo;
+      long long from = 0;
+      if (ok) {
+        const int entry = pos >> a.page_shift, page = entry < a.max_blocks ? table[entry] : -1;
+        if (page <= 0 || page >= a.num_pages) {
+          if (c == 0) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, tok0);
+          ok = false;
+        } else {
+          from = (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (a.page_size - 1)) >> 4)) * pk_block_bytes(HD);
+        }
+      }
+      if (c == 0) raw_ok[t & 1][b] = ok;
+      if (ok) cp_async_16(raw + (t & 1) * RAW_BYTES + e * 16, source + from + c * 16, true);
+    }
+  };
+  auto expand = [&](int t) {
+    __nv_bfloat16* const ks = ring;
+    __nv_bfloat16* const vs = ks + PRE_BN * KROW;
+    const unsigned char* const blocks = raw + (t & 1) * RAW_BYTES;
+    const int k0 = first_tile + t * PRE_BN;
+    const uint4 zeros = make_uint4(0, 0, 0, 0);
+    for (int e = threadIdx.x; e < PRE_BN * CHUNKS; e += PRE_WARPS * 32) {
+      const int j = e / CHUNKS, c = e - j * CHUNKS, p = j & (PK_BLOCK - 1);
+      const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
+      const bool ok = raw_ok[t & 1][j >> 4] && k0 + j >= lo && k0 + j < hi;
+      const unsigned short* const params = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
+      *reinterpret_cast<uint4*>(ks + j * KROW + c * 8) =
+          ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_twice(params[0]), pk_twice(params[HD / 32]))
+             : zeros;
+    }
+    for (int e = threadIdx.x; e < PRE_BN / 2 * CHUNKS; e += PRE_WARPS * 32) {
+      const int pair = e / CHUNKS, c = e - pair * CHUNKS, j = 2 * pair, own = pair & (PK_BLOCK / 2 - 1);
+      const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
+      const unsigned char* const words = block + pk_value_word<HD>(own >> 2, 2 * (c & 3), own & 3, c >> 2);
+      const unsigned char* const params = block + pk_value_step<HD>(own, c >> 2);
+      uint4 even, odd;
+      pk_value_channels(*reinterpret_cast<const unsigned*>(words), *reinterpret_cast<const unsigned*>(words + HD / 2),
+                        *reinterpret_cast<const unsigned*>(params), *reinterpret_cast<const unsigned*>(params + HD / 8), even, odd);
+      const bool page_ok = raw_ok[t & 1][j >> 4];
+      *reinterpret_cast<uint4*>(vs + j * KROW + c * 8) = page_ok && k0 + j >= lo && k0 + j < hi ? even : zeros;
+      *reinterpret_cast<uint4*>(vs + (j + 1) * KROW + c * 8) = page_ok && k0 + j + 1 >= lo && k0 + j + 1 < hi ? odd : zeros;
+    }
+  };
   auto load_tile = [&](int t) {
     __nv_bfloat16* ks = ring + (t % NS) * STAGE;
     __nv_bfloat16* vs = ks + PRE_BN * KROW;
@@ -166,7 +221,11 @@ paged_prefill_kernel(const PrefillArgs a) {
   };
 #pragma unroll
   for (int t = 0; t < NS - 1; ++t) {         // one group of copies a tile, empty ones past the end
-    if (t < n_tiles) load_tile(t);
+    if (PACKED) {
+      if (t < n_tiles) load_packed(t);
+    } else if (t < n_tiles) {
+      load_tile(t);
+    }
     cp_async_commit();
   }
 
@@ -210,8 +269,15 @@ paged_prefill_kernel(const PrefillArgs a) {
   for (int t = 0; t < n_tiles; ++t) {
     cp_async_wait<NS - 2>();
     __syncthreads();                 // tile t (and, the first time, Q) has landed; tile t-1 is no longer read
-    if (t + NS - 1 < n_tiles) load_tile(t + NS - 1);
-    cp_async_commit();
+    if (PACKED) {
+      if (t + 1 < n_tiles) load_packed(t + 1);
+      cp_async_commit();
+      expand(t);
+      __syncthreads();
+    } else {
+      if (t + NS - 1 < n_tiles) load_tile(t + NS - 1);
+      cp_async_commit();
+    }
     if (t == 0) {
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
@@ -223,7 +289,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     if (!warp_active) continue;                          // uniform over the warp, as are the next two
     if (run == 0 && k0 >= warp_seen) continue;
     if (run == 2 && (k0 > warp_last_pos || (k0 + PRE_BN <= warp_first_visible && k0 >= a.keep_first))) continue;
-    const __nv_bfloat16* ks_tile = ring + (t % NS) * STAGE;
+    const __nv_bfloat16* ks_tile = ring + (PACKED ? 0 : t % NS) * STAGE;
     const __nv_bfloat16* vs_tile = ks_tile + PRE_BN * KROW;
 
     // The key tiles of 8 this warp works on: all eight of the 64 keys, or (DEC) the warp's own one.
@@ -420,6 +486,15 @@ int prefill_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream, bool 
   return launch_result();
 }
 
+template <int HD>
+int prefill_packed_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream) {
+  const size_t smem = (static_cast<size_t>(PRE_BM) + 2 * PRE_BN) * (HD + 8) * sizeof(__nv_bfloat16) + 2 * (PRE_BN / PK_BLOCK) * pk_block_bytes(HD);
+  auto kernel = paged_prefill_kernel<HD, false, 2, false, true>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return ERR_CUDA;
+  kernel<<<dim3(a.nh, n_tiles), PRE_WARPS * 32, smem, stream>>>(a);
+  return launch_result();
+}
+
 }  // namespace zb
 
 using namespace zb;
@@ -503,4 +578,35 @@ ZB_API int zb_paged_prefill(void* out, const void* q, const void* kv_cache, cons
   return zb_paged_prefill_masked(out, q, kv_cache, block_table, max_blocks, page_size, num_pages, num_rows, tile_row,
                                  tile_q0, n_tiles, row_q_start, row_q_len, row_ctx, nh, nkv, hd, window, 0, scale, 0.0f, 0,
                                  nullptr, status, stream);
+}
+
+// The same over a 4-bit cache (packed.cuh), pages of a power of two of positions from 16 on; head sizes 32, 64, 96 and 128.
+ZB_API int zb_paged_prefill_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
+                                   int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles,
+                                   const int* row_q_start, const int* row_q_len, const int* row_ctx, int nh, int nkv, int hd, int window,
+                                   int chunk, float scale, float softcap, const float* sinks, int* status, void* stream) {
+  const int page_shift = pk_page_shift(page_size);
+  if (n_tiles < 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || nh <= 0 || nkv <= 0 || nh % nkv != 0) return ERR_BAD_ARGUMENT;
+  if (!pk_head_dim_ok(hd) || nh > 65535 || n_tiles > 65535) return ERR_UNSUPPORTED;
+  if (n_tiles == 0) return OK;
+  PrefillArgs a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.kv_cache = static_cast<const __nv_bfloat16*>(packed);
+  a.block_table = block_table; a.tile_row = tile_row; a.tile_q0 = tile_q0;
+  a.row_q_start = row_q_start; a.row_q_len = row_q_len; a.row_ctx = row_ctx;
+  a.max_blocks = max_blocks; a.page_size = page_size; a.num_pages = num_pages; a.num_rows = num_rows;
+  a.page_shift = page_shift;
+  a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk; a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.softcap_log2 = softcap * 1.4426950408889634f;
+  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  a.status = status;
+  const auto s = static_cast<cudaStream_t>(stream);
+  switch (hd) {
+    case 32: return prefill_packed_launch<32>(a, n_tiles, s);
+    case 64: return prefill_packed_launch<64>(a, n_tiles, s);
+    case 96: return prefill_packed_launch<96>(a, n_tiles, s);
+    default: return prefill_packed_launch<128>(a, n_tiles, s);
+  }
 }

@@ -46,6 +46,7 @@
 
 #include "common.cuh"
 #include "mma.cuh"
+#include "packed.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
@@ -242,12 +243,21 @@ __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, 
 // FORM: which of the masks and biases beside causality and a window the kernel knows (forms of their own, so that the plain one
 // keeps its registers: with the chunk in it, seven prompts of 300 tokens took 58.8 us, 57.2 without).
 enum { TC_FORM_PLAIN, TC_FORM_BIASED, TC_FORM_CHUNKED, TC_FORM_KEPT };      // KEPT: first tokens kept, and a chunk
-template <int FORM, int HD, bool SHARED>
+// PACKED: over a 4-bit cache (packed.cuh), whose blocks the loader warps copy and turn into the ring's bfloat16 rows, an item a warp in
+// turn: some 1500 instructions for 128 positions, three warps' together as many as the products and the softmax of a tile leave time
+// for.  A key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every eight), and the queries' in the same.
+constexpr int TC_PACKED_STAGES = 4;
+constexpr int TC_PACKED_HALF = TC_BN / 2;                                                     // positions that a warp has copied ahead
+constexpr int TC_PACKED_RAW = TC_PACKED_HALF / PK_BLOCK * pk_block_bytes(128) / 2;            // their keys' or values' bytes
+constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_LOADER_WARPS * 2 * TC_PACKED_RAW;
+static_assert(TC_PACKED_SMEM <= 225 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
+
+template <int FORM, int HD, bool SHARED, bool PACKED = false>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   constexpr bool BIASED_SCORES = FORM == TC_FORM_BIASED, KEPT = FORM == TC_FORM_KEPT, CHUNKED = KEPT || FORM == TC_FORM_CHUNKED;
   using Shape = TcShape<HD, SHARED>;
-  constexpr int STAGES = Shape::STAGES, BLOCK = Shape::BLOCK, BLOCK_BYTES = Shape::BLOCK_BYTES, ITEM_BYTES = Shape::ITEM_BYTES;
+  constexpr int STAGES = PACKED ? TC_PACKED_STAGES : Shape::STAGES, BLOCK = Shape::BLOCK, BLOCK_BYTES = Shape::BLOCK_BYTES, ITEM_BYTES = Shape::ITEM_BYTES;
   constexpr int CHUNKS = HD / 8, BLOCK_CHUNKS = BLOCK / 8;      // 16-byte pieces of a row, and of a block's row
   // Shared memory: the slots' queries, then the ring of key and value tiles (a stage holds either; keys_j, values_j,
   // keys_j+1 ... in turn), all on 1024-byte boundaries as the swizzles want them.
@@ -355,7 +365,115 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     abort_flag = 1;
   };
 
-  if (warp > TC_MMA_WARP) {
+  if (PACKED && warp > TC_MMA_WARP) {
+    // ------------------------------------------------------------------------- the loaders of a 4-bit cache
+    // Items (a tile's keys, then its values) go to the warps in turn, half an item at a time: the next half's bytes are on their way
+    // while one is turned into rows.
+    constexpr int PART = pk_block_bytes(128) / 2, PIECES = PART / 16;          // a block's keys, or its values: bytes, 16-byte copies
+    const int own = warp - TC_MMA_WARP - 1;
+    unsigned char* const raw = ring + STAGES * ITEM_BYTES + own * 2 * TC_PACKED_RAW;
+    const int* table = a.block_table + static_cast<size_t>(row) * a.max_blocks;
+    const unsigned char* const cache = reinterpret_cast<const unsigned char*>(a.kv_cache);
+    // Lanes 0 .. 7: where the item's blocks lie, as a number of blocks from the cache's start; -1: nowhere, or nothing of it is seen.
+    auto look_up = [&](int item) {
+      const int j = item >> 1, pos = tile_start(j) + lane * PK_BLOCK;
+      if (lane >= TC_BN / PK_BLOCK || j >= n_tiles || pos >= run_hi(j) || pos + PK_BLOCK <= run_lo(j)) return -1LL;
+      const int entry = pos >> a.page_shift, page = entry < a.max_blocks ? table[entry] : -1;
+      if (page <= 0 || page >= a.num_pages) {
+        report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, tok0);
+        return -1LL;
+      }
+      return ((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (page_size - 1)) >> 4);
+    };
+    auto copy_half = [&](int item, int half, long long blocks) {
+      unsigned char* const dst = raw + half * TC_PACKED_RAW;
+#pragma unroll
+      for (int i = 0; i < TC_PACKED_RAW / 512; ++i) {
+        const int e = lane + 32 * i, b = e / PIECES;
+        const long long block = __shfl_sync(0xffffffffu, blocks, half * (TC_PACKED_HALF / PK_BLOCK) + b);
+        if (block >= 0) cp_async_16(dst + e * 16, cache + block * pk_block_bytes(128) + (item & 1) * PART + (e - b * PIECES) * 16, true);
+      }
+    };
+    const int items = 2 * n_tiles;
+    long long blocks = look_up(own), next_blocks = -1;
+    if (own < items) copy_half(own, 0, blocks);
+    cp_async_commit();
+    for (int item = own; item < items; item += TC_LOADER_WARPS) {
+      const int j = item >> 1, stage = item % STAGES, k0 = tile_start(j);
+      const int from = run_lo(j) - k0, until = run_hi(j) - k0;                // the rows that count
+      unsigned char* const dst = ring + stage * ITEM_BYTES;
+      if (!__all_sync(0xffffffffu, wait(&kv_empty[stage], ((item / STAGES) & 1) ^ 1))) {
+        give_up(-1);
+        break;
+      }
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        // The half behind this one.
+        if (half == 0) {
+          copy_half(item, 1, blocks);
+          next_blocks = look_up(item + TC_LOADER_WARPS);
+        } else {
+          blocks = next_blocks;
+          if (item + TC_LOADER_WARPS < items) copy_half(item + TC_LOADER_WARPS, 0, blocks);
+        }
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncwarp();                // every lane's part of this half is there
+        const unsigned char* const source = raw + half * TC_PACKED_RAW;
+        if ((item & 1) == 0) {
+          // A lane four words, one of every group, of a position; positions in an order that spreads the rows' chunks over the banks.
+          const int t = lane & 3, spread = (lane >> 2 & 1) * 4 + (lane >> 3);
+#pragma unroll 2
+          for (int i = 0; i < TC_PACKED_HALF / 8; ++i) {
+            const int p = 8 * i + spread, r = half * TC_PACKED_HALF + p;
+            const unsigned char* const block = source + (p >> 4) * PART;
+            const uint4 words = *reinterpret_cast<const uint4*>(block + pk_key_word<128>(p & 15, t, 0));
+            const uint4 params = *reinterpret_cast<const uint4*>(block + pk_key_step<128>(p & 15, 0));
+            const unsigned w[4] = {words.x, words.y, words.z, words.w};
+            const unsigned steps[4] = {__byte_perm(params.x, 0u, 0x1010), __byte_perm(params.x, 0u, 0x3232), __byte_perm(params.y, 0u, 0x1010), __byte_perm(params.y, 0u, 0x3232)};
+            const unsigned offsets[4] = {__byte_perm(params.z, 0u, 0x1010), __byte_perm(params.z, 0u, 0x3232), __byte_perm(params.w, 0u, 0x1010), __byte_perm(params.w, 0u, 0x3232)};
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int c = 4 * g + t;
+              *reinterpret_cast<uint4*>(dst + (c >> 3) * BLOCK_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(pk_values<0>(w[g], steps[g], offsets[g]), pk_values<1>(w[g], steps[g], offsets[g]),
+                             pk_values<2>(w[g], steps[g], offsets[g]), pk_values<3>(w[g], steps[g], offsets[g]));
+            }
+          }
+        } else {
+          // A lane two neighbouring words of every group of a pair of positions; rows that do not count become zeros, so that a zero
+          // probability times what a page held before stays zero.
+          const int t = lane & 3, gp = lane >> 2 & 3, h = lane >> 4;
+#pragma unroll 1
+          for (int i = 0; i < TC_PACKED_HALF / PK_BLOCK; ++i) {
+            const int r = half * TC_PACKED_HALF + 16 * i + 8 * h + 2 * t;
+            const unsigned char* const block = source + i * PART - pk_value_codes(128);
+            const uint4 low = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp, t, 0));
+            const uint4 high = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp + 1, t, 0));
+            const uint4 steps = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0));
+            const uint4 offsets = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0) + 16);
+            const unsigned lo4[4] = {low.x, low.y, low.z, low.w}, hi4[4] = {high.x, high.y, high.z, high.w};
+            const unsigned s4[4] = {steps.x, steps.y, steps.z, steps.w}, o4[4] = {offsets.x, offsets.y, offsets.z, offsets.w};
+            const bool even_ok = r >= from && r < until, odd_ok = r + 1 >= from && r + 1 < until;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int c = 4 * g + gp;
+              uint4 even, odd;
+              pk_value_channels(lo4[g], hi4[g], s4[g], o4[g], even, odd);
+              unsigned char* const at = dst + (c >> 3) * BLOCK_BYTES + r * 128;
+              *reinterpret_cast<uint4*>(at + (((c & 7) ^ (r & 7)) << 4)) = even_ok ? even : make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(at + 128 + (((c & 7) ^ ((r + 1) & 7)) << 4)) = odd_ok ? odd : make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        __syncwarp();                // every lane has read this half: the half after the next may come in its place
+      }
+      fence_proxy_async();           // the tensor core reads these rows through the asynchronous proxy
+      __syncwarp();
+      if (lane == 0) tc_mbar_arrive(&kv_full[stage]);
+    }
+    cp_async_wait<0>();
+  } else if (!PACKED && warp > TC_MMA_WARP) {
     // ------------------------------------------------------------------------- the loaders
     // One warp fetches the keys and one the values, each at its own pace; rows that are both have all three.
     constexpr int KIND_THREADS = Shape::KIND_WARPS * 32;
@@ -562,6 +680,9 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
 #pragma unroll
         for (int c = 0; c < HALF; ++c) {
           const int stored = (c0 + c) ^ turn;
+          if (PACKED)
+            v[c] = make_uint4(__byte_perm(v[c].x, v[c].z, 0x5410), __byte_perm(v[c].x, v[c].z, 0x7632), __byte_perm(v[c].y, v[c].w, 0x5410),
+                              __byte_perm(v[c].y, v[c].w, 0x7632));
           *reinterpret_cast<uint4*>(dst + (stored / BLOCK_CHUNKS) * BLOCK_BYTES + r * (BLOCK * 2) + (stored % BLOCK_CHUNKS) * 16) = v[c];
         }
       }
@@ -793,6 +914,15 @@ int prefill_tc_launch(PrefillTcArgs& a, long long cache_rows, int page_size, cud
   return launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(TC_THREADS), Shape::SMEM, stream, false, a);
 }
 
+template <int FORM>
+int prefill_tc_packed_launch(const PrefillTcArgs& a, cudaStream_t stream) {
+  auto kernel = paged_prefill_tc_kernel<FORM, 128, false, true>;
+  if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_PACKED_SMEM))) return ERR_CUDA;
+  const long long ctas = static_cast<long long>(a.n_split) * a.nh + static_cast<long long>(a.n_tiles - a.n_split) * (a.nh / 2);
+  if (ctas >= (1LL << 31)) return ERR_UNSUPPORTED;
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(TC_THREADS), TC_PACKED_SMEM, stream, false, a);
+}
+
 }  // namespace zb
 
 using namespace zb;
@@ -884,4 +1014,38 @@ ZB_API int zb_paged_prefill_tc(void* out, const void* q, const void* kv_cache, c
   return zb_paged_prefill_tc_masked(out, q, kv_cache, block_table, max_blocks, page_size, num_pages, num_rows, tile_row,
                                     tile_q0, n_tiles, num_rows, row_q_start, row_q_len, row_ctx, nh, nkv, hd, window, hd, 0, 0, scale, 0.0f, 0,
                                     nullptr, nullptr, nullptr, status, stream);
+}
+
+// The same over a 4-bit cache (packed.cuh): head size 128, pages of a power of two of positions from 16 on.
+ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
+                                      int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles, int tile_rows,
+                                      const int* row_q_start, const int* row_q_len, const int* row_ctx, int nh, int nkv, int window,
+                                      int chunk, float scale, float softcap, const float* sinks, int* status, void* stream) {
+  const int page_shift = pk_page_shift(page_size);
+  if (n_tiles < 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || nh <= 0 || nkv <= 0 || nh % nkv != 0) return ERR_BAD_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(packed) % 16 != 0)
+    return ERR_BAD_ARGUMENT;
+  if (n_tiles == 0) return OK;
+  if (tile_rows <= 0) return ERR_BAD_ARGUMENT;
+  if (n_tiles > 65535 || nh > 65535) return ERR_UNSUPPORTED;
+  int device = 0, sms = 0;
+  if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
+  PrefillTcArgs a = {};
+  a.n_tiles = n_tiles;
+  a.n_split = tc_split_tiles(nh, nkv, n_tiles, tile_rows, sms);
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.kv_cache = static_cast<const __nv_bfloat16*>(packed);
+  a.block_table = block_table; a.tile_row = tile_row; a.tile_q0 = tile_q0;
+  a.row_q_start = row_q_start; a.row_q_len = row_q_len; a.row_ctx = row_ctx;
+  a.max_blocks = max_blocks; a.num_pages = num_pages; a.num_rows = num_rows;
+  a.page_shift = page_shift;
+  a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.softcap_log2 = softcap * 1.4426950408889634f;
+  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  a.sinks = sinks;
+  a.status = status;
+  const auto s = static_cast<cudaStream_t>(stream);
+  return chunk > 0 ? prefill_tc_packed_launch<TC_FORM_CHUNKED>(a, s) : prefill_tc_packed_launch<TC_FORM_PLAIN>(a, s);
 }

@@ -86,4 +86,22 @@ __device__ __forceinline__ void pk_load_words(unsigned (&w)[N], const unsigned c
 __device__ __forceinline__ float pk_low(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pk_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// A word of a key as its eight channels in order, four bfloat16 pairs.
+__device__ __forceinline__ uint4 pk_key_channels(unsigned word, unsigned steps, unsigned offsets) {
+  const unsigned a = pk_values<0>(word, steps, offsets), b = pk_values<1>(word, steps, offsets);        // channels 0 4, 1 5
+  const unsigned c = pk_values<2>(word, steps, offsets), d = pk_values<3>(word, steps, offsets);        // 2 6, 3 7
+  return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
+}
+// Two neighbouring words of a pair of values (the four channels of g, and those of g + 1) as eight channels of either position.
+__device__ __forceinline__ void pk_value_channels(unsigned low, unsigned high, unsigned steps, unsigned offsets, uint4& even, uint4& odd) {
+  const unsigned a = pk_values<0>(low, steps, offsets), b = pk_values<1>(low, steps, offsets);
+  const unsigned c = pk_values<2>(low, steps, offsets), d = pk_values<3>(low, steps, offsets);
+  const unsigned e = pk_values<0>(high, steps, offsets), f = pk_values<1>(high, steps, offsets);
+  const unsigned g = pk_values<2>(high, steps, offsets), h = pk_values<3>(high, steps, offsets);
+  even = make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(e, f, 0x5410), __byte_perm(g, h, 0x5410));
+  odd = make_uint4(__byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), __byte_perm(e, f, 0x7632), __byte_perm(g, h, 0x7632));
+}
+// A bfloat16 twice.
+__device__ __forceinline__ unsigned pk_twice(unsigned short v) { return v * 0x10001u; }
+
 }  // namespace zb

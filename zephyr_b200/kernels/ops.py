@@ -123,6 +123,11 @@ _SIGNATURES = {
     "zb_paged_decode_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                c_longlong, c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_int, c_void_p,
                                c_void_p, c_void_p],
+    "zb_paged_prefill_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p],
+    "zb_paged_prefill_tc_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p,
+                                   c_void_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
                        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_head_mix": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -1538,6 +1543,34 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
         block_table.shape[0], rows.data_ptr(), n_rows, row_q_start.data_ptr(), row_ctx.data_ptr(), max_context, q.shape[0], nh, nkv, hd,
         window, chunk, scale, softcap, _ptr(sinks), mode, ctas, _ptr(scratch), status.data_ptr(), _stream()), "paged_decode_packed",
         1 if mode == PACKED_CLUSTERS else 2)
+    return out
+
+
+def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, tile_row: torch.Tensor, tile_q0: torch.Tensor,
+                         row_q_start: torch.Tensor, row_q_len: torch.Tensor, row_ctx: torch.Tensor, nh: int, nkv: int, hd: int,
+                         window: int, scale: float, status: torch.Tensor, out: torch.Tensor, chunk: int = 0,
+                         sinks: torch.Tensor | None = None, softcap: float = 0.0, tile_rows: int | None = None,
+                         tensor_memory: bool = True) -> torch.Tensor:
+    """``paged_prefill`` over a 4-bit cache: attention of rows with several new tokens, cut into tiles of
+    ``paged_prefill_tile_tokens()``, whose keys and values the cache holds already; writes those tokens' rows of ``out``.  bfloat16;
+    ``window``, ``chunk``, ``sinks``, ``softcap`` and ``tile_rows`` as there.  Head size 128 runs on tcgen05 (but the shortest prompts,
+    ``short_prompts``, and everything without ``tensor_memory``), other sizes on mma.sync."""
+    _i32(block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx)
+    pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk,
+                                              softcap, sinks)
+    tiles = tile_row.numel()
+    if row_q_len.numel() < block_table.shape[0] or tile_q0.numel() != tiles:
+        raise InvalidArgumentError("one length per row, and one first token per tile")
+    _same_device(q, packed, block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status, out, sinks)
+    lists = (out.data_ptr(), q.data_ptr(), packed.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, pages,
+             block_table.shape[0], tile_row.data_ptr(), tile_q0.data_ptr(), tiles)
+    rows = (row_q_start.data_ptr(), row_q_len.data_ptr(), row_ctx.data_ptr(), nh, nkv)
+    masks = (window, chunk, scale, softcap, _ptr(sinks), status.data_ptr(), _stream())
+    if hd == 128 and tensor_memory and USE_TCGEN05_PREFILL and not short_prompts(block_table, page_size, nh, tiles):
+        tile_rows = block_table.shape[0] if tile_rows is None else int(tile_rows)
+        _check(library().zb_paged_prefill_tc_packed(*lists, tile_rows, *rows, *masks), "paged_prefill_tc_packed")
+    else:
+        _check(library().zb_paged_prefill_packed(*lists, *rows, hd, *masks), "paged_prefill_packed")
     return out
 
 
