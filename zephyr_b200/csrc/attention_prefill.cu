@@ -166,7 +166,7 @@ paged_prefill_kernel(const PrefillArgs a) {
       const bool ok = raw_ok[t & 1][j >> 4] && k0 + j >= lo && k0 + j < hi;
       const unsigned short* const params = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
       *reinterpret_cast<uint4*>(ks + j * KROW + c * 8) =
-          ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_twice(params[0]), pk_twice(params[HD / 32]))
+          ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_half_twice(pk_low(params[0])), pk_half_twice(pk_low(params[HD / 32])))
              : zeros;
     }
     for (int e = threadIdx.x; e < PRE_BN / 2 * CHUNKS; e += PRE_WARPS * 32) {
@@ -282,6 +282,12 @@ paged_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         ldmatrix_x4(qa[ks], q_s + (warp_row0 + (lane & 7) + ((lane >> 3) & 1) * 8) * KROW + ks * 16 + (lane >> 4) * 8);
+      if (PACKED) {                  // keys are half-precision values there
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qa[ks][i] = pk_to_half(qa[ks][i]);
+      }
     }
     const int run = t < pool_tiles ? 0 : (t < pool_tiles + kept_tiles ? 1 : 2);
     const int k0 = run == 0 ? t * PRE_BN : (run == 1 ? (t - pool_tiles) * PRE_BN
@@ -303,8 +309,13 @@ paged_prefill_kernel(const PrefillArgs a) {
       for (int kk = 0; kk < HD / 32; ++kk) {
         unsigned b[4];
         ldmatrix_x4(b, ks_tile + (nt * 8 + (lane & 7)) * KROW + kk * 32 + (lane >> 3) * 8);
-        mma_bf16_16816(s[i], qa[2 * kk], b[0], b[1]);
-        mma_bf16_16816(s[i], qa[2 * kk + 1], b[2], b[3]);
+        if (PACKED) {
+          mma_f16_16816(s[i], qa[2 * kk], b[0], b[1]);
+          mma_f16_16816(s[i], qa[2 * kk + 1], b[2], b[3]);
+        } else {
+          mma_bf16_16816(s[i], qa[2 * kk], b[0], b[1]);
+          mma_bf16_16816(s[i], qa[2 * kk + 1], b[2], b[3]);
+        }
       }
     }
 
@@ -598,9 +609,9 @@ ZB_API int zb_paged_prefill_packed(void* out, const void* q, const void* packed,
   a.max_blocks = max_blocks; a.page_size = page_size; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
   a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk; a.sinks = sinks;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
   a.softcap_log2 = softcap * 1.4426950408889634f;
-  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);
   switch (hd) {

@@ -243,17 +243,23 @@ __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, 
 // FORM: which of the masks and biases beside causality and a window the kernel knows (forms of their own, so that the plain one
 // keeps its registers: with the chunk in it, seven prompts of 300 tokens took 58.8 us, 57.2 without).
 enum { TC_FORM_PLAIN, TC_FORM_BIASED, TC_FORM_CHUNKED, TC_FORM_KEPT };      // KEPT: first tokens kept, and a chunk
-// PACKED: over a 4-bit cache (packed.cuh), whose blocks the loader warps copy and turn into the ring's bfloat16 rows, an item a warp in
-// turn: some 1500 instructions for 128 positions, three warps' together as many as the products and the softmax of a tile leave time
-// for.  A key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every eight), and the queries' in the same.
+// PACKED: over a 4-bit cache (packed.cuh), whose blocks six loader warps copy and turn into the ring's rows: two warps an item, three
+// items at a time.  Some 3000 instructions a tile of keys and values, which beside the softmax of both slots need as many warps as that
+// (three, with an item each: 1024 tokens behind 7000, 32/8 heads, 276 us); so the softmax warps take registers over from the others.
+// Keys are half-precision values (packed.cuh), a key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every
+// eight), and the queries' in the same.
+constexpr int TC_PACKED_THREADS = 512;             // warps 9 .. 14 load, the last one has nothing to do
 constexpr int TC_PACKED_STAGES = 4;
-constexpr int TC_PACKED_HALF = TC_BN / 2;                                                     // positions that a warp has copied ahead
-constexpr int TC_PACKED_RAW = TC_PACKED_HALF / PK_BLOCK * pk_block_bytes(128) / 2;            // their keys' or values' bytes
-constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_LOADER_WARPS * 2 * TC_PACKED_RAW;
-static_assert(TC_PACKED_SMEM <= 225 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
+constexpr int TC_PACKED_TEAMS = 3;
+constexpr int TC_PACKED_AHEAD = 3;                 // blocks of 16 positions that a warp has copied, the one that it works on among them
+constexpr int TC_PACKED_PART = pk_block_bytes(128) / 2;         // a block's keys, or its values
+constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_PART;
+constexpr int TC_PACKED_SOFTMAX_REGISTERS = 168, TC_PACKED_OTHER_REGISTERS = 88;
+static_assert(TC_PACKED_SMEM <= 223 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
+static_assert(256 * (TC_PACKED_SOFTMAX_REGISTERS + TC_PACKED_OTHER_REGISTERS) <= TC_PACKED_THREADS * 128, "no more registers than at launch");
 
 template <int FORM, int HD, bool SHARED, bool PACKED = false>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(PACKED ? TC_PACKED_THREADS : TC_THREADS, 1)
 paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   constexpr bool BIASED_SCORES = FORM == TC_FORM_BIASED, KEPT = FORM == TC_FORM_KEPT, CHUNKED = KEPT || FORM == TC_FORM_CHUNKED;
   using Shape = TcShape<HD, SHARED>;
@@ -278,7 +284,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int b = 0; b < STAGES; ++b) {
-      mbar_init(&kv_full[b], Shape::KIND_WARPS);
+      mbar_init(&kv_full[b], PACKED ? 2 : Shape::KIND_WARPS);
       mbar_init(&kv_empty[b], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -351,6 +357,10 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   __syncthreads();
   tc_fence_after_sync();
   const unsigned tmem_base = tmem_base_s;
+  if (PACKED) {
+    if (warp < TC_SOFTMAX_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(TC_PACKED_SOFTMAX_REGISTERS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(TC_PACKED_OTHER_REGISTERS));
+  }
 
   auto wait = [&](unsigned long long* bar, unsigned parity) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
@@ -367,107 +377,119 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
 
   if (PACKED && warp > TC_MMA_WARP) {
     // ------------------------------------------------------------------------- the loaders of a 4-bit cache
-    // Items (a tile's keys, then its values) go to the warps in turn, half an item at a time: the next half's bytes are on their way
-    // while one is turned into rows.
-    constexpr int PART = pk_block_bytes(128) / 2, PIECES = PART / 16;          // a block's keys, or its values: bytes, 16-byte copies
-    const int own = warp - TC_MMA_WARP - 1;
-    unsigned char* const raw = ring + STAGES * ITEM_BYTES + own * 2 * TC_PACKED_RAW;
+    // Items (a tile's keys, its values) go to teams of two warps in turn, in the order in which the products read them, half of the
+    // positions each, block by block: the next blocks' bytes are on their way while one is turned into rows.
+    constexpr int PART = TC_PACKED_PART, PIECES = PART / 16, AHEAD = TC_PACKED_AHEAD;
+    const int team = (warp - TC_MMA_WARP - 1) >> 1, member = (warp - TC_MMA_WARP - 1) & 1;
+    unsigned char* const raw = ring + STAGES * ITEM_BYTES + (2 * team + member) * AHEAD * PART;
     const int* table = a.block_table + static_cast<size_t>(row) * a.max_blocks;
     const unsigned char* const cache = reinterpret_cast<const unsigned char*>(a.kv_cache);
-    // Lanes 0 .. 7: where the item's blocks lie, as a number of blocks from the cache's start; -1: nowhere, or nothing of it is seen.
+    const int items = team < TC_PACKED_TEAMS ? 2 * n_tiles : 0;
+    // Item -> 2 * tile + (values ? 1 : 0); key_item and value_item below are its inverse.
+    auto order = [&](int item) {
+      if (!split || item == 0 || item == 2 * n_tiles - 1) return item;
+      return item & 1 ? item + 1 : item - 1;
+    };
+    // Lanes 0 .. 3: where the half's blocks lie, as a number of blocks from the cache's start; -1: nowhere, or nothing of it is seen.
     auto look_up = [&](int item) {
-      const int j = item >> 1, pos = tile_start(j) + lane * PK_BLOCK;
-      if (lane >= TC_BN / PK_BLOCK || j >= n_tiles || pos >= run_hi(j) || pos + PK_BLOCK <= run_lo(j)) return -1LL;
+      const int j = order(item) >> 1, pos = tile_start(j) + (4 * member + lane) * PK_BLOCK;
+      if (lane >= 4 || item >= items || pos >= run_hi(j) || pos + PK_BLOCK <= run_lo(j)) return -1;
       const int entry = pos >> a.page_shift, page = entry < a.max_blocks ? table[entry] : -1;
       if (page <= 0 || page >= a.num_pages) {
         report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, tok0);
-        return -1LL;
+        return -1;
       }
-      return ((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (page_size - 1)) >> 4);
+      return ((page * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (page_size - 1)) >> 4);
     };
-    auto copy_half = [&](int item, int half, long long blocks) {
-      unsigned char* const dst = raw + half * TC_PACKED_RAW;
+    int issued = 0;
+    auto copy = [&](int item, int b, int blocks) {         // block b of the half, in turn
+      unsigned char* const dst = raw + issued % AHEAD * PART;
+      ++issued;
+      const int block = __shfl_sync(0xffffffffu, blocks, b);
+      if (block >= 0) {
+        const unsigned char* const src = cache + static_cast<long long>(block) * pk_block_bytes(128) + (order(item) & 1) * PART;
 #pragma unroll
-      for (int i = 0; i < TC_PACKED_RAW / 512; ++i) {
-        const int e = lane + 32 * i, b = e / PIECES;
-        const long long block = __shfl_sync(0xffffffffu, blocks, half * (TC_PACKED_HALF / PK_BLOCK) + b);
-        if (block >= 0) cp_async_16(dst + e * 16, cache + block * pk_block_bytes(128) + (item & 1) * PART + (e - b * PIECES) * 16, true);
+        for (int e = lane; e < PIECES; e += 32) cp_async_16(dst + e * 16, src + e * 16, true);
       }
+      cp_async_commit();
     };
-    const int items = 2 * n_tiles;
-    long long blocks = look_up(own), next_blocks = -1;
-    if (own < items) copy_half(own, 0, blocks);
-    cp_async_commit();
-    for (int item = own; item < items; item += TC_LOADER_WARPS) {
-      const int j = item >> 1, stage = item % STAGES, k0 = tile_start(j);
+    int blocks = look_up(team), next_blocks = -1, taken = 0;
+#pragma unroll
+    for (int b = 0; b < AHEAD - 1; ++b) copy(team, b, blocks);
+    for (int item = team; item < items; item += TC_PACKED_TEAMS) {
+      const int which = order(item), j = which >> 1, stage = item % STAGES, k0 = tile_start(j);
       const int from = run_lo(j) - k0, until = run_hi(j) - k0;                // the rows that count
       unsigned char* const dst = ring + stage * ITEM_BYTES;
-      if (!__all_sync(0xffffffffu, wait(&kv_empty[stage], ((item / STAGES) & 1) ^ 1))) {
+      // A barrier's parity tells a phase from its neighbours only: a team waits for the stages of the other teams' items too, so that it
+      // misses no phase of any stage.
+      bool free = true;
+      for (int i = max(item - TC_PACKED_TEAMS + 1, 0); i <= item; ++i)
+        free = free && __all_sync(0xffffffffu, wait(&kv_empty[i % STAGES], ((i / STAGES) & 1) ^ 1));
+      if (!free) {
         give_up(-1);
         break;
       }
+      next_blocks = look_up(item + TC_PACKED_TEAMS);
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        // The half behind this one.
-        if (half == 0) {
-          copy_half(item, 1, blocks);
-          next_blocks = look_up(item + TC_LOADER_WARPS);
-        } else {
-          blocks = next_blocks;
-          if (item + TC_LOADER_WARPS < items) copy_half(item + TC_LOADER_WARPS, 0, blocks);
-        }
-        cp_async_commit();
-        cp_async_wait<1>();
-        __syncwarp();                // every lane's part of this half is there
-        const unsigned char* const source = raw + half * TC_PACKED_RAW;
-        if ((item & 1) == 0) {
+      for (int b = 0; b < 4; ++b) {
+        const int then = b + AHEAD - 1;
+        copy(then < 4 ? item : item + TC_PACKED_TEAMS, then & 3, then < 4 ? blocks : next_blocks);
+        cp_async_wait<AHEAD - 1>();
+        __syncwarp();                // every lane's part of this block is there
+        const unsigned char* const source = raw + taken % AHEAD * PART;
+        ++taken;
+        const int r0 = 64 * member + 16 * b;
+        if ((which & 1) == 0) {
           // A lane four words, one of every group, of a position; positions in an order that spreads the rows' chunks over the banks.
           const int t = lane & 3, spread = (lane >> 2 & 1) * 4 + (lane >> 3);
-#pragma unroll 2
-          for (int i = 0; i < TC_PACKED_HALF / 8; ++i) {
-            const int p = 8 * i + spread, r = half * TC_PACKED_HALF + p;
-            const unsigned char* const block = source + (p >> 4) * PART;
-            const uint4 words = *reinterpret_cast<const uint4*>(block + pk_key_word<128>(p & 15, t, 0));
-            const uint4 params = *reinterpret_cast<const uint4*>(block + pk_key_step<128>(p & 15, 0));
-            const unsigned w[4] = {words.x, words.y, words.z, words.w};
-            const unsigned steps[4] = {__byte_perm(params.x, 0u, 0x1010), __byte_perm(params.x, 0u, 0x3232), __byte_perm(params.y, 0u, 0x1010), __byte_perm(params.y, 0u, 0x3232)};
-            const unsigned offsets[4] = {__byte_perm(params.z, 0u, 0x1010), __byte_perm(params.z, 0u, 0x3232), __byte_perm(params.w, 0u, 0x1010), __byte_perm(params.w, 0u, 0x3232)};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int p = 8 * i + spread, r = r0 + p;
+            const uint4 words = *reinterpret_cast<const uint4*>(source + pk_key_word<128>(p, t, 0));
+            const uint4 params = *reinterpret_cast<const uint4*>(source + pk_key_step<128>(p, 0));
+            const unsigned w[4] = {words.x, words.y, words.z, words.w}, s2[2] = {params.x, params.y}, o2[2] = {params.z, params.w};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const int c = 4 * g + t;
-              *reinterpret_cast<uint4*>(dst + (c >> 3) * BLOCK_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-                  make_uint4(pk_values<0>(w[g], steps[g], offsets[g]), pk_values<1>(w[g], steps[g], offsets[g]),
-                             pk_values<2>(w[g], steps[g], offsets[g]), pk_values<3>(w[g], steps[g], offsets[g]));
+              unsigned v[4];
+              pk_half_values(w[g], pk_half_twice(g & 1 ? pk_high(s2[g >> 1]) : pk_low(s2[g >> 1])),
+                             pk_half_twice(g & 1 ? pk_high(o2[g >> 1]) : pk_low(o2[g >> 1])), v);
+              *reinterpret_cast<uint4*>(dst + (c >> 3) * BLOCK_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
         } else {
           // A lane two neighbouring words of every group of a pair of positions; rows that do not count become zeros, so that a zero
           // probability times what a page held before stays zero.
-          const int t = lane & 3, gp = lane >> 2 & 3, h = lane >> 4;
-#pragma unroll 1
-          for (int i = 0; i < TC_PACKED_HALF / PK_BLOCK; ++i) {
-            const int r = half * TC_PACKED_HALF + 16 * i + 8 * h + 2 * t;
-            const unsigned char* const block = source + i * PART - pk_value_codes(128);
-            const uint4 low = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp, t, 0));
-            const uint4 high = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp + 1, t, 0));
-            const uint4 steps = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0));
-            const uint4 offsets = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0) + 16);
-            const unsigned lo4[4] = {low.x, low.y, low.z, low.w}, hi4[4] = {high.x, high.y, high.z, high.w};
-            const unsigned s4[4] = {steps.x, steps.y, steps.z, steps.w}, o4[4] = {offsets.x, offsets.y, offsets.z, offsets.w};
-            const bool even_ok = r >= from && r < until, odd_ok = r + 1 >= from && r + 1 < until;
+          const int t = lane & 3, gp = lane >> 2 & 3, h = lane >> 4, r = r0 + 8 * h + 2 * t;
+          const unsigned char* const block = source - pk_value_codes(128);
+          const uint4 low = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp, t, 0));
+          const uint4 high = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp + 1, t, 0));
+          const uint4 steps = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0));
+          const uint4 offsets = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0) + 16);
+          const unsigned lo4[4] = {low.x, low.y, low.z, low.w}, hi4[4] = {high.x, high.y, high.z, high.w};
+          unsigned s4[4] = {steps.x, steps.y, steps.z, steps.w}, o4[4] = {offsets.x, offsets.y, offsets.z, offsets.w};
+          if (r0 < from || r0 + 16 > until) {
+            const unsigned keep = (r >= from && r < until ? 0x0000ffffu : 0u) | (r + 1 >= from && r + 1 < until ? 0xffff0000u : 0u);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const int c = 4 * g + gp;
-              uint4 even, odd;
-              pk_value_channels(lo4[g], hi4[g], s4[g], o4[g], even, odd);
-              unsigned char* const at = dst + (c >> 3) * BLOCK_BYTES + r * 128;
-              *reinterpret_cast<uint4*>(at + (((c & 7) ^ (r & 7)) << 4)) = even_ok ? even : make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(at + 128 + (((c & 7) ^ ((r + 1) & 7)) << 4)) = odd_ok ? odd : make_uint4(0, 0, 0, 0);
+              s4[g] &= keep;
+              o4[g] &= keep;
             }
           }
+          unsigned char* const at = dst + r * 128;
+          const int turn = r & 7;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int c = 4 * g + gp;
+            uint4 even, odd;
+            pk_value_channels(lo4[g], hi4[g], s4[g], o4[g], even, odd);
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + (((c & 7) ^ turn) << 4)) = even;
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + 128 + (((c & 7) ^ (turn + 1)) << 4)) = odd;
+          }
         }
-        __syncwarp();                // every lane has read this half: the half after the next may come in its place
+        __syncwarp();                // every lane has read this block: another may come in its place
       }
+      blocks = next_blocks;
       fence_proxy_async();           // the tensor core reads these rows through the asynchronous proxy
       __syncwarp();
       if (lane == 0) tc_mbar_arrive(&kv_full[stage]);
@@ -597,12 +619,14 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     // The whole warp takes every turn and wait, one elected thread issues: operands of the products are then the same in
     // all lanes.
     {
-      constexpr unsigned IDESC_QK = tc_idesc(false), IDESC_PV = tc_idesc(true);
+      constexpr unsigned HALVES = PACKED ? (1u << 7) | (1u << 10) : 0u;      // (both operands' type: bits off, half precision)
+      constexpr unsigned IDESC_QK = tc_idesc(false) & ~HALVES, IDESC_PV = tc_idesc(true);
       constexpr int KSTEP = BLOCK * 2 * 16;        // bytes between 16 positions' values
       const bool leader = elect_one();
       const int count0 = slot_tiles(0), count1 = slot_tiles(1);
-      auto key_item = [&](int t) { return SHARED ? t : 2 * t; };
-      auto value_item = [&](int t) { return SHARED ? t : 2 * t + 1; };
+      // PACKED with tiles split between the slots: K0 K1 V0 K2 V1 K3 .. V, as the products below read them.
+      auto key_item = [&](int t) { return SHARED ? t : (PACKED && split && t > 0 ? 2 * t - 1 : 2 * t); };
+      auto value_item = [&](int t) { return SHARED ? t : (PACKED && split && t + 1 < n_tiles ? 2 * t + 2 : 2 * t + 1); };
       auto arrived = [&](unsigned long long* bar, unsigned parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
       auto landed = [&](int item) { return arrived(&kv_full[item % STAGES], (item / STAGES) & 1); };
       auto issue_scores = [&](int slot, int i) -> bool {
@@ -681,8 +705,8 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
         for (int c = 0; c < HALF; ++c) {
           const int stored = (c0 + c) ^ turn;
           if (PACKED)
-            v[c] = make_uint4(__byte_perm(v[c].x, v[c].z, 0x5410), __byte_perm(v[c].x, v[c].z, 0x7632), __byte_perm(v[c].y, v[c].w, 0x5410),
-                              __byte_perm(v[c].y, v[c].w, 0x7632));
+            v[c] = make_uint4(pk_to_half(__byte_perm(v[c].x, v[c].z, 0x5410)), pk_to_half(__byte_perm(v[c].x, v[c].z, 0x7632)),
+                              pk_to_half(__byte_perm(v[c].y, v[c].w, 0x5410)), pk_to_half(__byte_perm(v[c].y, v[c].w, 0x7632)));
           *reinterpret_cast<uint4*>(dst + (stored / BLOCK_CHUNKS) * BLOCK_BYTES + r * (BLOCK * 2) + (stored % BLOCK_CHUNKS) * 16) = v[c];
         }
       }
@@ -920,7 +944,7 @@ int prefill_tc_packed_launch(const PrefillTcArgs& a, cudaStream_t stream) {
   if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_PACKED_SMEM))) return ERR_CUDA;
   const long long ctas = static_cast<long long>(a.n_split) * a.nh + static_cast<long long>(a.n_tiles - a.n_split) * (a.nh / 2);
   if (ctas >= (1LL << 31)) return ERR_UNSUPPORTED;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(TC_THREADS), TC_PACKED_SMEM, stream, false, a);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(TC_PACKED_THREADS), TC_PACKED_SMEM, stream, false, a);
 }
 
 }  // namespace zb
@@ -1027,7 +1051,7 @@ ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* pack
     return ERR_BAD_ARGUMENT;
   if (n_tiles == 0) return OK;
   if (tile_rows <= 0) return ERR_BAD_ARGUMENT;
-  if (n_tiles > 65535 || nh > 65535) return ERR_UNSUPPORTED;
+  if (n_tiles > 65535 || nh > 65535 || (static_cast<long long>(num_pages) * nkv << (page_shift - 4)) >= (1LL << 31)) return ERR_UNSUPPORTED;
   int device = 0, sms = 0;
   if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
   PrefillTcArgs a = {};
@@ -1041,9 +1065,9 @@ ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* pack
   a.max_blocks = max_blocks; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
   a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
   a.softcap_log2 = softcap * 1.4426950408889634f;
-  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
   a.sinks = sinks;
   a.status = status;
   const auto s = static_cast<cudaStream_t>(stream);

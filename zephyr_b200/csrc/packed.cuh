@@ -86,11 +86,54 @@ __device__ __forceinline__ void pk_load_words(unsigned (&w)[N], const unsigned c
 __device__ __forceinline__ float pk_low(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pk_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// A word of a key as its eight channels in order, four bfloat16 pairs.
+// ---- Keys for a prompt's products, as half-precision values times 2^-6: three bits more than bfloat16's eight, since what a key is off
+// by moves all of a query's weights (at most 2^-11 of a value here; with bfloat16 keys a prompt's result was 0.0054 off where the weights' and
+// the results' own roundings make 0.0025).  Keys up to 2^22 and queries up to 65504 fit; what is below 2^-19 is off by up to that.
+constexpr float PK_KEY_SCALE = 0.015625f, PK_KEY_UNSCALE = 64.0f;
+
+// A key's step or offset (bfloat16) on that scale, twice.
+__device__ __forceinline__ unsigned pk_half_twice(float v) {
+  unsigned r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %1;\n" : "=r"(r) : "f"(v * PK_KEY_SCALE));
+  return r;
+}
+__device__ __forceinline__ unsigned pk_fma_f16x2(unsigned a, unsigned b, unsigned c) {
+  unsigned r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// Eight codes as half-precision values, nibbles 0 4, 1 5, 2 6, 3 7 side by side.  A code in the last bits of 1024's mantissa is 1024 +
+// code, four bits further up 1024 + 16 code: what is left after the 1024 is exact.
+__device__ __forceinline__ void pk_half_values(unsigned word, unsigned steps, unsigned offsets, unsigned (&r)[4]) {
+  const unsigned high = word >> 8;
+  unsigned x[4];
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;\n" : "=r"(x[0]) : "r"(word));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;\n" : "=r"(x[1]) : "r"(word));
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;\n" : "=r"(x[2]) : "r"(high));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;\n" : "=r"(x[3]) : "r"(high));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned code = i & 1 ? pk_fma_f16x2(x[i], 0x2c002c00u, 0xd400d400u) : pk_fma_f16x2(x[i], 0x3c003c00u, 0xe400e400u);    // / 16 - 64, - 1024
+    r[i] = pk_fma_f16x2(code, steps, offsets);
+  }
+}
+// Two bfloat16 values as half-precision ones.
+__device__ __forceinline__ unsigned pk_to_half(unsigned pair) {
+  unsigned r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(__uint_as_float(pair & 0xffff0000u)), "f"(__uint_as_float(pair << 16)));
+  return r;
+}
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A word of a key as its eight channels in order, four such pairs.
 __device__ __forceinline__ uint4 pk_key_channels(unsigned word, unsigned steps, unsigned offsets) {
-  const unsigned a = pk_values<0>(word, steps, offsets), b = pk_values<1>(word, steps, offsets);        // channels 0 4, 1 5
-  const unsigned c = pk_values<2>(word, steps, offsets), d = pk_values<3>(word, steps, offsets);        // 2 6, 3 7
-  return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
+  unsigned r[4];
+  pk_half_values(word, steps, offsets, r);
+  return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410), __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
 }
 // Two neighbouring words of a pair of values (the four channels of g, and those of g + 1) as eight channels of either position.
 __device__ __forceinline__ void pk_value_channels(unsigned low, unsigned high, unsigned steps, unsigned offsets, uint4& even, uint4& odd) {
@@ -101,7 +144,4 @@ __device__ __forceinline__ void pk_value_channels(unsigned low, unsigned high, u
   even = make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(e, f, 0x5410), __byte_perm(g, h, 0x5410));
   odd = make_uint4(__byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), __byte_perm(e, f, 0x7632), __byte_perm(g, h, 0x7632));
 }
-// A bfloat16 twice.
-__device__ __forceinline__ unsigned pk_twice(unsigned short v) { return v * 0x10001u; }
-
 }  // namespace zb
