@@ -35,7 +35,8 @@ class PagedCacheSpec:
     ``keep_first``: a windowed cache whose first n positions stay readable for good (the window passes
     them, their pages are never given back).
     ``every``: n > 1: the store holds one entry per run of n positions (entry b stands for positions
-    b n .. b n + n - 1: a mean of a block, say), so its tables cover ceil(positions / n) entries."""
+    b n .. b n + n - 1: a mean of a block, say), so its tables cover ceil(positions / n) entries.
+    ``bits``: 4: keys and values are held as codes of 4 bits (``storage.py``); 0: in the model's type."""
 
     num_kv_heads: int
     key_dim: int
@@ -45,10 +46,15 @@ class PagedCacheSpec:
     keys_only: bool = False
     keep_first: int = 0
     every: int = 1
+    bits: int = 0
 
     def __post_init__(self) -> None:
         if self.value_dim == 0:
             object.__setattr__(self, "value_dim", self.key_dim)
+        if self.bits not in (0, 4):
+            raise InvalidArgumentError("a cache is held in the model's type or in 4 bits")
+        if self.bits and (self.key_dim != self.value_dim or self.keys_only or self.every != 1):
+            raise InvalidArgumentError("a 4-bit cache holds a key and a value of one width for every position")
 
     @property
     def head_dim(self) -> int:
@@ -61,7 +67,7 @@ class PagedCacheSpec:
     @property
     def group_key(self) -> tuple:
         return ("paged", self.num_kv_heads, self.key_dim, self.value_dim, self.window, self.chunk, self.keys_only,
-                self.keep_first if self.window > 0 else 0, self.every)
+                self.keep_first if self.window > 0 else 0, self.every, self.bits)
 
     @property
     def stored_per_position(self) -> int:

@@ -14,6 +14,10 @@ row (the ``head_dim`` values of one position and head) the 16-byte chunks are pe
 read by the tensor-core loads without bank conflicts.  Only the kernels (and tests that fill a cache
 by hand) know of the permutation.  A state cache is ``[num_slots, *shape]``.
 
+A paged cache in 4 bits (``PagedCacheSpec.bits``) is ``[num_pages, kv_heads, page_size / 16, 20 * head_dim]`` bytes: of every 16
+positions of a head the keys' codes, their steps and offsets (a bfloat16 each for every 32 values), then the values' (csrc/packed.cuh).
+It has no views of keys and values; ``kernels.ops.unpack_pages`` reads pages back.
+
 The reference keeps two tensors per layer, keys packed ``[blocks, kvh, hd/x, bs, x]`` and values
 ``[blocks, kvh, hd, bs]`` (src/kv_cache/cache_engine.cpp:66-102), a layout made for scalar loads.
 """
@@ -22,10 +26,14 @@ from __future__ import annotations
 
 import torch
 
+from ..config.errors import ConfigError, InvalidArgumentError
+from ..kernels import ops
 from .manager import CacheManager, PagedCacheSpec, StateCacheSpec
 
 
 def paged_cache_bytes_per_page(spec: PagedCacheSpec, page_size: int, dtype: torch.dtype) -> int:
+    if spec.bits:
+        return ops.packed_block_bytes(spec.head_dim) * (page_size // ops.PACKED_BLOCK) * spec.num_kv_heads
     return spec.stored_per_position * page_size * torch.empty((), dtype=dtype).element_size()
 
 
@@ -42,6 +50,13 @@ class CacheStorage:
         for cache_id, spec in enumerate(manager.cache_specs):
             if isinstance(spec, PagedCacheSpec):
                 pages = manager.groups[manager.group_of_cache[cache_id]].pool.num_pages
+                if spec.bits:
+                    if not ops.packed_page_size_ok(self.page_size) or spec.head_dim not in ops.PACKED_HEAD_DIMS:
+                        raise ConfigError(f"a 4-bit cache takes pages of 16 positions or a larger power of two and head sizes "
+                                          f"{ops.PACKED_HEAD_DIMS}, not {self.page_size} and {spec.head_dim}")
+                    shape = ops.packed_cache_shape(pages, spec.num_kv_heads, self.page_size, spec.head_dim)
+                    self.tensors.append(torch.zeros(shape, dtype=torch.uint8, device=device))
+                    continue
                 # Zeros, not empty: the null page is read by nothing, but a debugger should see zeros there.
                 if spec.key_dim == spec.value_dim and not spec.keys_only:
                     shape = (pages, 2, spec.num_kv_heads, manager.page_size, spec.key_dim)
@@ -60,6 +75,7 @@ class CacheStorage:
     def keys(self, cache_id: int) -> torch.Tensor:
         """[num_pages, kv_heads, page_size, key_dim]: a view of the pages' key halves."""
         spec, tensor = self.specs[cache_id], self.tensors[cache_id]
+        self._check_unpacked(spec)
         if spec.keys_only:
             return tensor.view(tensor.shape[0], spec.num_kv_heads, self.page_size, spec.key_dim)
         if spec.key_dim == spec.value_dim:
@@ -70,12 +86,18 @@ class CacheStorage:
     def values(self, cache_id: int) -> torch.Tensor:
         """[num_pages, kv_heads, page_size, value_dim]: a view of the pages' value halves."""
         spec, tensor = self.specs[cache_id], self.tensors[cache_id]
+        self._check_unpacked(spec)
         if spec.keys_only:
             return self.keys(cache_id)
         if spec.key_dim == spec.value_dim:
             return tensor[:, 1]
         split = spec.num_kv_heads * self.page_size * spec.key_dim
         return tensor[:, split:].view(tensor.shape[0], spec.num_kv_heads, self.page_size, spec.value_dim)
+
+    @staticmethod
+    def _check_unpacked(spec: PagedCacheSpec) -> None:
+        if spec.bits:
+            raise InvalidArgumentError("a 4-bit cache has no views of its keys and values; ops.unpack_pages reads pages back")
 
     def reset_state_slot(self, manager: CacheManager, slot: int) -> None:
         """A slot that a new request takes starts from zero."""
@@ -104,4 +126,5 @@ class CacheStorage:
             return
         index = torch.tensor(live, dtype=torch.long, device=self.tensors[manager.groups[group].cache_ids[0]].device)
         for cache_id in manager.groups[group].cache_ids:
-            self.tensors[cache_id].index_fill_(0, index, float("nan"))
+            # In a 4-bit cache every bit set makes every step and offset NaN.
+            self.tensors[cache_id].index_fill_(0, index, 0xFF if self.specs[cache_id].bits else float("nan"))

@@ -63,6 +63,7 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--max-num-batched-tokens", type=_positive_int)
     gen.add_argument("--max-prefill-chunk-tokens", type=_positive_int)
     gen.add_argument("--kv-block-size", type=_positive_int, default=16)
+    gen.add_argument("--kv-bits", type=int, choices=(4,), help="hold keys and values in 4 bits (default: in the model's type)")
     gen.add_argument("--num-kv-blocks", type=_positive_int, help="fix the number of cache pages")
     gen.add_argument("--json", action="store_true", help="print one JSON object per request")
     gen.add_argument("--log-level", choices=("critical", "error", "warning", "info", "debug", "trace"), default="warning")
@@ -106,7 +107,8 @@ def _generate(args, parser) -> int:
         engine = Engine(args.model, dtype=args.dtype, max_seq_len=args.max_model_len or 0,
                         gpu_memory_utilization=args.gpu_memory_utilization,
                         scheduler=PagedSchedulerConfig(**scheduler_args),
-                        kv_cache=KvCacheOptions(block_size=args.kv_block_size, num_blocks=args.num_kv_blocks))
+                        kv_cache=KvCacheOptions(block_size=args.kv_block_size, num_blocks=args.num_kv_blocks,
+                                                bits=args.kv_bits))
         params = GenerationParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
                                   top_p=args.top_p, min_p=args.min_p, frequency_penalty=args.frequency_penalty,
                                   presence_penalty=args.presence_penalty, repetition_penalty=args.repetition_penalty,

@@ -712,10 +712,10 @@ template <int HD>
 __global__ void __launch_bounds__(256)
 paged_decode_packed_merge_kernel(const PackedDecodeArgs a) {
   constexpr int COLUMNS = HD / 4, BATCH = 8;
-  __shared__ float4 sums[256];
-  __shared__ float2 mls[256];
   wait_for_prior_grids();
   let_dependents_launch();
+  __shared__ float4 sums[256];
+  __shared__ float2 mls[256];
   const int pair = blockIdx.x, pairs_a_row = a.nkv * a.subs, group = a.nh / a.nkv;
   const int4 cut = a.cuts[pair];
   if (cut.y <= 1) return;

@@ -24,7 +24,7 @@ import torch
 
 from ..config import ConfigError, InvalidArgumentError, load_model_config
 from ..kernels import ops
-from ..parts import Model
+from ..parts import Model, with_cache_bits
 from ..sampling import MT19937_64, Sampler, SamplingParams
 from ..weights import Checkpoint
 from .params import (Choice, FinishReason, GenerationOutput, GenerationParams, KvCacheOptions, RequestStatus, Usage)
@@ -100,13 +100,19 @@ class Engine:
             model_config = load_model_config(model)
         self.model_config = model_config
         spec = model_config.to_model_spec()
+        limit = spec.max_seq_len if max_seq_len in (0, None) else min(max_seq_len, spec.max_seq_len)
+        if kv_cache.bits is not None:
+            if self.dtype != torch.bfloat16:
+                raise ConfigError("a cache in 4 bits is built for bfloat16 models")
+            if not ops.packed_page_size_ok(kv_cache.block_size):
+                raise ConfigError("a cache in 4 bits takes a block_size of 16 or a larger power of two")
+            spec = with_cache_bits(spec, kv_cache.bits, limit)
         self.generation_defaults = self._read_generation_defaults(model) if model is not None else {}
         store = weights if weights is not None else Checkpoint(model)
         self.model = Model.load(spec, store, self.dtype, self.device)
         torch.cuda.empty_cache()        # loading may hold copies (fused matrices) that it no longer needs
         _LOGGER.info("model ready: %s, %s, %.2f s", spec.architecture, self.dtype, time.perf_counter() - started)
 
-        limit = spec.max_seq_len if max_seq_len in (0, None) else min(max_seq_len, spec.max_seq_len)
         num_pages = self._size_cache(kv_cache, gpu_memory_utilization, limit)
         self.runner = ModelRunner(self.model, kv_cache.block_size, num_pages, self.scheduler_config.max_num_seqs,
                                   max_seq_len=limit)

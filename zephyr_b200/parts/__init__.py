@@ -12,7 +12,7 @@ from .ends import Embedding, NormHead
 from .feed_forward import SwiGLU, UngatedFeedForward
 from .latent import LatentAttention
 from .routed import RoutedFeedForward
-from .model import Model, cache_specs, expected_weights, run_order_for, tile_requests
+from .model import Model, cache_specs, expected_weights, run_order_for, tile_requests, with_cache_bits
 from .norms import LayerNorm, RMSNorm
 from .position import NoPosition, RopeNeox, RopePairs, rope_tables
 from .recurrent import GatedLinearAttention, Mamba2, ParallelMixers, Retention
@@ -25,5 +25,5 @@ __all__ = [
     "PositionEncoding", "PreNormResidual", "RMSNorm", "ResidualStream", "Retention", "SIDES", "SidePart", "RopeNeox", "StepContext", "SwiGLU", "TokenGate",
     "cache_specs", "expected_weights", "lookup", "register_block", "register_feed_forward", "register_input",
     "register_mixer", "register_norm", "register_output", "register_position_encoding", "register_side",
-    "rope_tables", "tile_requests",
+    "rope_tables", "tile_requests", "with_cache_bits",
 ]

@@ -46,6 +46,11 @@ sigmoid(Wg x)_h with Wg [heads, hidden], whose product rides along with the proj
 ``value_mix`` = {"group", "share"}: layers that name one group hand values on within a step.  Its first layer (``share``
 None) leaves its values as projected; every later one caches (1 - m) v + m v_first, m being the tensor ``share`` and
 v_first the first layer's values of the same tokens, both unrounded.
+
+``cache_bits`` = 4 holds keys and values in 4 bits (bfloat16 models; heads of 32, 64, 96 or 128 channels, keys and values of one width).
+Bias, norms, rotation and the write into the cache are then one kernel (``ops.qk_norm_rope_packed``), which turns halves or adjacent
+pairs by tables of cosines and sines, and prompts and single tokens have an attention kernel each; windows, chunks, sinks, the bound on
+scores, gates and a scale of its own stay, whatever else of the above is refused.
 """
 
 from __future__ import annotations
@@ -61,6 +66,7 @@ from ..config.spec import LayerCall, MixerSpec
 from ..kernels import ops
 from ..weights.loader import ROLE_LINEAR, ROLE_NORM, ROLE_ZERO, WeightDecl
 from .base import POSITION_ENCODINGS, Mixer, StepContext, lookup, register_mixer
+from .position import rotation_tables
 
 
 class Attention(Mixer):
@@ -160,12 +166,15 @@ class Attention(Mixer):
             raise ConfigError("the rotation of halves and its companions do not combine with a rotation of "
                               "adjacent pairs, keys as values, unit norms or a query multiplier")
         # What only the general path takes.
+        self.cache_bits = int(p.get("cache_bits") or 0)
         self.general = (pairs is not None or self.vd != self.hd or self.chunk > 0 or self.sinks is not None
                         or self.qkv_bias is not None or self.o_bias is not None or p.get("scale") is not None
                         or self.values_from_keys or self.unit_norm or self.softcap > 0.0 or self.q_temp is not None
                         or self.halves or self.score_mix is not None or self.distance_bias is not None or self.head_gate)
         if self.general:
             self._init_general(p)
+            if self.cache_bits:
+                self._init_packed(p)
             return
         if self.hd % 16 != 0 or self.hd < 16:
             raise ConfigError(f"attention kernels take head sizes 16..256 in steps of 16, not {self.hd}")
@@ -188,6 +197,32 @@ class Attention(Mixer):
         self.fast_prefill = self.score_slopes is None and ops.paged_prefill_supported(self.nh, self.nkv, self.hd, dtype)
         self.float32_tiles = self.score_slopes is None and ops.paged_attention_f32_supported(self.nh, self.nkv, self.hd, dtype)
         self.prefill_tile_tokens = ops.paged_prefill_tile_tokens()
+        if self.cache_bits:
+            self._init_packed(p)
+
+    def _init_packed(self, p) -> None:
+        """What the kernels over a 4-bit cache take, and the tables that they rotate by."""
+        if self.cache_bits != 4 or self.dtype != torch.bfloat16:
+            raise ConfigError("a cache of keys and values in fewer bits is built for 4 bits and bfloat16 models")
+        if self.hd not in ops.PACKED_HEAD_DIMS or self.vd != self.hd:
+            raise ConfigError(f"a cache in 4 bits takes keys and values of one width out of {ops.PACKED_HEAD_DIMS}, not {self.hd} and {self.vd}")
+        refused = {"values_from_keys": self.values_from_keys, "unit_qk_norm": self.unit_norm, "q_temp": self.q_temp is not None,
+                   "qk_norm 'whole'": self.qk_norm == "whole", "value_unit_norm": self.value_unit_norm, "keep_first": self.keep_first > 0,
+                   "pool": self.pool > 0, "head_mix": self.head_mix is not None, "score_mix": self.score_mix is not None,
+                   "distance_bias": self.distance_bias is not None, "value_mix": self.value_group is not None,
+                   "a bias on the scores": self.score_slopes is not None, "a position encoding of another kind": not (self.general or self.fused_position)}
+        named = [name for name, asked in refused.items() if asked]
+        if named:
+            raise ConfigError(f"a cache in 4 bits is not built with {', '.join(named)}")
+        self.pair_layout = "pairs" if self.pair_freqs is not None else "halves"
+        if self.general:
+            freqs = self.pair_freqs if self.pair_freqs is not None else self.half_freqs
+            positions = min(n for n in (int(p.get("cache_positions") or 0), getattr(self.position, "max_positions", 0)) if n > 0) if freqs is not None else 0
+            if self.half_freqs is not None and self.half_dims % 8 != 0:
+                raise ConfigError("a cache in 4 bits takes rotations of halves of a multiple of 8 channels")
+            self.tables = rotation_tables(freqs, self.half_mult, positions) if freqs is not None else None      # (shared while it is held)
+            self.cos, self.sin = (self.tables.cos, self.tables.sin) if freqs is not None else (None, None)
+        self.fast_decode = self.fast_prefill = True      # (both have kernels over such a cache)
 
     def _init_general(self, p) -> None:
         if self.hd % 2 != 0 and self.pair_freqs is not None:
@@ -278,10 +313,19 @@ class Attention(Mixer):
         window, pool = int(p.get("window", 0)), int(p.get("pool") or 0)
         sizes = dict(key_dim=int(p["head_dim"]), value_dim=int(p.get("value_dim") or p["head_dim"]))
         tokens = PagedCacheSpec(int(p["num_kv_heads"]), window=max(window, pool) if window > 0 else 0,
-                                chunk=int(p.get("chunk") or 0), keep_first=int(p.get("keep_first") or 0), **sizes)
+                                chunk=int(p.get("chunk") or 0), keep_first=int(p.get("keep_first") or 0), **sizes,
+                                **Attention._packed_sizes(p))
         if pool <= 0:
             return tokens
         return tokens, PagedCacheSpec(int(p["num_kv_heads"]), every=pool, **sizes)
+
+    @staticmethod
+    def _packed_sizes(p) -> dict:
+        bits = int(p.get("cache_bits") or 0)
+        widths = {int(p["head_dim"]), int(p.get("value_dim") or p["head_dim"])}
+        if bits and (len(widths) > 1 or not widths <= set(ops.PACKED_HEAD_DIMS)):
+            raise ConfigError(f"a cache in 4 bits takes keys and values of one width out of {ops.PACKED_HEAD_DIMS}")
+        return {"bits": bits}
 
     @staticmethod
     def tile_requests(spec: MixerSpec) -> list[tuple[int, str]]:
@@ -301,11 +345,32 @@ class Attention(Mixer):
         nh, nkv, hd = self.nh, self.nkv, self.hd
         table = ctx.block_table(call.cache)
         cos, sin = self.cos, self.sin
+        if self.cache_bits:
+            return self._store_packed(projected, None, ctx, call)
         if call.writes_cache:
             return ops.qk_norm_rope_cache(projected, nh, nkv, hd, self.q_norm, self.k_norm, self.eps, cos, sin,
                                           ctx.positions, ctx.token_row, ctx.caches[call.cache], table, ctx.status)
         return ops.qk_norm_rope_cache(projected, nh, 1, hd, self.q_norm, self.k_norm, self.eps, cos, sin,
                                       ctx.positions, ctx.token_row, None, table, ctx.status)
+
+    def _store_packed(self, projected: torch.Tensor, bias: torch.Tensor | None, ctx: StepContext, call: LayerCall) -> torch.Tensor:
+        """Bias, per-head norm, rotation and the write of keys and values as 4-bit codes in one kernel; returns the queries."""
+        return ops.qk_norm_rope_packed(projected, self.nh, self.nkv, self.hd, self.q_norm, self.k_norm, self.eps, self.cos, self.sin,
+                                       ctx.positions, ctx.token_row, ctx.caches[call.cache] if call.writes_cache else None,
+                                       ctx.block_table(call.cache), ctx.status, self.dtype, self.pair_layout, bias)
+
+    def _attend_packed(self, q: torch.Tensor, ctx: StepContext, call: LayerCall) -> torch.Tensor:
+        cache, table = ctx.caches[call.cache], ctx.block_table(call.cache)
+        out = torch.empty((q.shape[0], self.nh * self.hd), dtype=q.dtype, device=q.device)
+        common = (self.nh, self.nkv, self.hd, self.window, self.scale, ctx.status, out)
+        masks = {"chunk": self.chunk, "sinks": self.sinks, "softcap": self.softcap}
+        if ctx.num_decode_rows > 0:
+            ops.paged_decode_packed(q, cache, table, ctx.decode_rows, ctx.row_q_start, ctx.row_ctx, ctx.max_decode_context, *common, **masks)
+        tile_row, tile_q0 = ctx.tiles[(self.prefill_tile_tokens, "multi")]
+        if tile_row.numel() > 0:
+            ops.paged_prefill_packed(q, cache, table, tile_row, tile_q0, ctx.row_q_start, ctx.row_q_len, ctx.row_ctx, *common,
+                                     tile_rows=ctx.rows_with_tiles("multi"), **masks)
+        return out
 
     def _project_and_store(self, x: torch.Tensor, ctx: StepContext, call: LayerCall) -> torch.Tensor:
         nh, nkv, hd = self.nh, self.nkv, self.hd
@@ -338,6 +403,8 @@ class Attention(Mixer):
         tensor-core prompt kernel, where those kernels take this shape and type, or in 32 bits to the
         tiled kernel; whatever is left goes to the general kernel.  A row's kernel hangs on that row
         alone."""
+        if self.cache_bits:
+            return self._attend_packed(q, ctx, call)
         cache = ctx.caches[call.cache]
         table = ctx.block_table(call.cache)
         if self.general and self.heads_tile_tokens > 0:
@@ -448,6 +515,8 @@ class Attention(Mixer):
             weight, cache = self.w_q, None
             bias = bias[: self.nh * self.hd] if bias is not None else None
         projected = ops.linear(x, weight, out_dtype=torch.float32)
+        if self.cache_bits:
+            return self._project_out(self.attend(self._store_packed(projected, bias, ctx, call), ctx, call), projected, out_dtype)
         if self.halves:
             return self._forward_halves(projected, bias, ctx, call, cache, table, out_dtype)
         q = ops.qkv_pairs(projected, self.nh, self.nkv, self.hd, self.vd, bias, self.q_norm, self.k_norm, self.eps,
@@ -510,7 +579,7 @@ class Attention(Mixer):
         return self.attend(self._store_projected(projected, ctx, call), ctx, call)
 
     def _decodes_in_one(self, projected: torch.Tensor, ctx: StepContext, call: LayerCall) -> bool:
-        return (self.fast_decode and self.fused_position and call.writes_cache and projected.dtype == torch.bfloat16
+        return (self.fast_decode and not self.cache_bits and self.fused_position and call.writes_cache and projected.dtype == torch.bfloat16
                 and ctx.num_decode_rows == ctx.num_rows == ctx.num_tokens and ctx.num_rows >= self.fuse_decode_rows)
 
 

@@ -13,7 +13,7 @@ import torch
 
 from ..cache import PagedCacheSpec, StateCacheSpec
 from ..config.errors import ConfigError
-from ..config.spec import LayerSpec, ModelSpec
+from ..config.spec import LayerSpec, MixerSpec, ModelSpec
 from ..kernels import ops
 from ..weights.loader import WeightDecl, WeightStore, load_weights
 from .base import (BLOCKS, FEED_FORWARDS, INPUTS, MIXERS, NORMS, OUTPUTS, SIDES, ResidualStream, StepContext, lookup)
@@ -84,6 +84,33 @@ def cache_specs(spec: ModelSpec) -> list[PagedCacheSpec | StateCacheSpec | None]
     if need is not None:
         out.append(need)
     return out
+
+
+def with_cache_bits(spec: ModelSpec, bits: int, max_positions: int = 0) -> ModelSpec:
+    """``spec`` with the keys and values of all its layers held in ``bits`` bits (4); states of fixed size stay as they are.  Layers
+    whose attention has no kernels for that are refused when the model is built.  ``max_positions``: the longest context that will
+    be asked for, if it is below the model's own (tables of rotations end there)."""
+    if bits != 4:
+        raise ConfigError(f"keys and values are held in the model's type or in 4 bits, not in {bits}")
+    paged = False
+
+    def packed(mixer: MixerSpec) -> MixerSpec:
+        nonlocal paged
+        if "branches" in mixer.params:
+            branches = tuple((packed(sub), scale) for sub, scale in mixer.params["branches"])
+            return dataclasses.replace(mixer, params={**mixer.params, "branches": branches})
+        needs = lookup(MIXERS, "mixer", mixer.kind).cache_spec(mixer)
+        if not any(isinstance(need, PagedCacheSpec) for need in (needs if isinstance(needs, tuple) else (needs,))):
+            return mixer
+        if mixer.kind != "attention":
+            raise ConfigError(f"a cache in 4 bits is built for the 'attention' mixer, not for '{mixer.kind}'")
+        paged = True
+        return dataclasses.replace(mixer, params={**mixer.params, "cache_bits": bits, "cache_positions": max_positions})
+
+    layers = tuple(dataclasses.replace(layer, mixer=packed(layer.mixer)) for layer in spec.layers)
+    if not paged:
+        raise ConfigError("this model keeps no keys and values that could be held in 4 bits")
+    return dataclasses.replace(spec, layers=layers)
 
 
 def run_order_for(layers) -> tuple:

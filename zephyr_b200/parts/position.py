@@ -18,6 +18,7 @@ multiplier on cosine and sine.
 from __future__ import annotations
 
 import math
+import weakref
 
 import torch
 
@@ -34,6 +35,26 @@ def rope_tables(head_dim: int, max_positions: int, theta: float) -> tuple[torch.
     inv_freq = 1.0 / torch.pow(torch.tensor(float(theta), dtype=torch.float32), exponent)
     angles = torch.arange(max_positions, dtype=torch.float32)[:, None] * inv_freq[None, :]
     return torch.cos(angles).contiguous(), torch.sin(angles).contiguous()
+
+
+_TABLES: "weakref.WeakValueDictionary[tuple, _Tables]" = weakref.WeakValueDictionary()
+
+
+class _Tables:
+    def __init__(self, cos: torch.Tensor, sin: torch.Tensor):
+        self.cos, self.sin = cos, sin
+
+
+def rotation_tables(freqs: torch.Tensor, mult: float, positions: int) -> "_Tables":
+    """m cos(p f_i) and m sin(p f_i), float32 [positions, frequencies] on the frequencies' device, for the kernels that turn by tables;
+    angles are float32 products, as in the kernels that form them.  Layers of one rotation share one pair of tables while any of them
+    lives."""
+    key = (tuple(freqs.tolist()), mult, positions, freqs.device)
+    tables = _TABLES.get(key)
+    if tables is None:
+        angles = torch.arange(positions, dtype=torch.float32, device=freqs.device)[:, None] * freqs[None, :]
+        tables = _TABLES[key] = _Tables(angles.cos().mul_(mult), angles.sin_().mul_(mult))
+    return tables
 
 
 class RopeNeox(PositionEncoding):
