@@ -311,6 +311,9 @@ PROMPTS = [
     (8, 4, 128, 32, [300], [1000], {}),
     (6, 2, 128, 64, [200, 17], [64, 0], dict(window=90, sinks=True, softcap=15.0)),
     (4, 4, 128, 16, [260, 50], [33, 250], dict(chunk=100)),
+    (4, 2, 128, 16, [200], [5000], {}),                        # a head a CTA, many tiles
+    (32, 8, 128, 16, [600, 65], [2000, 3], {}),                # pairs of heads
+    (18, 3, 128, 32, [900, 150], [100, 777], dict(window=300, sinks=True, softcap=20.0)),
     (3, 3, 128, 16, [40], [129], dict(window=1)),
     (20, 2, 128, 16, [140], [0], dict(sinks=True)),
     (12, 4, 64, 16, [333, 90, 2], [100, 0, 61], {}),

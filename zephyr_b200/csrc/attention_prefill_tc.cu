@@ -244,8 +244,9 @@ __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, 
 // keeps its registers: with the chunk in it, seven prompts of 300 tokens took 58.8 us, 57.2 without).
 enum { TC_FORM_PLAIN, TC_FORM_BIASED, TC_FORM_CHUNKED, TC_FORM_KEPT };      // KEPT: first tokens kept, and a chunk
 // PACKED: over a 4-bit cache (packed.cuh), whose blocks six loader warps copy and turn into the ring's rows: two warps an item, three
-// items at a time.  Some 3000 instructions a tile of keys and values, which beside the softmax of both slots need as many warps as that
-// (three, with an item each: 1024 tokens behind 7000, 32/8 heads, 276 us); so the softmax warps take registers over from the others.
+// items at a time; the softmax warps take registers over from the others.  Some 4000 instructions a tile of keys and values, half of what
+// the softmax of a pair of heads takes, are issued between that softmax's own, and bound the kernel with it: 1024 tokens behind 7000,
+// 32/8 heads, 167 us (753 TFLOP/s) where the cache in bfloat16 takes 144; 8192 new tokens 660 against 530.
 // Keys are half-precision values (packed.cuh), a key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every
 // eight), and the queries' in the same.
 constexpr int TC_PACKED_THREADS = 512;             // warps 9 .. 14 load, the last one has nothing to do
@@ -254,7 +255,7 @@ constexpr int TC_PACKED_TEAMS = 3;
 constexpr int TC_PACKED_AHEAD = 3;                 // blocks of 16 positions that a warp has copied, the one that it works on among them
 constexpr int TC_PACKED_PART = pk_block_bytes(128) / 2;         // a block's keys, or its values
 constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_PART;
-constexpr int TC_PACKED_SOFTMAX_REGISTERS = 168, TC_PACKED_OTHER_REGISTERS = 88;
+constexpr int TC_PACKED_SOFTMAX_REGISTERS = 152, TC_PACKED_OTHER_REGISTERS = 104;
 static_assert(TC_PACKED_SMEM <= 223 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
 static_assert(256 * (TC_PACKED_SOFTMAX_REGISTERS + TC_PACKED_OTHER_REGISTERS) <= TC_PACKED_THREADS * 128, "no more registers than at launch");
 
@@ -926,6 +927,13 @@ int tc_split_tiles(int nh, int nkv, int n_tiles, int tile_rows, int sms) {
   return single <= sms || (single / 2 <= sms && n_tiles >= 4LL * tile_rows) ? n_tiles : 0;
 }
 
+// Over a 4-bit cache: a head a CTA turns a tile's codes into rows for half as many products, so pairs of heads unless every head gets
+// an SM at once.  (us, heads singly / in pairs, 32/8 heads: 640 tokens behind 8000 264 / 180, 1024 behind 7000 246 / 167, 1024 behind 300
+// 45 / 41, 1024 new 33 / 31; 16/8 heads, 300 new 13.4 / 15.7, 2048 new 46 / 49.)
+int tc_packed_split_tiles(int nh, int nkv, int n_tiles, int sms) {
+  return nh / nkv % 2 != 0 || static_cast<long long>(nh) * n_tiles <= sms ? n_tiles : 0;
+}
+
 template <int FORM, int HD, bool SHARED>
 int prefill_tc_launch(PrefillTcArgs& a, long long cache_rows, int page_size, cudaStream_t stream) {
   using Shape = TcShape<HD, SHARED>;
@@ -1042,7 +1050,7 @@ ZB_API int zb_paged_prefill_tc(void* out, const void* q, const void* kv_cache, c
 
 // The same over a 4-bit cache (packed.cuh): head size 128, pages of a power of two of positions from 16 on.
 ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
-                                      int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles, int tile_rows,
+                                      int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles,
                                       const int* row_q_start, const int* row_q_len, const int* row_ctx, int nh, int nkv, int window,
                                       int chunk, float scale, float softcap, const float* sinks, int* status, void* stream) {
   const int page_shift = pk_page_shift(page_size);
@@ -1050,13 +1058,12 @@ ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* pack
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(packed) % 16 != 0)
     return ERR_BAD_ARGUMENT;
   if (n_tiles == 0) return OK;
-  if (tile_rows <= 0) return ERR_BAD_ARGUMENT;
   if (n_tiles > 65535 || nh > 65535 || (static_cast<long long>(num_pages) * nkv << (page_shift - 4)) >= (1LL << 31)) return ERR_UNSUPPORTED;
   int device = 0, sms = 0;
   if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
   PrefillTcArgs a = {};
   a.n_tiles = n_tiles;
-  a.n_split = tc_split_tiles(nh, nkv, n_tiles, tile_rows, sms);
+  a.n_split = tc_packed_split_tiles(nh, nkv, n_tiles, sms);
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.kv_cache = static_cast<const __nv_bfloat16*>(packed);

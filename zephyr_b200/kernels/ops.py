@@ -125,7 +125,7 @@ _SIGNATURES = {
                                c_void_p, c_void_p],
     "zb_paged_prefill_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p],
-    "zb_paged_prefill_tc_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+    "zb_paged_prefill_tc_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
                                    c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p,
                                    c_void_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
@@ -369,7 +369,10 @@ def device_status(device: torch.device | str) -> torch.Tensor:
 def _device_status_pointer(device: torch.device) -> int | None:
     """Its address for a kernel that is called without one.  A capture that finds no word yet makes none, whose memory and zeros would be that
     graph's; the kernel then reports nowhere."""
-    if device not in _device_status and torch.cuda.is_current_stream_capturing():
+    word = _device_status.get(device)
+    if word is not None:
+        return word.data_ptr()
+    if torch.cuda.is_current_stream_capturing():
         return None
     return _ptr(device_status(device))
 
@@ -1360,31 +1363,49 @@ def packed_cache_shape(pages: int, nkv: int, page_size: int, hd: int) -> tuple[i
     return pages, nkv, page_size // PACKED_BLOCK, packed_block_bytes(hd)
 
 
-# (The calls below are made for every layer of a step: their checks make a message only where one fails.)
+# The calls below are made for every layer of a step: a tensor's type, order, place and address are asked for once each, and a message
+# is made only where a check fails (writing and reading back, two calls: 28.7 -> 25.9 us on the host).
 def _check_packed(packed: torch.Tensor, nkv: int, hd: int) -> tuple[int, int]:
-    block, shape = packed_block_bytes(hd), packed.shape
-    if len(shape) != 4 or shape[1] != nkv or shape[3] != block or packed.dtype != torch.uint8 or not packed.is_contiguous():
-        raise InvalidArgumentError(f"a 4-bit cache must be a contiguous uint8 [pages, {nkv}, page_size / 16, {block}] tensor")
-    page_size = shape[2] * PACKED_BLOCK
-    if not packed_page_size_ok(page_size):
+    if hd not in PACKED_HEAD_DIMS:
+        packed_block_bytes(hd)
+    shape = packed.shape
+    if len(shape) != 4 or shape[1] != nkv or shape[3] != 20 * hd or packed.dtype is not torch.uint8 or not packed.is_contiguous():
+        raise InvalidArgumentError(f"a 4-bit cache must be a contiguous uint8 [pages, {nkv}, page_size / 16, {20 * hd}] tensor")
+    blocks = shape[2]
+    if blocks < 1 or blocks & (blocks - 1) != 0:
         raise InvalidArgumentError("the pages of a 4-bit cache hold a power of two of positions, 16 or more")
-    if packed.data_ptr() % 16 != 0:
-        raise InvalidArgumentError("a 4-bit cache must start on a 16-byte boundary")
-    return shape[0], page_size
+    return shape[0], blocks * PACKED_BLOCK
 
 
-def _same_device(*tensors: torch.Tensor | None) -> None:
-    """Kernels are launched on the current device's current stream: all they are given lies there."""
-    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+def _check_index(*tensors: torch.Tensor) -> None:
     for t in tensors:
-        if t is not None and t.get_device() != current:       # (-1: a tensor on the CPU)
-            _cuda(t)
-            raise InvalidArgumentError(f"tensors of one call lie on the current device, cuda:{current}, not on {t.device}")
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            raise InvalidArgumentError("index tensors and status words must be contiguous int32")
 
 
-def _check_status_word(status: torch.Tensor) -> None:
-    if status.dtype != torch.int32 or status.numel() < 3 or not status.is_contiguous():
-        raise InvalidArgumentError("status must be an int32 status word (new_status)")
+def _addresses(*tensors: torch.Tensor | None) -> tuple[list, int]:
+    """The tensors' addresses (None for None), and the place of the first that lies elsewhere than kernels are launched, on the current
+    device's current stream (-1: a tensor on the CPU; that device itself where there is none)."""
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    place, at = current, []
+    for t in tensors:
+        if t is None:
+            at.append(None)
+            continue
+        if place == current:
+            place = t.get_device()
+        at.append(t.data_ptr())
+    if place != current:
+        return at, place
+    return at, -3
+
+
+def _check_place(place: int) -> None:
+    if place == -3:
+        return
+    if place < 0:
+        raise KernelError("zephyr_b200 kernels run on CUDA tensors only; there is no CPU path")
+    raise InvalidArgumentError(f"tensors of one call lie on the current device, cuda:{torch.cuda.current_device()}, not on cuda:{place}")
 
 
 def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w: torch.Tensor | None, k_norm_w: torch.Tensor | None,
@@ -1400,22 +1421,24 @@ def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w:
     float32 [positions, D / 2]; the first D channels of a head turn, in pairs (i, i + D / 2) with ``layout`` "halves" (D a multiple
     of 8), (2i, 2i + 1) with "pairs"; any scaling of frequencies and any multiplier is in the tables.  ``bias``: float32, one value a
     column.  A (row, position) comes once in a call."""
-    _i32(positions, token_row, block_table)
-    _check_status_word(status)
-    T, in_dtype = qkv.shape[0], qkv.dtype
+    _check_index(positions, token_row, block_table, status)
+    shape, table_shape, in_dtype = qkv.shape, block_table.shape, qkv.dtype
+    T = shape[0]
     dtype = dtype or in_dtype
     if hd not in PACKED_HEAD_DIMS or nh <= 0 or nkv <= 0:
         raise InvalidArgumentError(f"a 4-bit cache takes positive head counts and head sizes {PACKED_HEAD_DIMS}, not {nh}, {nkv}, {hd}")
     width = (nh + 2 * nkv) * hd if packed is not None else nh * hd
-    if qkv.dim() != 2 or qkv.shape[1] < width or qkv.stride(1) != 1 or in_dtype not in DTYPE_CODE:
+    if len(shape) != 2 or shape[1] < width or in_dtype not in DTYPE_CODE:
         raise InvalidArgumentError("qkv must be [T, (heads + 2*kv_heads)*head_dim] with unit inner stride")
-    stride = qkv.stride(0) if T > 1 else width
-    if stride < width or stride % 4 != 0 or qkv.data_ptr() % (16 if in_dtype == torch.float32 else 8) != 0:
-        raise InvalidArgumentError("rows of qkv must not overlap and must start on boundaries of four values")
-    if dtype != torch.bfloat16 and not (dtype == in_dtype == torch.float32):
+    stride, inner = qkv.stride()
+    if T <= 1:
+        stride = width
+    if inner != 1:
+        raise InvalidArgumentError("qkv must be [T, (heads + 2*kv_heads)*head_dim] with unit inner stride")
+    if dtype is not torch.bfloat16 and not (dtype is in_dtype is torch.float32):
         raise InvalidArgumentError("the queries are bfloat16, or float32 where qkv is")
-    if positions.numel() != T or token_row.numel() != T or block_table.dim() != 2:
-        raise InvalidArgumentError("one position and row per token, and a block_table [rows, blocks]")
+    if positions.numel() != T or token_row.numel() != T or len(table_shape) != 2 or status.numel() < 3:
+        raise InvalidArgumentError("one position and row per token, a block_table [rows, blocks] and a status word (new_status)")
     w_code = 0
     if q_norm_w is not None or k_norm_w is not None:
         if q_norm_w is None or k_norm_w is None or q_norm_w.dtype != k_norm_w.dtype:
@@ -1426,66 +1449,85 @@ def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w:
         raise InvalidArgumentError("layout is 'halves' or 'pairs', and cos and sin come together")
     half, max_positions = 0, 0
     if cos is not None:
-        if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+        rotated = cos.shape
+        if (len(rotated) != 2 or rotated != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
                 or not cos.is_contiguous() or not sin.is_contiguous()):
             raise InvalidArgumentError("cos/sin must be contiguous float32 [positions, rotated / 2]")
-        max_positions, half = cos.shape
-        if not 0 < 2 * half <= hd or (layout == "halves" and (half % 4 != 0 or cos.data_ptr() % 16 != 0 or sin.data_ptr() % 16 != 0)):
-            raise InvalidArgumentError("the rotated channels are part of the head, in halves a multiple of 8 of them with cos/sin on "
-                                       "16-byte boundaries")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != width or not bias.is_contiguous()):
+        max_positions, half = rotated
+    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != width or not bias.is_contiguous()):
         raise InvalidArgumentError(f"bias: {width} float32 values")
     pages, page_size = _check_packed(packed, nkv, hd) if packed is not None else (0, PACKED_BLOCK)
-    _same_device(qkv, positions, token_row, block_table, status, packed, q_norm_w, k_norm_w, cos, sin, bias, q_out)
     if q_out is None:
-        q_out = torch.empty((T, nh * hd), dtype=dtype, device=qkv.device)
-    elif q_out.shape != (T, nh * hd) or q_out.dtype != dtype or not q_out.is_contiguous() or q_out.data_ptr() % 16 != 0:
+        q_out = qkv.new_empty((T, nh * hd), dtype=dtype)
+    elif q_out.shape != (T, nh * hd) or q_out.dtype is not dtype or not q_out.is_contiguous():
         raise InvalidArgumentError("q_out must be contiguous [T, heads*head_dim] on a 16-byte boundary")
+    (qkv_at, positions_at, rows_at, table_at, status_at, packed_at, qw_at, kw_at, cos_at, sin_at, bias_at, out_at), place = _addresses(
+        qkv, positions, token_row, block_table, status, packed, q_norm_w, k_norm_w, cos, sin, bias, q_out)
+    if stride < width or stride % 4 != 0 or qkv_at % (16 if in_dtype is torch.float32 else 8) != 0:
+        raise InvalidArgumentError("rows of qkv must not overlap and must start on boundaries of four values")
+    if half and (2 * half > hd or (layout == "halves" and (half % 4 != 0 or cos_at % 16 != 0 or sin_at % 16 != 0))) or (cos is not None and not half):
+        raise InvalidArgumentError("the rotated channels are part of the head, in halves a multiple of 8 of them with cos/sin on "
+                                   "16-byte boundaries")
+    if out_at % 16 != 0 or (packed_at or 0) % 16 != 0:
+        raise InvalidArgumentError("q_out and a 4-bit cache start on 16-byte boundaries")
+    _check_place(place)
     _check(library().zb_qk_norm_rope_packed(
-        q_out.data_ptr(), qkv.data_ptr(), stride, _ptr(bias), _ptr(q_norm_w), _ptr(k_norm_w), w_code, eps, _ptr(cos), _ptr(sin), half,
-        max_positions, layout == "pairs", positions.data_ptr(), token_row.data_ptr(), _ptr(packed), block_table.data_ptr(),
-        block_table.shape[1], page_size, pages, block_table.shape[0], T, nh, nkv, hd, DTYPE_CODE[in_dtype], DTYPE_CODE[dtype],
-        status.data_ptr(), _stream()), "qk_norm_rope_packed")
+        out_at, qkv_at, stride, bias_at, qw_at, kw_at, w_code, eps, cos_at, sin_at, half, max_positions, layout == "pairs", positions_at,
+        rows_at, packed_at, table_at, table_shape[1], page_size, pages, table_shape[0], T, nh, nkv, hd, DTYPE_CODE[in_dtype],
+        DTYPE_CODE[dtype], status_at, _stream()), "qk_norm_rope_packed")
     return q_out
 
 
 def unpack_pages(packed: torch.Tensor, pages: torch.Tensor, dtype: torch.dtype, status: torch.Tensor | None = None) -> torch.Tensor:
     """What the given pages (int32) of a 4-bit cache stand for: [pages, 2 (keys, values), kv_heads, page_size, head_dim] in ``dtype``,
     channels in their natural order.  A page outside the cache is reported, and its part of the result is not written."""
-    _i32(pages)
+    _check_index(pages)
     if dtype not in DTYPE_CODE:
         raise InvalidArgumentError("values are bfloat16 or float32")
-    if packed.dim() != 4 or packed.shape[3] % 20 != 0:
+    shape = packed.shape
+    if len(shape) != 4 or shape[3] % 20 != 0:
         raise InvalidArgumentError("a 4-bit cache must be [pages, kv_heads, page_size / 16, 20 * head_dim]")
-    nkv, hd = packed.shape[1], packed.shape[3] // 20
+    nkv, hd, n = shape[1], shape[3] // 20, pages.numel()
     num_pages, page_size = _check_packed(packed, nkv, hd)
     if status is not None:
-        _check_status_word(status)
-    _same_device(packed, pages, status)
-    out = torch.empty((pages.numel(), 2, nkv, page_size, hd), dtype=dtype, device=packed.device)
+        _check_index(status)
+        if status.numel() < 3:
+            raise InvalidArgumentError("status must be a status word (new_status)")
+    (packed_at, pages_at, status_at), place = _addresses(packed, pages, status)
+    if packed_at % 16 != 0:
+        raise InvalidArgumentError("a 4-bit cache must start on a 16-byte boundary")
+    _check_place(place)
+    out = packed.new_empty((n, 2, nkv, page_size, hd), dtype=dtype)
     _check(library().zb_unpack_pages(
-        out.data_ptr(), packed.data_ptr(), pages.data_ptr(), pages.numel(), num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
-        status.data_ptr() if status is not None else _device_status_pointer(packed.device), _stream()), "unpack_pages")
+        out.data_ptr(), packed_at, pages_at, n, num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
+        status_at if status is not None else _device_status_pointer(packed.device), _stream()), "unpack_pages")
     return out
 
 
 def _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk, softcap,
-                           sinks) -> tuple[int, int]:
-    """(pages, page size), once everything that the two kinds of attention over a 4-bit cache share is found right."""
-    _check_status_word(status)
+                           sinks) -> tuple[int, int, int, int, int]:
+    """(tokens, rows, blocks a row, pages, page size), once what the two kinds of attention over a 4-bit cache share is found right."""
     if nh <= 0 or nkv <= 0 or nh % nkv != 0:
         raise InvalidArgumentError("head counts must be positive, heads divisible by kv_heads")
-    if q.dim() != 2 or q.shape[1] != nh * hd or q.dtype != torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16 != 0:
+    shape, table_shape = q.shape, block_table.shape
+    if len(shape) != 2 or shape[1] != nh * hd or q.dtype is not torch.bfloat16 or not q.is_contiguous():
         raise InvalidArgumentError("q must be contiguous bfloat16 [T, heads*head_dim] on a 16-byte boundary")
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16 != 0:
+    if out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous():
         raise InvalidArgumentError("out must match q")
-    if block_table.dim() != 2 or row_q_start.numel() < block_table.shape[0] or row_ctx.numel() < block_table.shape[0]:
-        raise InvalidArgumentError("block_table is [rows, blocks], with one start and context per row")
+    if len(table_shape) != 2 or row_q_start.numel() < table_shape[0] or row_ctx.numel() < table_shape[0] or status.numel() < 3:
+        raise InvalidArgumentError("block_table is [rows, blocks], with one start and context per row, and status a status word")
     if window < 0 or chunk < 0 or not softcap >= 0.0:
         raise InvalidArgumentError("window, chunk and softcap are not negative")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nh or not sinks.is_contiguous()):
+    if sinks is not None and (sinks.dtype is not torch.float32 or sinks.numel() != nh or not sinks.is_contiguous()):
         raise InvalidArgumentError("one float32 sink per query head")
-    return _check_packed(packed, nkv, hd)
+    return shape[0], *table_shape, *_check_packed(packed, nkv, hd)
+
+
+def _check_boundaries(place: int, *addresses: int) -> None:
+    for at in addresses:
+        if at % 16 != 0:
+            raise InvalidArgumentError("queries, results and a 4-bit cache start on 16-byte boundaries")
+    _check_place(place)
 
 
 PACKED_CLUSTERS, PACKED_CTA_SHARES, PACKED_WARP_SHARES = 0, 1, 2
@@ -1524,10 +1566,12 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
     writes those tokens' rows of ``out``.  bfloat16; ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  ``max_context`` is at
     least the longest context of the rows, the new token included.  ``plan``: as ``packed_decode_plan`` gives it (None: chosen by
     that).  The scratch of a launch is the call's own."""
-    _i32(block_table, rows, row_q_start, row_ctx)
-    pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk,
-                                              softcap, sinks)
-    _same_device(q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
+    _check_index(block_table, rows, row_q_start, row_ctx, status)
+    tokens, n_table, max_blocks, pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh,
+                                                                           nkv, hd, window, chunk, softcap, sinks)
+    (q_at, packed_at, table_at, rows_at, start_at, ctx_at, status_at, out_at, sinks_at), place = _addresses(
+        q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
+    _check_boundaries(place, q_at, packed_at, out_at)
     n_rows = rows.numel()
     if plan is None:
         visible = min(max_context, window) if window else max_context
@@ -1539,9 +1583,8 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
         scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(ctas, int(mode == PACKED_WARP_SHARES), pairs, hd)),
                               dtype=torch.float32, device=q.device)
     _check(library().zb_paged_decode_packed(
-        out.data_ptr(), q.data_ptr(), packed.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, pages,
-        block_table.shape[0], rows.data_ptr(), n_rows, row_q_start.data_ptr(), row_ctx.data_ptr(), max_context, q.shape[0], nh, nkv, hd,
-        window, chunk, scale, softcap, _ptr(sinks), mode, ctas, _ptr(scratch), status.data_ptr(), _stream()), "paged_decode_packed",
+        out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, rows_at, n_rows, start_at, ctx_at, max_context, tokens, nh,
+        nkv, hd, window, chunk, scale, softcap, sinks_at, mode, ctas, _ptr(scratch), status_at, _stream()), "paged_decode_packed",
         1 if mode == PACKED_CLUSTERS else 2)
     return out
 
@@ -1549,26 +1592,25 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
 def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, tile_row: torch.Tensor, tile_q0: torch.Tensor,
                          row_q_start: torch.Tensor, row_q_len: torch.Tensor, row_ctx: torch.Tensor, nh: int, nkv: int, hd: int,
                          window: int, scale: float, status: torch.Tensor, out: torch.Tensor, chunk: int = 0,
-                         sinks: torch.Tensor | None = None, softcap: float = 0.0, tile_rows: int | None = None,
-                         tensor_memory: bool = True) -> torch.Tensor:
+                         sinks: torch.Tensor | None = None, softcap: float = 0.0, tensor_memory: bool = True) -> torch.Tensor:
     """``paged_prefill`` over a 4-bit cache: attention of rows with several new tokens, cut into tiles of
     ``paged_prefill_tile_tokens()``, whose keys and values the cache holds already; writes those tokens' rows of ``out``.  bfloat16;
-    ``window``, ``chunk``, ``sinks``, ``softcap`` and ``tile_rows`` as there.  Head size 128 runs on tcgen05 (but the shortest prompts,
+    ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  Head size 128 runs on tcgen05 (but the shortest prompts,
     ``short_prompts``, and everything without ``tensor_memory``), other sizes on mma.sync."""
-    _i32(block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx)
-    pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd, window, chunk,
-                                              softcap, sinks)
+    _check_index(block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status)
+    _, n_table, max_blocks, pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd,
+                                                                      window, chunk, softcap, sinks)
     tiles = tile_row.numel()
-    if row_q_len.numel() < block_table.shape[0] or tile_q0.numel() != tiles:
+    if row_q_len.numel() < n_table or tile_q0.numel() != tiles:
         raise InvalidArgumentError("one length per row, and one first token per tile")
-    _same_device(q, packed, block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status, out, sinks)
-    lists = (out.data_ptr(), q.data_ptr(), packed.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, pages,
-             block_table.shape[0], tile_row.data_ptr(), tile_q0.data_ptr(), tiles)
-    rows = (row_q_start.data_ptr(), row_q_len.data_ptr(), row_ctx.data_ptr(), nh, nkv)
-    masks = (window, chunk, scale, softcap, _ptr(sinks), status.data_ptr(), _stream())
+    (q_at, packed_at, table_at, tile_row_at, tile_q0_at, start_at, len_at, ctx_at, status_at, out_at, sinks_at), place = _addresses(
+        q, packed, block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status, out, sinks)
+    _check_boundaries(place, q_at, packed_at, out_at)
+    lists = (out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, tile_row_at, tile_q0_at, tiles)
+    rows = (start_at, len_at, ctx_at, nh, nkv)
+    masks = (window, chunk, scale, softcap, sinks_at, status_at, _stream())
     if hd == 128 and tensor_memory and USE_TCGEN05_PREFILL and not short_prompts(block_table, page_size, nh, tiles):
-        tile_rows = block_table.shape[0] if tile_rows is None else int(tile_rows)
-        _check(library().zb_paged_prefill_tc_packed(*lists, tile_rows, *rows, *masks), "paged_prefill_tc_packed")
+        _check(library().zb_paged_prefill_tc_packed(*lists, *rows, *masks), "paged_prefill_tc_packed")
     else:
         _check(library().zb_paged_prefill_packed(*lists, *rows, hd, *masks), "paged_prefill_packed")
     return out

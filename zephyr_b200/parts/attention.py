@@ -368,8 +368,7 @@ class Attention(Mixer):
             ops.paged_decode_packed(q, cache, table, ctx.decode_rows, ctx.row_q_start, ctx.row_ctx, ctx.max_decode_context, *common, **masks)
         tile_row, tile_q0 = ctx.tiles[(self.prefill_tile_tokens, "multi")]
         if tile_row.numel() > 0:
-            ops.paged_prefill_packed(q, cache, table, tile_row, tile_q0, ctx.row_q_start, ctx.row_q_len, ctx.row_ctx, *common,
-                                     tile_rows=ctx.rows_with_tiles("multi"), **masks)
+            ops.paged_prefill_packed(q, cache, table, tile_row, tile_q0, ctx.row_q_start, ctx.row_q_len, ctx.row_ctx, *common, **masks)
         return out
 
     def _project_and_store(self, x: torch.Tensor, ctx: StepContext, call: LayerCall) -> torch.Tensor:
