@@ -76,8 +76,10 @@ struct PrefillArgs {
 // NS: stages of the ring of key/value tiles.  Two leave room for two CTAs an SM; three and four were measured
 // for tiles of one token (a decode step of 8 requests: 2.63 against 2.59 ms) and are not used.
 // DISTANT: with the distance bias (a form of its own, so that the others keep their registers).
-// PACKED: over a 4-bit cache (packed.cuh): a tile's blocks are copied as they are one tile ahead, and become bfloat16 rows in shared
-// memory between two barriers; without pooled blocks and kept tokens.
+// PACKED: over a 4-bit cache (packed.cuh): a tile's blocks are copied as they are two tiles ahead, where they lie is looked up three
+// ahead, and they become rows in shared memory one ahead, beside the products of the tile before (with a tile's rows made between two
+// barriers and its blocks looked up as they were copied: 333 tokens behind 1200, 12/4 heads of 64, 60 us
+// against 56); without pooled blocks and kept tokens.
 template <int HD, bool DEC, int NS, bool DISTANT, bool PACKED = false>
 __global__ void __launch_bounds__(PRE_WARPS * 32, 1)
 paged_prefill_kernel(const PrefillArgs a) {
@@ -130,32 +132,30 @@ paged_prefill_kernel(const PrefillArgs a) {
                             : static_cast<size_t>(tok0 + (ok ? j : 0)) * a.nh + head;
     cp_async_16(q_s + j * KROW + c, a.q + from * HD + c, ok);
   }
-  // PACKED: two tiles' blocks behind the ring's one stage, and whether a block's page was found.
+  // PACKED: two tiles' blocks behind the ring, and where the blocks of four tiles lie (-1: nowhere, or nothing of it is seen).
   constexpr int RAW_BLOCKS = PRE_BN / PK_BLOCK, RAW_BYTES = RAW_BLOCKS * pk_block_bytes(HD);
-  unsigned char* const raw = reinterpret_cast<unsigned char*>(ring + STAGE);
-  __shared__ int raw_ok[2][RAW_BLOCKS];
+  unsigned char* const raw = reinterpret_cast<unsigned char*>(ring + 2 * STAGE);
+  __shared__ long long raw_from[4][RAW_BLOCKS];
+  auto look_up = [&](int block) {    // counted from the first tile's first
+    const int pos = first_tile + block * PK_BLOCK;
+    if (pos >= hi || pos + PK_BLOCK <= lo) return -1LL;
+    const int entry = pos >> a.page_shift, page = entry < a.max_blocks ? table[entry] : -1;
+    if (page <= 0 || page >= a.num_pages) {
+      report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, tok0);
+      return -1LL;
+    }
+    return (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (a.page_size - 1)) >> 4)) * pk_block_bytes(HD);
+  };
   auto load_packed = [&](int t) {
     constexpr int PIECES = pk_block_bytes(HD) / 16;
     const unsigned char* const source = reinterpret_cast<const unsigned char*>(a.kv_cache);
     for (int e = threadIdx.x; e < RAW_BLOCKS * PIECES; e += PRE_WARPS * 32) {
-      const int b = e / PIECES, c = e - b * PIECES, pos = first_tile + t * PRE_BN + b * PK_BLOCK;
-      bool ok = pos < hi && pos + PK_BLOCK > lo;
-      long long from = 0;
-      if (ok) {
-        const int entry = pos >> a.page_shift, page = entry < a.max_blocks ? table[entry] : -1;
-        if (page <= 0 || page >= a.num_pages) {
-          if (c == 0) report(a.status, STATUS_PAGE_OUT_OF_RANGE, page, tok0);
-          ok = false;
-        } else {
-          from = (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (a.page_size - 1)) >> 4)) * pk_block_bytes(HD);
-        }
-      }
-      if (c == 0) raw_ok[t & 1][b] = ok;
-      if (ok) cp_async_16(raw + (t & 1) * RAW_BYTES + e * 16, source + from + c * 16, true);
+      const long long from = raw_from[t & 3][e / PIECES];
+      if (from >= 0) cp_async_16(raw + (t & 1) * RAW_BYTES + e * 16, source + from + e % PIECES * 16, true);
     }
   };
   auto expand = [&](int t) {
-    __nv_bfloat16* const ks = ring;
+    __nv_bfloat16* const ks = ring + (t & 1) * STAGE;
     __nv_bfloat16* const vs = ks + PRE_BN * KROW;
     const unsigned char* const blocks = raw + (t & 1) * RAW_BYTES;
     const int k0 = first_tile + t * PRE_BN;
@@ -163,7 +163,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     for (int e = threadIdx.x; e < PRE_BN * CHUNKS; e += PRE_WARPS * 32) {
       const int j = e / CHUNKS, c = e - j * CHUNKS, p = j & (PK_BLOCK - 1);
       const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
-      const bool ok = raw_ok[t & 1][j >> 4] && k0 + j >= lo && k0 + j < hi;
+      const bool ok = raw_from[t & 3][j >> 4] >= 0 && k0 + j >= lo && k0 + j < hi;
       const unsigned short* const params = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
       *reinterpret_cast<uint4*>(ks + j * KROW + c * 8) =
           ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_half_twice(pk_low(params[0])), pk_half_twice(pk_low(params[HD / 32])))
@@ -177,7 +177,7 @@ paged_prefill_kernel(const PrefillArgs a) {
       uint4 even, odd;
       pk_value_channels(*reinterpret_cast<const unsigned*>(words), *reinterpret_cast<const unsigned*>(words + HD / 2),
                         *reinterpret_cast<const unsigned*>(params), *reinterpret_cast<const unsigned*>(params + HD / 8), even, odd);
-      const bool page_ok = raw_ok[t & 1][j >> 4];
+      const bool page_ok = raw_from[t & 3][j >> 4] >= 0;
       *reinterpret_cast<uint4*>(vs + j * KROW + c * 8) = page_ok && k0 + j >= lo && k0 + j < hi ? even : zeros;
       *reinterpret_cast<uint4*>(vs + (j + 1) * KROW + c * 8) = page_ok && k0 + j + 1 >= lo && k0 + j + 1 < hi ? odd : zeros;
     }
@@ -221,12 +221,19 @@ paged_prefill_kernel(const PrefillArgs a) {
   };
 #pragma unroll
   for (int t = 0; t < NS - 1; ++t) {         // one group of copies a tile, empty ones past the end
-    if (PACKED) {
-      if (t < n_tiles) load_packed(t);
-    } else if (t < n_tiles) {
-      load_tile(t);
-    }
+    if (!PACKED && t < n_tiles) load_tile(t);
     cp_async_commit();
+  }
+  if (PACKED) {
+    if (threadIdx.x < 3 * RAW_BLOCKS) raw_from[threadIdx.x / RAW_BLOCKS][threadIdx.x % RAW_BLOCKS] = look_up(threadIdx.x);
+    __syncthreads();
+    load_packed(0);
+    cp_async_commit();
+    if (1 < n_tiles) load_packed(1);
+    cp_async_commit();
+    cp_async_wait<1>();
+    __syncthreads();
+    expand(0);
   }
 
   // This warp's 16 query rows; this lane's two rows sit at positions qpos[0] and qpos[1].
@@ -269,11 +276,11 @@ paged_prefill_kernel(const PrefillArgs a) {
   for (int t = 0; t < n_tiles; ++t) {
     cp_async_wait<NS - 2>();
     __syncthreads();                 // tile t (and, the first time, Q) has landed; tile t-1 is no longer read
-    if (PACKED) {
-      if (t + 1 < n_tiles) load_packed(t + 1);
+    if (PACKED) {                    // tile t's rows are made, t + 1's blocks have landed, it is known where t + 2's lie
+      if (t + 2 < n_tiles) load_packed(t + 2);
       cp_async_commit();
-      expand(t);
-      __syncthreads();
+      if (threadIdx.x < RAW_BLOCKS) raw_from[(t + 3) & 3][threadIdx.x] = look_up((t + 3) * RAW_BLOCKS + threadIdx.x);
+      if (t + 1 < n_tiles) expand(t + 1);
     } else {
       if (t + NS - 1 < n_tiles) load_tile(t + NS - 1);
       cp_async_commit();
@@ -295,7 +302,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     if (!warp_active) continue;                          // uniform over the warp, as are the next two
     if (run == 0 && k0 >= warp_seen) continue;
     if (run == 2 && (k0 > warp_last_pos || (k0 + PRE_BN <= warp_first_visible && k0 >= a.keep_first))) continue;
-    const __nv_bfloat16* ks_tile = ring + (PACKED ? 0 : t % NS) * STAGE;
+    const __nv_bfloat16* ks_tile = ring + t % NS * STAGE;
     const __nv_bfloat16* vs_tile = ks_tile + PRE_BN * KROW;
 
     // The key tiles of 8 this warp works on: all eight of the 64 keys, or (DEC) the warp's own one.
@@ -499,7 +506,7 @@ int prefill_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream, bool 
 
 template <int HD>
 int prefill_packed_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream) {
-  const size_t smem = (static_cast<size_t>(PRE_BM) + 2 * PRE_BN) * (HD + 8) * sizeof(__nv_bfloat16) + 2 * (PRE_BN / PK_BLOCK) * pk_block_bytes(HD);
+  const size_t smem = (static_cast<size_t>(PRE_BM) + 4 * PRE_BN) * (HD + 8) * sizeof(__nv_bfloat16) + 2 * (PRE_BN / PK_BLOCK) * pk_block_bytes(HD);
   auto kernel = paged_prefill_kernel<HD, false, 2, false, true>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return ERR_CUDA;
   kernel<<<dim3(a.nh, n_tiles), PRE_WARPS * 32, smem, stream>>>(a);
