@@ -80,13 +80,22 @@ struct PrefillArgs {
 // ahead, and they become rows in shared memory one ahead, beside the products of the tile before (with a tile's rows made between two
 // barriers and its blocks looked up as they were copied: 333 tokens behind 1200, 12/4 heads of 64, 60 us
 // against 56); without pooled blocks and kept tokens.
+// GROUPS: of eight warps each, which take the tiles in turn, with rings of their own, and whose results meet at the end; two where
+// PACKED and the registers last (heads of 32 to 96), since eight warps, an SM's fill, leave it idle half of the time (the above 56 us
+// with one group, 46 with two; 1024 tokens behind 2000, 16/8 heads of 64, 104 and 83).  Instructions bound it then: of some 800 a warp
+// and tile, scales that join a score in its exponent, 2^x without its range's ends and sums that are rescaled only where a maximum
+// moved took 150 (42 and 76 us).
+template <int HD, bool PACKED>
+constexpr int PRE_GROUPS = PACKED && HD <= 96 ? 2 : 1;
+
 template <int HD, bool DEC, int NS, bool DISTANT, bool PACKED = false>
-__global__ void __launch_bounds__(PRE_WARPS * 32, 1)
+__global__ void __launch_bounds__(PRE_WARPS * 32 * PRE_GROUPS<HD, PACKED>, 1)
 paged_prefill_kernel(const PrefillArgs a) {
   static_assert(HD % 32 == 0 && HD <= 256, "head sizes that are multiples of 32, up to 256");
   constexpr int KROW = HD + 8;                      // padded rows: conflict-free ldmatrix
   constexpr int CHUNKS = HD / 8;
   constexpr int STAGE = 2 * PRE_BN * KROW;
+  constexpr int GROUPS = PRE_GROUPS<HD, PACKED>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __nv_bfloat16* q_s = reinterpret_cast<__nv_bfloat16*>(smem_raw);     // [PRE_BM][KROW]
   __nv_bfloat16* ring = q_s + PRE_BM * KROW;                             // [2][keys, values][PRE_BN][KROW]
@@ -108,7 +117,8 @@ paged_prefill_kernel(const PrefillArgs a) {
   const int n_tok = DEC ? min(1, q_len - q0) : min(PRE_BM, q_len - q0);
   if (n_tok <= 0) return;
   const int n_rows = DEC ? min(g, PRE_BM) : n_tok;       // query rows of this CTA: heads of the group, or tokens
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = GROUPS > 1 ? threadIdx.x / (PRE_WARPS * 32) : 0, tid = GROUPS > 1 ? threadIdx.x % (PRE_WARPS * 32) : threadIdx.x;
+  const int warp = tid >> 5, lane = threadIdx.x & 31;
   const int quad_row = lane >> 2, quad_col = (lane & 3) * 2;
   const int* table = a.block_table + static_cast<size_t>(row) * a.max_blocks;
 
@@ -125,17 +135,20 @@ paged_prefill_kernel(const PrefillArgs a) {
   const int n_tiles = pool_tiles + kept_tiles + (hi - first_tile + PRE_BN - 1) / PRE_BN;
   const int* pool_table = a.pool > 0 ? a.pool_table + static_cast<size_t>(row) * a.pool_max_blocks : nullptr;
 
-  for (int e = threadIdx.x; e < PRE_BM * CHUNKS; e += PRE_WARPS * 32) {
+  for (int e = threadIdx.x; e < PRE_BM * CHUNKS; e += GROUPS * PRE_WARPS * 32) {
     const int j = e / CHUNKS, c = (e - j * CHUNKS) * 8;
     const bool ok = j < n_rows;
     const size_t from = DEC ? static_cast<size_t>(tok0) * a.nh + head + (ok ? j : 0)
                             : static_cast<size_t>(tok0 + (ok ? j : 0)) * a.nh + head;
     cp_async_16(q_s + j * KROW + c, a.q + from * HD + c, ok);
   }
-  // PACKED: two tiles' blocks behind the ring, and where the blocks of four tiles lie (-1: nowhere, or nothing of it is seen).
+  // PACKED: two tiles' blocks behind the group's ring, and where the blocks of four tiles lie (-1: nowhere, or nothing of it is seen).
   constexpr int RAW_BLOCKS = PRE_BN / PK_BLOCK, RAW_BYTES = RAW_BLOCKS * pk_block_bytes(HD);
+  __nv_bfloat16* const first_ring = ring;
+  if (GROUPS > 1) ring += group * (2 * STAGE + RAW_BYTES);
   unsigned char* const raw = reinterpret_cast<unsigned char*>(ring + 2 * STAGE);
-  __shared__ long long raw_from[4][RAW_BLOCKS];
+  __shared__ long long raw_from_s[GROUPS][4][RAW_BLOCKS];
+  auto& raw_from = raw_from_s[group];
   auto look_up = [&](int block) {    // counted from the first tile's first
     const int pos = first_tile + block * PK_BLOCK;
     if (pos >= hi || pos + PK_BLOCK <= lo) return -1LL;
@@ -146,30 +159,31 @@ paged_prefill_kernel(const PrefillArgs a) {
     }
     return (((static_cast<long long>(page) * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (a.page_size - 1)) >> 4)) * pk_block_bytes(HD);
   };
-  auto load_packed = [&](int t) {
+  // A group's i-th tile is tile i * GROUPS + group.
+  auto load_packed = [&](int i) {
     constexpr int PIECES = pk_block_bytes(HD) / 16;
     const unsigned char* const source = reinterpret_cast<const unsigned char*>(a.kv_cache);
-    for (int e = threadIdx.x; e < RAW_BLOCKS * PIECES; e += PRE_WARPS * 32) {
-      const long long from = raw_from[t & 3][e / PIECES];
-      if (from >= 0) cp_async_16(raw + (t & 1) * RAW_BYTES + e * 16, source + from + e % PIECES * 16, true);
+    for (int e = tid; e < RAW_BLOCKS * PIECES; e += PRE_WARPS * 32) {
+      const long long from = raw_from[i & 3][e / PIECES];
+      if (from >= 0) cp_async_16(raw + (i & 1) * RAW_BYTES + e * 16, source + from + e % PIECES * 16, true);
     }
   };
-  auto expand = [&](int t) {
-    __nv_bfloat16* const ks = ring + (t & 1) * STAGE;
+  auto expand = [&](int i) {
+    __nv_bfloat16* const ks = ring + (i & 1) * STAGE;
     __nv_bfloat16* const vs = ks + PRE_BN * KROW;
-    const unsigned char* const blocks = raw + (t & 1) * RAW_BYTES;
-    const int k0 = first_tile + t * PRE_BN;
+    const unsigned char* const blocks = raw + (i & 1) * RAW_BYTES;
+    const int k0 = first_tile + (i * GROUPS + group) * PRE_BN;
     const uint4 zeros = make_uint4(0, 0, 0, 0);
-    for (int e = threadIdx.x; e < PRE_BN * CHUNKS; e += PRE_WARPS * 32) {
+    for (int e = tid; e < PRE_BN * CHUNKS; e += PRE_WARPS * 32) {
       const int j = e / CHUNKS, c = e - j * CHUNKS, p = j & (PK_BLOCK - 1);
       const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
-      const bool ok = raw_from[t & 3][j >> 4] >= 0 && k0 + j >= lo && k0 + j < hi;
+      const bool ok = raw_from[i & 3][j >> 4] >= 0 && k0 + j >= lo && k0 + j < hi;
       const unsigned short* const params = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
       *reinterpret_cast<uint4*>(ks + j * KROW + c * 8) =
           ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_half_twice(pk_low(params[0])), pk_half_twice(pk_low(params[HD / 32])))
              : zeros;
     }
-    for (int e = threadIdx.x; e < PRE_BN / 2 * CHUNKS; e += PRE_WARPS * 32) {
+    for (int e = tid; e < PRE_BN / 2 * CHUNKS; e += PRE_WARPS * 32) {
       const int pair = e / CHUNKS, c = e - pair * CHUNKS, j = 2 * pair, own = pair & (PK_BLOCK / 2 - 1);
       const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
       const unsigned char* const words = block + pk_value_word<HD>(own >> 2, 2 * (c & 3), own & 3, c >> 2);
@@ -177,7 +191,7 @@ paged_prefill_kernel(const PrefillArgs a) {
       uint4 even, odd;
       pk_value_channels(*reinterpret_cast<const unsigned*>(words), *reinterpret_cast<const unsigned*>(words + HD / 2),
                         *reinterpret_cast<const unsigned*>(params), *reinterpret_cast<const unsigned*>(params + HD / 8), even, odd);
-      const bool page_ok = raw_from[t & 3][j >> 4] >= 0;
+      const bool page_ok = raw_from[i & 3][j >> 4] >= 0;
       *reinterpret_cast<uint4*>(vs + j * KROW + c * 8) = page_ok && k0 + j >= lo && k0 + j < hi ? even : zeros;
       *reinterpret_cast<uint4*>(vs + (j + 1) * KROW + c * 8) = page_ok && k0 + j + 1 >= lo && k0 + j + 1 < hi ? odd : zeros;
     }
@@ -225,11 +239,12 @@ paged_prefill_kernel(const PrefillArgs a) {
     cp_async_commit();
   }
   if (PACKED) {
-    if (threadIdx.x < 3 * RAW_BLOCKS) raw_from[threadIdx.x / RAW_BLOCKS][threadIdx.x % RAW_BLOCKS] = look_up(threadIdx.x);
+    if (tid < 3 * RAW_BLOCKS)
+      raw_from[tid / RAW_BLOCKS][tid % RAW_BLOCKS] = look_up((tid / RAW_BLOCKS * GROUPS + group) * RAW_BLOCKS + tid % RAW_BLOCKS);
     __syncthreads();
     load_packed(0);
     cp_async_commit();
-    if (1 < n_tiles) load_packed(1);
+    load_packed(1);
     cp_async_commit();
     cp_async_wait<1>();
     __syncthreads();
@@ -260,8 +275,12 @@ paged_prefill_kernel(const PrefillArgs a) {
       r2[h] = a.bias_r2[row_head];
     }
   }
+  // PACKED: the scale joins a score in its exponent, where scores have no bound and the scale keeps their order.
+  const bool late_scale = PACKED && a.softcap_log2 == 0.0f && a.scale_log2 > 0.0f;
+  const float late = late_scale ? a.scale_log2 : 1.0f;
   // A raw score of this lane's row h whose key lies at `pos`, scaled, bounded and biased.
   auto finished = [&](float raw, int h, int pos) {
+    if (late_scale) return raw;
     float v = a.softcap_log2 > 0.0f ? a.softcap_log2 * tanhf(raw * a.scale_over_cap) : raw * a.scale_log2;
     if (DISTANT) v = fmaf(-r1[h], __log2f(fmaf(r2[h], static_cast<float>(qpos[h] - pos), 1.0f)), v);
     return v;
@@ -273,19 +292,21 @@ paged_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
   for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
-  for (int t = 0; t < n_tiles; ++t) {
+  for (int t = group; t < n_tiles; t += GROUPS) {
     cp_async_wait<NS - 2>();
-    __syncthreads();                 // tile t (and, the first time, Q) has landed; tile t-1 is no longer read
-    if (PACKED) {                    // tile t's rows are made, t + 1's blocks have landed, it is known where t + 2's lie
-      if (t + 2 < n_tiles) load_packed(t + 2);
+    if (GROUPS > 1) asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(PRE_WARPS * 32) : "memory");
+    else __syncthreads();            // tile t (and, the first time, Q) has landed; tile t-1 is no longer read
+    if (PACKED) {                    // the tile's rows are made, the next one's blocks have landed, it is known where those of the one after lie
+      const int i = t / GROUPS;
+      load_packed(i + 2);
       cp_async_commit();
-      if (threadIdx.x < RAW_BLOCKS) raw_from[(t + 3) & 3][threadIdx.x] = look_up((t + 3) * RAW_BLOCKS + threadIdx.x);
-      if (t + 1 < n_tiles) expand(t + 1);
+      if (tid < RAW_BLOCKS) raw_from[(i + 3) & 3][tid] = look_up((t + 3 * GROUPS) * RAW_BLOCKS + tid);
+      if (t + GROUPS < n_tiles) expand(i + 1);
     } else {
       if (t + NS - 1 < n_tiles) load_tile(t + NS - 1);
       cp_async_commit();
     }
-    if (t == 0) {
+    if (t == group) {
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         ldmatrix_x4(qa[ks], q_s + (warp_row0 + (lane & 7) + ((lane >> 3) & 1) * 8) * KROW + ks * 16 + (lane >> 4) * 8);
@@ -302,7 +323,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     if (!warp_active) continue;                          // uniform over the warp, as are the next two
     if (run == 0 && k0 >= warp_seen) continue;
     if (run == 2 && (k0 > warp_last_pos || (k0 + PRE_BN <= warp_first_visible && k0 >= a.keep_first))) continue;
-    const __nv_bfloat16* ks_tile = ring + t % NS * STAGE;
+    const __nv_bfloat16* ks_tile = ring + t / GROUPS % NS * STAGE;
     const __nv_bfloat16* vs_tile = ks_tile + PRE_BN * KROW;
 
     // The key tiles of 8 this warp works on: all eight of the 64 keys, or (DEC) the warp's own one.
@@ -367,6 +388,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     for (int h = 0; h < 2; ++h) {
       tile_max[h] = fmaxf(tile_max[h], __shfl_xor_sync(0xffffffffu, tile_max[h], 1));
       tile_max[h] = fmaxf(tile_max[h], __shfl_xor_sync(0xffffffffu, tile_max[h], 2));
+      if (PACKED) tile_max[h] *= late;
       const float new_m = fmaxf(m_run[h], tile_max[h]);
       m_use[h] = new_m == -INFINITY ? 0.0f : new_m;      // a row that has seen no key yet: keep exp2 finite
       corr[h] = exp2f(m_run[h] - m_use[h]);              // 0 while the running maximum is -inf
@@ -377,7 +399,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     for (int i = 0; i < NTS; ++i) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        s[i][c] = exp2f(s[i][c] - m_use[c >> 1]);
+        s[i][c] = PACKED ? pk_exp2(fmaf(s[i][c], late, -m_use[c >> 1])) : exp2f(s[i][c] - m_use[c >> 1]);
         row_sum[c >> 1] += s[i][c];
       }
     }
@@ -387,9 +409,11 @@ paged_prefill_kernel(const PrefillArgs a) {
       row_sum[h] += __shfl_xor_sync(0xffffffffu, row_sum[h], 2);
       l_run[h] = l_run[h] * corr[h] + row_sum[h];
     }
+    if (!PACKED || __any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-      o[n][0] *= corr[0]; o[n][1] *= corr[0]; o[n][2] *= corr[1]; o[n][3] *= corr[1];
+      for (int n = 0; n < HD / 8; ++n) {
+        o[n][0] *= corr[0]; o[n][1] *= corr[0]; o[n][2] *= corr[1]; o[n][3] *= corr[1];
+      }
     }
     if (DEC) {
       // 8 keys: the product's second half of 8 takes zero weights (and reads the same 8 value rows again).
@@ -462,6 +486,39 @@ paged_prefill_kernel(const PrefillArgs a) {
     }
     return;
   }
+  if (GROUPS > 1) {
+    // The second group's sums join the first's, on the larger of the two maxima.
+    float* const part_o = reinterpret_cast<float*>(first_ring);      // [PRE_BM][HD]
+    float2* const part_ml = reinterpret_cast<float2*>(q_s);          // [PRE_BM]
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = warp_row0 + quad_row + 8 * h;
+        if ((lane & 3) == 0) part_ml[r] = make_float2(m_run[h], l_run[h]);
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+          *reinterpret_cast<float2*>(part_o + r * HD + n * 8 + quad_col) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+      }
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = warp_row0 + quad_row + 8 * h;
+      const float2 ml = part_ml[r];
+      const float top = fmaxf(m_run[h], ml.x);
+      const float own = m_run[h] > -INFINITY ? exp2f(m_run[h] - top) : 0.0f, other = ml.x > -INFINITY ? exp2f(ml.x - top) : 0.0f;
+      m_run[h] = top;
+      l_run[h] = l_run[h] * own + ml.y * other;
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) {
+        const float2 x = *reinterpret_cast<const float2*>(part_o + r * HD + n * 8 + quad_col);
+        o[n][2 * h] = o[n][2 * h] * own + x.x * other;
+        o[n][2 * h + 1] = o[n][2 * h + 1] * own + x.y * other;
+      }
+    }
+  }
   if (!warp_active) return;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -506,10 +563,12 @@ int prefill_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream, bool 
 
 template <int HD>
 int prefill_packed_launch(const PrefillArgs& a, int n_tiles, cudaStream_t stream) {
-  const size_t smem = (static_cast<size_t>(PRE_BM) + 4 * PRE_BN) * (HD + 8) * sizeof(__nv_bfloat16) + 2 * (PRE_BN / PK_BLOCK) * pk_block_bytes(HD);
+  constexpr int GROUPS = PRE_GROUPS<HD, true>;
+  const size_t smem = (static_cast<size_t>(PRE_BM) + GROUPS * 4 * PRE_BN) * (HD + 8) * sizeof(__nv_bfloat16) +
+                      GROUPS * 2 * (PRE_BN / PK_BLOCK) * pk_block_bytes(HD);
   auto kernel = paged_prefill_kernel<HD, false, 2, false, true>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return ERR_CUDA;
-  kernel<<<dim3(a.nh, n_tiles), PRE_WARPS * 32, smem, stream>>>(a);
+  kernel<<<dim3(a.nh, n_tiles), GROUPS * PRE_WARPS * 32, smem, stream>>>(a);
   return launch_result();
 }
 

@@ -129,6 +129,13 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 2^x, off by at most 2^-22 of it.
+__device__ __forceinline__ float pk_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // A word of a key as its eight channels in order, four such pairs.
 __device__ __forceinline__ uint4 pk_key_channels(unsigned word, unsigned steps, unsigned offsets) {
   unsigned r[4];
