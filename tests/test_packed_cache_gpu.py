@@ -349,6 +349,28 @@ def test_prompts(ops, cuda_device, nh, nkv, hd, page, new, cached, masks, tensor
         assert ((out[mine].cpu().double().view(n, nh, hd) - expected).abs() <= bound).all(), r
 
 
+@pytest.mark.parametrize("hd,tensor_memory", [(64, False), (128, False), (128, True)])
+def test_a_query_that_is_not_finite_spoils_its_own_result_only(ops, cuda_device, hd, tensor_memory):
+    packed, table, _ = paged_case(cuda_device, 2, hd, 16, [150, 70], 67)
+    q = torch.randn((70, 4 * hd), generator=torch.Generator().manual_seed(71)).to(torch.bfloat16).to(cuda_device)
+    status, outs, tile = ops.new_status(cuda_device), [], ops.paged_prefill_tile_tokens()
+    assert tile >= 70
+    for value in (0.5, float("inf"), float("nan")):
+        q[69, hd + 5] = value
+        out = torch.zeros_like(q)
+        ops.paged_prefill_packed(q, packed, table, i32(cuda_device, [0]), i32(cuda_device, [0]), i32(cuda_device, [0, 0]), i32(cuda_device, [70, 0]),
+                                 i32(cuda_device, [80, 0]), 4, 2, hd, 0, hd ** -0.5, status, out, tensor_memory=tensor_memory)
+        one = torch.zeros_like(q)
+        ops.paged_decode_packed(q, packed, table, i32(cuda_device, [0]), i32(cuda_device, [69, 0]), i32(cuda_device, [149, 69]), 150, 4, 2, hd, 0,
+                                hd ** -0.5, status, one)
+        outs.append(torch.stack([out, one]).view(2, 70, 4, hd))
+    ops.check_status(status)
+    for bad in outs[1:]:
+        assert not torch.isfinite(bad[:, 69, 1]).any()
+        bad[:, 69, 1] = outs[0][:, 69, 1]
+        assert torch.equal(bad, outs[0])
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompts_report_bad_pages_and_rows(ops, cuda_device, hd):
     nh, nkv, new, cached = 4, 2, [150, 140], [40, 20]

@@ -781,9 +781,9 @@ int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStr
   static std::atomic<unsigned long long> raised{0};          // devices on which the kernel may have all it can ever ask for
   int device = 0, sms = 0;
   if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
-  // Where every CTA can have an SM, it asks for more than half of one's shared memory: else some SMs get two CTAs and others none
+  // Where every CTA can have an SM (of the share that the launch may take), it asks for more than half of one's shared memory: else some SMs get two CTAs and others none
   // (8 rows of 4096, 8 key/value heads, 128 CTAs: 18.2 or, as often, 24.1 us).
-  if (grid <= sms && smem < PD_MORE_THAN_HALF) smem = PD_MORE_THAN_HALF;
+  if (grid <= shared_sm_count(sms) && smem < PD_MORE_THAN_HALF) smem = PD_MORE_THAN_HALF;
   if (smem > 227 * 1024) return ERR_UNSUPPORTED;
   const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
   if ((raised.load(std::memory_order_relaxed) & bit) == 0) {

@@ -117,10 +117,10 @@ __device__ __forceinline__ void pk_half_values(unsigned word, unsigned steps, un
     r[i] = pk_fma_f16x2(code, steps, offsets);
   }
 }
-// Two bfloat16 values as half-precision ones.
+// Two bfloat16 values as half-precision ones (exact from 2^-17 on; beyond 65504 infinite).
 __device__ __forceinline__ unsigned pk_to_half(unsigned pair) {
   unsigned r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(__uint_as_float(pair & 0xffff0000u)), "f"(__uint_as_float(pair << 16)));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(__uint_as_float(pair & 0xffff0000u)), "f"(__uint_as_float(pair << 16)));
   return r;
 }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
