@@ -177,3 +177,13 @@ def test_generation_with_four_bits(model_folders, cuda_device):
     sized = engine(memory_bytes=200 * 16 * 2 * 2 * 160)
     assert sized.runner.manager.num_free_pages() == 192 and sized.runner.cache_bytes_per_token() == 640
     assert [list(o.token_ids) for o in sized.generate(prompts[:1], max_tokens=24, temperature=0.0, ignore_eos=True)][0]
+
+
+def test_the_timing_program_times_it(cuda_device, capsys):
+    import json
+
+    from zephyr_b200.kernels import timing
+
+    assert timing.main(["packed_cache", "--warmup", "1", "--iters", "2", "--batch", "2", "--context", "300", "--tokens", "70", "--head-dim", "64"]) == 0
+    line = json.loads(capsys.readouterr().out)
+    assert set(line["us"]) == {"decode", "decode_bfloat16", "prompt", "prompt_bfloat16", "write", "write_bfloat16", "read_back"}

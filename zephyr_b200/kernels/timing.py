@@ -16,6 +16,7 @@
     python -m zephyr_b200.kernels.timing experts --tokens 2048 --hidden 2048 --ffn 1536 --experts 16 --top 4
     python -m zephyr_b200.kernels.timing head_linear --tokens 2048 --heads 16 --n 128 --k 128
     python -m zephyr_b200.kernels.timing stream_parts --tokens 2048 --hidden 2048 --ffn 6144
+    python -m zephyr_b200.kernels.timing packed_cache --batch 8 --context 4096 --tokens 1024 --heads 32
 
 Each case rotates over several copies of its large operands, together larger than the L2 cache, so
 that a kernel bound by memory is timed against memory and not against L2.  Time is taken with CUDA
@@ -1025,6 +1026,58 @@ def plus_one_parts(args) -> dict:
 CASES.update({"retention": retention, "plus_one_parts": plus_one_parts})
 CASES.update({"mixed_scores": mixed_scores, "distance_bias": distance_bias, "prenorm_parts": prenorm_parts})
 CASES.update({"delta_rule": delta_rule, "windowed_attention": windowed_attention, "window_parts": window_parts})
+
+
+# ---- a cache in 4 bits (csrc/packed_cache.cu, csrc/attention_packed.cu and the prompt kernels' forms) ----
+def packed_cache(args) -> dict:
+    """A cache in 4 bits, each call beside its like over bfloat16 pages: ``--batch`` single tokens at ``--context``, the last
+    ``--tokens`` tokens of one row of that context, and the writing of those tokens; and reading their pages back."""
+    device, bf = torch.device("cuda"), torch.bfloat16
+    nh, nkv, hd, B, ctx, page = args.heads, args.kv_heads, args.head_dim, args.batch, args.context, args.page_size
+    T = min(args.tokens, ctx)
+    plain, table = _paged_inputs(B, ctx, nkv, hd, page, device)
+    packed = [torch.zeros(ops.packed_cache_shape(c.shape[0], nkv, page, hd), dtype=torch.uint8, device=device) for c in plain]
+    status, scale, chunk = ops.new_status(device), 1 / math.sqrt(hd), args.chunk
+    masks = dict(chunk=chunk, sinks=torch.zeros(nh, device=device) if chunk else None, softcap=args.softcap)
+    i32 = lambda values: torch.tensor(values, dtype=torch.int32, device=device)
+    one = torch.ones(hd, device=device)
+    for cache in packed:                # every row's keys and values
+        for row in range(B):
+            ops.qk_norm_rope_packed(torch.randn((ctx, (1 + 2 * nkv) * hd), device=device, dtype=bf), 1, nkv, hd, one, one, 1e-6, None, None,
+                                    torch.arange(ctx, dtype=torch.int32, device=device), torch.full((ctx,), row, dtype=torch.int32, device=device),
+                                    cache, table, status)
+    seen = lambda context: min(context, args.window or context, (context - 1) % chunk + 1 if chunk else context)
+    q, rows, row_ctx = torch.randn((B, nh * hd), device=device, dtype=bf), i32(list(range(B))), i32([ctx - 1] * B)
+    out = torch.empty_like(q)
+    decode = (table, rows, rows, row_ctx, ctx, nh, nkv, hd, args.window, scale, status, out)
+    us = {"decode": _time(lambda i: ops.paged_decode_packed(q, packed[i % len(packed)], *decode, **masks), args.warmup, args.iters),
+          "decode_bfloat16": _time(lambda i: ops.paged_decode(q, plain[i % len(plain)], *decode, **masks), args.warmup, args.iters)}
+    tile = ops.paged_prefill_tile_tokens()
+    starts = list(range(0, T, tile))
+    new = torch.randn((T, nh * hd), device=device, dtype=bf)
+    done = torch.empty_like(new)
+    prompt = (table[:1], i32([0] * len(starts)), i32(starts), i32([0]), i32([T]), i32([ctx - T]), nh, nkv, hd, args.window, scale, status, done)
+    us["prompt"] = _time(lambda i: ops.paged_prefill_packed(new, packed[i % len(packed)], *prompt, **masks), args.warmup, args.iters)
+    us["prompt_bfloat16"] = _time(lambda i: ops.paged_prefill(new, plain[i % len(plain)], *prompt, **masks), args.warmup, args.iters)
+    width = (nh + 2 * nkv) * hd
+    qkv = [torch.randn((T, width), device=device, dtype=bf) for _ in range(_copies(T * width * 2))]
+    angles = torch.rand((ctx, hd // 2), device=device)
+    write = (nh, nkv, hd, one, one, 1e-6, angles.cos(), angles.sin(), torch.arange(ctx - T, ctx, dtype=torch.int32, device=device),
+             torch.zeros(T, dtype=torch.int32, device=device))
+    us["write"] = _time(lambda i: ops.qk_norm_rope_packed(qkv[i % len(qkv)], *write, packed[i % len(packed)], table, status), args.warmup, args.iters)
+    us["write_bfloat16"] = _time(lambda i: ops.qk_norm_rope_cache(qkv[i % len(qkv)], *write, plain[i % len(plain)], table, status), args.warmup, args.iters)
+    pages = table[0, (ctx - T) // page:].contiguous()
+    us["read_back"] = _time(lambda i: ops.unpack_pages(packed[i % len(packed)], pages, bf, status), args.warmup, args.iters)
+    ops.check_status(status, "packed_cache")
+    read = B * seen(ctx) * nkv * hd * 5 // 4
+    flops = 4 * hd * nh * sum(seen(c) for c in range(ctx - T + 1, ctx + 1))
+    return {"kernel": "packed_cache", "batch": B, "context": ctx, "tokens": T, "heads": nh, "kv_heads": nkv, "head_dim": hd, "page_size": page,
+            "window": args.window, "chunk": chunk, "softcap": args.softcap, "us": {name: round(t, 2) for name, t in us.items()},
+            "decode_gbs": round(read / us["decode"] / 1e3, 1), "prompt_tflops": round(flops / us["prompt"] / 1e6, 1),
+            "write_gbs": round(T * (2 * width + 2 * nh * hd + nkv * hd * 5 / 4) / us["write"] / 1e3, 1)}
+
+
+CASES.update({"packed_cache": packed_cache})
 
 
 def main(argv=None) -> int:
