@@ -52,46 +52,59 @@ __device__ __forceinline__ void store_four(__nv_bfloat16* p, const float (&x)[4]
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
 }
 
-// Codes of a lane's four values, nibble i for value i, and its group's step and offset (eight lanes); all lanes call.
-__device__ __forceinline__ unsigned pk_quantise(const float (&x)[4], __nv_bfloat16& step, __nv_bfloat16& offset) {
-  float low = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  // (A product of a value that is not finite with zero is a NaN.)
-  const float zero = fmaf(x[0], 0.0f, fmaf(x[1], 0.0f, fmaf(x[2], 0.0f, x[3] * 0.0f)));
+// Codes of a lane's four values, nibble i for value i, and its group's step and offset (eight lanes), U times; all lanes call.
+template <int U>
+__device__ __forceinline__ void pk_quantise(const float (&x)[U][4], unsigned (&codes)[U], __nv_bfloat16 (&step)[U], __nv_bfloat16 (&offset)[U]) {
+  float low[U], high[U];
+  unsigned any_bad[U];
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  for (int u = 0; u < U; ++u) {
+    low[u] = fminf(fminf(x[u][0], x[u][1]), fminf(x[u][2], x[u][3]));
+    high[u] = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
+    // (A product of a value that is not finite with zero is a NaN.)
+    const float zero = fmaf(x[u][0], 0.0f, fmaf(x[u][1], 0.0f, fmaf(x[u][2], 0.0f, x[u][3] * 0.0f)));
+    any_bad[u] = __ballot_sync(0xffffffffu, !(zero == 0.0f)) >> (threadIdx.x & 24) & 0xffu;
   }
-  const unsigned any_bad = __ballot_sync(0xffffffffu, !(zero == 0.0f)) >> (threadIdx.x & 24) & 0xffu;
-  offset = __float2bfloat16_rd(low);
-  const float base = __bfloat162float(offset);
-  step = __float2bfloat16_ru(__fdiv_rn(high - base, 15.0f));
-  const float width = __bfloat162float(step);
-  unsigned codes = 0;
-  if (any_bad || !(width <= 3.0e38f)) {
-    offset = __ushort_as_bfloat16(0x7fc0);
-    step = __ushort_as_bfloat16(0);
-  } else if (width >= 1.0e-30f) {
-    // The quotient from a reciprocal is off by some 2^-22: the whole number next to it is right, or off by one where the quotient is
-    // half way between two.  What is left over (exact in float32: a code of 4 bits times a step of 8) says so: it may be half a step,
-    // or with an odd code less than that, so that ties go to the even one.  (No code is below 0 or above 15: the offset is rounded
-    // down, the step up.)
-    constexpr float MAGIC = 12582912.0f;         // 1.5 * 2^23: a sum with it is rounded to whole numbers, ties to even, in its last bits
-    const float inv = __fdiv_rn(1.0f, width), half = 0.5f * width;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float y = x[e] - base, t = fmaf(y, inv, MAGIC), left = fmaf(MAGIC - t, width, y);
-      unsigned code = __float_as_uint(t) & 15u;
-      const float most = __uint_as_float(__float_as_uint(half) - (code & 1u));
-      if (left > most) ++code;
-      if (left < -most) --code;
-      codes |= code << (4 * e);
+  for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      low[u] = fminf(low[u], __shfl_xor_sync(0xffffffffu, low[u], o));
+      high[u] = fmaxf(high[u], __shfl_xor_sync(0xffffffffu, high[u], o));
     }
-  } else if (width > 0.0f) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) codes |= static_cast<unsigned>(rintf(__fdiv_rn(x[e] - base, width))) << (4 * e);
+  for (int u = 0; u < U; ++u) {
+    offset[u] = __float2bfloat16_rd(low[u]);
+    const float base = __bfloat162float(offset[u]);
+    step[u] = __float2bfloat16_ru(__fdiv_rn(high[u] - base, 15.0f));
+    const float width = __bfloat162float(step[u]);
+    codes[u] = 0;
+    if (any_bad[u] || !(width <= 3.0e38f)) {
+      offset[u] = __ushort_as_bfloat16(0x7fc0);
+      step[u] = __ushort_as_bfloat16(0);
+    } else if (width >= 1.0e-30f) {
+      // The quotient from a reciprocal is off by some 2^-22: the whole number next to it is right, or off by one where the quotient is
+      // half way between two.  What is left over (exact in float32: a code of 4 bits times a step of 8) says so: it may be half a step,
+      // or with an odd code less than that, so that ties go to the even one.  (No code is below 0 or above 15: the offset is rounded
+      // down, the step up.)
+      constexpr float MAGIC = 12582912.0f;       // 1.5 * 2^23: a sum with it is rounded to whole numbers, ties to even, in its last bits
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(width));
+      const float half = 0.5f * width;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = x[u][e] - base, t = fmaf(y, inv, MAGIC), left = fmaf(MAGIC - t, width, y);
+        unsigned code = __float_as_uint(t) & 15u;
+        const float most = __uint_as_float(__float_as_uint(half) - (code & 1u));
+        if (left > most) ++code;
+        if (left < -most) --code;
+        codes[u] |= code << (4 * e);
+      }
+    } else if (width > 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) codes[u] |= static_cast<unsigned>(rintf(__fdiv_rn(x[u][e] - base, width))) << (4 * e);
+    }
   }
-  return codes;
 }
 
 __device__ __forceinline__ void load_scales(const void* w, int w_dtype, int d, float (&s)[4]) {
@@ -101,9 +114,11 @@ __device__ __forceinline__ void load_scales(const void* w, int w_dtype, int d, f
 
 // A warp takes every so many'th run of query, key and value heads of one token (a run: as many heads as have lanes in a warp), UNITS of
 // them at a time, whose values are all asked for before the first is used; the token's place, its angles and the scales serve all.
-// (Eight channels a lane take as many instructions and more registers: 2048 tokens of 32 / 8 heads 24 to 30 us.)
+// What bounds it is instructions, some 110 a head (60 % of issue slots), and for few tokens the chain from a token's position to its
+// page and angles; 64 registers, a few of them spilled, so that an SM holds eight CTAs (2048 tokens of 32/8 heads 18.9 us, 2.4 TB/s; six
+// CTAs of 80 registers 23.5; a head's steps one head after the other 21.9; eight channels a lane 24 to 30).
 template <int HD, int UNITS, typename TI, typename TO>
-__global__ void __launch_bounds__(PKW_WARPS * 32)
+__global__ void __launch_bounds__(PKW_WARPS * 32, 8)
 qk_norm_rope_packed_kernel(const PackedWriteArgs a) {
   constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, NG = HD / 32;      // (24 lanes: one head a warp)
   wait_for_prior_grids();
@@ -165,88 +180,136 @@ qk_norm_rope_packed_kernel(const PackedWriteArgs a) {
   const int partner = !mine ? lane : front ? lane + a.half / 4 : lane - a.half / 4;
   const int g = sub & 7, m = sub >> 3;          // the lane's place in its group of channels, and the group
 
-  // The heads of one kind: 0 queries, 1 keys, 2 values.
+  // The heads of one kind: 0 queries, 1 keys, 2 values.  TURN: 0 nothing turns, 1 halves, 2 adjacent pairs.
   // (Runs of all kinds are counted through, so that every warp has as many.)
-  auto work = [&](auto which, int head0, int heads, int passed, const void* norm_w) {
-    constexpr int KIND = decltype(which)::value;
+  const int head_step = stride * HEADS;
+  auto work = [&](auto which, auto how, auto at_once, int head0, int heads, int passed, const void* norm_w) {
+    constexpr int KIND = decltype(which)::value, TURN = decltype(how)::value, U = decltype(at_once)::value;
     const int start = (own - passed % stride + stride) % stride;
     if (start * HEADS >= heads) return;
-    float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-    if (KIND < 2 && normed) load_scales(norm_w, a.norm_w_dtype, d, scale);
-    // A codes' place: of the keys' word that two lanes share, or of the values' half word.
-    unsigned char* const codes_to = KIND == 1 ? to + pk_key_word<HD>(p, g >> 1, m) : to + pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m) + 2 * (p & 1);
-    unsigned char* const steps_to = KIND == 1 ? to + pk_key_step<HD>(p, m) : to + pk_value_step<HD>(p >> 1, m) + 2 * (p & 1);
-    for (int first = start * HEADS; first < heads; first += UNITS * stride * HEADS) {
-      float x[UNITS][4];
+    // What a value and its partner are multiplied by, scale and angle in one.
+    float mul[4] = {1.0f, 1.0f, 1.0f, 1.0f}, partner_mul[4];
+    if (KIND < 2 && normed) load_scales(norm_w, a.norm_w_dtype, d, mul);
+    if (TURN > 0) {
+      float theirs[4];
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int head = first + u * stride * HEADS + among;
-        x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
-        if (head < heads && lane_ok) load_four(from + static_cast<size_t>(head0 + head) * HD, x[u]);
+      for (int e = 0; e < 4; ++e) theirs[e] = TURN == 2 ? mul[e ^ 1] : __shfl_sync(0xffffffffu, mul[e], partner);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        mul[e] *= cs[e];
+        partner_mul[e] = theirs[e] * sn[e];
       }
+    }
+    // A codes' place: of the keys' word that two lanes share, or of the values' half word.
+    const int head_bytes = pk_block_bytes(HD) << (a.page_shift - 4);
+    int left = heads - start * HEADS - among;                // heads from this lane's first on
+    if (!lane_ok) left = 0;
+    unsigned char* codes_to = to + (KIND == 1 ? pk_key_word<HD>(p, g >> 1, m) : pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m) + 2 * (p & 1)) +
+                              static_cast<long long>(start * HEADS + among) * head_bytes;
+    constexpr int VALUES_STEP = KIND == 1 ? 2 : 4;
+    const int steps_at = KIND == 1 ? pk_key_step<HD>(p, m) - pk_key_word<HD>(p, g >> 1, m)
+                                   : pk_value_step<HD>(p >> 1, m) - pk_value_word<HD>(p >> 3, g, (p & 7) >> 1, m);
+    const TI* source = from + (head0 + start * HEADS + among) * HD;
+    const float* bias = a.bias + (head0 + start * HEADS + among) * HD + d;
+    TO* out = static_cast<TO*>(a.q_out) + static_cast<size_t>(t) * a.nh * HD + (start * HEADS + among) * HD + d;
+    for (int rest = heads - start * HEADS; rest > 0; rest -= U * head_step, left -= U * head_step) {      // (rest: the warp's)
+      float x[U][4];
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        if (first + u * stride * HEADS >= heads) break;               // (the same for the warp)
-        const int head = first + u * stride * HEADS + among;
-        const bool active = head < heads && lane_ok;
-        float (&v)[4] = x[u];
-        if (a.bias != nullptr && active) {
+      for (int u = 0; u < U; ++u) {
+        x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+        if (u * head_step < left) load_four(source + u * head_step * HD, x[u]);
+      }
+      source += U * head_step * HD;
+      if (a.bias != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += a.bias[(head0 + head) * HD + d + e];
+        for (int u = 0; u < U; ++u) {
+          if (u * head_step >= left) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][e] += bias[u * head_step * HD + e];
         }
-        if (KIND < 2 && normed) {
-          float ss = fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3])));
+        bias += U * head_step * HD;
+      }
+      if (KIND < 2) {
+        float sum[U];
 #pragma unroll
-          for (int o = 1; o < (HEADS > 1 ? LANES : 32); o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float inv = rsqrtf(ss * (1.0f / static_cast<float>(HD)) + a.eps);
+        for (int u = 0; u < U; ++u) sum[u] = fmaf(x[u][0], x[u][0], fmaf(x[u][1], x[u][1], fmaf(x[u][2], x[u][2], x[u][3] * x[u][3])));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= inv * scale[e];
-        }
-        if (KIND < 2 && turned) {
+        for (int u = 0; u < U; ++u) {
           float y[4];
-          if (a.pairs) {
+          if (TURN > 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = v[e ^ 1];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, v[e], partner);
+            for (int e = 0; e < 4; ++e) y[e] = TURN == 2 ? x[u][e ^ 1] : __shfl_sync(0xffffffffu, x[u][e], partner);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], sn[e], v[e] * cs[e]);      // (times 0 and 1 where nothing turns)
+          for (int e = 0; e < 4; ++e) x[u][e] = TURN > 0 ? fmaf(y[e], partner_mul[e], x[u][e] * mul[e]) : x[u][e] * mul[e];      // (times 0 and 1 where nothing turns)
         }
-        if (KIND == 0) {
-          if (active) store_four(static_cast<TO*>(a.q_out) + (static_cast<size_t>(t) * a.nh + head) * HD + d, v);
-          continue;
-        }
-        __nv_bfloat16 step, offset;
-        unsigned codes = pk_quantise(v, step, offset);
-        if (KIND == 1) codes |= __shfl_xor_sync(0xffffffffu, codes, 1) << 16;
-        if (!active || to == nullptr) continue;
-        const long long at = (static_cast<long long>(head) << (a.page_shift - 4)) * pk_block_bytes(HD);
-        if (KIND == 1 && (g & 1) == 0) *reinterpret_cast<unsigned*>(codes_to + at) = codes;
-        if (KIND == 2) *reinterpret_cast<unsigned short*>(codes_to + at) = static_cast<unsigned short>(codes);
-        if (g == 0) {
-          *reinterpret_cast<__nv_bfloat16*>(steps_to + at) = step;
-          *reinterpret_cast<__nv_bfloat16*>(steps_to + at + (KIND == 1 ? 2 : 4) * NG) = offset;
+        if (normed) {
+#pragma unroll
+          for (int o = 1; o < (HEADS > 1 ? LANES : 32); o <<= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float inv;
+            asm("rsqrt.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(fmaf(sum[u], 1.0f / static_cast<float>(HD), a.eps)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] *= inv;
+          }
         }
       }
+      if (KIND == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u * head_step < left) store_four(out + u * head_step * HD, x[u]);
+        out += U * head_step * HD;
+        continue;
+      }
+      __nv_bfloat16 step[U], offset[U];
+      unsigned codes[U];
+      pk_quantise(x, codes, step, offset);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (KIND == 1) codes[u] |= __shfl_xor_sync(0xffffffffu, codes[u], 1) << 16;
+        if (u * head_step >= left || to == nullptr) continue;
+        unsigned char* const at = codes_to + static_cast<long long>(u * head_step) * head_bytes;
+        if (KIND == 1 && (g & 1) == 0) *reinterpret_cast<unsigned*>(at) = codes[u];
+        if (KIND == 2) *reinterpret_cast<unsigned short*>(at) = static_cast<unsigned short>(codes[u]);
+        if (g == 0) {
+          *reinterpret_cast<__nv_bfloat16*>(at + steps_at) = step[u];
+          *reinterpret_cast<__nv_bfloat16*>(at + steps_at + VALUES_STEP * NG) = offset[u];
+        }
+      }
+      codes_to += static_cast<long long>(U * head_step) * head_bytes;
     }
   };
   const int q_runs = (a.nh + HEADS - 1) / HEADS, k_runs = (a.nkv + HEADS - 1) / HEADS;
-  work(std::integral_constant<int, 0>{}, 0, a.nh, 0, a.q_norm_w);
-  if (a.packed == nullptr) return;
-  work(std::integral_constant<int, 1>{}, a.nh, a.nkv, q_runs, a.k_norm_w);
-  work(std::integral_constant<int, 2>{}, a.nh + a.nkv, a.nkv, q_runs + k_runs, nullptr);
+  constexpr std::integral_constant<int, UNITS> all{};
+  constexpr std::integral_constant<int, UNITS < 2 ? 1 : 2> half{};
+  constexpr std::integral_constant<int, 0> zero{};
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  auto turn = [&](auto how) {
+    work(zero, how, all, 0, a.nh, 0, a.q_norm_w);
+    if (a.packed != nullptr) work(one, how, half, a.nh, a.nkv, q_runs, a.k_norm_w);
+  };
+  if (!turned) turn(zero);
+  else if (a.pairs) turn(two);
+  else turn(one);
+  if (a.packed != nullptr) work(two, zero, half, a.nh + a.nkv, a.nkv, q_runs + k_runs, nullptr);
 }
 
-// Many tokens: SHARED warps a token, four runs of heads at a time.  Few: a run a warp.
+// Many tokens: two warps a token, four where a CTA a token fills the SMs a few times only, four runs of heads at a time (us, two / four
+// warps, 32/8 heads of 128: 65 tokens 7.9 / 5.6, 512 8.9 / 7.3, 1024 10.6 / 10.7, 2048 18.9 / 20.0, 8192 59 / 67; 2048 of 16/8 heads of 64
+// 9.8 / 15.0).  Few: a run a warp (8 tokens 3.3).
 template <int HD, typename TI, typename TO>
 int packed_write_launch(PackedWriteArgs& a, cudaStream_t stream) {
-  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1, SHARED = 2;
+  constexpr int LANES = HD / 4, HEADS = LANES <= 16 ? 32 / LANES : 1;
   const dim3 threads(PKW_WARPS * 32);
   if (a.tokens > 64) {
-    a.shared = SHARED;
-    const int tokens = PKW_WARPS / SHARED;
+    int device = 0, sms = 0;
+    if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
+    a.shared = a.tokens <= 4 * sms ? 4 : 2;
+    const int tokens = PKW_WARPS / a.shared;
     return launch_dependent(qk_norm_rope_packed_kernel<HD, 4, TI, TO>, dim3((a.tokens + tokens - 1) / tokens), threads, 0, stream, false, a);
   }
   const int runs = (a.nh + HEADS - 1) / HEADS + (a.packed != nullptr ? 2 * ((a.nkv + HEADS - 1) / HEADS) : 0), across = (runs + PKW_WARPS - 1) / PKW_WARPS;
