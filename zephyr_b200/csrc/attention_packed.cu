@@ -832,42 +832,53 @@ ZB_API long long zb_paged_decode_packed_scratch_floats(int ctas, int by_warp, in
   return 2LL * ctas * (by_warp ? PD_WARPS : 1) * PD_HEADS * (hd + 2) + 4LL * pairs;
 }
 
+// What zb_paged_decode_packed is given: eight bytes a field, in this order.
+struct PackedDecodeCall {
+  void* out; const void* q; const void* packed; const int* block_table; long long max_blocks, page_size, num_pages, num_rows;
+  const int* rows; long long n_rows; const int* row_q_start; const int* row_ctx;
+  long long max_context, tokens, nh, nkv, hd, window, chunk; double scale, softcap; const float* sinks; long long mode, ctas;
+  float* scratch; int* status; void* stream;
+};
+
 // Attention of one new token a row over its context in the 4-bit cache.  `mode` 0: a cluster of `ctas` CTAs (1, 2, 4 or 8) a (row,
 // key/value head) pair; 1 and 2: `ctas` CTAs, each or each of whose warps has an equal share of all pairs' tiles, and a second kernel,
 // with `scratch` (zb_paged_decode_packed_scratch_floats, 16-byte aligned, any contents).
-ZB_API int zb_paged_decode_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
-                                  int num_pages, int num_rows, const int* rows, int n_rows, const int* row_q_start, const int* row_ctx,
-                                  long long max_context, long long tokens, int nh, int nkv, int hd, int window, int chunk, float scale, float softcap,
-                                  const float* sinks, int mode, int ctas, float* scratch, int* status, void* stream) {
+ZB_API int zb_paged_decode_packed(const void* call) {
+  const PackedDecodeCall& c = *static_cast<const PackedDecodeCall*>(call);
+  const int max_blocks = static_cast<int>(c.max_blocks), page_size = static_cast<int>(c.page_size);
+  const int num_pages = static_cast<int>(c.num_pages), num_rows = static_cast<int>(c.num_rows), n_rows = static_cast<int>(c.n_rows);
+  const int nh = static_cast<int>(c.nh), nkv = static_cast<int>(c.nkv), hd = static_cast<int>(c.hd), window = static_cast<int>(c.window);
+  const int chunk = static_cast<int>(c.chunk), mode = static_cast<int>(c.mode), ctas = static_cast<int>(c.ctas);
+  const float scale = static_cast<float>(c.scale), softcap = static_cast<float>(c.softcap);
   const int page_shift = pk_page_shift(page_size);
-  if (n_rows < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || max_context < 0 ||
+  if (n_rows < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || c.max_context < 0 ||
       mode < PD_CLUSTERS || mode > PD_WARP_SHARES || ctas <= 0 || (mode == PD_CLUSTERS && ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) ||
-      (mode != PD_CLUSTERS && scratch == nullptr))
+      (mode != PD_CLUSTERS && c.scratch == nullptr))
     return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
   if (n_rows == 0) return OK;
   const int subs = (nh / nkv + PD_HEADS - 1) / PD_HEADS;
   const long long pairs = static_cast<long long>(n_rows) * nkv * subs;
   // (Blocks and tiles are counted in 32 bits.)
-  if (static_cast<long long>(num_pages) * nkv * (page_size / PK_BLOCK) >= (1LL << 31) || pairs * 8 >= (1LL << 31) || pairs * (max_context / PD_TILE + 16) >= (1LL << 30)) return ERR_UNSUPPORTED;
+  if (static_cast<long long>(num_pages) * nkv * (page_size / PK_BLOCK) >= (1LL << 31) || pairs * 8 >= (1LL << 31) || pairs * (c.max_context / PD_TILE + 16) >= (1LL << 30)) return ERR_UNSUPPORTED;
   PackedDecodeArgs a = {};
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.packed = static_cast<const unsigned char*>(packed);
-  a.block_table = block_table; a.rows = rows; a.row_q_start = row_q_start; a.row_ctx = row_ctx;
+  a.q = static_cast<const __nv_bfloat16*>(c.q);
+  a.out = static_cast<__nv_bfloat16*>(c.out);
+  a.packed = static_cast<const unsigned char*>(c.packed);
+  a.block_table = c.block_table; a.rows = c.rows; a.row_q_start = c.row_q_start; a.row_ctx = c.row_ctx;
   if (mode != PD_CLUSTERS) {
-    a.cuts = reinterpret_cast<int4*>(scratch);
-    a.part_o = scratch + 4 * pairs;
+    a.cuts = reinterpret_cast<int4*>(c.scratch);
+    a.part_o = c.scratch + 4 * pairs;
     a.part_ml = a.part_o + 2LL * ctas * (mode == PD_WARP_SHARES ? PD_WARPS : 1) * PD_HEADS * hd;
   }
-  a.q_values = tokens * nh * hd;
+  a.q_values = c.tokens * nh * hd;
   a.max_blocks = max_blocks; a.page_shift = page_shift; a.num_pages = num_pages; a.num_rows = num_rows; a.n_rows = n_rows;
-  a.nh = nh; a.nkv = nkv; a.subs = subs; a.window = window; a.chunk = chunk; a.sinks = sinks;
+  a.nh = nh; a.nkv = nkv; a.subs = subs; a.window = window; a.chunk = chunk; a.sinks = c.sinks;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.softcap_log2 = softcap * 1.4426950408889634f;
   a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
-  a.status = status;
-  const auto s = static_cast<cudaStream_t>(stream);
+  a.status = c.status;
+  const auto s = static_cast<cudaStream_t>(c.stream);
   switch (hd) {
     case 32: return packed_decode_run<32>(a, mode, ctas, s);
     case 64: return packed_decode_run<64>(a, mode, ctas, s);

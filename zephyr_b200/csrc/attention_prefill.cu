@@ -658,28 +658,31 @@ ZB_API int zb_paged_prefill(void* out, const void* q, const void* kv_cache, cons
 }
 
 // The same over a 4-bit cache (packed.cuh), pages of a power of two of positions from 16 on; head sizes 32, 64, 96 and 128.
-ZB_API int zb_paged_prefill_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
-                                   int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles,
-                                   const int* row_q_start, const int* row_q_len, const int* row_ctx, int nh, int nkv, int hd, int window,
-                                   int chunk, float scale, float softcap, const float* sinks, int* status, void* stream) {
+ZB_API int zb_paged_prefill_packed(const void* call) {
+  const PackedPromptCall& c = *static_cast<const PackedPromptCall*>(call);
+  const int max_blocks = static_cast<int>(c.max_blocks), page_size = static_cast<int>(c.page_size);
+  const int num_pages = static_cast<int>(c.num_pages), num_rows = static_cast<int>(c.num_rows), n_tiles = static_cast<int>(c.n_tiles);
+  const int nh = static_cast<int>(c.nh), nkv = static_cast<int>(c.nkv), hd = static_cast<int>(c.hd), window = static_cast<int>(c.window);
+  const int chunk = static_cast<int>(c.chunk);
+  const float scale = static_cast<float>(c.scale), softcap = static_cast<float>(c.softcap);
   const int page_shift = pk_page_shift(page_size);
   if (n_tiles < 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || nh <= 0 || nkv <= 0 || nh % nkv != 0) return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd) || nh > 65535 || n_tiles > 65535) return ERR_UNSUPPORTED;
   if (n_tiles == 0) return OK;
   PrefillArgs a = {};
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.kv_cache = static_cast<const __nv_bfloat16*>(packed);
-  a.block_table = block_table; a.tile_row = tile_row; a.tile_q0 = tile_q0;
-  a.row_q_start = row_q_start; a.row_q_len = row_q_len; a.row_ctx = row_ctx;
+  a.q = static_cast<const __nv_bfloat16*>(c.q);
+  a.out = static_cast<__nv_bfloat16*>(c.out);
+  a.kv_cache = static_cast<const __nv_bfloat16*>(c.packed);
+  a.block_table = c.block_table; a.tile_row = c.tile_row; a.tile_q0 = c.tile_q0;
+  a.row_q_start = c.row_q_start; a.row_q_len = c.row_q_len; a.row_ctx = c.row_ctx;
   a.max_blocks = max_blocks; a.page_size = page_size; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
-  a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk; a.sinks = sinks;
+  a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk; a.sinks = c.sinks;
   a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
   a.softcap_log2 = softcap * 1.4426950408889634f;
   a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
-  a.status = status;
-  const auto s = static_cast<cudaStream_t>(stream);
+  a.status = c.status;
+  const auto s = static_cast<cudaStream_t>(c.stream);
   switch (hd) {
     case 32: return prefill_packed_launch<32>(a, n_tiles, s);
     case 64: return prefill_packed_launch<64>(a, n_tiles, s);

@@ -1049,13 +1049,17 @@ ZB_API int zb_paged_prefill_tc(void* out, const void* q, const void* kv_cache, c
 }
 
 // The same over a 4-bit cache (packed.cuh): head size 128, pages of a power of two of positions from 16 on.
-ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* packed, const int* block_table, int max_blocks, int page_size,
-                                      int num_pages, int num_rows, const int* tile_row, const int* tile_q0, int n_tiles,
-                                      const int* row_q_start, const int* row_q_len, const int* row_ctx, int nh, int nkv, int window,
-                                      int chunk, float scale, float softcap, const float* sinks, int* status, void* stream) {
+ZB_API int zb_paged_prefill_tc_packed(const void* call) {
+  const PackedPromptCall& c = *static_cast<const PackedPromptCall*>(call);
+  const int max_blocks = static_cast<int>(c.max_blocks), page_size = static_cast<int>(c.page_size);
+  const int num_pages = static_cast<int>(c.num_pages), num_rows = static_cast<int>(c.num_rows), n_tiles = static_cast<int>(c.n_tiles);
+  const int nh = static_cast<int>(c.nh), nkv = static_cast<int>(c.nkv), window = static_cast<int>(c.window);
+  const int chunk = static_cast<int>(c.chunk);
+  const float scale = static_cast<float>(c.scale), softcap = static_cast<float>(c.softcap);
   const int page_shift = pk_page_shift(page_size);
+  if (c.hd != 128) return ERR_UNSUPPORTED;
   if (n_tiles < 0 || page_shift < 0 || window < 0 || chunk < 0 || softcap < 0.0f || nh <= 0 || nkv <= 0 || nh % nkv != 0) return ERR_BAD_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(packed) % 16 != 0)
+  if (reinterpret_cast<uintptr_t>(c.q) % 16 != 0 || reinterpret_cast<uintptr_t>(c.out) % 16 != 0 || reinterpret_cast<uintptr_t>(c.packed) % 16 != 0)
     return ERR_BAD_ARGUMENT;
   if (n_tiles == 0) return OK;
   if (n_tiles > 65535 || nh > 65535 || (static_cast<long long>(num_pages) * nkv << (page_shift - 4)) >= (1LL << 31)) return ERR_UNSUPPORTED;
@@ -1064,19 +1068,19 @@ ZB_API int zb_paged_prefill_tc_packed(void* out, const void* q, const void* pack
   PrefillTcArgs a = {};
   a.n_tiles = n_tiles;
   a.n_split = tc_packed_split_tiles(nh, nkv, n_tiles, sms);
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.kv_cache = static_cast<const __nv_bfloat16*>(packed);
-  a.block_table = block_table; a.tile_row = tile_row; a.tile_q0 = tile_q0;
-  a.row_q_start = row_q_start; a.row_q_len = row_q_len; a.row_ctx = row_ctx;
+  a.q = static_cast<const __nv_bfloat16*>(c.q);
+  a.out = static_cast<__nv_bfloat16*>(c.out);
+  a.kv_cache = static_cast<const __nv_bfloat16*>(c.packed);
+  a.block_table = c.block_table; a.tile_row = c.tile_row; a.tile_q0 = c.tile_q0;
+  a.row_q_start = c.row_q_start; a.row_q_len = c.row_q_len; a.row_ctx = c.row_ctx;
   a.max_blocks = max_blocks; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
   a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk;
   a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
   a.softcap_log2 = softcap * 1.4426950408889634f;
   a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
-  a.sinks = sinks;
-  a.status = status;
-  const auto s = static_cast<cudaStream_t>(stream);
+  a.sinks = c.sinks;
+  a.status = c.status;
+  const auto s = static_cast<cudaStream_t>(c.stream);
   return chunk > 0 ? prefill_tc_packed_launch<TC_FORM_CHUNKED>(a, s) : prefill_tc_packed_launch<TC_FORM_PLAIN>(a, s);
 }

@@ -151,4 +151,11 @@ __device__ __forceinline__ void pk_value_channels(unsigned low, unsigned high, u
   even = make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(e, f, 0x5410), __byte_perm(g, h, 0x5410));
   odd = make_uint4(__byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632), __byte_perm(e, f, 0x7632), __byte_perm(g, h, 0x7632));
 }
+// What zb_paged_prefill_packed and zb_paged_prefill_tc_packed are given: eight bytes a field, in this order.
+struct PackedPromptCall {
+  void* out; const void* q; const void* packed; const int* block_table; long long max_blocks, page_size, num_pages, num_rows;
+  const int* tile_row; const int* tile_q0; long long n_tiles; const int* row_q_start; const int* row_q_len; const int* row_ctx;
+  long long nh, nkv, hd, window, chunk; double scale, softcap; const float* sinks; int* status; void* stream;
+};
+
 }  // namespace zb

@@ -389,22 +389,34 @@ using namespace zb;
 // Bytes of a block of 16 positions of one head; 0 for a head size that the packed cache does not take.
 ZB_API int zb_packed_block_bytes(int hd) { return pk_head_dim_ok(hd) ? pk_block_bytes(hd) : 0; }
 
+// What zb_qk_norm_rope_packed is given: eight bytes a field, in this order.
+struct PackedWriteCall {
+  void* q_out; const void* qkv; long long qkv_stride; const float* bias; const void* q_norm_w; const void* k_norm_w;
+  long long norm_w_dtype; double eps; const float* cos_table; const float* sin_table; long long half, max_positions, pairs;
+  const int* positions; const int* token_row; void* packed; const int* block_table;
+  long long max_blocks, page_size, num_pages, num_rows, tokens, nh, nkv, hd, in_dtype, out_dtype; int* status; void* stream;
+};
+
 // `packed` null: the queries alone (qkv then holds nh heads).  `pairs`: adjacent channels are partners, else halves of the rotated part.
-ZB_API int zb_qk_norm_rope_packed(void* q_out, const void* qkv, long long qkv_stride, const float* bias, const void* q_norm_w,
-                                  const void* k_norm_w, int norm_w_dtype, float eps, const float* cos_table, const float* sin_table, int half,
-                                  int max_positions, int pairs, const int* positions, const int* token_row, void* packed,
-                                  const int* block_table, int max_blocks, int page_size, int num_pages, int num_rows, int tokens, int nh,
-                                  int nkv, int hd, int in_dtype, int out_dtype, int* status, void* stream) {
-  const int page_shift = packed != nullptr ? pk_page_shift(page_size) : 4;
-  if (tokens < 0 || nh <= 0 || nkv <= 0 || page_shift < 0 || half < 0 || 2 * half > hd || (cos_table != nullptr && half == 0) ||
-      (!pairs && half % 4 != 0) || qkv_stride % 4 != 0)
+ZB_API int zb_qk_norm_rope_packed(const void* call) {
+  const PackedWriteCall& c = *static_cast<const PackedWriteCall*>(call);
+  const int norm_w_dtype = static_cast<int>(c.norm_w_dtype), half = static_cast<int>(c.half);
+  const int max_positions = static_cast<int>(c.max_positions), pairs = static_cast<int>(c.pairs);
+  const int max_blocks = static_cast<int>(c.max_blocks), page_size = static_cast<int>(c.page_size);
+  const int num_pages = static_cast<int>(c.num_pages), num_rows = static_cast<int>(c.num_rows), tokens = static_cast<int>(c.tokens);
+  const int nh = static_cast<int>(c.nh), nkv = static_cast<int>(c.nkv), hd = static_cast<int>(c.hd);
+  const int in_dtype = static_cast<int>(c.in_dtype), out_dtype = static_cast<int>(c.out_dtype);
+  const float eps = static_cast<float>(c.eps);
+  const int page_shift = c.packed != nullptr ? pk_page_shift(page_size) : 4;
+  if (tokens < 0 || nh <= 0 || nkv <= 0 || page_shift < 0 || half < 0 || 2 * half > hd || (c.cos_table != nullptr && half == 0) ||
+      (!pairs && half % 4 != 0) || c.qkv_stride % 4 != 0)
     return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
   if (tokens == 0) return OK;
-  PackedWriteArgs a = {q_out, qkv, qkv_stride, bias, q_norm_w, k_norm_w, norm_w_dtype, eps, cos_table, sin_table, half, max_positions,
-                             pairs, positions, token_row, static_cast<unsigned char*>(packed), block_table, max_blocks, page_shift, num_pages,
-                             num_rows, tokens, nh, nkv, PKW_WARPS, status};
-  const auto s = static_cast<cudaStream_t>(stream);
+  PackedWriteArgs a = {c.q_out, c.qkv, c.qkv_stride, c.bias, c.q_norm_w, c.k_norm_w, norm_w_dtype, eps, c.cos_table, c.sin_table, half, max_positions,
+                             pairs, c.positions, c.token_row, static_cast<unsigned char*>(c.packed), c.block_table, max_blocks, page_shift, num_pages,
+                             num_rows, tokens, nh, nkv, PKW_WARPS, c.status};
+  const auto s = static_cast<cudaStream_t>(c.stream);
   switch (hd) {
     case 32: return packed_write_types<32>(a, in_dtype, out_dtype, s);
     case 64: return packed_write_types<64>(a, in_dtype, out_dtype, s);
@@ -413,18 +425,25 @@ ZB_API int zb_qk_norm_rope_packed(void* q_out, const void* qkv, long long qkv_st
   }
 }
 
-ZB_API int zb_unpack_pages(void* out, const void* packed, const int* pages, int n_pages, int num_pages, int nkv, int page_size, int hd,
-                           int dtype, int* status, void* stream) {
+// What zb_unpack_pages is given: eight bytes a field, in this order.
+struct UnpackCall {
+  void* out; const void* packed; const int* pages; long long n_pages, num_pages, nkv, page_size, hd, dtype; int* status; void* stream;
+};
+
+ZB_API int zb_unpack_pages(const void* call) {
+  const UnpackCall& c = *static_cast<const UnpackCall*>(call);
+  const int n_pages = static_cast<int>(c.n_pages), num_pages = static_cast<int>(c.num_pages), nkv = static_cast<int>(c.nkv);
+  const int page_size = static_cast<int>(c.page_size), hd = static_cast<int>(c.hd), dtype = static_cast<int>(c.dtype);
   const int page_shift = pk_page_shift(page_size);
   if (n_pages < 0 || nkv <= 0 || page_shift < 0) return ERR_BAD_ARGUMENT;
   if (!pk_head_dim_ok(hd)) return ERR_UNSUPPORTED;
   if (n_pages == 0) return OK;
-  const auto* from = static_cast<const unsigned char*>(packed);
-  const auto s = static_cast<cudaStream_t>(stream);
+  const auto* from = static_cast<const unsigned char*>(c.packed);
+  const auto s = static_cast<cudaStream_t>(c.stream);
   switch (hd) {
-    case 32: return unpack_launch<32>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
-    case 64: return unpack_launch<64>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
-    case 96: return unpack_launch<96>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
-    default: return unpack_launch<128>(out, from, pages, n_pages, num_pages, nkv, page_shift, dtype, status, s);
+    case 32: return unpack_launch<32>(c.out, from, c.pages, n_pages, num_pages, nkv, page_shift, dtype, c.status, s);
+    case 64: return unpack_launch<64>(c.out, from, c.pages, n_pages, num_pages, nkv, page_shift, dtype, c.status, s);
+    case 96: return unpack_launch<96>(c.out, from, c.pages, n_pages, num_pages, nkv, page_shift, dtype, c.status, s);
+    default: return unpack_launch<128>(c.out, from, c.pages, n_pages, num_pages, nkv, page_shift, dtype, c.status, s);
   }
 }

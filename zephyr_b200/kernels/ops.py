@@ -15,7 +15,7 @@ import math
 import os
 import struct
 import threading
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -116,18 +116,8 @@ _SIGNATURES = {
                       c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                       c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_packed_block_bytes": [c_int],
-    "zb_qk_norm_rope_packed": [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p, c_int,
-                               c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                               c_int, c_int, c_int, c_void_p, c_void_p],
-    "zb_unpack_pages": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
-    "zb_paged_decode_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                               c_longlong, c_longlong, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_int, c_int, c_void_p,
-                               c_void_p, c_void_p],
-    "zb_paged_prefill_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
-                                c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p],
-    "zb_paged_prefill_tc_packed": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
-                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p,
-                                   c_void_p],
+    "zb_qk_norm_rope_packed": [c_char_p], "zb_unpack_pages": [c_char_p], "zb_paged_decode_packed": [c_char_p],
+    "zb_paged_prefill_packed": [c_char_p], "zb_paged_prefill_tc_packed": [c_char_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
                        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "zb_head_mix": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
@@ -1364,7 +1354,7 @@ def packed_cache_shape(pages: int, nkv: int, page_size: int, hd: int) -> tuple[i
 
 
 # The calls below are made for every layer of a step: a tensor's type, order, place and address are asked for once each, and a message
-# is made only where a check fails (writing and reading back, two calls: 28.7 -> 25.9 us on the host).
+# is made only where a check fails (writing and reading back, two calls: 28.7 -> 25.9 us on the host, 22 with their values in one structure).
 def _check_packed(packed: torch.Tensor, nkv: int, hd: int) -> tuple[int, int]:
     if hd not in PACKED_HEAD_DIMS:
         packed_block_bytes(hd)
@@ -1384,13 +1374,13 @@ def _check_index(*tensors: torch.Tensor) -> None:
 
 
 def _addresses(*tensors: torch.Tensor | None) -> tuple[list, int]:
-    """The tensors' addresses (None for None), and the place of the first that lies elsewhere than kernels are launched, on the current
+    """The tensors' addresses (0 for None), and the place of the first that lies elsewhere than kernels are launched, on the current
     device's current stream (-1: a tensor on the CPU; that device itself where there is none)."""
     current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
     place, at = current, []
     for t in tensors:
         if t is None:
-            at.append(None)
+            at.append(0)
             continue
         if place == current:
             place = t.get_device()
@@ -1398,6 +1388,14 @@ def _addresses(*tensors: torch.Tensor | None) -> tuple[list, int]:
     if place != current:
         return at, place
     return at, -3
+
+
+# What these entry points are given, eight bytes a value (the structures beside them in csrc): ctypes takes 0.1 us for an argument of its
+# own (a single token's attention 12.4 -> 10.1 us).
+_PACKED_WRITE = struct.Struct("=2Qq3Qqd2Q3q4Q10q2Q").pack
+_PACKED_READ = struct.Struct("=3Q6q2Q").pack
+_PACKED_DECODE = struct.Struct("=4Q4qQq2Q7q2dQ2q3Q").pack
+_PACKED_PROMPT = struct.Struct("=4Q4q2Qq3Q5q2d3Q").pack
 
 
 def _check_place(place: int) -> None:
@@ -1468,13 +1466,13 @@ def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w:
     if half and (2 * half > hd or (layout == "halves" and (half % 4 != 0 or cos_at % 16 != 0 or sin_at % 16 != 0))) or (cos is not None and not half):
         raise InvalidArgumentError("the rotated channels are part of the head, in halves a multiple of 8 of them with cos/sin on "
                                    "16-byte boundaries")
-    if out_at % 16 != 0 or (packed_at or 0) % 16 != 0:
+    if out_at % 16 != 0 or packed_at % 16 != 0:
         raise InvalidArgumentError("q_out and a 4-bit cache start on 16-byte boundaries")
     _check_place(place)
-    _check(library().zb_qk_norm_rope_packed(
+    _check(library().zb_qk_norm_rope_packed(_PACKED_WRITE(
         out_at, qkv_at, stride, bias_at, qw_at, kw_at, w_code, eps, cos_at, sin_at, half, max_positions, layout == "pairs", positions_at,
         rows_at, packed_at, table_at, table_shape[1], page_size, pages, table_shape[0], T, nh, nkv, hd, DTYPE_CODE[in_dtype],
-        DTYPE_CODE[dtype], status_at, _stream()), "qk_norm_rope_packed")
+        DTYPE_CODE[dtype], status_at, _stream())), "qk_norm_rope_packed")
     return q_out
 
 
@@ -1498,9 +1496,9 @@ def unpack_pages(packed: torch.Tensor, pages: torch.Tensor, dtype: torch.dtype, 
         raise InvalidArgumentError("a 4-bit cache must start on a 16-byte boundary")
     _check_place(place)
     out = packed.new_empty((n, 2, nkv, page_size, hd), dtype=dtype)
-    _check(library().zb_unpack_pages(
+    _check(library().zb_unpack_pages(_PACKED_READ(
         out.data_ptr(), packed_at, pages_at, n, num_pages, nkv, page_size, hd, DTYPE_CODE[dtype],
-        status_at if status is not None else _device_status_pointer(packed.device), _stream()), "unpack_pages")
+        status_at if status is not None else _device_status_pointer(packed.device) or 0, _stream())), "unpack_pages")
     return out
 
 
@@ -1582,9 +1580,10 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
         pairs = n_rows * nkv * -(-nh // nkv // 8)
         scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(ctas, int(mode == PACKED_WARP_SHARES), pairs, hd)),
                               dtype=torch.float32, device=q.device)
-    _check(library().zb_paged_decode_packed(
+    _check(library().zb_paged_decode_packed(_PACKED_DECODE(
         out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, rows_at, n_rows, start_at, ctx_at, max_context, tokens, nh,
-        nkv, hd, window, chunk, scale, softcap, sinks_at, mode, ctas, _ptr(scratch), status_at, _stream()), "paged_decode_packed",
+        nkv, hd, window, chunk, scale, softcap, sinks_at, mode, ctas, 0 if scratch is None else scratch.data_ptr(),
+        status_at, _stream())), "paged_decode_packed",
         1 if mode == PACKED_CLUSTERS else 2)
     return out
 
@@ -1607,13 +1606,12 @@ def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: tor
     (q_at, packed_at, table_at, tile_row_at, tile_q0_at, start_at, len_at, ctx_at, status_at, out_at, sinks_at), place = _addresses(
         q, packed, block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status, out, sinks)
     _check_boundaries(place, q_at, packed_at, out_at)
-    lists = (out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, tile_row_at, tile_q0_at, tiles)
-    rows = (start_at, len_at, ctx_at, nh, nkv)
-    masks = (window, chunk, scale, softcap, sinks_at, status_at, _stream())
+    call = _PACKED_PROMPT(out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, tile_row_at, tile_q0_at, tiles, start_at,
+                          len_at, ctx_at, nh, nkv, hd, window, chunk, scale, softcap, sinks_at, status_at, _stream())
     if hd == 128 and tensor_memory and USE_TCGEN05_PREFILL and not short_prompts(block_table, page_size, nh, tiles):
-        _check(library().zb_paged_prefill_tc_packed(*lists, *rows, *masks), "paged_prefill_tc_packed")
+        _check(library().zb_paged_prefill_tc_packed(call), "paged_prefill_tc_packed")
     else:
-        _check(library().zb_paged_prefill_packed(*lists, *rows, hd, *masks), "paged_prefill_packed")
+        _check(library().zb_paged_prefill_packed(call), "paged_prefill_packed")
     return out
 
 
