@@ -80,11 +80,13 @@ def attention(q, keys, vals, pos, scale, window=0, chunk=0, sinks=None, softcap=
 
     The bound, with u = 2^-8 the most that a rounding to bfloat16 moves a value: the result is rounded, u |o|.  The single tokens'
     kernel rounds a group's weights step p for codes that count from 8, and weights p for offset + 8 step: u sum p (|code - 8| step +
-    |offset + 8 step|).  A prompts' kernel (``rounded``) rounds p and the values: 2 u sum p |v|.  A score that is off by d moves
+    |offset + 8 step|).  A prompts' kernel (``rounded``) rounds p and the values: 2 u sum p |v| (or less:
+    half precision's u is an eighth).  A score that is off by d moves
     every weight by a factor of at most e^(2 d): 2 d (1 + d) sum p |v| more.  d, in a prompts' kernel: keys are rounded to half precision
-    (times 2^-6), u / 8 |k| or 2^-19, and sums are added up in float32 (40 roundings of 2^-23).  Else: a query channel is off by at most 2^-17 of the head's largest (two parts of 4 bits of a value scaled
-    to 128 .. 256, the second on a grid of 2^-9), which a code multiplies by up to 15 steps, and sums of up to 32 terms and of
-    groups are added up in float32, 40 roundings of at most 2^-23 of what is summed, codes and offsets apart."""
+    (times 2^-6), u / 8 |k| or 2^-19, and sums are added up in float32 (40 roundings of 2^-23).  Else: a query channel is off by at most
+    2^-17 of the head's largest (two parts of 4 bits of a value scaled to 128 .. 256, the second on a grid of 2^-9), which a code multiplies
+    by up to 15 steps, and sums of up to 32 terms and of groups are added up in float32, 40 roundings of at most 2^-23 of what is summed,
+    codes and offsets apart."""
     group = q.shape[1] // keys[0].shape[1]
     (kc, ks, ko), (vc, vs, vo) = ([x.to(F64).repeat_interleave(group, dim=1) for x in part] for part in (keys, vals))
     k, v = ko + ks * kc, vo + vs * vc

@@ -349,6 +349,31 @@ def test_prompts(ops, cuda_device, nh, nkv, hd, page, new, cached, masks, tensor
         assert ((out[mine].cpu().double().view(n, nh, hd) - expected).abs() <= bound).all(), r
 
 
+@pytest.mark.parametrize("power", [-90, -40, 0, 40, 100])
+@pytest.mark.parametrize("hd,tensor_memory", [(64, False), (128, False), (128, True)])
+def test_prompts_over_values_of_any_size(ops, cuda_device, hd, tensor_memory, power):
+    """Values times a power of two give results times it, but for roundings; keys stay.  Behind the end of the row a position holds what
+    would be far out of range."""
+    g, nkv, nh, n, context = torch.Generator().manual_seed(73), 2, 4, 200, 441
+    keys, values = torch.randn((context + 1, nkv, hd), generator=g), torch.randn((context + 1, nkv, hd), generator=g)
+    values[context] = 2.0 ** 20
+    qkv = torch.cat([torch.zeros((context + 1, hd)), keys.flatten(1), values.flatten(1) * 2.0 ** power], dim=1).to(cuda_device)
+    table, status = torch.arange(1, 29, dtype=torch.int32, device=cuda_device).view(1, -1), ops.new_status(cuda_device)
+    packed = torch.zeros(ops.packed_cache_shape(30, nkv, 16, hd), dtype=torch.uint8, device=cuda_device)
+    ops.qk_norm_rope_packed(qkv, 1, nkv, hd, None, None, 1e-6, None, None, i32(cuda_device, list(range(context + 1))),
+                            torch.zeros(context + 1, dtype=torch.int32, device=cuda_device), packed, table, status)
+    held = plain.read(packed[1:29].squeeze(2).cpu())                  # (codes, steps, offsets) [pages, heads, page, hd], of keys and of values
+    k, v = ([x.transpose(1, 2).reshape(-1, nkv, hd)[:context] for x in part] for part in held)
+    q = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16)
+    out, tile = torch.empty_like(q, device=cuda_device), ops.paged_prefill_tile_tokens()
+    starts = list(range(0, n, tile))
+    ops.paged_prefill_packed(q.to(cuda_device), packed, table, i32(cuda_device, [0] * len(starts)), i32(cuda_device, starts), i32(cuda_device, [0]),
+                             i32(cuda_device, [n]), i32(cuda_device, [context - n]), nh, nkv, hd, 0, hd ** -0.5, status, out, tensor_memory=tensor_memory)
+    ops.check_status(status)
+    expected, bound = plain.attention(q.double().view(n, nh, hd), k, v, context - n + torch.arange(n), hd ** -0.5, rounded=True)
+    assert ((out.cpu().double().view(n, nh, hd) - expected).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("hd,tensor_memory", [(64, False), (128, False), (128, True)])
 def test_a_query_that_is_not_finite_spoils_its_own_result_only(ops, cuda_device, hd, tensor_memory):
     packed, table, _ = paged_case(cuda_device, 2, hd, 16, [150, 70], 67)

@@ -117,12 +117,14 @@ __device__ __forceinline__ void pk_half_values(unsigned word, unsigned steps, un
     r[i] = pk_fma_f16x2(code, steps, offsets);
   }
 }
-// Two bfloat16 values as half-precision ones (exact from 2^-17 on; beyond 65504 infinite).
-__device__ __forceinline__ unsigned pk_to_half(unsigned pair) {
+// Two values as half-precision ones, the first in the low half.
+__device__ __forceinline__ unsigned pk_pack_half(float low, float high) {
   unsigned r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(__uint_as_float(pair & 0xffff0000u)), "f"(__uint_as_float(pair << 16)));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(high), "f"(low));
   return r;
 }
+// Two bfloat16 values as half-precision ones (exact from 2^-17 on; beyond 65504 infinite).
+__device__ __forceinline__ unsigned pk_to_half(unsigned pair) { return pk_pack_half(pk_low(pair), pk_high(pair)); }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
