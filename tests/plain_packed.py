@@ -92,11 +92,11 @@ def attention(q, keys, vals, pos, scale, window=0, chunk=0, sinks=None, softcap=
     k, v = ko + ks * kc, vo + vs * vc
     s = torch.einsum("thd,khd->htk", q, k) * scale
     if rounded:
-        d = torch.einsum("thd,khd->htk", q.abs(), k.abs() * (2.0 ** -11 + 40 * 2.0 ** -23) + 2.0 ** -19) * scale
+        d = torch.einsum("thd,khd->htk", q.abs(), k.abs() * (2.0 ** -11 + 40 * 2.0 ** -23) + 2.0 ** -19) * abs(scale)
         weight = 2 * v.abs()
     else:
         d = torch.einsum("thd,khd->htk", q.abs(), ks * kc + ko.abs()) * 40 * 2.0 ** -23
-        d = scale * (d + 15 * 2.0 ** -17 * q.abs().amax(-1).T.unsqueeze(-1) * ks.sum(-1).T.unsqueeze(1))
+        d = abs(scale) * (d + 15 * 2.0 ** -17 * q.abs().amax(-1).T.unsqueeze(-1) * ks.sum(-1).T.unsqueeze(1))
         weight = (vc - 8).abs() * vs + (vo + 8 * vs).abs()
     d = d + 2.0 ** -20 * (1 + s.abs())
     if softcap:

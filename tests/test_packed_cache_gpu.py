@@ -349,6 +349,25 @@ def test_prompts(ops, cuda_device, nh, nkv, hd, page, new, cached, masks, tensor
         assert ((out[mine].cpu().double().view(n, nh, hd) - expected).abs() <= bound).all(), r
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_that_are_not_positive(ops, cuda_device, hd, scale):
+    packed, table, rows = paged_case(cuda_device, 2, hd, 16, [150], 79)
+    q = torch.randn((130, 4 * hd), generator=torch.Generator().manual_seed(83)).to(torch.bfloat16)
+    status, out, one = ops.new_status(cuda_device), torch.zeros_like(q, device=cuda_device), torch.zeros_like(q, device=cuda_device)
+    tile = ops.paged_prefill_tile_tokens()
+    starts = list(range(0, 130, tile))
+    ops.paged_prefill_packed(q.to(cuda_device), packed, table, i32(cuda_device, [0] * len(starts)), i32(cuda_device, starts), i32(cuda_device, [0]),
+                             i32(cuda_device, [130]), i32(cuda_device, [20]), 4, 2, hd, 0, scale, status, out)
+    ops.paged_decode_packed(q.to(cuda_device), packed, table, i32(cuda_device, [0]), i32(cuda_device, [129]), i32(cuda_device, [149]), 150, 4, 2,
+                            hd, 0, scale, status, one)
+    ops.check_status(status)
+    for got, some, rounded in ((out, slice(0, 130), True), (one, slice(129, 130), False)):
+        n = some.stop - some.start
+        expected, bound = plain.attention(q[some].double().view(n, 4, hd), *rows[0], 20 + torch.arange(some.start, some.stop), scale, rounded=rounded)
+        assert ((got[some].cpu().double().view(n, 4, hd) - expected).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("power", [-90, -40, 0, 40, 100])
 @pytest.mark.parametrize("hd,tensor_memory", [(64, False), (128, False), (128, True)])
 def test_prompts_over_values_of_any_size(ops, cuda_device, hd, tensor_memory, power):

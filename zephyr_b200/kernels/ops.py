@@ -1596,7 +1596,7 @@ def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: tor
     ``paged_prefill_tile_tokens()``, whose keys and values the cache holds already; writes those tokens' rows of ``out``.  bfloat16;
     ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  Queries and keys are multiplied as half-precision values, keys times
     2^-6: queries up to 65504 and keys up to 2^22 in magnitude.  Head size 128 runs on tcgen05 (but the shortest prompts,
-    ``short_prompts``, and everything without ``tensor_memory``), other sizes on mma.sync."""
+    ``short_prompts``, and everything without ``tensor_memory`` or a positive scale), other sizes on mma.sync."""
     _check_index(block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status)
     _, n_table, max_blocks, pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh, nkv, hd,
                                                                       window, chunk, softcap, sinks)
@@ -1608,7 +1608,8 @@ def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: tor
     _check_boundaries(place, q_at, packed_at, out_at)
     call = _PACKED_PROMPT(out_at, q_at, packed_at, table_at, max_blocks, page_size, pages, n_table, tile_row_at, tile_q0_at, tiles, start_at,
                           len_at, ctx_at, nh, nkv, hd, window, chunk, scale, softcap, sinks_at, status_at, _stream())
-    if hd == 128 and tensor_memory and USE_TCGEN05_PREFILL and not short_prompts(block_table, page_size, nh, tiles):
+    # (The tcgen05 kernel takes a row's largest raw score for its largest exponent.)
+    if hd == 128 and tensor_memory and scale > 0.0 and USE_TCGEN05_PREFILL and not short_prompts(block_table, page_size, nh, tiles):
         _check(library().zb_paged_prefill_tc_packed(call), "paged_prefill_tc_packed")
     else:
         _check(library().zb_paged_prefill_packed(call), "paged_prefill_packed")
