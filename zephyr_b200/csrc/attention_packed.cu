@@ -782,8 +782,9 @@ int packed_decode_launch(const PackedDecodeArgs& a, int grid, int ranks, cudaStr
   int device = 0, sms = 0;
   if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
   // Where every CTA can have an SM (of the share that the launch may take), it asks for more than half of one's shared memory: else some SMs get two CTAs and others none
-  // (8 rows of 4096, 8 key/value heads, 128 CTAs: 18.2 or, as often, 24.1 us).
-  if (grid <= shared_sm_count(sms) && smem < PD_MORE_THAN_HALF) smem = PD_MORE_THAN_HALF;
+  // (8 rows of 4096, 8 key/value heads, 128 CTAs: 18.2 or, as often, 24.1 us).  Not so large clusters that they would wait for a free part
+  // of the chip (16 of 8 CTAs, 2 rows of 20000, 36 us so, 26 without).
+  if (grid <= shared_sm_count(sms) / (ranks > 4 ? 2 : 1) && smem < PD_MORE_THAN_HALF) smem = PD_MORE_THAN_HALF;
   if (smem > 227 * 1024) return ERR_UNSUPPORTED;
   const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
   if ((raised.load(std::memory_order_relaxed) & bit) == 0) {

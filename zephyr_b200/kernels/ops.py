@@ -1533,27 +1533,33 @@ PACKED_CLUSTERS, PACKED_CTA_SHARES, PACKED_WARP_SHARES = 0, 1, 2
 
 def packed_decode_plan(n_rows: int, nh: int, nkv: int, visible: int) -> tuple[int, int]:
     """How ``paged_decode_packed`` cuts contexts of which up to ``visible`` positions are seen: a cluster of n CTAs a (row, key/value
-    head) pair, or equal shares of all pairs for n CTAs or their warps, whose parts a second kernel merges (some 9 us more).
+    head) pair, or equal shares of all pairs for n CTAs or their warps, whose parts a second kernel merges.
 
-    Two CTAs an SM.  A cluster doubles while its shares stay above 128 positions and every CTA has an SM, and on to two an SM while
-    shares stay above 2048 (us: 4 rows of 600, 8 key/value heads, 1 / 2 / 4 / 8 CTAs 8.4 / 8.3 / 7.7 / 9.0; 12 of 1000, 1 / 2 10.2 /
-    11.5; 8 of 4096, 2 / 4 18.2 / 18.4; 4 of 16384, 4 / 8 33 / 26).  A warp takes 1.2 us for 32 positions while few
-    SMs read, 2 with two CTAs on every SM; so long contexts of few pairs are cheaper in shares (1 row of 40000 in clusters of 8 / shares 32 / 24, 2 rows 46 /
-    33; 1 of 4096 8.9 / 10.2), and more pairs than CTAs in warps' shares, which also even out rows of unequal lengths (64 rows of 4096
-    in whole contexts / shares 74 / 74, of 1 to 4096 56 / 47, 256 of 64 41 / 16), unless they are not many and short (64 of 300 17.5 /
-    20.5, of 1000 31 / 33)."""
+    What a launch takes is, near enough, a fixed time and one for every 32 positions of a warp, which is 1.2 us while every CTA has an SM
+    to itself and 1.9 with two: a cluster 8.6 or 10.7 us beside that, shares 13.5 or 17.7.  The least of these is taken, among clusters
+    whose CTAs have 128 positions or more; shares where they gain a tenth, since contexts may be shorter than ``visible``, which a captured
+    step rounds up.  (Measured, us, 32/8 heads: 8 rows of 8024 in clusters of 2 / 4 / 148 / 296 shares 27.6 / 26.0 /
+    32.3 / 30.9, 4 of 16000 in 4 / 8 / 148 / 296 27.4 / 25.9 / 31.4 / 29.9, 16 of 8000 in 1 / 2 / 296 45.1 / 40.7 / 47.9, 2 of 20000 in 4 / 148
+    31.3 / 23.4, 1 of 120001 in 8 / 148 / 296 77 / 45.6 / 41.9, 12 of 1000 in 1 / 2 10.2 / 11.5.)  More pairs than CTAs go in warps' shares, which
+    also even out rows of unequal lengths (64 rows of 4096 in whole contexts / shares 74 / 74, of 1 to 4096 56 / 47, 256 of 64 41 / 16), unless
+    they are not many and short (64 of 300 17.5 / 20.5, of 1000 31 / 33)."""
     pairs = n_rows * nkv * -(-nh // nkv // 8)
     sms = _sm_count()
     if pairs > 2 * sms:
         return (PACKED_CLUSTERS, 1) if pairs <= 4 * sms and visible <= 1024 else (PACKED_WARP_SHARES, 2 * sms)
-    ctas = 1
-    while ctas < 8 and visible > 256 * ctas and (2 * ctas * pairs <= sms or (2 * ctas * pairs <= 2 * sms and visible >= 4096 * ctas)):
+    tiles = visible / 32
+    best, plan, ctas = math.inf, (PACKED_CLUSTERS, 1), 1
+    while ctas <= 8 and pairs * ctas <= 2 * sms and (ctas == 1 or visible > 128 * ctas):
+        alone = pairs * ctas * (2 if ctas == 8 else 1) <= sms         # (as the launch has it)
+        us = (8.6 + 1.2 * tiles / (8 * ctas)) if alone else (10.7 + 1.9 * tiles / (8 * ctas))
+        if us < best:
+            best, plan = us, (PACKED_CLUSTERS, ctas)
         ctas *= 2
-    tiles = -(-visible // 32)
-    us = 1.2 if 2 * pairs * ctas <= sms else (1.6 if pairs * ctas <= sms else 2.0)
-    if tiles / (8 * ctas) * us <= pairs * tiles / (8 * sms) + 9.0:
-        return PACKED_CLUSTERS, ctas
-    return PACKED_CTA_SHARES, (1 if pairs * tiles < 8192 else 2) * sms
+    shared = pairs * tiles / (8 * sms)
+    for us, ctas in ((13.5 + 1.2 * shared, sms), (17.7 + 0.95 * shared, 2 * sms)):
+        if 1.1 * us < best:
+            best, plan = 1.1 * us, (PACKED_CTA_SHARES, ctas)
+    return plan
 
 
 def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, row_q_start: torch.Tensor,
