@@ -476,12 +476,10 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       const int which = order(item), j = which >> 1, stage = item % STAGES, k0 = tile_start(j);
       const int from = run_lo(j) - k0, until = run_hi(j) - k0;                // the rows that count
       unsigned char* const dst = ring + stage * ITEM_BYTES;
-      // A barrier's parity tells a phase from its neighbours only: a team waits for the stages of the other teams' items too, so that it
-      // misses no phase of any stage.
-      bool free = true;
-      for (int i = max(item - TC_PACKED_TEAMS + 1, 0); i <= item; ++i)
-        free = free && __all_sync(0xffffffffu, wait(&kv_empty[i % STAGES], ((i / STAGES) & 1) ^ 1));
-      if (!free) {
+      // A barrier's parity tells a phase from its neighbours only.  The item two turns of this stage ago was consumed before the one that
+      // this team waited for last, since products take items in order; and the next phase cannot end before this item is here.  (The stages of
+      // the other teams' items can be a phase further on: a team does not look at them.)
+      if (!__all_sync(0xffffffffu, wait(&kv_empty[stage], ((item / STAGES) & 1) ^ 1))) {
         give_up(-1);
         break;
       }
