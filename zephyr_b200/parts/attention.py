@@ -233,7 +233,9 @@ class Attention(Mixer):
                 and self.position.as_rotation_tables() != (None, None)):
             raise ConfigError("the general attention path rotates adjacent pairs, halves of part of a head, or nothing")
         if self.w_gate is not None:
-            self.w_qkv = torch.cat([self.w_qkv, self.w_gate], dim=0).contiguous()
+            # (The kernel that writes into a 4-bit cache reads rows of the product that start on boundaries of four values.)
+            unused = -(self.w_qkv.shape[0] + self.w_gate.shape[0]) % 4 if self.cache_bits else 0
+            self.w_qkv = torch.cat([self.w_qkv, self.w_gate, self.w_qkv.new_zeros((unused, self.w_qkv.shape[1]))], dim=0).contiguous()
             self.w_q = self.w_qkv[: self.nh * self.hd]
         self.q_norm = self.q_norm.float().contiguous() if self.q_norm is not None else None
         self.k_norm = self.k_norm.float().contiguous() if self.k_norm is not None else None
