@@ -1577,12 +1577,14 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
         q, packed, block_table, rows, row_q_start, row_ctx, status, out, sinks)
     _check_boundaries(place, q_at, packed_at, out_at)
     n_rows = rows.numel()
+    if n_rows == 0:
+        return out
     if plan is None:
         visible = min(max_context, window) if window else max_context
         plan = packed_decode_plan(n_rows, nh, nkv, min(visible, chunk) if chunk else visible)
     mode, ctas = plan
     scratch = None
-    if mode != PACKED_CLUSTERS and n_rows > 0:
+    if mode != PACKED_CLUSTERS:
         pairs = n_rows * nkv * -(-nh // nkv // 8)
         scratch = torch.empty(int(library().zb_paged_decode_packed_scratch_floats(ctas, int(mode == PACKED_WARP_SHARES), pairs, hd)),
                               dtype=torch.float32, device=q.device)
