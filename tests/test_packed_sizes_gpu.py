@@ -1,0 +1,112 @@
+"""The 4-bit cache over keys, queries and values of any size.  Sizes are powers of two, so results are compared after the power has been
+taken out again: no bound here has a part that does not shrink with what it bounds."""
+
+import math
+
+import pytest
+import torch
+
+import plain_packed as plain
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from zephyr_b200.kernels import ops
+    return ops
+
+
+def i32(device, values):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def held_cache(ops, device, keys, values, page=16):
+    """A cache of one row that holds keys and values [positions, kv_heads, hd] (float32), its table, and what it holds as (codes, steps,
+    offsets), [positions, kv_heads, hd] each in float64."""
+    n, nkv, hd = keys.shape
+    blocks = -(-n // page)
+    packed = torch.zeros(ops.packed_cache_shape(blocks + 1, nkv, page, hd), dtype=torch.uint8, device=device)
+    table, status = torch.arange(1, blocks + 1, dtype=torch.int32, device=device).view(1, -1), ops.new_status(device)
+    qkv = torch.cat([torch.zeros((n, hd)), keys.flatten(1), values.flatten(1)], dim=1).to(device)
+    ops.qk_norm_rope_packed(qkv, 1, nkv, hd, None, None, 1e-6, None, None, i32(device, list(range(n))), i32(device, [0] * n), packed, table, status)
+    ops.check_status(status)
+    held = plain.read(packed[1:].cpu())                                # [blocks, heads, page / 16, 16, hd]
+    return packed, table, [[x.permute(0, 2, 3, 1, 4).reshape(-1, nkv, hd)[:n].double() for x in part] for part in held]
+
+
+def times(part, power):
+    codes, steps, offsets = part
+    return codes, steps * 2.0 ** power, offsets * 2.0 ** power
+
+
+def decode(ops, device, packed, table, q, n, nh, nkv, hd, scale, plan, **masks):
+    status = ops.new_status(device)
+    out = ops.paged_decode_packed(q.to(device), packed, table, i32(device, [0]), i32(device, [0]), i32(device, [n - 1]), n, nh, nkv, hd,
+                                  masks.pop("window", 0), scale, status, torch.empty_like(q, device=device), plan=plan, **masks)
+    ops.check_status(status)
+    return out.cpu().double().view(1, nh, hd)
+
+
+PLANS = [(0, 1), (0, 4), (1, 3), (2, 2)]
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("power", [-100, -70, -45, -25, 25, 50, 66, 100])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (8, 2, 128), (2, 1, 96), (3, 3, 32)])
+def test_single_tokens_over_values_of_any_size(ops, cuda_device, nh, nkv, hd, power, plan):
+    n, g = 700, torch.Generator().manual_seed(5)
+    keys, values = torch.randn((n, nkv, hd), generator=g), torch.randn((n, nkv, hd), generator=g)
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys, values * 2.0 ** power)
+    q = torch.randn((1, nh * hd), generator=g).to(torch.bfloat16)
+    got = decode(ops, cuda_device, packed, table, q, n, nh, nkv, hd, hd ** -0.5, plan) * 2.0 ** -power
+    expected, bound = plain.attention(q.double().view(1, nh, hd), k, times(v, -power), torch.tensor([n - 1]), hd ** -0.5)
+    assert ((got - expected).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("powers", [(0, 40), (40, 0), (-60, 0), (0, -60), (-90, -30, 20, 80), (80, -90), (None, -50, 10), (None, None, 60)])
+def test_single_tokens_over_values_of_several_sizes(ops, cuda_device, powers, plan):
+    """Runs of positions whose values differ in size (None: zeros), none of which begins where a tile does."""
+    nh, nkv, hd, n, g = 6, 2, 64, 900, torch.Generator().manual_seed(7)
+    keys, values = torch.randn((n, nkv, hd), generator=g), torch.randn((n, nkv, hd), generator=g)
+    run = -(-n // len(powers)) + 5
+    for i, power in enumerate(powers):
+        values[i * run:(i + 1) * run] *= 0.0 if power is None else 2.0 ** power
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys, values)
+    q = torch.randn((1, nh * hd), generator=g).to(torch.bfloat16)
+    top = max(p for p in powers if p is not None)
+    for length in (n, run, run + 1, n - 3):
+        got = decode(ops, cuda_device, packed, table, q, length, nh, nkv, hd, hd ** -0.5, plan)
+        seen = [p for i, p in enumerate(powers) if i * run < length and p is not None]
+        by = max(seen) if seen else top
+        expected, bound = plain.attention(q.double().view(1, nh, hd), [x[:length] for x in k], times([x[:length] for x in v], -by),
+                                          torch.tensor([length - 1]), hd ** -0.5)
+        assert ((got * 2.0 ** -by - expected).abs() <= bound).all(), length
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("power", [30, 100])
+def test_single_tokens_do_not_hang_on_values_that_they_do_not_see(ops, cuda_device, power, plan):
+    nh, nkv, hd, n, window, g = 4, 2, 64, 400, 77, torch.Generator().manual_seed(11)
+    keys, values = torch.randn((n, nkv, hd), generator=g), torch.randn((n, nkv, hd), generator=g)
+    loud = values.clone()
+    loud[:n - window] *= 2.0 ** power
+    q, outs = torch.randn((1, nh * hd), generator=g).to(torch.bfloat16), []
+    for one in (values, loud):
+        packed, table, _ = held_cache(ops, cuda_device, keys, one)
+        outs.append(decode(ops, cuda_device, packed, table, q, n, nh, nkv, hd, hd ** -0.5, plan, window=window))
+    assert torch.isfinite(outs[0]).all() and torch.equal(*outs)
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("power", [-90, -16, -12, 10, 40, 90])
+def test_single_tokens_over_keys_of_any_size(ops, cuda_device, power, plan):
+    """Keys times a power of two under queries divided by it: the same scores."""
+    nh, nkv, hd, n, g = 8, 2, 128, 600, torch.Generator().manual_seed(13)
+    keys, values = torch.randn((n, nkv, hd), generator=g), torch.randn((n, nkv, hd), generator=g)
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys * 2.0 ** power, values)
+    q = (torch.randn((1, nh * hd), generator=g) * 2.0 ** -power).to(torch.bfloat16)
+    got = decode(ops, cuda_device, packed, table, q, n, nh, nkv, hd, hd ** -0.5, plan)
+    expected, bound = plain.attention(q.double().view(1, nh, hd) * 2.0 ** power, times(k, -power), v, torch.tensor([n - 1]), hd ** -0.5)
+    assert ((got - expected).abs() <= bound).all()

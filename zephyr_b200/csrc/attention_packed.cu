@@ -5,8 +5,12 @@
 // layout (packed.cuh) is the operands', codes become numbers by masks alone, and steps and offsets join where there is little:
 //   codes    The low four bits of a bfloat16's low byte are, as a number, code * 2^-133, the next four 16 times that: bfloat16's
 //            subnormals and its first binade are one line.  A word of eight codes is four operand registers after four masks and a
-//            shift.  What multiplies them carries a power of two (2^60 in weights, a head's own in queries) that keeps products and
-//            sums far from float32's ends; all of it is exact.
+//            shift.  What multiplies them carries a power of two (2^80 in weights, a head's own in queries) that keeps products and
+//            sums far from float32's ends; all of it is exact.  That holds for values while the largest step or offset that a warp has
+//            seen is 2^-30 to 2^12; else they carry a power of two as well, which follows that largest one (sums are rescaled with it, as
+//            with the scores' maximum).  So values of 2^-100 to 2^100 hold, and beside the largest product of a weight and a value what
+//            is 2^80 times smaller keeps its bits.  (The look at a tile's parameters takes some 15 of its 600 instructions: 52.2 -> 53.7 us
+//            for 48 rows of 1 to 6001 positions, 42.0 -> 43.5 for one of 120001, 18.3 -> 19.0 for 8 of 4096.)
 //   keys     S[h, p] = sum_j step_pj c_j[h, p] + sum_j offset_pj (sum_{d in j} q_hd), c_j being the product over the codes of a group
 //            of 32 channels.  The first sum in float32; the second a product of the position's parameters as they lie and the query
 //            sums as two bfloat16 parts.
@@ -36,7 +40,9 @@ constexpr int PD_WARPS = 8;
 constexpr int PD_STAGES = 2;              // a power of two
 constexpr int PD_TILE = 32;              // positions per tile: a warp's unit of work
 constexpr int PD_HEADS = 8;              // query heads on the products' columns
-constexpr float PD_LIFT = 60.0f;         // weights carry 2^60, results 2^(60 - 133)
+constexpr float PD_LIFT = 80.0f;         // weights carry 2^80, results 2^(80 - 133)
+constexpr unsigned PD_VALUES_FROM = 0x3080u, PD_VALUES_TO = 0x4580u;      // 2^-30 and 2^12 as bfloat16: between them values carry nothing
+constexpr float PD_VALUES_UNSEEN = 8.507059173023462e37f;                 // 2^126
 constexpr float PD_RESCALE = 8.0f;       // a running maximum (in powers of two) may be passed by this before sums are rescaled
 
 enum { PD_CLUSTERS, PD_CTA_SHARES, PD_WARP_SHARES };      // how contexts are cut
@@ -380,7 +386,7 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) scale_c[h] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * h) * 1.329227995784916e36f * (8192.0f * scale_d);
     }
-    // Heads 2 t and 2 t + 1: the maximum, what is added to scores so that it becomes 2^60's exponent, from where on it has to move; and
+    // Heads 2 t and 2 t + 1: the maximum, what is added to scores so that it becomes 2^80's exponent, from where on it has to move; and
     // the sums over this lane's positions.
     float m_run[2] = {-INFINITY, -INFINITY}, lift[2] = {0.0f, 0.0f}, limit[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
     float o[2 * NG][4], rest_c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, weights_c[(NG + 1) / 2][4];
@@ -388,6 +394,8 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
     for (int n = 0; n < (NG + 1) / 2; ++n) weights_c[n][0] = weights_c[n][1] = weights_c[n][2] = weights_c[n][3] = 0.0f;
 #pragma unroll
     for (int n = 0; n < 2 * NG; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    // The power of two that steps and offsets of values carry: it falls as the largest of them grows.
+    float value_scale = PD_VALUES_UNSEEN;
 
 #pragma unroll 1
     for (int j0 = WARPWISE ? 0 : warp; j0 < seg.count; j0 += STRIDE) {
@@ -499,6 +507,59 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           }
         }
       }
+      // Columns 0 .. NG - 1 of a pair of positions' parameters are steps, NG .. 2 NG - 1 offsets: this lane's, pairs t and t + 4.  Positions
+      // outside hold what was there before, a NaN maybe: their parameters become zeros.
+      auto seen = [&](int pos) { return pos >= seg.lo && pos < seg.hi; };
+      auto value_params = [&](int b, unsigned (&params)[2]) {
+        params[0] = params[1] = 0u;
+        if (NG == 4 || g < 2 * NG) {
+          params[0] = *reinterpret_cast<const unsigned*>(tile + b * BLOCK_BYTES + pk_value_step<HD>(t, 0) + 4 * g);
+          params[1] = *reinterpret_cast<const unsigned*>(tile + b * BLOCK_BYTES + pk_value_step<HD>(t + 4, 0) + 4 * g);
+        }
+        if constexpr (edge) {
+          auto keep = [&](int pos) { return (seen(pos) ? 0x0000ffffu : 0u) | (seen(pos + 1) ? 0xffff0000u : 0u); };
+          params[0] &= keep(pos0 + 16 * b + 2 * t);
+          params[1] &= keep(pos0 + 16 * b + 8 + 2 * t);
+        }
+      };
+      {
+        unsigned params[2], most = 0u;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          value_params(b, params);
+          most = __vmaxu2(most, __vmaxu2(params[0] & 0x7fff7fffu, params[1] & 0x7fff7fffu));
+        }
+        // (A half that is PD_VALUES_TO or more gets its highest bit.)
+        constexpr unsigned UP = (0x8000u - PD_VALUES_TO) * 0x10001u;
+        if (__any_sync(0xffffffffu, value_scale != 1.0f || (most + UP & 0x80008000u) != 0u)) {
+          unsigned top = 0u;
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            value_params(b, params);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const unsigned half = params[i >> 1] >> 16 * (i & 1) & 0x7fffu;
+              top = half < 0x7f80u ? max(top, half) : top;          // (a group that is not finite is a NaN, whatever it carries)
+            }
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          // To 2^11 or as near as 2^126 takes it.
+          float now = __uint_as_float(min(265 - static_cast<int>(top >> 7), 253) << 23);
+          if (top >= PD_VALUES_FROM && top < PD_VALUES_TO) now = 1.0f;
+          if (now < value_scale) {
+            const float factor = now * (1.0f / value_scale);
+            value_scale = now;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              rest_c[c] *= factor;
+#pragma unroll
+              for (int n = 0; n < (NG + 1) / 2; ++n) weights_c[n][c] *= factor;
+#pragma unroll
+              for (int n = 0; n < 2 * NG; ++n) o[n][c] *= factor;
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const unsigned char* const block = tile + b * BLOCK_BYTES;
@@ -514,24 +575,25 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
         pk_load_words(v1, block + pk_value_word<HD>(1, g, t, 0));
         pk_load_words(steps0, block + pk_value_step<HD>(g >> 1, 0));
         pk_load_words(steps1, block + pk_value_step<HD>((g >> 1) + 4, 0));
-        // Columns 0 .. NG - 1: steps, NG .. 2 NG - 1: offsets.
-        unsigned params[2] = {0u, 0u};
-        if (NG == 4 || g < 2 * NG) {
-          params[0] = *reinterpret_cast<const unsigned*>(block + pk_value_step<HD>(t, 0) + 4 * g);
-          params[1] = *reinterpret_cast<const unsigned*>(block + pk_value_step<HD>(t + 4, 0) + 4 * g);
-        }
+        unsigned params[2];
+        value_params(b, params);
         if constexpr (edge) {
-          // Positions outside hold what was there before, a NaN maybe: their parameters become zeros.
-          auto seen = [&](int pos) { return pos >= seg.lo && pos < seg.hi; };
-          auto keep = [&](int pos) { return (seen(pos) ? 0x0000ffffu : 0u) | (seen(pos + 1) ? 0xffff0000u : 0u); };
           const unsigned keep0 = seen(pos0 + 16 * b + g) ? 0xffffffffu : 0u, keep1 = seen(pos0 + 16 * b + 8 + g) ? 0xffffffffu : 0u;
 #pragma unroll
           for (int m = 0; m < NG; ++m) {
             steps0[m] &= keep0;
             steps1[m] &= keep1;
           }
-          params[0] &= keep(pos0 + 16 * b + 2 * t);
-          params[1] &= keep(pos0 + 16 * b + 8 + 2 * t);
+        }
+        if (value_scale != 1.0f) {
+          auto scaled = [&](unsigned pair) { return pack_bf16(pk_low(pair) * value_scale, pk_high(pair) * value_scale); };
+          params[0] = scaled(params[0]);
+          params[1] = scaled(params[1]);
+#pragma unroll
+          for (int m = 0; m < NG; ++m) {
+            steps0[m] = scaled(steps0[m]);
+            steps1[m] = scaled(steps1[m]);
+          }
         }
         // Weights have positions on rows, the products want them on their inner dimension: 8 x 8 pieces change sides.
         mma_rows8(rest_c, turned(pack_bf16(p[0], p[1])), turned(pack_bf16(p[2], p[3])), params[0], params[1]);
@@ -564,9 +626,10 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
       __syncwarp();                // every lane has read the tile: its place may be filled again
       issue();
     }
-    // The weights' power of two out, and the offsets' part in.  Lane (g, t): rest_c has sum step P and sum offset P of head g, columns
+    // The powers of two out, and the offsets' part in.  Lane (g, t): rest_c has sum step P and sum offset P of head g, columns
     // 2 t and 2 t + 1 of the parameters; weights_c -1 times the sums of the rounded weights of head g, a half of the positions each.
-    constexpr float DOWN = 8.673617379884035e-19f, CODE_UP = 9.44473296573929e21f;        // 2^-60, 2^73
+    constexpr float DOWN = 8.271806125530277e-25f, CODE_UP = 9007199254740992.0f;        // 2^-80, 2^53
+    const float unscale = 1.0f / value_scale;
     l_run[0] *= DOWN;
     l_run[1] *= DOWN;
 #pragma unroll
@@ -580,8 +643,8 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
         const float extra = DOWN * fmaf(8.0f, steps + __shfl_sync(0xffffffffu, weights, row), offsets);
 #pragma unroll
         for (int n = 2 * m; n < 2 * m + 2; ++n) {
-          o[n][h] = fmaf(o[n][h], CODE_UP, extra);
-          o[n][2 + h] = fmaf(o[n][2 + h], CODE_UP / 16.0f, extra);
+          o[n][h] = fmaf(o[n][h], CODE_UP, extra) * unscale;
+          o[n][2 + h] = fmaf(o[n][2 + h], CODE_UP / 16.0f, extra) * unscale;
         }
       }
     }

@@ -1569,7 +1569,7 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
     """``paged_decode`` over a 4-bit cache: attention of rows with one new token each, whose key and value the cache holds already;
     writes those tokens' rows of ``out``.  bfloat16; ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  ``max_context`` is at
     least the longest context of the rows, the new token included.  ``plan``: as ``packed_decode_plan`` gives it (None: chosen by
-    that).  The scratch of a launch is the call's own."""
+    that).  The scratch of a launch is the call's own.  Queries, keys and values of 2^-100 to 2^100 in magnitude."""
     _check_index(block_table, rows, row_q_start, row_ctx, status)
     tokens, n_table, max_blocks, pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh,
                                                                            nkv, hd, window, chunk, softcap, sinks)
