@@ -110,3 +110,70 @@ def test_single_tokens_over_keys_of_any_size(ops, cuda_device, power, plan):
     got = decode(ops, cuda_device, packed, table, q, n, nh, nkv, hd, hd ** -0.5, plan)
     expected, bound = plain.attention(q.double().view(1, nh, hd) * 2.0 ** power, times(k, -power), v, torch.tensor([n - 1]), hd ** -0.5)
     assert ((got - expected).abs() <= bound).all()
+
+
+# -------------------------------------------------------------------------------------------- prompts
+def prompt(ops, device, packed, table, q, n, context, nh, nkv, hd, scale, tensor_memory=True, **masks):
+    """The last n of ``context`` positions, queries [n, nh * hd]."""
+    status, out, tile = ops.new_status(device), torch.empty_like(q, device=device), ops.paged_prefill_tile_tokens()
+    starts = list(range(0, n, tile))
+    ops.paged_prefill_packed(q.to(device), packed, table, i32(device, [0] * len(starts)), i32(device, starts), i32(device, [0]), i32(device, [n]),
+                             i32(device, [context - n]), nh, nkv, hd, masks.pop("window", 0), scale, status, out, tensor_memory=tensor_memory, **masks)
+    ops.check_status(status)
+    return out.cpu().double().view(n, nh, hd)
+
+
+KERNELS = [(64, False), (96, False), (128, False), (128, True)]
+
+
+@pytest.mark.parametrize("nh", [4, 32])                 # (a head a CTA, pairs of heads)
+@pytest.mark.parametrize("power", [30, 40, 90, -40])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_earlier_tokens_do_not_hang_on_later_ones_values(ops, cuda_device, hd, tensor_memory, power, nh):
+    """From some position on values are of another size: what sees none of them is what it is without them, bit by bit."""
+    nkv, n, context, first, g = 2, 300, 420, 333, torch.Generator().manual_seed(17)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    loud = values.clone()
+    loud[first:] *= 2.0 ** power
+    q, outs = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16), []
+    for one in (values, loud):
+        packed, table, held = held_cache(ops, cuda_device, keys, one)
+        outs.append(prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory))
+    before = first - (context - n)
+    assert torch.equal(outs[0][:before], outs[1][:before])
+    expected, bound = plain.attention(q.double().view(n, nh, hd), held[0], times(held[1], -max(power, 0)), context - n + torch.arange(n), hd ** -0.5, rounded=True)
+    assert ((outs[1] * 2.0 ** -max(power, 0) - expected).abs() <= bound)[before:].all()
+
+
+@pytest.mark.parametrize("power", [40, 90])
+@pytest.mark.parametrize("masks", [dict(window=70), dict(chunk=64), dict(chunk=100, window=30)])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_tokens_do_not_hang_on_values_behind_their_window_or_chunk(ops, cuda_device, hd, tensor_memory, masks, power):
+    nh, nkv, n, context, last, g = 4, 2, 300, 420, 200, torch.Generator().manual_seed(19)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    loud = values.clone()
+    loud[:last] *= 2.0 ** power
+    q, outs = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16), []
+    for one in (values, loud):
+        packed, table, _ = held_cache(ops, cuda_device, keys, one)
+        outs.append(prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory, **masks))
+    pos = context - n + torch.arange(n)
+    seen = torch.zeros_like(pos)
+    if masks.get("window"):
+        seen = torch.maximum(seen, pos + 1 - masks["window"])
+    if masks.get("chunk"):
+        seen = torch.maximum(seen, pos // masks["chunk"] * masks["chunk"])
+    apart = seen >= last
+    assert apart.sum() > 100 and torch.isfinite(outs[1]).all() and torch.equal(outs[0][apart], outs[1][apart])
+
+
+@pytest.mark.parametrize("power", [-100, -60, -30, 30, 60, 100])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_prompts_over_values_of_other_sizes(ops, cuda_device, hd, tensor_memory, power):
+    nh, nkv, n, context, g = 4, 2, 200, 441, torch.Generator().manual_seed(23)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys, values * 2.0 ** power)
+    q = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16)
+    got = prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory) * 2.0 ** -power
+    expected, bound = plain.attention(q.double().view(n, nh, hd), k, times(v, -power), context - n + torch.arange(n), hd ** -0.5, rounded=True)
+    assert ((got - expected).abs() <= bound).all()

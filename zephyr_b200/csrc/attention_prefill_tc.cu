@@ -209,7 +209,7 @@ __device__ __forceinline__ float tc_row_max(unsigned tmem_row, int last, int fir
 // 64 columns (from `column0` on) of a row of S -> probabilities exp2(s * scale + neg_shift) as 32 words of two bfloat16 each,
 // and their sums on top of `sums`.  CAPPED: the exponent is cap_log2 * tanh(s * scale) + neg_shift, `scale` then being
 // scale / softcap.
-template <bool MASKED, bool CAPPED, bool HALVES>
+template <bool MASKED, bool CAPPED>
 __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, unsigned (&words)[32], unsigned long long (&sums)[4],
                                                 float scale, float neg_shift, int last, int first, float cap_log2) {
   const unsigned long long scale2 = pack_f32x2(scale, scale), shift2 = pack_f32x2(neg_shift, neg_shift);
@@ -235,7 +235,7 @@ __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, 
         p[e] = !MASKED || (column <= last && column >= first) ? exp2_approx(x[e]) : 0.0f;
       }
       sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(p[0], p[1]));
-      words[16 * c + (i >> 1)] = HALVES ? pk_pack_half(p[0], p[1]) : pack_bf16(p[0], p[1]);
+      words[16 * c + (i >> 1)] = pack_bf16(p[0], p[1]);
     }
   }
 }
@@ -248,25 +248,18 @@ enum { TC_FORM_PLAIN, TC_FORM_BIASED, TC_FORM_CHUNKED, TC_FORM_KEPT };      // K
 // the softmax of a pair of heads takes, are issued between that softmax's own, and bound the kernel with it: 1024 tokens behind 7000,
 // 32/8 heads, 171 us (738 TFLOP/s) where the cache in bfloat16 takes 142; 8192 new tokens 659 against 530.
 // Keys are half-precision values (packed.cuh), a key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every
-// eight), and the queries' in the same.  Values are half-precision too, times a power of two that the loaders find before the first of
-// them: twice the largest step x 15 or offset in the CTA's sight stays below 2^15, and what is 2^29 times smaller keeps all its bits.
-// Probabilities carry 2^7, so that one of 2^-21 does.  (With both in bfloat16 a result was 0.0027 off, with half precision 0.0017, which
-// is its own rounding; 167 and 171 us.)
+// eight), and the queries' in the same.  Values and weights are bfloat16, whose range no position's size takes from another's.  (Half
+// precision, off by a third less, 0.0017 against 0.0027 of the result, wants one power of two for all values in the CTA's sight: a value
+// that a query does not see, 2^27 and more times larger, then took bits from those that it does.)
 constexpr int TC_PACKED_THREADS = 512;             // warps 9 .. 14 load, the last one has nothing to do
 constexpr int TC_PACKED_STAGES = 4;
 constexpr int TC_PACKED_TEAMS = 3;
 constexpr int TC_PACKED_AHEAD = 3;                 // blocks of 16 positions that a warp has copied, the one that it works on among them
 constexpr int TC_PACKED_PART = pk_block_bytes(128) / 2;         // a block's keys, or its values
 constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_PART;
-constexpr float TC_PACKED_LIFT = 7.0f;               // (32768 for a probability that has passed its row's shift by all it may)
 constexpr int TC_PACKED_SOFTMAX_REGISTERS = 152, TC_PACKED_OTHER_REGISTERS = 104;
 static_assert(TC_PACKED_SMEM <= 223 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
 static_assert(256 * (TC_PACKED_SOFTMAX_REGISTERS + TC_PACKED_OTHER_REGISTERS) <= TC_PACKED_THREADS * 128, "no more registers than at launch");
-
-// 2^e for values whose steps times 15 and offsets stay below the given float's next power of two.
-__device__ __forceinline__ float tc_packed_value_scale(unsigned top) {
-  return __uint_as_float((267u - max(top >> 23, 27u)) << 23);
-}
 
 template <int FORM, int HD, bool SHARED, bool PACKED = false>
 __global__ void __launch_bounds__(PACKED ? TC_PACKED_THREADS : TC_THREADS, 1)
@@ -291,10 +284,8 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   __shared__ unsigned tmem_base_s;
   __shared__ volatile int abort_flag;
 
-  __shared__ unsigned value_top;              // PACKED: the bits of the largest step x 15 or offset of the values in sight
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    value_top = 0;
     for (int b = 0; b < STAGES; ++b) {
       mbar_init(&kv_full[b], PACKED ? 2 : Shape::KIND_WARPS);
       mbar_init(&kv_empty[b], 1);
@@ -425,53 +416,9 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       }
       cp_async_commit();
     };
-    // Half a warp a block's parameters of values, four pairs of blocks at a time, the first of them asked for ahead of all else.
-    constexpr int WARPS = 2 * TC_PACKED_TEAMS, AT_ONCE = 4;
-    uint4 asked[AT_ONCE];
-    auto ask = [&](int first) {
-#pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        const int n = first + u * 2 * WARPS, j = min(n >> 3, n_tiles - 1), pos = tile_start(j) + (n & 7) * PK_BLOCK;
-        const int entry = pos >> a.page_shift;
-        const int page = n < 4 * items && pos < run_hi(j) && pos + PK_BLOCK > run_lo(j) && entry < a.max_blocks ? table[entry] : -1;
-        asked[u] = make_uint4(0, 0, 0, 0);
-        if (page > 0 && page < a.num_pages)
-          asked[u] = *reinterpret_cast<const uint4*>(cache + static_cast<long long>(((page * a.nkv + kvh) << (a.page_shift - 4)) + ((pos & (page_size - 1)) >> 4)) *
-                                                                 pk_block_bytes(128) + pk_value_step<128>(0, 0) + (lane & 15) * 16);
-      }
-    };
-    int first = 2 * (2 * team + member) + (lane >> 4);
-    ask(first);
     int blocks = look_up(team), next_blocks = -1, taken = 0;
 #pragma unroll
     for (int b = 0; b < AHEAD - 1; ++b) copy(team, b, blocks);
-    float top = 0.0f;
-    for (; first < 4 * items;) {
-#pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        // Two positions' steps, or offsets, of the position's part that counts.
-        const int n = first + u * 2 * WARPS, j = min(n >> 3, n_tiles - 1), p = tile_start(j) + (n & 7) * PK_BLOCK + (lane & 14);
-        const unsigned w[4] = {asked[u].x, asked[u].y, asked[u].z, asked[u].w};
-        float low = 0.0f, high = 0.0f;           // (fmaxf passes a NaN by)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          low = fmaxf(low, fabsf(pk_low(w[g])));
-          high = fmaxf(high, fabsf(pk_high(w[g])));
-        }
-        const int lo = run_lo(j), hi = run_hi(j);
-        if (p >= lo && p < hi && low <= 3.4e38f) top = fmaxf(top, lane & 1 ? low : 15.0f * low);
-        if (p + 1 >= lo && p + 1 < hi && high <= 3.4e38f) top = fmaxf(top, lane & 1 ? high : 15.0f * high);
-      }
-      first += AT_ONCE * 2 * WARPS;
-      if (first < 4 * items) ask(first);
-    }
-    __syncwarp();
-    if (team < TC_PACKED_TEAMS) {
-      const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, 3.4e38f)));
-      if (lane == 0) atomicMax(&value_top, bits);
-      asm volatile("bar.sync 2, %0;\n" ::"n"(WARPS * 32) : "memory");
-    }
-    const float value_scale = tc_packed_value_scale(value_top);
     for (int item = team; item < items; item += TC_PACKED_TEAMS) {
       const int which = order(item), j = which >> 1, stage = item % STAGES, k0 = tile_start(j);
       const int from = run_lo(j) - k0, until = run_hi(j) - k0;                // the rows that count
@@ -519,34 +466,26 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
           const uint4 low = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp, t, 0));
           const uint4 high = *reinterpret_cast<const uint4*>(block + pk_value_word<128>(h, 2 * gp + 1, t, 0));
           const unsigned lo4[4] = {low.x, low.y, low.z, low.w}, hi4[4] = {high.x, high.y, high.z, high.w};
-          // (The four lanes of a pair of positions turn a group's step and offset into half precision each, and hand them round.)
-          unsigned own_step = *reinterpret_cast<const unsigned*>(block + pk_value_step<128>(4 * h + t, gp));
-          unsigned own_offset = *reinterpret_cast<const unsigned*>(block + pk_value_step<128>(4 * h + t, gp) + 16);
+          const uint4 steps = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0));
+          const uint4 offsets = *reinterpret_cast<const uint4*>(block + pk_value_step<128>(4 * h + t, 0) + 16);
+          unsigned s4[4] = {steps.x, steps.y, steps.z, steps.w}, o4[4] = {offsets.x, offsets.y, offsets.z, offsets.w};
           if (r0 < from || r0 + 16 > until) {
             const unsigned keep = (r >= from && r < until ? 0x0000ffffu : 0u) | (r + 1 >= from && r + 1 < until ? 0xffff0000u : 0u);
-            own_step &= keep;
-            own_offset &= keep;
-          }
-          own_step = pk_pack_half(pk_low(own_step) * value_scale, pk_high(own_step) * value_scale);
-          own_offset = pk_pack_half(pk_low(own_offset) * value_scale, pk_high(own_offset) * value_scale);
-          unsigned s4[4], o4[4];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            s4[g] = __shfl_sync(0xffffffffu, own_step, (lane & ~12) | g << 2);
-            o4[g] = __shfl_sync(0xffffffffu, own_offset, (lane & ~12) | g << 2);
+            for (int g = 0; g < 4; ++g) {
+              s4[g] &= keep;
+              o4[g] &= keep;
+            }
           }
           unsigned char* const at = dst + r * 128;
           const int turn = r & 7;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int c = 4 * g + gp;
-            unsigned lo[4], hi[4];
-            pk_half_values(lo4[g], s4[g], o4[g], lo);
-            pk_half_values(hi4[g], s4[g], o4[g], hi);
-            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + (((c & 7) ^ turn) << 4)) =
-                make_uint4(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410), __byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
-            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + 128 + (((c & 7) ^ (turn + 1)) << 4)) =
-                make_uint4(__byte_perm(lo[0], lo[1], 0x7632), __byte_perm(lo[2], lo[3], 0x7632), __byte_perm(hi[0], hi[1], 0x7632), __byte_perm(hi[2], hi[3], 0x7632));
+            uint4 even, odd;
+            pk_value_channels(lo4[g], hi4[g], s4[g], o4[g], even, odd);
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + (((c & 7) ^ turn) << 4)) = even;
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + 128 + (((c & 7) ^ (turn + 1)) << 4)) = odd;
           }
         }
         __syncwarp();                // every lane has read this block: another may come in its place
@@ -682,7 +621,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     // all lanes.
     {
       constexpr unsigned HALVES = PACKED ? (1u << 7) | (1u << 10) : 0u;      // (both operands' type: bits off, half precision)
-      constexpr unsigned IDESC_QK = tc_idesc(false) & ~HALVES, IDESC_PV = tc_idesc(true) & ~HALVES;
+      constexpr unsigned IDESC_QK = tc_idesc(false) & ~HALVES, IDESC_PV = tc_idesc(true);
       constexpr int KSTEP = BLOCK * 2 * 16;        // bytes between 16 positions' values
       const bool leader = elect_one();
       const int count0 = slot_tiles(0), count1 = slot_tiles(1);
@@ -836,7 +775,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
           tc_wait_st();
         }
       }
-      const float neg_shift = (PACKED ? TC_PACKED_LIFT : 0.0f) - (m_used == -INFINITY ? 0.0f : m_used);
+      const float neg_shift = m_used == -INFINITY ? 0.0f : -m_used;
       // Two probabilities a column, as the second product reads its A operand from tensor memory, over columns of S
       // that have been read; the product of the first 64 positions runs while the others are worked on.
       unsigned long long sums[4] = {0, 0, 0, 0};
@@ -844,11 +783,11 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       for (int half = 0; half < 2; ++half) {
         unsigned words[32];
         if (capped) {
-          tc_exponentials<true, true, PACKED>(tmem_s, 64 * half, words, sums, a.scale_over_cap, neg_shift, last, first, a.softcap_log2);
+          tc_exponentials<true, true>(tmem_s, 64 * half, words, sums, a.scale_over_cap, neg_shift, last, first, a.softcap_log2);
         } else if (open_tile) {
-          tc_exponentials<false, false, PACKED>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
+          tc_exponentials<false, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
         } else {
-          tc_exponentials<true, false, PACKED>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
+          tc_exponentials<true, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
         }
         tmem_st32(tmem_s + 32 * half, words);
         tc_wait_st();
@@ -865,9 +804,8 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     tc_fence_after_sync();
     // One more exponential: the sink, relative to the shift the row's sums were formed with (both in powers of two).
     auto with_sink = [&](float sum, float shift) {
-      return a.sinks != nullptr && shift > -INFINITY ? sum + exp2f(a.sinks[head] * 1.4426950408889634f - shift + (PACKED ? TC_PACKED_LIFT : 0.0f)) : sum;
+      return a.sinks != nullptr && shift > -INFINITY ? sum + exp2f(a.sinks[head] * 1.4426950408889634f - shift) : sum;
     };
-    auto unscale = [&] { return PACKED ? 1.0f / tc_packed_value_scale(value_top) : 1.0f; };      // (once the loaders' word is seen: behind a product, or the slots' barrier)
     // Each warp puts 32 rows x 64 columns into shared memory, 16-byte pieces permuted by the row so that neither the writes
     // (a thread a row) nor the reads (eight threads a row) meet in a bank, and then writes whole 128-byte row pieces, four rows
     // an instruction.  (A thread storing its own row's pieces touches 32 rows with every instruction, which cost 1.4 us a CTA.)
@@ -905,7 +843,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     if (!split) {
       // The slot's own queries are no longer read: its S are complete.
       if (!failed) {
-        const float l_row = with_sink(l_run, m_used), inv = (l_row > 0.0f ? 1.0f / l_row : 0.0f) * unscale();
+        const float l_row = with_sink(l_run, m_used), inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
         unsigned char* stage_out = smem + slot * Shape::Q_BYTES + (warp & 3) * 4096;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) store_half(stage_out, half, [&](float o, int) { return count > 0 ? o * inv : 0.0f; });
@@ -930,7 +868,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
                                                         __uint_as_float(v[4 * q4 + 2]), __uint_as_float(v[4 * q4 + 3]));
       }
       slots_meet();
-      const float l_row = with_sink(l_run * mine + note[slot ^ 1][r][1] * others, m), inv = (l_row > 0.0f ? 1.0f / l_row : 0.0f) * unscale();
+      const float l_row = with_sink(l_run * mine + note[slot ^ 1][r][1] * others, m), inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
       const float f_mine = mine * inv, f_others = others * inv;
       if (!abort_flag && !failed)
         store_half(smem + 65536 + warp * 4096, slot, [&](float o, int column) {
