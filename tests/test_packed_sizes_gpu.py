@@ -177,3 +177,69 @@ def test_prompts_over_values_of_other_sizes(ops, cuda_device, hd, tensor_memory,
     got = prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory) * 2.0 ** -power
     expected, bound = plain.attention(q.double().view(n, nh, hd), k, times(v, -power), context - n + torch.arange(n), hd ** -0.5, rounded=True)
     assert ((got - expected).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("nh", [4, 32])
+@pytest.mark.parametrize("power", [-90, -40, -16, -12, -5, 10, 12, 16, 24, 40, 90])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS + [(32, False)])
+def test_prompts_over_keys_of_any_size(ops, cuda_device, hd, tensor_memory, power, nh):
+    """Keys times a power of two under queries divided by it: the same scores."""
+    nkv, n, context, g = 2, 140, 333, torch.Generator().manual_seed(29)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys * 2.0 ** power, values)
+    q = (torch.randn((n, nh * hd), generator=g) * 2.0 ** -power).to(torch.bfloat16)
+    for masks in ({}, dict(window=90), dict(chunk=100, softcap=9.0)):
+        got = prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory, **masks)
+        expected, bound = plain.attention(q.double().view(n, nh, hd) * 2.0 ** power, times(k, -power), v, context - n + torch.arange(n), hd ** -0.5,
+                                          rounded=True, **masks)
+        assert ((got - expected).abs() <= bound).all(), masks
+
+
+@pytest.mark.parametrize("scale", [0.125, -0.1])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_prompts_over_positions_and_rows_of_several_sizes(ops, cuda_device, hd, tensor_memory, scale):
+    """Keys of one head far above one with queries far below, the other way round for the next; among the first's positions some whose
+    keys are 2^-30 of the others', and some that are zero."""
+    nh, nkv, n, context, g = 6, 3, 200, 300, torch.Generator().manual_seed(31)
+    size = torch.tensor([2.0 ** 35, 1.0, 2.0 ** -28]).view(1, 3, 1)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    keys[5::7, 0] *= 2.0 ** -30
+    keys[3::11] = 0.0
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys * size, values)
+    q = (torch.randn((n, nkv, nh // nkv, hd), generator=g) / size.view(1, 3, 1, 1)).to(torch.bfloat16)
+    got = prompt(ops, cuda_device, packed, table, q.view(n, -1), n, context, nh, nkv, hd, scale, tensor_memory)
+    unit = (k[0], k[1] / size.double(), k[2] / size.double())
+    expected, bound = plain.attention((q.double() * size.double().view(1, 3, 1, 1)).view(n, nh, hd), unit, v, context - n + torch.arange(n), scale, rounded=True)
+    assert ((got - expected).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("nh", [4, 32])
+@pytest.mark.parametrize("power", [-40, 13, 20, 50, 90])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_earlier_tokens_do_not_hang_on_later_ones_keys(ops, cuda_device, hd, tensor_memory, power, nh):
+    nkv, n, context, first, g = 2, 300, 420, 333, torch.Generator().manual_seed(37)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    loud = keys.clone()
+    loud[first:] *= 2.0 ** power
+    q, outs = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16), []
+    q[first - (context - n) + 5:] *= 2.0 ** power                     # (and rows of queries of that size)
+    for one in (keys, loud):
+        packed, table, _ = held_cache(ops, cuda_device, one, values)
+        outs.append(prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory))
+    before = first - (context - n)
+    assert torch.isfinite(outs[0][:before]).all() and torch.equal(outs[0][:before], outs[1][:before])
+
+
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_keys_that_are_not_finite_spoil_what_sees_them(ops, cuda_device, hd, tensor_memory):
+    """... and keys far out of the usual range beside them do not hide it."""
+    nh, nkv, n, context, first, g = 4, 2, 150, 200, 120, torch.Generator().manual_seed(41)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    keys[first - 3] *= 2.0 ** -40
+    keys[first, 0, 7] = math.nan
+    q = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16)
+    packed, table, _ = held_cache(ops, cuda_device, keys, values)
+    got = prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory)
+    spoiled = torch.zeros((n, nh), dtype=torch.bool)
+    spoiled[first - (context - n):, :2] = True
+    assert torch.equal(torch.isnan(got).all(-1), spoiled) and torch.equal(torch.isfinite(got).all(-1), ~spoiled)

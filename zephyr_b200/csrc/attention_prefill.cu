@@ -85,6 +85,9 @@ struct PrefillArgs {
 // with one group, 46 with two; 1024 tokens behind 2000, 16/8 heads of 64, 104 and 83).  Instructions bound it then: of some 800 a warp
 // and tile, scales that join a score in its exponent, 2^x without its range's ends and sums that are rescaled only where a maximum
 // moved took 150 (42 and 76 us).
+// A key's power of two (packed.cuh) is looked for where its row is made, and its inverse joins its scores in tiles that have one; the
+// queries' powers are found, and queries made half precision, in shared memory in front of the tiles, the inverses joining the scale
+// (2048 tokens, 16/8 heads of 64: 57.7 us without, 60.3; with the queries' part in registers inside the loop 61.7).
 template <int HD, bool PACKED>
 constexpr int PRE_GROUPS = PACKED && HD <= 96 ? 2 : 1;
 
@@ -149,6 +152,12 @@ paged_prefill_kernel(const PrefillArgs a) {
   unsigned char* const raw = reinterpret_cast<unsigned char*>(ring + 2 * STAGE);
   __shared__ long long raw_from_s[GROUPS][4][RAW_BLOCKS];
   auto& raw_from = raw_from_s[group];
+  // Of a tile some of whose scores are to be multiplied by something: its number, and a position's factor beside that number.
+  __shared__ int2 key_factor_s[GROUPS][2][PRE_BN];
+  __shared__ int factors_of_s[GROUPS][2];
+  __shared__ float row_scale_s[PRE_BM];      // the scale, and with it what a query's power of two leaves to be taken out
+  if (PACKED && tid < PRE_BN) key_factor_s[group][0][tid].x = key_factor_s[group][1][tid].x = -1;
+  if (PACKED && tid < 2) factors_of_s[group][tid] = -1;
   auto look_up = [&](int block) {    // counted from the first tile's first
     const int pos = first_tile + block * PK_BLOCK;
     if (pos >= hi || pos + PK_BLOCK <= lo) return -1LL;
@@ -178,10 +187,27 @@ paged_prefill_kernel(const PrefillArgs a) {
       const int j = e / CHUNKS, c = e - j * CHUNKS, p = j & (PK_BLOCK - 1);
       const unsigned char* const block = blocks + (j >> 4) * pk_block_bytes(HD);
       const bool ok = raw_from[i & 3][j >> 4] >= 0 && k0 + j >= lo && k0 + j < hi;
-      const unsigned short* const params = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
+      const unsigned short* const own = reinterpret_cast<const unsigned short*>(block + pk_key_step<HD>(p, c >> 2));
+      float step = pk_low(own[0]), offset = pk_low(own[HD / 32]);
+      unsigned params[HD / 32];              // all of the position's
+      if constexpr (HD == 96) {              // (rows of 12 bytes)
+#pragma unroll
+        for (int n = 0; n < 3; ++n) params[n] = reinterpret_cast<const unsigned*>(block + pk_key_step<HD>(p, 0))[n];
+      } else {
+        pk_load_words(params, block + pk_key_step<HD>(p, 0));
+      }
+      const unsigned top = pk_largest(params);
+      if (__builtin_expect(!pk_half_usual<PK_KEYS_TO>(top) && ok, 0)) {
+        const float power = pk_half_power<PK_KEYS_TO>(top);
+        if (power != 1.0f) {                 // (all of the position's threads write the same)
+          step *= power;
+          offset *= power;
+          key_factor_s[group][i & 1][j] = make_int2(i, __float_as_int(pk_inverse_power(power)));
+          factors_of_s[group][i & 1] = i;
+        }
+      }
       *reinterpret_cast<uint4*>(ks + j * KROW + c * 8) =
-          ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_half_twice(pk_low(params[0])), pk_half_twice(pk_low(params[HD / 32])))
-             : zeros;
+          ok ? pk_key_channels(*reinterpret_cast<const unsigned*>(block + pk_key_word<HD>(p, c & 3, c >> 2)), pk_half_twice(step), pk_half_twice(offset)) : zeros;
     }
     for (int e = tid; e < PRE_BN / 2 * CHUNKS; e += PRE_WARPS * 32) {
       const int pair = e / CHUNKS, c = e - pair * CHUNKS, j = 2 * pair, own = pair & (PK_BLOCK / 2 - 1);
@@ -249,6 +275,28 @@ paged_prefill_kernel(const PrefillArgs a) {
     cp_async_wait<1>();
     __syncthreads();
     expand(0);
+    // The queries, as half-precision values too: several neighbouring threads a row.
+    constexpr int PER_ROW = GROUPS * PRE_WARPS * 32 / PRE_BM, WORDS = HD / 2 / PER_ROW;
+    const int r = threadIdx.x / PER_ROW;
+    uint4* const at = reinterpret_cast<uint4*>(q_s + r * KROW + threadIdx.x % PER_ROW * (2 * WORDS));
+    unsigned words[WORDS];
+#pragma unroll
+    for (int n = 0; n < WORDS; n += 4) {
+      const uint4 v = at[n / 4];
+      words[n] = v.x; words[n + 1] = v.y; words[n + 2] = v.z; words[n + 3] = v.w;
+    }
+    unsigned top = pk_largest(words);
+#pragma unroll
+    for (int x = 1; x < PER_ROW; x <<= 1) top = pk_larger(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float power = pk_half_power<PK_QUERIES_TO>(top);
+    if (power != 1.0f) {
+#pragma unroll
+      for (int n = 0; n < WORDS; ++n) words[n] = pk_times(words[n], power);
+    }
+#pragma unroll
+    for (int n = 0; n < WORDS; n += 4) at[n / 4] = make_uint4(pk_to_half(words[n]), pk_to_half(words[n + 1]), pk_to_half(words[n + 2]), pk_to_half(words[n + 3]));
+    row_scale_s[r] = (a.softcap_log2 > 0.0f ? a.scale_over_cap : a.scale_log2) * pk_inverse_power(power);
+    __syncthreads();
   }
 
   // This warp's 16 query rows; this lane's two rows sit at positions qpos[0] and qpos[1].
@@ -277,11 +325,12 @@ paged_prefill_kernel(const PrefillArgs a) {
   }
   // PACKED: the scale joins a score in its exponent, where scores have no bound and the scale keeps their order.
   const bool late_scale = PACKED && a.softcap_log2 == 0.0f && a.scale_log2 > 0.0f;
-  const float late = late_scale ? a.scale_log2 : 1.0f;
+  auto row_scale = [&](int h) { return row_scale_s[warp_row0 + quad_row + 8 * h]; };
   // A raw score of this lane's row h whose key lies at `pos`, scaled, bounded and biased.
   auto finished = [&](float raw, int h, int pos) {
     if (late_scale) return raw;
-    float v = a.softcap_log2 > 0.0f ? a.softcap_log2 * tanhf(raw * a.scale_over_cap) : raw * a.scale_log2;
+    float v = a.softcap_log2 > 0.0f ? a.softcap_log2 * tanhf(raw * (PACKED ? row_scale(h) : a.scale_over_cap))
+                                    : raw * (PACKED ? row_scale(h) : a.scale_log2);
     if (DISTANT) v = fmaf(-r1[h], __log2f(fmaf(r2[h], static_cast<float>(qpos[h] - pos), 1.0f)), v);
     return v;
   };
@@ -310,12 +359,6 @@ paged_prefill_kernel(const PrefillArgs a) {
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         ldmatrix_x4(qa[ks], q_s + (warp_row0 + (lane & 7) + ((lane >> 3) & 1) * 8) * KROW + ks * 16 + (lane >> 4) * 8);
-      if (PACKED) {                  // keys are half-precision values there
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) qa[ks][i] = pk_to_half(qa[ks][i]);
-      }
     }
     const int run = t < pool_tiles ? 0 : (t < pool_tiles + kept_tiles ? 1 : 2);
     const int k0 = run == 0 ? t * PRE_BN : (run == 1 ? (t - pool_tiles) * PRE_BN
@@ -345,6 +388,17 @@ paged_prefill_kernel(const PrefillArgs a) {
           mma_bf16_16816(s[i], qa[2 * kk + 1], b[2], b[3]);
         }
       }
+    }
+    if (PACKED && __builtin_expect(factors_of_s[group][t / GROUPS & 1] == t / GROUPS, 0)) {
+#pragma unroll
+      for (int i = 0; i < NTS; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int2 factor = key_factor_s[group][t / GROUPS & 1][i * 8 + quad_col + c];
+          const float by = factor.x == t / GROUPS ? __int_as_float(factor.y) : 1.0f;
+          s[i][c] *= by;
+          s[i][2 + c] *= by;
+        }
     }
 
     float tile_max[2] = {-INFINITY, -INFINITY};
@@ -383,12 +437,15 @@ paged_prefill_kernel(const PrefillArgs a) {
         }
       }
     }
-    float corr[2], m_use[2];
+    float corr[2], m_use[2], late[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       tile_max[h] = fmaxf(tile_max[h], __shfl_xor_sync(0xffffffffu, tile_max[h], 1));
       tile_max[h] = fmaxf(tile_max[h], __shfl_xor_sync(0xffffffffu, tile_max[h], 2));
-      if (PACKED) tile_max[h] *= late;
+      if (PACKED) {
+        late[h] = late_scale ? row_scale(h) : 1.0f;
+        tile_max[h] *= late[h];
+      }
       const float new_m = fmaxf(m_run[h], tile_max[h]);
       m_use[h] = new_m == -INFINITY ? 0.0f : new_m;      // a row that has seen no key yet: keep exp2 finite
       corr[h] = exp2f(m_run[h] - m_use[h]);              // 0 while the running maximum is -inf
@@ -399,7 +456,7 @@ paged_prefill_kernel(const PrefillArgs a) {
     for (int i = 0; i < NTS; ++i) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        s[i][c] = PACKED ? pk_exp2(fmaf(s[i][c], late, -m_use[c >> 1])) : exp2f(s[i][c] - m_use[c >> 1]);
+        s[i][c] = PACKED ? pk_exp2(fmaf(s[i][c], late[c >> 1], -m_use[c >> 1])) : exp2f(s[i][c] - m_use[c >> 1]);
         row_sum[c >> 1] += s[i][c];
       }
     }
@@ -678,9 +735,9 @@ ZB_API int zb_paged_prefill_packed(const void* call) {
   a.max_blocks = max_blocks; a.page_size = page_size; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
   a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk; a.sinks = c.sinks;
-  a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
+  a.scale_log2 = scale * 1.4426950408889634f;
   a.softcap_log2 = softcap * 1.4426950408889634f;
-  a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
+  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
   a.status = c.status;
   const auto s = static_cast<cudaStream_t>(c.stream);
   switch (hd) {

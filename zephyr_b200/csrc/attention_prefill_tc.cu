@@ -259,6 +259,7 @@ constexpr int TC_PACKED_PART = pk_block_bytes(128) / 2;         // a block's key
 constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_PART;
 constexpr int TC_PACKED_SOFTMAX_REGISTERS = 152, TC_PACKED_OTHER_REGISTERS = 104;
 static_assert(TC_PACKED_SMEM <= 223 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
+static_assert(TC_PACKED_THREADS == 4 * TC_BN, "a thread a position of four tiles");
 static_assert(256 * (TC_PACKED_SOFTMAX_REGISTERS + TC_PACKED_OTHER_REGISTERS) <= TC_PACKED_THREADS * 128, "no more registers than at launch");
 
 template <int FORM, int HD, bool SHARED, bool PACKED = false>
@@ -283,9 +284,16 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   __shared__ unsigned long long edge_full;              // the pages of a tile at an edge have landed
   __shared__ unsigned tmem_base_s;
   __shared__ volatile int abort_flag;
+  // PACKED: of a tile some of whose scores are to be multiplied by something, its number, and a position's factor beside that number; of
+  // four tiles.  (Before the keys of tile j are made the products over those of j - 2, whose stage they take, are complete, and these follow
+  // the softmax of j - 3, or where slots take turns of j - 4: no softmax reads tile j - 4 any more.)
+  __shared__ int2 key_factors[4][PACKED ? TC_BN : 1];
+  __shared__ int factored[4];
 
+  if (PACKED) key_factors[threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0].x = -1;
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    if (PACKED) factored[0] = factored[1] = factored[2] = factored[3] = -1;
     for (int b = 0; b < STAGES; ++b) {
       mbar_init(&kv_full[b], PACKED ? 2 : Shape::KIND_WARPS);
       mbar_init(&kv_empty[b], 1);
@@ -447,7 +455,16 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
           for (int i = 0; i < 2; ++i) {
             const int p = 8 * i + spread, r = r0 + p;
             const uint4 words = *reinterpret_cast<const uint4*>(source + pk_key_word<128>(p, t, 0));
-            const uint4 params = *reinterpret_cast<const uint4*>(source + pk_key_step<128>(p, 0));
+            uint4 params = *reinterpret_cast<const uint4*>(source + pk_key_step<128>(p, 0));
+            const unsigned all_params[4] = {params.x, params.y, params.z, params.w}, top = pk_largest(all_params);
+            if (__builtin_expect(!pk_half_usual<PK_KEYS_TO>(top) && r >= from && r < until, 0)) {
+              const float power = pk_half_power<PK_KEYS_TO>(top);
+              if (power != 1.0f) {             // (all of the position's lanes write the same)
+                params = make_uint4(pk_times(params.x, power), pk_times(params.y, power), pk_times(params.z, power), pk_times(params.w, power));
+                key_factors[j & 3][r] = make_int2(j, __float_as_int(pk_inverse_power(power)));
+                factored[j & 3] = j;
+              }
+            }
             const unsigned w[4] = {words.x, words.y, words.z, words.w}, s2[2] = {params.x, params.y}, o2[2] = {params.z, params.w};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -689,6 +706,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     // --------------------------------------------------------------------------- the softmax
     const int slot = warp >> 2, r = threadIdx.x & (TC_BM - 1);
     const int head = split ? head0 : head0 + slot;
+    float query_power = 1.0f;
     // The queries, rows past the tile's tokens zero: a slot's head each, or half of the one head's values each.
     {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(tok0 + (r < n_tok ? r : 0)) * a.nh + head) * HD);
@@ -696,21 +714,34 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       constexpr int HALF = CHUNKS / 2;
       const int from = split && slot == 1 ? HALF : 0, until = split && slot == 0 ? HALF : CHUNKS;
       const int turn = kv_swizzle(r, CHUNKS);
+      // (PACKED: once more, times the row's power of two, where a row's largest channel says so.)
+      bool again = false;
+      do {
+        unsigned top = 0u;
 #pragma unroll
-      for (int c0 = 0; c0 < CHUNKS; c0 += HALF) {
-        if (c0 < from || c0 >= until) continue;
-        uint4 v[HALF];
+        for (int c0 = 0; c0 < CHUNKS; c0 += HALF) {
+          const bool own = c0 >= from && c0 < until;
+          if (!own && (!PACKED || again)) continue;
+          uint4 v[HALF];
 #pragma unroll
-        for (int c = 0; c < HALF; ++c) v[c] = r < n_tok ? src[c0 + c] : make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < HALF; ++c) v[c] = r < n_tok ? src[c0 + c] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int c = 0; c < HALF; ++c) {
-          const int stored = (c0 + c) ^ turn;
-          if (PACKED)
-            v[c] = make_uint4(pk_to_half(__byte_perm(v[c].x, v[c].z, 0x5410)), pk_to_half(__byte_perm(v[c].x, v[c].z, 0x7632)),
-                              pk_to_half(__byte_perm(v[c].y, v[c].w, 0x5410)), pk_to_half(__byte_perm(v[c].y, v[c].w, 0x7632)));
-          *reinterpret_cast<uint4*>(dst + (stored / BLOCK_CHUNKS) * BLOCK_BYTES + r * (BLOCK * 2) + (stored % BLOCK_CHUNKS) * 16) = v[c];
+          for (int c = 0; c < HALF; ++c) {
+            if (PACKED && !again) top = pk_larger(pk_larger(top, v[c].x), pk_larger(v[c].y, pk_larger(v[c].z, v[c].w)));
+            const int stored = (c0 + c) ^ turn;
+            if (PACKED && again)
+              v[c] = make_uint4(pk_times(v[c].x, query_power), pk_times(v[c].y, query_power), pk_times(v[c].z, query_power), pk_times(v[c].w, query_power));
+            if (PACKED)
+              v[c] = make_uint4(pk_to_half(__byte_perm(v[c].x, v[c].z, 0x5410)), pk_to_half(__byte_perm(v[c].x, v[c].z, 0x7632)),
+                                pk_to_half(__byte_perm(v[c].y, v[c].w, 0x5410)), pk_to_half(__byte_perm(v[c].y, v[c].w, 0x7632)));
+            if (own) *reinterpret_cast<uint4*>(dst + (stored / BLOCK_CHUNKS) * BLOCK_BYTES + r * (BLOCK * 2) + (stored % BLOCK_CHUNKS) * 16) = v[c];
+          }
         }
-      }
+        if (!PACKED || again) break;
+        const unsigned tops[1] = {top};
+        query_power = pk_half_power<PK_QUERIES_TO>(pk_largest(tops));
+        again = __any_sync(0xffffffffu, query_power != 1.0f);
+      } while (again);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) tc_mbar_arrive(q_full);
@@ -720,6 +751,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     const int qp = ctx + q0 + r;
     float m_used = -INFINITY, l_run = 0.0f;
     const bool capped = !BIASED_SCORES && a.softcap_log2 > 0.0f;
+    const float score_scale = (capped ? a.scale_over_cap : a.scale_log2) * (PACKED ? pk_inverse_power(query_power) : 1.0f);
     const float r1 = BIASED_SCORES ? a.bias_r1[head] : 0.0f, r2 = BIASED_SCORES ? a.bias_r2[head] : 0.0f;
     bool failed = false;
     // With a chunk: the last position that this row's window and chunk leave out, and the first key that all rows of the CTA see.
@@ -749,10 +781,30 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       const int at = qp - k0;
       const int after = in_kept ? -1 : CHUNKED ? passed - k0 : a.window > 0 ? qp - a.window - k0 : -(1 << 30);
       const int last = min(qp, run_hi(j) - 1) - k0, first = max(run_lo(j) - k0, after + 1);
-      const float raw_max = open_tile ? tc_row_max<false, BIASED_SCORES>(tmem_s, last, first, a.scale_log2, at, r1, r2)
-                                      : tc_row_max<true, BIASED_SCORES>(tmem_s, last, first, a.scale_log2, at, r1, r2);
+      int factors_of = PACKED ? factored[j & 3] : -1;
+      float raw_max;
+      do {
+        raw_max = open_tile ? tc_row_max<false, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2)
+                            : tc_row_max<true, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2);
+        if (!PACKED || __builtin_expect(factors_of != j, 1)) break;
+        // Once more, with the scores times their factors.  (Asked behind the first: a look at the flag in front of it cost 2 %.)
+        factors_of = -1;
+#pragma unroll 1
+        for (int c = 0; c < TC_BN; c += 32) {
+          unsigned v[32];
+          tmem_ld32(tmem_s + c, v);
+          tmem_wait_ld32(v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int2 factor = key_factors[j & 3][PACKED ? c + e : 0];
+            if (factor.x == j) v[e] = __float_as_uint(__uint_as_float(v[e]) * __int_as_float(factor.y));
+          }
+          tmem_st32(tmem_s + c, v);
+        }
+        tc_wait_st();
+      } while (true);
       // The scale is positive and the bound grows with its argument: the largest raw score gives the largest exponent.
-      const float row_max = capped ? a.softcap_log2 * tanh_from_exp2(raw_max * a.scale_over_cap) : BIASED_SCORES ? raw_max : raw_max * a.scale_log2;
+      const float row_max = capped ? a.softcap_log2 * tanh_from_exp2(raw_max * score_scale) : BIASED_SCORES ? raw_max : raw_max * score_scale;
       const bool grow = raw_max > -INFINITY && (row_max > m_used + TC_RESCALE_THRESHOLD || m_used == -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
         // Some row of the warp moves its shift: every lane takes part in the tensor-memory
@@ -783,11 +835,11 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       for (int half = 0; half < 2; ++half) {
         unsigned words[32];
         if (capped) {
-          tc_exponentials<true, true>(tmem_s, 64 * half, words, sums, a.scale_over_cap, neg_shift, last, first, a.softcap_log2);
+          tc_exponentials<true, true>(tmem_s, 64 * half, words, sums, score_scale, neg_shift, last, first, a.softcap_log2);
         } else if (open_tile) {
-          tc_exponentials<false, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
+          tc_exponentials<false, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
         } else {
-          tc_exponentials<true, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : a.scale_log2, neg_shift, last, first, 0.0f);
+          tc_exponentials<true, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
         }
         tmem_st32(tmem_s + 32 * half, words);
         tc_wait_st();
@@ -1076,9 +1128,9 @@ ZB_API int zb_paged_prefill_tc_packed(const void* call) {
   a.max_blocks = max_blocks; a.num_pages = num_pages; a.num_rows = num_rows;
   a.page_shift = page_shift;
   a.nh = nh; a.nkv = nkv; a.window = window; a.chunk = chunk;
-  a.scale_log2 = scale * 1.4426950408889634f * PK_KEY_UNSCALE;
+  a.scale_log2 = scale * 1.4426950408889634f;
   a.softcap_log2 = softcap * 1.4426950408889634f;
-  a.scale_over_cap = softcap > 0.0f ? scale * PK_KEY_UNSCALE / softcap : 0.0f;
+  a.scale_over_cap = softcap > 0.0f ? scale / softcap : 0.0f;
   a.sinks = c.sinks;
   a.status = c.status;
   const auto s = static_cast<cudaStream_t>(c.stream);

@@ -86,15 +86,43 @@ __device__ __forceinline__ void pk_load_words(unsigned (&w)[N], const unsigned c
 __device__ __forceinline__ float pk_low(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float pk_high(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// ---- Keys for a prompt's products, as half-precision values times 2^-6: three bits more than bfloat16's eight, since what a key is off
-// by moves all of a query's weights (at most 2^-11 of a value here; with bfloat16 keys a prompt's result was 0.0054 off where the weights' and
-// the results' own roundings make 0.0025).  Keys up to 2^22 and queries up to 65504 fit; what is below 2^-19 is off by up to that.
-constexpr float PK_KEY_SCALE = 0.015625f, PK_KEY_UNSCALE = 64.0f;
+// ---- Keys and queries for a prompt's products, as half-precision values: three bits more than bfloat16's eight, since what a key is off
+// by moves all of a query's weights (at most 2^-12 of a value here; with bfloat16 keys a prompt's result was 0.0054 off where the weights' and
+// the results' own roundings make 0.0025).  What half precision lacks is range.  So a position whose largest step or offset is not
+// 2^-5 to 2^11 (or zero), and a query whose largest channel is not 2^-5 to 2^15, is held times a power of two of its own that takes it to
+// the upper end, and its scores are multiplied by the power's inverse.  A channel is then off by 2^-12 of it or 2^-15 of the largest of
+// the position's, whichever is more.
+constexpr unsigned PK_HALF_FROM = 0x3d00u, PK_KEYS_TO = 0x4500u, PK_QUERIES_TO = 0x4700u;      // 2^-5, 2^11, 2^15 as bfloat16
 
-// A key's step or offset (bfloat16) on that scale, twice.
+// The larger magnitudes of two words' bfloat16 values, half by half, with some sign (a NaN's is not counted).
+__device__ __forceinline__ unsigned pk_larger(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// The largest magnitude of the words' values, as bits in both halves.
+template <int N>
+__device__ __forceinline__ unsigned pk_largest(const unsigned (&w)[N]) {
+  unsigned top = w[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = pk_larger(top, w[i]);
+  return pk_larger(top, __byte_perm(top, 0u, 0x1032)) & 0x7fff7fffu;
+}
+// Whether a position or query whose largest magnitude that is needs no power of two; and its power (one where it is zero or infinite).
+template <unsigned TO>
+__device__ __forceinline__ bool pk_half_usual(unsigned top) { return top - PK_HALF_FROM * 0x10001u < (TO - PK_HALF_FROM) * 0x10001u; }
+template <unsigned TO>
+__device__ __forceinline__ float pk_half_power(unsigned top) {
+  const unsigned bits = top & 0xffffu;
+  if (pk_half_usual<TO>(top) || bits == 0u || bits >= 0x7f80u) return 1.0f;
+  return __uint_as_float(min(127u + (TO >> 7) - 1u - (bits >> 7), 253u) << 23);
+}
+__device__ __forceinline__ float pk_inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+
+// A key's step or offset, twice.
 __device__ __forceinline__ unsigned pk_half_twice(float v) {
   unsigned r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %1;\n" : "=r"(r) : "f"(v * PK_KEY_SCALE));
+  asm("cvt.rn.f16x2.f32 %0, %1, %1;\n" : "=r"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ unsigned pk_fma_f16x2(unsigned a, unsigned b, unsigned c) {
@@ -123,8 +151,9 @@ __device__ __forceinline__ unsigned pk_pack_half(float low, float high) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(high), "f"(low));
   return r;
 }
-// Two bfloat16 values as half-precision ones (exact from 2^-17 on; beyond 65504 infinite).
+// Two bfloat16 values as half-precision ones, and times a power of two.
 __device__ __forceinline__ unsigned pk_to_half(unsigned pair) { return pk_pack_half(pk_low(pair), pk_high(pair)); }
+__device__ __forceinline__ unsigned pk_times(unsigned pair, float power) { return pack_bf16(pk_low(pair) * power, pk_high(pair) * power); }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
