@@ -243,3 +243,37 @@ def test_keys_that_are_not_finite_spoil_what_sees_them(ops, cuda_device, hd, ten
     spoiled = torch.zeros((n, nh), dtype=torch.bool)
     spoiled[first - (context - n):, :2] = True
     assert torch.equal(torch.isnan(got).all(-1), spoiled) and torch.equal(torch.isfinite(got).all(-1), ~spoiled)
+
+
+@pytest.mark.parametrize("powers", [(0, 40), (40, 0), (-60, 0, -20), (0, -60), (-90, -30, 20, 80), (80, -90, 0), (None, -50, 10), (None, None, 60)])
+@pytest.mark.parametrize("masks", [{}, dict(window=120), dict(chunk=200, softcap=7.0, sinks=True), dict(sinks=True)])
+@pytest.mark.parametrize("hd,tensor_memory", KERNELS)
+def test_prompts_over_values_of_several_sizes(ops, cuda_device, hd, tensor_memory, masks, powers):
+    """Runs of positions whose values differ in size (None: zeros), none of which begins where a tile does; keys of other sizes among them.
+    Every row is held against the largest that it sees."""
+    nh, nkv, n, context, g = 6, 2, 300, 420, torch.Generator().manual_seed(43)
+    keys, values = torch.randn((context, nkv, hd), generator=g), torch.randn((context, nkv, hd), generator=g)
+    keys[3::17] *= 2.0 ** -30
+    run = -(-context // len(powers)) + 5
+    size = torch.full((context,), -1000)
+    for i, power in enumerate(powers):
+        values[i * run:(i + 1) * run] *= 0.0 if power is None else 2.0 ** power
+        size[i * run:(i + 1) * run] = -1000 if power is None else power
+    masks = dict(masks)
+    sinks = torch.randn(nh, generator=g) if masks.pop("sinks", False) else None
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys, values)
+    q = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16)
+    got = prompt(ops, cuda_device, packed, table, q, n, context, nh, nkv, hd, hd ** -0.5, tensor_memory, **masks,
+                 sinks=None if sinks is None else sinks.to(cuda_device))
+    pos = context - n + torch.arange(n)
+    lowest = torch.zeros_like(pos)
+    if masks.get("window"):
+        lowest = torch.maximum(lowest, pos + 1 - masks["window"])
+    if masks.get("chunk"):
+        lowest = torch.maximum(lowest, pos // masks["chunk"] * masks["chunk"])
+    most = torch.stack([size[lo:p + 1].max() for lo, p in zip(lowest.tolist(), pos.tolist())])
+    for power in most.unique().tolist():
+        rows, by = most == power, 0 if power == -1000 else power
+        expected, bound = plain.attention(q[rows].double().view(-1, nh, hd), k, times(v, -by), pos[rows], hd ** -0.5, sinks=sinks, rounded=True, **masks)
+        # (What no row of these sees may be far out of range on their scale.)
+        assert ((got[rows] * 2.0 ** -by - expected).abs() <= bound).all(), power

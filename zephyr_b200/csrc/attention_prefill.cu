@@ -197,8 +197,8 @@ paged_prefill_kernel(const PrefillArgs a) {
         pk_load_words(params, block + pk_key_step<HD>(p, 0));
       }
       const unsigned top = pk_largest(params);
-      if (__builtin_expect(!pk_half_usual<PK_KEYS_TO>(top) && ok, 0)) {
-        const float power = pk_half_power<PK_KEYS_TO>(top);
+      if (__builtin_expect(!pk_half_usual<PK_HELD_TO>(top) && ok, 0)) {
+        const float power = pk_half_power<PK_HELD_TO>(top);
         if (power != 1.0f) {                 // (all of the position's threads write the same)
           step *= power;
           offset *= power;

@@ -209,7 +209,7 @@ __device__ __forceinline__ float tc_row_max(unsigned tmem_row, int last, int fir
 // 64 columns (from `column0` on) of a row of S -> probabilities exp2(s * scale + neg_shift) as 32 words of two bfloat16 each,
 // and their sums on top of `sums`.  CAPPED: the exponent is cap_log2 * tanh(s * scale) + neg_shift, `scale` then being
 // scale / softcap.
-template <bool MASKED, bool CAPPED>
+template <bool MASKED, bool CAPPED, bool HALVES>
 __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, unsigned (&words)[32], unsigned long long (&sums)[4],
                                                 float scale, float neg_shift, int last, int first, float cap_log2) {
   const unsigned long long scale2 = pack_f32x2(scale, scale), shift2 = pack_f32x2(neg_shift, neg_shift);
@@ -235,7 +235,7 @@ __device__ __forceinline__ void tc_exponentials(unsigned tmem_row, int column0, 
         p[e] = !MASKED || (column <= last && column >= first) ? exp2_approx(x[e]) : 0.0f;
       }
       sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(p[0], p[1]));
-      words[16 * c + (i >> 1)] = pack_bf16(p[0], p[1]);
+      words[16 * c + (i >> 1)] = HALVES ? pk_pack_half(p[0], p[1]) : pack_bf16(p[0], p[1]);
     }
   }
 }
@@ -246,21 +246,111 @@ enum { TC_FORM_PLAIN, TC_FORM_BIASED, TC_FORM_CHUNKED, TC_FORM_KEPT };      // K
 // PACKED: over a 4-bit cache (packed.cuh), whose blocks six loader warps copy and turn into the ring's rows: two warps an item, three
 // items at a time; the softmax warps take registers over from the others.  Some 4000 instructions a tile of keys and values, half of what
 // the softmax of a pair of heads takes, are issued between that softmax's own, and bound the kernel with it: 1024 tokens behind 7000,
-// 32/8 heads, 171 us (738 TFLOP/s) where the cache in bfloat16 takes 142; 8192 new tokens 659 against 530.
+// 32/8 heads, 175 us (722 TFLOP/s) where the cache in bfloat16 takes 142.  Softmax and loaders share the instruction cache: with both
+// halves of a tile's weights unrolled, as the other forms have them, the same took 190 us, and warps waited for instructions half as much
+// again.
 // Keys are half-precision values (packed.cuh), a key's channels lie in the order in which its words give them (0 4 1 5 2 6 3 7 of every
-// eight), and the queries' in the same.  Values and weights are bfloat16, whose range no position's size takes from another's.  (Half
-// precision, off by a third less, 0.0017 against 0.0027 of the result, wants one power of two for all values in the CTA's sight: a value
-// that a query does not see, 2^27 and more times larger, then took bits from those that it does.)
+// eight), and the queries' in the same.  Values and weights are half-precision ones too: with both in bfloat16 a result is off by
+// 0.0027 of it where its own rounding makes 0.0017 (and the above takes 162 us).  Weights carry 2^7, so that one of 2^-21 keeps its bits.
+// A position's key and value, and a query, hold any size by powers of two of their own (packed.cuh).  A key's joins its scores.  A value's,
+// 2^-f, leaves 2^f to its weight beside others, which the shift of a row's softmax bounds with them: it follows the largest score + f that
+// the row sees; the sum of the weights has them without.  A row that sees no such position is what it is without them, bit by bit.
+// Positions that have powers are noted with the tile's keys, whose copies bring the values' parameters along; tiles without one cost a look
+// at a flag.
 constexpr int TC_PACKED_THREADS = 512;             // warps 9 .. 14 load, the last one has nothing to do
 constexpr int TC_PACKED_STAGES = 4;
 constexpr int TC_PACKED_TEAMS = 3;
 constexpr int TC_PACKED_AHEAD = 3;                 // blocks of 16 positions that a warp has copied, the one that it works on among them
 constexpr int TC_PACKED_PART = pk_block_bytes(128) / 2;         // a block's keys, or its values
-constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_PART;
+constexpr int TC_PACKED_COPY = TC_PACKED_PART + 256;            // with the keys the values' steps and offsets
+constexpr int TC_PACKED_SMEM = 2 * TC_BM * 128 * 2 + TC_PACKED_STAGES * TC_BN * 128 * 2 + TC_PACKED_TEAMS * 2 * TC_PACKED_AHEAD * TC_PACKED_COPY;
+constexpr float TC_PACKED_LIFT = 7.0f;               // (32768 for a probability that has passed its row's shift by all it may)
 constexpr int TC_PACKED_SOFTMAX_REGISTERS = 152, TC_PACKED_OTHER_REGISTERS = 104;
-static_assert(TC_PACKED_SMEM <= 223 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
+static_assert(TC_PACKED_SMEM <= 219 * 1024, "the queries, the ring and the copies fit an SM's shared memory");
 static_assert(TC_PACKED_THREADS == 4 * TC_BN, "a thread a position of four tiles");
 static_assert(256 * (TC_PACKED_SOFTMAX_REGISTERS + TC_PACKED_OTHER_REGISTERS) <= TC_PACKED_THREADS * 128, "no more registers than at launch");
+
+// A position's note: its tile (of 2^31 positions' 2^24) beside the exponent of a power of two; and the exponent that a note has for a tile.
+__device__ __forceinline__ unsigned tc_packed_note(int tile, int exponent) { return static_cast<unsigned>(tile) << 8 | static_cast<unsigned>(exponent + 128); }
+__device__ __forceinline__ int tc_packed_exponent(unsigned note, int tile) { return note >> 8 == static_cast<unsigned>(tile) ? static_cast<int>(note & 255u) - 128 : 0; }
+// Whether one of the halves is too large to be held as it is, or (`small`) too small.
+__device__ __forceinline__ bool tc_packed_unusual(unsigned top, bool small) {
+  top &= 0x7fff7fffu;
+  const unsigned from = top + (small ? (0x8000u - PK_HALF_FROM) * 0x10001u : 0x80008000u);
+  return ((top + (0x8000u - PK_HELD_TO) * 0x10001u | ~from) & 0x80008000u) != 0u;
+}
+// A sum of weights on a shift that moved by `by` (factor: 2^by).  Where values' powers moved it by more than float32's exponents, what the
+// factor says of sums, nothing, does not hold of weights, which count whatever their values are.
+__device__ __forceinline__ float tc_packed_rescaled(float sum, float by, float factor) {
+  if (!(by <= -100.0f) || by == -INFINITY) return sum * factor;
+  const float half = exp2f(0.5f * by);
+  return sum * half * half;
+}
+// What a tile asks for in which some position has a power: its row's largest exponent, the exponents of values taken in ...
+struct TcPackedRow {
+  unsigned tmem_s;
+  const unsigned* notes;             // the tile's keys'; its values' 4 TC_BN further
+  int tile, last, first;
+  float score_scale, softcap_log2;
+  __device__ __forceinline__ float exponent(float raw, float shift) const {
+    return softcap_log2 > 0.0f ? fmaf(softcap_log2, tanh_from_exp2(raw * score_scale), shift) : fmaf(raw, score_scale, shift);
+  }
+};
+__device__ __noinline__ float tc_packed_row_max(const TcPackedRow a) {
+  float raw_max = -INFINITY, other_max = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < TC_BN; c += 16) {
+    unsigned v[16];
+    tmem_ld16(a.tmem_s + c, v);
+    tmem_wait_ld16(v);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int key = tc_packed_exponent(a.notes[c + e], a.tile), value = tc_packed_exponent(a.notes[4 * TC_BN + c + e], a.tile);
+      const float raw = __uint_as_float(v[e]) * pk_power(-key);
+      if (c + e > a.last || c + e < a.first) continue;
+      if (value == 0) raw_max = fmaxf(raw_max, raw);
+      else other_max = fmaxf(other_max, a.exponent(raw, static_cast<float>(-value)));
+    }
+  }
+  // (As without powers where no value has one.)
+  const float usual = a.softcap_log2 > 0.0f ? a.softcap_log2 * tanh_from_exp2(raw_max * a.score_scale) : raw_max * a.score_scale;
+  return fmaxf(raw_max > -INFINITY ? usual : -INFINITY, other_max);
+}
+// ... and its weights, whose sum without the values' powers comes back.
+__device__ __noinline__ float tc_packed_weights(const TcPackedRow a, float neg_shift, unsigned long long* p_full) {
+  unsigned long long sums[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int c = 0; c < TC_BN; c += 16) {
+    unsigned v[16], words[8];
+    tmem_ld16(a.tmem_s + c, v);
+    tmem_wait_ld16(v);
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      float p[2], counted[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int column = c + e + u, key = tc_packed_exponent(a.notes[column], a.tile), value = tc_packed_exponent(a.notes[4 * TC_BN + column], a.tile);
+        const float raw = __uint_as_float(v[e + u]) * pk_power(-key);
+        const bool visible = column <= a.last && column >= a.first;
+        p[u] = visible ? exp2_approx(a.exponent(raw, neg_shift - static_cast<float>(value))) : 0.0f;
+        // (Not the weight times 2^value: a small value's may be zero where others' are 2^90 times larger, and counts all the same.)
+        counted[u] = value == 0 ? p[u] : visible ? exp2_approx(a.exponent(raw, neg_shift)) : 0.0f;
+      }
+      sums[(e >> 1) & 3] = add_f32x2(sums[(e >> 1) & 3], pack_f32x2(counted[0], counted[1]));
+      words[e >> 1] = pk_pack_half(p[0], p[1]);
+    }
+    tmem_st8(a.tmem_s + c / 2, words);
+    if ((c & 63) == 48) {
+      tc_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) tc_mbar_arrive(p_full + (c >> 6));
+    }
+  }
+  float lo, hi;
+  unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), lo, hi);
+  return lo + hi;
+}
 
 template <int FORM, int HD, bool SHARED, bool PACKED = false>
 __global__ void __launch_bounds__(PACKED ? TC_PACKED_THREADS : TC_THREADS, 1)
@@ -284,16 +374,16 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   __shared__ unsigned long long edge_full;              // the pages of a tile at an edge have landed
   __shared__ unsigned tmem_base_s;
   __shared__ volatile int abort_flag;
-  // PACKED: of a tile some of whose scores are to be multiplied by something, its number, and a position's factor beside that number; of
-  // four tiles.  (Before the keys of tile j are made the products over those of j - 2, whose stage they take, are complete, and these follow
-  // the softmax of j - 3, or where slots take turns of j - 4: no softmax reads tile j - 4 any more.)
-  __shared__ int2 key_factors[4][PACKED ? TC_BN : 1];
-  __shared__ int factored[4];
+  // PACKED: of a tile some of whose positions have powers of two, its number, and its positions' notes for keys and for values; of four
+  // tiles.  (Before the keys of tile j are made the products over those of j - 2, whose stage they
+  // take, are complete, and these follow the softmax of j - 3, or where slots take turns of j - 4: no softmax reads tile j - 4 any more.)
+  __shared__ unsigned powers[2][4][PACKED ? TC_BN : 1];
+  __shared__ int powers_of[4];
 
-  if (PACKED) key_factors[threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0].x = -1;
+  if (PACKED) powers[0][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = powers[1][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = ~0u;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    if (PACKED) factored[0] = factored[1] = factored[2] = factored[3] = -1;
+    if (PACKED) powers_of[0] = powers_of[1] = powers_of[2] = powers_of[3] = -1;
     for (int b = 0; b < STAGES; ++b) {
       mbar_init(&kv_full[b], PACKED ? 2 : Shape::KIND_WARPS);
       mbar_init(&kv_empty[b], 1);
@@ -390,9 +480,9 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     // ------------------------------------------------------------------------- the loaders of a 4-bit cache
     // Items (a tile's keys, its values) go to teams of two warps in turn, in the order in which the products read them, half of the
     // positions each, block by block: the next blocks' bytes are on their way while one is turned into rows.
-    constexpr int PART = TC_PACKED_PART, PIECES = PART / 16, AHEAD = TC_PACKED_AHEAD;
+    constexpr int PART = TC_PACKED_PART, COPY = TC_PACKED_COPY, AHEAD = TC_PACKED_AHEAD;
     const int team = (warp - TC_MMA_WARP - 1) >> 1, member = (warp - TC_MMA_WARP - 1) & 1;
-    unsigned char* const raw = ring + STAGES * ITEM_BYTES + (2 * team + member) * AHEAD * PART;
+    unsigned char* const raw = ring + STAGES * ITEM_BYTES + (2 * team + member) * AHEAD * COPY;
     const int* table = a.block_table + static_cast<size_t>(row) * a.max_blocks;
     const unsigned char* const cache = reinterpret_cast<const unsigned char*>(a.kv_cache);
     const int items = team < TC_PACKED_TEAMS ? 2 * n_tiles : 0;
@@ -414,13 +504,18 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     };
     int issued = 0;
     auto copy = [&](int item, int b, int blocks) {         // block b of the half, in turn
-      unsigned char* const dst = raw + issued % AHEAD * PART;
+      unsigned char* const dst = raw + issued % AHEAD * COPY;
       ++issued;
       const int block = __shfl_sync(0xffffffffu, blocks, b);
       if (block >= 0) {
-        const unsigned char* const src = cache + static_cast<long long>(block) * pk_block_bytes(128) + (order(item) & 1) * PART;
+        // (A keys' copy ends with the values' parameters.)
+        const int values = order(item) & 1;
+        const unsigned char* const src = cache + static_cast<long long>(block) * pk_block_bytes(128) + values * PART;
 #pragma unroll
-        for (int e = lane; e < PIECES; e += 32) cp_async_16(dst + e * 16, src + e * 16, true);
+        for (int e = lane; e < COPY / 16; e += 32) {
+          if (e < PART / 16) cp_async_16(dst + e * 16, src + e * 16, true);
+          else if (!values) cp_async_16(dst + e * 16, src + e * 16 + pk_value_params(128) - PART, true);
+        }
       }
       cp_async_commit();
     };
@@ -445,24 +540,40 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
         copy(then < 4 ? item : item + TC_PACKED_TEAMS, then & 3, then < 4 ? blocks : next_blocks);
         cp_async_wait<AHEAD - 1>();
         __syncwarp();                // every lane's part of this block is there
-        const unsigned char* const source = raw + taken % AHEAD * PART;
+        const unsigned char* const source = raw + taken % AHEAD * COPY;
         ++taken;
         const int r0 = 64 * member + 16 * b;
         if ((which & 1) == 0) {
           // A lane four words, one of every group, of a position; positions in an order that spreads the rows' chunks over the banks.
           const int t = lane & 3, spread = (lane >> 2 & 1) * 4 + (lane >> 3);
+          // The values' parameters: a lane the steps, or the offsets, of a pair of positions.  Offsets alone within bounds are taken for usual.
+          {
+            const uint4 params = *reinterpret_cast<const uint4*>(source + PART + (lane & 15) * 16);
+            const unsigned top = pk_larger(pk_larger(params.x, params.y), pk_larger(params.z, params.w));
+            if (__builtin_expect(tc_packed_unusual(top, lane & 1), 0)) {
+              const unsigned char* const pair = source + PART + (lane & 14) * 16;
+              unsigned both = 0u;
+              for (int w = 0; w < 8; ++w) both = pk_larger(both, reinterpret_cast<const unsigned*>(pair)[w]);
+              for (int u = 0; u < 2; ++u) {
+                const int at = r0 + (lane & 14) + u, power = pk_exponent(pk_value_power((u ? both >> 16 : both) & 0x7fffu));
+                if (power == 0 || at < from || at >= until) continue;
+                powers[1][j & 3][at] = tc_packed_note(j, power);
+                powers_of[j & 3] = j;
+              }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int p = 8 * i + spread, r = r0 + p;
             const uint4 words = *reinterpret_cast<const uint4*>(source + pk_key_word<128>(p, t, 0));
             uint4 params = *reinterpret_cast<const uint4*>(source + pk_key_step<128>(p, 0));
             const unsigned all_params[4] = {params.x, params.y, params.z, params.w}, top = pk_largest(all_params);
-            if (__builtin_expect(!pk_half_usual<PK_KEYS_TO>(top) && r >= from && r < until, 0)) {
-              const float power = pk_half_power<PK_KEYS_TO>(top);
+            if (__builtin_expect(!pk_half_usual<PK_HELD_TO>(top) && r >= from && r < until, 0)) {
+              const float power = pk_half_power<PK_HELD_TO>(top);
+              params = make_uint4(pk_times(params.x, power), pk_times(params.y, power), pk_times(params.z, power), pk_times(params.w, power));
               if (power != 1.0f) {             // (all of the position's lanes write the same)
-                params = make_uint4(pk_times(params.x, power), pk_times(params.y, power), pk_times(params.z, power), pk_times(params.w, power));
-                key_factors[j & 3][r] = make_int2(j, __float_as_int(pk_inverse_power(power)));
-                factored[j & 3] = j;
+                powers[0][j & 3][r] = tc_packed_note(j, pk_exponent(power));
+                powers_of[j & 3] = j;
               }
             }
             const unsigned w[4] = {words.x, words.y, words.z, words.w}, s2[2] = {params.x, params.y}, o2[2] = {params.z, params.w};
@@ -494,15 +605,32 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
               o4[g] &= keep;
             }
           }
+          const unsigned top = pk_larger(pk_larger(pk_larger(s4[0], s4[1]), pk_larger(s4[2], s4[3])), pk_larger(pk_larger(o4[0], o4[1]), pk_larger(o4[2], o4[3])));
+          if (__builtin_expect(tc_packed_unusual(top, true), 0)) {
+            const float low = pk_value_power(top & 0x7fffu), high = pk_value_power(top >> 16 & 0x7fffu);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              s4[g] = pack_bf16(pk_low(s4[g]) * low, pk_high(s4[g]) * high);
+              o4[g] = pack_bf16(pk_low(o4[g]) * low, pk_high(o4[g]) * high);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            s4[g] = pk_to_half(s4[g]);
+            o4[g] = pk_to_half(o4[g]);
+          }
           unsigned char* const at = dst + r * 128;
           const int turn = r & 7;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int c = 4 * g + gp;
-            uint4 even, odd;
-            pk_value_channels(lo4[g], hi4[g], s4[g], o4[g], even, odd);
-            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + (((c & 7) ^ turn) << 4)) = even;
-            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + 128 + (((c & 7) ^ (turn + 1)) << 4)) = odd;
+            unsigned lo[4], hi[4];
+            pk_half_values(lo4[g], s4[g], o4[g], lo);
+            pk_half_values(hi4[g], s4[g], o4[g], hi);
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + (((c & 7) ^ turn) << 4)) =
+                make_uint4(__byte_perm(lo[0], lo[1], 0x5410), __byte_perm(lo[2], lo[3], 0x5410), __byte_perm(hi[0], hi[1], 0x5410), __byte_perm(hi[2], hi[3], 0x5410));
+            *reinterpret_cast<uint4*>(at + (c >> 3) * BLOCK_BYTES + 128 + (((c & 7) ^ (turn + 1)) << 4)) =
+                make_uint4(__byte_perm(lo[0], lo[1], 0x7632), __byte_perm(lo[2], lo[3], 0x7632), __byte_perm(hi[0], hi[1], 0x7632), __byte_perm(hi[2], hi[3], 0x7632));
           }
         }
         __syncwarp();                // every lane has read this block: another may come in its place
@@ -638,7 +766,7 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
     // all lanes.
     {
       constexpr unsigned HALVES = PACKED ? (1u << 7) | (1u << 10) : 0u;      // (both operands' type: bits off, half precision)
-      constexpr unsigned IDESC_QK = tc_idesc(false) & ~HALVES, IDESC_PV = tc_idesc(true);
+      constexpr unsigned IDESC_QK = tc_idesc(false) & ~HALVES, IDESC_PV = tc_idesc(true) & ~HALVES;
       constexpr int KSTEP = BLOCK * 2 * 16;        // bytes between 16 positions' values
       const bool leader = elect_one();
       const int count0 = slot_tiles(0), count1 = slot_tiles(1);
@@ -781,37 +909,26 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
       const int at = qp - k0;
       const int after = in_kept ? -1 : CHUNKED ? passed - k0 : a.window > 0 ? qp - a.window - k0 : -(1 << 30);
       const int last = min(qp, run_hi(j) - 1) - k0, first = max(run_lo(j) - k0, after + 1);
-      int factors_of = PACKED ? factored[j & 3] : -1;
-      float raw_max;
-      do {
-        raw_max = open_tile ? tc_row_max<false, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2)
-                            : tc_row_max<true, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2);
-        if (!PACKED || __builtin_expect(factors_of != j, 1)) break;
-        // Once more, with the scores times their factors.  (Asked behind the first: a look at the flag in front of it cost 2 %.)
-        factors_of = -1;
-#pragma unroll 1
-        for (int c = 0; c < TC_BN; c += 32) {
-          unsigned v[32];
-          tmem_ld32(tmem_s + c, v);
-          tmem_wait_ld32(v);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int2 factor = key_factors[j & 3][PACKED ? c + e : 0];
-            if (factor.x == j) v[e] = __float_as_uint(__uint_as_float(v[e]) * __int_as_float(factor.y));
-          }
-          tmem_st32(tmem_s + c, v);
-        }
-        tc_wait_st();
-      } while (true);
+      const int tile_powers = PACKED ? powers_of[j & 3] : -1;      // (asked for here, looked at behind the maximum: in front of it that cost 2 %)
+      const float raw_max = open_tile ? tc_row_max<false, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2)
+                                : tc_row_max<true, BIASED_SCORES>(tmem_s, last, first, score_scale, at, r1, r2);
       // The scale is positive and the bound grows with its argument: the largest raw score gives the largest exponent.
-      const float row_max = capped ? a.softcap_log2 * tanh_from_exp2(raw_max * score_scale) : BIASED_SCORES ? raw_max : raw_max * score_scale;
-      const bool grow = raw_max > -INFINITY && (row_max > m_used + TC_RESCALE_THRESHOLD || m_used == -INFINITY);
+      auto exponent = [&](float raw) { return capped ? a.softcap_log2 * tanh_from_exp2(raw * score_scale) : BIASED_SCORES ? raw : raw * score_scale; };
+      float row_max = exponent(raw_max);
+      bool some = raw_max > -INFINITY;
+      const bool by_powers = PACKED && __builtin_expect(tile_powers == j, 0);
+      auto in_tile = [&] { return TcPackedRow{tmem_s, powers[0][j & 3], j, last, first, score_scale, a.softcap_log2}; };
+      if (by_powers) {
+        row_max = tc_packed_row_max(in_tile());
+        some = row_max > -INFINITY;
+      }
+      const bool grow = some && (row_max > m_used + TC_RESCALE_THRESHOLD || m_used == -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {
         // Some row of the warp moves its shift: every lane takes part in the tensor-memory
         // instructions, rows that stay multiply by one.
         const float factor = grow ? exp2f(m_used - row_max) : 1.0f;       // 0 for a row's first keys
+        l_run = PACKED && grow ? tc_packed_rescaled(l_run, m_used - row_max, factor) : l_run * factor;
         if (grow) m_used = row_max;
-        l_run *= factor;
         if (i > 0) {
           // O holds the tiles before this one: their products were issued before this tile's S, which is complete, and this
           // tile's product waits for this warp's arrival below.
@@ -827,36 +944,40 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
           tc_wait_st();
         }
       }
-      const float neg_shift = m_used == -INFINITY ? 0.0f : -m_used;
+      const float neg_shift = (PACKED ? TC_PACKED_LIFT : 0.0f) - (m_used == -INFINITY ? 0.0f : m_used);
       // Two probabilities a column, as the second product reads its A operand from tensor memory, over columns of S
       // that have been read; the product of the first 64 positions runs while the others are worked on.
       unsigned long long sums[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        unsigned words[32];
-        if (capped) {
-          tc_exponentials<true, true>(tmem_s, 64 * half, words, sums, score_scale, neg_shift, last, first, a.softcap_log2);
-        } else if (open_tile) {
-          tc_exponentials<false, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
-        } else {
-          tc_exponentials<true, false>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
+      if (by_powers) {
+        l_run += tc_packed_weights(in_tile(), neg_shift, &p_full[2 * slot]);
+      } else {
+#pragma unroll (PACKED ? 1 : 2)
+        for (int half = 0; half < 2; ++half) {
+          unsigned words[32];
+          if (capped) {
+            tc_exponentials<true, true, PACKED>(tmem_s, 64 * half, words, sums, score_scale, neg_shift, last, first, a.softcap_log2);
+          } else if (open_tile) {
+            tc_exponentials<false, false, PACKED>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
+          } else {
+            tc_exponentials<true, false, PACKED>(tmem_s, 64 * half, words, sums, BIASED_SCORES ? 1.0f : score_scale, neg_shift, last, first, 0.0f);
+          }
+          tmem_st32(tmem_s + 32 * half, words);
+          tc_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc_mbar_arrive(&p_full[2 * slot + half]);
         }
-        tmem_st32(tmem_s + 32 * half, words);
-        tc_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc_mbar_arrive(&p_full[2 * slot + half]);
+        float sum_lo, sum_hi;
+        unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), sum_lo, sum_hi);
+        l_run += sum_lo + sum_hi;
       }
-      float sum_lo, sum_hi;
-      unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), sum_lo, sum_hi);
-      l_run += sum_lo + sum_hi;
       if (trace && threadIdx.x == 0 && i < 64) trace[4 * i + 2] = tc_timer_ns();
     }
     if (!failed && count > 0 && !__all_sync(0xffffffffu, wait(&o_done[slot], 0))) { give_up(-6); failed = true; }
     tc_fence_after_sync();
     // One more exponential: the sink, relative to the shift the row's sums were formed with (both in powers of two).
     auto with_sink = [&](float sum, float shift) {
-      return a.sinks != nullptr && shift > -INFINITY ? sum + exp2f(a.sinks[head] * 1.4426950408889634f - shift) : sum;
+      return a.sinks != nullptr && shift > -INFINITY ? sum + exp2f(a.sinks[head] * 1.4426950408889634f - shift + (PACKED ? TC_PACKED_LIFT : 0.0f)) : sum;
     };
     // Each warp puts 32 rows x 64 columns into shared memory, 16-byte pieces permuted by the row so that neither the writes
     // (a thread a row) nor the reads (eight threads a row) meet in a bank, and then writes whole 128-byte row pieces, four rows
@@ -920,7 +1041,9 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
                                                         __uint_as_float(v[4 * q4 + 2]), __uint_as_float(v[4 * q4 + 3]));
       }
       slots_meet();
-      const float l_row = with_sink(l_run * mine + note[slot ^ 1][r][1] * others, m), inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
+      const float l_both = PACKED ? tc_packed_rescaled(l_run, m_used - m, mine) + tc_packed_rescaled(note[slot ^ 1][r][1], m_other - m, others)
+                                  : l_run * mine + note[slot ^ 1][r][1] * others;
+      const float l_row = with_sink(l_both, m), inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
       const float f_mine = mine * inv, f_others = others * inv;
       if (!abort_flag && !failed)
         store_half(smem + 65536 + warp * 4096, slot, [&](float o, int column) {

@@ -89,10 +89,10 @@ __device__ __forceinline__ float pk_high(unsigned pair) { return __uint_as_float
 // ---- Keys and queries for a prompt's products, as half-precision values: three bits more than bfloat16's eight, since what a key is off
 // by moves all of a query's weights (at most 2^-12 of a value here; with bfloat16 keys a prompt's result was 0.0054 off where the weights' and
 // the results' own roundings make 0.0025).  What half precision lacks is range.  So a position whose largest step or offset is not
-// 2^-5 to 2^11 (or zero), and a query whose largest channel is not 2^-5 to 2^15, is held times a power of two of its own that takes it to
-// the upper end, and its scores are multiplied by the power's inverse.  A channel is then off by 2^-12 of it or 2^-15 of the largest of
-// the position's, whichever is more.
-constexpr unsigned PK_HALF_FROM = 0x3d00u, PK_KEYS_TO = 0x4500u, PK_QUERIES_TO = 0x4700u;      // 2^-5, 2^11, 2^15 as bfloat16
+// 2^-8 to 2^11 (or zero), and a query whose largest channel is not 2^-8 to 2^15, is held times a power of two of its own that takes it to
+// the upper end, and its scores are multiplied by the power's inverse.  A channel is then off by 2^-12 of it, or by 2^-12 of the
+// position's largest where that is near the lower end.
+constexpr unsigned PK_HALF_FROM = 0x3b80u, PK_HELD_TO = 0x4500u, PK_QUERIES_TO = 0x4700u;      // 2^-8, 2^11, 2^15 as bfloat16
 
 // The larger magnitudes of two words' bfloat16 values, half by half, with some sign (a NaN's is not counted).
 __device__ __forceinline__ unsigned pk_larger(unsigned a, unsigned b) {
@@ -114,7 +114,7 @@ __device__ __forceinline__ bool pk_half_usual(unsigned top) { return top - PK_HA
 template <unsigned TO>
 __device__ __forceinline__ float pk_half_power(unsigned top) {
   const unsigned bits = top & 0xffffu;
-  if (pk_half_usual<TO>(top) || bits == 0u || bits >= 0x7f80u) return 1.0f;
+  if (bits - PK_HALF_FROM < TO - PK_HALF_FROM || bits == 0u || bits >= 0x7f80u) return 1.0f;
   return __uint_as_float(min(127u + (TO >> 7) - 1u - (bits >> 7), 253u) << 23);
 }
 __device__ __forceinline__ float pk_inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
@@ -154,6 +154,15 @@ __device__ __forceinline__ unsigned pk_pack_half(float low, float high) {
 // Two bfloat16 values as half-precision ones, and times a power of two.
 __device__ __forceinline__ unsigned pk_to_half(unsigned pair) { return pk_pack_half(pk_low(pair), pk_high(pair)); }
 __device__ __forceinline__ unsigned pk_times(unsigned pair, float power) { return pack_bf16(pk_low(pair) * power, pk_high(pair) * power); }
+// A value's power of two, whose inverse is a factor of its weight beside others: 2^90 at most, so that the sum of 2^20 weights, as large as
+// that beside such values', is a float32 value.  Zeros have the most, since they leave others' weights as they are then.
+__device__ __forceinline__ float pk_value_power(unsigned top) {
+  constexpr float MOST = 1.2379400392853803e27f;
+  return top == 0u ? MOST : fminf(pk_half_power<PK_HELD_TO>(top), MOST);
+}
+// The exponent of a power of two, and the power of an exponent.
+__device__ __forceinline__ int pk_exponent(float power) { return static_cast<int>(__float_as_uint(power) >> 23) - 127; }
+__device__ __forceinline__ float pk_power(int exponent) { return __uint_as_float(static_cast<unsigned>(exponent + 127) << 23); }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
