@@ -60,12 +60,6 @@ __device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
-__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
-  float2 r;
-  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 
 // x and y as three pairs of bfloat16 values whose sums they are (of a value below 2^-110 the bits below 2^-133 are lost), the largest first.  A
 // value that would round to infinity keeps the largest bfloat16 as its first part; an infinity's parts are that, itself and a NaN.

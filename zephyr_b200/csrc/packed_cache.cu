@@ -386,9 +386,6 @@ int unpack_launch(void* out, const unsigned char* packed, const int* pages, int 
 
 using namespace zb;
 
-// Bytes of a block of 16 positions of one head; 0 for a head size that the packed cache does not take.
-ZB_API int zb_packed_block_bytes(int hd) { return pk_head_dim_ok(hd) ? pk_block_bytes(hd) : 0; }
-
 // What zb_qk_norm_rope_packed is given: eight bytes a field, in this order.
 struct PackedWriteCall {
   void* q_out; const void* qkv; long long qkv_stride; const float* bias; const void* q_norm_w; const void* k_norm_w;

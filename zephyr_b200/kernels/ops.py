@@ -115,7 +115,6 @@ _SIGNATURES = {
     "zb_qkv_halves": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int, c_float,
                       c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                       c_int, c_int, c_int, c_int, c_void_p, c_void_p],
-    "zb_packed_block_bytes": [c_int],
     "zb_qk_norm_rope_packed": [c_char_p], "zb_unpack_pages": [c_char_p], "zb_paged_decode_packed": [c_char_p],
     "zb_paged_prefill_packed": [c_char_p], "zb_paged_prefill_tc_packed": [c_char_p],
     "zb_pool_blocks": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
