@@ -374,16 +374,9 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   __shared__ unsigned long long edge_full;              // the pages of a tile at an edge have landed
   __shared__ unsigned tmem_base_s;
   __shared__ volatile int abort_flag;
-  // PACKED: of a tile some of whose positions have powers of two, its number, and its positions' notes for keys and for values; of four
-  // tiles.  (Before the keys of tile j are made the products over those of j - 2, whose stage they
-  // take, are complete, and these follow the softmax of j - 3, or where slots take turns of j - 4: no softmax reads tile j - 4 any more.)
-  __shared__ unsigned powers[2][4][PACKED ? TC_BN : 1];
-  __shared__ int powers_of[4];
 
-  if (PACKED) powers[0][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = powers[1][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = ~0u;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    if (PACKED) powers_of[0] = powers_of[1] = powers_of[2] = powers_of[3] = -1;
     for (int b = 0; b < STAGES; ++b) {
       mbar_init(&kv_full[b], PACKED ? 2 : Shape::KIND_WARPS);
       mbar_init(&kv_empty[b], 1);
@@ -400,6 +393,12 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   }
   wait_for_prior_grids();          // tiles, queries, keys and values: all of it earlier kernels' work
   let_dependents_launch();
+
+  // PACKED: of a tile some of whose positions have powers of two, its number, and its positions' notes for keys and for values; of four
+  // tiles.  (Before the keys of tile j are made the products over those of j - 2, whose stage they
+  // take, are complete, and these follow the softmax of j - 3, or where slots take turns of j - 4: no softmax reads tile j - 4 any more.)
+  __shared__ unsigned powers[2][4][PACKED ? TC_BN : 1];
+  __shared__ int powers_of[4];
 
   // The host lists the tiles by the number of keys they see, fewest first: take the list back to
   // front, and all heads of a tile before the next tile, so that the longest work of the whole
@@ -453,6 +452,10 @@ paged_prefill_tc_kernel(const __grid_constant__ PrefillTcArgs a) {
   if (warp == TC_MMA_WARP) {
     tmem_alloc(&tmem_base_s, TC_TMEM_COLUMNS);
     tmem_relinquish();
+  }
+  if (PACKED) {
+    powers[0][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = powers[1][threadIdx.x >> 7][PACKED ? threadIdx.x & 127 : 0] = ~0u;
+    if (threadIdx.x < 4) powers_of[threadIdx.x] = -1;
   }
   tc_fence_before_sync();
   __syncthreads();
