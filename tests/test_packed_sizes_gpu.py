@@ -277,3 +277,21 @@ def test_prompts_over_values_of_several_sizes(ops, cuda_device, hd, tensor_memor
         expected, bound = plain.attention(q[rows].double().view(-1, nh, hd), k, times(v, -by), pos[rows], hd ** -0.5, sinks=sinks, rounded=True, **masks)
         # (What no row of these sees may be far out of range on their scale.)
         assert ((got[rows] * 2.0 ** -by - expected).abs() <= bound).all(), power
+
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("power", [-90, 0, 90])
+def test_single_tokens_over_values_some_of_which_are_not_finite(ops, cuda_device, power, plan):
+    """A group that is not finite spoils its own channels; the others hold whatever their size is."""
+    nh, nkv, hd, n, g = 4, 2, 64, 200, torch.Generator().manual_seed(47)
+    keys, values = torch.randn((n, nkv, hd), generator=g), torch.randn((n, nkv, hd), generator=g) * 2.0 ** power
+    values[0, 0, 3], values[77, 1, 40] = math.nan, math.inf
+    packed, table, (k, v) = held_cache(ops, cuda_device, keys, values)
+    q = torch.randn((1, nh * hd), generator=g).to(torch.bfloat16)
+    got = decode(ops, cuda_device, packed, table, q, n, nh, nkv, hd, hd ** -0.5, plan) * 2.0 ** -power
+    spoiled = torch.zeros((1, nh, hd), dtype=torch.bool)
+    spoiled[:, :2, :32] = spoiled[:, 2:, 32:] = True
+    assert torch.equal(torch.isnan(got), spoiled)
+    finite = [torch.where(torch.isnan(x), torch.zeros_like(x), x) for x in times(v, -power)]
+    expected, bound = plain.attention(q.double().view(1, nh, hd), k, finite, torch.tensor([n - 1]), hd ** -0.5)
+    assert ((got - expected).abs() <= bound)[~spoiled].all()

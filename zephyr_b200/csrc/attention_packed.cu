@@ -8,9 +8,10 @@
 //            shift.  What multiplies them carries a power of two (2^80 in weights, a head's own in queries) that keeps products and
 //            sums far from float32's ends; all of it is exact.  That holds for values while the largest step or offset that a warp has
 //            seen is 2^-30 to 2^12; else they carry a power of two as well, which follows that largest one (sums are rescaled with it, as
-//            with the scores' maximum).  So values of 2^-100 to 2^100 hold, and beside the largest product of a weight and a value what
-//            is 2^80 times smaller keeps its bits.  (The look at a tile's parameters takes some 15 of its 600 instructions: 52.2 -> 53.7 us
-//            for 48 rows of 1 to 6001 positions, 42.0 -> 43.5 for one of 120001, 18.3 -> 19.0 for 8 of 4096.)
+//            with the scores' maximum).  So values of 2^-100 to 2^100 hold, and beside a context's largest weight times its largest value
+//            a product that is 2^70 times smaller keeps its bits (2^40 where that value is 2^-30).  (The look at a tile's parameters takes
+//            some 15 of its 600 instructions: 8 rows of 4096 16.0 -> 16.6 us on the device, 64 rows 74.4 -> 77.3, 8 of 2048 with 16/8 heads of
+//            64 7.9 -> 8.4.)
 //   keys     S[h, p] = sum_j step_pj c_j[h, p] + sum_j offset_pj (sum_{d in j} q_hd), c_j being the product over the codes of a group
 //            of 32 channels.  The first sum in float32; the second a product of the position's parameters as they lie and the query
 //            sums as two bfloat16 parts.
@@ -42,7 +43,7 @@ constexpr int PD_TILE = 32;              // positions per tile: a warp's unit of
 constexpr int PD_HEADS = 8;              // query heads on the products' columns
 constexpr float PD_LIFT = 80.0f;         // weights carry 2^80, results 2^(80 - 133)
 constexpr unsigned PD_VALUES_FROM = 0x3080u, PD_VALUES_TO = 0x4580u;      // 2^-30 and 2^12 as bfloat16: between them values carry nothing
-constexpr float PD_VALUES_UNSEEN = 8.507059173023462e37f;                 // 2^126
+constexpr float PD_VALUES_UNSEEN = 1.7014118346046923e38f;                // 2^127
 constexpr float PD_RESCALE = 8.0f;       // a running maximum (in powers of two) may be passed by this before sums are rescaled
 
 enum { PD_CLUSTERS, PD_CTA_SHARES, PD_WARP_SHARES };      // how contexts are cut
@@ -529,9 +530,12 @@ paged_decode_packed_kernel(const PackedDecodeArgs a) {
           value_params(b, params);
           most = __vmaxu2(most, __vmaxu2(params[0] & 0x7fff7fffu, params[1] & 0x7fff7fffu));
         }
-        // (A half that is PD_VALUES_TO or more gets its highest bit.)
-        constexpr unsigned UP = (0x8000u - PD_VALUES_TO) * 0x10001u;
-        if (__any_sync(0xffffffffu, value_scale != 1.0f || (most + UP & 0x80008000u) != 0u)) {
+        // (A half that is PD_VALUES_TO, or PD_VALUES_FROM, or more gets its highest bit.)
+        const bool large = (most + (0x8000u - PD_VALUES_TO) * 0x10001u & 0x80008000u) != 0u;
+        const bool usual = !large && (most + (0x8000u - PD_VALUES_FROM) * 0x10001u & 0x80008000u) != 0u;
+        // (The first values, which are the most tiles that a warp of a short context has, take the short way too.)
+        if (value_scale == PD_VALUES_UNSEEN && __any_sync(0xffffffffu, usual)) value_scale = 1.0f;
+        if (__any_sync(0xffffffffu, large || value_scale != 1.0f)) {
           unsigned top = 0u;
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
