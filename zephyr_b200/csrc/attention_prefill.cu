@@ -84,10 +84,10 @@ struct PrefillArgs {
 // PACKED and the registers last (heads of 32 to 96), since eight warps, an SM's fill, leave it idle half of the time (the above 56 us
 // with one group, 46 with two; 1024 tokens behind 2000, 16/8 heads of 64, 104 and 83).  Instructions bound it then: of some 800 a warp
 // and tile, scales that join a score in its exponent, 2^x without its range's ends and sums that are rescaled only where a maximum
-// moved took 150 (42 and 76 us).
+// moved took 150 (42 and 76 us; with the powers of two below 46 and 83).
 // A key's power of two (packed.cuh) is looked for where its row is made, and its inverse joins its scores in tiles that have one; the
 // queries' powers are found, and queries made half precision, in shared memory in front of the tiles, the inverses joining the scale
-// (2048 tokens, 16/8 heads of 64: 57.7 us without, 60.3; with the queries' part in registers inside the loop 61.7).
+// (2048 tokens, 16/8 heads of 64: 57.7 us without, 60.1; with the queries' part in registers inside the loop 61.7).
 template <int HD, bool PACKED>
 constexpr int PRE_GROUPS = PACKED && HD <= 96 ? 2 : 1;
 

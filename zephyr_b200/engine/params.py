@@ -31,8 +31,9 @@ class KvCacheOptions:
     """``block_size`` tokens per page; ``memory_bytes`` for the pool, or None to size it from
     ``gpu_memory_utilization`` (src/include/executor/causal_lm.hpp:16-20).  ``num_blocks`` (this
     engine's addition) fixes the number of pages directly and wins over both.  ``bits`` (likewise): None holds
-    keys and values in the model's type, 4 in codes of 4 bits with a step and an offset for every 32 channels, 3.2
-    times as many positions in the same memory."""
+    keys and values in the model's type, 4 in codes of 4 bits with a step and an offset for every 32 channels: 3.2
+    times as many positions in the same memory and faster decode steps, rounded keys and values (by up to half a step, a
+    thirtieth of what the 32 channels span) and prompts that take 3 to 12 % longer (2048 tokens)."""
 
     block_size: int = 16
     memory_bytes: int | None = None

@@ -1417,7 +1417,7 @@ def qk_norm_rope_packed(qkv: torch.Tensor, nh: int, nkv: int, hd: int, q_norm_w:
     (float32) or 8-byte boundaries; without ``packed`` only the queries are made, from the first nh*hd columns.  ``cos`` / ``sin``:
     float32 [positions, D / 2]; the first D channels of a head turn, in pairs (i, i + D / 2) with ``layout`` "halves" (D a multiple
     of 8), (2i, 2i + 1) with "pairs"; any scaling of frequencies and any multiplier is in the tables.  ``bias``: float32, one value a
-    column.  A (row, position) comes once in a call."""
+    column.  A (row, position) comes once in a call.  A group that is not finite, or spans more than float32's range, reads back as NaN."""
     _check_index(positions, token_row, block_table, status)
     shape, table_shape, in_dtype = qkv.shape, block_table.shape, qkv.dtype
     T = shape[0]
@@ -1536,7 +1536,7 @@ def packed_decode_plan(n_rows: int, nh: int, nkv: int, visible: int) -> tuple[in
 
     What a launch takes is, near enough, a fixed time and one for every 32 positions of a warp, which is 1.2 us while every CTA has an SM
     to itself and 1.9 with two: a cluster 8.6 or 10.7 us beside that, shares 13.5 or 17.7.  The least of these is taken, among clusters
-    whose CTAs have 128 positions or more; shares where they gain a tenth, since contexts may be shorter than ``visible``, which a captured
+    whose CTAs have 128 positions or more (heads of 128; smaller ones, whose tiles cost less, take the same); shares where they gain a tenth, since contexts may be shorter than ``visible``, which a captured
     step rounds up.  (Measured, us, 32/8 heads: 8 rows of 8024 in clusters of 2 / 4 / 148 / 296 shares 27.6 / 26.0 /
     32.3 / 30.9, 4 of 16000 in 4 / 8 / 148 / 296 27.4 / 25.9 / 31.4 / 29.9, 16 of 8000 in 1 / 2 / 296 45.1 / 40.7 / 47.9, 2 of 20000 in 4 / 148
     31.3 / 23.4, 1 of 120001 in 8 / 148 / 296 77 / 45.6 / 41.9, 12 of 1000 in 1 / 2 10.2 / 11.5.)  More pairs than CTAs go in warps' shares, which
