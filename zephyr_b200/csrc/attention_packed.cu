@@ -8,7 +8,7 @@
 //            shift.  What multiplies them carries a power of two (2^80 in weights, a head's own in queries) that keeps products and
 //            sums far from float32's ends; all of it is exact.  That holds for values while the largest step or offset that a warp has
 //            seen is 2^-30 to 2^12; else they carry a power of two as well, which follows that largest one (sums are rescaled with it, as
-//            with the scores' maximum).  So values of 2^-100 to 2^100 hold, and beside a context's largest weight times its largest value
+//            with the scores' maximum).  So values of 2^-90 to 2^90 hold, and beside a context's largest weight times its largest value
 //            a product that is 2^70 times smaller keeps its bits (2^40 where that value is 2^-30).  (The look at a tile's parameters takes
 //            some 15 of its 600 instructions: 8 rows of 4096 16.0 -> 16.6 us on the device, 64 rows 74.4 -> 77.3, 8 of 2048 with 16/8 heads of
 //            64 7.9 -> 8.4.)

@@ -1568,7 +1568,7 @@ def paged_decode_packed(q: torch.Tensor, packed: torch.Tensor, block_table: torc
     """``paged_decode`` over a 4-bit cache: attention of rows with one new token each, whose key and value the cache holds already;
     writes those tokens' rows of ``out``.  bfloat16; ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  ``max_context`` is at
     least the longest context of the rows, the new token included.  ``plan``: as ``packed_decode_plan`` gives it (None: chosen by
-    that).  The scratch of a launch is the call's own.  Queries, keys and values of 2^-100 to 2^100 in magnitude."""
+    that).  The scratch of a launch is the call's own.  Queries, keys and values of 2^-90 to 2^90 in magnitude."""
     _check_index(block_table, rows, row_q_start, row_ctx, status)
     tokens, n_table, max_blocks, pages, page_size = _packed_attention_args(q, packed, block_table, row_q_start, row_ctx, status, out, nh,
                                                                            nkv, hd, window, chunk, softcap, sinks)
@@ -1602,7 +1602,7 @@ def paged_prefill_packed(q: torch.Tensor, packed: torch.Tensor, block_table: tor
     """``paged_prefill`` over a 4-bit cache: attention of rows with several new tokens, cut into tiles of
     ``paged_prefill_tile_tokens()``, whose keys and values the cache holds already; writes those tokens' rows of ``out``.  bfloat16;
     ``window``, ``chunk``, ``sinks`` and ``softcap`` as there.  Queries and keys are multiplied as half-precision values, each position's key and
-    each query times a power of two of its own where its size asks for one: queries, keys and values of 2^-100 to 2^100 in magnitude.  Head
+    each query times a power of two of its own where its size asks for one: queries, keys and values of 2^-90 to 2^90 in magnitude.  Head
     size 128 runs on tcgen05 (but the shortest prompts, ``short_prompts``, and everything without ``tensor_memory`` or a positive scale),
     other sizes on mma.sync."""
     _check_index(block_table, tile_row, tile_q0, row_q_start, row_q_len, row_ctx, status)
