@@ -1,0 +1,98 @@
+// Matrices and rows in 8-bit floating point (e4m3) with a scale for each block of 128: the rule that finds a scale, conversions, and where
+// scales lie.
+//
+// A scale is a power of two 2^s, kept as the byte s + 127: the least one for which the block's largest finite magnitude is at most
+// 448 * 2^s (448 is the largest e4m3 number), s >= -126.  A division by it is exact, so a code is the value rounded once, and it costs no accuracy
+// beside any other factor: e4m3 numbers are as dense, relative to their size, wherever they lie.  Powers of two are what the tensor cores
+// multiply a block's sums with themselves (kind::mxf8f6f4), and their exponents are all that has to be stored.
+//
+// Codes: rows of pitch Kp, K rounded up to 128, zeros behind K.  Scales: pieces of 512 bytes, one for 128 rows and four neighbouring
+// blocks of K; row r's four bytes lie at 16 (r % 32) + 4 (r / 32), which is how tcgen05.cp brings a piece into tensor memory.  A matrix has one scale for
+// 128 rows; its pieces hold it 128 times (0.8 % of the codes' bytes), so that both operands of a product look alike.
+#pragma once
+
+#include "common.cuh"
+
+namespace zb {
+
+constexpr int B8_BLOCK = 128;
+constexpr int B8_PIECE = 512;          // bytes of scales of 128 rows x 4 blocks of K
+
+__host__ __device__ inline int b8_blocks(int n) { return (n + B8_BLOCK - 1) / B8_BLOCK; }
+__host__ __device__ inline int b8_pieces(int k) { return (k + 4 * B8_BLOCK - 1) / (4 * B8_BLOCK); }
+__host__ __device__ inline int b8_pitch(int k) { return b8_blocks(k) * B8_BLOCK; }
+
+// Bits of |x| where x is finite, else zero: their maximum is the block's.
+__device__ __forceinline__ unsigned b8_magnitude(float x) {
+  const unsigned bits = __float_as_uint(x) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;
+}
+// The scale's byte for a block whose largest magnitude has these bits: 448 is 1.75 * 2^8.
+__device__ __forceinline__ unsigned b8_scale_byte(unsigned largest) {
+  const int byte = static_cast<int>(largest >> 23) - 8 + ((largest & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return static_cast<unsigned>(byte < 1 ? 1 : byte);
+}
+__device__ __forceinline__ float b8_power(unsigned byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ float b8_inverse(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+
+// Four values divided by the block's scale, as codes, the first in the lowest byte.  What is not finite becomes NaN (the conversion alone would
+// make an infinity the largest code).
+__device__ __forceinline__ unsigned b8_codes(float a, float b, float c, float d, float inverse) {
+  unsigned short lo, hi;
+  const float nan = __uint_as_float(0x7fffffffu);
+  a = fabsf(a) < __uint_as_float(0x7f800000u) ? a * inverse : nan;
+  b = fabsf(b) < __uint_as_float(0x7f800000u) ? b * inverse : nan;
+  c = fabsf(c) < __uint_as_float(0x7f800000u) ? c * inverse : nan;
+  d = fabsf(d) < __uint_as_float(0x7f800000u) ? d * inverse : nan;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<unsigned>(lo) | (static_cast<unsigned>(hi) << 16);
+}
+
+// 16 neighbouring values of a row, zeros from `left` on (left may be negative).  `wide`: the row's start and pitch allow 16-byte loads.
+__device__ __forceinline__ void b8_load16(const float* p, int left, bool wide, float (&v)[16]) {
+  if (wide && left >= 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(p + 4 * i);
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i < left ? p[i] : 0.0f;
+  }
+}
+__device__ __forceinline__ void b8_load16(const __nv_bfloat16* p, int left, bool wide, float (&v)[16]) {
+  if (wide && left >= 16) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + 8 * i);
+      const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i < left ? __bfloat162float(p[i]) : 0.0f;
+  }
+}
+
+// A warp codes 512 values of a row, 16 a lane, eight lanes a block: this lane's 16 codes, and in every lane the scales' four bytes.
+__device__ __forceinline__ uint4 b8_code_row_piece(const float (&v)[16], unsigned& scales) {
+  unsigned largest = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) largest = max(largest, b8_magnitude(v[i]));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+  const unsigned byte = b8_scale_byte(largest);
+  const float inverse = b8_inverse(byte);
+  scales = __shfl_sync(0xffffffffu, byte, 0) | __shfl_sync(0xffffffffu, byte, 8) << 8 | __shfl_sync(0xffffffffu, byte, 16) << 16 |
+           __shfl_sync(0xffffffffu, byte, 24) << 24;
+  return make_uint4(b8_codes(v[0], v[1], v[2], v[3], inverse), b8_codes(v[4], v[5], v[6], v[7], inverse),
+                    b8_codes(v[8], v[9], v[10], v[11], inverse), b8_codes(v[12], v[13], v[14], v[15], inverse));
+}
+
+}  // namespace zb

@@ -84,6 +84,15 @@ _SIGNATURES = {
     "zb_expert_product": [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                           c_int, c_int, c_int, c_float, c_float, c_float, c_int, c_int, c_void_p],
     "zb_route_align_runs": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "zb_route_align_strided": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
+    "zb_matrix_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "zb_code_rows": [c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p],
+    "zb_gemm_block8": [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                       c_int, c_void_p, c_void_p, c_float, c_float, c_float, c_void_p, c_void_p],
+    "zb_gemm_block8_small_supported": [c_int, c_int, c_int],
+    "zb_gemm_block8_small": [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                             c_float, c_float, c_float, c_void_p],
     "zb_gather_places": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "zb_gemm_tc_experts_run": [c_int, c_int],
     "zb_gemm_tc_experts": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int,
@@ -2371,9 +2380,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
     layers do (src/layer/linear.cpp:22-24 -> cuBLASLt), where that is the faster one; with
     ``USE_LIBRARY_PRODUCTS`` off they run on this package's tcgen05 kernel (``gemm_tc``), so that no
     library kernel is left on the path.  Accumulation is float32 everywhere.  A ``bias`` [N] is
-    added to the product's (rounded) output by a kernel of its own."""
+    added to the product's (rounded) output by a kernel of its own.  A ``BlockMatrix`` goes to ``block_linear``."""
     if bias is not None:
         return add_bias(linear(x, w, out_dtype), bias)
+    if type(w) is BlockMatrix:
+        return block_linear(x, w, out_dtype)
     _cuda(x, w)
     if x.dtype == torch.float32:
         return gemm_nt_simt(x, w, out_dtype)
@@ -2485,7 +2496,17 @@ def routed_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_
     are multiplied by the weight ahead of the activation; no identity experts).  ``bounded`` (without biases): the
     bounded gate of the unrounded gate and up sums in the activation's place.  bfloat16 with the interleaved layout: each product is ONE
     launch of a tcgen05 kernel over runs of an expert's tokens; otherwise tiles on mma.sync
-    (bfloat16) or CUDA cores (float32)."""
+    (bfloat16) or CUDA cores (float32).  ``w_gate`` (interleaved) and ``w_down`` may be ``BlockMatrix``es [E, 2 ff, width] and [E, width, ff]:
+    the products then run in 8-bit floating point, the hidden values stay in float32 until they are coded for the second one."""
+    if type(w_gate) is BlockMatrix or type(w_down) is BlockMatrix:
+        _require(type(w_gate) is type(w_down) and w_up is None, "both matrices in 8-bit floating point, gate and up rows in one")
+        _require(act in ACTIVATIONS, f"the gate's activation is one of {sorted(ACTIVATIONS)}")
+        _require(bounded is None or (bounded.bias is None and bounded.limit > 0.0 and not weigh_inputs),
+                 "experts' bounded gates have a positive limit, no biases and weights on the outputs")
+        _i32(ids)
+        _require(ids.dim() == 2 and x.dim() == 2 and ids.shape[0] == x.shape[0] and weights.dtype == torch.float32 and weights.is_contiguous()
+                 and weights.shape == ids.shape, "one id and weight per choice")
+        return _routed_blocks(x, ids, weights, w_gate, w_down, act, weigh_inputs, bounded)
     _cuda(x, ids, weights, w_gate, w_up, w_down)
     T, width = x.shape
     top = ids.shape[1]
@@ -2552,6 +2573,214 @@ def routed_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_
 
 
 USE_GROUPED_TCGEN05 = True      # off: a routed layer's products stay on the mma.sync tiles whatever the token count
+
+
+# ------------------------------------------- matrices in 8-bit floating point, a scale for each block of 128
+BLOCK8 = 128                  # rows and columns of a matrix, values of a row of activations, that share a scale
+BLOCK8_FEW_ROWS = 16          # up to here a product streams the matrix and codes its rows on the way
+_BLOCK8_KINDS = {"silu": 1, "relu": 2}
+
+
+class BlockMatrix:
+    """A matrix [N, K], or several of one shape [matrices, N, K], in 8-bit floating point (e4m3) with a power of two for each block of 128 x
+    128: the least one, from 2^-126 on, for which the block's largest finite magnitude is at most 448 times it.  A value is
+    code * power; one that was not finite is NaN.  ``pack_matrix`` makes it from a bfloat16 or float32 tensor, ``BlockMatrix.from_codes`` from codes that
+    exist; ``linear``, ``block_linear``, ``block_feed_forward`` and ``routed_experts`` take it where they take a matrix.
+
+    ``codes``: uint8 [matrices * N, K rounded up to 128], zeros behind K; ``scales``: uint8 [matrices, N / 128 up, K / 512 up, 512], the bytes (exponent +
+    127) of four neighbouring blocks of K for each of a block's 128 rows, as the tensor cores read them."""
+
+    __slots__ = ("codes", "scales", "matrices", "N", "K", "shape", "device")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Sequence[int]):
+        self.codes, self.scales, self.shape, self.device = codes, scales, torch.Size(shape), codes.device
+        self.matrices = shape[0] if len(shape) == 3 else 1
+        self.N, self.K = shape[-2:]
+
+    @staticmethod
+    def _empty(shape: Sequence[int], device) -> "BlockMatrix":
+        matrices, (n, k) = shape[0] if len(shape) == 3 else 1, shape[-2:]
+        _require(len(shape) in (2, 3) and min(shape) > 0, "a matrix [N, K] or matrices [matrices, N, K] that are not empty")
+        _require(matrices * n < 2 ** 31 and n <= 65535 * BLOCK8 and matrices <= 65535 and k < 2 ** 31 - 512, "sizes that 32 bits can count")
+        codes = torch.empty((matrices * n, -(-k // BLOCK8) * BLOCK8), dtype=torch.uint8, device=device)
+        return BlockMatrix(codes, torch.empty((matrices, -(-n // BLOCK8), -(-k // (4 * BLOCK8)), 512), dtype=torch.uint8, device=device), shape)
+
+    @staticmethod
+    def from_codes(codes: torch.Tensor, exponents: torch.Tensor) -> "BlockMatrix":
+        """From codes [N, K] or [matrices, N, K] (float8_e4m3fn, or their bytes as uint8) and the blocks' bytes [N / 128 up, K / 128 up] (exponent +
+        127, between 1 and 254; this reads them).  Both are copied into the layout above."""
+        _cuda(codes, exponents)
+        _require(codes.dim() in (2, 3) and codes.dtype in (torch.uint8, torch.float8_e4m3fn) and exponents.dtype is torch.uint8,
+                 "codes in 8 bits (float8_e4m3fn or uint8) and uint8 exponents")
+        made = BlockMatrix._empty(codes.shape, codes.device)
+        blocks = (-(-made.N // BLOCK8), -(-made.K // BLOCK8))
+        _require(tuple(exponents.shape) == (*codes.shape[:-2], *blocks) and exponents.device == codes.device,
+                 f"one exponent for each block of 128 x 128: {[*codes.shape[:-2], *blocks]}")
+        _require(bool(((exponents >= 1) & (exponents <= 254)).all()), "exponents are bytes between 1 and 254 (2^-126 to 2^127)")
+        made.codes.zero_()
+        made.codes[:, : made.K] = codes.reshape(-1, made.K).view(torch.uint8)
+        padded = torch.ones((made.matrices, blocks[0], made.scales.shape[2] * 4), dtype=torch.uint8, device=codes.device)
+        padded[:, :, : blocks[1]] = exponents.view(made.matrices, *blocks)
+        made.scales.copy_(padded.view(made.matrices, blocks[0], -1, 1, 4).expand(-1, -1, -1, 128, -1).reshape(made.scales.shape))
+        return made
+
+    def exponents(self) -> torch.Tensor:
+        """The blocks' bytes, exponent + 127: uint8 [N / 128 up, K / 128 up], with ``matrices`` ahead where there are several."""
+        found = self.scales[..., :4].flatten(2)[:, :, : -(-self.K // BLOCK8)]
+        return (found if len(self.shape) == 3 else found[0]).contiguous()
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """What the codes stand for (exact in bfloat16 but below its normal numbers)."""
+        _require(dtype in DTYPE_CODE, "values are bfloat16 or float32")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        (out_at, codes_at, scales_at), place = _addresses(out, self.codes, self.scales)
+        _check_place(place)
+        _check(library().zb_matrix_values(out_at, codes_at, scales_at, self.matrices, self.N, self.K, DTYPE_CODE[dtype], _stream()), "matrix_values")
+        return out
+
+    def tensors(self) -> list[torch.Tensor]:
+        return [self.codes, self.scales]
+
+
+def pack_matrix(w: torch.Tensor) -> BlockMatrix:
+    """``w`` [N, K] or [matrices, N, K], bfloat16 or float32 with contiguous rows, in 8-bit floating point with a scale for each block of
+    128 x 128 (``BlockMatrix``)."""
+    _require(w.dim() in (2, 3) and w.dtype in DTYPE_CODE and (w.stride(-1) == 1 or w.shape[-1] == 1), "w [N, K] or [matrices, N, K], bfloat16 or float32 "
+             "with unit inner stride")
+    _cuda(w)
+    made = BlockMatrix._empty(w.shape, w.device)
+    (codes_at, scales_at, w_at), place = _addresses(made.codes, made.scales, w)
+    _check_place(place)
+    _check(library().zb_pack_matrix(codes_at, scales_at, w_at, made.matrices, w.stride(0) if w.dim() == 3 else 0, w.stride(-2), made.N, made.K,
+                                    DTYPE_CODE[w.dtype], _stream()), "pack_matrix")
+    return made
+
+
+def _block8_run(rows: int) -> tuple[int, int]:
+    """How many of so many rows form a run of the product's, and how far apart the runs' places begin: as few runs as 256 rows
+    allow, of equal length (a multiple of 16)."""
+    runs = -(-rows // 256)
+    run = -(-rows // (16 * runs)) * 16
+    return run, 64 if rows <= 64 else 128 if rows <= 128 else 256
+
+
+def _check_block8_rows(x: torch.Tensor, K: int) -> int:
+    """Checks rows [M, K] as a product's input and gives their pitch."""
+    if x.dim() != 2 or x.shape[1] != K or x.dtype not in DTYPE_CODE:
+        raise InvalidArgumentError(f"x must be [M, {K}] in bfloat16 or float32, not {list(x.shape)} in {x.dtype}")
+    pitch, inner = x.stride()
+    if x.shape[0] <= 1:
+        pitch = K
+    if (inner != 1 and K > 1) or pitch < K:
+        raise InvalidArgumentError("x's rows must have unit inner stride and not overlap")
+    return pitch
+
+
+def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None = None, swiglu: bool = False, act: str = "silu",
+                 bounded: BoundedGate | None = None, product_act: str | None = None) -> torch.Tensor:
+    """x [M, K] (bfloat16 or float32) times a matrix [N, K] in 8-bit floating point: x's rows are coded as the matrix is, in blocks of 128
+    values, and y[m, n] = sum_k x~[m, k] w~[n, k] over what the codes stand for, summed in float32, in ``out_dtype`` (None: x's).  ``swiglu``: the rows of w are
+    blocks of 8 gate rows and their 8 up rows, and the result is act(gate) * up (``act`` "silu" or "relu"; ``bounded``: the bounded gate), [M, N /
+    2]; ``product_act`` (without ``swiglu``): one of ``PRODUCT_ACTS`` of the sums.  Up to 16 rows are coded inside the product's kernel, which streams
+    the matrix; more by a kernel of their own ahead of it."""
+    if w.matrices != 1 or len(w.shape) != 2:
+        raise InvalidArgumentError("a product takes one matrix")
+    M, K, N = x.shape[0], w.K, w.N
+    pitch = _check_block8_rows(x, K)
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in DTYPE_CODE:
+        raise InvalidArgumentError("the result is bfloat16 or float32")
+    kind, bias, limits = 0, None, (0.0, 1.0, 0.0)
+    if swiglu:
+        if product_act is not None or N % 16 != 0 or act not in ACTIVATIONS:
+            raise InvalidArgumentError(f"swiglu takes a multiple of 16 rows and one of {sorted(ACTIVATIONS)}")
+        kind = _BLOCK8_KINDS[act]
+        if bounded is not None:
+            bias, *limits = _bounded_args(bounded, N)
+            kind = 3
+    elif bounded is not None or product_act is not None:
+        if bounded is not None or product_act not in PRODUCT_ACTS:
+            raise InvalidArgumentError(f"an ungated product's epilogue is one of {sorted(PRODUCT_ACTS)}; the bounded gate is a gated one")
+        kind = 3 + PRODUCT_ACTS[product_act]
+    out = torch.empty((M, N // 2 if swiglu else N), dtype=out_dtype, device=x.device)
+    (out_at, x_at, codes_at, scales_at, _), place = _addresses(out, x, w.codes, w.scales, bounded.bias if bounded is not None else None)
+    _check_place(place)
+    if M == 0:
+        return out
+    lib, x_code, y_code, width = library(), DTYPE_CODE[x.dtype], DTYPE_CODE[out_dtype], out.shape[1]
+    if M <= BLOCK8_FEW_ROWS and lib.zb_gemm_block8_small_supported(M, N, K):
+        _check(lib.zb_gemm_block8_small(out_at, width, y_code, x_at, pitch, x_code, codes_at, scales_at, M, N, K, kind, bias, *limits, _stream()),
+               "gemm_block8_small")
+        return out
+    stream = _stream()
+    run, cap = _block8_run(M)
+    rows, row_scales = _block8_workspace(x, -(-M // run) * cap, cap, K)
+    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, x_at, pitch, None, M, K, run, cap, 0, None, None, x_code, stream), "code_rows")
+    _check(lib.zb_gemm_block8(out_at, width, y_code, rows.data_ptr(), row_scales, codes_at, scales_at, None, 0, 1, M, run, cap, N, K, kind, bias, None,
+                              *limits, _device_status_pointer(x.device), stream), "gemm_block8")
+    return out
+
+
+def _block8_workspace(x: torch.Tensor, places: int, cap: int, K: int) -> tuple[torch.Tensor, int]:
+    """Room for the codes of so many places and, behind them, their scales: the tensor that holds both, and the scales' address."""
+    codes = places * (-(-K // BLOCK8) * BLOCK8)
+    work = torch.empty(codes + places // cap * -(-cap // 128) * -(-K // 512) * 512, dtype=torch.uint8, device=x.device)
+    return work, work.data_ptr() + codes
+
+
+def block_feed_forward(x: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix, act: str = "silu", bounded: BoundedGate | None = None,
+                       out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """down(act(gate x) * up x) on matrices in 8-bit floating point: ``gate_up`` [2 ff, K] in blocks of 8 gate rows and their 8 up rows, ``down`` [N,
+    ff].  The hidden values stay in float32 until they are coded for the second product."""
+    if gate_up.matrices != 1 or down.matrices != 1 or gate_up.N != 2 * down.K:
+        raise InvalidArgumentError(f"gate_up [2 ff, K] and down [N, ff], not {list(gate_up.shape)} and {list(down.shape)}")
+    hidden = block_linear(x, gate_up, torch.float32, swiglu=True, act=act, bounded=bounded)
+    return block_linear(hidden, down, out_dtype or x.dtype)
+
+
+def _routed_blocks(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix, act: str,
+                   weigh_inputs: bool, bounded: BoundedGate | None) -> torch.Tensor:
+    """``routed_experts`` on matrices in 8-bit floating point: the rows are coded where they are gathered, the hidden values stay in float32 until
+    they are coded for the second product, an expert's output is rounded to x's type before it is weighted."""
+    T, width = x.shape
+    top, E, ff = ids.shape[1], gate_up.matrices, down.K
+    pitch = _check_block8_rows(x, gate_up.K)
+    if (len(gate_up.shape) != 3 or len(down.shape) != 3 or down.matrices != E or gate_up.N != 2 * ff or down.N != width or ff % 8 != 0):
+        raise InvalidArgumentError(f"expert matrices [E, 2 ff, width] and [E, width, ff], ff a multiple of 8, not {list(gate_up.shape)} and {list(down.shape)}")
+    out = torch.empty((T, width), dtype=x.dtype, device=x.device)
+    (out_at, x_at, ids_at, weights_at, up_at, up_scales, down_at, down_scales), place = _addresses(
+        out, x, ids, weights, gate_up.codes, gate_up.scales, down.codes, down.scales)
+    _check_place(place)
+    if T == 0 or top == 0:
+        return out.zero_()
+    lib, device, code, stream = library(), x.device, DTYPE_CODE[x.dtype], _stream()
+    status = _device_status_pointer(device)
+    num_slots = T * top
+    run = lib.zb_gemm_tc_experts_run(num_slots, E)
+    runs = num_slots // run + E
+    places = runs * run
+    numbers = torch.empty(1 + 3 * runs + places + num_slots, dtype=torch.int32, device=device)
+    plan = numbers.data_ptr()
+    slots = plan + 4 * (1 + 3 * runs)
+    place_of_slot = slots + 4 * places
+    _check(lib.zb_route_align_strided(plan, slots, place_of_slot, ids_at, num_slots, E, runs, run, places, stream), "route_align")
+    kind = 3 if bounded is not None else _BLOCK8_KINDS[act]
+    bounds = (float(bounded.limit), float(bounded.alpha), float(bounded.shift)) if bounded is not None else (0.0, 1.0, 0.0)
+    rows, row_scales = _block8_workspace(x, places, run, width)
+    place_scale = torch.empty(places, dtype=torch.float32, device=device) if weigh_inputs else None
+    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, x_at, pitch, slots, places, width, run, run, top, _ptr(place_scale), weights_at, code,
+                            stream), "code_rows")
+    hidden = torch.empty((places, ff), dtype=torch.float32, device=device)
+    _check(lib.zb_gemm_block8(hidden.data_ptr(), ff, 0, rows.data_ptr(), row_scales, up_at, up_scales, plan, runs, E, 0, run, run, 2 * ff, width, kind,
+                              None, _ptr(place_scale), *bounds, status, stream), "gemm_block8")
+    rows, row_scales = _block8_workspace(x, places, run, ff)
+    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, hidden.data_ptr(), ff, slots, places, ff, run, run, 0, None, None, 0, stream), "code_rows")
+    y = torch.empty((places, width), dtype=x.dtype, device=device)
+    _check(lib.zb_gemm_block8(y.data_ptr(), width, code, rows.data_ptr(), row_scales, down_at, down_scales, plan, runs, E, 0, run, run, width, ff, 0,
+                              None, None, 0.0, 1.0, 0.0, status, stream), "gemm_block8")
+    _check(lib.zb_route_combine(out_at, y.data_ptr(), width, code, x_at, pitch, ids_at, None if weigh_inputs else weights_at, place_of_slot, T, width,
+                                top, code, stream), "route_combine")
+    return out
 
 
 # ------------------------------------------------------------------------------ sampling
