@@ -151,11 +151,11 @@ def test_activations_of_the_sums(m, form):
 
 
 # ------------------------------------------------------------------------------------------------- feed-forwards and experts
-def _feed_forward(x, up, down, act):
+def _feed_forward(x, up, down, act, limits=LIMITS, bias=None):
     """The value in 64 bits and a bound on its error ahead of the last rounding."""
     sums, magnitude = plain.product(x, up)
-    hidden = plain.gated(sums, act, LIMITS)
-    off = plain.gated_error(sums, plain.sum_error(up.shape[1]) * magnitude, act, LIMITS)
+    hidden = plain.gated(sums, act, limits, bias)
+    off = plain.gated_error(sums, plain.sum_error(up.shape[1]) * magnitude, act, limits, bias)
     want, size = plain.product(hidden, down)
     return want, plain.code_spread(hidden, off) @ down.abs().t() * (1 + 1e-4) + plain.sum_error(down.shape[1]) * size * 1.01
 

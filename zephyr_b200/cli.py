@@ -64,6 +64,7 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--max-prefill-chunk-tokens", type=_positive_int)
     gen.add_argument("--kv-block-size", type=_positive_int, default=16)
     gen.add_argument("--kv-bits", type=int, choices=(4,), help="hold keys and values in 4 bits: 3.2 times as many positions, slower prompts (default: in the model's type)")
+    gen.add_argument("--weight-bits", type=int, choices=(8,), help="hold the layers' matrices in 8-bit floating point with a scale for each block of 128 x 128: half the memory, faster products (default: in the model's type)")
     gen.add_argument("--num-kv-blocks", type=_positive_int, help="fix the number of cache pages")
     gen.add_argument("--json", action="store_true", help="print one JSON object per request")
     gen.add_argument("--log-level", choices=("critical", "error", "warning", "info", "debug", "trace"), default="warning")
@@ -108,7 +109,7 @@ def _generate(args, parser) -> int:
                         gpu_memory_utilization=args.gpu_memory_utilization,
                         scheduler=PagedSchedulerConfig(**scheduler_args),
                         kv_cache=KvCacheOptions(block_size=args.kv_block_size, num_blocks=args.num_kv_blocks,
-                                                bits=args.kv_bits))
+                                                bits=args.kv_bits), weight_bits=args.weight_bits)
         params = GenerationParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k,
                                   top_p=args.top_p, min_p=args.min_p, frequency_penalty=args.frequency_penalty,
                                   presence_penalty=args.presence_penalty, repetition_penalty=args.repetition_penalty,

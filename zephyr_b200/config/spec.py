@@ -133,6 +133,7 @@ class ModelSpec:
     output: OutputSpec
     eos_token_ids: tuple[int, ...] = ()
     ignorable_weights: tuple[str, ...] = ()   # names a checkpoint may carry that are not read
+    weight_bits: int = 0                      # 8: the layers' large matrices in 8-bit floating point; 0: in the model's type
 
     @property
     def num_caches(self) -> int:

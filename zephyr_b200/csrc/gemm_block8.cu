@@ -112,9 +112,9 @@ __device__ __forceinline__ unsigned tc_idesc_scaled_pair(unsigned n) { return ((
 template <int RUN, typename TOut, bool GATED, bool SCALED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_block8_kernel(const __grid_constant__ Block8Args a) {
   using Shape = Block8Shape<RUN>;
-  extern __shared__ unsigned char g8_smem_raw[];
+  extern __shared__ unsigned char smem_raw[];
   __shared__ Block8Shared sh;
-  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(g8_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* scale_ring = ring + Shape::STAGES * Shape::STAGE_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_rank()), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;

@@ -54,14 +54,14 @@ static size_t block8_small_smem(int blocks, int token_tiles) {
 template <int MT, int TEAM, typename TOut, bool GATED>
 __global__ void __launch_bounds__(G9_WARPS * 32, 1) gemm_block8_small_kernel(const Block8SmallArgs a) {
   constexpr int TEAMS = G9_WARPS / TEAM, SUMS = MT * 128;
-  extern __shared__ __align__(16) unsigned char g9_smem[];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / TEAM, slice = warp % TEAM;
   const int g = lane >> 2, t = lane & 3;
   const int split = gridDim.y, part = blockIdx.y;
   const int all_blocks = b8_blocks(a.K), pieces = b8_pieces(a.K), pitch = all_blocks * B8_BLOCK;
   // This CTA's blocks of K begin on a piece of scales, so that a warp of its codes 512 values at a time.
   const int first_block = pieces * part / split * 4, end_block = min(pieces * (part + 1) / split * 4, all_blocks), blocks = end_block - first_block;
-  float* red = reinterpret_cast<float*>(g9_smem);            // (where it is in every CTA of a cluster)
+  float* red = reinterpret_cast<float*>(smem_raw);            // (where it is in every CTA of a cluster)
   uint4* rings = reinterpret_cast<uint4*>(red + G9_WARPS * SUMS);
   uint4* ring = rings + warp * G9_DEPTH * 64 + lane;
   uint4* x_s = rings + G9_WARPS * G9_DEPTH * 64;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(G9_WARPS * 32, 1) gemm_block8_small_kernel(con
   auto scale_of = [&](int tile) {
     const int b = b_begin + lane;
     return tile < tiles && b < b_end
-               ? b8_power(a.scales[(static_cast<size_t>(tile * 16 / B8_BLOCK) * pieces + b / 4) * B8_PIECE + b % 4]) : 0.0f;
+               ? b8_power(*(a.scales + (static_cast<size_t>(tile * 16 / B8_BLOCK) * pieces + b / 4) * B8_PIECE + b % 4)) : 0.0f;
   };
 #pragma unroll
   for (int u = 0; u < G9_DEPTH; ++u) copy_next();

@@ -24,7 +24,7 @@ import torch
 
 from ..config import ConfigError, InvalidArgumentError, load_model_config
 from ..kernels import ops
-from ..parts import Model, with_cache_bits
+from ..parts import Model, with_cache_bits, with_weight_bits
 from ..sampling import MT19937_64, Sampler, SamplingParams
 from ..weights import Checkpoint
 from .params import (Choice, FinishReason, GenerationOutput, GenerationParams, KvCacheOptions, RequestStatus, Usage)
@@ -76,12 +76,14 @@ class _Flight:
 
 
 class Engine:
-    """One model on one GPU; synchronous batch generation."""
+    """One model on one GPU; synchronous batch generation.  ``weight_bits`` = 8 holds the layers' large matrices in 8-bit floating point with a
+    scale for each block of 128 x 128, made from the model's own as it is loaded (``parts.with_weight_bits``)."""
 
     def __init__(self, model: str | Path, *, dtype: str | torch.dtype = "bfloat16", max_seq_len: int = 0,
                  gpu_memory_utilization: float = 0.9, scheduler: PagedSchedulerConfig | None = None,
                  kv_cache: KvCacheOptions | None = None, eos_token_ids: Sequence[int] | None = None,
-                 devices: Sequence[int] = (0,), weights: Any = None, model_config: Any = None):
+                 devices: Sequence[int] = (0,), weights: Any = None, model_config: Any = None,
+                 weight_bits: int | None = None):
         if not torch.cuda.is_available():
             raise ops.KernelError("zephyr_b200 needs a CUDA device (sm_100a); there is no CPU path")
         if len(tuple(devices)) != 1:
@@ -107,6 +109,10 @@ class Engine:
             if not ops.packed_page_size_ok(kv_cache.block_size):
                 raise ConfigError("a cache in 4 bits takes a block_size of 16 or a larger power of two")
             spec = with_cache_bits(spec, kv_cache.bits, limit)
+        if weight_bits is not None:
+            if self.dtype != torch.bfloat16:
+                raise ConfigError("matrices in 8 bits are built for bfloat16 models")
+            spec = with_weight_bits(spec, weight_bits)
         self.generation_defaults = self._read_generation_defaults(model) if model is not None else {}
         store = weights if weights is not None else Checkpoint(model)
         self.model = Model.load(spec, store, self.dtype, self.device)

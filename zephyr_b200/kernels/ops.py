@@ -2591,6 +2591,7 @@ class BlockMatrix:
     127) of four neighbouring blocks of K for each of a block's 128 rows, as the tensor cores read them."""
 
     __slots__ = ("codes", "scales", "matrices", "N", "K", "shape", "device")
+    dtype = torch.float8_e4m3fn
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Sequence[int]):
         self.codes, self.scales, self.shape, self.device = codes, scales, torch.Size(shape), codes.device
@@ -2599,8 +2600,8 @@ class BlockMatrix:
 
     @staticmethod
     def _empty(shape: Sequence[int], device) -> "BlockMatrix":
-        matrices, (n, k) = shape[0] if len(shape) == 3 else 1, shape[-2:]
         _require(len(shape) in (2, 3) and min(shape) > 0, "a matrix [N, K] or matrices [matrices, N, K] that are not empty")
+        matrices, (n, k) = shape[0] if len(shape) == 3 else 1, shape[-2:]
         _require(matrices * n < 2 ** 31 and n <= 65535 * BLOCK8 and matrices <= 65535 and k < 2 ** 31 - 512, "sizes that 32 bits can count")
         codes = torch.empty((matrices * n, -(-k // BLOCK8) * BLOCK8), dtype=torch.uint8, device=device)
         return BlockMatrix(codes, torch.empty((matrices, -(-n // BLOCK8), -(-k // (4 * BLOCK8)), 512), dtype=torch.uint8, device=device), shape)
@@ -2624,6 +2625,11 @@ class BlockMatrix:
         made.scales.copy_(padded.view(made.matrices, blocks[0], -1, 1, 4).expand(-1, -1, -1, 128, -1).reshape(made.scales.shape))
         return made
 
+    def first_rows(self, rows: int) -> "BlockMatrix":
+        """The first rows of one matrix, a multiple of 128 of them, over the same memory."""
+        _require(len(self.shape) == 2 and 0 < rows <= self.N and (rows % BLOCK8 == 0 or rows == self.N), "whole blocks of a matrix's rows")
+        return BlockMatrix(self.codes[:rows], self.scales[:, : -(-rows // BLOCK8)], (rows, self.K))
+
     def exponents(self) -> torch.Tensor:
         """The blocks' bytes, exponent + 127: uint8 [N / 128 up, K / 128 up], with ``matrices`` ahead where there are several."""
         found = self.scales[..., :4].flatten(2)[:, :, : -(-self.K // BLOCK8)]
@@ -2645,8 +2651,8 @@ class BlockMatrix:
 def pack_matrix(w: torch.Tensor) -> BlockMatrix:
     """``w`` [N, K] or [matrices, N, K], bfloat16 or float32 with contiguous rows, in 8-bit floating point with a scale for each block of
     128 x 128 (``BlockMatrix``)."""
-    _require(w.dim() in (2, 3) and w.dtype in DTYPE_CODE and (w.stride(-1) == 1 or w.shape[-1] == 1), "w [N, K] or [matrices, N, K], bfloat16 or float32 "
-             "with unit inner stride")
+    _require(w.dim() in (2, 3) and w.numel() > 0 and w.dtype in DTYPE_CODE and (w.stride(-1) == 1 or w.shape[-1] == 1),
+             "w [N, K] or [matrices, N, K], not empty, bfloat16 or float32 with unit inner stride")
     _cuda(w)
     made = BlockMatrix._empty(w.shape, w.device)
     (codes_at, scales_at, w_at), place = _addresses(made.codes, made.scales, w)

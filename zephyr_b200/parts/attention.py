@@ -303,6 +303,15 @@ class Attention(Mixer):
                 decls[p[name]] = WeightDecl((size,), ROLE_ZERO)
         return decls
 
+    block_matrices = ("w_qkv", "w_o")
+
+    def hold_in_8_bits(self) -> bool:
+        queries = self.w_q.shape[0]
+        super().hold_in_8_bits()
+        # The queries' rows alone, for a layer that reads another layer's cache: a view where they end with a block.
+        self.w_q = self.w_qkv.first_rows(queries) if queries % ops.BLOCK8 == 0 else ops.pack_matrix(self.w_q)
+        return True
+
     def weights_read(self) -> list[torch.Tensor]:
         return [t for t in (self.w_qkv, self.w_o, self.q_norm, self.k_norm, self.head_mix, self.score_mix) if t is not None]
 

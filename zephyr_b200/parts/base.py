@@ -20,6 +20,7 @@ import torch
 from ..cache import CacheStorage, PagedCacheSpec, StateCacheSpec
 from ..config.errors import ConfigError
 from ..config.spec import FeedForwardSpec, InputSpec, LayerCall, MixerSpec, NormSpec, OutputSpec, PositionSpec, SideSpec
+from ..kernels import ops
 from ..weights.loader import WeightDecl
 
 
@@ -78,15 +79,29 @@ class Part:
     # belongs to steps whose rows bring the same numbers of tokens).
     graph_safe = False
 
+    # The names of the matrices that may be held in 8-bit floating point: those the part hands to ``ops.linear`` and its likes, which take
+    # a ``BlockMatrix`` in a matrix's place.
+    block_matrices: tuple[str, ...] = ()
+
+    def hold_in_8_bits(self) -> bool:
+        """Puts ``block_matrices`` into 8-bit floating point with a scale for each block of 128 x 128; whether there were any.  A part
+        without any keeps its tensors as they are."""
+        for name in self.block_matrices:
+            w = getattr(self, name)
+            if isinstance(w, torch.Tensor):
+                setattr(self, name, ops.pack_matrix(w))
+        return len(self.block_matrices) > 0
+
     @staticmethod
     def weight_decls(spec) -> dict[str, WeightDecl]:
         """Full tensor names this part reads, with shapes and roles."""
         return {}
 
-    def weights_read(self) -> list[torch.Tensor]:
+    def weights_read(self) -> list["torch.Tensor | ops.BlockMatrix"]:
         """The weight tensors one forward pass reads.  Some may share memory (the query rows of a fused
         q/k/v matrix); whoever adds up bytes counts a piece of memory once."""
-        return [value for value in vars(self).values() if isinstance(value, torch.Tensor) and value.is_floating_point()]
+        return [value for value in vars(self).values()
+                if isinstance(value, ops.BlockMatrix) or (isinstance(value, torch.Tensor) and value.is_floating_point())]
 
 
 class Norm(Part):

@@ -85,9 +85,22 @@ class SwiGLU(FeedForward):
                 decls[p[key]] = WeightDecl((size,), ROLE_ZERO)
         return decls
 
+    block_matrices = ("w_gate_up", "w_down")
+
+    def hold_in_8_bits(self) -> bool:
+        if not self.blocked:
+            raise ConfigError(f"a gated feed-forward in 8-bit floating point is a multiple of 8 wide, not {self.intermediate}")
+        return super().hold_in_8_bits()
+
     def as_gated_products(self) -> tuple[torch.Tensor, torch.Tensor] | None:
         # The chain of small products has SiLU in its epilogue; another activation keeps the layer off it.
-        return (self.w_gate_up, self.w_down) if self.blocked and self.activation == "silu" else None
+        chained = self.blocked and self.activation == "silu" and isinstance(self.w_down, torch.Tensor)
+        return (self.w_gate_up, self.w_down) if chained else None
+
+    def _block_forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        bounded = ops.BoundedGate(self.b_gate_up, self.limit, self.alpha, self.up_shift) if self.clamped else None
+        return ops.block_feed_forward(x, self.w_gate_up, self.w_down, act="silu" if self.clamped else self.activation, bounded=bounded,
+                                      out_dtype=out_dtype)
 
     def _bounded_hidden(self, x: torch.Tensor) -> torch.Tensor:
         # Biases, bounds and the gate where the products' float32 sums leave the tensor cores: a decode step's
@@ -105,10 +118,14 @@ class SwiGLU(FeedForward):
 
     def forward_summands(self, x: torch.Tensor) -> tuple[torch.Tensor, ...]:
         if self.clamped and self.b_down is not None:      # the last bias joins the sum into the stream, in float32
+            if isinstance(self.w_down, ops.BlockMatrix):
+                return self._block_forward(x), self.b_down
             return ops.linear(self._bounded_hidden(x), self.w_down), self.b_down
         return (self.forward(x),)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if isinstance(self.w_down, ops.BlockMatrix):
+            return self._block_forward(x) if self.b_down is None else ops.add_bias(self._block_forward(x, torch.float32), self.b_down)
         if self.clamped:
             hidden = self._bounded_hidden(x)
             if self.b_down is None:
@@ -145,7 +162,11 @@ class UngatedFeedForward(FeedForward):
         hidden, inter = int(p["hidden_size"]), int(p["intermediate_size"])
         return {p["up_proj"]: WeightDecl((inter, hidden), ROLE_LINEAR), p["down_proj"]: WeightDecl((hidden, inter), ROLE_LINEAR)}
 
+    block_matrices = ("w_up", "w_down")
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if isinstance(self.w_up, ops.BlockMatrix):      # (the hidden values in float32 until they are coded)
+            return ops.block_linear(ops.block_linear(x, self.w_up, torch.float32, product_act=self.activation), self.w_down, x.dtype)
         if x.shape[0] <= ops.SMALL_GEMM_ROWS and ops.gemm_small_supported(x, self.w_up):
             hidden = ops.gemm_small(x, self.w_up, product_act=self.activation)
         elif ((x.shape[0] >= ops.GEMM_TC_MIN_ROWS or not ops.USE_LIBRARY_PRODUCTS)

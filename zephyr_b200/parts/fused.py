@@ -85,7 +85,8 @@ class DecodeChains:
                 return None
             plans.append(plan)
         for call in run_order:
-            if plans[call.layer].mixer.projections(call) is None:
+            matrices = plans[call.layer].mixer.projections(call)
+            if matrices is None or not all(isinstance(w, torch.Tensor) for w in matrices):
                 return None
         return cls(plans, run_order, hidden)
 

@@ -114,6 +114,8 @@ class LatentAttention(Mixer):
             decls[p["sinks"]] = WeightDecl((nh,), ROLE_ZERO)
         return decls
 
+    block_matrices = ("w_in", "w_q_up", "w_o")          # (the maps into and out of the latent space are products head by head)
+
     def weights_read(self) -> list[torch.Tensor]:
         return [w for w in (self.w_in, self.w_q_up, self.q_norm, self.w_q_to_latent, self.w_latent_to_v, self.w_o,
                             self.latent_norm) if w is not None]

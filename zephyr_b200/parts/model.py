@@ -113,6 +113,14 @@ def with_cache_bits(spec: ModelSpec, bits: int, max_positions: int = 0) -> Model
     return dataclasses.replace(spec, layers=layers)
 
 
+def with_weight_bits(spec: ModelSpec, bits: int) -> ModelSpec:
+    """``spec`` with the layers' large matrices (projections, feed-forwards, experts) held in 8-bit floating point with a scale for each block of
+    128 x 128; tables, the vocabulary projection, routers, norms, and what a layer multiplies head by head stay in the model's type."""
+    if bits != 8:
+        raise ConfigError(f"matrices are held in the model's type or in 8 bits, not in {bits}")
+    return dataclasses.replace(spec, weight_bits=bits)
+
+
 def run_order_for(layers) -> tuple:
     """Every layer once, in order, each with stores of its own: as many cache ids as its mixer keeps stores."""
     from ..config.spec import LayerCall
@@ -153,6 +161,8 @@ class Model:
                                      ffn(layer.feed_forward, weights, dtype) if ffn is not None else None,
                                      {name: cls(layer.norms[name], weights, dtype) for name, cls in norms.items()},
                                      **extra))
+        if spec.weight_bits:
+            self._hold_in_8_bits()
         self.cache_specs = cache_specs(spec)
         if len(self.cache_specs) > spec.num_caches:
             self.input.cache_id = spec.num_caches
@@ -178,6 +188,13 @@ class Model:
         self._layer_bytes = None
         self._side_stream = None
 
+    def _hold_in_8_bits(self) -> None:
+        if self.spec.weight_bits != 8 or self.dtype != torch.bfloat16:
+            raise ConfigError("matrices in fewer bits are built for 8 bits and bfloat16 models")
+        found = [part.hold_in_8_bits() for block in self.layers for part in (block.mixer, block.feed_forward) if part is not None]
+        if not any(found):
+            raise ConfigError("this model has no matrices that could be held in 8 bits")
+
     @classmethod
     def load(cls, spec: ModelSpec, store: WeightStore, dtype: torch.dtype, device: torch.device | str) -> "Model":
         weights = load_weights(store, expected_weights(spec), dtype, device, spec.ignorable_weights)
@@ -189,7 +206,11 @@ class Model:
         by_storage: dict[int, dict[tuple[int, int], int]] = {}     # storage -> {(address, bytes) of a tensor}
         sizes: dict[int, int] = {}
 
-        def add(t: torch.Tensor) -> None:
+        def add(t: "torch.Tensor | ops.BlockMatrix") -> None:
+            if isinstance(t, ops.BlockMatrix):
+                for tensor in t.tensors():
+                    add(tensor)
+                return
             storage = t.untyped_storage()
             sizes[storage.data_ptr()] = storage.nbytes()
             by_storage.setdefault(storage.data_ptr(), {})[(t.data_ptr(), t.numel() * t.element_size())] = 1

@@ -100,6 +100,8 @@ class GatedLinearAttention(Mixer):
             p["a2_bias"]: WeightDecl((hd,), ROLE_ZERO),
         }
 
+    block_matrices = ("w_in", "w_o")
+
     def weights_read(self) -> list[torch.Tensor]:
         return [self.w_in, self.w_a2, self.w_o, self.a2_bias, self.norm]
 
@@ -173,6 +175,8 @@ class Mamba2(Mixer):
             p["skip"]: WeightDecl((heads,), ROLE_NORM), p["norm"]: WeightDecl((inner,), ROLE_NORM),
             p["o"]: WeightDecl((hidden, inner), ROLE_LINEAR),
         }
+
+    block_matrices = ("w_in", "w_o")
 
     def weights_read(self) -> list[torch.Tensor]:
         return [self.w_in, self.w_o, self.conv_w, self.conv_b, self.norm]
@@ -261,6 +265,8 @@ class GatedDeltaRule(Mixer):
             p["a_log"]: WeightDecl((heads,), ROLE_ZERO), p["dt_bias"]: WeightDecl((heads,), ROLE_ZERO),
             p["norm"]: WeightDecl((int(p["value_dim"]),), ROLE_NORM), p["o"]: WeightDecl((hidden, hv), ROLE_LINEAR),
         }
+
+    block_matrices = ("w_in", "w_g", "w_o")
 
     def weights_read(self) -> list[torch.Tensor]:
         return [self.w_in, self.w_g, self.w_o, self.conv_w, self.norm]
@@ -367,6 +373,8 @@ class Retention(Mixer):
                 p["v"]: WeightDecl((hv, hidden), ROLE_LINEAR), p["g"]: WeightDecl((hv, hidden), ROLE_LINEAR),
                 p["o"]: WeightDecl((hidden, hv), ROLE_LINEAR)}
 
+    block_matrices = ("w_in", "w_o")
+
     def weights_read(self) -> list[torch.Tensor]:
         return [self.w_in, self.w_o]
 
@@ -441,6 +449,9 @@ class ParallelMixers(Mixer):
         for sub, _ in spec.params["branches"]:
             decls.update(lookup(MIXERS, "mixer", sub.kind).weight_decls(sub))
         return decls
+
+    def hold_in_8_bits(self) -> bool:
+        return any([branch.hold_in_8_bits() for branch in self.branches])
 
     def weights_read(self) -> list[torch.Tensor]:
         return [tensor for branch in self.branches for tensor in branch.weights_read()]

@@ -116,6 +116,15 @@ class RoutedFeedForward(FeedForward):
             decls.update(lookup(FEED_FORWARDS, "feed-forward", "gated").weight_decls(FeedForwardSpec("gated", p["shared"])))
         return decls
 
+    block_matrices = ("w_gate", "w_down")              # (the router stays in the model's type)
+
+    def hold_in_8_bits(self) -> bool:
+        if self.w_up is not None:
+            raise ConfigError(f"experts in 8-bit floating point are a multiple of 8 wide, not {self.intermediate}")
+        if self.shared is not None:
+            self.shared.hold_in_8_bits()
+        return super().hold_in_8_bits()
+
     def weights_read(self) -> list[torch.Tensor]:
         own = [w for w in (self.w_router, self.w_gate, self.w_up, self.w_down) if w is not None]
         return own + (self.shared.weights_read() if self.shared is not None else [])
