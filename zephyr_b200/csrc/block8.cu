@@ -5,59 +5,98 @@
 
 namespace zb {
 
-// One CTA a block of 128 x 128: 16 warps, eight rows a warp, four values a lane, held in registers between the look at the largest
-// and the conversion, so that the matrix is read once.
-constexpr int B8_PACK_THREADS = 512;
+// One CTA a block of 128 x 128, 256 threads: a thread takes PER neighbouring values (16 bytes) of every (256 * PER / 128)-th row and keeps them
+// between the look at the largest and the conversion, so that the matrix is read once.
+constexpr int B8_PACK_THREADS = 256;
 
-__device__ __forceinline__ void load4(const float* p, int left, bool wide, float (&v)[4]) {
-  if (wide && left >= 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-  } else {
+template <typename T> struct PackValues;
+template <> struct PackValues<__nv_bfloat16> {
+  static constexpr int PER = 8;
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int left, bool wide) {
+    if (wide && left >= 8) {
+      u = *reinterpret_cast<const uint4*>(p);
+    } else {
+      unsigned w[4];
+      const unsigned short* bits = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.0f;
+      for (int i = 0; i < 4; ++i) w[i] = (2 * i < left ? bits[2 * i] : 0u) | (2 * i + 1 < left ? static_cast<unsigned>(bits[2 * i + 1]) << 16 : 0u);
+      u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
-}
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, int left, bool wide, float (&v)[4]) {
-  if (wide && left >= 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-    v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? __bfloat162float(p[i]) : 0.0f;
+  __device__ __forceinline__ float value(int i) const {
+    const unsigned w = i / 2 == 0 ? u.x : i / 2 == 1 ? u.y : i / 2 == 2 ? u.z : u.w;
+    return __uint_as_float(i % 2 == 0 ? w << 16 : w & 0xffff0000u);
   }
-}
+  __device__ __forceinline__ unsigned largest() const {
+    const unsigned m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
+};
+template <> struct PackValues<float> {
+  static constexpr int PER = 4;
+  float4 f;
+  __device__ __forceinline__ void load(const float* p, int left, bool wide) {
+    if (wide && left >= 4) f = *reinterpret_cast<const float4*>(p);
+    else f = make_float4(0 < left ? p[0] : 0.0f, 1 < left ? p[1] : 0.0f, 2 < left ? p[2] : 0.0f, 3 < left ? p[3] : 0.0f);
+  }
+  __device__ __forceinline__ float value(int i) const { return i == 0 ? f.x : i == 1 ? f.y : i == 2 ? f.z : f.w; }
+  __device__ __forceinline__ unsigned largest() const {
+    return max(max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu), max(__float_as_uint(f.z) & 0x7fffffffu, __float_as_uint(f.w) & 0x7fffffffu));
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(B8_PACK_THREADS)
 pack_matrix_kernel(unsigned char* codes, unsigned char* scales, const T* w, long long matrix_stride, long long ldw, int N, int K, bool wide) {
-  const int kb = blockIdx.x, nb = blockIdx.y, matrix = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int PER = PackValues<T>::PER, LANES = B8_BLOCK / PER, STEP = B8_PACK_THREADS / LANES, ROWS = B8_BLOCK / STEP;
+  const int kb = blockIdx.x, nb = blockIdx.y, matrix = blockIdx.z;
   const int pitch = b8_pitch(K), pieces = b8_pieces(K);
   const T* source = w + matrix * matrix_stride;
-  const int k = kb * B8_BLOCK + 4 * lane;
-  float v[8][4];
+  const int k = kb * B8_BLOCK + threadIdx.x % LANES * PER, row0 = nb * B8_BLOCK + threadIdx.x / LANES;
+  PackValues<T> v[ROWS];
   unsigned largest = 0;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int row = nb * B8_BLOCK + warp + 16 * r;
-    load4(source + static_cast<long long>(row < N ? row : 0) * ldw + k, row < N ? K - k : 0, wide, v[r]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) largest = max(largest, b8_magnitude(v[r][i]));
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + STEP * r;
+    v[r].load(source + static_cast<long long>(row < N ? row : 0) * ldw + (k < K ? k : 0), row < N ? K - k : 0, wide);
   }
-  __shared__ unsigned parts[B8_PACK_THREADS / 32];
-  largest = __reduce_max_sync(0xffffffffu, largest);
-  if (lane == 0) parts[warp] = largest;
-  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < B8_PACK_THREADS / 32; ++i) largest = max(largest, parts[i]);
+  for (int r = 0; r < ROWS; ++r) largest = max(largest, v[r].largest());
+  __shared__ unsigned parts[2][B8_PACK_THREADS / 32];
+  auto block_largest = [&](unsigned own, unsigned* parts_of) {
+    own = __reduce_max_sync(0xffffffffu, own);
+    if (threadIdx.x % 32 == 0) parts_of[threadIdx.x / 32] = own;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < B8_PACK_THREADS / 32; ++i) own = max(own, parts_of[i]);
+    return own;
+  };
+  largest = block_largest(largest, parts[0]);
+  const bool wild = largest >= 0x7f800000u;           // something is not finite: the largest of what is
+  if (wild) {
+    largest = 0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) largest = max(largest, b8_magnitude(v[r].value(i)));
+    largest = block_largest(largest, parts[1]);
+  }
   const unsigned byte = b8_scale_byte(largest);
   const float inverse = b8_inverse(byte);
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int row = nb * B8_BLOCK + warp + 16 * r;
-    if (row < N)
-      *reinterpret_cast<unsigned*>(codes + (static_cast<size_t>(matrix) * N + row) * pitch + k) = b8_codes(v[r][0], v[r][1], v[r][2], v[r][3], inverse);
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + STEP * r;
+    if (row >= N) continue;
+    unsigned c[PER / 4];
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      const float a = v[r].value(4 * i), b = v[r].value(4 * i + 1), d = v[r].value(4 * i + 2), e = v[r].value(4 * i + 3);
+      c[i] = wild ? b8_codes(a, b, d, e, inverse) : b8_codes_finite(make_float2(a, b), make_float2(d, e), make_float2(inverse, inverse));
+    }
+    unsigned char* to = codes + (static_cast<size_t>(matrix) * N + row) * pitch + k;
+    if constexpr (PER == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<unsigned*>(to) = c[0];
   }
   // The scale's 128 copies; behind the last block of K the piece is filled with the scale of zeros.
   unsigned char* piece = scales + ((static_cast<size_t>(matrix) * gridDim.y + nb) * pieces + kb / 4) * B8_PIECE;
@@ -69,34 +108,44 @@ pack_matrix_kernel(unsigned char* codes, unsigned char* scales, const T* w, long
   }
 }
 
+// 16 codes a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
-matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* scales, int N, int K, bool wide) {
-  const int row = blockIdx.x, matrix = blockIdx.y, pitch = b8_pitch(K), pieces = b8_pieces(K);
-  const unsigned char* from = codes + (static_cast<size_t>(matrix) * N + row) * pitch;
-  const unsigned char* piece = scales + (static_cast<size_t>(matrix) * b8_blocks(N) + row / B8_BLOCK) * pieces * B8_PIECE;
-  T* to = out + (static_cast<size_t>(matrix) * N + row) * K;
-  for (int k = threadIdx.x * 4; k < K; k += blockDim.x * 4) {
-    const unsigned c = *reinterpret_cast<const unsigned*>(from + k);
-    const float scale = b8_power(piece[static_cast<size_t>(k / (4 * B8_BLOCK)) * B8_PIECE + k / B8_BLOCK % 4]);
-    unsigned h[2];
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[0]) : "h"(static_cast<unsigned short>(c)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[1]) : "h"(static_cast<unsigned short>(c >> 16)));
-    float v[4];
+matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* scales, long long rows, int N, int K, bool wide) {
+  const int pitch = b8_pitch(K), pieces = b8_pieces(K), units = (K + 15) / 16;
+  const long long unit = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, row = unit / units;
+  if (row >= rows) return;
+  const int k = static_cast<int>(unit % units) * 16;
+  const long long matrix = row / N;
+  const int group = static_cast<int>(row % N) / B8_BLOCK;
+  const uint4 c = *reinterpret_cast<const uint4*>(codes + row * pitch + k);
+  const float scale = b8_power(scales[((matrix * b8_blocks(N) + group) * pieces + k / (4 * B8_BLOCK)) * B8_PIECE + k / B8_BLOCK % 4]);
+  const unsigned words[4] = {c.x, c.y, c.z, c.w};
+  float v[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f;
-      asm("cvt.f32.f16 %0, %1;\n" : "=f"(f) : "h"(static_cast<unsigned short>(h[i / 2] >> (16 * (i % 2)))));
-      v[i] = f * scale;
-    }
-    if (wide) {
-      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to + k) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-      else *reinterpret_cast<float4*>(to + k) = make_float4(v[0], v[1], v[2], v[3]);
+  for (int i = 0; i < 8; ++i) {
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(static_cast<unsigned short>(words[i / 2] >> (16 * (i % 2)))));
+    float lo, hi;
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.f32.f16 %0, l;\ncvt.f32.f16 %1, h;\n}\n" : "=f"(lo), "=f"(hi) : "r"(h));
+    v[2 * i] = lo * scale;
+    v[2 * i + 1] = hi * scale;
+  }
+  T* to = out + row * K + k;
+  if (wide) {                                     // (K is a multiple of 16)
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                                                           pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (k + i < K) to[k + i] = from_float<T>(v[i]);
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k + i < K) to[i] = from_float<T>(v[i]);
   }
 }
 
@@ -136,10 +185,11 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
     place = index / a.run * a.cap + index % a.run;
   }
   const int k = piece * 512 + lane * 16;
-  float v[16];
-  b8_load16(static_cast<const T*>(a.x) + row * a.ldx + k, a.K - k, a.wide, v);
-  unsigned scales;
-  const uint4 codes = b8_code_row_piece(v, scales);
+  B8Values<T> v;
+  v.load(static_cast<const T*>(a.x) + row * a.ldx + k, a.K - k, a.wide);
+  unsigned byte;
+  const uint4 codes = b8_code_row_piece(v, byte);
+  const unsigned scales = b8_four_bytes(byte);
   const int pitch = b8_pitch(a.K);
   if (k < pitch) *reinterpret_cast<uint4*>(a.codes + place * pitch + k) = codes;
   if (lane == 0) {
@@ -160,7 +210,7 @@ ZB_API int zb_pack_matrix(void* codes, void* scales, const void* w, int matrices
                           void* stream) {
   if (matrices <= 0 || matrices > 65535 || N <= 0 || K <= 0 || b8_blocks(N) > 65535 || !b8_aligned(codes, 16) || !b8_aligned(scales, 16)) return ERR_BAD_ARGUMENT;
   const int element = dtype == DTYPE_F32 ? 4 : 2;
-  const bool wide = b8_aligned(w, 4 * element) && ldw % 4 == 0 && matrix_stride % 4 == 0;
+  const bool wide = b8_aligned(w, 16) && ldw % (16 / element) == 0 && matrix_stride % (16 / element) == 0;
   const dim3 grid(b8_blocks(K), b8_blocks(N), matrices);
   auto s = static_cast<cudaStream_t>(stream);
   if (dtype == DTYPE_F32)
@@ -174,14 +224,16 @@ ZB_API int zb_pack_matrix(void* codes, void* scales, const void* w, int matrices
 
 // out [matrices][N][K] = what a matrix's codes stand for (exact in bfloat16 but below its normal numbers).
 ZB_API int zb_matrix_values(void* out, const void* codes, const void* scales, int matrices, int N, int K, int dtype, void* stream) {
-  if (matrices <= 0 || matrices > 65535 || N <= 0 || K <= 0) return ERR_BAD_ARGUMENT;
-  const bool wide = K % 4 == 0 && b8_aligned(out, dtype == DTYPE_F32 ? 16 : 8);
-  const dim3 grid(N, matrices);
+  if (matrices <= 0 || N <= 0 || K <= 0 || !b8_aligned(codes, 16)) return ERR_BAD_ARGUMENT;
+  const bool wide = K % 16 == 0 && b8_aligned(out, 16);
+  const long long rows = static_cast<long long>(matrices) * N, ctas = (rows * ((K + 15) / 16) + 255) / 256;
+  if (ctas >= (1LL << 31)) return ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(ctas));
   auto s = static_cast<cudaStream_t>(stream);
   const auto* c = static_cast<const unsigned char*>(codes);
   const auto* e = static_cast<const unsigned char*>(scales);
-  if (dtype == DTYPE_F32) matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(out), c, e, N, K, wide);
-  else matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<__nv_bfloat16*>(out), c, e, N, K, wide);
+  if (dtype == DTYPE_F32) matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(out), c, e, rows, N, K, wide);
+  else matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<__nv_bfloat16*>(out), c, e, rows, N, K, wide);
   return launch_result();
 }
 

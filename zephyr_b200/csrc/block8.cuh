@@ -12,6 +12,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "mma.cuh"
 
 namespace zb {
 
@@ -49,50 +50,91 @@ __device__ __forceinline__ unsigned b8_codes(float a, float b, float c, float d,
   return static_cast<unsigned>(lo) | (static_cast<unsigned>(hi) << 16);
 }
 
-// 16 neighbouring values of a row, zeros from `left` on (left may be negative).  `wide`: the row's start and pitch allow 16-byte loads.
-__device__ __forceinline__ void b8_load16(const float* p, int left, bool wide, float (&v)[16]) {
-  if (wide && left >= 16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 f = *reinterpret_cast<const float4*>(p + 4 * i);
-      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < left ? p[i] : 0.0f;
-  }
-}
-__device__ __forceinline__ void b8_load16(const __nv_bfloat16* p, int left, bool wide, float (&v)[16]) {
-  if (wide && left >= 16) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + 8 * i);
-      const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < left ? __bfloat162float(p[i]) : 0.0f;
-  }
+// The same of values that are all finite.
+__device__ __forceinline__ unsigned b8_codes_finite(float2 ab, float2 cd, float2 inverse) {
+  unsigned short lo, hi;
+  ab = mul_pair(ab, inverse);
+  cd = mul_pair(cd, inverse);
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(ab.y), "f"(ab.x));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(cd.y), "f"(cd.x));
+  return static_cast<unsigned>(lo) | (static_cast<unsigned>(hi) << 16);
 }
 
-// A warp codes 512 values of a row, 16 a lane, eight lanes a block: this lane's 16 codes, and in every lane the scales' four bytes.
-__device__ __forceinline__ uint4 b8_code_row_piece(const float (&v)[16], unsigned& scales) {
-  unsigned largest = 0;
+// 16 neighbouring values of a row as they lie in memory, zeros from `left` on (left may be negative).  `wide`: the row's start and pitch
+// allow 16-byte loads.
+template <typename T> struct B8Values;
+template <> struct B8Values<__nv_bfloat16> {
+  unsigned v[8];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int left, bool wide) {
+    if (wide && left >= 16) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 8);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const unsigned short* bits = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) largest = max(largest, b8_magnitude(v[i]));
+      for (int i = 0; i < 8; ++i) v[i] = (2 * i < left ? bits[2 * i] : 0u) | (2 * i + 1 < left ? static_cast<unsigned>(bits[2 * i + 1]) << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u)); }
+  // Bits of the largest magnitude; at least 0x7f800000 where something is not finite.
+  __device__ __forceinline__ unsigned largest() const {
+    unsigned m = v[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, v[i] & 0x7fff7fffu);
+    return max(m << 16, m & 0xffff0000u);
+  }
+};
+template <> struct B8Values<float> {
+  float v[16];
+  __device__ __forceinline__ void load(const float* p, int left, bool wide) {
+    if (wide && left >= 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 f = *reinterpret_cast<const float4*>(p + 4 * i);
+        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = i < left ? p[i] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(v[2 * i], v[2 * i + 1]); }
+  __device__ __forceinline__ unsigned largest() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
+};
+
+// A warp codes 512 values of a row, 16 a lane, eight lanes a block: this lane's 16 codes, and its block's byte.
+template <typename T>
+__device__ __forceinline__ uint4 b8_code_row_piece(const B8Values<T>& x, unsigned& byte) {
+  unsigned largest = x.largest();
+  const bool wild = __any_sync(0xffffffffu, largest >= 0x7f800000u);
+  if (wild) {
+    largest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = max(largest, max(b8_magnitude(x.pair(i).x), b8_magnitude(x.pair(i).y)));
+  }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-  const unsigned byte = b8_scale_byte(largest);
+  byte = b8_scale_byte(largest);
   const float inverse = b8_inverse(byte);
-  scales = __shfl_sync(0xffffffffu, byte, 0) | __shfl_sync(0xffffffffu, byte, 8) << 8 | __shfl_sync(0xffffffffu, byte, 16) << 16 |
-           __shfl_sync(0xffffffffu, byte, 24) << 24;
-  return make_uint4(b8_codes(v[0], v[1], v[2], v[3], inverse), b8_codes(v[4], v[5], v[6], v[7], inverse),
-                    b8_codes(v[8], v[9], v[10], v[11], inverse), b8_codes(v[12], v[13], v[14], v[15], inverse));
+  unsigned c[4];
+  if (wild) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = b8_codes(x.pair(2 * i).x, x.pair(2 * i).y, x.pair(2 * i + 1).x, x.pair(2 * i + 1).y, inverse);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = b8_codes_finite(x.pair(2 * i), x.pair(2 * i + 1), make_float2(inverse, inverse));
+  }
+  return make_uint4(c[0], c[1], c[2], c[3]);
+}
+// The four bytes of a warp's 512 values, in every lane.
+__device__ __forceinline__ unsigned b8_four_bytes(unsigned byte) {
+  return __shfl_sync(0xffffffffu, byte, 0) | __shfl_sync(0xffffffffu, byte, 8) << 8 | __shfl_sync(0xffffffffu, byte, 16) << 16 |
+         __shfl_sync(0xffffffffu, byte, 24) << 24;
 }
 
 }  // namespace zb

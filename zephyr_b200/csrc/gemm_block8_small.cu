@@ -112,16 +112,22 @@ __global__ void __launch_bounds__(G9_WARPS * 32, 1) gemm_block8_small_kernel(con
   const int x_pieces = (blocks + 3) / 4;
   for (int task = warp; task < x_pieces * MT * 8; task += G9_WARPS) {
     const int token = task % (MT * 8), piece = task / (MT * 8), block = 4 * piece + lane / 8, k = (first_block + 4 * piece) * B8_BLOCK + 16 * lane;
-    float v[16];
     const int left = token < a.M ? a.K - k : 0;
     const size_t row = static_cast<size_t>(token < a.M ? token : 0) * a.ldx;
-    if (a.x_dtype == DTYPE_F32) b8_load16(static_cast<const float*>(a.x) + row + k, left, a.wide, v);
-    else b8_load16(static_cast<const __nv_bfloat16*>(a.x) + row + k, left, a.wide, v);
-    unsigned scales;
-    const uint4 codes = b8_code_row_piece(v, scales);
+    unsigned byte;
+    uint4 codes;
+    if (a.x_dtype == DTYPE_F32) {
+      B8Values<float> v;
+      v.load(static_cast<const float*>(a.x) + row + k, left, a.wide);
+      codes = b8_code_row_piece(v, byte);
+    } else {
+      B8Values<__nv_bfloat16> v;
+      v.load(static_cast<const __nv_bfloat16*>(a.x) + row + k, left, a.wide);
+      codes = b8_code_row_piece(v, byte);
+    }
     if (block < blocks) {
       x_s[((2 * block + lane % 8 / 4) * MT + token / 8) * 32 + token % 8 * 4 + lane % 4] = codes;
-      if (lane % 8 == 0) x_scale[block * (MT * 8) + token] = b8_power(scales >> (8 * (lane / 8)) & 255u);
+      if (lane % 8 == 0) x_scale[block * (MT * 8) + token] = b8_power(byte);
     }
   }
   __syncthreads();
