@@ -20,12 +20,14 @@ def _matrix(*shape):
 
 def test_layout():
     m = _matrix(300, 1100)
-    assert m.codes.shape == (300, 1152) and m.scales.shape == (1, 3, 3, 512) and m.shape == (300, 1100) and m.matrices == 1
+    assert m.codes.shape == (1, 3, 9, 128, 128) and m.scales.shape == (1, 3, 3, 512) and m.shape == (300, 1100) and m.matrices == 1
     several = _matrix(4, 129, 16)
-    assert several.codes.shape == (516, 128) and several.scales.shape == (4, 2, 1, 512) and several.matrices == 4
-    m.scales.copy_(torch.arange(m.scales.numel(), dtype=torch.int64).remainder(200).view(m.scales.shape))
+    assert several.codes.shape == (4, 2, 1, 128, 128) and several.scales.shape == (4, 2, 1, 512) and several.matrices == 4
     assert m.exponents().shape == (3, 9) and several.exponents().shape == (4, 2, 1)
-    assert m.exponents()[1, 4:8].tolist() == m.scales[0, 1, 1, :4].tolist()
+    m.exponents().copy_(torch.arange(27, dtype=torch.uint8).view(3, 9))
+    parts = [t.data_ptr() for t in (m.codes, m.scales, m.exponents())]
+    assert parts == [m.data.data_ptr(), m.data.data_ptr() + 27 * 128 * 128, m.data.data_ptr() + 27 * 128 * 128 + 9 * 512]
+    assert parts[:2] == [m.codes_at, m.scales_at] and m.data.numel() == 27 * 128 * 128 + 9 * 512 + 27
     first = m.first_rows(256)
     assert first.shape == (256, 1100) and first.codes.data_ptr() == m.codes.data_ptr() and first.scales.shape == (1, 2, 3, 512)
     assert torch.equal(first.exponents(), m.exponents()[:2]) and m.first_rows(300).shape == m.shape
@@ -34,13 +36,6 @@ def test_layout():
             m.first_rows(rows)
     with pytest.raises(InvalidArgumentError):
         several.first_rows(128)
-
-
-def test_runs_of_a_products_rows():
-    for rows in range(1, 3000):
-        run, cap = ops._block8_run(rows)
-        runs = -(-rows // run)
-        assert run % 16 == 0 and run <= cap and cap in (64, 128, 256) and (runs == 1 or cap == 256) and runs == -(-rows // 256)
 
 
 @pytest.mark.parametrize("shape", [(3,), (0, 4), (4, 0), (2, 0, 4), (1, 2, 3, 4)])

@@ -48,10 +48,10 @@ template <> struct PackValues<float> {
 
 template <typename T>
 __global__ void __launch_bounds__(B8_PACK_THREADS)
-pack_matrix_kernel(unsigned char* codes, unsigned char* scales, const T* w, long long matrix_stride, long long ldw, int N, int K, bool wide) {
+pack_matrix_kernel(unsigned char* codes, unsigned char* scales, unsigned char* exponents, const T* w, long long matrix_stride, long long ldw, int N, int K, bool wide) {
   constexpr int PER = PackValues<T>::PER, LANES = B8_BLOCK / PER, STEP = B8_PACK_THREADS / LANES, ROWS = B8_BLOCK / STEP;
   const int kb = blockIdx.x, nb = blockIdx.y, matrix = blockIdx.z;
-  const int pitch = b8_pitch(K), pieces = b8_pieces(K);
+  const int pieces = b8_pieces(K);
   const T* source = w + matrix * matrix_stride;
   const int k = kb * B8_BLOCK + threadIdx.x % LANES * PER, row0 = nb * B8_BLOCK + threadIdx.x / LANES;
   PackValues<T> v[ROWS];
@@ -87,19 +87,19 @@ pack_matrix_kernel(unsigned char* codes, unsigned char* scales, const T* w, long
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int row = row0 + STEP * r;
-    if (row >= N) continue;
     unsigned c[PER / 4];
 #pragma unroll
     for (int i = 0; i < PER / 4; ++i) {
       const float a = v[r].value(4 * i), b = v[r].value(4 * i + 1), d = v[r].value(4 * i + 2), e = v[r].value(4 * i + 3);
       c[i] = wild ? b8_codes(a, b, d, e, inverse) : b8_codes_finite(make_float2(a, b), make_float2(d, e), make_float2(inverse, inverse));
     }
-    unsigned char* to = codes + (static_cast<size_t>(matrix) * N + row) * pitch + k;
+    unsigned char* to = codes + (b8_block_row(matrix, nb, kb, N, K) + row - nb * B8_BLOCK) * B8_BLOCK + k - kb * B8_BLOCK;
     if constexpr (PER == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
     else *reinterpret_cast<unsigned*>(to) = c[0];
   }
   // The scale's 128 copies; behind the last block of K the piece is filled with the scale of zeros.
   unsigned char* piece = scales + ((static_cast<size_t>(matrix) * gridDim.y + nb) * pieces + kb / 4) * B8_PIECE;
+  if (threadIdx.x == 0) exponents[(static_cast<size_t>(matrix) * gridDim.y + nb) * gridDim.x + kb] = static_cast<unsigned char>(byte);
   if (threadIdx.x < 128) {
     unsigned char* at = piece + threadIdx.x % 32 * 16 + threadIdx.x / 32 * 4;
     at[kb % 4] = static_cast<unsigned char>(byte);
@@ -112,14 +112,13 @@ pack_matrix_kernel(unsigned char* codes, unsigned char* scales, const T* w, long
 template <typename T>
 __global__ void __launch_bounds__(256)
 matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* scales, long long rows, int N, int K, bool wide) {
-  const int pitch = b8_pitch(K), pieces = b8_pieces(K), units = (K + 15) / 16;
+  const int pieces = b8_pieces(K), units = (K + 15) / 16;
   const long long unit = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, row = unit / units;
   if (row >= rows) return;
   const int k = static_cast<int>(unit % units) * 16;
-  const long long matrix = row / N;
-  const int group = static_cast<int>(row % N) / B8_BLOCK;
-  const uint4 c = *reinterpret_cast<const uint4*>(codes + row * pitch + k);
-  const float scale = b8_power(scales[((matrix * b8_blocks(N) + group) * pieces + k / (4 * B8_BLOCK)) * B8_PIECE + k / B8_BLOCK % 4]);
+  const int matrix = static_cast<int>(row / N), own = static_cast<int>(row % N), group = own / B8_BLOCK;
+  const uint4 c = *reinterpret_cast<const uint4*>(codes + (b8_block_row(matrix, group, k / B8_BLOCK, N, K) + own % B8_BLOCK) * B8_BLOCK + k % B8_BLOCK);
+  const float scale = b8_power(scales[((static_cast<long long>(matrix) * b8_blocks(N) + group) * pieces + k / (4 * B8_BLOCK)) * B8_PIECE + k / B8_BLOCK % 4]);
   const unsigned words[4] = {c.x, c.y, c.z, c.w};
   float v[16];
 #pragma unroll
@@ -153,19 +152,7 @@ matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* sc
 //   * without `slots`, row m goes to place m / run * cap + m % run: the rows of a run of the product lie together, at its start;
 //   * with `slots`, place p gets row slots[p] / top of x (row p with `top` 0), or stays as it was where slots[p] < 0; with `place_scale` also
 //     the slot's weight (zero where there is none).
-// The scales of a run's places begin a new group of 128.
-struct CodeRowsArgs {
-  unsigned char* codes;
-  unsigned char* scales;
-  const void* x;
-  long long ldx;
-  const int* slots;
-  int places, K, run, cap, top;
-  float* place_scale;
-  const float* weights;
-  bool wide;
-};
-
+// The scales of a run's places: [run][piece][group of 128 places].
 template <typename T>
 __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   const int lane = threadIdx.x & 31, pieces = b8_pieces(a.K);
@@ -174,6 +161,7 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   const int piece = static_cast<int>(task % pieces);
   wait_for_prior_grids();
   let_dependents_launch();
+  if (task < a.zero_count && a.zeros != nullptr && lane == 0) a.zeros[task] = 0;
   if (index >= a.places) return;
   long long row = index, place = index;
   if (a.slots != nullptr) {
@@ -193,20 +181,28 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   const int pitch = b8_pitch(a.K);
   if (k < pitch) *reinterpret_cast<uint4*>(a.codes + place * pitch + k) = codes;
   if (lane == 0) {
-    const long long group = place / a.cap * ((a.cap + 127) / 128) + place % a.cap / 128;
-    const int r = static_cast<int>(place % a.cap % 128);
-    *reinterpret_cast<unsigned*>(a.scales + (group * pieces + piece) * B8_PIECE + r % 32 * 16 + r / 32 * 4) = scales;
+    const int groups = (a.cap + 127) / 128, own = static_cast<int>(place % a.cap), r = own % 128;
+    *reinterpret_cast<unsigned*>(a.scales + ((place / a.cap * pieces + piece) * groups + own / 128) * B8_PIECE + r % 32 * 16 + r / 32 * 4) = scales;
   }
+}
+
+static bool b8_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int block8_code_rows(CodeRowsArgs a, int dtype, cudaStream_t stream) {
+  a.wide = b8_aligned(a.x, 16) && a.ldx % (dtype == DTYPE_F32 ? 4 : 8) == 0;
+  const long long own = static_cast<long long>(a.places) * b8_pieces(a.K), tasks = own > a.zero_count ? own : a.zero_count;
+  if ((tasks + 7) / 8 >= (1LL << 31)) return ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>((tasks + 7) / 8));
+  return dtype == DTYPE_F32 ? launch_dependent(code_rows_kernel<float>, grid, dim3(256), 0, stream, false, a)
+                            : launch_dependent(code_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, false, a);
 }
 
 }  // namespace zb
 
 using namespace zb;
 
-static bool b8_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-
-// codes [matrices * N][K up to 128], scales [matrices][N / 128 up][K / 512 up][512] from w [matrices][N][K] (strides in elements, K contiguous).
-ZB_API int zb_pack_matrix(void* codes, void* scales, const void* w, int matrices, long long matrix_stride, long long ldw, int N, int K, int dtype,
+// codes [matrices][N / 128 up][K / 128 up][128][128], scales [matrices][N / 128 up][K / 512 up][512], exponents [matrices][N / 128 up][K / 128 up] from w [matrices][N][K] (strides in elements, K contiguous).
+ZB_API int zb_pack_matrix(void* codes, void* scales, void* exponents, const void* w, int matrices, long long matrix_stride, long long ldw, int N, int K, int dtype,
                           void* stream) {
   if (matrices <= 0 || matrices > 65535 || N <= 0 || K <= 0 || b8_blocks(N) > 65535 || !b8_aligned(codes, 16) || !b8_aligned(scales, 16)) return ERR_BAD_ARGUMENT;
   const int element = dtype == DTYPE_F32 ? 4 : 2;
@@ -214,10 +210,10 @@ ZB_API int zb_pack_matrix(void* codes, void* scales, const void* w, int matrices
   const dim3 grid(b8_blocks(K), b8_blocks(N), matrices);
   auto s = static_cast<cudaStream_t>(stream);
   if (dtype == DTYPE_F32)
-    pack_matrix_kernel<<<grid, B8_PACK_THREADS, 0, s>>>(static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales),
+    pack_matrix_kernel<<<grid, B8_PACK_THREADS, 0, s>>>(static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), static_cast<unsigned char*>(exponents),
                                                         static_cast<const float*>(w), matrix_stride, ldw, N, K, wide);
   else
-    pack_matrix_kernel<<<grid, B8_PACK_THREADS, 0, s>>>(static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales),
+    pack_matrix_kernel<<<grid, B8_PACK_THREADS, 0, s>>>(static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), static_cast<unsigned char*>(exponents),
                                                         static_cast<const __nv_bfloat16*>(w), matrix_stride, ldw, N, K, wide);
   return launch_result();
 }
@@ -235,19 +231,4 @@ ZB_API int zb_matrix_values(void* out, const void* codes, const void* scales, in
   if (dtype == DTYPE_F32) matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<float*>(out), c, e, rows, N, K, wide);
   else matrix_values_kernel<<<grid, 256, 0, s>>>(static_cast<__nv_bfloat16*>(out), c, e, rows, N, K, wide);
   return launch_result();
-}
-
-// Rows of x [.., K] (pitch ldx) as codes and scales at their places (see code_rows_kernel).  `places`: rows of x, or with `slots` entries of it.
-ZB_API int zb_code_rows(void* codes, void* scales, const void* x, long long ldx, const int* slots, int places, int K, int run, int cap, int top,
-                        float* place_scale, const float* weights, int dtype, void* stream) {
-  if (places < 0 || K <= 0 || run <= 0 || cap < run || cap % 64 != 0 || top < 0 || (place_scale != nullptr && (weights == nullptr || slots == nullptr)) || !b8_aligned(codes, 16) || !b8_aligned(scales, 16)) return ERR_BAD_ARGUMENT;
-  if (places == 0) return OK;
-  CodeRowsArgs a{static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), x, ldx, slots, places, K, run, cap, top, place_scale, weights, false};
-  a.wide = b8_aligned(x, 16) && ldx % (dtype == DTYPE_F32 ? 4 : 8) == 0;
-  const long long tasks = static_cast<long long>(places) * b8_pieces(K);
-  if ((tasks + 7) / 8 >= (1LL << 31)) return ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>((tasks + 7) / 8));
-  auto s = static_cast<cudaStream_t>(stream);
-  return dtype == DTYPE_F32 ? launch_dependent(code_rows_kernel<float>, grid, dim3(256), 0, s, false, a)
-                            : launch_dependent(code_rows_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, false, a);
 }

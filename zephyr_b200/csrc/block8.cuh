@@ -6,7 +6,9 @@
 // beside any other factor: e4m3 numbers are as dense, relative to their size, wherever they lie.  Powers of two are what the tensor cores
 // multiply a block's sums with themselves (kind::mxf8f6f4), and their exponents are all that has to be stored.
 //
-// Codes: rows of pitch Kp, K rounded up to 128, zeros behind K.  Scales: pieces of 512 bytes, one for 128 rows and four neighbouring
+// A matrix's codes: block by block, 128 rows of 128 bytes each, the blocks of K of 128 rows one behind the other, zeros behind N and K: what a copy
+// fetches lies in one piece of memory.  (Row by row, 4096 bytes a row, PLACEHOLDER.)  Codes of activations: rows of pitch Kp, K rounded
+// up to 128, zeros behind K.  Scales: pieces of 512 bytes, one for 128 rows and four neighbouring
 // blocks of K; row r's four bytes lie at 16 (r % 32) + 4 (r / 32), which is how tcgen05.cp brings a piece into tensor memory.  A matrix has one scale for
 // 128 rows; its pieces hold it 128 times (0.8 % of the codes' bytes), so that both operands of a product look alike.
 #pragma once
@@ -21,7 +23,50 @@ constexpr int B8_PIECE = 512;          // bytes of scales of 128 rows x 4 blocks
 
 __host__ __device__ inline int b8_blocks(int n) { return (n + B8_BLOCK - 1) / B8_BLOCK; }
 __host__ __device__ inline int b8_pieces(int k) { return (k + 4 * B8_BLOCK - 1) / (4 * B8_BLOCK); }
+// The first row of a matrix's block when all its codes are taken as rows of 128 bytes.
+__host__ __device__ inline long long b8_block_row(int matrix, int nb, int kb, int N, int K) {
+  return ((static_cast<long long>(matrix) * b8_blocks(N) + nb) * b8_blocks(K) + kb) * B8_BLOCK;
+}
 __host__ __device__ inline int b8_pitch(int k) { return b8_blocks(k) * B8_BLOCK; }
+
+// ---- What the files of this form offer one another (host) ----
+constexpr int G8_PAIRS = 74;           // of SMs: the most that the product for many rows takes
+
+struct Block8Product {
+  void* y; long long ldy; int y_dtype;
+  const void *x_codes, *x_scales, *w_codes, *w_scales;
+  const int* plan; int max_runs, matrices;
+  int M, run, cap, N, K;               // a run's places begin `cap` (64, 128 or 256) apart
+  int kind;                            // 0 the sums, 1 silu(gate) * up, 2 max(gate, 0) * up, 3 the bounded gate, 4 gelu_tanh of the sums, 5 the square of max(sum, 0)
+  const float *bias, *row_scale; float limit, alpha, shift;
+  bool halves; float* parts; int* flags; int least;
+  int* status;
+};
+struct CodeRowsArgs {
+  unsigned char* codes;
+  unsigned char* scales;
+  const void* x;
+  long long ldx;
+  const int* slots;
+  int places, K, run, cap, top;
+  float* place_scale;
+  const float* weights;
+  int* zeros;                          // what a later kernel finds as zeros, or null
+  int zero_count;
+  bool wide;
+};
+struct Block8Small {
+  void* y; long long ldy; int y_dtype;
+  const void* x; long long ldx; int x_dtype;
+  const void *w_codes, *w_scales;
+  int M, N, K, kind;
+  const float* bias; float limit, alpha, shift;
+  int* status;
+};
+int block8_product(const Block8Product& p, cudaStream_t stream);          // gemm_block8.cu
+int block8_code_rows(CodeRowsArgs a, int dtype, cudaStream_t stream);     // block8.cu
+bool block8_small_fits(int M, int K);                                     // gemm_block8_small.cu
+int block8_small_product(const Block8Small& p, cudaStream_t stream);
 
 // Bits of |x| where x is finite, else zero: their maximum is the block's.
 __device__ __forceinline__ unsigned b8_magnitude(float x) {

@@ -1,0 +1,233 @@
+// What is asked of matrices in 8-bit floating point (block8.cuh) in one call each: a product, a gated feed-forward, a layer of routed experts.  A call
+// brings one piece of memory for everything between its kernels; how large it has to be, the functions ending in `_work` say from the sizes alone.
+#include "block8.cuh"
+
+// (routed.cu, gemm_tc_experts.cu)
+ZB_API int zb_route_align_strided(int* plan, int* slots, int* place_of_slot, const int* ids, int num_slots, int experts, int max_runs, int run,
+                                  int places, void* stream);
+ZB_API int zb_gemm_tc_experts_run(int choices, int experts);
+ZB_API int zb_route_combine(void* out, const void* y, long long y_stride, int y_dtype, const void* x, long long x_stride, const int* ids,
+                            const float* weights, const int* place_of_slot, int tokens, int width, int top, int dtype, void* stream);
+
+namespace zb {
+
+constexpr long long FLAGS = G8_PAIRS * 2 * 8;            // ints
+
+// Pieces of a call's memory, each from a multiple of 256 bytes on; with a null base only their sizes are added up.
+struct Pieces {
+  char* base;
+  long long at = 0;
+  template <typename T> T* take(long long count) {
+    T* piece = base != nullptr ? reinterpret_cast<T*>(base + at) : nullptr;
+    at += (count * static_cast<long long>(sizeof(T)) + 255) / 256 * 256;
+    return piece;
+  }
+};
+
+// Whether few rows go to the kernel that streams the matrix, and how many others are.  The streaming kernel codes all of x in every CTA and has four
+// warps or sixteen on a tile; the tensor cores' kernel waits for x's codes and for a tile's whole K (8 rows, us, streaming / tensor cores: PLACEHOLDER).
+constexpr long long STREAM_VALUES = 28LL << 20;
+static bool streams(int M, int N, int K) { return static_cast<long long>(N) * K <= STREAM_VALUES && block8_small_fits(M, K); }
+
+// Whether the pairs share all tiles' blocks of K evenly instead of taking whole tiles: where the rounds of whole tiles leave more of the pairs
+// without work than the parts cost to be handed over.  In units of a block of K on a pair (PLACEHOLDER us).
+static bool in_parts(long long items, int k_blocks, int cap) {
+  const long long rounds = (items + G8_PAIRS - 1) / G8_PAIRS;
+  const long long whole = rounds * k_blocks, even = (items * k_blocks + G8_PAIRS - 1) / G8_PAIRS;
+  return whole - even > (cap == 64 ? 24 : cap == 128 ? 28 : 32);
+}
+constexpr int LEAST_BLOCKS = 8;
+
+struct Rows {
+  int run, cap, runs;
+};
+// Rows in as few runs of equal length (a multiple of 16) as up to `most` rows a run allow.
+static Rows rows_of(int M, int most) {
+  const int runs = (M + most - 1) / most, run = ((M + runs - 1) / runs + 15) / 16 * 16;
+  return {run, M <= 64 ? 64 : M <= 128 || most == 128 ? 128 : 256, runs};
+}
+// Float32 results of long rows are summed in two accumulators: the tensor cores cut what a sum's 24 bits do not hold, always towards zero, so a
+// sum is off by 7e-8 of itself for every 1024 values of K (14336: 1e-6).
+static bool sums_in_halves(int K, int y_dtype) { return y_dtype == DTYPE_F32 && K > 8192; }
+
+struct ProductWork {
+  Rows rows;
+  bool halves;
+  int* flags;
+  float* parts;
+  unsigned char *codes, *scales;
+};
+static ProductWork product_work(Pieces& memory, int M, int N, int K, bool halves) {
+  ProductWork w;
+  w.rows = rows_of(M, halves ? 128 : 256);
+  w.halves = halves;
+  const long long places = static_cast<long long>(w.rows.runs) * w.rows.cap, items = static_cast<long long>(w.rows.runs) * ((N + 255) / 256);
+  const bool parts = in_parts(items, b8_blocks(K), w.rows.cap);
+  w.flags = memory.take<int>(FLAGS);
+  w.parts = parts ? memory.take<float>(static_cast<long long>(G8_PAIRS) * 2 * w.rows.cap * 128) : nullptr;
+  if (!parts) w.flags = nullptr;
+  w.codes = memory.take<unsigned char>(places * b8_pitch(K));
+  w.scales = memory.take<unsigned char>(places / w.rows.cap * ((w.rows.cap + 127) / 128) * b8_pieces(K) * B8_PIECE);
+  return w;
+}
+
+struct Operand {
+  const void *codes, *scales;
+  int N, K;
+};
+struct Gate {
+  int kind;
+  const float* bias;
+  float limit, alpha, shift;
+};
+
+// y [M, N, or N / 2 gated] = x w^T.  `final`: a float32 result is what the caller asked for (hidden values are coded next).
+static int product(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& w, int M, const Gate& g,
+                   bool final, int* status, cudaStream_t stream) {
+  if (streams(M, w.N, w.K))
+    return memory.base == nullptr ? OK : block8_small_product({y, ldy, y_dtype, x, ldx, x_dtype, w.codes, w.scales, M, w.N, w.K, g.kind, g.bias, g.limit, g.alpha,
+                                                               g.shift, status}, stream);
+  const ProductWork work = product_work(memory, M, w.N, w.K, final && sums_in_halves(w.K, y_dtype));
+  if (memory.base == nullptr) return OK;
+  CodeRowsArgs c = {work.codes, work.scales, x, ldx, nullptr, M, w.K, work.rows.run, work.rows.cap, 0, nullptr, nullptr, work.flags,
+                    work.flags != nullptr ? static_cast<int>(FLAGS) : 0, false};
+  const int rc = block8_code_rows(c, x_dtype, stream);
+  if (rc != OK) return rc;
+  return block8_product({y, ldy, y_dtype, work.codes, work.scales, w.codes, w.scales, nullptr, 0, 1, M, work.rows.run, work.rows.cap, w.N, w.K, g.kind, g.bias,
+                         nullptr, g.limit, g.alpha, g.shift, work.halves, work.parts, work.flags, LEAST_BLOCKS, status}, stream);
+}
+
+static int feed_forward(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& up, const Operand& down,
+                        int M, const Gate& g, int* status, cudaStream_t stream) {
+  float* hidden = memory.take<float>(static_cast<long long>(M) * down.K);
+  const int rc = product(memory, hidden, down.K, DTYPE_F32, x, ldx, x_dtype, up, M, g, false, status, stream);
+  if (rc != OK) return rc;
+  return product(memory, y, ldy, y_dtype, hidden, down.K, DTYPE_F32, down, M, Gate{0, nullptr, 0.0f, 1.0f, 0.0f}, true, status, stream);
+}
+
+struct Experts {
+  void* y;
+  const void* x;
+  long long ldx;
+  int dtype;
+  const int* ids;
+  const float* weights;
+  int T, top, E, width, ff;
+  bool weigh_inputs;
+};
+// The rows are coded where they are gathered, the hidden values stay in float32 until they are coded for the second product, an expert's
+// output is rounded to x's type before it is weighted.
+static int experts(Pieces& memory, const Experts& e, const Operand& up, const Operand& down, const Gate& g, int* status, cudaStream_t stream) {
+  const int num_slots = e.T * e.top, cap = zb_gemm_tc_experts_run(num_slots, e.E), runs = num_slots / cap + e.E;
+  const long long places = static_cast<long long>(runs) * cap;
+  const int groups = (cap + 127) / 128;
+  int* plan = memory.take<int>(1 + 3LL * runs);
+  int* slots = memory.take<int>(places);
+  int* place_of_slot = memory.take<int>(num_slots);
+  float* place_scale = e.weigh_inputs ? memory.take<float>(places) : nullptr;
+  int* flags = memory.take<int>(FLAGS);
+  float* parts = cap <= 128 ? memory.take<float>(static_cast<long long>(G8_PAIRS) * 2 * cap * 128) : nullptr;
+  unsigned char* codes = memory.take<unsigned char>(places * b8_pitch(e.width));
+  unsigned char* scales = memory.take<unsigned char>(static_cast<long long>(runs) * groups * b8_pieces(e.width) * B8_PIECE);
+  float* hidden = memory.take<float>(places * e.ff);
+  unsigned char* hidden_codes = memory.take<unsigned char>(places * b8_pitch(e.ff));
+  unsigned char* hidden_scales = memory.take<unsigned char>(static_cast<long long>(runs) * groups * b8_pieces(e.ff) * B8_PIECE);
+  char* out = memory.take<char>(places * e.width * (e.dtype == DTYPE_F32 ? 4 : 2));
+  if (places >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (memory.base == nullptr) return OK;
+  const int zeros = parts != nullptr ? static_cast<int>(FLAGS) : 0;
+  int rc = zb_route_align_strided(plan, slots, place_of_slot, e.ids, num_slots, e.E, runs, cap, static_cast<int>(places), stream);
+  if (rc != OK) return rc;
+  rc = block8_code_rows({codes, scales, e.x, e.ldx, slots, static_cast<int>(places), e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
+  if (rc != OK) return rc;
+  rc = block8_product({hidden, e.ff, DTYPE_F32, codes, scales, up.codes, up.scales, plan, runs, e.E, 0, cap, cap, up.N, up.K, g.kind, nullptr, place_scale, g.limit,
+                       g.alpha, g.shift, false, parts, flags, LEAST_BLOCKS, status}, stream);
+  if (rc != OK) return rc;
+  rc = block8_code_rows({hidden_codes, hidden_scales, hidden, e.ff, slots, static_cast<int>(places), e.ff, cap, cap, 0, nullptr, nullptr, flags, zeros, false}, DTYPE_F32, stream);
+  if (rc != OK) return rc;
+  rc = block8_product({out, e.width, e.dtype, hidden_codes, hidden_scales, down.codes, down.scales, plan, runs, e.E, 0, cap, cap, down.N, down.K, 0, nullptr, nullptr,
+                       0.0f, 1.0f, 0.0f, false, parts, flags, LEAST_BLOCKS, status}, stream);
+  if (rc != OK) return rc;
+  return zb_route_combine(e.y, out, e.width, e.dtype, e.x, e.ldx, e.ids, e.weigh_inputs ? nullptr : e.weights, place_of_slot, e.T, e.width, e.top, e.dtype, stream);
+}
+
+static bool sizes_ok(long long a, long long b, long long c) { return a > 0 && b > 0 && c > 0 && a < (1LL << 31) && b < (1LL << 31) && c < (1LL << 31) - 512; }
+static bool gate_ok(long long kind, long long N, double limit, const float* bias, bool gated) {
+  if (gated != (kind >= 1 && kind <= 3)) return false;
+  return kind >= 0 && kind <= 5 && (!gated || N % 16 == 0) && (kind != 3 || limit > 0.0) && (kind == 3 || bias == nullptr);
+}
+
+}  // namespace zb
+
+using namespace zb;
+
+// What the calls are given: eight bytes a field, in this order.
+struct ProductCall {
+  void* y; long long ldy, y_dtype; const void* x; long long ldx, x_dtype; const void *w_codes, *w_scales; long long M, N, K, kind; const float* bias;
+  double limit, alpha, shift; void* work; int* status; void* stream;
+};
+struct FeedForwardCall {
+  void* y; long long ldy, y_dtype; const void* x; long long ldx, x_dtype; const void *up_codes, *up_scales, *down_codes, *down_scales; long long M, K, ff, N, kind;
+  const float* bias; double limit, alpha, shift; void* work; int* status; void* stream;
+};
+struct ExpertsCall {
+  void* y; const void* x; long long ldx, dtype; const int* ids; const float* weights; const void *up_codes, *up_scales, *down_codes, *down_scales;
+  long long T, top, E, width, ff, kind, weigh_inputs; double limit, alpha, shift; void* work; int* status; void* stream;
+};
+
+static Gate gate_of(long long kind, const float* bias, double limit, double alpha, double shift) {
+  return {static_cast<int>(kind), bias, static_cast<float>(limit), static_cast<float>(alpha), static_cast<float>(shift)};
+}
+
+ZB_API long long zb_block8_product_work(long long M, long long N, long long K, int y_dtype) {
+  Pieces memory{nullptr};
+  product(memory, nullptr, 0, y_dtype, nullptr, 0, 0, {nullptr, nullptr, static_cast<int>(N), static_cast<int>(K)}, static_cast<int>(M), {}, true, nullptr, nullptr);
+  return memory.at;
+}
+ZB_API int zb_block8_product(const void* call) {
+  const ProductCall& c = *static_cast<const ProductCall*>(call);
+  const bool gated = c.kind >= 1 && c.kind <= 3;
+  if (!sizes_ok(c.M, c.N, c.K) || !gate_ok(c.kind, c.N, c.limit, c.bias, gated) || c.ldx < c.K || c.ldy < (gated ? c.N / 2 : c.N)) return ERR_BAD_ARGUMENT;
+  Pieces memory{static_cast<char*>(c.work)};
+  if (memory.base == nullptr) memory.base = reinterpret_cast<char*>(256);       // (nothing is taken of it)
+  return product(memory, c.y, c.ldy, static_cast<int>(c.y_dtype), c.x, c.ldx, static_cast<int>(c.x_dtype), {c.w_codes, c.w_scales, static_cast<int>(c.N), static_cast<int>(c.K)},
+                 static_cast<int>(c.M), gate_of(c.kind, c.bias, c.limit, c.alpha, c.shift), true, c.status, static_cast<cudaStream_t>(c.stream));
+}
+// How many kernels the call launches.
+ZB_API int zb_block8_product_kernels(int M, int N, int K) { return streams(M, N, K) ? 1 : 2; }
+
+ZB_API long long zb_block8_feed_forward_work(long long M, long long K, long long ff, long long N, int y_dtype) {
+  Pieces memory{nullptr};
+  feed_forward(memory, nullptr, 0, y_dtype, nullptr, 0, 0, {nullptr, nullptr, static_cast<int>(2 * ff), static_cast<int>(K)},
+               {nullptr, nullptr, static_cast<int>(N), static_cast<int>(ff)}, static_cast<int>(M), {}, nullptr, nullptr);
+  return memory.at;
+}
+ZB_API int zb_block8_feed_forward(const void* call) {
+  const FeedForwardCall& c = *static_cast<const FeedForwardCall*>(call);
+  if (!sizes_ok(c.M, 2 * c.ff, c.K) || !sizes_ok(c.M, c.N, c.ff) || !gate_ok(c.kind, 2 * c.ff, c.limit, c.bias, true) || c.ldx < c.K || c.ldy < c.N || c.work == nullptr)
+    return ERR_BAD_ARGUMENT;
+  Pieces memory{static_cast<char*>(c.work)};
+  return feed_forward(memory, c.y, c.ldy, static_cast<int>(c.y_dtype), c.x, c.ldx, static_cast<int>(c.x_dtype),
+                      {c.up_codes, c.up_scales, static_cast<int>(2 * c.ff), static_cast<int>(c.K)}, {c.down_codes, c.down_scales, static_cast<int>(c.N), static_cast<int>(c.ff)},
+                      static_cast<int>(c.M), gate_of(c.kind, c.bias, c.limit, c.alpha, c.shift), c.status, static_cast<cudaStream_t>(c.stream));
+}
+
+ZB_API long long zb_block8_experts_work(long long T, long long top, long long E, long long width, long long ff, int dtype, int weigh_inputs) {
+  Pieces memory{nullptr};
+  Experts e = {};
+  e.dtype = dtype; e.T = static_cast<int>(T); e.top = static_cast<int>(top); e.E = static_cast<int>(E); e.width = static_cast<int>(width); e.ff = static_cast<int>(ff);
+  e.weigh_inputs = weigh_inputs != 0;
+  experts(memory, e, {}, {}, {}, nullptr, nullptr);
+  return memory.at;
+}
+ZB_API int zb_block8_experts(const void* call) {
+  const ExpertsCall& c = *static_cast<const ExpertsCall*>(call);
+  if (!sizes_ok(c.T * c.top, 2 * c.ff, c.width) || !sizes_ok(c.T * c.top, c.width, c.ff) || c.E <= 0 || !gate_ok(c.kind, 2 * c.ff, c.limit, nullptr, true) ||
+      (c.weigh_inputs && c.kind == 3) || c.ldx < c.width || c.work == nullptr)
+    return ERR_BAD_ARGUMENT;
+  Pieces memory{static_cast<char*>(c.work)};
+  const int width = static_cast<int>(c.width), ff = static_cast<int>(c.ff);
+  return experts(memory, {c.y, c.x, c.ldx, static_cast<int>(c.dtype), c.ids, c.weights, static_cast<int>(c.T), static_cast<int>(c.top), static_cast<int>(c.E), width, ff,
+                          c.weigh_inputs != 0}, {c.up_codes, c.up_scales, 2 * ff, width}, {c.down_codes, c.down_scales, width, ff},
+                 gate_of(c.kind, nullptr, c.limit, c.alpha, c.shift), c.status, static_cast<cudaStream_t>(c.stream));
+}

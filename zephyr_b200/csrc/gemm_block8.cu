@@ -11,13 +11,16 @@
 // The matrix takes the tensor core's row side, 256 rows on a pair of SMs (cta_group::2), a run of up to RUN rows of x the other: a
 // matrix is fetched once for each run, a CTA fetches its 128 rows of it beside half of the run's rows of x.  Persistent: a pair
 // takes (256 rows of w, run) in turn, the runs that share rows of w next to each other in time.  Roles of a CTA's ten warps:
-//   * warp 0: per block of K (128 bytes a row) tiled copies of its 128 rows of w and of its half of the run's rows, 32 a copy, into a ring; every
-//     fourth block also the pieces of scales of its rows of w and of all the run's rows;
+//   * warp 0, one thread: per block of K (128 bytes a row) tiled copies of its 128 rows of w and of its half of the run's rows (always RUN / 2 of
+//     them: what lies behind a run's rows ends in columns that nobody reads) into a ring; every fourth block also the pieces of scales of its rows
+//     of w and of all the run's rows;
 //   * warp 1 of the first CTA: every fourth block the copies of the scales into tensor memory (tcgen05.cp, in order with the products), then
 //     four products 256 x run x 32, all by one elected lane;
 //   * warps 2..9: a thread owns a row of w (its TMEM lane) and reads 32 sums of x's rows at a time, every other 32 of them; what a warp has for
 //     32 rows goes through shared memory to wide stores.
 // Every wait is bounded and reports instead of hanging; tensor memory is given back on every path.
+#include <atomic>
+
 #include "block8.cuh"
 #include "mma.cuh"
 #include "tcgen05.cuh"
@@ -29,7 +32,6 @@ constexpr int G8_THREADS = 320;
 constexpr int G8_WAIT_LIMIT = 1 << 18;
 constexpr int G8_MAX_STAGES = 10;
 constexpr int G8_W_BYTES = 128 * 128;
-constexpr int G8_X_BOX = 32;               // rows of x per copy
 constexpr int G8_SCALES = 3 * B8_PIECE;    // of one CTA's rows of w, and of up to 256 rows of x
 constexpr int G8_STAGING = 32 * 144;       // an epilogue warp's 32 rows x 32 outputs, float32, rows 144 bytes apart
 constexpr int G8_SCALE_COLUMN = 256;       // where scales begin in tensor memory; 12 columns a piece of K
@@ -38,6 +40,7 @@ constexpr int G8_SCALE_COLUMN = 256;       // where scales begin in tensor memor
 // holds one stage at least, so the products that read it are through (the stage that brings the new one was free), and so is its copy to tensor memory.
 template <int RUN> struct Block8Shape {
   static constexpr int STAGE_BYTES = G8_W_BYTES + RUN / 2 * 128;
+  static constexpr int X_SCALES = (RUN + 127) / 128 * B8_PIECE;
   static constexpr int STAGES = RUN == 256 ? 5 : RUN == 128 ? 7 : 8;
   static constexpr int ACCUMULATORS = RUN == 256 ? 1 : 2;
   static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + G8_SCALES) + 8 * G8_STAGING + 1024;
@@ -46,17 +49,21 @@ template <int RUN> struct Block8Shape {
 };
 
 struct Block8Args {
-  CUtensorMap w_map;             // codes of w as rows of bytes; box 128 x 128
+  CUtensorMap w_map;             // codes of w, blocks as rows of 128 bytes; box 128 x 128: one block
   CUtensorMap w_scale_map;       // its scales as rows of 128 bytes; box 128 x 4: one piece
-  CUtensorMap x_map;             // codes of x; box 128 x 32
-  CUtensorMap x_scale_map;
+  CUtensorMap x_map;             // codes of x; box 128 x RUN / 2
+  CUtensorMap x_scale_map;       // its scales; box 128 x 4 or 8: a piece of each of a run's groups
   void* y;
   long long ldy;
   int N, row_blocks, scale_groups;       // rows of a matrix, in blocks of 256, in groups of 128
-  int k_blocks, pieces;
+  int k_blocks, pieces, w_groups;        // w_groups: groups of 128 rows of all matrices
   int run_groups;                        // groups of 128 places that the scales of a run take: places a run / 128, rounded up
   const int* plan;                       // [0] runs; then per run its matrix, first place and number of places that count; null: one matrix
   int M, run, cap;                       // without a plan: rows in runs of `run`, whose places begin `cap` apart
+  bool halves;                           // (RUN up to 128) a tile's sums in two accumulators, each over half of its blocks of K
+  int least;                             // blocks of K a pair takes at least
+  float* parts;                          // [pair][CTA][column][128 rows]: sums of a tile that another pair finishes; null: pairs take whole tiles
+  int* flags;                            // [pair][CTA][warp], zeros when the kernel starts
   bool wide;                             // y's rows allow 16-byte stores
   int act;
   GateForm gate;
@@ -85,6 +92,50 @@ __device__ __forceinline__ Run8 run_of(const Block8Args& a, int i) {
   if (a.plan != nullptr) return {a.plan[1 + 3 * i], a.plan[2 + 3 * i], a.plan[3 + 3 * i], a.plan[2 + 3 * i]};
   return {0, i * a.cap, min(a.run, a.M - i * a.run), i * a.run};
 }
+
+// What a pair of CTAs computes.  Without `parts` it takes whole tiles (256 rows of w, run) in turn.  With `parts` all tiles' blocks of K, one tile behind the
+// other, are cut into equal shares, whatever the tiles' borders: a share is then the end of one tile, whole tiles, and the beginning of another
+// one.  The pair that has a tile's end finishes it; the others leave their sums in `parts` and set their flags.  Each pair walks its share from
+// the back, so that what others wait for comes first and what it waits for itself last.
+struct Share {
+  long long begin, at;          // with `parts`: blocks still to come
+  int item, items, pair, pairs, k_blocks;
+  __device__ __forceinline__ Share(const Block8Args& a, int runs, int pair_, int pairs_) : pair(pair_), pairs(pairs_), k_blocks(a.k_blocks) {
+    items = runs * a.row_blocks;
+    item = pair - pairs;
+    if (a.parts != nullptr) {
+      const long long all = static_cast<long long>(items) * k_blocks;
+      pairs = static_cast<int>(min(static_cast<long long>(pairs), (all + a.least - 1) / a.least));
+      begin = border(pair);
+      at = border(pair + 1);
+    }
+  }
+  __device__ __forceinline__ long long border(int p) const { return static_cast<long long>(items) * k_blocks * min(p, pairs) / pairs; }
+  // The next tile and its blocks of K from `first` to before `end`; false: there is none.
+  __device__ __forceinline__ bool next(const Block8Args& a, int& tile, int& first, int& end) {
+    if (a.parts == nullptr) {
+      item += pairs;
+      tile = item;
+      first = 0;
+      end = k_blocks;
+      return item < items;
+    }
+    if (at <= begin) return false;
+    tile = static_cast<int>((at - 1) / k_blocks);
+    const long long start = static_cast<long long>(tile) * k_blocks;
+    end = static_cast<int>(at - start);
+    at = max(begin, start);
+    first = static_cast<int>(at - start);
+    return true;
+  }
+};
+
+// The group of 128 rows of w that a CTA of a pair takes of a block of 256 of a matrix (what lies behind the last matrix is the last group once more).
+__device__ __forceinline__ int w_group_of(const Block8Args& a, int matrix, int block, int rank) {
+  return min(matrix * a.scale_groups + 2 * block + rank, a.w_groups - 1);
+}
+// Does the stage of block `kb` bring the scales of its piece of K?
+__device__ __forceinline__ bool brings_scales(int kb, int first) { return kb % 4 == 0 || kb == first; }
 
 // One scaled product of 256 x N x 32: D (+)= A B, each operand's sums times the powers of two in tensor memory at `a_scales` and `b_scales`.
 __device__ __forceinline__ void tc_mma_scaled_pair(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc,
@@ -140,61 +191,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
   cluster_sync_all();                               // both CTAs' barriers and tensor memory are there
   tc_fence_after_sync();
   const unsigned tmem_base = sh.tmem_base;
+  // While the kernel ahead still runs: the first stages' blocks of w, which nothing ahead writes.  (Where runs come from a plan, a kernel ahead writes it.)
+  int ahead = 0;
+  if (warp == 0 && a.plan == nullptr && elect_one()) {
+    Share first_share(a, runs_of(a), pair, pairs);
+    int tile, first, end;
+    if (first_share.next(a, tile, first, end)) {
+      const int w_group = w_group_of(a, 0, tile / runs_of(a), rank);
+      for (; ahead < Shape::STAGES && first + ahead < end; ++ahead) {
+        const int kb = first + ahead;
+        if (rank == 0) mbar_arrive_expect_tx(&sh.full[ahead], 2 * (Shape::STAGE_BYTES + (brings_scales(kb, first) ? B8_PIECE + Shape::X_SCALES : 0)));
+        tiled_copy_2d_g2s_pair(ring + ahead * Shape::STAGE_BYTES, &a.w_map, 0, (w_group * a.k_blocks + kb) * 128, in_cta_of_rank(smem_u32(&sh.full[ahead]), 0));
+      }
+    }
+  }
   wait_for_prior_grids();
   let_dependents_launch();
-  const int runs = runs_of(a), items = runs * a.row_blocks;
+  const int runs = runs_of(a);
+  Share share(a, runs, pair, pairs);
+  int item, k_first, k_end;
+  const int accumulators = a.halves ? 1 : Shape::ACCUMULATORS;
   // The product's columns: a run's rows up to a multiple of 64, half of them in each CTA.
   auto half_columns = [](int rows) { return (rows + 63) / 64 * 32; };
 
   if (warp == 0) {
-    // A copy a lane: lane 0 the rows of w, 1 to 4 the rows of x, 5 the scales of w, 6 and 7 those of x.
-    int stage = 0, scales = 0;
-    unsigned phase = 0;
-    for (int item = pair; item < items; item += pairs) {
-      const Run8 run = run_of(a, item % runs);
-      const int block = item / runs, half = half_columns(run.rows), boxes = half / G8_X_BOX, groups = (2 * half + 127) / 128, box = lane - 1;
-      const int row = lane == 0 ? run.matrix * a.N + block * 256 + 128 * rank : run.place + half * rank + box * G8_X_BOX;
-      const unsigned offset = lane == 0 ? 0 : G8_W_BYTES + box * G8_X_BOX * 128;
-      const CUtensorMap* map = lane == 0 ? &a.w_map : &a.x_map;
-      const int group = lane == 5 ? run.matrix * a.scale_groups + 2 * block + rank : run.place / a.cap * a.run_groups + lane - 6;
-      bool ok = true;
-      for (int kb = 0; kb < a.k_blocks; ++kb) {
-        ok = __all_sync(0xffffffffu, g8_wait(sh, &sh.empty[stage], phase ^ 1));
-        if (!ok) break;
-        const bool brings_scales = kb % 4 == 0;
-        if (rank == 0 && lane == 0)
-          mbar_arrive_expect_tx(&sh.full[stage], 2 * (G8_W_BYTES + boxes * G8_X_BOX * 128 + (brings_scales ? (1 + groups) * B8_PIECE : 0)));
-        const unsigned full = in_cta_of_rank(smem_u32(&sh.full[stage]), 0);
-        if (lane <= boxes) {
-          tiled_copy_2d_g2s_pair(ring + stage * Shape::STAGE_BYTES + offset, map, kb * 128, row, full);
-        } else if (brings_scales && lane >= 5 && lane <= 5 + groups) {
-          tiled_copy_2d_g2s_pair(scale_ring + scales * G8_SCALES + (lane - 5) * B8_PIECE, lane == 5 ? &a.w_scale_map : &a.x_scale_map, 0,
-                                 (group * a.pieces + kb / 4) * 4, full);
+    // One thread, with its maps and addresses the same for the whole warp: a copy instruction takes them from uniform registers, and lanes that ask
+    // for a copy each, with maps of their own, are served one after the other (PLACEHOLDER).
+    if (elect_one()) {
+      int stage = 0, scales = 0;
+      unsigned phase = 0;
+      while (share.next(a, item, k_first, k_end)) {
+        const Run8 run = run_of(a, item % runs);
+        const int block = item / runs, half = half_columns(run.rows);
+        const int w_group = w_group_of(a, run.matrix, block, rank), w_row = w_group * a.k_blocks * 128;
+        const int x_row = run.place + half * rank, w_scales = w_group * a.pieces * 4, x_scales = run.place / a.cap * a.pieces * 4 * a.run_groups;
+        bool ok = true;
+        for (int kb = k_first; kb < k_end; ++kb) {
+          ok = g8_wait(sh, &sh.empty[stage], phase ^ 1);
+          if (!ok) break;
+          const bool with_scales = brings_scales(kb, k_first), asked = ahead > 0;       // (its block of w is on its way already)
+          if (asked) --ahead;
+          if (rank == 0 && !asked)
+            mbar_arrive_expect_tx(&sh.full[stage], 2 * (Shape::STAGE_BYTES + (with_scales ? B8_PIECE + Shape::X_SCALES : 0)));
+          const unsigned full = in_cta_of_rank(smem_u32(&sh.full[stage]), 0);
+          unsigned char* slot = ring + stage * Shape::STAGE_BYTES;
+          if (!asked) tiled_copy_2d_g2s_pair(slot, &a.w_map, 0, w_row + kb * 128, full);
+          tiled_copy_2d_g2s_pair(slot + G8_W_BYTES, &a.x_map, kb * 128, x_row, full);
+          if (with_scales) {
+            unsigned char* at = scale_ring + scales * G8_SCALES;
+            tiled_copy_2d_g2s_pair(at, &a.w_scale_map, 0, w_scales + kb / 4 * 4, full);
+            tiled_copy_2d_g2s_pair(at + B8_PIECE, &a.x_scale_map, 0, x_scales + kb / 4 * 4 * a.run_groups, full);
+            if (++scales == Shape::STAGES) scales = 0;
+          }
+          if (++stage == Shape::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-        if (brings_scales && ++scales == Shape::STAGES) scales = 0;
-        if (++stage == Shape::STAGES) {
-          stage = 0;
-          phase ^= 1;
+        if (!ok) {
+          if (!sh.failed) report(a.status, STATUS_COPY_TIMEOUT, item, stage);
+          sh.failed = 1;
+          break;
         }
-      }
-      if (!ok) {
-        if (lane == 0 && !sh.failed) report(a.status, STATUS_COPY_TIMEOUT, item, stage);
-        sh.failed = 1;
-        break;
       }
     }
+    __syncwarp();
   } else if (warp == 1 && rank == 0) {
     const bool leader = elect_one();
     int stage = 0, acc = 0, scales = 0;
     unsigned phase = 0, acc_phase = 0;
-    for (int item = pair; item < items; item += pairs) {
+    while (share.next(a, item, k_first, k_end)) {
       const unsigned columns = 2 * half_columns(run_of(a, item % runs).rows), idesc = tc_idesc_scaled_pair(columns);
       bool ok = __all_sync(0xffffffffu, g8_wait(sh, &sh.acc_empty[acc], acc_phase ^ 1));
       if (!ok && leader && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -1);
       tc_fence_after_sync();
-      const unsigned d = tmem_base + acc * RUN;
-      unsigned scale_at = 0;
-      for (int kb = 0; kb < a.k_blocks && ok; ++kb) {
+      unsigned d = tmem_base + acc * RUN, scale_at = 0;
+      const int middle = a.halves ? (k_first + k_end) / 2 : k_first;
+      if (a.halves) d = tmem_base;
+      for (int kb = k_first; kb < k_end && ok; ++kb) {
         ok = __all_sync(0xffffffffu, g8_wait(sh, &sh.full[stage], phase));
         if (!ok) {
           if (leader && !sh.failed) report(a.status, STATUS_COPY_TIMEOUT, item, -2 - kb);
@@ -203,22 +277,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         tc_fence_after_sync();
         const unsigned slot = smem_u32(ring + stage * Shape::STAGE_BYTES);
         const unsigned long long w_desc = desc_k_major(slot), x_desc = desc_k_major(slot + G8_W_BYTES);
-        if (kb % 4 == 0) {
+        if (brings_scales(kb, k_first)) {
           scale_at = tmem_base + G8_SCALE_COLUMN + 12 * scales;
           if (leader) {
             const unsigned from = smem_u32(scale_ring + scales * G8_SCALES);
             tc_copy_scales_pair(scale_at, desc_scales(from));
             tc_copy_scales_pair(scale_at + 4, desc_scales(from + B8_PIECE));
-            if (columns > 128) tc_copy_scales_pair(scale_at + 8, desc_scales(from + 2 * B8_PIECE));
+            if (RUN > 128 && columns > 128) tc_copy_scales_pair(scale_at + 8, desc_scales(from + 2 * B8_PIECE));
           }
           if (++scales == Shape::STAGES) scales = 0;
         }
+        if (kb == middle && kb != k_first) d += RUN;
         if (leader) {
           const unsigned chosen = idesc | (kb & 3) << 4 | (kb & 3) << 29;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_scaled_pair(d, w_desc + 2 * k, x_desc + 2 * k, chosen, scale_at, scale_at + 4, (kb | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) tc_mma_scaled_pair(d, w_desc + 2 * k, x_desc + 2 * k, chosen, scale_at, scale_at + 4, (kb != k_first && kb != middle) || k != 0 ? 1u : 0u);
           tc_commit_pair(&sh.empty[stage]);
-          if (kb + 1 == a.k_blocks) tc_commit_pair(&sh.acc_full[acc]);
+          if (kb + 1 == k_end) tc_commit_pair(&sh.acc_full[acc]);
         }
         if (++stage == Shape::STAGES) {
           stage = 0;
@@ -229,7 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         sh.failed = 1;
         break;
       }
-      if (++acc == Shape::ACCUMULATORS) {
+      if (++acc == accumulators) {
         acc = 0;
         acc_phase ^= 1;
       }
@@ -245,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     TOut* y = static_cast<TOut*>(a.y);
     int acc = 0;
     unsigned acc_phase = 0;
-    for (int item = pair; item < items; item += pairs) {
+    while (share.next(a, item, k_first, k_end)) {
       const Run8 run = run_of(a, item % runs);
       const int row = item / runs * 256 + 128 * rank + 32 * quarter + lane, column0 = (row - lane) / (GATED ? 2 : 1);
       const float bias = a.gate.bias != nullptr && row < a.N ? a.gate.bias[row] : 0.0f;
@@ -256,10 +331,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       }
       tc_fence_after_sync();
       const unsigned tmem_row = tmem_base + (static_cast<unsigned>(32 * quarter) << 16) + acc * RUN;
-      for (int c = 32 * (warp > 5); c < run.rows; c += 64) {          // (columns beyond the product's are read and not used)
-        unsigned v[32];
+      const bool two = a.halves && (k_first + k_end) / 2 != k_first;
+      auto read_sums = [&](int c, unsigned (&v)[32]) {
         tmem_ld32(tmem_row + c, v);
         tmem_wait_ld32(v);
+        if (RUN <= 128 && two) {
+          unsigned more[32];
+          tmem_ld32(tmem_row + RUN + c, more);
+          tmem_wait_ld32(more);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(more[i]));
+        }
+      };
+      // Another pair's or this one's part of a tile: [column][row].
+      auto part_of = [&](int p) { return a.parts + (static_cast<size_t>(p) * 2 + rank) * RUN * 128 + 32 * quarter + lane; };
+      auto flag_of = [&](int p) { return a.flags + (p * 2 + rank) * 8 + warp - 2; };
+      if (k_end < a.k_blocks) {                       // (only with `parts`) the tile's end is another pair's
+        float* part = part_of(pair);
+        for (int c = 32 * (warp > 5); c < run.rows; c += 64) {
+          unsigned v[32];
+          read_sums(c, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) __stcg(part + (c + i) * 128, __uint_as_float(v[i]));
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) atomicExch(flag_of(pair), 1);
+      }
+      int others = 0;                                 // pairs in front of this one that have blocks of the tile
+      if (k_end == a.k_blocks && k_first > 0) {
+        const long long start = static_cast<long long>(item) * a.k_blocks;
+        do ++others; while (share.border(pair - others) > start);
+        bool ok = true;
+        for (int p = pair - others; p < pair && ok; ++p) {
+          int waited = 0;
+          while (*static_cast<volatile int*>(flag_of(p)) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(64);
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -4);
+          sh.failed = 1;
+          break;
+        }
+        __threadfence();
+      }
+      for (int c = 32 * (warp > 5); c < run.rows && k_end == a.k_blocks; c += 64) {          // (columns beyond the product's are read and not used)
+        unsigned v[32];
+        read_sums(c, v);
+        // The others' parts in the order of K's blocks, 16 columns of two pairs on their way at a time.
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (c + 16 * half >= run.rows) break;
+          for (int p = pair - others; p < pair; p += 2) {
+            const float *part = part_of(p) + (c + 16 * half) * 128, *next = p + 1 < pair ? part_of(p + 1) + (c + 16 * half) * 128 : part;
+            float one[16], other[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) one[i] = __ldcg(part + i * 128);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) other[i] = __ldcg(next + i * 128);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float sum = __uint_as_float(v[16 * half + i]) + one[i];
+              v[16 * half + i] = __float_as_uint(p + 1 < pair ? sum + other[i] : sum);
+            }
+          }
+        }
         TOut* mine = staging + (GATED ? (lane >> 4) * 8 + (lane & 7) : lane);
         if (GATED) {
           // Lane l holds the gates, lane l + 8 their ups of 32 rows: the first finishes 16 of them, the second the others.
@@ -312,7 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
-      if (++acc == Shape::ACCUMULATORS) {
+      if (++acc == accumulators) {
         acc = 0;
         acc_phase ^= 1;
       }
@@ -332,33 +467,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
   }
 }
 
-// A map of rows of `columns` bytes, `pitch` bytes apart, in boxes of 128 bytes x box_rows rows.
-static bool byte_rows_map(CUtensorMap* out, const void* base, long long rows, long long columns, long long pitch, int box_rows, bool swizzled) {
-  const EncodeTiled encode = tensor_map_encoder();
-  if (encode == nullptr || rows <= 0) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t element_strides[2] = {1, 1};
-  return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+// How many pairs of this kernel the device holds at once (0: the runtime has failed).
+template <typename Kernel>
+int pairs_at_once(Kernel kernel, int smem, int sms) {
+  if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return 0;
+  cudaLaunchConfig_t config = {};
+  config.blockDim = dim3(G8_THREADS);
+  config.dynamicSmemBytes = smem;
+  config.gridDim = dim3(2 * (sms / 2));
+  int clusters = 0;
+  if (cuda_failed(cudaOccupancyMaxActiveClusters(&clusters, kernel, &config))) return 0;
+  return clusters < G8_PAIRS ? clusters : G8_PAIRS;
 }
 
 template <int RUN, typename TOut, bool GATED, bool SCALED>
-int block8_launch(const Block8Args& a, long long max_runs, int sms, cudaStream_t stream) {
+int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) {
   using Shape = Block8Shape<RUN>;
   auto kernel = gemm_block8_kernel<RUN, TOut, GATED, SCALED>;
-  if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM_BYTES))) return ERR_CUDA;
+  static std::atomic<int> known[64];                // by device: asking takes the host 3 us
+  int device = 0, sms = 0;
+  if (cuda_failed(cudaGetDevice(&device))) return ERR_CUDA;
+  int pairs = device < 64 ? known[device].load() : 0;
+  if (pairs == 0) {
+    if (cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
+    pairs = pairs_at_once(kernel, Shape::SMEM_BYTES, sms);
+    if (pairs <= 0) return ERR_CUDA;
+    if (device < 64) known[device].store(pairs);
+  }
+  const long long items = max_runs * a.row_blocks;
   cudaLaunchConfig_t config = {};
+  // (With `parts` pairs wait for one another: all of them are on the device at once.)
+  config.gridDim = dim3(2 * static_cast<unsigned>(a.parts != nullptr || items > pairs ? pairs : items));
   config.blockDim = dim3(G8_THREADS);
   config.dynamicSmemBytes = Shape::SMEM_BYTES;
   config.stream = stream;
-  config.gridDim = dim3(2 * (sms / 2));
-  int clusters = 0;                                 // how many pairs the device holds at once
-  if (cuda_failed(cudaOccupancyMaxActiveClusters(&clusters, kernel, &config)) || clusters <= 0) return ERR_CUDA;
-  const long long items = max_runs * a.row_blocks;
-  config.gridDim = dim3(2 * static_cast<unsigned>(items < clusters ? items : clusters));
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
@@ -367,55 +509,39 @@ int block8_launch(const Block8Args& a, long long max_runs, int sms, cudaStream_t
   return cuda_failed(cudaLaunchKernelEx(&config, kernel, a)) ? ERR_CUDA : launch_result();
 }
 template <int RUN, typename TOut>
-int block8_form(const Block8Args& a, bool gated, long long max_runs, int sms, cudaStream_t stream) {
-  if (!gated) return block8_launch<RUN, TOut, false, false>(a, max_runs, sms, stream);
-  return a.gate.row_scale != nullptr ? block8_launch<RUN, TOut, true, true>(a, max_runs, sms, stream)
-                                     : block8_launch<RUN, TOut, true, false>(a, max_runs, sms, stream);
+int block8_form(const Block8Args& a, bool gated, long long max_runs, cudaStream_t stream) {
+  if (!gated) return block8_launch<RUN, TOut, false, false>(a, max_runs, stream);
+  return a.gate.row_scale != nullptr ? block8_launch<RUN, TOut, true, true>(a, max_runs, stream)
+                                     : block8_launch<RUN, TOut, true, false>(a, max_runs, stream);
 }
 template <typename TOut>
-int block8_run(const Block8Args& a, bool gated, long long max_runs, int sms, cudaStream_t stream) {
-  return a.cap == 64 ? block8_form<64, TOut>(a, gated, max_runs, sms, stream)
-         : a.cap == 128 ? block8_form<128, TOut>(a, gated, max_runs, sms, stream) : block8_form<256, TOut>(a, gated, max_runs, sms, stream);
+int block8_run(const Block8Args& a, bool gated, long long max_runs, cudaStream_t stream) {
+  return a.cap == 64 ? block8_form<64, TOut>(a, gated, max_runs, stream)
+         : a.cap == 128 ? block8_form<128, TOut>(a, gated, max_runs, stream) : block8_form<256, TOut>(a, gated, max_runs, stream);
+}
+
+// The operands and results of a product (block8.cuh): y = x w^T in blocks.  Without `plan` M rows of x in runs of `run`, one matrix, y [M]; with it
+// (zb_route_align_strided) `max_runs` runs at most of `matrices`, y by place.
+int block8_product(const Block8Product& p, cudaStream_t stream) {
+  const bool gated = p.kind >= 1 && p.kind <= 3;
+  Block8Args a = {};
+  const long long runs = p.plan != nullptr ? p.max_runs : (p.M + p.run - 1) / p.run;
+  a.y = p.y; a.ldy = p.ldy; a.N = p.N; a.row_blocks = (p.N + 255) / 256; a.scale_groups = b8_blocks(p.N); a.k_blocks = b8_blocks(p.K); a.pieces = b8_pieces(p.K);
+  a.w_groups = p.matrices * a.scale_groups; a.run_groups = (p.cap + 127) / 128; a.plan = p.plan; a.M = p.M; a.run = p.run; a.cap = p.cap; a.status = p.status;
+  a.parts = p.parts; a.flags = p.flags; a.least = p.least; a.halves = p.halves;
+  const int per_piece = p.y_dtype == DTYPE_F32 ? 4 : 8;
+  a.wide = p.ldy % per_piece == 0 && (gated ? p.N / 2 : p.N) % per_piece == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  a.act = p.kind == 4 ? ACT_GELU : p.kind == 5 ? ACT_RELU2 : ACT_NONE;
+  a.gate = p.kind == 3 ? GateForm{GATE_BOUNDED, p.bias, p.limit, p.alpha, p.shift, nullptr} : plain_gate(p.kind == 2 ? GATE_RELU : GATE_SILU);
+  a.gate.row_scale = p.row_scale;
+  const long long pitch = b8_pitch(p.K), w_rows = static_cast<long long>(a.w_groups) * a.k_blocks * 128;
+  const long long scale_rows = static_cast<long long>(a.w_groups) * a.pieces * 4, x_scale_rows = runs * a.run_groups * a.pieces * 4;
+  if (w_rows >= (1LL << 31) || runs * p.cap >= (1LL << 31) || x_scale_rows >= (1LL << 31) || runs * a.row_blocks >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (!byte_rows_map(&a.w_map, p.w_codes, w_rows, 128, 128, 128, true) || !byte_rows_map(&a.x_map, p.x_codes, runs * p.cap, pitch, pitch, p.cap / 2, true) ||
+      !byte_rows_map(&a.w_scale_map, p.w_scales, scale_rows, 128, 128, 4, false) ||
+      !byte_rows_map(&a.x_scale_map, p.x_scales, x_scale_rows, 128, 128, 4 * a.run_groups, false))
+    return ERR_CUDA;
+  return p.y_dtype == DTYPE_F32 ? block8_run<float>(a, gated, runs, stream) : block8_run<__nv_bfloat16>(a, gated, runs, stream);
 }
 
 }  // namespace zb
-
-using namespace zb;
-
-// y = x w^T in blocks.  Rows of x lie as codes at places, runs of them `cap` (64, 128 or 256) places apart (zb_code_rows).  Without `plan`: M rows
-// in runs of `run`, one matrix, y [M]; with it (zb_route_align_strided): `max_runs` runs at most, `matrices` of them, y by place.  kind: 0 the sums,
-// 1 silu(gate) * up, 2 max(gate, 0) * up, 3 the bounded gate (`bias`: float32 [N] or null), 4 gelu_tanh of the sums, 5 the square of max(sum, 0).
-ZB_API int zb_gemm_block8(void* y, long long ldy, int y_dtype, const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
-                          const int* plan, int max_runs, int matrices, int M, int run, int cap, int N, int K, int kind, const float* bias,
-                          const float* row_scale, float limit, float alpha, float shift, int* status, void* stream) {
-  const bool gated = kind >= 1 && kind <= 3;
-  if (matrices <= 0 || N <= 0 || K <= 0 || (cap != 64 && cap != 128 && cap != 256) || kind < 0 || kind > 5 || (gated && N % 16 != 0) ||
-      ldy < (gated ? N / 2 : N) || (y_dtype != DTYPE_F32 && y_dtype != DTYPE_BF16) || (kind == 3 && !(limit > 0.0f)) || (kind != 3 && bias != nullptr) ||
-      (row_scale != nullptr && (kind == 0 || kind > 2)) || (plan == nullptr ? M <= 0 || run <= 0 || run > cap || run % 16 != 0 || matrices != 1 : max_runs <= 0))
-    return ERR_BAD_ARGUMENT;
-  const auto unaligned = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
-  if (unaligned(x_codes, 16) || unaligned(x_scales, 16) || unaligned(w_codes, 16) || unaligned(w_scales, 16) || unaligned(bias, 4)) return ERR_BAD_ARGUMENT;
-  int device = 0, sms = 0;
-  if (cuda_failed(cudaGetDevice(&device)) || cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
-  Block8Args a = {};
-  const long long runs = plan != nullptr ? max_runs : (M + run - 1) / run;
-  a.y = y; a.ldy = ldy; a.N = N; a.row_blocks = (N + 255) / 256; a.scale_groups = b8_blocks(N); a.k_blocks = b8_blocks(K); a.pieces = b8_pieces(K);
-  a.run_groups = (cap + 127) / 128; a.plan = plan; a.M = M; a.run = run; a.cap = cap; a.status = status;
-  const int per_piece = y_dtype == DTYPE_F32 ? 4 : 8;
-  a.wide = ldy % per_piece == 0 && (gated ? N / 2 : N) % per_piece == 0 && !unaligned(y, 16);
-  a.act = kind == 4 ? ACT_GELU : kind == 5 ? ACT_RELU2 : ACT_NONE;
-  a.gate = kind == 3 ? GateForm{GATE_BOUNDED, bias, limit, alpha, shift, nullptr} : plain_gate(kind == 2 ? GATE_RELU : GATE_SILU);
-  a.gate.row_scale = row_scale;
-  const long long scale_rows = static_cast<long long>(matrices) * a.scale_groups * a.pieces * 4, x_scale_rows = runs * a.run_groups * a.pieces * 4;
-  if (static_cast<long long>(matrices) * N >= (1LL << 31) || runs * cap >= (1LL << 31) || scale_rows >= (1LL << 31) || x_scale_rows >= (1LL << 31) ||
-      runs * a.row_blocks >= (1LL << 31))
-    return ERR_UNSUPPORTED;
-  const long long pitch = b8_pitch(K);
-  if (!byte_rows_map(&a.w_map, w_codes, static_cast<long long>(matrices) * N, pitch, pitch, 128, true) ||
-      !byte_rows_map(&a.x_map, x_codes, runs * cap, pitch, pitch, G8_X_BOX, true) ||
-      !byte_rows_map(&a.w_scale_map, w_scales, scale_rows, 128, 128, 4, false) ||
-      !byte_rows_map(&a.x_scale_map, x_scales, x_scale_rows, 128, 128, 4, false))
-    return ERR_CUDA;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return y_dtype == DTYPE_F32 ? block8_run<float>(a, gated, runs, sms, s) : block8_run<__nv_bfloat16>(a, gated, runs, sms, s);
-}

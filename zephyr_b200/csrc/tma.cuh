@@ -27,6 +27,19 @@ inline EncodeTiled tensor_map_encoder() {
   return encoder;
 }
 
+// A map of rows of `columns` bytes, `pitch` bytes apart, in boxes of 128 bytes x box_rows rows.
+inline bool byte_rows_map(CUtensorMap* out, const void* base, long long rows, long long columns, long long pitch, int box_rows, bool swizzled) {
+  const EncodeTiled encode = tensor_map_encoder();
+  if (encode == nullptr || rows <= 0) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t element_strides[2] = {1, 1};
+  return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // One tiled copy of a two-dimensional box at (x, y) into shared memory; x * element size must be a
 // multiple of 16 bytes.  Completion is counted in bytes on `bar`.
 __device__ __forceinline__ void tiled_copy_2d_g2s(void* smem_dst, const CUtensorMap* map, int x, int y,

@@ -85,14 +85,9 @@ _SIGNATURES = {
                           c_int, c_int, c_int, c_float, c_float, c_float, c_int, c_int, c_void_p],
     "zb_route_align_runs": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "zb_route_align_strided": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
-    "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
+    "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
     "zb_matrix_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
-    "zb_code_rows": [c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p],
-    "zb_gemm_block8": [c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                       c_int, c_void_p, c_void_p, c_float, c_float, c_float, c_void_p, c_void_p],
-    "zb_gemm_block8_small_supported": [c_int, c_int, c_int],
-    "zb_gemm_block8_small": [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
-                             c_float, c_float, c_float, c_void_p],
+    "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int],
     "zb_gather_places": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "zb_gemm_tc_experts_run": [c_int, c_int],
     "zb_gemm_tc_experts": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int,
@@ -273,6 +268,11 @@ def library() -> ctypes.CDLL:
             lib.zb_paged_decode_balanced_scratch_floats.restype = c_longlong
             lib.zb_paged_decode_packed_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
             lib.zb_paged_decode_packed_scratch_floats.restype = c_longlong
+            lib.zb_block8_product_work.argtypes = [c_longlong, c_longlong, c_longlong, c_int]
+            lib.zb_block8_feed_forward_work.argtypes = [c_longlong, c_longlong, c_longlong, c_longlong, c_int]
+            lib.zb_block8_experts_work.argtypes = [c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, c_int]
+            for name in ("zb_block8_product_work", "zb_block8_feed_forward_work", "zb_block8_experts_work"):
+                getattr(lib, name).restype = c_longlong
             if os.environ.get("ZEPHYR_B200_DEPENDENT_LAUNCH", "1") == "0":
                 lib.zb_set_dependent_launch(0)
             _lib = lib
@@ -2550,7 +2550,7 @@ def routed_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_
         _check(lib.zb_gather_places(rows, _ptr(x), x.stride(0), slots, places, width, top, _ptr(place_scale), _ptr(weights), stream),
                "gather_places")
         _check(lib.zb_gemm_tc_experts(hidden, rows, _ptr(w_gate), plan, runs, run, places, E, 2 * ff, width, width, ff, 1 + act_code,
-                                      _ptr(place_scale), *bounds, status, stream), "gemm_tc_grouped")
+                                      _ptr(place_scale), *bounds, None, None, 0, status, stream), "gemm_tc_grouped")
         _check(lib.zb_gemm_tc_experts(_ptr(y), hidden, _ptr(w_down), plan, runs, run, places, E, width, ff, ff, ldy, 0, None, *bounds,
                                       status, stream), "gemm_tc_grouped")
     else:
@@ -2577,7 +2577,6 @@ USE_GROUPED_TCGEN05 = True      # off: a routed layer's products stay on the mma
 
 # ------------------------------------------- matrices in 8-bit floating point, a scale for each block of 128
 BLOCK8 = 128                  # rows and columns of a matrix, values of a row of activations, that share a scale
-BLOCK8_FEW_ROWS = 16          # up to here a product streams the matrix and codes its rows on the way
 _BLOCK8_KINDS = {"silu": 1, "relu": 2}
 
 
@@ -2587,24 +2586,45 @@ class BlockMatrix:
     code * power; one that was not finite is NaN.  ``pack_matrix`` makes it from a bfloat16 or float32 tensor, ``BlockMatrix.from_codes`` from codes that
     exist; ``linear``, ``block_linear``, ``block_feed_forward`` and ``routed_experts`` take it where they take a matrix.
 
-    ``codes``: uint8 [matrices * N, K rounded up to 128], zeros behind K; ``scales``: uint8 [matrices, N / 128 up, K / 512 up, 512], the bytes (exponent +
-    127) of four neighbouring blocks of K for each of a block's 128 rows, as the tensor cores read them."""
+    Everything lies in one uint8 tensor, ``data``: ``codes`` [matrices, N / 128 up, K / 128 up, 128, 128], block by block, zeros behind N and K;
+    ``scales`` [matrices, N / 128 up, K / 512 up, 512], the bytes (exponent + 127) of four neighbouring blocks of K for each of a block's 128 rows, as
+    the tensor cores read them; and the bytes once a block, ``exponents()``."""
 
-    __slots__ = ("codes", "scales", "matrices", "N", "K", "shape", "device")
+    __slots__ = ("data", "shape", "matrices", "N", "K", "blocks", "codes_at", "scales_at", "_total")
     dtype = torch.float8_e4m3fn
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Sequence[int]):
-        self.codes, self.scales, self.shape, self.device = codes, scales, torch.Size(shape), codes.device
+    def __init__(self, data: torch.Tensor, shape: Sequence[int], total: tuple[int, int]):
+        """``total``: the bytes of codes and of scales in ``data``."""
+        self.data, self.shape, self._total = data, torch.Size(shape), total
         self.matrices = shape[0] if len(shape) == 3 else 1
         self.N, self.K = shape[-2:]
+        self.blocks = (-(-self.N // BLOCK8), -(-self.K // BLOCK8))
+        self.codes_at = data.data_ptr()
+        self.scales_at = self.codes_at + total[0]
 
     @staticmethod
     def _empty(shape: Sequence[int], device) -> "BlockMatrix":
-        _require(len(shape) in (2, 3) and min(shape) > 0, "a matrix [N, K] or matrices [matrices, N, K] that are not empty")
-        matrices, (n, k) = shape[0] if len(shape) == 3 else 1, shape[-2:]
-        _require(matrices * n < 2 ** 31 and n <= 65535 * BLOCK8 and matrices <= 65535 and k < 2 ** 31 - 512, "sizes that 32 bits can count")
-        codes = torch.empty((matrices * n, -(-k // BLOCK8) * BLOCK8), dtype=torch.uint8, device=device)
-        return BlockMatrix(codes, torch.empty((matrices, -(-n // BLOCK8), -(-k // (4 * BLOCK8)), 512), dtype=torch.uint8, device=device), shape)
+        if len(shape) not in (2, 3) or min(shape) <= 0:
+            raise InvalidArgumentError("a matrix [N, K] or matrices [matrices, N, K] that are not empty")
+        matrices, n, k = shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1]
+        rows, columns = -(-n // BLOCK8), -(-k // BLOCK8)
+        if rows > 65535 or matrices > 65535 or matrices * rows * columns * BLOCK8 >= 2 ** 31:
+            raise InvalidArgumentError("sizes that 32 bits can count")
+        codes, scales = matrices * rows * columns * BLOCK8 * BLOCK8, matrices * rows * -(-columns // 4) * 512
+        return BlockMatrix(torch.empty(codes + scales + matrices * rows * columns, dtype=torch.uint8, device=device), shape, (codes, scales))
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[: self.matrices * self.blocks[0] * self.blocks[1] * BLOCK8 ** 2].view(self.matrices, *self.blocks, BLOCK8, BLOCK8)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        pieces = -(-self.blocks[1] // 4)
+        return self.data[self._total[0] :][: self.matrices * self.blocks[0] * pieces * 512].view(self.matrices, self.blocks[0], pieces, 512)
 
     @staticmethod
     def from_codes(codes: torch.Tensor, exponents: torch.Tensor) -> "BlockMatrix":
@@ -2614,34 +2634,37 @@ class BlockMatrix:
         _require(codes.dim() in (2, 3) and codes.dtype in (torch.uint8, torch.float8_e4m3fn) and exponents.dtype is torch.uint8,
                  "codes in 8 bits (float8_e4m3fn or uint8) and uint8 exponents")
         made = BlockMatrix._empty(codes.shape, codes.device)
-        blocks = (-(-made.N // BLOCK8), -(-made.K // BLOCK8))
-        _require(tuple(exponents.shape) == (*codes.shape[:-2], *blocks) and exponents.device == codes.device,
-                 f"one exponent for each block of 128 x 128: {[*codes.shape[:-2], *blocks]}")
+        rows, columns = made.blocks
+        _require(tuple(exponents.shape) == (*codes.shape[:-2], rows, columns) and exponents.device == codes.device,
+                 f"one exponent for each block of 128 x 128: {[*codes.shape[:-2], rows, columns]}")
         _require(bool(((exponents >= 1) & (exponents <= 254)).all()), "exponents are bytes between 1 and 254 (2^-126 to 2^127)")
-        made.codes.zero_()
-        made.codes[:, : made.K] = codes.reshape(-1, made.K).view(torch.uint8)
-        padded = torch.ones((made.matrices, blocks[0], made.scales.shape[2] * 4), dtype=torch.uint8, device=codes.device)
-        padded[:, :, : blocks[1]] = exponents.view(made.matrices, *blocks)
-        made.scales.copy_(padded.view(made.matrices, blocks[0], -1, 1, 4).expand(-1, -1, -1, 128, -1).reshape(made.scales.shape))
+        padded = torch.zeros((made.matrices, rows * BLOCK8, columns * BLOCK8), dtype=torch.uint8, device=codes.device)
+        padded[:, : made.N, : made.K] = codes.contiguous().view(torch.uint8).view(made.matrices, made.N, made.K)
+        made.codes.copy_(padded.view(made.matrices, rows, BLOCK8, columns, BLOCK8).transpose(2, 3))
+        pieces = torch.ones((made.matrices, rows, -(-columns // 4) * 4), dtype=torch.uint8, device=codes.device)
+        pieces[:, :, :columns] = exponents.view(made.matrices, rows, columns)
+        made.scales.copy_(pieces.view(made.matrices, rows, -1, 1, 4).expand(-1, -1, -1, 128, -1).reshape(made.scales.shape))
+        made.data[sum(made._total) :] = exponents.reshape(-1)
         return made
 
     def first_rows(self, rows: int) -> "BlockMatrix":
         """The first rows of one matrix, a multiple of 128 of them, over the same memory."""
         _require(len(self.shape) == 2 and 0 < rows <= self.N and (rows % BLOCK8 == 0 or rows == self.N), "whole blocks of a matrix's rows")
-        return BlockMatrix(self.codes[:rows], self.scales[:, : -(-rows // BLOCK8)], (rows, self.K))
+        return BlockMatrix(self.data, (rows, self.K), self._total)
 
     def exponents(self) -> torch.Tensor:
         """The blocks' bytes, exponent + 127: uint8 [N / 128 up, K / 128 up], with ``matrices`` ahead where there are several."""
-        found = self.scales[..., :4].flatten(2)[:, :, : -(-self.K // BLOCK8)]
-        return (found if len(self.shape) == 3 else found[0]).contiguous()
+        at = self._total[0] + self._total[1]
+        return self.data[at : at + self.matrices * self.blocks[0] * self.blocks[1]].view(*self.shape[:-2], *self.blocks)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the codes stand for (exact in bfloat16 but below its normal numbers)."""
-        _require(dtype in DTYPE_CODE, "values are bfloat16 or float32")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        (out_at, codes_at, scales_at), place = _addresses(out, self.codes, self.scales)
+        if dtype not in DTYPE_CODE:
+            raise InvalidArgumentError("values are bfloat16 or float32")
+        out = torch.empty(self.shape, dtype=dtype, device=self.data.device)
+        (out_at, _), place = _addresses(out, self.data)
         _check_place(place)
-        _check(library().zb_matrix_values(out_at, codes_at, scales_at, self.matrices, self.N, self.K, DTYPE_CODE[dtype], _stream()), "matrix_values")
+        _check(library().zb_matrix_values(out_at, self.codes_at, self.scales_at, self.matrices, self.N, self.K, DTYPE_CODE[dtype], _stream()), "matrix_values")
         return out
 
     def tensors(self) -> list[torch.Tensor]:
@@ -2651,35 +2674,61 @@ class BlockMatrix:
 def pack_matrix(w: torch.Tensor) -> BlockMatrix:
     """``w`` [N, K] or [matrices, N, K], bfloat16 or float32 with contiguous rows, in 8-bit floating point with a scale for each block of
     128 x 128 (``BlockMatrix``)."""
-    _require(w.dim() in (2, 3) and w.numel() > 0 and w.dtype in DTYPE_CODE and (w.stride(-1) == 1 or w.shape[-1] == 1),
-             "w [N, K] or [matrices, N, K], not empty, bfloat16 or float32 with unit inner stride")
-    _cuda(w)
-    made = BlockMatrix._empty(w.shape, w.device)
-    (codes_at, scales_at, w_at), place = _addresses(made.codes, made.scales, w)
+    shape = w.shape
+    if len(shape) not in (2, 3) or w.numel() == 0 or w.dtype not in DTYPE_CODE or (w.stride(-1) != 1 and shape[-1] != 1):
+        raise InvalidArgumentError("w [N, K] or [matrices, N, K], not empty, bfloat16 or float32 with unit inner stride")
+    (w_at,), place = _addresses(w)
     _check_place(place)
-    _check(library().zb_pack_matrix(codes_at, scales_at, w_at, made.matrices, w.stride(0) if w.dim() == 3 else 0, w.stride(-2), made.N, made.K,
-                                    DTYPE_CODE[w.dtype], _stream()), "pack_matrix")
+    made = BlockMatrix._empty(shape, w.device)
+    _check(library().zb_pack_matrix(made.codes_at, made.scales_at, made.scales_at + made._total[1], w_at, made.matrices, w.stride(0) if len(shape) == 3 else 0,
+                                    w.stride(-2), made.N, made.K, DTYPE_CODE[w.dtype], _stream()), "pack_matrix")
     return made
-
-
-def _block8_run(rows: int) -> tuple[int, int]:
-    """How many of so many rows form a run of the product's, and how far apart the runs' places begin: as few runs as 256 rows
-    allow, of equal length (a multiple of 16)."""
-    runs = -(-rows // 256)
-    run = -(-rows // (16 * runs)) * 16
-    return run, 64 if rows <= 64 else 128 if rows <= 128 else 256
 
 
 def _check_block8_rows(x: torch.Tensor, K: int) -> int:
     """Checks rows [M, K] as a product's input and gives their pitch."""
-    if x.dim() != 2 or x.shape[1] != K or x.dtype not in DTYPE_CODE:
-        raise InvalidArgumentError(f"x must be [M, {K}] in bfloat16 or float32, not {list(x.shape)} in {x.dtype}")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != K or x.dtype not in DTYPE_CODE:
+        raise InvalidArgumentError(f"x must be [M, {K}] in bfloat16 or float32, not {list(shape)} in {x.dtype}")
     pitch, inner = x.stride()
-    if x.shape[0] <= 1:
+    if shape[0] <= 1:
         pitch = K
     if (inner != 1 and K > 1) or pitch < K:
         raise InvalidArgumentError("x's rows must have unit inner stride and not overlap")
     return pitch
+
+
+# What the calls are given, eight bytes a value (the structures beside them in csrc).
+_BLOCK8_PRODUCT = struct.Struct("=Q2qQ2q2Q4qQ3d3Q").pack
+_BLOCK8_FEED_FORWARD = struct.Struct("=Q2qQ2q4Q5qQ3d3Q").pack
+_BLOCK8_EXPERTS = struct.Struct("=2Q2q6Q7q3d3Q").pack
+
+
+@functools.lru_cache(maxsize=4096)
+def _block8_product_plan(M: int, N: int, K: int, y_code: int) -> tuple[int, int]:
+    """The bytes between a product's kernels, and how many kernels."""
+    return library().zb_block8_product_work(M, N, K, y_code), library().zb_block8_product_kernels(M, N, K)
+
+
+@functools.lru_cache(maxsize=4096)
+def _block8_feed_forward_plan(M: int, K: int, ff: int, N: int, y_code: int) -> tuple[int, int]:
+    lib = library()
+    return lib.zb_block8_feed_forward_work(M, K, ff, N, y_code), lib.zb_block8_product_kernels(M, 2 * ff, K) + lib.zb_block8_product_kernels(M, N, ff)
+
+
+@functools.lru_cache(maxsize=4096)
+def _block8_experts_work(T: int, top: int, E: int, width: int, ff: int, code: int, weigh_inputs: bool) -> int:
+    return library().zb_block8_experts_work(T, top, E, width, ff, code, int(weigh_inputs))
+
+
+def _block8_gate(rows: int, act: str, bounded: BoundedGate | None) -> tuple[int, int, float, float, float]:
+    """The gated epilogue's code, its bias's address and its constants."""
+    if rows % 16 != 0 or act not in ACTIVATIONS:
+        raise InvalidArgumentError(f"gate and up rows come in blocks of 8, their activation is one of {sorted(ACTIVATIONS)}")
+    if bounded is None:
+        return _BLOCK8_KINDS[act], 0, 0.0, 1.0, 0.0
+    bias, limit, alpha, shift = _bounded_args(bounded, rows)
+    return 3, bias or 0, limit, alpha, shift
 
 
 def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None = None, swiglu: bool = False, act: str = "silu",
@@ -2687,105 +2736,82 @@ def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None 
     """x [M, K] (bfloat16 or float32) times a matrix [N, K] in 8-bit floating point: x's rows are coded as the matrix is, in blocks of 128
     values, and y[m, n] = sum_k x~[m, k] w~[n, k] over what the codes stand for, summed in float32, in ``out_dtype`` (None: x's).  ``swiglu``: the rows of w are
     blocks of 8 gate rows and their 8 up rows, and the result is act(gate) * up (``act`` "silu" or "relu"; ``bounded``: the bounded gate), [M, N /
-    2]; ``product_act`` (without ``swiglu``): one of ``PRODUCT_ACTS`` of the sums.  Up to 16 rows are coded inside the product's kernel, which streams
-    the matrix; more by a kernel of their own ahead of it."""
-    if w.matrices != 1 or len(w.shape) != 2:
+    2]; ``product_act`` (without ``swiglu``): one of ``PRODUCT_ACTS`` of the sums.  Up to 16 rows of a matrix that is not large are coded inside the
+    product's kernel, which streams the matrix; others by a kernel of their own ahead of it."""
+    if len(w.shape) != 2:
         raise InvalidArgumentError("a product takes one matrix")
-    M, K, N = x.shape[0], w.K, w.N
-    pitch = _check_block8_rows(x, K)
+    pitch = _check_block8_rows(x, w.K)
+    M, N = x.shape[0], w.N
     out_dtype = out_dtype or x.dtype
     if out_dtype not in DTYPE_CODE:
         raise InvalidArgumentError("the result is bfloat16 or float32")
-    kind, bias, limits = 0, None, (0.0, 1.0, 0.0)
+    gate = (0, 0, 0.0, 1.0, 0.0)
     if swiglu:
-        if product_act is not None or N % 16 != 0 or act not in ACTIVATIONS:
-            raise InvalidArgumentError(f"swiglu takes a multiple of 16 rows and one of {sorted(ACTIVATIONS)}")
-        kind = _BLOCK8_KINDS[act]
-        if bounded is not None:
-            bias, *limits = _bounded_args(bounded, N)
-            kind = 3
+        if product_act is not None:
+            raise InvalidArgumentError("a gated product has its gate's activation")
+        gate = _block8_gate(N, act, bounded)
     elif bounded is not None or product_act is not None:
         if bounded is not None or product_act not in PRODUCT_ACTS:
             raise InvalidArgumentError(f"an ungated product's epilogue is one of {sorted(PRODUCT_ACTS)}; the bounded gate is a gated one")
-        kind = 3 + PRODUCT_ACTS[product_act]
-    out = torch.empty((M, N // 2 if swiglu else N), dtype=out_dtype, device=x.device)
-    (out_at, x_at, codes_at, scales_at, _), place = _addresses(out, x, w.codes, w.scales, bounded.bias if bounded is not None else None)
+        gate = (3 + PRODUCT_ACTS[product_act], 0, 0.0, 1.0, 0.0)
+    (x_at, _, _), place = _addresses(x, w.data, bounded.bias if bounded is not None else None)
     _check_place(place)
+    width, y_code = N // 2 if swiglu else N, DTYPE_CODE[out_dtype]
+    out = torch.empty((M, width), dtype=out_dtype, device=x.device)
     if M == 0:
         return out
-    lib, x_code, y_code, width = library(), DTYPE_CODE[x.dtype], DTYPE_CODE[out_dtype], out.shape[1]
-    if M <= BLOCK8_FEW_ROWS and lib.zb_gemm_block8_small_supported(M, N, K):
-        _check(lib.zb_gemm_block8_small(out_at, width, y_code, x_at, pitch, x_code, codes_at, scales_at, M, N, K, kind, bias, *limits, _stream()),
-               "gemm_block8_small")
-        return out
-    stream = _stream()
-    run, cap = _block8_run(M)
-    rows, row_scales = _block8_workspace(x, -(-M // run) * cap, cap, K)
-    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, x_at, pitch, None, M, K, run, cap, 0, None, None, x_code, stream), "code_rows")
-    _check(lib.zb_gemm_block8(out_at, width, y_code, rows.data_ptr(), row_scales, codes_at, scales_at, None, 0, 1, M, run, cap, N, K, kind, bias, None,
-                              *limits, _device_status_pointer(x.device), stream), "gemm_block8")
+    bytes_, kernels = _block8_product_plan(M, N, w.K, y_code)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device) if bytes_ else None
+    _check(library().zb_block8_product(_BLOCK8_PRODUCT(
+        out.data_ptr(), width, y_code, x_at, pitch, DTYPE_CODE[x.dtype], w.codes_at, w.scales_at, M, N, w.K, *gate, work.data_ptr() if bytes_ else 0,
+        _device_status_pointer(x.device) or 0, _stream())), "block_linear", kernels)
     return out
-
-
-def _block8_workspace(x: torch.Tensor, places: int, cap: int, K: int) -> tuple[torch.Tensor, int]:
-    """Room for the codes of so many places and, behind them, their scales: the tensor that holds both, and the scales' address."""
-    codes = places * (-(-K // BLOCK8) * BLOCK8)
-    work = torch.empty(codes + places // cap * -(-cap // 128) * -(-K // 512) * 512, dtype=torch.uint8, device=x.device)
-    return work, work.data_ptr() + codes
 
 
 def block_feed_forward(x: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix, act: str = "silu", bounded: BoundedGate | None = None,
                        out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """down(act(gate x) * up x) on matrices in 8-bit floating point: ``gate_up`` [2 ff, K] in blocks of 8 gate rows and their 8 up rows, ``down`` [N,
     ff].  The hidden values stay in float32 until they are coded for the second product."""
-    if gate_up.matrices != 1 or down.matrices != 1 or gate_up.N != 2 * down.K:
+    if len(gate_up.shape) != 2 or len(down.shape) != 2 or gate_up.N != 2 * down.K:
         raise InvalidArgumentError(f"gate_up [2 ff, K] and down [N, ff], not {list(gate_up.shape)} and {list(down.shape)}")
-    hidden = block_linear(x, gate_up, torch.float32, swiglu=True, act=act, bounded=bounded)
-    return block_linear(hidden, down, out_dtype or x.dtype)
+    pitch = _check_block8_rows(x, gate_up.K)
+    M, N, ff = x.shape[0], down.N, down.K
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in DTYPE_CODE:
+        raise InvalidArgumentError("the result is bfloat16 or float32")
+    gate = _block8_gate(gate_up.N, act, bounded)
+    (x_at, _, _, _), place = _addresses(x, gate_up.data, down.data, bounded.bias if bounded is not None else None)
+    _check_place(place)
+    y_code = DTYPE_CODE[out_dtype]
+    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    if M == 0:
+        return out
+    bytes_, kernels = _block8_feed_forward_plan(M, gate_up.K, ff, N, y_code)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device)
+    _check(library().zb_block8_feed_forward(_BLOCK8_FEED_FORWARD(
+        out.data_ptr(), N, y_code, x_at, pitch, DTYPE_CODE[x.dtype], gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, M, gate_up.K, ff, N,
+        *gate, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "block_feed_forward", kernels)
+    return out
 
 
 def _routed_blocks(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix, act: str,
                    weigh_inputs: bool, bounded: BoundedGate | None) -> torch.Tensor:
-    """``routed_experts`` on matrices in 8-bit floating point: the rows are coded where they are gathered, the hidden values stay in float32 until
-    they are coded for the second product, an expert's output is rounded to x's type before it is weighted."""
-    T, width = x.shape
-    top, E, ff = ids.shape[1], gate_up.matrices, down.K
+    """``routed_experts`` on matrices in 8-bit floating point."""
     pitch = _check_block8_rows(x, gate_up.K)
-    if (len(gate_up.shape) != 3 or len(down.shape) != 3 or down.matrices != E or gate_up.N != 2 * ff or down.N != width or ff % 8 != 0):
+    (T, width), top, E, ff = x.shape, ids.shape[1], gate_up.matrices, down.K
+    if len(gate_up.shape) != 3 or len(down.shape) != 3 or down.matrices != E or gate_up.N != 2 * ff or down.N != width or ff % 8 != 0:
         raise InvalidArgumentError(f"expert matrices [E, 2 ff, width] and [E, width, ff], ff a multiple of 8, not {list(gate_up.shape)} and {list(down.shape)}")
-    out = torch.empty((T, width), dtype=x.dtype, device=x.device)
-    (out_at, x_at, ids_at, weights_at, up_at, up_scales, down_at, down_scales), place = _addresses(
-        out, x, ids, weights, gate_up.codes, gate_up.scales, down.codes, down.scales)
+    kind, _, *bounds = _block8_gate(gate_up.N, act, bounded)
+    (x_at, ids_at, weights_at, _, _), place = _addresses(x, ids, weights, gate_up.data, down.data)
     _check_place(place)
+    out = torch.empty((T, width), dtype=x.dtype, device=x.device)
     if T == 0 or top == 0:
         return out.zero_()
-    lib, device, code, stream = library(), x.device, DTYPE_CODE[x.dtype], _stream()
-    status = _device_status_pointer(device)
-    num_slots = T * top
-    run = lib.zb_gemm_tc_experts_run(num_slots, E)
-    runs = num_slots // run + E
-    places = runs * run
-    numbers = torch.empty(1 + 3 * runs + places + num_slots, dtype=torch.int32, device=device)
-    plan = numbers.data_ptr()
-    slots = plan + 4 * (1 + 3 * runs)
-    place_of_slot = slots + 4 * places
-    _check(lib.zb_route_align_strided(plan, slots, place_of_slot, ids_at, num_slots, E, runs, run, places, stream), "route_align")
-    kind = 3 if bounded is not None else _BLOCK8_KINDS[act]
-    bounds = (float(bounded.limit), float(bounded.alpha), float(bounded.shift)) if bounded is not None else (0.0, 1.0, 0.0)
-    rows, row_scales = _block8_workspace(x, places, run, width)
-    place_scale = torch.empty(places, dtype=torch.float32, device=device) if weigh_inputs else None
-    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, x_at, pitch, slots, places, width, run, run, top, _ptr(place_scale), weights_at, code,
-                            stream), "code_rows")
-    hidden = torch.empty((places, ff), dtype=torch.float32, device=device)
-    _check(lib.zb_gemm_block8(hidden.data_ptr(), ff, 0, rows.data_ptr(), row_scales, up_at, up_scales, plan, runs, E, 0, run, run, 2 * ff, width, kind,
-                              None, _ptr(place_scale), *bounds, status, stream), "gemm_block8")
-    rows, row_scales = _block8_workspace(x, places, run, ff)
-    _check(lib.zb_code_rows(rows.data_ptr(), row_scales, hidden.data_ptr(), ff, slots, places, ff, run, run, 0, None, None, 0, stream), "code_rows")
-    y = torch.empty((places, width), dtype=x.dtype, device=device)
-    _check(lib.zb_gemm_block8(y.data_ptr(), width, code, rows.data_ptr(), row_scales, down_at, down_scales, plan, runs, E, 0, run, run, width, ff, 0,
-                              None, None, 0.0, 1.0, 0.0, status, stream), "gemm_block8")
-    _check(lib.zb_route_combine(out_at, y.data_ptr(), width, code, x_at, pitch, ids_at, None if weigh_inputs else weights_at, place_of_slot, T, width,
-                                top, code, stream), "route_combine")
+    code = DTYPE_CODE[x.dtype]
+    work = torch.empty(_block8_experts_work(T, top, E, width, ff, code, weigh_inputs), dtype=torch.uint8, device=x.device)
+    _check(library().zb_block8_experts(_BLOCK8_EXPERTS(
+        out.data_ptr(), x_at, pitch, code, ids_at, weights_at, gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, T, top, E, width, ff, kind,
+        weigh_inputs, *bounds, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "routed_blocks", 6)
     return out
 
 
