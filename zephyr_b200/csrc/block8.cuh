@@ -30,7 +30,16 @@ __host__ __device__ inline long long b8_block_row(int matrix, int nb, int kb, in
 __host__ __device__ inline int b8_pitch(int k) { return b8_blocks(k) * B8_BLOCK; }
 
 // ---- What the files of this form offer one another (host) ----
+constexpr int B8_T0 = 24, B8_T1 = 28, B8_T2 = 32;
 constexpr int G8_PAIRS = 74;           // of SMs: the most that the product for many rows takes
+
+// Whether the pairs share all tiles' blocks of K evenly instead of taking whole tiles: where the rounds of whole tiles leave more of the pairs
+// without work than the parts cost to be handed over (PLACEHOLDER).  In blocks of K on a pair.
+__host__ __device__ inline bool b8_in_parts(long long items, int k_blocks, int cap) {
+  const long long rounds = (items + G8_PAIRS - 1) / G8_PAIRS;
+  const long long whole = rounds * k_blocks, even = (items * k_blocks + G8_PAIRS - 1) / G8_PAIRS;
+  return whole - even > (cap == 64 ? B8_T0 : cap == 128 ? B8_T1 : B8_T2);
+}
 
 struct Block8Product {
   void* y; long long ldy; int y_dtype;
@@ -57,7 +66,7 @@ struct CodeRowsArgs {
 };
 struct Block8Small {
   void* y; long long ldy; int y_dtype;
-  const void* x; long long ldx; int x_dtype;
+  const void* x; const void* x_scales; long long ldx; int x_dtype;
   const void *w_codes, *w_scales;
   int M, N, K, kind;
   const float* bias; float limit, alpha, shift;

@@ -24,18 +24,14 @@ struct Pieces {
   }
 };
 
-// Whether few rows go to the kernel that streams the matrix, and how many others are.  The streaming kernel codes all of x in every CTA and has four
-// warps or sixteen on a tile; the tensor cores' kernel waits for x's codes and for a tile's whole K (8 rows, us, streaming / tensor cores: PLACEHOLDER).
+// Whether few rows go to the kernel that streams the matrix.  It has four warps or sixteen on a tile, the tensor cores' kernel waits for a tile's whole K:
+// up to 8 rows it is ahead or level everywhere (us, streaming / tensor cores: PLACEHOLDER), up to 16, which take twice its instructions, where the matrix is small (PLACEHOLDER).
 constexpr long long STREAM_VALUES = 28LL << 20;
-static bool streams(int M, int N, int K) { return static_cast<long long>(N) * K <= STREAM_VALUES && block8_small_fits(M, K); }
+static bool streams(int M, int N, int K) { return block8_small_fits(M, K) && (M <= 8 || static_cast<long long>(N) * K <= STREAM_VALUES); }
+// Whether its rows are coded by a kernel ahead of it instead of in every CTA for itself (8 rows, us, ahead / in each: K = 1024 4.6 / 4.3, 4096 7.6 / 8.0,
+// 12288 13.3 / 18.5).
+static bool coded_ahead(int M, int K) { return M <= 8 && b8_pieces(K) * M >= 64; }
 
-// Whether the pairs share all tiles' blocks of K evenly instead of taking whole tiles: where the rounds of whole tiles leave more of the pairs
-// without work than the parts cost to be handed over.  In units of a block of K on a pair (PLACEHOLDER us).
-static bool in_parts(long long items, int k_blocks, int cap) {
-  const long long rounds = (items + G8_PAIRS - 1) / G8_PAIRS;
-  const long long whole = rounds * k_blocks, even = (items * k_blocks + G8_PAIRS - 1) / G8_PAIRS;
-  return whole - even > (cap == 64 ? 24 : cap == 128 ? 28 : 32);
-}
 constexpr int LEAST_BLOCKS = 8;
 
 struct Rows {
@@ -62,7 +58,7 @@ static ProductWork product_work(Pieces& memory, int M, int N, int K, bool halves
   w.rows = rows_of(M, halves ? 128 : 256);
   w.halves = halves;
   const long long places = static_cast<long long>(w.rows.runs) * w.rows.cap, items = static_cast<long long>(w.rows.runs) * ((N + 255) / 256);
-  const bool parts = in_parts(items, b8_blocks(K), w.rows.cap);
+  const bool parts = b8_in_parts(items, b8_blocks(K), w.rows.cap);
   w.flags = memory.take<int>(FLAGS);
   w.parts = parts ? memory.take<float>(static_cast<long long>(G8_PAIRS) * 2 * w.rows.cap * 128) : nullptr;
   if (!parts) w.flags = nullptr;
@@ -84,9 +80,19 @@ struct Gate {
 // y [M, N, or N / 2 gated] = x w^T.  `final`: a float32 result is what the caller asked for (hidden values are coded next).
 static int product(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& w, int M, const Gate& g,
                    bool final, int* status, cudaStream_t stream) {
-  if (streams(M, w.N, w.K))
-    return memory.base == nullptr ? OK : block8_small_product({y, ldy, y_dtype, x, ldx, x_dtype, w.codes, w.scales, M, w.N, w.K, g.kind, g.bias, g.limit, g.alpha,
-                                                               g.shift, status}, stream);
+  if (streams(M, w.N, w.K)) {
+    Block8Small s = {y, ldy, y_dtype, x, nullptr, ldx, x_dtype, w.codes, w.scales, M, w.N, w.K, g.kind, g.bias, g.limit, g.alpha, g.shift, status};
+    if (coded_ahead(M, w.K)) {
+      unsigned char* codes = memory.take<unsigned char>(64LL * b8_pitch(w.K));
+      unsigned char* scales = memory.take<unsigned char>(static_cast<long long>(b8_pieces(w.K)) * B8_PIECE);
+      if (memory.base == nullptr) return OK;
+      const int rc = block8_code_rows({codes, scales, x, ldx, nullptr, M, w.K, 64, 64, 0, nullptr, nullptr, nullptr, 0, false}, x_dtype, stream);
+      if (rc != OK) return rc;
+      s.x = codes;
+      s.x_scales = scales;
+    }
+    return memory.base == nullptr ? OK : block8_small_product(s, stream);
+  }
   const ProductWork work = product_work(memory, M, w.N, w.K, final && sums_in_halves(w.K, y_dtype));
   if (memory.base == nullptr) return OK;
   CodeRowsArgs c = {work.codes, work.scales, x, ldx, nullptr, M, w.K, work.rows.run, work.rows.cap, 0, nullptr, nullptr, work.flags,
@@ -194,7 +200,7 @@ ZB_API int zb_block8_product(const void* call) {
                  static_cast<int>(c.M), gate_of(c.kind, c.bias, c.limit, c.alpha, c.shift), true, c.status, static_cast<cudaStream_t>(c.stream));
 }
 // How many kernels the call launches.
-ZB_API int zb_block8_product_kernels(int M, int N, int K) { return streams(M, N, K) ? 1 : 2; }
+ZB_API int zb_block8_product_kernels(int M, int N, int K) { return streams(M, N, K) && !coded_ahead(M, K) ? 1 : 2; }
 
 ZB_API long long zb_block8_feed_forward_work(long long M, long long K, long long ff, long long N, int y_dtype) {
   Pieces memory{nullptr};

@@ -93,17 +93,19 @@ __device__ __forceinline__ Run8 run_of(const Block8Args& a, int i) {
   return {0, i * a.cap, min(a.run, a.M - i * a.run), i * a.run};
 }
 
-// What a pair of CTAs computes.  Without `parts` it takes whole tiles (256 rows of w, run) in turn.  With `parts` all tiles' blocks of K, one tile behind the
+// What a pair of CTAs computes: whole tiles (256 rows of w, run) in turn, or a part of everything: all tiles' blocks of K, one tile behind the
 // other, are cut into equal shares, whatever the tiles' borders: a share is then the end of one tile, whole tiles, and the beginning of another
 // one.  The pair that has a tile's end finishes it; the others leave their sums in `parts` and set their flags.  Each pair walks its share from
 // the back, so that what others wait for comes first and what it waits for itself last.
 struct Share {
-  long long begin, at;          // with `parts`: blocks still to come
+  long long begin, at;          // in parts: blocks still to come
   int item, items, pair, pairs, k_blocks;
+  bool parts;
   __device__ __forceinline__ Share(const Block8Args& a, int runs, int pair_, int pairs_) : pair(pair_), pairs(pairs_), k_blocks(a.k_blocks) {
     items = runs * a.row_blocks;
     item = pair - pairs;
-    if (a.parts != nullptr) {
+    parts = a.parts != nullptr && b8_in_parts(items, k_blocks, a.cap);
+    if (parts) {
       const long long all = static_cast<long long>(items) * k_blocks;
       pairs = static_cast<int>(min(static_cast<long long>(pairs), (all + a.least - 1) / a.least));
       begin = border(pair);
@@ -113,7 +115,7 @@ struct Share {
   __device__ __forceinline__ long long border(int p) const { return static_cast<long long>(items) * k_blocks * min(p, pairs) / pairs; }
   // The next tile and its blocks of K from `first` to before `end`; false: there is none.
   __device__ __forceinline__ bool next(const Block8Args& a, int& tile, int& first, int& end) {
-    if (a.parts == nullptr) {
+    if (!parts) {
       item += pairs;
       tile = item;
       first = 0;
@@ -148,6 +150,11 @@ __device__ __forceinline__ void tc_mma_scaled_pair(unsigned d_tmem, unsigned lon
 // the pair (each from its own shared memory).
 __device__ __forceinline__ void tc_copy_scales_pair(unsigned tmem, unsigned long long desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 // Descriptor of such a piece: no swizzle, groups of eight 16-byte rows 128 bytes apart.
 __device__ __forceinline__ unsigned long long desc_scales(unsigned smem_address) {
@@ -346,7 +353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       // Another pair's or this one's part of a tile: [column][row].
       auto part_of = [&](int p) { return a.parts + (static_cast<size_t>(p) * 2 + rank) * RUN * 128 + 32 * quarter + lane; };
       auto flag_of = [&](int p) { return a.flags + (p * 2 + rank) * 8 + warp - 2; };
-      if (k_end < a.k_blocks) {                       // (only with `parts`) the tile's end is another pair's
+      if (k_end < a.k_blocks) {                       // the tile's end is another pair's
         float* part = part_of(pair);
         for (int c = 32 * (warp > 5); c < run.rows; c += 64) {
           unsigned v[32];
@@ -362,39 +369,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       if (k_end == a.k_blocks && k_first > 0) {
         const long long start = static_cast<long long>(item) * a.k_blocks;
         do ++others; while (share.border(pair - others) > start);
+        // A flag a lane: one look at all of them takes as long as one at one.
         bool ok = true;
-        for (int p = pair - others; p < pair && ok; ++p) {
+        for (int p = pair - others + lane; p < pair && ok; p += 32) {
           int waited = 0;
-          while (*static_cast<volatile int*>(flag_of(p)) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(64);
+          while (load_acquire(flag_of(p)) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(32);
         }
         if (!__all_sync(0xffffffffu, ok)) {
           if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -4);
           sh.failed = 1;
           break;
         }
-        __threadfence();
+        // The others' parts, in the order of K's blocks, are added where the sums are: 16 columns of four pairs on their way at a time.
+        for (int c = 16 * (warp > 5); c < run.rows; c += 32) {
+          unsigned v[16];
+          tmem_ld16(tmem_row + c, v);
+          tmem_wait_ld16(v);
+          for (int p = pair - others; p < pair; p += 4) {
+            float part[4][16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (p + q < pair) {
+                const float* from = part_of(p + q) + c * 128;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[q][i] = __ldcg(from + i * 128);
+              }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (p + q < pair) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + part[q][i]);
+              }
+          }
+          tmem_st16(tmem_row + c, v);
+        }
+        tc_wait_st();
+        tc_fence_before_sync();
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        tc_fence_after_sync();
       }
       for (int c = 32 * (warp > 5); c < run.rows && k_end == a.k_blocks; c += 64) {          // (columns beyond the product's are read and not used)
         unsigned v[32];
         read_sums(c, v);
-        // The others' parts in the order of K's blocks, 16 columns of two pairs on their way at a time.
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (c + 16 * half >= run.rows) break;
-          for (int p = pair - others; p < pair; p += 2) {
-            const float *part = part_of(p) + (c + 16 * half) * 128, *next = p + 1 < pair ? part_of(p + 1) + (c + 16 * half) * 128 : part;
-            float one[16], other[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) one[i] = __ldcg(part + i * 128);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) other[i] = __ldcg(next + i * 128);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float sum = __uint_as_float(v[16 * half + i]) + one[i];
-              v[16 * half + i] = __float_as_uint(p + 1 < pair ? sum + other[i] : sum);
-            }
-          }
-        }
         TOut* mine = staging + (GATED ? (lane >> 4) * 8 + (lane & 7) : lane);
         if (GATED) {
           // Lane l holds the gates, lane l + 8 their ups of 32 rows: the first finishes 16 of them, the second the others.

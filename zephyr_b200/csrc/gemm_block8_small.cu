@@ -31,7 +31,8 @@ constexpr size_t G9_SMEM = 226 * 1024;
 struct Block8SmallArgs {
   CUtensorMap w_map;                         // codes, blocks as rows of 128 bytes; box 128 x 16
   void* y;
-  const void* x;
+  const void* x;                             // the rows as they are, or their codes
+  const unsigned char* x_scales;             // with codes: their scales' pieces
   const unsigned char* scales;
   int* status;
   int M, N, K;
@@ -112,11 +113,12 @@ __device__ __forceinline__ void finish_tile(const Block8SmallArgs& a, int n0, in
   }
 }
 
-template <int MT, int TEAM, typename TOut, bool GATED>
+// CODED: x comes as zb_code_rows leaves it.
+template <int MT, int TEAM, bool CODED, typename TOut, bool GATED>
 __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_small_kernel(const __grid_constant__ Block8SmallArgs a) {
   constexpr int TEAMS = G9_WARPS / TEAM, SUMS = MT * 128;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ unsigned long long bars[G9_WARPS * G9_DEPTH];
+  __shared__ unsigned long long bars[G9_WARPS * G9_DEPTH + 1];
   __shared__ volatile int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = warp / TEAM, slice = warp % TEAM;
   const int g = lane >> 2, t = lane & 3;
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
   };
   if (lane == 0) {
     for (int u = 0; u < G9_DEPTH; ++u) mbar_init(bar + u, 1);
+    if (CODED && warp == 0) mbar_init(bars + G9_WARPS * G9_DEPTH, 1);
     fence_barrier_init();
     for (int u = 0; u < G9_DEPTH; ++u) copy_next(u);
   }
@@ -155,17 +158,40 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
     return tile < tiles && b < b_end ? *(a.scales + (static_cast<size_t>(tile * 16 / B8_BLOCK) * pieces + b / 4) * B8_PIECE + b % 4) : 0u;
   };
   unsigned w_scale = scale_of(first_tile);
+  bool gave_up = false;
   wait_for_prior_grids();
   let_dependents_launch();
   // (Tokens that are not there are columns of the products that nobody reads, whatever lies in their places.)
-  if (a.x_dtype == DTYPE_F32) code_tokens<MT, float>(a, blocks, x_s, x_pitch, x_scale);
-  else code_tokens<MT, __nv_bfloat16>(a, blocks, x_s, x_pitch, x_scale);
-  __syncthreads();
+  // (Tokens that are not there are columns of the products that nobody reads, whatever lies in their places.)
+  if (CODED) {
+    unsigned long long* x_bar = bars + G9_WARPS * G9_DEPTH;
+    if (threadIdx.x == 0) {
+      mbar_arrive_expect_tx(x_bar, static_cast<unsigned>(a.M * blocks * B8_BLOCK));
+      for (int i = 0; i < a.M; ++i)
+        bulk_copy_g2s(x_s + i * x_pitch, static_cast<const unsigned char*>(a.x) + static_cast<size_t>(i) * blocks * B8_BLOCK, blocks * B8_BLOCK, x_bar);
+    }
+    for (int i = threadIdx.x; i < pieces * a.M; i += G9_WARPS * 32) {
+      const int piece = i / a.M, token = i % a.M;
+      const unsigned bytes = *reinterpret_cast<const unsigned*>(a.x_scales + static_cast<size_t>(piece) * B8_PIECE + token * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * piece + j < blocks) x_scale[(4 * piece + j) * (MT * 8) + token] = b8_power(bytes >> (8 * j) & 255u);
+    }
+    __syncthreads();
+    gave_up = !mbar_wait(x_bar, 0, G9_WAIT_LIMIT);
+    if (gave_up) {
+      if (threadIdx.x == 0) report(a.status, STATUS_COPY_TIMEOUT, -1, blockIdx.x);
+      failed = 1;
+    }
+  } else {
+    if (a.x_dtype == DTYPE_F32) code_tokens<MT, float>(a, blocks, x_s, x_pitch, x_scale);
+    else code_tokens<MT, __nv_bfloat16>(a, blocks, x_s, x_pitch, x_scale);
+    __syncthreads();
+  }
 
   auto team_barrier = [&]() { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + team), "n"(TEAM * 32) : "memory"); };
   int slot = 0;
   unsigned phase = 0;
-  bool gave_up = false;
   for (int tile = first_tile, round = 0; tile < tiles; tile += tile_step, ++round) {
     float acc[MT][4];
 #pragma unroll
@@ -245,19 +271,23 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
   if (failed) let_copies_land();
 }
 
-template <int MT, int TEAM, typename TOut, bool GATED>
+template <int MT, int TEAM, bool CODED, typename TOut, bool GATED>
 int block8_small_launch(const Block8SmallArgs& a, cudaStream_t stream) {
-  auto kernel = gemm_block8_small_kernel<MT, TEAM, TOut, GATED>;
+  auto kernel = gemm_block8_small_kernel<MT, TEAM, CODED, TOut, GATED>;
   const size_t smem = block8_small_smem(b8_blocks(a.K), MT);
   if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
   return launch_dependent(kernel, dim3(std::min(148, (a.N + 15) / 16)), dim3(G9_WARPS * 32), smem, stream, false, a);
 }
-// All 16 warps on a tile where no SM has more than one of them and K has blocks enough; else four (8 rows, us, 16 warps / four: 1024 x 2048
-// 4.0 / 4.6, 1024 x 4096 5.2 / 6.2; 4096 x 1024 5.3 / 4.4, 6144 x 4096 10.1 / 9.1).
+// All 16 warps on a tile where no SM has more than two of them and K has blocks enough; else four (8 rows, us, 16 warps / four: 1024 x 2048
+// 4.0 / 4.6, 1024 x 4096 5.2 / 6.2, 4096 x 4096 8.0 / 8.2, 4096 x 12288 13.3 / 15.6; 4096 x 1024 5.3 / 4.4, 6144 x 4096 10.1 / 9.1, 24576 x 4096 22.9 / 21.5).
 template <int MT, typename TOut, bool GATED>
 int block8_small_team(const Block8SmallArgs& a, cudaStream_t stream) {
-  const bool all = (a.N + 15) / 16 <= 148 && b8_blocks(a.K) >= 16;
-  return all || b8_blocks(a.K) > 4 * G9_MAX_BLOCKS ? block8_small_launch<MT, 16, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, TOut, GATED>(a, stream);
+  const bool all = ((a.N + 15) / 16 <= 2 * 148 && b8_blocks(a.K) >= 16) || b8_blocks(a.K) > 4 * G9_MAX_BLOCKS;
+  if constexpr (MT == 1) {                   // (more rows of which the codes would pay have the tensor cores' kernel)
+    if (a.x_scales != nullptr)
+      return all ? block8_small_launch<MT, 16, true, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, true, TOut, GATED>(a, stream);
+  }
+  return all ? block8_small_launch<MT, 16, false, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, false, TOut, GATED>(a, stream);
 }
 template <typename TOut, bool GATED>
 int block8_small_rows(const Block8SmallArgs& a, cudaStream_t stream) {
@@ -268,14 +298,15 @@ bool block8_small_fits(int M, int K) {
   return M >= 1 && M <= 16 && K >= 1 && block8_small_smem(b8_blocks(K), (M + 7) / 8) <= G9_SMEM && b8_blocks(K) <= 16 * G9_MAX_BLOCKS;
 }
 
-// y = x w^T in blocks for up to 16 rows of x as they are (bfloat16 or float32).
+// y = x w^T in blocks for up to 16 rows of x as they are (bfloat16 or float32), or with `x_scales` for up to 8 as codes.
 int block8_small_product(const Block8Small& p, cudaStream_t stream) {
   const bool gated = p.kind >= 1 && p.kind <= 3;
-  if (!block8_small_fits(p.M, p.K) || b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K) >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (!block8_small_fits(p.M, p.K) || (p.x_scales != nullptr && p.M > 8) || b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K) >= (1LL << 31)) return ERR_UNSUPPORTED;
   Block8SmallArgs a = {};
   a.y = p.y; a.ldy = p.ldy; a.x = p.x; a.ldx = p.ldx; a.x_dtype = p.x_dtype;
   if (!byte_rows_map(&a.w_map, p.w_codes, b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K), 128, 128, 16, true)) return ERR_CUDA;
   a.scales = static_cast<const unsigned char*>(p.w_scales);
+  a.x_scales = static_cast<const unsigned char*>(p.x_scales);
   a.M = p.M; a.N = p.N; a.K = p.K; a.status = p.status;
   a.m_inverse = static_cast<unsigned>(((1ULL << 32) + p.M - 1) / p.M);
   a.wide = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % (p.x_dtype == DTYPE_F32 ? 4 : 8) == 0;
