@@ -30,7 +30,7 @@ __host__ __device__ inline long long b8_block_row(int matrix, int nb, int kb, in
 __host__ __device__ inline int b8_pitch(int k) { return b8_blocks(k) * B8_BLOCK; }
 
 // ---- What the files of this form offer one another (host) ----
-constexpr int B8_T0 = 24, B8_T1 = 28, B8_T2 = 32;
+constexpr int B8_T0 = 40, B8_T1 = 60, B8_T2 = 70;
 constexpr int G8_PAIRS = 74;           // of SMs: the most that the product for many rows takes
 
 // Whether the pairs share all tiles' blocks of K evenly instead of taking whole tiles: where the rounds of whole tiles leave more of the pairs
@@ -43,6 +43,7 @@ __host__ __device__ inline bool b8_in_parts(long long items, int k_blocks, int c
 
 struct Block8Product {
   void* y; long long ldy; int y_dtype;
+  void* y_scales;                      // not null: y takes a gated product's results as codes at the runs' places, this their scales
   const void *x_codes, *x_scales, *w_codes, *w_scales;
   const int* plan; int max_runs, matrices;
   int M, run, cap, N, K;               // a run's places begin `cap` (64, 128 or 256) apart

@@ -99,16 +99,41 @@ static int product(Pieces& memory, void* y, long long ldy, int y_dtype, const vo
                     work.flags != nullptr ? static_cast<int>(FLAGS) : 0, false};
   const int rc = block8_code_rows(c, x_dtype, stream);
   if (rc != OK) return rc;
-  return block8_product({y, ldy, y_dtype, work.codes, work.scales, w.codes, w.scales, nullptr, 0, 1, M, work.rows.run, work.rows.cap, w.N, w.K, g.kind, g.bias,
+  return block8_product({y, ldy, y_dtype, nullptr, work.codes, work.scales, w.codes, w.scales, nullptr, 0, 1, M, work.rows.run, work.rows.cap, w.N, w.K, g.kind, g.bias,
                          nullptr, g.limit, g.alpha, g.shift, work.halves, work.parts, work.flags, LEAST_BLOCKS, status}, stream);
 }
 
+// Whether a feed-forward's hidden values go from the first product's kernel to the second's as codes.
+static bool hands_codes_on(int M, const Operand& up, const Operand& down) { return !streams(M, up.N, up.K) && !streams(M, down.N, down.K); }
+
 static int feed_forward(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& up, const Operand& down,
                         int M, const Gate& g, int* status, cudaStream_t stream) {
-  float* hidden = memory.take<float>(static_cast<long long>(M) * down.K);
-  const int rc = product(memory, hidden, down.K, DTYPE_F32, x, ldx, x_dtype, up, M, g, false, status, stream);
+  if (!hands_codes_on(M, up, down)) {
+    float* hidden = memory.take<float>(static_cast<long long>(M) * down.K);
+    const int rc = product(memory, hidden, down.K, DTYPE_F32, x, ldx, x_dtype, up, M, g, false, status, stream);
+    if (rc != OK) return rc;
+    return product(memory, y, ldy, y_dtype, hidden, down.K, DTYPE_F32, down, M, Gate{0, nullptr, 0.0f, 1.0f, 0.0f}, true, status, stream);
+  }
+  const bool halves = sums_in_halves(down.K, y_dtype);
+  const Rows rows = rows_of(M, halves ? 128 : 256);
+  const long long places = static_cast<long long>(rows.runs) * rows.cap, groups = places / rows.cap * ((rows.cap + 127) / 128);
+  int* flags = memory.take<int>(2 * FLAGS);
+  const bool up_parts = b8_in_parts(static_cast<long long>(rows.runs) * ((up.N + 255) / 256), b8_blocks(up.K), rows.cap);
+  const bool down_parts = b8_in_parts(static_cast<long long>(rows.runs) * ((down.N + 255) / 256), b8_blocks(down.K), rows.cap);
+  float* parts = up_parts || down_parts ? memory.take<float>(static_cast<long long>(G8_PAIRS) * 2 * rows.cap * 128) : nullptr;
+  unsigned char* codes = memory.take<unsigned char>(places * b8_pitch(up.K));
+  unsigned char* scales = memory.take<unsigned char>(groups * b8_pieces(up.K) * B8_PIECE);
+  unsigned char* hidden = memory.take<unsigned char>(places * b8_pitch(down.K));
+  unsigned char* hidden_scales = memory.take<unsigned char>(groups * b8_pieces(down.K) * B8_PIECE);
+  if (memory.base == nullptr) return OK;
+  int rc = block8_code_rows({codes, scales, x, ldx, nullptr, M, up.K, rows.run, rows.cap, 0, nullptr, nullptr, flags, parts != nullptr ? static_cast<int>(2 * FLAGS) : 0, false},
+                            x_dtype, stream);
   if (rc != OK) return rc;
-  return product(memory, y, ldy, y_dtype, hidden, down.K, DTYPE_F32, down, M, Gate{0, nullptr, 0.0f, 1.0f, 0.0f}, true, status, stream);
+  rc = block8_product({hidden, up.N / 2, DTYPE_F32, hidden_scales, codes, scales, up.codes, up.scales, nullptr, 0, 1, M, rows.run, rows.cap, up.N, up.K, g.kind, g.bias, nullptr,
+                       g.limit, g.alpha, g.shift, false, up_parts ? parts : nullptr, flags, LEAST_BLOCKS, status}, stream);
+  if (rc != OK) return rc;
+  return block8_product({y, ldy, y_dtype, nullptr, hidden, hidden_scales, down.codes, down.scales, nullptr, 0, 1, M, rows.run, rows.cap, down.N, down.K, 0, nullptr, nullptr, 0.0f,
+                         1.0f, 0.0f, halves, down_parts ? parts : nullptr, flags + FLAGS, LEAST_BLOCKS, status}, stream);
 }
 
 struct Experts {
@@ -121,8 +146,8 @@ struct Experts {
   int T, top, E, width, ff;
   bool weigh_inputs;
 };
-// The rows are coded where they are gathered, the hidden values stay in float32 until they are coded for the second product, an expert's
-// output is rounded to x's type before it is weighted.
+// The rows are coded where they are gathered, the hidden values where the first product's sums are read out, an expert's output is rounded to x's
+// type before it is weighted.
 static int experts(Pieces& memory, const Experts& e, const Operand& up, const Operand& down, const Gate& g, int* status, cudaStream_t stream) {
   const int num_slots = e.T * e.top, cap = zb_gemm_tc_experts_run(num_slots, e.E), runs = num_slots / cap + e.E;
   const long long places = static_cast<long long>(runs) * cap;
@@ -131,28 +156,25 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
   int* slots = memory.take<int>(places);
   int* place_of_slot = memory.take<int>(num_slots);
   float* place_scale = e.weigh_inputs ? memory.take<float>(places) : nullptr;
-  int* flags = memory.take<int>(FLAGS);
+  int* flags = memory.take<int>(2 * FLAGS);
   float* parts = cap <= 128 ? memory.take<float>(static_cast<long long>(G8_PAIRS) * 2 * cap * 128) : nullptr;
   unsigned char* codes = memory.take<unsigned char>(places * b8_pitch(e.width));
   unsigned char* scales = memory.take<unsigned char>(static_cast<long long>(runs) * groups * b8_pieces(e.width) * B8_PIECE);
-  float* hidden = memory.take<float>(places * e.ff);
   unsigned char* hidden_codes = memory.take<unsigned char>(places * b8_pitch(e.ff));
   unsigned char* hidden_scales = memory.take<unsigned char>(static_cast<long long>(runs) * groups * b8_pieces(e.ff) * B8_PIECE);
   char* out = memory.take<char>(places * e.width * (e.dtype == DTYPE_F32 ? 4 : 2));
   if (places >= (1LL << 31)) return ERR_UNSUPPORTED;
   if (memory.base == nullptr) return OK;
-  const int zeros = parts != nullptr ? static_cast<int>(FLAGS) : 0;
+  const int zeros = parts != nullptr ? static_cast<int>(2 * FLAGS) : 0;
   int rc = zb_route_align_strided(plan, slots, place_of_slot, e.ids, num_slots, e.E, runs, cap, static_cast<int>(places), stream);
   if (rc != OK) return rc;
   rc = block8_code_rows({codes, scales, e.x, e.ldx, slots, static_cast<int>(places), e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
   if (rc != OK) return rc;
-  rc = block8_product({hidden, e.ff, DTYPE_F32, codes, scales, up.codes, up.scales, plan, runs, e.E, 0, cap, cap, up.N, up.K, g.kind, nullptr, place_scale, g.limit,
+  rc = block8_product({hidden_codes, e.ff, DTYPE_F32, hidden_scales, codes, scales, up.codes, up.scales, plan, runs, e.E, 0, cap, cap, up.N, up.K, g.kind, nullptr, place_scale, g.limit,
                        g.alpha, g.shift, false, parts, flags, LEAST_BLOCKS, status}, stream);
   if (rc != OK) return rc;
-  rc = block8_code_rows({hidden_codes, hidden_scales, hidden, e.ff, slots, static_cast<int>(places), e.ff, cap, cap, 0, nullptr, nullptr, flags, zeros, false}, DTYPE_F32, stream);
-  if (rc != OK) return rc;
-  rc = block8_product({out, e.width, e.dtype, hidden_codes, hidden_scales, down.codes, down.scales, plan, runs, e.E, 0, cap, cap, down.N, down.K, 0, nullptr, nullptr,
-                       0.0f, 1.0f, 0.0f, false, parts, flags, LEAST_BLOCKS, status}, stream);
+  rc = block8_product({out, e.width, e.dtype, nullptr, hidden_codes, hidden_scales, down.codes, down.scales, plan, runs, e.E, 0, cap, cap, down.N, down.K, 0, nullptr, nullptr,
+                       0.0f, 1.0f, 0.0f, false, parts, flags + FLAGS, LEAST_BLOCKS, status}, stream);
   if (rc != OK) return rc;
   return zb_route_combine(e.y, out, e.width, e.dtype, e.x, e.ldx, e.ids, e.weigh_inputs ? nullptr : e.weights, place_of_slot, e.T, e.width, e.top, e.dtype, stream);
 }
@@ -207,6 +229,11 @@ ZB_API long long zb_block8_feed_forward_work(long long M, long long K, long long
   feed_forward(memory, nullptr, 0, y_dtype, nullptr, 0, 0, {nullptr, nullptr, static_cast<int>(2 * ff), static_cast<int>(K)},
                {nullptr, nullptr, static_cast<int>(N), static_cast<int>(ff)}, static_cast<int>(M), {}, nullptr, nullptr);
   return memory.at;
+}
+// How many kernels the call launches.
+ZB_API int zb_block8_feed_forward_kernels(int M, int K, int ff, int N) {
+  if (hands_codes_on(M, {nullptr, nullptr, 2 * ff, K}, {nullptr, nullptr, N, ff})) return 3;
+  return zb_block8_product_kernels(M, 2 * ff, K) + zb_block8_product_kernels(M, N, ff);
 }
 ZB_API int zb_block8_feed_forward(const void* call) {
   const FeedForwardCall& c = *static_cast<const FeedForwardCall*>(call);

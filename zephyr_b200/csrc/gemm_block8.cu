@@ -54,6 +54,7 @@ struct Block8Args {
   CUtensorMap x_map;             // codes of x; box 128 x RUN / 2
   CUtensorMap x_scale_map;       // its scales; box 128 x 4 or 8: a piece of each of a run's groups
   void* y;
+  unsigned char* y_scales;               // of coded results
   long long ldy;
   int N, row_blocks, scale_groups;       // rows of a matrix, in blocks of 256, in groups of 128
   int k_blocks, pieces, w_groups;        // w_groups: groups of 128 rows of all matrices
@@ -71,7 +72,7 @@ struct Block8Args {
 };
 
 struct Block8Shared {
-  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2];
+  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], merged, peaks[2];
   unsigned tmem_base;
   volatile int failed;
 };
@@ -166,10 +167,11 @@ __device__ __forceinline__ unsigned tc_idesc_scaled_pair(unsigned n) { return ((
 
 
 // GATED: w's rows come in blocks of 8 gates and their 8 ups; y has N / 2 columns.  SCALED: both sums of a place times
-// gate.row_scale[place] first.
+// gate.row_scale[place] first.  TOut = unsigned char (GATED): the results are coded in blocks of 128 as rows of activations are.
 template <int RUN, typename TOut, bool GATED, bool SCALED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_block8_kernel(const __grid_constant__ Block8Args a) {
   using Shape = Block8Shape<RUN>;
+  constexpr bool CODED = sizeof(TOut) == 1;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Block8Shared sh;
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -185,7 +187,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
       mbar_init(&sh.acc_empty[b], 16);               // eight epilogue warps in each CTA
+      mbar_init(&sh.peaks[b], 8);                    // four of them in each CTA
     }
+    mbar_init(&sh.merged, 8);
     sh.failed = 0;
     fence_barrier_init();
   }
@@ -321,12 +325,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     constexpr int OUTPUTS = GATED ? 16 : 32;        // of a warp, a row of x
     constexpr int PER_PIECE = 16 / static_cast<int>(sizeof(TOut)), PIECES = OUTPUTS / PER_PIECE;
     constexpr int PITCH = 144 / static_cast<int>(sizeof(TOut));
+    static_assert(!CODED || GATED, "coded results are a gated product's");
     TOut* staging = reinterpret_cast<TOut*>(scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * G8_STAGING);
     const int width = GATED ? a.N / 2 : a.N;
     const bool holds_gate = (lane & 8) == 0;
     TOut* y = static_cast<TOut*>(a.y);
     int acc = 0;
-    unsigned acc_phase = 0;
+    unsigned acc_phase = 0, merged_phase = 0, peaks_phase = 0;
     while (share.next(a, item, k_first, k_end)) {
       const Run8 run = run_of(a, item % runs);
       const int row = item / runs * 256 + 128 * rank + 32 * quarter + lane, column0 = (row - lane) / (GATED ? 2 : 1);
@@ -350,9 +355,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(more[i]));
         }
       };
+      // Lane l holds the gates, lane l + 8 their ups of 32 rows of x: the first finishes 16 of them, the second the others.
+      auto gate_pairs = [&](int c, const unsigned (&v)[32], auto take) {
+        const float* scale = SCALED ? a.gate.row_scale + run.place + c + (holds_gate ? 0 : 16) : nullptr;
+        auto finish = [&](auto activation) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float own = __uint_as_float(holds_gate ? v[i] : v[16 + i]) + bias;
+            const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(holds_gate ? v[16 + i] : v[i]) + bias, 8);
+            float gate = holds_gate ? own : other, up = holds_gate ? other : own;
+            if (SCALED) {
+              const float s = c + (holds_gate ? 0 : 16) + i < run.rows ? scale[i] : 0.0f;
+              gate *= s;
+              up *= s;
+            }
+            take(i, activation(gate, up));
+          }
+        };
+        if (a.gate.kind == GATE_SILU) finish([](float gate, float up) { return silu_fast(gate) * up; });
+        else if (a.gate.kind == GATE_RELU) finish([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
+        else finish([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
+      };
       // Another pair's or this one's part of a tile: [column][row].
       auto part_of = [&](int p) { return a.parts + (static_cast<size_t>(p) * 2 + rank) * RUN * 128 + 32 * quarter + lane; };
-      auto flag_of = [&](int p) { return a.flags + (p * 2 + rank) * 8 + warp - 2; };
+      auto flag_of = [&](int p, int w) { return a.flags + (p * 2 + rank) * 8 + w; };
       if (k_end < a.k_blocks) {                       // the tile's end is another pair's
         float* part = part_of(pair);
         for (int c = 32 * (warp > 5); c < run.rows; c += 64) {
@@ -363,17 +389,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         }
         __threadfence();
         __syncwarp();
-        if (lane == 0) atomicExch(flag_of(pair), 1);
+        if (lane == 0) atomicExch(flag_of(pair, warp - 2), 1);
       }
       int others = 0;                                 // pairs in front of this one that have blocks of the tile
       if (k_end == a.k_blocks && k_first > 0) {
         const long long start = static_cast<long long>(item) * a.k_blocks;
         do ++others; while (share.border(pair - others) > start);
-        // A flag a lane: one look at all of them takes as long as one at one.
+        // A flag a lane: one look at all of them takes as long as one at one.  Of each pair those of the two warps that have this warp's rows.
         bool ok = true;
-        for (int p = pair - others + lane; p < pair && ok; p += 32) {
+        for (int i = lane; i < 2 * others && ok; i += 32) {
+          const int* flag = flag_of(pair - others + i / 2, (warp - 2) ^ (4 * (i & 1)));
           int waited = 0;
-          while (load_acquire(flag_of(p)) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(32);
+          while (load_acquire(flag) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(32);
         }
         if (!__all_sync(0xffffffffu, ok)) {
           if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -4);
@@ -405,33 +432,117 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         }
         tc_wait_st();
         tc_fence_before_sync();
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc_mbar_arrive(&sh.merged);
+        if (!__all_sync(0xffffffffu, g8_wait(sh, &sh.merged, merged_phase))) {
+          if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -5);
+          sh.failed = 1;
+          break;
+        }
+        merged_phase ^= 1;
         tc_fence_after_sync();
       }
+      if constexpr (CODED) {
+        if (k_end == a.k_blocks) {
+          // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
+          // CTA) gives the scale.  The values wait in registers, and the accumulator is free, while the warps' largest ones go to both CTAs.
+          const int half = warp > 5, turn = peaks_phase & 1;
+          float hidden[RUN / 64][16];
+#pragma unroll
+          for (int j = 0; j < RUN / 64; ++j) {
+            const int c = 64 * j + 32 * half;
+            if (c < run.rows) {
+              unsigned v[32];
+              read_sums(c, v);
+              gate_pairs(c, v, [&](int i, float h) { hidden[j][i] = row < a.N ? h : 0.0f; });
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
+          // [turn][CTA][quarter][row of x]; lane l ends up with row `own` of 32.
+          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + 8 * G8_STAGING) + turn * 8 * RUN;
+          const int own = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
+#pragma unroll
+          for (int j = 0; j < RUN / 64; ++j) {
+            const int c = 64 * j + 32 * half;
+            if (c < run.rows) {
+              unsigned m[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) m[i] = b8_magnitude(hidden[j][i]);
+              auto meet = [&](int bit, int count) {     // with the lane across `bit`: each keeps half of the rows
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (i < count) {
+                    const unsigned keep = lane & bit ? m[count + i] : m[i], give = lane & bit ? m[i] : m[count + i];
+                    m[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, bit));
+                  }
+              };
+              meet(16, 8);
+              meet(4, 4);
+              meet(2, 2);
+              meet(1, 1);
+              unsigned* at = peaks + (rank * 4 + quarter) * RUN + c + own;
+              *at = m[0];
+              asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(in_cta_of_rank(smem_u32(at), rank ^ 1)), "r"(m[0]) : "memory");
+            }
+          }
+          __syncwarp();
+          if (lane < 2) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.peaks[half]), lane));
+          bool ok = false;
+          for (int i = 0; i < G8_WAIT_LIMIT && !ok && !((i & 255) == 255 && sh.failed); ++i) ok = mbar_try_wait_cluster(&sh.peaks[half], peaks_phase);
+          if (!__all_sync(0xffffffffu, ok)) {
+            if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -6);
+            sh.failed = 1;
+            break;
+          }
+          unsigned char* bytes = reinterpret_cast<unsigned char*>(staging);
+          const int block = item / runs, pitch = b8_pitch(a.N / 2), hidden_pieces = b8_pieces(a.N / 2);
+#pragma unroll
+          for (int j = 0; j < RUN / 64; ++j) {
+            const int c = 64 * j + 32 * half;
+            if (c < run.rows) {
+              unsigned largest = 0;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) largest = max(largest, peaks[q * RUN + c + own]);
+              const unsigned byte = b8_scale_byte(largest);
+              const float inverse = b8_inverse(byte);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float one = __shfl_sync(0xffffffffu, inverse, (lane & 8) | (i & 8) << 1 | (i & 7));
+                const float two = __shfl_sync(0xffffffffu, inverse, (lane & 8) | (i & 8) << 1 | (i & 7) + 1);
+                const unsigned codes = b8_codes(hidden[j][i] * one, hidden[j][i + 1] * two, 0.0f, 0.0f, 1.0f);
+                unsigned char* to = bytes + ((lane & 8) * 2 + i) * 16 + (lane >> 4) * 8 + (lane & 7);
+                to[0] = static_cast<unsigned char>(codes);
+                to[16] = static_cast<unsigned char>(codes >> 8);
+              }
+              __syncwarp();
+              if (c + lane < run.rows)
+                *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place + c + lane) * pitch + block * 128 + rank * 64 + quarter * 16) =
+                    *reinterpret_cast<const uint4*>(bytes + lane * 16);
+              if (rank == 0 && quarter == 0 && c + own < run.rows) {
+                const int r = c + own;
+                a.y_scales[((static_cast<size_t>(run.place / a.cap) * hidden_pieces + block / 4) * a.run_groups + r / 128) * B8_PIECE + r % 32 * 16 + r % 128 / 32 * 4 +
+                           block % 4] = static_cast<unsigned char>(byte);
+              }
+              __syncwarp();
+            }
+          }
+          peaks_phase ^= 1;
+          if (++acc == accumulators) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+          continue;
+        }
+      }
+      if constexpr (!CODED) {
       for (int c = 32 * (warp > 5); c < run.rows && k_end == a.k_blocks; c += 64) {          // (columns beyond the product's are read and not used)
         unsigned v[32];
         read_sums(c, v);
         TOut* mine = staging + (GATED ? (lane >> 4) * 8 + (lane & 7) : lane);
         if (GATED) {
-          // Lane l holds the gates, lane l + 8 their ups of 32 rows: the first finishes 16 of them, the second the others.
-          const float* scale = SCALED ? a.gate.row_scale + run.place + c + (holds_gate ? 0 : 16) : nullptr;
-          auto finish = [&](auto activation) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float own = __uint_as_float(holds_gate ? v[i] : v[16 + i]) + bias;
-              const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(holds_gate ? v[16 + i] : v[i]) + bias, 8);
-              float gate = holds_gate ? own : other, up = holds_gate ? other : own;
-              if (SCALED) {
-                const float s = c + (holds_gate ? 0 : 16) + i < run.rows ? scale[i] : 0.0f;
-                gate *= s;
-                up *= s;
-              }
-              mine[((holds_gate ? 0 : 16) + i) * PITCH] = from_float<TOut>(activation(gate, up));
-            }
-          };
-          if (a.gate.kind == GATE_SILU) finish([](float gate, float up) { return silu_fast(gate) * up; });
-          else if (a.gate.kind == GATE_RELU) finish([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
-          else finish([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
+          gate_pairs(c, v, [&](int i, float h) { mine[((holds_gate ? 0 : 16) + i) * PITCH] = from_float<TOut>(h); });
         } else {
           auto finish = [&](auto activation) {
 #pragma unroll
@@ -459,6 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           }
         }
         __syncwarp();
+      }
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -498,7 +610,8 @@ int pairs_at_once(Kernel kernel, int smem, int sms) {
 
 template <int RUN, typename TOut, bool GATED, bool SCALED>
 int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) {
-  using Shape = Block8Shape<RUN>;
+  constexpr int SMEM_BYTES = Block8Shape<RUN>::SMEM_BYTES + (sizeof(TOut) == 1 ? 2 * 8 * RUN * 4 : 0);
+  static_assert(SMEM_BYTES <= 227 * 1024 - 512, "shared memory");
   auto kernel = gemm_block8_kernel<RUN, TOut, GATED, SCALED>;
   static std::atomic<int> known[64];                // by device: asking takes the host 3 us
   int device = 0, sms = 0;
@@ -506,7 +619,7 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
   int pairs = device < 64 ? known[device].load() : 0;
   if (pairs == 0) {
     if (cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
-    pairs = pairs_at_once(kernel, Shape::SMEM_BYTES, sms);
+    pairs = pairs_at_once(kernel, SMEM_BYTES, sms);
     if (pairs <= 0) return ERR_CUDA;
     if (device < 64) known[device].store(pairs);
   }
@@ -515,7 +628,7 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
   // (With `parts` pairs wait for one another: all of them are on the device at once.)
   config.gridDim = dim3(2 * static_cast<unsigned>(a.parts != nullptr || items > pairs ? pairs : items));
   config.blockDim = dim3(G8_THREADS);
-  config.dynamicSmemBytes = Shape::SMEM_BYTES;
+  config.dynamicSmemBytes = SMEM_BYTES;
   config.stream = stream;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -526,7 +639,9 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
 }
 template <int RUN, typename TOut>
 int block8_form(const Block8Args& a, bool gated, long long max_runs, cudaStream_t stream) {
-  if (!gated) return block8_launch<RUN, TOut, false, false>(a, max_runs, stream);
+  if constexpr (sizeof(TOut) > 1) {
+    if (!gated) return block8_launch<RUN, TOut, false, false>(a, max_runs, stream);
+  }
   return a.gate.row_scale != nullptr ? block8_launch<RUN, TOut, true, true>(a, max_runs, stream)
                                      : block8_launch<RUN, TOut, true, false>(a, max_runs, stream);
 }
@@ -542,7 +657,7 @@ int block8_product(const Block8Product& p, cudaStream_t stream) {
   const bool gated = p.kind >= 1 && p.kind <= 3;
   Block8Args a = {};
   const long long runs = p.plan != nullptr ? p.max_runs : (p.M + p.run - 1) / p.run;
-  a.y = p.y; a.ldy = p.ldy; a.N = p.N; a.row_blocks = (p.N + 255) / 256; a.scale_groups = b8_blocks(p.N); a.k_blocks = b8_blocks(p.K); a.pieces = b8_pieces(p.K);
+  a.y = p.y; a.y_scales = static_cast<unsigned char*>(p.y_scales); a.ldy = p.ldy; a.N = p.N; a.row_blocks = (p.N + 255) / 256; a.scale_groups = b8_blocks(p.N); a.k_blocks = b8_blocks(p.K); a.pieces = b8_pieces(p.K);
   a.w_groups = p.matrices * a.scale_groups; a.run_groups = (p.cap + 127) / 128; a.plan = p.plan; a.M = p.M; a.run = p.run; a.cap = p.cap; a.status = p.status;
   a.parts = p.parts; a.flags = p.flags; a.least = p.least; a.halves = p.halves;
   const int per_piece = p.y_dtype == DTYPE_F32 ? 4 : 8;
@@ -557,6 +672,7 @@ int block8_product(const Block8Product& p, cudaStream_t stream) {
       !byte_rows_map(&a.w_scale_map, p.w_scales, scale_rows, 128, 128, 4, false) ||
       !byte_rows_map(&a.x_scale_map, p.x_scales, x_scale_rows, 128, 128, 4 * a.run_groups, false))
     return ERR_CUDA;
+  if (p.y_scales != nullptr) return gated ? block8_run<unsigned char>(a, gated, runs, stream) : ERR_BAD_ARGUMENT;
   return p.y_dtype == DTYPE_F32 ? block8_run<float>(a, gated, runs, stream) : block8_run<__nv_bfloat16>(a, gated, runs, stream);
 }
 

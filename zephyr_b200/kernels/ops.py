@@ -87,7 +87,7 @@ _SIGNATURES = {
     "zb_route_align_strided": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
     "zb_matrix_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
-    "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int],
+    "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int], "zb_block8_feed_forward_kernels": [c_int, c_int, c_int, c_int],
     "zb_gather_places": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "zb_gemm_tc_experts_run": [c_int, c_int],
     "zb_gemm_tc_experts": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int,
@@ -2713,7 +2713,7 @@ def _block8_product_plan(M: int, N: int, K: int, y_code: int) -> tuple[int, int]
 @functools.lru_cache(maxsize=4096)
 def _block8_feed_forward_plan(M: int, K: int, ff: int, N: int, y_code: int) -> tuple[int, int]:
     lib = library()
-    return lib.zb_block8_feed_forward_work(M, K, ff, N, y_code), lib.zb_block8_product_kernels(M, 2 * ff, K) + lib.zb_block8_product_kernels(M, N, ff)
+    return lib.zb_block8_feed_forward_work(M, K, ff, N, y_code), lib.zb_block8_feed_forward_kernels(M, K, ff, N)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2771,7 +2771,8 @@ def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None 
 def block_feed_forward(x: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix, act: str = "silu", bounded: BoundedGate | None = None,
                        out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """down(act(gate x) * up x) on matrices in 8-bit floating point: ``gate_up`` [2 ff, K] in blocks of 8 gate rows and their 8 up rows, ``down`` [N,
-    ff].  The hidden values stay in float32 until they are coded for the second product."""
+    ff].  The hidden values are float32 ones until they are coded for the second product; where both products run on the tensor cores' kernel for many
+    rows the first one codes them."""
     if len(gate_up.shape) != 2 or len(down.shape) != 2 or gate_up.N != 2 * down.K:
         raise InvalidArgumentError(f"gate_up [2 ff, K] and down [N, ff], not {list(gate_up.shape)} and {list(down.shape)}")
     pitch = _check_block8_rows(x, gate_up.K)
@@ -2811,7 +2812,7 @@ def _routed_blocks(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ga
     work = torch.empty(_block8_experts_work(T, top, E, width, ff, code, weigh_inputs), dtype=torch.uint8, device=x.device)
     _check(library().zb_block8_experts(_BLOCK8_EXPERTS(
         out.data_ptr(), x_at, pitch, code, ids_at, weights_at, gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, T, top, E, width, ff, kind,
-        weigh_inputs, *bounds, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "routed_blocks", 6)
+        weigh_inputs, *bounds, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "routed_blocks", 5)
     return out
 
 
