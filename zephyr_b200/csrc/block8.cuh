@@ -105,6 +105,15 @@ __device__ __forceinline__ unsigned b8_codes(float a, float b, float c, float d,
   return static_cast<unsigned>(lo) | (static_cast<unsigned>(hi) << 16);
 }
 
+// Two values of two blocks, likewise.
+__device__ __forceinline__ unsigned b8_two_codes(float a, float a_inverse, float b, float b_inverse) {
+  unsigned short codes;
+  const float nan = __uint_as_float(0x7fffffffu);
+  a = fabsf(a) < __uint_as_float(0x7f800000u) ? a * a_inverse : nan;
+  b = fabsf(b) < __uint_as_float(0x7f800000u) ? b * b_inverse : nan;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(codes) : "f"(b), "f"(a));
+  return codes;
+}
 // The same of values that are all finite.
 __device__ __forceinline__ unsigned b8_codes_finite(float2 ab, float2 cd, float2 inverse) {
   unsigned short lo, hi;

@@ -11,7 +11,7 @@ ZB_API int zb_route_combine(void* out, const void* y, long long y_stride, int y_
 
 namespace zb {
 
-constexpr long long FLAGS = G8_PAIRS * 2 * 8;            // ints
+constexpr long long FLAGS = G8_PAIRS * 2 * 16;           // ints: one a pair, CTA and warp
 
 // Pieces of a call's memory, each from a multiple of 256 bytes on; with a null base only their sizes are added up.
 struct Pieces {

@@ -16,8 +16,8 @@
 //     of w and of all the run's rows;
 //   * warp 1 of the first CTA: every fourth block the copies of the scales into tensor memory (tcgen05.cp, in order with the products), then
 //     four products 256 x run x 32, all by one elected lane;
-//   * warps 2..9: a thread owns a row of w (its TMEM lane) and reads 32 sums of x's rows at a time, every other 32 of them; what a warp has for
-//     32 rows goes through shared memory to wide stores.
+//   * warps 2..9: a thread owns a row of w (its TMEM lane) and reads 32 sums of x's rows at a time, every other 32 of them, all before anything is
+//     stored, so that the accumulator is free for the tile after the next; results go through shared memory to tiled stores.
 // Every wait is bounded and reports instead of hanging; tensor memory is given back on every path.
 #include <atomic>
 
@@ -28,13 +28,13 @@
 
 namespace zb {
 
-constexpr int G8_THREADS = 320;
+constexpr int G8_EPILOGUE_WARPS = 8;       // two for each quarter of a CTA's rows
+constexpr int G8_STAGING = 4096;           // an epilogue warp's 32 rows x 32 results on their way out: float32, or two of bfloat16
+constexpr int G8_THREADS = 64 + 32 * G8_EPILOGUE_WARPS;
 constexpr int G8_WAIT_LIMIT = 1 << 18;
 constexpr int G8_MAX_STAGES = 10;
 constexpr int G8_W_BYTES = 128 * 128;
 constexpr int G8_SCALES = 3 * B8_PIECE;    // of one CTA's rows of w, and of up to 256 rows of x
-constexpr int G8_STAGING = 32 * 144;       // an epilogue warp's 32 rows x 32 outputs, float32, rows 144 bytes apart
-constexpr int G8_SCALE_COLUMN = 256;       // where scales begin in tensor memory; 12 columns a piece of K
 
 // RUN: the longest run of a launch.  A buffer of scales is written again when as many pieces as there are stages have gone by: each piece
 // holds one stage at least, so the products that read it are through (the stage that brings the new one was free), and so is its copy to tensor memory.
@@ -42,16 +42,22 @@ template <int RUN> struct Block8Shape {
   static constexpr int STAGE_BYTES = G8_W_BYTES + RUN / 2 * 128;
   static constexpr int X_SCALES = (RUN + 127) / 128 * B8_PIECE;
   static constexpr int STAGES = RUN == 256 ? 5 : RUN == 128 ? 7 : 8;
-  static constexpr int ACCUMULATORS = RUN == 256 ? 1 : 2;
-  static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + G8_SCALES) + 8 * G8_STAGING + 1024;
-  static_assert(STAGES <= G8_MAX_STAGES && SMEM_BYTES <= 227 * 1024 - 512, "shared memory");
-  static_assert(ACCUMULATORS * RUN <= G8_SCALE_COLUMN && G8_SCALE_COLUMN + 12 * STAGES <= 512, "tensor memory");
+  // Two accumulators.  Beside the scales, 12 columns a piece of K, two of 256 columns have no room: the second one begins 64 columns before the first
+  // one ends, and a tile's products wait until those 64 columns of the tile before have been read, which are read first.
+  static constexpr int SECOND = RUN == 256 ? 192 : RUN;
+  static constexpr int SCALE_COLUMN = RUN == 256 ? 448 : 256;
+  static constexpr int RING_BYTES = STAGES * (STAGE_BYTES + G8_SCALES);
+  // Behind the ring what results pass through: staging, or where they are coded 512 bytes a warp and the largest magnitudes of eight warps' rows, twice.
+  static constexpr int smem_bytes(bool coded) { return RING_BYTES + (coded ? G8_EPILOGUE_WARPS * 512 + 2 * 8 * RUN * 4 : G8_EPILOGUE_WARPS * G8_STAGING) + 1024; }
+  static_assert(STAGES <= G8_MAX_STAGES && smem_bytes(true) <= 227 * 1024 - 512 && smem_bytes(false) <= 227 * 1024 - 512, "shared memory");
+  static_assert(SECOND + RUN <= SCALE_COLUMN && SCALE_COLUMN + 12 * STAGES <= 512, "tensor memory");
 };
 
 struct Block8Args {
   CUtensorMap w_map;             // codes of w, blocks as rows of 128 bytes; box 128 x 128: one block
   CUtensorMap w_scale_map;       // its scales as rows of 128 bytes; box 128 x 4: one piece
   CUtensorMap x_map;             // codes of x; box 128 x RUN / 2
+  CUtensorMap y_map;             // results, 32 columns x 32 rows a copy (`tiled`)
   CUtensorMap x_scale_map;       // its scales; box 128 x 4 or 8: a piece of each of a run's groups
   void* y;
   unsigned char* y_scales;               // of coded results
@@ -65,14 +71,14 @@ struct Block8Args {
   int least;                             // blocks of K a pair takes at least
   float* parts;                          // [pair][CTA][column][128 rows]: sums of a tile that another pair finishes; null: pairs take whole tiles
   int* flags;                            // [pair][CTA][warp], zeros when the kernel starts
-  bool wide;                             // y's rows allow 16-byte stores
+  bool tiled;                            // y's rows allow tiled copies
   int act;
   GateForm gate;
   int* status;
 };
 
 struct Block8Shared {
-  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], merged, peaks[2];
+  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], acc_edge, merged, peaks[2];
   unsigned tmem_base;
   volatile int failed;
 };
@@ -99,7 +105,7 @@ __device__ __forceinline__ Run8 run_of(const Block8Args& a, int i) {
 // one.  The pair that has a tile's end finishes it; the others leave their sums in `parts` and set their flags.  Each pair walks its share from
 // the back, so that what others wait for comes first and what it waits for itself last.
 struct Share {
-  long long begin, at;          // in parts: blocks still to come
+  int begin, at;                // in parts: blocks still to come
   int item, items, pair, pairs, k_blocks;
   bool parts;
   __device__ __forceinline__ Share(const Block8Args& a, int runs, int pair_, int pairs_) : pair(pair_), pairs(pairs_), k_blocks(a.k_blocks) {
@@ -107,13 +113,12 @@ struct Share {
     item = pair - pairs;
     parts = a.parts != nullptr && b8_in_parts(items, k_blocks, a.cap);
     if (parts) {
-      const long long all = static_cast<long long>(items) * k_blocks;
-      pairs = static_cast<int>(min(static_cast<long long>(pairs), (all + a.least - 1) / a.least));
+      pairs = min(pairs, (items * k_blocks + a.least - 1) / a.least);
       begin = border(pair);
       at = border(pair + 1);
     }
   }
-  __device__ __forceinline__ long long border(int p) const { return static_cast<long long>(items) * k_blocks * min(p, pairs) / pairs; }
+  __device__ __forceinline__ int border(int p) const { return static_cast<int>(static_cast<long long>(items) * k_blocks * min(p, pairs) / pairs); }
   // The next tile and its blocks of K from `first` to before `end`; false: there is none.
   __device__ __forceinline__ bool next(const Block8Args& a, int& tile, int& first, int& end) {
     if (!parts) {
@@ -124,11 +129,11 @@ struct Share {
       return item < items;
     }
     if (at <= begin) return false;
-    tile = static_cast<int>((at - 1) / k_blocks);
-    const long long start = static_cast<long long>(tile) * k_blocks;
-    end = static_cast<int>(at - start);
+    tile = (at - 1) / k_blocks;
+    const int start = tile * k_blocks;
+    end = at - start;
     at = max(begin, start);
-    first = static_cast<int>(at - start);
+    first = at - start;
     return true;
   }
 };
@@ -139,6 +144,15 @@ __device__ __forceinline__ int w_group_of(const Block8Args& a, int matrix, int b
 }
 // Does the stage of block `kb` bring the scales of its piece of K?
 __device__ __forceinline__ bool brings_scales(int kb, int first) { return kb % 4 == 0 || kb == first; }
+
+// One box from shared memory to the matrix behind `map` at (x, y), part of the thread's current bulk group.
+__device__ __forceinline__ void tiled_store_2d_s2g(const CUtensorMap* map, int x, int y, const void* smem_src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+               ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(smem_src)) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
 // One scaled product of 256 x N x 32: D (+)= A B, each operand's sums times the powers of two in tensor memory at `a_scales` and `b_scales`.
 __device__ __forceinline__ void tc_mma_scaled_pair(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc,
@@ -186,10 +200,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
-      mbar_init(&sh.acc_empty[b], 16);               // eight epilogue warps in each CTA
-      mbar_init(&sh.peaks[b], 8);                    // four of them in each CTA
+      mbar_init(&sh.acc_empty[b], 2 * G8_EPILOGUE_WARPS);      // of both CTAs
     }
-    mbar_init(&sh.merged, 8);
+    for (int g = 0; g < 2; ++g) mbar_init(&sh.peaks[g], 8);     // four warps of each CTA
+    mbar_init(&sh.acc_edge, 2 * G8_EPILOGUE_WARPS);
+    mbar_init(&sh.merged, G8_EPILOGUE_WARPS);
     sh.failed = 0;
     fence_barrier_init();
   }
@@ -221,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
   const int runs = runs_of(a);
   Share share(a, runs, pair, pairs);
   int item, k_first, k_end;
-  const int accumulators = a.halves ? 1 : Shape::ACCUMULATORS;
+  const int accumulators = a.halves ? 1 : 2;
   // The product's columns: a run's rows up to a multiple of 64, half of them in each CTA.
   auto half_columns = [](int rows) { return (rows + 63) / 64 * 32; };
 
@@ -270,13 +285,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
   } else if (warp == 1 && rank == 0) {
     const bool leader = elect_one();
     int stage = 0, acc = 0, scales = 0;
-    unsigned phase = 0, acc_phase = 0;
+    unsigned phase = 0, acc_phase = 0, edge_phase = 1;
     while (share.next(a, item, k_first, k_end)) {
       const unsigned columns = 2 * half_columns(run_of(a, item % runs).rows), idesc = tc_idesc_scaled_pair(columns);
       bool ok = __all_sync(0xffffffffu, g8_wait(sh, &sh.acc_empty[acc], acc_phase ^ 1));
+      if (RUN == 256) ok = ok && __all_sync(0xffffffffu, g8_wait(sh, &sh.acc_edge, edge_phase));
+      edge_phase ^= 1;
       if (!ok && leader && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -1);
       tc_fence_after_sync();
-      unsigned d = tmem_base + acc * RUN, scale_at = 0;
+      unsigned d = tmem_base + acc * Shape::SECOND, scale_at = 0;
       const int middle = a.halves ? (k_first + k_end) / 2 : k_first;
       if (a.halves) d = tmem_base;
       for (int kb = k_first; kb < k_end && ok; ++kb) {
@@ -289,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         const unsigned slot = smem_u32(ring + stage * Shape::STAGE_BYTES);
         const unsigned long long w_desc = desc_k_major(slot), x_desc = desc_k_major(slot + G8_W_BYTES);
         if (brings_scales(kb, k_first)) {
-          scale_at = tmem_base + G8_SCALE_COLUMN + 12 * scales;
+          scale_at = tmem_base + Shape::SCALE_COLUMN + 12 * scales;
           if (leader) {
             const unsigned from = smem_u32(scale_ring + scales * G8_SCALES);
             tc_copy_scales_pair(scale_at, desc_scales(from));
@@ -322,15 +339,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     }
   } else if (warp > 1) {
     const int quarter = warp & 3;                   // the TMEM lanes this warp may read: 32 quarter .. + 31
-    constexpr int OUTPUTS = GATED ? 16 : 32;        // of a warp, a row of x
-    constexpr int PER_PIECE = 16 / static_cast<int>(sizeof(TOut)), PIECES = OUTPUTS / PER_PIECE;
-    constexpr int PITCH = 144 / static_cast<int>(sizeof(TOut));
-    static_assert(!CODED || GATED, "coded results are a gated product's");
-    TOut* staging = reinterpret_cast<TOut*>(scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * G8_STAGING);
+    const int group = (warp - 2) >> 2;              // and of every 64 columns (rows of x) it takes 32 group .. + 31
+    constexpr int CHUNKS = RUN / 64;
     const int width = GATED ? a.N / 2 : a.N;
     const bool holds_gate = (lane & 8) == 0;
-    TOut* y = static_cast<TOut*>(a.y);
-    int acc = 0;
+    unsigned char* staging = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * G8_STAGING;
+    int acc = 0, stores = 0;
     unsigned acc_phase = 0, merged_phase = 0, peaks_phase = 0;
     while (share.next(a, item, k_first, k_end)) {
       const Run8 run = run_of(a, item % runs);
@@ -342,46 +356,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         break;
       }
       tc_fence_after_sync();
-      const unsigned tmem_row = tmem_base + (static_cast<unsigned>(32 * quarter) << 16) + acc * RUN;
+      const unsigned tmem_row = tmem_base + (static_cast<unsigned>(32 * quarter) << 16) + acc * Shape::SECOND;
       const bool two = a.halves && (k_first + k_end) / 2 != k_first;
       auto read_sums = [&](int c, unsigned (&v)[32]) {
         tmem_ld32(tmem_row + c, v);
         tmem_wait_ld32(v);
         if (RUN <= 128 && two) {
-          unsigned more[32];
-          tmem_ld32(tmem_row + RUN + c, more);
-          tmem_wait_ld32(more);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(more[i]));
+          for (int h = 0; h < 4; ++h) {
+            unsigned more[8];
+            tmem_ld8(tmem_row + RUN + c + 8 * h, more);
+            tmem_wait_ld8(more);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[8 * h + i] = __float_as_uint(__uint_as_float(v[8 * h + i]) + __uint_as_float(more[i]));
+          }
         }
       };
-      // Lane l holds the gates, lane l + 8 their ups of 32 rows of x: the first finishes 16 of them, the second the others.
-      auto gate_pairs = [&](int c, const unsigned (&v)[32], auto take) {
-        const float* scale = SCALED ? a.gate.row_scale + run.place + c + (holds_gate ? 0 : 16) : nullptr;
-        auto finish = [&](auto activation) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float own = __uint_as_float(holds_gate ? v[i] : v[16 + i]) + bias;
-            const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(holds_gate ? v[16 + i] : v[i]) + bias, 8);
-            float gate = holds_gate ? own : other, up = holds_gate ? other : own;
-            if (SCALED) {
-              const float s = c + (holds_gate ? 0 : 16) + i < run.rows ? scale[i] : 0.0f;
-              gate *= s;
-              up *= s;
-            }
-            take(i, activation(gate, up));
-          }
-        };
-        if (a.gate.kind == GATE_SILU) finish([](float gate, float up) { return silu_fast(gate) * up; });
-        else if (a.gate.kind == GATE_RELU) finish([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
-        else finish([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
+      // The columns that the two accumulators of 256 share have been read: the last 64 of the first one, the first 64 of the second.
+      auto free_edge = [&]() {
+        if (RUN == 256) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_edge), 0));
+        }
+      };
+      // A warp's chunks of 32 columns, the first and the last one first.
+      auto chunk = [](int s) { return s == 0 ? 0 : s == 1 ? CHUNKS - 1 : s - 1; };
+      constexpr int EDGE = CHUNKS > 1 ? 1 : 0;      // behind which the edge is free
+      auto free_accumulator = [&]() {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
+        if (++acc == accumulators) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
       };
       // Another pair's or this one's part of a tile: [column][row].
       auto part_of = [&](int p) { return a.parts + (static_cast<size_t>(p) * 2 + rank) * RUN * 128 + 32 * quarter + lane; };
-      auto flag_of = [&](int p, int w) { return a.flags + (p * 2 + rank) * 8 + w; };
+      auto flag_of = [&](int p, int g) { return a.flags + (p * 2 + rank) * G8_EPILOGUE_WARPS + 4 * g + quarter; };
       if (k_end < a.k_blocks) {                       // the tile's end is another pair's
         float* part = part_of(pair);
-        for (int c = 32 * (warp > 5); c < run.rows; c += 64) {
+        for (int c = 32 * group; c < run.rows; c += 64) {
           unsigned v[32];
           read_sums(c, v);
 #pragma unroll
@@ -389,16 +405,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         }
         __threadfence();
         __syncwarp();
-        if (lane == 0) atomicExch(flag_of(pair, warp - 2), 1);
+        if (lane == 0) atomicExch(flag_of(pair, group), 1);
+        free_edge();
+        free_accumulator();
+        continue;
       }
-      int others = 0;                                 // pairs in front of this one that have blocks of the tile
-      if (k_end == a.k_blocks && k_first > 0) {
-        const long long start = static_cast<long long>(item) * a.k_blocks;
+      if (k_first > 0) {
+        int others = 0;                               // pairs in front of this one that have blocks of the tile
+        const int start = item * a.k_blocks;
         do ++others; while (share.border(pair - others) > start);
         // A flag a lane: one look at all of them takes as long as one at one.  Of each pair those of the two warps that have this warp's rows.
         bool ok = true;
         for (int i = lane; i < 2 * others && ok; i += 32) {
-          const int* flag = flag_of(pair - others + i / 2, (warp - 2) ^ (4 * (i & 1)));
+          const int* flag = flag_of(pair - others + i / 2, i % 2);
           int waited = 0;
           while (load_acquire(flag) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(32);
         }
@@ -408,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           break;
         }
         // The others' parts, in the order of K's blocks, are added where the sums are: 16 columns of four pairs on their way at a time.
-        for (int c = 16 * (warp > 5); c < run.rows; c += 32) {
+        for (int c = 16 * group; c < run.rows; c += 32) {
           unsigned v[16];
           tmem_ld16(tmem_row + c, v);
           tmem_wait_ld16(v);
@@ -442,30 +461,125 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         merged_phase ^= 1;
         tc_fence_after_sync();
       }
-      if constexpr (CODED) {
-        if (k_end == a.k_blocks) {
-          // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
-          // CTA) gives the scale.  The values wait in registers, and the accumulator is free, while the warps' largest ones go to both CTAs.
-          const int half = warp > 5, turn = peaks_phase & 1;
-          float hidden[RUN / 64][16];
+      // (Columns beyond the run's rows are read and not used.)
+      if constexpr (!GATED) {
+        // bfloat16: words of two columns of x's rows 2 i (an even lane's, of its own column and its neighbour's) and 2 i + 1 (the odd one's).
+        constexpr int WORDS = sizeof(TOut) == 2 ? 16 : 32;
+        unsigned out[CHUNKS][WORDS];
+        auto take = [&](auto activation) {
 #pragma unroll
-          for (int j = 0; j < RUN / 64; ++j) {
-            const int c = 64 * j + 32 * half;
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int j = chunk(s), c = 64 * j + 32 * group;
             if (c < run.rows) {
               unsigned v[32];
               read_sums(c, v);
-              gate_pairs(c, v, [&](int i, float h) { hidden[j][i] = row < a.N ? h : 0.0f; });
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(TOut) == 2) {
+                  const float one = activation(__uint_as_float(v[2 * i])), other = activation(__uint_as_float(v[2 * i + 1]));
+                  const float met = __shfl_xor_sync(0xffffffffu, lane & 1 ? one : other, 1);
+                  out[j][i] = lane & 1 ? pack_bf16(met, other) : pack_bf16(one, met);
+                } else {
+                  out[j][i] = __float_as_uint(activation(__uint_as_float(v[i])));
+                }
+              }
+            }
+            if (s == EDGE) free_edge();
+          }
+        };
+        if (a.act == ACT_NONE) take([](float z) { return z; });
+        else if (a.act == ACT_GELU) take([](float z) { return gelu_tanh_fast(z); });
+        else take([](float z) { return relu_squared(z); });
+        free_accumulator();
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) {
+          const int c = 64 * j + 32 * group, rows = run.rows - c;
+          if (rows <= 0) continue;
+          // A run's last rows may be followed by another run's (without a plan): those go out one by one.
+          if (a.tiled && (rows >= 32 || a.plan != nullptr || run.out + run.rows == a.M)) {
+            unsigned char* buffer = staging + (sizeof(TOut) == 2 ? (stores & 1) * 2048 : 0);
+            if (lane == 0) {
+              if (sizeof(TOut) == 2) bulk_wait_read<1>();
+              else bulk_wait_read<0>();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+              if constexpr (sizeof(TOut) == 2) *reinterpret_cast<unsigned*>(buffer + (2 * i + (lane & 1)) * 64 + (lane & ~1) * 2) = out[j][i];
+              else *reinterpret_cast<unsigned*>(buffer + i * 128 + lane * 4) = out[j][i];
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              if (column0 < a.N) tiled_store_2d_s2g(&a.y_map, column0, run.out + c, buffer);
+              bulk_commit();
+            }
+            ++stores;
+          } else {
+            const int pair_row = lane & 1, column = row & ~1;
+            TOut* at = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + c) * a.ldy;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+              if constexpr (sizeof(TOut) == 2) {
+                unsigned short* bits = reinterpret_cast<unsigned short*>(at) + static_cast<size_t>(2 * i + pair_row) * a.ldy + column;
+                if (2 * i + pair_row < rows && column < a.N) bits[0] = static_cast<unsigned short>(out[j][i]);
+                if (2 * i + pair_row < rows && column + 1 < a.N) bits[1] = static_cast<unsigned short>(out[j][i] >> 16);
+              } else {
+                if (i < rows && row < a.N) at[static_cast<size_t>(i) * a.ldy + row] = __uint_as_float(out[j][i]);
+              }
             }
           }
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
-          // [turn][CTA][quarter][row of x]; lane l ends up with row `own` of 32.
-          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + 8 * G8_STAGING) + turn * 8 * RUN;
-          const int own = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
+        }
+      } else {
+        // Lane l holds the gates, lane l + 8 their ups of 32 rows of x: the first finishes 16 of them, the second the others.
+        const int own_row = holds_gate ? 0 : 16, own_column = (lane >> 4) * 8 + (lane & 7);
+        float hidden[CHUNKS][16];
+        auto gate_pairs = [&](auto activation) {
 #pragma unroll
-          for (int j = 0; j < RUN / 64; ++j) {
-            const int c = 64 * j + 32 * half;
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int j = chunk(s), c = 64 * j + 32 * group;
+            if (c < run.rows) {
+              unsigned v[32];
+              read_sums(c, v);
+              const float* scale = SCALED ? a.gate.row_scale + run.place + c + own_row : nullptr;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float own = __uint_as_float(holds_gate ? v[i] : v[16 + i]) + bias;
+                const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(holds_gate ? v[16 + i] : v[i]) + bias, 8);
+                float gate = holds_gate ? own : other, up = holds_gate ? other : own;
+                if (SCALED) {
+                  const float s = c + own_row + i < run.rows ? scale[i] : 0.0f;
+                  gate *= s;
+                  up *= s;
+                }
+                hidden[j][i] = row < a.N ? activation(gate, up) : 0.0f;
+              }
+            }
+            if (s == EDGE) free_edge();
+          }
+        };
+        if (a.gate.kind == GATE_SILU) gate_pairs([](float gate, float up) { return silu_fast(gate) * up; });
+        else if (a.gate.kind == GATE_RELU) gate_pairs([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
+        else gate_pairs([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
+        free_accumulator();
+        if constexpr (!CODED) {
+          TOut* y = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + own_row) * a.ldy + column0 + own_column;
+#pragma unroll
+          for (int j = 0; j < CHUNKS; ++j) {
+            const int c = 64 * j + 32 * group;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (c + own_row + i < run.rows && column0 + own_column < width) y[static_cast<size_t>(c + i) * a.ldy] = from_float<TOut>(hidden[j][i]);
+          }
+        } else {
+          // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
+          // CTA) gives the scale.  [turn][CTA][quarter][row of x], in both CTAs; lane l finds and hands over row `mine` of 32.
+          unsigned char* bytes = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * 512;
+          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + G8_EPILOGUE_WARPS * 512) + peaks_phase * 8 * RUN;
+          const int mine = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
+#pragma unroll
+          for (int j = 0; j < CHUNKS; ++j) {
+            const int c = 64 * j + 32 * group;
             if (c < run.rows) {
               unsigned m[16];
 #pragma unroll
@@ -482,104 +596,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
               meet(4, 4);
               meet(2, 2);
               meet(1, 1);
-              unsigned* at = peaks + (rank * 4 + quarter) * RUN + c + own;
+              unsigned* at = peaks + (rank * 4 + quarter) * RUN + c + mine;
               *at = m[0];
               asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(in_cta_of_rank(smem_u32(at), rank ^ 1)), "r"(m[0]) : "memory");
             }
           }
           __syncwarp();
-          if (lane < 2) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.peaks[half]), lane));
+          if (lane < 2) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.peaks[group]), lane));
           bool ok = false;
-          for (int i = 0; i < G8_WAIT_LIMIT && !ok && !((i & 255) == 255 && sh.failed); ++i) ok = mbar_try_wait_cluster(&sh.peaks[half], peaks_phase);
+          for (int i = 0; i < G8_WAIT_LIMIT && !ok && !((i & 255) == 255 && sh.failed); ++i) ok = mbar_try_wait_cluster(&sh.peaks[group], peaks_phase);
           if (!__all_sync(0xffffffffu, ok)) {
             if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -6);
             sh.failed = 1;
             break;
           }
-          unsigned char* bytes = reinterpret_cast<unsigned char*>(staging);
-          const int block = item / runs, pitch = b8_pitch(a.N / 2), hidden_pieces = b8_pieces(a.N / 2);
+          peaks_phase ^= 1;
+          const int block = item / runs, pitch = b8_pitch(width), hidden_pieces = b8_pieces(width);
+          unsigned char* codes_at = static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place) * pitch + block * 128 + rank * 64 + quarter * 16;
 #pragma unroll
-          for (int j = 0; j < RUN / 64; ++j) {
-            const int c = 64 * j + 32 * half;
+          for (int j = 0; j < CHUNKS; ++j) {
+            const int c = 64 * j + 32 * group;
             if (c < run.rows) {
               unsigned largest = 0;
 #pragma unroll
-              for (int q = 0; q < 8; ++q) largest = max(largest, peaks[q * RUN + c + own]);
+              for (int q = 0; q < 8; ++q) largest = max(largest, peaks[q * RUN + c + mine]);
               const unsigned byte = b8_scale_byte(largest);
               const float inverse = b8_inverse(byte);
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
-                const float one = __shfl_sync(0xffffffffu, inverse, (lane & 8) | (i & 8) << 1 | (i & 7));
-                const float two = __shfl_sync(0xffffffffu, inverse, (lane & 8) | (i & 8) << 1 | (i & 7) + 1);
-                const unsigned codes = b8_codes(hidden[j][i] * one, hidden[j][i + 1] * two, 0.0f, 0.0f, 1.0f);
-                unsigned char* to = bytes + ((lane & 8) * 2 + i) * 16 + (lane >> 4) * 8 + (lane & 7);
+                const int from = (lane & 8) | (i & 8) << 1 | (i & 7);
+                const float one = __shfl_sync(0xffffffffu, inverse, from), two = __shfl_sync(0xffffffffu, inverse, from + 1);
+                const unsigned codes = b8_two_codes(hidden[j][i], one, hidden[j][i + 1], two);
+                unsigned char* to = bytes + (own_row + i) * 16 + own_column;
                 to[0] = static_cast<unsigned char>(codes);
                 to[16] = static_cast<unsigned char>(codes >> 8);
               }
               __syncwarp();
-              if (c + lane < run.rows)
-                *reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place + c + lane) * pitch + block * 128 + rank * 64 + quarter * 16) =
-                    *reinterpret_cast<const uint4*>(bytes + lane * 16);
-              if (rank == 0 && quarter == 0 && c + own < run.rows) {
-                const int r = c + own;
+              if (c + lane < run.rows) *reinterpret_cast<uint4*>(codes_at + static_cast<size_t>(c + lane) * pitch) = *reinterpret_cast<const uint4*>(bytes + lane * 16);
+              if (rank == 0 && quarter == 0 && c + mine < run.rows) {
+                const int r = c + mine;
                 a.y_scales[((static_cast<size_t>(run.place / a.cap) * hidden_pieces + block / 4) * a.run_groups + r / 128) * B8_PIECE + r % 32 * 16 + r % 128 / 32 * 4 +
                            block % 4] = static_cast<unsigned char>(byte);
               }
               __syncwarp();
             }
           }
-          peaks_phase ^= 1;
-          if (++acc == accumulators) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
-          continue;
         }
-      }
-      if constexpr (!CODED) {
-      for (int c = 32 * (warp > 5); c < run.rows && k_end == a.k_blocks; c += 64) {          // (columns beyond the product's are read and not used)
-        unsigned v[32];
-        read_sums(c, v);
-        TOut* mine = staging + (GATED ? (lane >> 4) * 8 + (lane & 7) : lane);
-        if (GATED) {
-          gate_pairs(c, v, [&](int i, float h) { mine[((holds_gate ? 0 : 16) + i) * PITCH] = from_float<TOut>(h); });
-        } else {
-          auto finish = [&](auto activation) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mine[i * PITCH] = from_float<TOut>(activation(__uint_as_float(v[i])));
-          };
-          if (a.act == ACT_NONE) finish([](float z) { return z; });
-          else if (a.act == ACT_GELU) finish([](float z) { return gelu_tanh_fast(z); });
-          else finish([](float z) { return relu_squared(z); });
-        }
-        __syncwarp();
-        if (a.wide) {
-#pragma unroll
-          for (int i = 0; i < PIECES; ++i) {
-            const int token = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
-            if (c + token < run.rows && column0 + piece * PER_PIECE < width)
-              *reinterpret_cast<uint4*>(y + static_cast<size_t>(run.out + c + token) * a.ldy + column0 + piece * PER_PIECE) =
-                  *reinterpret_cast<const uint4*>(staging + token * PITCH + piece * PER_PIECE);
-          }
-        } else {
-#pragma unroll 4
-          for (int i = 0; i < OUTPUTS; ++i) {
-            const int token = i * (32 / OUTPUTS) + lane / OUTPUTS, column = lane % OUTPUTS;
-            if (c + token < run.rows && column0 + column < width)
-              y[static_cast<size_t>(run.out + c + token) * a.ldy + column0 + column] = staging[token * PITCH + column];
-          }
-        }
-        __syncwarp();
-      }
-      }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
-      if (++acc == accumulators) {
-        acc = 0;
-        acc_phase ^= 1;
       }
     }
+    if (!GATED && lane == 0) bulk_wait_all();       // the staging buffers are read, the rows written
   }
 
   // Both CTAs meet here on every path (the other's barriers and tensor memory are used until then), and the warps that took the
@@ -610,8 +675,7 @@ int pairs_at_once(Kernel kernel, int smem, int sms) {
 
 template <int RUN, typename TOut, bool GATED, bool SCALED>
 int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) {
-  constexpr int SMEM_BYTES = Block8Shape<RUN>::SMEM_BYTES + (sizeof(TOut) == 1 ? 2 * 8 * RUN * 4 : 0);
-  static_assert(SMEM_BYTES <= 227 * 1024 - 512, "shared memory");
+  constexpr int SMEM_BYTES = Block8Shape<RUN>::smem_bytes(sizeof(TOut) == 1);
   auto kernel = gemm_block8_kernel<RUN, TOut, GATED, SCALED>;
   static std::atomic<int> known[64];                // by device: asking takes the host 3 us
   int device = 0, sms = 0;
@@ -651,6 +715,17 @@ int block8_run(const Block8Args& a, bool gated, long long max_runs, cudaStream_t
          : a.cap == 128 ? block8_form<128, TOut>(a, gated, max_runs, stream) : block8_form<256, TOut>(a, gated, max_runs, stream);
 }
 
+// Results [rows][N], `ldy` elements between rows, in boxes of 32 x 32.
+static bool result_map(CUtensorMap* out, void* y, long long rows, int N, long long ldy, int element) {
+  const EncodeTiled encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldy) * element};
+  const cuuint32_t box[2] = {32, 32}, element_strides[2] = {1, 1};
+  return encode(out, element == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, y, dims, strides, box, element_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The operands and results of a product (block8.cuh): y = x w^T in blocks.  Without `plan` M rows of x in runs of `run`, one matrix, y [M]; with it
 // (zb_route_align_strided) `max_runs` runs at most of `matrices`, y by place.
 int block8_product(const Block8Product& p, cudaStream_t stream) {
@@ -660,18 +735,19 @@ int block8_product(const Block8Product& p, cudaStream_t stream) {
   a.y = p.y; a.y_scales = static_cast<unsigned char*>(p.y_scales); a.ldy = p.ldy; a.N = p.N; a.row_blocks = (p.N + 255) / 256; a.scale_groups = b8_blocks(p.N); a.k_blocks = b8_blocks(p.K); a.pieces = b8_pieces(p.K);
   a.w_groups = p.matrices * a.scale_groups; a.run_groups = (p.cap + 127) / 128; a.plan = p.plan; a.M = p.M; a.run = p.run; a.cap = p.cap; a.status = p.status;
   a.parts = p.parts; a.flags = p.flags; a.least = p.least; a.halves = p.halves;
-  const int per_piece = p.y_dtype == DTYPE_F32 ? 4 : 8;
-  a.wide = p.ldy % per_piece == 0 && (gated ? p.N / 2 : p.N) % per_piece == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
   a.act = p.kind == 4 ? ACT_GELU : p.kind == 5 ? ACT_RELU2 : ACT_NONE;
   a.gate = p.kind == 3 ? GateForm{GATE_BOUNDED, p.bias, p.limit, p.alpha, p.shift, nullptr} : plain_gate(p.kind == 2 ? GATE_RELU : GATE_SILU);
   a.gate.row_scale = p.row_scale;
   const long long pitch = b8_pitch(p.K), w_rows = static_cast<long long>(a.w_groups) * a.k_blocks * 128;
   const long long scale_rows = static_cast<long long>(a.w_groups) * a.pieces * 4, x_scale_rows = runs * a.run_groups * a.pieces * 4;
-  if (w_rows >= (1LL << 31) || runs * p.cap >= (1LL << 31) || x_scale_rows >= (1LL << 31) || runs * a.row_blocks >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (w_rows >= (1LL << 31) || runs * p.cap >= (1LL << 31) || x_scale_rows >= (1LL << 31) || runs * a.row_blocks * a.k_blocks >= (1LL << 31)) return ERR_UNSUPPORTED;
   if (!byte_rows_map(&a.w_map, p.w_codes, w_rows, 128, 128, 128, true) || !byte_rows_map(&a.x_map, p.x_codes, runs * p.cap, pitch, pitch, p.cap / 2, true) ||
       !byte_rows_map(&a.w_scale_map, p.w_scales, scale_rows, 128, 128, 4, false) ||
       !byte_rows_map(&a.x_scale_map, p.x_scales, x_scale_rows, 128, 128, 4 * a.run_groups, false))
     return ERR_CUDA;
+  const int element = p.y_dtype == DTYPE_F32 ? 4 : 2;
+  a.tiled = !gated && p.ldy * element % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  if (a.tiled && !result_map(&a.y_map, p.y, p.plan != nullptr ? runs * p.cap : p.M, p.N, p.ldy, element)) return ERR_CUDA;
   if (p.y_scales != nullptr) return gated ? block8_run<unsigned char>(a, gated, runs, stream) : ERR_BAD_ARGUMENT;
   return p.y_dtype == DTYPE_F32 ? block8_run<float>(a, gated, runs, stream) : block8_run<__nv_bfloat16>(a, gated, runs, stream);
 }
