@@ -149,9 +149,9 @@ matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* sc
 }
 
 // Rows of activations into codes: a warp takes 512 values of a row, 16 a lane.  Where a row goes, and what it is:
-//   * without `slots`, row m goes to place m / run * cap + m % run: the rows of a run of the product lie together, at its start;
-//   * with `slots`, place p gets row slots[p] / top of x (row p with `top` 0), or stays as it was where slots[p] < 0; with `place_scale` also
-//     the slot's weight (zero where there is none).
+//   * without `place_of_slot`, row m goes to place m / run * cap + m % run: the rows of a run of the product lie together, at its start;
+//   * with `place_of_slot`, row s / top goes to place_of_slot[s], or nowhere where that is negative; with `place_scale` the place also gets the
+//     slot's weight.
 // The scales of a run's places: [run][piece][group of 128 places].
 template <typename T>
 __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
@@ -161,14 +161,14 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   const int piece = static_cast<int>(task % pieces);
   wait_for_prior_grids();
   let_dependents_launch();
-  if (task < a.zero_count && a.zeros != nullptr && lane == 0) a.zeros[task] = 0;
-  if (index >= a.places) return;
+  if (task * 32 + lane < a.zero_count) a.zeros[task * 32 + lane] = 0;
+  if (index >= a.rows) return;
   long long row = index, place = index;
-  if (a.slots != nullptr) {
-    const int slot = a.slots[index];
-    if (a.place_scale != nullptr && piece == 0 && lane == 0) a.place_scale[index] = slot >= 0 ? a.weights[slot] : 0.0f;
-    if (slot < 0) return;
-    if (a.top > 0) row = slot / a.top;
+  if (a.place_of_slot != nullptr) {
+    place = a.place_of_slot[index];
+    if (place < 0) return;
+    row = index / a.top;
+    if (a.place_scale != nullptr && piece == 0 && lane == 0) a.place_scale[place] = a.weights[index];
   } else {
     place = index / a.run * a.cap + index % a.run;
   }
@@ -186,11 +186,104 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   }
 }
 
+// Runs of a routed layer's rows: an expert's slots (choices) are cut into as few runs as `run` rows allow, of equal length (a multiple of 16), whose places
+// begin `run` apart.  plan[0]: the number of runs; then per run its expert, first place and rows.  One CTA; which place a slot gets inside its
+// expert's runs depends on the order of arrival, no result does.  A thread asks for eight slots' experts at once.
+// Each warp counts for itself (one table of counters for all warps: 32 of them take turns at an expert's, 7300 slots of 16 experts PLACEHOLDER us); then an
+// expert's counts become its first numbers, warp by warp.
+constexpr int B8_PLAN_THREADS = 1024, B8_PLAN_WARPS = B8_PLAN_THREADS / 32, B8_PLAN_BATCH = 8;
+__global__ void __launch_bounds__(B8_PLAN_THREADS)
+block8_plan_kernel(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run) {
+  wait_for_prior_grids();
+  let_dependents_launch();
+  extern __shared__ int smem[];
+  int *length = smem, *start = length + experts, *total = start + experts, *counts = total + experts;      // counts: [warp][expert]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < B8_PLAN_WARPS * experts; i += B8_PLAN_THREADS) counts[i] = 0;
+  __syncthreads();
+  int* own = counts + warp * experts;
+  // The number of each of the thread's slots among its expert's, as far as this warp has them: use(slot, expert or -1, number).
+  auto each = [&](auto use) {
+    for (int base = 0; base < num_slots; base += B8_PLAN_THREADS * B8_PLAN_BATCH) {
+      int e[B8_PLAN_BATCH];
+#pragma unroll
+      for (int j = 0; j < B8_PLAN_BATCH; ++j) {
+        const int i = base + j * B8_PLAN_THREADS + threadIdx.x;
+        e[j] = i < num_slots ? ids[i] : -1;
+        if (e[j] < 0 || e[j] >= experts) e[j] = -1;
+      }
+#pragma unroll
+      for (int j = 0; j < B8_PLAN_BATCH; ++j) {
+        if (base + j * B8_PLAN_THREADS + 32 * warp >= num_slots) break;
+        const unsigned same = __match_any_sync(0xffffffffu, e[j]);
+        const int first = __ffs(same) - 1;
+        int before = 0;
+        if (e[j] >= 0 && lane == first) {
+          before = own[e[j]];
+          own[e[j]] = before + __popc(same);
+        }
+        __syncwarp();
+        use(base + j * B8_PLAN_THREADS + static_cast<int>(threadIdx.x), e[j], __shfl_sync(0xffffffffu, before, first) + __popc(same & ((1u << lane) - 1)));
+      }
+    }
+  };
+  each([](int, int, int) {});
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += B8_PLAN_THREADS) {
+    int sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < B8_PLAN_WARPS; ++w) {
+      const int n = counts[w * experts + e];
+      counts[w * experts + e] = sum;
+      sum += n;
+    }
+    total[e] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int runs = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+      const int e = e0 + lane, n = e < experts ? total[e] : 0, pieces = (n + run - 1) / run;
+      const int rows = n > 0 ? ((n + pieces - 1) / pieces + 15) / 16 * 16 : 1, taken = (n + rows - 1) / rows;
+      int end = taken;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += other;
+      }
+      const int at = runs + end - taken;
+      if (e < experts) {
+        length[e] = rows;
+        start[e] = at * run;
+      }
+      for (int p = 0; p < taken; ++p) {
+        plan[1 + 3 * (at + p)] = e;
+        plan[2 + 3 * (at + p)] = (at + p) * run;
+        plan[3 + 3 * (at + p)] = min(rows, n - p * rows);
+      }
+      runs += __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (lane == 0) plan[0] = runs;
+  }
+  __syncthreads();
+  each([&](int slot, int e, int nth) {
+    if (slot < num_slots) place_of_slot[slot] = e >= 0 ? start[e] + nth / length[e] * run + nth % length[e] : -1;
+  });
+}
+
 static bool b8_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// `plan` has room for num_slots / run + experts runs.
+int block8_plan(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run, cudaStream_t stream) {
+  const size_t smem = (3 + B8_PLAN_WARPS) * static_cast<size_t>(experts) * sizeof(int);
+  if (smem > 224 * 1024) return ERR_UNSUPPORTED;              // (1638 experts)
+  if (cuda_failed(cudaFuncSetAttribute(block8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
+  return launch_dependent(block8_plan_kernel, dim3(1), dim3(B8_PLAN_THREADS), smem, stream, false, plan, place_of_slot, ids, num_slots, experts, run);
+}
 
 int block8_code_rows(CodeRowsArgs a, int dtype, cudaStream_t stream) {
   a.wide = b8_aligned(a.x, 16) && a.ldx % (dtype == DTYPE_F32 ? 4 : 8) == 0;
-  const long long own = static_cast<long long>(a.places) * b8_pieces(a.K), tasks = own > a.zero_count ? own : a.zero_count;
+  const long long own = static_cast<long long>(a.rows) * b8_pieces(a.K), zeros = (a.zero_count + 31) / 32, tasks = own > zeros ? own : zeros;
   if ((tasks + 7) / 8 >= (1LL << 31)) return ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>((tasks + 7) / 8));
   return dtype == DTYPE_F32 ? launch_dependent(code_rows_kernel<float>, grid, dim3(256), 0, stream, false, a)

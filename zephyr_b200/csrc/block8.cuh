@@ -57,8 +57,8 @@ struct CodeRowsArgs {
   unsigned char* scales;
   const void* x;
   long long ldx;
-  const int* slots;
-  int places, K, run, cap, top;
+  const int* place_of_slot;
+  int rows, K, run, cap, top;          // `rows`: of x, or slots
   float* place_scale;
   const float* weights;
   int* zeros;                          // what a later kernel finds as zeros, or null
@@ -74,6 +74,7 @@ struct Block8Small {
   int* status;
 };
 int block8_product(const Block8Product& p, cudaStream_t stream);          // gemm_block8.cu
+int block8_plan(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run, cudaStream_t stream);      // block8.cu
 int block8_code_rows(CodeRowsArgs a, int dtype, cudaStream_t stream);     // block8.cu
 bool block8_small_fits(int M, int K);                                     // gemm_block8_small.cu
 int block8_small_product(const Block8Small& p, cudaStream_t stream);

@@ -3,8 +3,6 @@
 #include "block8.cuh"
 
 // (routed.cu, gemm_tc_experts.cu)
-ZB_API int zb_route_align_strided(int* plan, int* slots, int* place_of_slot, const int* ids, int num_slots, int experts, int max_runs, int run,
-                                  int places, void* stream);
 ZB_API int zb_gemm_tc_experts_run(int choices, int experts);
 ZB_API int zb_route_combine(void* out, const void* y, long long y_stride, int y_dtype, const void* x, long long x_stride, const int* ids,
                             const float* weights, const int* place_of_slot, int tokens, int width, int top, int dtype, void* stream);
@@ -153,7 +151,6 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
   const long long places = static_cast<long long>(runs) * cap;
   const int groups = (cap + 127) / 128;
   int* plan = memory.take<int>(1 + 3LL * runs);
-  int* slots = memory.take<int>(places);
   int* place_of_slot = memory.take<int>(num_slots);
   float* place_scale = e.weigh_inputs ? memory.take<float>(places) : nullptr;
   int* flags = memory.take<int>(2 * FLAGS);
@@ -166,9 +163,9 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
   if (places >= (1LL << 31)) return ERR_UNSUPPORTED;
   if (memory.base == nullptr) return OK;
   const int zeros = parts != nullptr ? static_cast<int>(2 * FLAGS) : 0;
-  int rc = zb_route_align_strided(plan, slots, place_of_slot, e.ids, num_slots, e.E, runs, cap, static_cast<int>(places), stream);
+  int rc = block8_plan(plan, place_of_slot, e.ids, num_slots, e.E, cap, stream);
   if (rc != OK) return rc;
-  rc = block8_code_rows({codes, scales, e.x, e.ldx, slots, static_cast<int>(places), e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
+  rc = block8_code_rows({codes, scales, e.x, e.ldx, place_of_slot, num_slots, e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
   if (rc != OK) return rc;
   rc = block8_product({hidden_codes, e.ff, DTYPE_F32, hidden_scales, codes, scales, up.codes, up.scales, plan, runs, e.E, 0, cap, cap, up.N, up.K, g.kind, nullptr, place_scale, g.limit,
                        g.alpha, g.shift, false, parts, flags, LEAST_BLOCKS, status}, stream);

@@ -10,14 +10,14 @@
 //
 // The matrix takes the tensor core's row side, 256 rows on a pair of SMs (cta_group::2), a run of up to RUN rows of x the other: a
 // matrix is fetched once for each run, a CTA fetches its 128 rows of it beside half of the run's rows of x.  Persistent: a pair
-// takes (256 rows of w, run) in turn, the runs that share rows of w next to each other in time.  Roles of a CTA's ten warps:
+// takes (256 rows of w, run) in turn, the runs that share rows of w next to each other in time.  Roles of a CTA's warps:
 //   * warp 0, one thread: per block of K (128 bytes a row) tiled copies of its 128 rows of w and of its half of the run's rows (always RUN / 2 of
 //     them: what lies behind a run's rows ends in columns that nobody reads) into a ring; every fourth block also the pieces of scales of its rows
 //     of w and of all the run's rows;
 //   * warp 1 of the first CTA: every fourth block the copies of the scales into tensor memory (tcgen05.cp, in order with the products), then
 //     four products 256 x run x 32, all by one elected lane;
-//   * warps 2..9: a thread owns a row of w (its TMEM lane) and reads 32 sums of x's rows at a time, every other 32 of them, all before anything is
-//     stored, so that the accumulator is free for the tile after the next; results go through shared memory to tiled stores.
+//   * the other warps: a thread owns a row of w (its TMEM lane) and reads 32 sums of x's rows at a time, of every 64 or 128; results go through shared
+//     memory to tiled stores.
 // Every wait is bounded and reports instead of hanging; tensor memory is given back on every path.
 #include <atomic>
 
@@ -28,11 +28,14 @@
 
 namespace zb {
 
-constexpr int G8_EPILOGUE_WARPS = 8;       // two for each quarter of a CTA's rows
+// Warps that read sums out, for each quarter of a CTA's rows two, or four where results are coded: that takes a tile of 256 x 256 some 15000 cycles with
+// two, mostly waiting (its products, K = 2048: 8200), and ungated sums a third of that.
+__host__ __device__ constexpr int g8_epilogue_warps(bool coded) { return coded ? 16 : 8; }
 constexpr int G8_STAGING = 4096;           // an epilogue warp's 32 rows x 32 results on their way out: float32, or two of bfloat16
-constexpr int G8_THREADS = 64 + 32 * G8_EPILOGUE_WARPS;
+__host__ __device__ constexpr int g8_threads(bool coded) { return 64 + 32 * g8_epilogue_warps(coded); }
 constexpr int G8_WAIT_LIMIT = 1 << 18;
 constexpr int G8_MAX_STAGES = 10;
+constexpr int G8_PLAN_RUNS = 384;          // runs of a plan that a CTA keeps in shared memory
 constexpr int G8_W_BYTES = 128 * 128;
 constexpr int G8_SCALES = 3 * B8_PIECE;    // of one CTA's rows of w, and of up to 256 rows of x
 
@@ -48,7 +51,7 @@ template <int RUN> struct Block8Shape {
   static constexpr int SCALE_COLUMN = RUN == 256 ? 448 : 256;
   static constexpr int RING_BYTES = STAGES * (STAGE_BYTES + G8_SCALES);
   // Behind the ring what results pass through: staging, or where they are coded 512 bytes a warp and the largest magnitudes of eight warps' rows, twice.
-  static constexpr int smem_bytes(bool coded) { return RING_BYTES + (coded ? G8_EPILOGUE_WARPS * 512 + 2 * 8 * RUN * 4 : G8_EPILOGUE_WARPS * G8_STAGING) + 1024; }
+  static constexpr int smem_bytes(bool coded) { return RING_BYTES + (coded ? g8_epilogue_warps(true) * 512 + 2 * 8 * RUN * 4 : g8_epilogue_warps(false) * G8_STAGING) + 1024; }
   static_assert(STAGES <= G8_MAX_STAGES && smem_bytes(true) <= 227 * 1024 - 512 && smem_bytes(false) <= 227 * 1024 - 512, "shared memory");
   static_assert(SECOND + RUN <= SCALE_COLUMN && SCALE_COLUMN + 12 * STAGES <= 512, "tensor memory");
 };
@@ -78,9 +81,10 @@ struct Block8Args {
 };
 
 struct Block8Shared {
-  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], acc_edge, merged, peaks[2];
+  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], acc_edge, merged, peaks[4];
   unsigned tmem_base;
   volatile int failed;
+  int plan[3 * G8_PLAN_RUNS];                     // the plan's runs, as many as there is room for
 };
 
 __device__ __forceinline__ bool g8_wait(Block8Shared& sh, unsigned long long* bar, unsigned parity) {
@@ -95,8 +99,11 @@ struct Run8 {
   int matrix, place, rows, out;          // `out`: the first row of y
 };
 __device__ __forceinline__ int runs_of(const Block8Args& a) { return a.plan != nullptr ? a.plan[0] : (a.M + a.run - 1) / a.run; }
-__device__ __forceinline__ Run8 run_of(const Block8Args& a, int i) {
-  if (a.plan != nullptr) return {a.plan[1 + 3 * i], a.plan[2 + 3 * i], a.plan[3 + 3 * i], a.plan[2 + 3 * i]};
+__device__ __forceinline__ Run8 run_of(const Block8Args& a, const Block8Shared& sh, int i) {
+  if (a.plan != nullptr) {
+    const int* run = i < G8_PLAN_RUNS ? sh.plan + 3 * i : a.plan + 1 + 3 * i;
+    return {run[0], run[1], run[2], run[1]};
+  }
   return {0, i * a.cap, min(a.run, a.M - i * a.run), i * a.run};
 }
 
@@ -183,9 +190,10 @@ __device__ __forceinline__ unsigned tc_idesc_scaled_pair(unsigned n) { return ((
 // GATED: w's rows come in blocks of 8 gates and their 8 ups; y has N / 2 columns.  SCALED: both sums of a place times
 // gate.row_scale[place] first.  TOut = unsigned char (GATED): the results are coded in blocks of 128 as rows of activations are.
 template <int RUN, typename TOut, bool GATED, bool SCALED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_block8_kernel(const __grid_constant__ Block8Args a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TOut) == 1), 1) gemm_block8_kernel(const __grid_constant__ Block8Args a) {
   using Shape = Block8Shape<RUN>;
   constexpr bool CODED = sizeof(TOut) == 1;
+  constexpr int EPILOGUE_WARPS = g8_epilogue_warps(CODED), GROUPS = EPILOGUE_WARPS / 4;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Block8Shared sh;
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -200,11 +208,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
-      mbar_init(&sh.acc_empty[b], 2 * G8_EPILOGUE_WARPS);      // of both CTAs
+      mbar_init(&sh.acc_empty[b], 2 * EPILOGUE_WARPS);      // of both CTAs
     }
-    for (int g = 0; g < 2; ++g) mbar_init(&sh.peaks[g], 8);     // four warps of each CTA
-    mbar_init(&sh.acc_edge, 2 * G8_EPILOGUE_WARPS);
-    mbar_init(&sh.merged, G8_EPILOGUE_WARPS);
+    for (int g = 0; g < GROUPS; ++g) mbar_init(&sh.peaks[g], 8);     // four warps of each CTA
+    mbar_init(&sh.acc_edge, 2 * EPILOGUE_WARPS);
+    mbar_init(&sh.merged, EPILOGUE_WARPS);
     sh.failed = 0;
     fence_barrier_init();
   }
@@ -234,6 +242,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
   wait_for_prior_grids();
   let_dependents_launch();
   const int runs = runs_of(a);
+  if (a.plan != nullptr) {                          // (a run's numbers from global memory would keep every tile waiting for 0.7 us in each role)
+    for (int i = threadIdx.x; i < 3 * min(runs, G8_PLAN_RUNS); i += g8_threads(CODED)) sh.plan[i] = a.plan[1 + i];
+    __syncthreads();
+  }
   Share share(a, runs, pair, pairs);
   int item, k_first, k_end;
   const int accumulators = a.halves ? 1 : 2;
@@ -247,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       int stage = 0, scales = 0;
       unsigned phase = 0;
       while (share.next(a, item, k_first, k_end)) {
-        const Run8 run = run_of(a, item % runs);
+        const Run8 run = run_of(a, sh, item % runs);
         const int block = item / runs, half = half_columns(run.rows);
         const int w_group = w_group_of(a, run.matrix, block, rank), w_row = w_group * a.k_blocks * 128;
         const int x_row = run.place + half * rank, w_scales = w_group * a.pieces * 4, x_scales = run.place / a.cap * a.pieces * 4 * a.run_groups;
@@ -287,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     int stage = 0, acc = 0, scales = 0;
     unsigned phase = 0, acc_phase = 0, edge_phase = 1;
     while (share.next(a, item, k_first, k_end)) {
-      const unsigned columns = 2 * half_columns(run_of(a, item % runs).rows), idesc = tc_idesc_scaled_pair(columns);
+      const unsigned columns = 2 * half_columns(run_of(a, sh, item % runs).rows), idesc = tc_idesc_scaled_pair(columns);
       bool ok = __all_sync(0xffffffffu, g8_wait(sh, &sh.acc_empty[acc], acc_phase ^ 1));
       if (RUN == 256) ok = ok && __all_sync(0xffffffffu, g8_wait(sh, &sh.acc_edge, edge_phase));
       edge_phase ^= 1;
@@ -339,15 +351,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
     }
   } else if (warp > 1) {
     const int quarter = warp & 3;                   // the TMEM lanes this warp may read: 32 quarter .. + 31
-    const int group = (warp - 2) >> 2;              // and of every 64 columns (rows of x) it takes 32 group .. + 31
-    constexpr int CHUNKS = RUN / 64;
+    const int group = (warp - 2) >> 2;              // and of every COLUMNS columns (rows of x) it takes 32 group .. + 31
+    constexpr int COLUMNS = 32 * GROUPS, CHUNKS = (RUN + COLUMNS - 1) / COLUMNS;
     const int width = GATED ? a.N / 2 : a.N;
     const bool holds_gate = (lane & 8) == 0;
     unsigned char* staging = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * G8_STAGING;
     int acc = 0, stores = 0;
     unsigned acc_phase = 0, merged_phase = 0, peaks_phase = 0;
     while (share.next(a, item, k_first, k_end)) {
-      const Run8 run = run_of(a, item % runs);
+      const Run8 run = run_of(a, sh, item % runs);
       const int row = item / runs * 256 + 128 * rank + 32 * quarter + lane, column0 = (row - lane) / (GATED ? 2 : 1);
       const float bias = a.gate.bias != nullptr && row < a.N ? a.gate.bias[row] : 0.0f;
       if (!__all_sync(0xffffffffu, g8_wait(sh, &sh.acc_full[acc], acc_phase))) {
@@ -394,10 +406,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
       };
       // Another pair's or this one's part of a tile: [column][row].
       auto part_of = [&](int p) { return a.parts + (static_cast<size_t>(p) * 2 + rank) * RUN * 128 + 32 * quarter + lane; };
-      auto flag_of = [&](int p, int g) { return a.flags + (p * 2 + rank) * G8_EPILOGUE_WARPS + 4 * g + quarter; };
+      auto flag_of = [&](int p, int g) { return a.flags + (p * 2 + rank) * EPILOGUE_WARPS + 4 * g + quarter; };
       if (k_end < a.k_blocks) {                       // the tile's end is another pair's
         float* part = part_of(pair);
-        for (int c = 32 * group; c < run.rows; c += 64) {
+        for (int c = 32 * group; c < run.rows; c += COLUMNS) {
           unsigned v[32];
           read_sums(c, v);
 #pragma unroll
@@ -414,10 +426,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         int others = 0;                               // pairs in front of this one that have blocks of the tile
         const int start = item * a.k_blocks;
         do ++others; while (share.border(pair - others) > start);
-        // A flag a lane: one look at all of them takes as long as one at one.  Of each pair those of the two warps that have this warp's rows.
+        // A flag a lane: one look at all of them takes as long as one at one.  Of each pair those of all warps that have this warp's rows.
         bool ok = true;
-        for (int i = lane; i < 2 * others && ok; i += 32) {
-          const int* flag = flag_of(pair - others + i / 2, i % 2);
+        for (int i = lane; i < GROUPS * others && ok; i += 32) {
+          const int* flag = flag_of(pair - others + i / GROUPS, i % GROUPS);
           int waited = 0;
           while (load_acquire(flag) == 0 && (ok = ++waited < G8_WAIT_LIMIT && !sh.failed)) __nanosleep(32);
         }
@@ -426,22 +438,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           sh.failed = 1;
           break;
         }
-        // The others' parts, in the order of K's blocks, are added where the sums are: 16 columns of four pairs on their way at a time.
-        for (int c = 16 * group; c < run.rows; c += 32) {
+        // The others' parts, in the order of K's blocks, are added where the sums are: 16 columns of some pairs on their way at a time.
+        constexpr int PARTS = CODED ? 2 : 4;
+        for (int c = 16 * group; c < run.rows; c += 16 * GROUPS) {
           unsigned v[16];
           tmem_ld16(tmem_row + c, v);
           tmem_wait_ld16(v);
-          for (int p = pair - others; p < pair; p += 4) {
-            float part[4][16];
+          for (int p = pair - others; p < pair; p += PARTS) {
+            float part[PARTS][16];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < PARTS; ++q)
               if (p + q < pair) {
                 const float* from = part_of(p + q) + c * 128;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) part[q][i] = __ldcg(from + i * 128);
               }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < PARTS; ++q)
               if (p + q < pair) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + part[q][i]);
@@ -462,82 +475,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
         tc_fence_after_sync();
       }
       // (Columns beyond the run's rows are read and not used.)
-      if constexpr (!GATED) {
-        // bfloat16: words of two columns of x's rows 2 i (an even lane's, of its own column and its neighbour's) and 2 i + 1 (the odd one's).
-        constexpr int WORDS = sizeof(TOut) == 2 ? 16 : 32;
-        unsigned out[CHUNKS][WORDS];
-        auto take = [&](auto activation) {
-#pragma unroll
-          for (int s = 0; s < CHUNKS; ++s) {
-            const int j = chunk(s), c = 64 * j + 32 * group;
-            if (c < run.rows) {
-              unsigned v[32];
-              read_sums(c, v);
-#pragma unroll
-              for (int i = 0; i < WORDS; ++i) {
-                if constexpr (sizeof(TOut) == 2) {
-                  const float one = activation(__uint_as_float(v[2 * i])), other = activation(__uint_as_float(v[2 * i + 1]));
-                  const float met = __shfl_xor_sync(0xffffffffu, lane & 1 ? one : other, 1);
-                  out[j][i] = lane & 1 ? pack_bf16(met, other) : pack_bf16(one, met);
-                } else {
-                  out[j][i] = __float_as_uint(activation(__uint_as_float(v[i])));
-                }
-              }
-            }
-            if (s == EDGE) free_edge();
-          }
-        };
-        if (a.act == ACT_NONE) take([](float z) { return z; });
-        else if (a.act == ACT_GELU) take([](float z) { return gelu_tanh_fast(z); });
-        else take([](float z) { return relu_squared(z); });
-        free_accumulator();
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-          const int c = 64 * j + 32 * group, rows = run.rows - c;
-          if (rows <= 0) continue;
-          // A run's last rows may be followed by another run's (without a plan): those go out one by one.
-          if (a.tiled && (rows >= 32 || a.plan != nullptr || run.out + run.rows == a.M)) {
-            unsigned char* buffer = staging + (sizeof(TOut) == 2 ? (stores & 1) * 2048 : 0);
-            if (lane == 0) {
-              if (sizeof(TOut) == 2) bulk_wait_read<1>();
-              else bulk_wait_read<0>();
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) {
-              if constexpr (sizeof(TOut) == 2) *reinterpret_cast<unsigned*>(buffer + (2 * i + (lane & 1)) * 64 + (lane & ~1) * 2) = out[j][i];
-              else *reinterpret_cast<unsigned*>(buffer + i * 128 + lane * 4) = out[j][i];
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              if (column0 < a.N) tiled_store_2d_s2g(&a.y_map, column0, run.out + c, buffer);
-              bulk_commit();
-            }
-            ++stores;
-          } else {
-            const int pair_row = lane & 1, column = row & ~1;
-            TOut* at = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + c) * a.ldy;
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) {
-              if constexpr (sizeof(TOut) == 2) {
-                unsigned short* bits = reinterpret_cast<unsigned short*>(at) + static_cast<size_t>(2 * i + pair_row) * a.ldy + column;
-                if (2 * i + pair_row < rows && column < a.N) bits[0] = static_cast<unsigned short>(out[j][i]);
-                if (2 * i + pair_row < rows && column + 1 < a.N) bits[1] = static_cast<unsigned short>(out[j][i] >> 16);
-              } else {
-                if (i < rows && row < a.N) at[static_cast<size_t>(i) * a.ldy + row] = __uint_as_float(out[j][i]);
-              }
-            }
-          }
-        }
-      } else {
+      if constexpr (GATED) {
         // Lane l holds the gates, lane l + 8 their ups of 32 rows of x: the first finishes 16 of them, the second the others.
         const int own_row = holds_gate ? 0 : 16, own_column = (lane >> 4) * 8 + (lane & 7);
         float hidden[CHUNKS][16];
         auto gate_pairs = [&](auto activation) {
 #pragma unroll
           for (int s = 0; s < CHUNKS; ++s) {
-            const int j = chunk(s), c = 64 * j + 32 * group;
+            const int j = chunk(s), c = COLUMNS * j + 32 * group;
             if (c < run.rows) {
               unsigned v[32];
               read_sums(c, v);
@@ -566,7 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           TOut* y = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + own_row) * a.ldy + column0 + own_column;
 #pragma unroll
           for (int j = 0; j < CHUNKS; ++j) {
-            const int c = 64 * j + 32 * group;
+            const int c = COLUMNS * j + 32 * group;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (c + own_row + i < run.rows && column0 + own_column < width) y[static_cast<size_t>(c + i) * a.ldy] = from_float<TOut>(hidden[j][i]);
@@ -575,11 +520,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
           // CTA) gives the scale.  [turn][CTA][quarter][row of x], in both CTAs; lane l finds and hands over row `mine` of 32.
           unsigned char* bytes = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * 512;
-          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + G8_EPILOGUE_WARPS * 512) + peaks_phase * 8 * RUN;
+          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + peaks_phase * 8 * RUN;
           const int mine = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
 #pragma unroll
           for (int j = 0; j < CHUNKS; ++j) {
-            const int c = 64 * j + 32 * group;
+            const int c = COLUMNS * j + 32 * group;
             if (c < run.rows) {
               unsigned m[16];
 #pragma unroll
@@ -615,7 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
           unsigned char* codes_at = static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place) * pitch + block * 128 + rank * 64 + quarter * 16;
 #pragma unroll
           for (int j = 0; j < CHUNKS; ++j) {
-            const int c = 64 * j + 32 * group;
+            const int c = COLUMNS * j + 32 * group;
             if (c < run.rows) {
               unsigned largest = 0;
 #pragma unroll
@@ -642,6 +587,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
             }
           }
         }
+      } else {
+        // bfloat16: words of two columns of x's rows 2 i (an even lane's, of its own column and its neighbour's) and 2 i + 1 (the odd one's).
+        constexpr int WORDS = sizeof(TOut) == 2 ? 16 : 32;
+        auto take = [&](auto activation) {
+#pragma unroll 1
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int c = COLUMNS * chunk(s) + 32 * group, rows = run.rows - c;
+            unsigned out[WORDS];
+            if (rows > 0) {
+              unsigned v[32];
+              read_sums(c, v);
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(TOut) == 2) {
+                  const float one = activation(__uint_as_float(v[2 * i])), other = activation(__uint_as_float(v[2 * i + 1]));
+                  const float met = __shfl_xor_sync(0xffffffffu, lane & 1 ? one : other, 1);
+                  out[i] = lane & 1 ? pack_bf16(met, other) : pack_bf16(one, met);
+                } else {
+                  out[i] = __float_as_uint(activation(__uint_as_float(v[i])));
+                }
+              }
+            }
+            if (s == EDGE) free_edge();
+            if (s == CHUNKS - 1) free_accumulator();
+            if (rows <= 0) continue;
+            // A run's last rows may be followed by another run's (without a plan): those go out one by one.
+            if (a.tiled && (rows >= 32 || a.plan != nullptr || run.out + run.rows == a.M)) {
+              unsigned char* buffer = staging + (sizeof(TOut) == 2 ? (stores & 1) * 2048 : 0);
+              if (lane == 0) {
+                if (sizeof(TOut) == 2) bulk_wait_read<1>();
+                else bulk_wait_read<0>();
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(TOut) == 2) *reinterpret_cast<unsigned*>(buffer + (2 * i + (lane & 1)) * 64 + (lane & ~1) * 2) = out[i];
+                else *reinterpret_cast<unsigned*>(buffer + i * 128 + lane * 4) = out[i];
+              }
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                if (column0 < a.N) tiled_store_2d_s2g(&a.y_map, column0, run.out + c, buffer);
+                bulk_commit();
+              }
+              ++stores;
+            } else {
+              [[maybe_unused]] const int pair_row = lane & 1, column = row & ~1;
+              TOut* at = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + c) * a.ldy;
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(TOut) == 2) {
+                  unsigned short* bits = reinterpret_cast<unsigned short*>(at) + static_cast<size_t>(2 * i + pair_row) * a.ldy + column;
+                  if (2 * i + pair_row < rows && column < a.N) bits[0] = static_cast<unsigned short>(out[i]);
+                  if (2 * i + pair_row < rows && column + 1 < a.N) bits[1] = static_cast<unsigned short>(out[i] >> 16);
+                } else {
+                  if (i < rows && row < a.N) at[static_cast<size_t>(i) * a.ldy + row] = __uint_as_float(out[i]);
+                }
+              }
+            }
+          }
+        };
+        if (a.act == ACT_NONE) take([](float z) { return z; });
+        else if (a.act == ACT_GELU) take([](float z) { return gelu_tanh_fast(z); });
+        else take([](float z) { return relu_squared(z); });
       }
     }
     if (!GATED && lane == 0) bulk_wait_all();       // the staging buffers are read, the rows written
@@ -662,10 +671,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1) gemm_
 
 // How many pairs of this kernel the device holds at once (0: the runtime has failed).
 template <typename Kernel>
-int pairs_at_once(Kernel kernel, int smem, int sms) {
+int pairs_at_once(Kernel kernel, int threads, int smem, int sms) {
   if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return 0;
   cudaLaunchConfig_t config = {};
-  config.blockDim = dim3(G8_THREADS);
+  config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.gridDim = dim3(2 * (sms / 2));
   int clusters = 0;
@@ -675,7 +684,7 @@ int pairs_at_once(Kernel kernel, int smem, int sms) {
 
 template <int RUN, typename TOut, bool GATED, bool SCALED>
 int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) {
-  constexpr int SMEM_BYTES = Block8Shape<RUN>::smem_bytes(sizeof(TOut) == 1);
+  constexpr int SMEM_BYTES = Block8Shape<RUN>::smem_bytes(sizeof(TOut) == 1), THREADS = g8_threads(sizeof(TOut) == 1);
   auto kernel = gemm_block8_kernel<RUN, TOut, GATED, SCALED>;
   static std::atomic<int> known[64];                // by device: asking takes the host 3 us
   int device = 0, sms = 0;
@@ -683,7 +692,7 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
   int pairs = device < 64 ? known[device].load() : 0;
   if (pairs == 0) {
     if (cuda_failed(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device))) return ERR_CUDA;
-    pairs = pairs_at_once(kernel, SMEM_BYTES, sms);
+    pairs = pairs_at_once(kernel, THREADS, SMEM_BYTES, sms);
     if (pairs <= 0) return ERR_CUDA;
     if (device < 64) known[device].store(pairs);
   }
@@ -691,7 +700,7 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
   cudaLaunchConfig_t config = {};
   // (With `parts` pairs wait for one another: all of them are on the device at once.)
   config.gridDim = dim3(2 * static_cast<unsigned>(a.parts != nullptr || items > pairs ? pairs : items));
-  config.blockDim = dim3(G8_THREADS);
+  config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = SMEM_BYTES;
   config.stream = stream;
   cudaLaunchAttribute attribute[1];
@@ -727,7 +736,7 @@ static bool result_map(CUtensorMap* out, void* y, long long rows, int N, long lo
 }
 
 // The operands and results of a product (block8.cuh): y = x w^T in blocks.  Without `plan` M rows of x in runs of `run`, one matrix, y [M]; with it
-// (zb_route_align_strided) `max_runs` runs at most of `matrices`, y by place.
+// (block8_plan) `max_runs` runs at most of `matrices`, y by place.
 int block8_product(const Block8Product& p, cudaStream_t stream) {
   const bool gated = p.kind >= 1 && p.kind <= 3;
   Block8Args a = {};

@@ -237,11 +237,9 @@ align_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int num_
 
 // The same for products that run as one launch of the tcgen05 kernel (gemm_tc_experts.cu): an expert's tokens are cut into runs
 // of up to `run` places of equal length (a multiple of 16), plan[0] is the number of runs, plan[1 + 3 i ...] run i's expert,
-// first place and places that count, and slots[place] is -1 where a place pads a run.  With a `stride` (not 0) the runs' places begin that
-// many apart, whatever the runs' lengths, instead of one behind the other.
+// first place and places that count, and slots[place] is -1 where a place pads a run.
 __global__ void __launch_bounds__(ALIGN_THREADS)
-align_runs_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int num_slots, int experts, int max_runs, int run, int places,
-                  int stride) {
+align_runs_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int num_slots, int experts, int max_runs, int run, int places) {
   wait_for_prior_grids();
   let_dependents_launch();
   extern __shared__ int align_smem[];
@@ -273,8 +271,7 @@ align_runs_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int
     int runs = 0, first_place = 0;
     for (int e0 = 0; e0 < experts; e0 += 32) {
       const int e = e0 + lane, n = e < experts ? count[e] : 0, length = length_of(n), pieces = n > 0 ? (n + length - 1) / length : 0;
-      const int taken = pieces * (stride != 0 ? stride : length);
-      int runs_end = pieces, places_end = taken;
+      int runs_end = pieces, places_end = pieces * length;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int r = __shfl_up_sync(0xffffffffu, runs_end, o), p = __shfl_up_sync(0xffffffffu, places_end, o);
@@ -283,11 +280,11 @@ align_runs_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int
           places_end += p;
         }
       }
-      const int at = runs + runs_end - pieces, place = first_place + places_end - taken;
+      const int at = runs + runs_end - pieces, place = first_place + places_end - pieces * length;
       if (e < experts) start[e] = place;
       for (int p = 0; p < pieces && at + p < max_runs; ++p) {
         plan[1 + 3 * (at + p)] = e;
-        plan[2 + 3 * (at + p)] = place + p * (stride != 0 ? stride : length);
+        plan[2 + 3 * (at + p)] = place + p * length;
         plan[3 + 3 * (at + p)] = min(length, n - p * length);
       }
       runs += __shfl_sync(0xffffffffu, runs_end, 31);
@@ -300,11 +297,7 @@ align_runs_kernel(int* plan, int* slots, int* place_of_slot, const int* ids, int
     const int i = i0 + threadIdx.x, e = i < num_slots ? ids[i] : -1;
     const bool valid = e >= 0 && e < experts;
     const int nth = add(fill, e, valid);
-    int place = valid ? start[e] + nth : -1;            // (an expert's runs lie one behind the other, without gaps between them)
-    if (valid && stride != 0) {
-      const int length = length_of(count[e]);
-      place = start[e] + nth / length * stride + nth % length;
-    }
+    const int place = valid ? start[e] + nth : -1;      // (an expert's runs lie one behind the other, without gaps between them)
     if (place >= 0 && place < places) slots[place] = i;
     if (i < num_slots) place_of_slot[i] = place;
   }
@@ -636,20 +629,8 @@ ZB_API int zb_route_align_runs(int* plan, int* slots, int* place_of_slot, const 
   const size_t smem = 3 * static_cast<size_t>(experts) * sizeof(int);
   if (smem > 48 * 1024) return ERR_UNSUPPORTED;
   launch_dependent(align_runs_kernel, dim3(1), dim3(ALIGN_THREADS), smem, static_cast<cudaStream_t>(stream), false, plan,
-      slots, place_of_slot, ids, num_slots, experts, max_runs, run, places, 0);
+      slots, place_of_slot, ids, num_slots, experts, max_runs, run, places);
   return launch_result();
-}
-
-// The same with the runs' places `run` apart: run i's begin at i * run.  `places` >= max_runs * run.
-ZB_API int zb_route_align_strided(int* plan, int* slots, int* place_of_slot, const int* ids, int num_slots, int experts, int max_runs,
-                                  int run, int places, void* stream) {
-  if (num_slots < 0 || experts <= 0 || run <= 0 || run % 16 != 0 || max_runs < num_slots / run + experts ||
-      static_cast<long long>(max_runs) * run > places)
-    return ERR_BAD_ARGUMENT;
-  const size_t smem = 3 * static_cast<size_t>(experts) * sizeof(int);
-  if (smem > 48 * 1024) return ERR_UNSUPPORTED;
-  return launch_dependent(align_runs_kernel, dim3(1), dim3(ALIGN_THREADS), smem, static_cast<cudaStream_t>(stream), false, plan, slots,
-                          place_of_slot, ids, num_slots, experts, max_runs, run, places, run);
 }
 
 // out [places, width] = the tokens' rows in the order of `slots` (bfloat16; width a multiple of 8, 16-byte aligned rows).

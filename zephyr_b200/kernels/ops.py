@@ -84,7 +84,6 @@ _SIGNATURES = {
     "zb_expert_product": [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                           c_int, c_int, c_int, c_float, c_float, c_float, c_int, c_int, c_void_p],
     "zb_route_align_runs": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
-    "zb_route_align_strided": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
     "zb_matrix_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int], "zb_block8_feed_forward_kernels": [c_int, c_int, c_int, c_int],
