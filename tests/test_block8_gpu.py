@@ -87,12 +87,16 @@ def test_products(m, n, k, x_dtype, y_dtype):
     _close(ops.linear(x, packed, y_dtype), want, plain.sum_error(k) * magnitude, y_dtype)
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 5120, 25600), (16, 512, 25600), (12, 4096, 12288), (8, 30000, 256), (100, 640, 9000)])
-def test_products_of_long_rows(m, n, k):
+# Few rows of long matrices; then rows and columns for runs of 64, 128 and 256 rows, tiles of whole and shared K, result rows that are and are not
+# multiples of 16 bytes.
+@pytest.mark.parametrize("m,n,k", [(3, 5120, 25600), (16, 512, 25600), (12, 4096, 12288), (8, 30000, 256), (100, 640, 9000),
+                                   (130, 2500, 14336), (100, 6400, 14336), (1000, 4864, 10240), (300, 8200, 640), (600, 4105, 260), (1030, 4110, 384), (333, 1030, 9100)])
+def test_products_of_long_rows_and_of_many(m, n, k):
     x = _random((m, k), 8, dtype=torch.bfloat16)
     packed, w = _matrix((n, k), 9)
     want, magnitude = plain.product(x, w)
-    _close(ops.linear(x, packed, torch.float32), want, plain.sum_error(k) * magnitude, torch.float32)
+    for y in (torch.float32, torch.bfloat16):
+        _close(ops.linear(x, packed, y), want, plain.sum_error(k) * magnitude, y)
 
 
 @pytest.mark.parametrize("m", [5, 40, 300])
@@ -163,7 +167,8 @@ def _feed_forward(x, up, down, act, limits=LIMITS, bias=None):
 
 
 @pytest.mark.parametrize("m,width,ff,act", [(1, 256, 128, "silu"), (16, 1024, 904, "relu"), (17, 130, 8, "silu"), (64, 300, 1000, "bounded"),
-                                            (200, 1024, 512, "silu"), (600, 640, 1544, "bounded")])
+                                            (200, 1024, 512, "silu"), (600, 640, 1544, "bounded"), (600, 4100, 4104, "silu"),
+                                            (40, 12288, 640, "silu"), (40, 1000, 9000, "relu"), (100, 14336, 3200, "silu"), (1024, 10240, 2432, "bounded")])
 def test_feed_forwards(m, width, ff, act):
     x = _random((m, width), 20, dtype=torch.bfloat16)
     (up, up_values), (down, down_values) = _matrix((2 * ff, width), 21, 0.1), _matrix((width, ff), 22, 0.1)
@@ -176,7 +181,8 @@ def test_feed_forwards(m, width, ff, act):
 @pytest.mark.parametrize("tokens,width,ff,experts,identity,top,act,skew", [
     (1, 256, 128, 4, 0, 2, "silu", 0.0), (8, 512, 136, 16, 2, 4, "relu", 0.5), (100, 136, 72, 5, 0, 5, "bounded", 0.0),
     (300, 300, 200, 8, 3, 3, "silu", 4.0), (777, 256, 264, 60, 0, 6, "bounded", 2.0), (1500, 128, 128, 4, 0, 2, "silu", 6.0),
-    (40, 129, 16, 3, 1, 2, "silu", 0.0)])
+    (40, 129, 16, 3, 1, 2, "silu", 0.0), (20, 8192, 256, 4, 0, 2, "silu", 0.0), (30, 256, 6144, 3, 0, 2, "relu", 0.0), (300, 8192, 200, 4, 0, 1, "silu", 0.0),
+    (500, 128, 16, 400, 0, 2, "silu", 0.0), (900, 128, 16, 3, 0, 1, "silu", 3.0)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_routed_experts(tokens, width, ff, experts, identity, top, act, skew, dtype):
     x = _random((tokens, width), 30, dtype=dtype)
@@ -214,3 +220,35 @@ def test_routed_experts(tokens, width, ff, experts, identity, top, act, skew, dt
             want[token] += y
             error[token] += off + HALF_STEP[dtype] * (y.abs() + off) + 2.0 ** -22 * y.abs()
         _close(got, want, error, dtype)
+
+
+# ------------------------------------------------------------------------------------------------- calls side by side
+def test_calls_on_two_streams_at_once():
+    """Calls that share a matrix, on two streams with no order between them, give what the same calls give one after the other, bit for bit."""
+    (up, _), (down, _) = _matrix((2 * 1024, 640), 40, 0.1), _matrix((640, 1024), 41, 0.1)
+    (ups, _), (downs, _) = _matrix((8, 512, 640), 42, 0.1), _matrix((8, 640, 256), 43, 0.1)
+    long, _ = _matrix((640, 12800), 44)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    inputs = [[_random((m, 640), 45 + 10 * s + m, dtype=torch.bfloat16) for m in (3, 40, 300)] for s in range(2)]
+    wide = [_random((40, 12800), 90 + s, dtype=torch.bfloat16) for s in range(2)]
+    chosen = [_random((300, 8), 50 + s).softmax(1).topk(2, 1) for s in range(2)]
+
+    def calls(s):
+        out = []
+        for x in inputs[s]:
+            out += [ops.linear(x, up), ops.block_feed_forward(x, up, down)]
+        out.append(ops.linear(wide[s], long))
+        out.append(ops.routed_experts(inputs[s][2], chosen[s][1].int().contiguous(), chosen[s][0].contiguous(), ups, None, downs))
+        return out
+
+    want = [calls(0), calls(1)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for s in (0, 1):
+            with torch.cuda.stream(streams[s]):
+                got[s].append(calls(s))
+    torch.cuda.synchronize()
+    for s in (0, 1):
+        for run in got[s]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[s]))

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
 // Runs of a routed layer's rows: an expert's slots (choices) are cut into as few runs as `run` rows allow, of equal length (a multiple of 16), whose places
 // begin `run` apart.  plan[0]: the number of runs; then per run its expert, first place and rows.  One CTA; which place a slot gets inside its
 // expert's runs depends on the order of arrival, no result does.  A thread asks for eight slots' experts at once.
-// Each warp counts for itself (one table of counters for all warps: 32 of them take turns at an expert's, 7300 slots of 16 experts PLACEHOLDER us); then an
+// Each warp counts for itself (one table of counters for all warps would have 32 of them take turns at an expert's); then an
 // expert's counts become its first numbers, warp by warp.
 constexpr int B8_PLAN_THREADS = 1024, B8_PLAN_WARPS = B8_PLAN_THREADS / 32, B8_PLAN_BATCH = 8;
 __global__ void __launch_bounds__(B8_PLAN_THREADS)

@@ -23,7 +23,8 @@ struct Pieces {
 };
 
 // Whether few rows go to the kernel that streams the matrix.  It has four warps or sixteen on a tile, the tensor cores' kernel waits for a tile's whole K:
-// up to 8 rows it is ahead or level everywhere (us, streaming / tensor cores: PLACEHOLDER), up to 16, which take twice its instructions, where the matrix is small (PLACEHOLDER).
+// up to 8 rows it is ahead or level everywhere (8 rows, us, streaming / tensor cores: 24576 x 4096 21.3 / 25.2, 51200 x 5120 45.3 / 46.0), up to 16, which take twice its
+// instructions, where the matrix is small (16 rows: 4096 x 4096 9.3 / 12.4, 24576 x 4096 24.0 / 26.0, but 10240 x 5120 18.5 / 16.0).
 constexpr long long STREAM_VALUES = 28LL << 20;
 static bool streams(int M, int N, int K) { return block8_small_fits(M, K) && (M <= 8 || static_cast<long long>(N) * K <= STREAM_VALUES); }
 // Whether its rows are coded by a kernel ahead of it instead of in every CTA for itself (8 rows, us, ahead / in each: K = 1024 4.6 / 4.3, 4096 7.6 / 8.0,
@@ -35,10 +36,16 @@ constexpr int LEAST_BLOCKS = 8;
 struct Rows {
   int run, cap, runs;
 };
-// Rows in as few runs of equal length (a multiple of 16) as up to `most` rows a run allow.
-static Rows rows_of(int M, int most) {
+// Rows in as few runs of equal length (a multiple of 16) as up to 256 rows a run allow, or 128, or 64 where more tiles still all run at
+// once: a tile's sums wait for its whole K and are read out behind it, and a shorter run's tile is through sooner on pairs that had none (256 / 128 / 64 rows a
+// run, us: 256 x 1024 x 1024 11.2 / 9.1 / 8.5, 333 x 4096 x 4096 17.8 / 16.3 / 23.2).  Every run fetches the matrix again, and with more than
+// two thirds of the pairs on it that costs runs of 64 rows more than it gives (512 x 2048 x 2048, 32 tiles of 128 / 64 of 64: 11.3 / 12.2).
+static Rows rows_of(int M, int N, int most) {
+  auto tiles = [&](int run) { return static_cast<long long>((M + run - 1) / run) * ((N + 255) / 256); };
+  if (tiles(128) <= G8_PAIRS && most > 128) most = 128;
+  if (tiles(64) <= G8_PAIRS * 2 / 3) most = 64;
   const int runs = (M + most - 1) / most, run = ((M + runs - 1) / runs + 15) / 16 * 16;
-  return {run, M <= 64 ? 64 : M <= 128 || most == 128 ? 128 : 256, runs};
+  return {run, run <= 64 ? 64 : run <= 128 ? 128 : 256, runs};
 }
 // Float32 results of long rows are summed in two accumulators: the tensor cores cut what a sum's 24 bits do not hold, always towards zero, so a
 // sum is off by 7e-8 of itself for every 1024 values of K (14336: 1e-6).
@@ -53,7 +60,7 @@ struct ProductWork {
 };
 static ProductWork product_work(Pieces& memory, int M, int N, int K, bool halves) {
   ProductWork w;
-  w.rows = rows_of(M, halves ? 128 : 256);
+  w.rows = rows_of(M, N, halves ? 128 : 256);
   w.halves = halves;
   const long long places = static_cast<long long>(w.rows.runs) * w.rows.cap, items = static_cast<long long>(w.rows.runs) * ((N + 255) / 256);
   const bool parts = b8_in_parts(items, b8_blocks(K), w.rows.cap);
@@ -113,7 +120,7 @@ static int feed_forward(Pieces& memory, void* y, long long ldy, int y_dtype, con
     return product(memory, y, ldy, y_dtype, hidden, down.K, DTYPE_F32, down, M, Gate{0, nullptr, 0.0f, 1.0f, 0.0f}, true, status, stream);
   }
   const bool halves = sums_in_halves(down.K, y_dtype);
-  const Rows rows = rows_of(M, halves ? 128 : 256);
+  const Rows rows = rows_of(M, up.N > down.N ? up.N : down.N, halves ? 128 : 256);
   const long long places = static_cast<long long>(rows.runs) * rows.cap, groups = places / rows.cap * ((rows.cap + 127) / 128);
   int* flags = memory.take<int>(2 * FLAGS);
   const bool up_parts = b8_in_parts(static_cast<long long>(rows.runs) * ((up.N + 255) / 256), b8_blocks(up.K), rows.cap);

@@ -4,9 +4,8 @@
 //
 // The matrix's rows sit on the 16-row side of m16n8k16, the tokens on the 8-column side.  Inside a half block of 64 k, lane t of a quad owns the 16
 // values k = 16 t .. 16 t + 15 of its row: one 16-byte piece feeds four products, which see k in a permuted order, the same for both operands.  The
-// codes become half-precision numbers first, which hold them exactly (the 8-bit form of the instruction is done with conversions as well here, of the
-// matrix's codes once for every 8 tokens: 233 instructions a block of 16 x 128 in place of PLACEHOLDER).  A block's products start from zero, and their sums
-// join the warp's own in float32, times the block's two scales.
+// codes become half-precision numbers first, which hold them exactly (the 8-bit form of the instruction took as many instructions and the same time).
+// A block's products start from zero, and their sums join the warp's own in float32, times the block's two scales.
 //
 // One CTA an SM walks tiles of 16 rows; a team of TEAM of its 16 warps shares a tile, each a slice of the blocks of K.  x lies in shared memory as
 // codes; the matrix passes through a ring of two blocks of 16 x 128 a warp, each one tiled copy (128-byte swizzle) that the warp's first lane asks
