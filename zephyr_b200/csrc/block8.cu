@@ -148,49 +148,52 @@ matrix_values_kernel(T* out, const unsigned char* codes, const unsigned char* sc
   }
 }
 
-// Rows of activations into codes: a warp takes 512 values of a row, 16 a lane.  Where a row goes, and what it is:
-//   * without `place_of_slot`, row m goes to place m / run * cap + m % run: the rows of a run of the product lie together, at its start;
-//   * with `place_of_slot`, row s / top goes to place_of_slot[s], or nowhere where that is negative; with `place_scale` the place also gets the
-//     slot's weight.
+// Rows of activations into codes: a warp takes 512 values of a row, 16 a lane.  Where a row goes:
+//   * without `place_of_slot`, row m to place m / run * cap + m % run: the rows of a run of the product lie together, at its start;
+//   * with `place_of_slot`, row m to the places of its slots top m .. top m + top - 1, nowhere for those that are negative; with `place_scale` a place
+//     also gets its slot's weight.
 // The scales of a run's places: [run][piece][group of 128 places].
 template <typename T>
 __global__ void __launch_bounds__(256) code_rows_kernel(const CodeRowsArgs a) {
   const int lane = threadIdx.x & 31, pieces = b8_pieces(a.K);
   const long long task = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const long long index = task / pieces;
+  const long long row = task / pieces;
   const int piece = static_cast<int>(task % pieces);
   wait_for_prior_grids();
   let_dependents_launch();
   if (task * 32 + lane < a.zero_count) a.zeros[task * 32 + lane] = 0;
-  if (index >= a.rows) return;
-  long long row = index, place = index;
-  if (a.place_of_slot != nullptr) {
-    place = a.place_of_slot[index];
-    if (place < 0) return;
-    row = index / a.top;
-    if (a.place_scale != nullptr && piece == 0 && lane == 0) a.place_scale[place] = a.weights[index];
-  } else {
-    place = index / a.run * a.cap + index % a.run;
-  }
+  if (row >= a.rows) return;
   const int k = piece * 512 + lane * 16;
   B8Values<T> v;
   v.load(static_cast<const T*>(a.x) + row * a.ldx + k, a.K - k, a.wide);
+  int places = lane < a.top ? *(a.place_of_slot + row * a.top + lane) : -1;
   unsigned byte;
   const uint4 codes = b8_code_row_piece(v, byte);
   const unsigned scales = b8_four_bytes(byte);
-  const int pitch = b8_pitch(a.K);
-  if (k < pitch) *reinterpret_cast<uint4*>(a.codes + place * pitch + k) = codes;
-  if (lane == 0) {
-    const int groups = (a.cap + 127) / 128, own = static_cast<int>(place % a.cap), r = own % 128;
-    *reinterpret_cast<unsigned*>(a.scales + ((place / a.cap * pieces + piece) * groups + own / 128) * B8_PIECE + r % 32 * 16 + r / 32 * 4) = scales;
+  const int pitch = b8_pitch(a.K), groups = (a.cap + 127) / 128;
+  auto put = [&](long long place) {
+    if (k < pitch) *reinterpret_cast<uint4*>(a.codes + place * pitch + k) = codes;
+    if (lane == 0) {
+      const int own = static_cast<int>(place % a.cap), r = own % 128;
+      *reinterpret_cast<unsigned*>(a.scales + ((place / a.cap * pieces + piece) * groups + own / 128) * B8_PIECE + r % 32 * 16 + r / 32 * 4) = scales;
+    }
+  };
+  if (a.place_of_slot == nullptr) put(row / a.run * a.cap + row % a.run);
+  for (int j0 = 0; j0 < a.top; j0 += 32) {          // (without places `top` is 0)
+    if (j0 > 0) places = j0 + lane < a.top ? *(a.place_of_slot + row * a.top + j0 + lane) : -1;
+    if (a.place_scale != nullptr && piece == 0 && places >= 0) a.place_scale[places] = a.weights[row * a.top + j0 + lane];
+    for (int j = 0; j < min(32, a.top - j0); ++j) {
+      const int place = __shfl_sync(0xffffffffu, places, j);
+      if (place >= 0) put(place);
+    }
   }
 }
 
 // Runs of a routed layer's rows: an expert's slots (choices) are cut into as few runs as `run` rows allow, of equal length (a multiple of 16), whose places
 // begin `run` apart.  plan[0]: the number of runs; then per run its expert, first place and rows.  One CTA; which place a slot gets inside its
-// expert's runs depends on the order of arrival, no result does.  A thread asks for eight slots' experts at once.
-// Each warp counts for itself (one table of counters for all warps would have 32 of them take turns at an expert's); then an
-// expert's counts become its first numbers, warp by warp.
+// expert's runs depends on the order of arrival, no result does.  A thread asks for eight slots' experts at once, and keeps their numbers among their warp's in
+// place_of_slot until the warps' counts are known.  Each warp counts for itself (one table of counters for all warps would have 32 of them take turns at an
+// expert's); then an expert's counts become its first numbers, warp by warp.
 constexpr int B8_PLAN_THREADS = 1024, B8_PLAN_WARPS = B8_PLAN_THREADS / 32, B8_PLAN_BATCH = 8;
 __global__ void __launch_bounds__(B8_PLAN_THREADS)
 block8_plan_kernel(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run) {
@@ -202,32 +205,27 @@ block8_plan_kernel(int* plan, int* place_of_slot, const int* ids, int num_slots,
   for (int i = threadIdx.x; i < B8_PLAN_WARPS * experts; i += B8_PLAN_THREADS) counts[i] = 0;
   __syncthreads();
   int* own = counts + warp * experts;
-  // The number of each of the thread's slots among its expert's, as far as this warp has them: use(slot, expert or -1, number).
-  auto each = [&](auto use) {
+  // Of each of the thread's slots: load(slot) for eight at a time, then use(slot, expert or -1, what was loaded).
+  auto each = [&](auto load, auto use) {
     for (int base = 0; base < num_slots; base += B8_PLAN_THREADS * B8_PLAN_BATCH) {
-      int e[B8_PLAN_BATCH];
+      int e[B8_PLAN_BATCH], loaded[B8_PLAN_BATCH];
 #pragma unroll
       for (int j = 0; j < B8_PLAN_BATCH; ++j) {
         const int i = base + j * B8_PLAN_THREADS + threadIdx.x;
         e[j] = i < num_slots ? ids[i] : -1;
-        if (e[j] < 0 || e[j] >= experts) e[j] = -1;
+        loaded[j] = i < num_slots ? load(i) : 0;
+        if (e[j] >= experts) e[j] = -1;
       }
 #pragma unroll
       for (int j = 0; j < B8_PLAN_BATCH; ++j) {
-        if (base + j * B8_PLAN_THREADS + 32 * warp >= num_slots) break;
-        const unsigned same = __match_any_sync(0xffffffffu, e[j]);
-        const int first = __ffs(same) - 1;
-        int before = 0;
-        if (e[j] >= 0 && lane == first) {
-          before = own[e[j]];
-          own[e[j]] = before + __popc(same);
-        }
-        __syncwarp();
-        use(base + j * B8_PLAN_THREADS + static_cast<int>(threadIdx.x), e[j], __shfl_sync(0xffffffffu, before, first) + __popc(same & ((1u << lane) - 1)));
+        const int i = base + j * B8_PLAN_THREADS + threadIdx.x;
+        if (i < num_slots) use(i, e[j], loaded[j]);
       }
     }
   };
-  each([](int, int, int) {});
+  each([](int) { return 0; }, [&](int slot, int e, int) {
+    if (e >= 0) place_of_slot[slot] = atomicAdd(own + e, 1);
+  });
   __syncthreads();
   for (int e = threadIdx.x; e < experts; e += B8_PLAN_THREADS) {
     int sum = 0;
@@ -266,8 +264,9 @@ block8_plan_kernel(int* plan, int* place_of_slot, const int* ids, int num_slots,
     if (lane == 0) plan[0] = runs;
   }
   __syncthreads();
-  each([&](int slot, int e, int nth) {
-    if (slot < num_slots) place_of_slot[slot] = e >= 0 ? start[e] + nth / length[e] * run + nth % length[e] : -1;
+  each([&](int slot) { return place_of_slot[slot]; }, [&](int slot, int e, int nth) {
+    if (e >= 0) nth += own[e];
+    place_of_slot[slot] = e >= 0 ? start[e] + nth / length[e] * run + nth % length[e] : -1;
   });
 }
 

@@ -58,7 +58,7 @@ struct CodeRowsArgs {
   const void* x;
   long long ldx;
   const int* place_of_slot;
-  int rows, K, run, cap, top;          // `rows`: of x, or slots
+  int rows, K, run, cap, top;          // `top`: slots a row, 0 without places
   float* place_scale;
   const float* weights;
   int* zeros;                          // what a later kernel finds as zeros, or null

@@ -172,7 +172,7 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
   const int zeros = parts != nullptr ? static_cast<int>(2 * FLAGS) : 0;
   int rc = block8_plan(plan, place_of_slot, e.ids, num_slots, e.E, cap, stream);
   if (rc != OK) return rc;
-  rc = block8_code_rows({codes, scales, e.x, e.ldx, place_of_slot, num_slots, e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
+  rc = block8_code_rows({codes, scales, e.x, e.ldx, place_of_slot, e.T, e.width, cap, cap, e.top, place_scale, e.weights, flags, zeros, false}, e.dtype, stream);
   if (rc != OK) return rc;
   rc = block8_product({hidden_codes, e.ff, DTYPE_F32, hidden_scales, codes, scales, up.codes, up.scales, plan, runs, e.E, 0, cap, cap, up.N, up.K, g.kind, nullptr, place_scale, g.limit,
                        g.alpha, g.shift, false, parts, flags, LEAST_BLOCKS, status}, stream);
