@@ -393,9 +393,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_edge), 0));
         }
       };
-      // A warp's chunks of 32 columns, the first and the last one first.
-      auto chunk = [](int s) { return s == 0 ? 0 : s == 1 ? CHUNKS - 1 : s - 1; };
-      constexpr int EDGE = CHUNKS > 1 ? 1 : 0;      // behind which the edge is free
+      // A warp's chunks of 32 columns, the one that may lie on the edge first.
+      const bool last_first = RUN == 256 && acc == 0;
+      auto chunk = [&](int s) { return last_first ? (s == 0 ? CHUNKS - 1 : s - 1) : s; };
       auto free_accumulator = [&]() {
         tc_fence_before_sync();
         __syncwarp();
@@ -483,10 +483,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
         auto gate_pairs = [&](auto activation) {
 #pragma unroll
           for (int s = 0; s < CHUNKS; ++s) {
-            const int j = chunk(s), c = COLUMNS * j + 32 * group;
+            const int c = COLUMNS * chunk(s) + 32 * group;
             if (c < run.rows) {
               unsigned v[32];
               read_sums(c, v);
+              if (s == 0) free_edge();
               const float* scale = SCALED ? a.gate.row_scale + run.place + c + own_row : nullptr;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -498,10 +499,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
                   gate *= s;
                   up *= s;
                 }
-                hidden[j][i] = row < a.N ? activation(gate, up) : 0.0f;
+                hidden[s][i] = row < a.N ? activation(gate, up) : 0.0f;
               }
+            } else if (s == 0) {
+              free_edge();
             }
-            if (s == EDGE) free_edge();
           }
         };
         if (a.gate.kind == GATE_SILU) gate_pairs([](float gate, float up) { return silu_fast(gate) * up; });
@@ -511,11 +513,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
         if constexpr (!CODED) {
           TOut* y = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + own_row) * a.ldy + column0 + own_column;
 #pragma unroll
-          for (int j = 0; j < CHUNKS; ++j) {
-            const int c = COLUMNS * j + 32 * group;
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int c = COLUMNS * chunk(s) + 32 * group;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (c + own_row + i < run.rows && column0 + own_column < width) y[static_cast<size_t>(c + i) * a.ldy] = from_float<TOut>(hidden[j][i]);
+              if (c + own_row + i < run.rows && column0 + own_column < width) y[static_cast<size_t>(c + i) * a.ldy] = from_float<TOut>(hidden[s][i]);
           }
         } else {
           // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
@@ -524,12 +526,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + peaks_phase * 8 * RUN;
           const int mine = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
 #pragma unroll
-          for (int j = 0; j < CHUNKS; ++j) {
-            const int c = COLUMNS * j + 32 * group;
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int c = COLUMNS * chunk(s) + 32 * group;
             if (c < run.rows) {
               unsigned m[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) m[i] = b8_magnitude(hidden[j][i]);
+              for (int i = 0; i < 16; ++i) m[i] = b8_magnitude(hidden[s][i]);
               auto meet = [&](int bit, int count) {     // with the lane across `bit`: each keeps half of the rows
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -560,8 +562,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           const int block = item / runs, pitch = b8_pitch(width), hidden_pieces = b8_pieces(width);
           unsigned char* codes_at = static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place) * pitch + block * 128 + rank * 64 + quarter * 16;
 #pragma unroll
-          for (int j = 0; j < CHUNKS; ++j) {
-            const int c = COLUMNS * j + 32 * group;
+          for (int s = 0; s < CHUNKS; ++s) {
+            const int c = COLUMNS * chunk(s) + 32 * group;
             if (c < run.rows) {
               unsigned largest = 0;
 #pragma unroll
@@ -572,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
               for (int i = 0; i < 16; i += 2) {
                 const int from = (lane & 8) | (i & 8) << 1 | (i & 7);
                 const float one = __shfl_sync(0xffffffffu, inverse, from), two = __shfl_sync(0xffffffffu, inverse, from + 1);
-                const unsigned codes = b8_two_codes(hidden[j][i], one, hidden[j][i + 1], two);
+                const unsigned codes = b8_two_codes(hidden[s][i], one, hidden[s][i + 1], two);
                 unsigned char* to = bytes + (own_row + i) * 16 + own_column;
                 to[0] = static_cast<unsigned char>(codes);
                 to[16] = static_cast<unsigned char>(codes >> 8);
@@ -610,7 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
                 }
               }
             }
-            if (s == EDGE) free_edge();
+            if (s == 0) free_edge();
             if (s == CHUNKS - 1) free_accumulator();
             if (rows <= 0) continue;
             // A run's last rows may be followed by another run's (without a plan): those go out one by one.
@@ -634,16 +636,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
               }
               ++stores;
             } else {
-              [[maybe_unused]] const int pair_row = lane & 1, column = row & ~1;
-              TOut* at = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + c) * a.ldy;
+              const int first = sizeof(TOut) == 2 ? lane & 1 : 0, step = sizeof(TOut) == 2 ? 2 : 1, column = sizeof(TOut) == 2 ? row & ~1 : row;
+              TOut* at = static_cast<TOut*>(a.y) + static_cast<size_t>(run.out + c + first) * a.ldy + column;
 #pragma unroll
-              for (int i = 0; i < WORDS; ++i) {
+              for (int i = 0; i < WORDS; ++i, at += step * a.ldy) {
+                if (first + step * i >= rows) continue;
                 if constexpr (sizeof(TOut) == 2) {
-                  unsigned short* bits = reinterpret_cast<unsigned short*>(at) + static_cast<size_t>(2 * i + pair_row) * a.ldy + column;
-                  if (2 * i + pair_row < rows && column < a.N) bits[0] = static_cast<unsigned short>(out[i]);
-                  if (2 * i + pair_row < rows && column + 1 < a.N) bits[1] = static_cast<unsigned short>(out[i] >> 16);
+                  unsigned short* bits = reinterpret_cast<unsigned short*>(at);
+                  if (column < a.N) bits[0] = static_cast<unsigned short>(out[i]);
+                  if (column + 1 < a.N) bits[1] = static_cast<unsigned short>(out[i] >> 16);
                 } else {
-                  if (i < rows && row < a.N) at[static_cast<size_t>(i) * a.ldy + row] = __uint_as_float(out[i]);
+                  if (column < a.N) *at = __uint_as_float(out[i]);
                 }
               }
             }
