@@ -276,7 +276,7 @@ static bool b8_aligned(const void* p, int bytes) { return reinterpret_cast<uintp
 int block8_plan(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run, cudaStream_t stream) {
   const size_t smem = (3 + B8_PLAN_WARPS) * static_cast<size_t>(experts) * sizeof(int);
   if (smem > 224 * 1024) return ERR_UNSUPPORTED;              // (1638 experts)
-  if (cuda_failed(cudaFuncSetAttribute(block8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
+  if (smem > 48 * 1024 && cuda_failed(cudaFuncSetAttribute(block8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
   return launch_dependent(block8_plan_kernel, dim3(1), dim3(B8_PLAN_THREADS), smem, stream, false, plan, place_of_slot, ids, num_slots, experts, run);
 }
 

@@ -22,14 +22,14 @@ struct Pieces {
   }
 };
 
-// Whether few rows go to the kernel that streams the matrix.  It has four warps or sixteen on a tile, the tensor cores' kernel waits for a tile's whole K:
-// up to 8 rows it is ahead or level everywhere (8 rows, us, streaming / tensor cores: 24576 x 4096 21.3 / 25.2, 51200 x 5120 45.3 / 46.0), up to 16, which take twice its
-// instructions, where the matrix is small (16 rows: 4096 x 4096 9.3 / 12.4, 24576 x 4096 24.0 / 26.0, but 10240 x 5120 18.5 / 16.0).
-constexpr long long STREAM_VALUES = 28LL << 20;
-static bool streams(int M, int N, int K) { return block8_small_fits(M, K) && (M <= 8 || static_cast<long long>(N) * K <= STREAM_VALUES); }
-// Whether its rows are coded by a kernel ahead of it instead of in every CTA for itself (8 rows, us, ahead / in each: K = 1024 4.6 / 4.3, 4096 7.6 / 8.0,
-// 12288 13.3 / 18.5).
-static bool coded_ahead(int M, int K) { return M <= 8 && b8_pieces(K) * M >= 64; }
+// Whether few rows go to the kernel that streams the matrix: wherever their codes fit beside its rings (up to 16 rows; K up to 7936 for more than 8).  It has four
+// warps or sixteen on a tile, where the tensor cores' kernel waits for a tile's whole K on one SM in a pair (us, streaming / tensor cores: 8 rows 24576 x 4096
+// 21.3 / 25.2, 51200 x 5120 45.3 / 46.0; 16 rows 4096 x 4096 7.8 / 13.6, 8192 x 4096 10.6 / 13.9, 10240 x 5120 16.5 / 16.5, 28672 x 4096 27.4 / 27.3).
+static bool streams(int M, int K) { return block8_small_fits(M, K); }
+// Whether its rows are coded by a kernel ahead of it instead of in every CTA for itself, which reads them from L2 as often as there are CTAs (us, ahead / in each,
+// bfloat16 rows: 8 x 4096 x 4096 6.8 / 6.7, 16 x 4096 x 4096 7.8 / 9.1, 8 x 1024 x 6144 5.4 / 6.8, 16 x 1024 x 2048 4.7 / 4.3; float32: 8 x 1024 x 3072
+// 4.9 / 5.5, 8 x 1024 x 2048 4.3 / 4.2).
+static bool coded_ahead(int M, int K, int x_dtype) { return b8_pieces(K) * M >= (x_dtype == DTYPE_F32 ? 48 : 72); }
 
 constexpr int LEAST_BLOCKS = 8;
 
@@ -85,9 +85,9 @@ struct Gate {
 // y [M, N, or N / 2 gated] = x w^T.  `final`: a float32 result is what the caller asked for (hidden values are coded next).
 static int product(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& w, int M, const Gate& g,
                    bool final, int* status, cudaStream_t stream) {
-  if (streams(M, w.N, w.K)) {
+  if (streams(M, w.K)) {
     Block8Small s = {y, ldy, y_dtype, x, nullptr, ldx, x_dtype, w.codes, w.scales, M, w.N, w.K, g.kind, g.bias, g.limit, g.alpha, g.shift, status};
-    if (coded_ahead(M, w.K)) {
+    if (coded_ahead(M, w.K, x_dtype)) {
       unsigned char* codes = memory.take<unsigned char>(64LL * b8_pitch(w.K));
       unsigned char* scales = memory.take<unsigned char>(static_cast<long long>(b8_pieces(w.K)) * B8_PIECE);
       if (memory.base == nullptr) return OK;
@@ -109,11 +109,11 @@ static int product(Pieces& memory, void* y, long long ldy, int y_dtype, const vo
 }
 
 // Whether a feed-forward's hidden values go from the first product's kernel to the second's as codes.
-static bool hands_codes_on(int M, const Operand& up, const Operand& down) { return !streams(M, up.N, up.K) && !streams(M, down.N, down.K); }
+static bool hands_codes_on(int M, int K, int ff) { return !streams(M, K) && !streams(M, ff); }
 
 static int feed_forward(Pieces& memory, void* y, long long ldy, int y_dtype, const void* x, long long ldx, int x_dtype, const Operand& up, const Operand& down,
                         int M, const Gate& g, int* status, cudaStream_t stream) {
-  if (!hands_codes_on(M, up, down)) {
+  if (!hands_codes_on(M, up.K, down.K)) {
     float* hidden = memory.take<float>(static_cast<long long>(M) * down.K);
     const int rc = product(memory, hidden, down.K, DTYPE_F32, x, ldx, x_dtype, up, M, g, false, status, stream);
     if (rc != OK) return rc;
@@ -183,7 +183,7 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
   return zb_route_combine(e.y, out, e.width, e.dtype, e.x, e.ldx, e.ids, e.weigh_inputs ? nullptr : e.weights, place_of_slot, e.T, e.width, e.top, e.dtype, stream);
 }
 
-static bool sizes_ok(long long a, long long b, long long c) { return a > 0 && b > 0 && c > 0 && a < (1LL << 31) && b < (1LL << 31) && c < (1LL << 31) - 512; }
+static bool sizes_ok(long long a, long long b, long long c) { return a > 0 && b > 0 && c > 0 && a < (1LL << 31) - 512 && b < (1LL << 31) - 512 && c < (1LL << 31) - 512; }
 static bool gate_ok(long long kind, long long N, double limit, const float* bias, bool gated) {
   if (gated != (kind >= 1 && kind <= 3)) return false;
   return kind >= 0 && kind <= 5 && (!gated || N % 16 == 0) && (kind != 3 || limit > 0.0) && (kind == 3 || bias == nullptr);
@@ -211,9 +211,9 @@ static Gate gate_of(long long kind, const float* bias, double limit, double alph
   return {static_cast<int>(kind), bias, static_cast<float>(limit), static_cast<float>(alpha), static_cast<float>(shift)};
 }
 
-ZB_API long long zb_block8_product_work(long long M, long long N, long long K, int y_dtype) {
+ZB_API long long zb_block8_product_work(long long M, long long N, long long K, int x_dtype, int y_dtype) {
   Pieces memory{nullptr};
-  product(memory, nullptr, 0, y_dtype, nullptr, 0, 0, {nullptr, nullptr, static_cast<int>(N), static_cast<int>(K)}, static_cast<int>(M), {}, true, nullptr, nullptr);
+  product(memory, nullptr, 0, y_dtype, nullptr, 0, x_dtype, {nullptr, nullptr, static_cast<int>(N), static_cast<int>(K)}, static_cast<int>(M), {}, true, nullptr, nullptr);
   return memory.at;
 }
 ZB_API int zb_block8_product(const void* call) {
@@ -226,18 +226,18 @@ ZB_API int zb_block8_product(const void* call) {
                  static_cast<int>(c.M), gate_of(c.kind, c.bias, c.limit, c.alpha, c.shift), true, c.status, static_cast<cudaStream_t>(c.stream));
 }
 // How many kernels the call launches.
-ZB_API int zb_block8_product_kernels(int M, int N, int K) { return streams(M, N, K) && !coded_ahead(M, K) ? 1 : 2; }
+ZB_API int zb_block8_product_kernels(int M, int K, int x_dtype) { return streams(M, K) && !coded_ahead(M, K, x_dtype) ? 1 : 2; }
 
-ZB_API long long zb_block8_feed_forward_work(long long M, long long K, long long ff, long long N, int y_dtype) {
+ZB_API long long zb_block8_feed_forward_work(long long M, long long K, long long ff, long long N, int x_dtype, int y_dtype) {
   Pieces memory{nullptr};
-  feed_forward(memory, nullptr, 0, y_dtype, nullptr, 0, 0, {nullptr, nullptr, static_cast<int>(2 * ff), static_cast<int>(K)},
+  feed_forward(memory, nullptr, 0, y_dtype, nullptr, 0, x_dtype, {nullptr, nullptr, static_cast<int>(2 * ff), static_cast<int>(K)},
                {nullptr, nullptr, static_cast<int>(N), static_cast<int>(ff)}, static_cast<int>(M), {}, nullptr, nullptr);
   return memory.at;
 }
 // How many kernels the call launches.
-ZB_API int zb_block8_feed_forward_kernels(int M, int K, int ff, int N) {
-  if (hands_codes_on(M, {nullptr, nullptr, 2 * ff, K}, {nullptr, nullptr, N, ff})) return 3;
-  return zb_block8_product_kernels(M, 2 * ff, K) + zb_block8_product_kernels(M, N, ff);
+ZB_API int zb_block8_feed_forward_kernels(int M, int K, int ff, int x_dtype) {
+  if (hands_codes_on(M, K, ff)) return 3;
+  return zb_block8_product_kernels(M, K, x_dtype) + zb_block8_product_kernels(M, ff, DTYPE_F32);
 }
 ZB_API int zb_block8_feed_forward(const void* call) {
   const FeedForwardCall& c = *static_cast<const FeedForwardCall*>(call);

@@ -1,6 +1,6 @@
 // Products of matrices and rows in 8-bit floating point with a scale for each block of 128 (block8.cuh) for the few rows of a decode step
-// (M <= 16): a weight streamer.  One launch takes the rows as they are, bfloat16 or float32, codes them on the way (each CTA for itself,
-// 8 rows of 4096: 64 values a thread) and reads every weight once.
+// (M <= 16): a weight streamer.  It reads every weight once, and takes the rows as they are, bfloat16 or float32, and codes them on the way (each CTA for
+// itself, 8 rows of 4096: 64 values a thread), or as codes where they are many and long.
 //
 // The matrix's rows sit on the 16-row side of m16n8k16, the tokens on the 8-column side.  Inside a half block of 64 k, lane t of a quad owns the 16
 // values k = 16 t .. 16 t + 15 of its row: one 16-byte piece feeds four products, which see k in a permuted order, the same for both operands.  The
@@ -13,6 +13,7 @@
 // memory let the next kernel's CTA lie beside this one's with its first copies on their way.  Partial sums meet in shared memory, in two buffers that
 // take turns, and are added in a fixed order.
 #include <algorithm>
+#include <atomic>
 
 #include "block8.cuh"
 #include "mma.cuh"
@@ -112,7 +113,7 @@ __device__ __forceinline__ void finish_tile(const Block8SmallArgs& a, int n0, in
   }
 }
 
-// CODED: x comes as zb_code_rows leaves it.
+// CODED: x comes as code_rows_kernel leaves it.
 template <int MT, int TEAM, bool CODED, typename TOut, bool GATED>
 __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_small_kernel(const __grid_constant__ Block8SmallArgs a) {
   constexpr int TEAMS = G9_WARPS / TEAM, SUMS = MT * 128;
@@ -160,7 +161,6 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
   bool gave_up = false;
   wait_for_prior_grids();
   let_dependents_launch();
-  // (Tokens that are not there are columns of the products that nobody reads, whatever lies in their places.)
   // (Tokens that are not there are columns of the products that nobody reads, whatever lies in their places.)
   if (CODED) {
     unsigned long long* x_bar = bars + G9_WARPS * G9_DEPTH;
@@ -273,19 +273,22 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
 template <int MT, int TEAM, bool CODED, typename TOut, bool GATED>
 int block8_small_launch(const Block8SmallArgs& a, cudaStream_t stream) {
   auto kernel = gemm_block8_small_kernel<MT, TEAM, CODED, TOut, GATED>;
-  const size_t smem = block8_small_smem(b8_blocks(a.K), MT);
-  if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))) return ERR_CUDA;
-  return launch_dependent(kernel, dim3(std::min(148, (a.N + 15) / 16)), dim3(G9_WARPS * 32), smem, stream, false, a);
+  static std::atomic<bool> allowed[64];             // by device: saying it takes the host 0.5 us
+  int device = 0;
+  if (cuda_failed(cudaGetDevice(&device))) return ERR_CUDA;
+  if (device >= 64 || !allowed[device].load()) {
+    if (cuda_failed(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(G9_SMEM)))) return ERR_CUDA;
+    if (device < 64) allowed[device].store(true);
+  }
+  return launch_dependent(kernel, dim3(std::min(148, (a.N + 15) / 16)), dim3(G9_WARPS * 32), block8_small_smem(b8_blocks(a.K), MT), stream, false, a);
 }
 // All 16 warps on a tile where no SM has more than two of them and K has blocks enough; else four (8 rows, us, 16 warps / four: 1024 x 2048
 // 4.0 / 4.6, 1024 x 4096 5.2 / 6.2, 4096 x 4096 8.0 / 8.2, 4096 x 12288 13.3 / 15.6; 4096 x 1024 5.3 / 4.4, 6144 x 4096 10.1 / 9.1, 24576 x 4096 22.9 / 21.5).
 template <int MT, typename TOut, bool GATED>
 int block8_small_team(const Block8SmallArgs& a, cudaStream_t stream) {
   const bool all = ((a.N + 15) / 16 <= 2 * 148 && b8_blocks(a.K) >= 16) || b8_blocks(a.K) > 4 * G9_MAX_BLOCKS;
-  if constexpr (MT == 1) {                   // (more rows of which the codes would pay have the tensor cores' kernel)
-    if (a.x_scales != nullptr)
-      return all ? block8_small_launch<MT, 16, true, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, true, TOut, GATED>(a, stream);
-  }
+  if (a.x_scales != nullptr)
+    return all ? block8_small_launch<MT, 16, true, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, true, TOut, GATED>(a, stream);
   return all ? block8_small_launch<MT, 16, false, TOut, GATED>(a, stream) : block8_small_launch<MT, 4, false, TOut, GATED>(a, stream);
 }
 template <typename TOut, bool GATED>
@@ -297,10 +300,10 @@ bool block8_small_fits(int M, int K) {
   return M >= 1 && M <= 16 && K >= 1 && block8_small_smem(b8_blocks(K), (M + 7) / 8) <= G9_SMEM && b8_blocks(K) <= 16 * G9_MAX_BLOCKS;
 }
 
-// y = x w^T in blocks for up to 16 rows of x as they are (bfloat16 or float32), or with `x_scales` for up to 8 as codes.
+// y = x w^T in blocks for up to 16 rows of x as they are (bfloat16 or float32), or with `x_scales` as codes.
 int block8_small_product(const Block8Small& p, cudaStream_t stream) {
   const bool gated = p.kind >= 1 && p.kind <= 3;
-  if (!block8_small_fits(p.M, p.K) || (p.x_scales != nullptr && p.M > 8) || b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K) >= (1LL << 31)) return ERR_UNSUPPORTED;
+  if (!block8_small_fits(p.M, p.K) || b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K) >= (1LL << 31)) return ERR_UNSUPPORTED;
   Block8SmallArgs a = {};
   a.y = p.y; a.ldy = p.ldy; a.x = p.x; a.ldx = p.ldx; a.x_dtype = p.x_dtype;
   if (!byte_rows_map(&a.w_map, p.w_codes, b8_block_row(0, b8_blocks(p.N), 0, p.N, p.K), 128, 128, 16, true)) return ERR_CUDA;

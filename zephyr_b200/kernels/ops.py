@@ -267,8 +267,8 @@ def library() -> ctypes.CDLL:
             lib.zb_paged_decode_balanced_scratch_floats.restype = c_longlong
             lib.zb_paged_decode_packed_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
             lib.zb_paged_decode_packed_scratch_floats.restype = c_longlong
-            lib.zb_block8_product_work.argtypes = [c_longlong, c_longlong, c_longlong, c_int]
-            lib.zb_block8_feed_forward_work.argtypes = [c_longlong, c_longlong, c_longlong, c_longlong, c_int]
+            lib.zb_block8_product_work.argtypes = [c_longlong, c_longlong, c_longlong, c_int, c_int]
+            lib.zb_block8_feed_forward_work.argtypes = [c_longlong, c_longlong, c_longlong, c_longlong, c_int, c_int]
             lib.zb_block8_experts_work.argtypes = [c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, c_int]
             for name in ("zb_block8_product_work", "zb_block8_feed_forward_work", "zb_block8_experts_work"):
                 getattr(lib, name).restype = c_longlong
@@ -2660,7 +2660,7 @@ class BlockMatrix:
         """What the codes stand for (exact in bfloat16 but below its normal numbers)."""
         if dtype not in DTYPE_CODE:
             raise InvalidArgumentError("values are bfloat16 or float32")
-        out = torch.empty(self.shape, dtype=dtype, device=self.data.device)
+        out = torch.empty(*self.shape, dtype=dtype, device=self.data.device)
         (out_at, _), place = _addresses(out, self.data)
         _check_place(place)
         _check(library().zb_matrix_values(out_at, self.codes_at, self.scales_at, self.matrices, self.N, self.K, DTYPE_CODE[dtype], _stream()), "matrix_values")
@@ -2689,6 +2689,8 @@ def _check_block8_rows(x: torch.Tensor, K: int) -> int:
     shape = x.shape
     if len(shape) != 2 or shape[1] != K or x.dtype not in DTYPE_CODE:
         raise InvalidArgumentError(f"x must be [M, {K}] in bfloat16 or float32, not {list(shape)} in {x.dtype}")
+    if shape[0] >= 2 ** 31 - 512:
+        raise InvalidArgumentError("rows that 32 bits can count")
     pitch, inner = x.stride()
     if shape[0] <= 1:
         pitch = K
@@ -2704,15 +2706,16 @@ _BLOCK8_EXPERTS = struct.Struct("=2Q2q6Q7q3d3Q").pack
 
 
 @functools.lru_cache(maxsize=4096)
-def _block8_product_plan(M: int, N: int, K: int, y_code: int) -> tuple[int, int]:
+def _block8_product_plan(M: int, N: int, K: int, x_code: int, y_code: int) -> tuple[int, int]:
     """The bytes between a product's kernels, and how many kernels."""
-    return library().zb_block8_product_work(M, N, K, y_code), library().zb_block8_product_kernels(M, N, K)
+    lib = library()
+    return lib.zb_block8_product_work(M, N, K, x_code, y_code), lib.zb_block8_product_kernels(M, K, x_code)
 
 
 @functools.lru_cache(maxsize=4096)
-def _block8_feed_forward_plan(M: int, K: int, ff: int, N: int, y_code: int) -> tuple[int, int]:
+def _block8_feed_forward_plan(M: int, K: int, ff: int, N: int, x_code: int, y_code: int) -> tuple[int, int]:
     lib = library()
-    return lib.zb_block8_feed_forward_work(M, K, ff, N, y_code), lib.zb_block8_feed_forward_kernels(M, K, ff, N)
+    return lib.zb_block8_feed_forward_work(M, K, ff, N, x_code, y_code), lib.zb_block8_feed_forward_kernels(M, K, ff, x_code)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2735,8 +2738,8 @@ def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None 
     """x [M, K] (bfloat16 or float32) times a matrix [N, K] in 8-bit floating point: x's rows are coded as the matrix is, in blocks of 128
     values, and y[m, n] = sum_k x~[m, k] w~[n, k] over what the codes stand for, summed in float32, in ``out_dtype`` (None: x's).  ``swiglu``: the rows of w are
     blocks of 8 gate rows and their 8 up rows, and the result is act(gate) * up (``act`` "silu" or "relu"; ``bounded``: the bounded gate), [M, N /
-    2]; ``product_act`` (without ``swiglu``): one of ``PRODUCT_ACTS`` of the sums.  Up to 16 rows of a matrix that is not large are coded inside the
-    product's kernel, which streams the matrix; others by a kernel of their own ahead of it."""
+    2]; ``product_act`` (without ``swiglu``): one of ``PRODUCT_ACTS`` of the sums.  A few short rows are coded inside the product's
+    kernel, others by a kernel of their own ahead of it."""
     if len(w.shape) != 2:
         raise InvalidArgumentError("a product takes one matrix")
     pitch = _check_block8_rows(x, w.K)
@@ -2755,14 +2758,14 @@ def block_linear(x: torch.Tensor, w: BlockMatrix, out_dtype: torch.dtype | None 
         gate = (3 + PRODUCT_ACTS[product_act], 0, 0.0, 1.0, 0.0)
     (x_at, _, _), place = _addresses(x, w.data, bounded.bias if bounded is not None else None)
     _check_place(place)
-    width, y_code = N // 2 if swiglu else N, DTYPE_CODE[out_dtype]
-    out = torch.empty((M, width), dtype=out_dtype, device=x.device)
+    width, x_code, y_code = N // 2 if swiglu else N, DTYPE_CODE[x.dtype], DTYPE_CODE[out_dtype]
+    out = torch.empty(M, width, dtype=out_dtype, device=x.device)
     if M == 0:
         return out
-    bytes_, kernels = _block8_product_plan(M, N, w.K, y_code)
+    bytes_, kernels = _block8_product_plan(M, N, w.K, x_code, y_code)
     work = torch.empty(bytes_, dtype=torch.uint8, device=x.device) if bytes_ else None
     _check(library().zb_block8_product(_BLOCK8_PRODUCT(
-        out.data_ptr(), width, y_code, x_at, pitch, DTYPE_CODE[x.dtype], w.codes_at, w.scales_at, M, N, w.K, *gate, work.data_ptr() if bytes_ else 0,
+        out.data_ptr(), width, y_code, x_at, pitch, x_code, w.codes_at, w.scales_at, M, N, w.K, *gate, work.data_ptr() if bytes_ else 0,
         _device_status_pointer(x.device) or 0, _stream())), "block_linear", kernels)
     return out
 
@@ -2782,14 +2785,14 @@ def block_feed_forward(x: torch.Tensor, gate_up: BlockMatrix, down: BlockMatrix,
     gate = _block8_gate(gate_up.N, act, bounded)
     (x_at, _, _, _), place = _addresses(x, gate_up.data, down.data, bounded.bias if bounded is not None else None)
     _check_place(place)
-    y_code = DTYPE_CODE[out_dtype]
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    x_code, y_code = DTYPE_CODE[x.dtype], DTYPE_CODE[out_dtype]
+    out = torch.empty(M, N, dtype=out_dtype, device=x.device)
     if M == 0:
         return out
-    bytes_, kernels = _block8_feed_forward_plan(M, gate_up.K, ff, N, y_code)
+    bytes_, kernels = _block8_feed_forward_plan(M, gate_up.K, ff, N, x_code, y_code)
     work = torch.empty(bytes_, dtype=torch.uint8, device=x.device)
     _check(library().zb_block8_feed_forward(_BLOCK8_FEED_FORWARD(
-        out.data_ptr(), N, y_code, x_at, pitch, DTYPE_CODE[x.dtype], gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, M, gate_up.K, ff, N,
+        out.data_ptr(), N, y_code, x_at, pitch, x_code, gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, M, gate_up.K, ff, N,
         *gate, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "block_feed_forward", kernels)
     return out
 
@@ -2804,9 +2807,11 @@ def _routed_blocks(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ga
     kind, _, *bounds = _block8_gate(gate_up.N, act, bounded)
     (x_at, ids_at, weights_at, _, _), place = _addresses(x, ids, weights, gate_up.data, down.data)
     _check_place(place)
-    out = torch.empty((T, width), dtype=x.dtype, device=x.device)
+    out = torch.empty(T, width, dtype=x.dtype, device=x.device)
     if T == 0 or top == 0:
         return out.zero_()
+    if T * top >= 2 ** 31 - 512:
+        raise InvalidArgumentError("choices that 32 bits can count")
     code = DTYPE_CODE[x.dtype]
     work = torch.empty(_block8_experts_work(T, top, E, width, ff, code, weigh_inputs), dtype=torch.uint8, device=x.device)
     _check(library().zb_block8_experts(_BLOCK8_EXPERTS(
