@@ -210,3 +210,14 @@ def test_a_captured_run_of_products(cuda_device):
             for got in results:
                 assert all(torch.equal(a, b) for a, b in zip(got, eager))
     ops.check_status(ops.device_status("cuda"))
+
+
+def test_the_timing_program_times_it(cuda_device, capsys):
+    import json
+
+    from zephyr_b200.kernels import timing
+
+    for tokens in ("3", "70"):
+        assert timing.main(["block_matrix", "--warmup", "1", "--iters", "2", "--tokens", tokens, "--hidden", "256", "--ffn", "384", "--experts", "4", "--top", "2"]) == 0
+        line = json.loads(capsys.readouterr().out)
+        assert {"product", "feed_forward", "experts", "pack", "read_back", "product_bfloat16"} <= set(line["us"])

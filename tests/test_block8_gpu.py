@@ -252,3 +252,19 @@ def test_calls_on_two_streams_at_once():
     for s in (0, 1):
         for run in got[s]:
             assert all(torch.equal(a, b) for a, b in zip(run, want[s]))
+
+
+def test_the_same_layer_on_bfloat16_matrices_captured(cuda_device):
+    """Every kernel of a routed layer in the model's type is on the caller's stream: a capture holds them all."""
+    x = _random((8, 256), 60, dtype=torch.bfloat16)
+    ups, downs = _random((5, 2 * 72, 256), 61, 0.1, torch.bfloat16), _random((5, 256, 72), 62, 0.1, torch.bfloat16)
+    weights, ids = _random((8, 5), 63).softmax(1).topk(2, 1)
+    ids, weights = ids.int().contiguous(), weights.contiguous()
+    want = ops.routed_experts(x, ids, weights, ups, None, downs)
+    graph = torch.cuda.CUDAGraph()
+    with ops.capture(graph):
+        got = ops.routed_experts(x, ids, weights, ups, None, downs)
+    got.fill_(7)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -2549,7 +2549,7 @@ def routed_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_
         _check(lib.zb_gather_places(rows, _ptr(x), x.stride(0), slots, places, width, top, _ptr(place_scale), _ptr(weights), stream),
                "gather_places")
         _check(lib.zb_gemm_tc_experts(hidden, rows, _ptr(w_gate), plan, runs, run, places, E, 2 * ff, width, width, ff, 1 + act_code,
-                                      _ptr(place_scale), *bounds, None, None, 0, status, stream), "gemm_tc_grouped")
+                                      _ptr(place_scale), *bounds, status, stream), "gemm_tc_grouped")
         _check(lib.zb_gemm_tc_experts(_ptr(y), hidden, _ptr(w_down), plan, runs, run, places, E, width, ff, ff, ldy, 0, None, *bounds,
                                       status, stream), "gemm_tc_grouped")
     else:

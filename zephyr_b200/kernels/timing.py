@@ -17,6 +17,7 @@
     python -m zephyr_b200.kernels.timing head_linear --tokens 2048 --heads 16 --n 128 --k 128
     python -m zephyr_b200.kernels.timing stream_parts --tokens 2048 --hidden 2048 --ffn 6144
     python -m zephyr_b200.kernels.timing packed_cache --batch 8 --context 4096 --tokens 1024 --heads 32
+    python -m zephyr_b200.kernels.timing block_matrix --tokens 64 --hidden 4096 --ffn 12288 [--experts 16 --top 4]
 
 Each case rotates over several copies of its large operands, together larger than the L2 cache, so
 that a kernel bound by memory is timed against memory and not against L2.  Time is taken with CUDA
@@ -1078,6 +1079,47 @@ def packed_cache(args) -> dict:
 
 
 CASES.update({"packed_cache": packed_cache})
+
+
+# ---- matrices in 8-bit floating point (csrc/block8.cu, csrc/gemm_block8.cu, csrc/gemm_block8_small.cu) ----
+def block_matrix(args) -> dict:
+    """Matrices in 8-bit floating point, each call beside its like on bfloat16 matrices: ``--tokens`` rows of width ``--hidden`` through a square
+    product and a gated feed-forward of inner size ``--ffn``, and through a routed layer (``--experts`` experts, ``--top`` choices a token);
+    and packing and reading back the feed-forward's down matrix."""
+    device, bf = torch.device("cuda"), torch.bfloat16
+    T, H, F, E, top = args.tokens, args.hidden, args.ffn, args.experts, args.top
+    small = lambda *shape: torch.randn(shape, device=device, dtype=bf) * shape[-1] ** -0.5
+    several = lambda *shape: [small(*shape) for _ in range(_copies(2 * math.prod(shape)))]
+    x = small(T, H)
+    square, up, down, ups, downs = (several(*shape) for shape in ((H, H), (2 * F, H), (H, F), (E, 2 * F, H), (E, H, F)))
+    at = lambda matrices, i: matrices[i % len(matrices)]
+    spread = lambda matrices: [ops.pack_matrix(w) for w in matrices for _ in range(2)]       # (half the bytes: twice as many are larger than L2)
+    ids = torch.stack([torch.randperm(E, device=device)[:top] for _ in range(T)]).int().contiguous()
+    weights = torch.rand((T, top), device=device)
+
+    def plain_feed_forward(i):
+        if ops.gemm_small_supported(x, at(up, i)) and T <= ops.SMALL_GEMM_ROWS:
+            return ops.linear(ops.gemm_small(x, at(up, i), swiglu=True), at(down, i))
+        return ops.linear(ops.gemm_tc(x, at(up, i), swiglu=True), at(down, i))
+
+    time = lambda run: _time(run, args.warmup, args.iters)
+    us = {"product_bfloat16": time(lambda i: ops.linear(x, at(square, i))), "feed_forward_bfloat16": time(plain_feed_forward),
+          "experts_bfloat16": time(lambda i: ops.routed_experts(x, ids, weights, at(ups, i), None, at(downs, i))),
+          "pack": time(lambda i: ops.pack_matrix(at(down, i)))}
+    square, up, down, ups, downs = (spread(m) for m in (square, up, down, ups, downs))
+    us.update({"product": time(lambda i: ops.linear(x, at(square, i))),
+               "feed_forward": time(lambda i: ops.block_feed_forward(x, at(up, i), at(down, i))),
+               "experts": time(lambda i: ops.routed_experts(x, ids, weights, at(ups, i), None, at(downs, i))),
+               "read_back": time(lambda i: at(down, i).values(bf))})
+    ops.check_status(ops.device_status(device), "block_matrix")
+    rate = lambda flops, name: round(flops * T / us[name] / 1e6, 1)
+    return {"kernel": "block_matrix", "tokens": T, "hidden": H, "ffn": F, "experts": E, "top": top, "us": {name: round(t, 2) for name, t in us.items()},
+            "tflops": {"product": rate(2 * H * H, "product"), "feed_forward": rate(6 * H * F, "feed_forward"), "experts": rate(6 * top * H * F, "experts")},
+            "weights_gbs": {"product": round(H * H / us["product"] / 1e3, 1), "feed_forward": round(3 * H * F / us["feed_forward"] / 1e3, 1),
+                            "pack": round(3 * H * F / us["pack"] / 1e3, 1), "read_back": round(3 * H * F / us["read_back"] / 1e3, 1)}}
+
+
+CASES.update({"block_matrix": block_matrix})
 
 
 def main(argv=None) -> int:
