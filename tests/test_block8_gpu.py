@@ -182,7 +182,8 @@ def test_feed_forwards(m, width, ff, act):
     (1, 256, 128, 4, 0, 2, "silu", 0.0), (8, 512, 136, 16, 2, 4, "relu", 0.5), (100, 136, 72, 5, 0, 5, "bounded", 0.0),
     (300, 300, 200, 8, 3, 3, "silu", 4.0), (777, 256, 264, 60, 0, 6, "bounded", 2.0), (1500, 128, 128, 4, 0, 2, "silu", 6.0),
     (40, 129, 16, 3, 1, 2, "silu", 0.0), (20, 8192, 256, 4, 0, 2, "silu", 0.0), (30, 256, 6144, 3, 0, 2, "relu", 0.0), (300, 8192, 200, 4, 0, 1, "silu", 0.0),
-    (500, 128, 16, 400, 0, 2, "silu", 0.0), (900, 128, 16, 3, 0, 1, "silu", 3.0)])
+    (500, 128, 16, 400, 0, 2, "silu", 0.0), (900, 128, 16, 3, 0, 1, "silu", 3.0), (60, 200, 72, 64, 2, 4, "bounded", 4.0), (170, 1024, 264, 160, 0, 3, "silu", 1.0),
+    (50, 130, 200, 40, 0, 3, "relu", 5.0), (2, 300, 4200, 3, 0, 2, "silu", 0.0), (1, 9000, 16, 8, 0, 3, "silu", 0.0)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_routed_experts(tokens, width, ff, experts, identity, top, act, skew, dtype):
     x = _random((tokens, width), 30, dtype=dtype)
@@ -220,6 +221,25 @@ def test_routed_experts(tokens, width, ff, experts, identity, top, act, skew, dt
             want[token] += y
             error[token] += off + HALF_STEP[dtype] * (y.abs() + off) + 2.0 ** -22 * y.abs()
         _close(got, want, error, dtype)
+
+
+@pytest.mark.parametrize("tokens,experts", [(3, 4), (30, 16), (30, 4)])
+def test_one_token_chooses_an_expert_twice(tokens, experts):
+    width, ff = 256, 72
+    x = _random((tokens, width), 70, dtype=torch.bfloat16)
+    (up, up_values), (down, down_values) = _matrix((experts, 2 * ff, width), 71, 0.1), _matrix((experts, width, ff), 72, 0.1)
+    ids = torch.arange(tokens, device="cuda")[:, None].expand(tokens, 2).remainder(experts).int().contiguous()
+    weights = _random((tokens, 2), 73).abs().contiguous()
+    got = ops.routed_experts(x, ids, weights, up, None, down)
+    want = torch.empty((tokens, width), dtype=F64, device="cuda")
+    error = torch.empty_like(want)
+    for e in range(min(tokens, experts)):
+        token = torch.arange(e, tokens, experts, device="cuda")
+        y, off = _feed_forward(x[token], up_values[e], down_values[e], "silu")
+        off = off + HALF_STEP[torch.bfloat16] * (y.abs() + off)
+        weight = weights[token].double().sum(1, keepdim=True)
+        want[token], error[token] = weight * y, weight * off + 2.0 ** -21 * (weight * y).abs()
+    _close(got, want, error, torch.bfloat16)
 
 
 # ------------------------------------------------------------------------------------------------- calls side by side

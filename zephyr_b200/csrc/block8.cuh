@@ -76,6 +76,18 @@ struct Block8Small {
 int block8_product(const Block8Product& p, cudaStream_t stream);          // gemm_block8.cu
 int block8_plan(int* plan, int* place_of_slot, const int* ids, int num_slots, int experts, int run, cudaStream_t stream);      // block8.cu
 int block8_code_rows(CodeRowsArgs a, int dtype, cudaStream_t stream);     // block8.cu
+// A routed layer's product for few choices: `x` by token, or by slot; y by slot (hidden values float32, or outputs).
+struct RoutedBlock8 {
+  void* y; long long ldy; int y_dtype;
+  const void* x; long long ldx; int x_dtype; bool by_slot;
+  const void *w_codes, *w_scales;
+  const int* ids; const float* weights; int* place_of_slot;
+  int slots, top, experts, N, K, kind;
+  float limit, alpha, shift;
+  int* status;
+};
+bool routed_block8_fits(int slots, int experts, int K);                   // routed_block8_small.cu
+int routed_block8_product(const RoutedBlock8& p, cudaStream_t stream);
 bool block8_small_fits(int M, int K);                                     // gemm_block8_small.cu
 int block8_small_product(const Block8Small& p, cudaStream_t stream);
 

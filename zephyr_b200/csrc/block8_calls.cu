@@ -151,9 +151,30 @@ struct Experts {
   int T, top, E, width, ff;
   bool weigh_inputs;
 };
+// Whether a routed layer's products stream their matrices (three kernels) instead of planning runs for the tensor cores (five): up to four choices an expert,
+// mostly one run of eight then (us, streams / tensor cores: 16 experts of 2048 x 1536, four choices a token, 1 token 18.5 / 26.6, 8 tokens 43.6 / 48.3, 16 44.8 /
+// 48.8, 32 57.5 / 49.7; 128 of 1024 x 512, eight choices, 64 tokens 61.2 / 74.7).
+static bool few(int T, int top, int E, int width, int ff) {
+  return T * top <= 4 * E && routed_block8_fits(T * top, E, width) && routed_block8_fits(T * top, E, ff);
+}
+static int few_experts(Pieces& memory, const Experts& e, const Operand& up, const Operand& down, const Gate& g, int* status, cudaStream_t stream) {
+  const int slots = e.T * e.top;
+  int* place_of_slot = memory.take<int>(slots);
+  float* hidden = memory.take<float>(static_cast<long long>(slots) * e.ff);
+  char* out = memory.take<char>(static_cast<long long>(slots) * e.width * (e.dtype == DTYPE_F32 ? 4 : 2));
+  if (memory.base == nullptr) return OK;
+  int rc = routed_block8_product({hidden, e.ff, DTYPE_F32, e.x, e.ldx, e.dtype, false, up.codes, up.scales, e.ids, e.weigh_inputs ? e.weights : nullptr, place_of_slot, slots,
+                                  e.top, e.E, up.N, up.K, g.kind, g.limit, g.alpha, g.shift, status}, stream);
+  if (rc != OK) return rc;
+  rc = routed_block8_product({out, e.width, e.dtype, hidden, e.ff, DTYPE_F32, true, down.codes, down.scales, e.ids, nullptr, nullptr, slots, e.top, e.E, down.N, down.K, 0,
+                              0.0f, 1.0f, 0.0f, status}, stream);
+  if (rc != OK) return rc;
+  return zb_route_combine(e.y, out, e.width, e.dtype, e.x, e.ldx, e.ids, e.weigh_inputs ? nullptr : e.weights, place_of_slot, e.T, e.width, e.top, e.dtype, stream);
+}
 // The rows are coded where they are gathered, the hidden values where the first product's sums are read out, an expert's output is rounded to x's
 // type before it is weighted.
 static int experts(Pieces& memory, const Experts& e, const Operand& up, const Operand& down, const Gate& g, int* status, cudaStream_t stream) {
+  if (few(e.T, e.top, e.E, e.width, e.ff)) return few_experts(memory, e, up, down, g, status, stream);
   const int num_slots = e.T * e.top, cap = zb_gemm_tc_experts_run(num_slots, e.E), runs = num_slots / cap + e.E;
   const long long places = static_cast<long long>(runs) * cap;
   const int groups = (cap + 127) / 128;
@@ -257,6 +278,8 @@ ZB_API long long zb_block8_experts_work(long long T, long long top, long long E,
   experts(memory, e, {}, {}, {}, nullptr, nullptr);
   return memory.at;
 }
+// How many kernels the call launches.
+ZB_API int zb_block8_experts_kernels(int T, int top, int E, int width, int ff) { return few(T, top, E, width, ff) ? 3 : 5; }
 ZB_API int zb_block8_experts(const void* call) {
   const ExpertsCall& c = *static_cast<const ExpertsCall*>(call);
   if (!sizes_ok(c.T * c.top, 2 * c.ff, c.width) || !sizes_ok(c.T * c.top, c.width, c.ff) || c.E <= 0 || !gate_ok(c.kind, 2 * c.ff, c.limit, nullptr, true) ||

@@ -15,18 +15,9 @@
 #include <algorithm>
 #include <atomic>
 
-#include "block8.cuh"
-#include "mma.cuh"
-#include "tma.cuh"
+#include "block8_stream.cuh"
 
 namespace zb {
-
-constexpr int G9_WARPS = 16;
-constexpr int G9_SLOT = 16 * 128;            // a block of a tile
-constexpr int G9_DEPTH = 2;                  // of a ring
-constexpr int G9_WAIT_LIMIT = 1 << 18;
-constexpr int G9_MAX_BLOCKS = 32;            // blocks of K a warp: a lane holds the scale of one
-constexpr size_t G9_SMEM = 226 * 1024;
 
 struct Block8SmallArgs {
   CUtensorMap w_map;                         // codes, blocks as rows of 128 bytes; box 128 x 16
@@ -43,15 +34,6 @@ struct Block8SmallArgs {
   int act;
   GateForm gate;
 };
-
-// Four codes as two pairs of half-precision numbers (exact).
-__device__ __forceinline__ void halves_of(unsigned codes, unsigned& lo, unsigned& hi) {
-  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
-}
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // Shared memory, from a multiple of 1024 on: the rings, the slices' sums twice [turn][team][slice][mt * 128], x's codes (rows 64 bytes longer than
 // they are), its scales [block][8 mt].
@@ -95,17 +77,12 @@ __device__ __forceinline__ void finish_tile(const Block8SmallArgs& a, int n0, in
     const int r = i / 8 % (GATED ? 8 : 16), mt = i / (GATED ? 64 : 128), token = mt * 8 + i % 8, row = n0 + r;
     if (token >= a.M || row + (GATED ? 8 : 0) >= a.N) continue;
     if (GATED) {                                        // rows 0 to 7 of a tile are gates, 8 to 15 their ups
-      float gate = total_of(mt * 128 + r * 8 + i % 8), up = total_of(mt * 128 + 64 + r * 8 + i % 8), v;
-      if (a.gate.kind == GATE_BOUNDED) {
-        if (a.gate.bias != nullptr) {
-          gate += a.gate.bias[row];
-          up += a.gate.bias[row + 8];
-        }
-        v = bounded_gate<false>(gate, up, a.gate);
-      } else {
-        v = (a.gate.kind == GATE_RELU ? fmaxf(gate, 0.0f) : gate / (1.0f + expf(-gate))) * up;
+      float gate = total_of(mt * 128 + r * 8 + i % 8), up = total_of(mt * 128 + 64 + r * 8 + i % 8);
+      if (a.gate.bias != nullptr) {                     // (of the bounded gate)
+        gate += a.gate.bias[row];
+        up += a.gate.bias[row + 8];
       }
-      y[static_cast<size_t>(token) * a.ldy + n0 / 2 + r] = from_float<TOut>(v);
+      y[static_cast<size_t>(token) * a.ldy + n0 / 2 + r] = from_float<TOut>(stream_gate(gate, up, a.gate));
     } else {
       const float sum = total_of(i);
       y[static_cast<size_t>(token) * a.ldy + row] = from_float<TOut>(a.act == ACT_GELU ? gelu_tanh(sum) : a.act == ACT_RELU2 ? relu_squared(sum) : sum);
@@ -204,47 +181,14 @@ __global__ void __launch_bounds__(G9_WARPS * 32, MT == 1 ? 2 : 1) gemm_block8_sm
         break;
       }
       float sum[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sum[mt][0] = sum[mt][1] = sum[mt][2] = sum[mt][3] = 0.0f;
-      const unsigned char* rows_at = ring + slot * G9_SLOT + own_row * 128;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 wl = *reinterpret_cast<const uint4*>(rows_at + (((4 * h + t) ^ own_row) << 4));
-        const uint4 wh = *reinterpret_cast<const uint4*>(rows_at + 1024 + (((4 * h + t) ^ own_row) << 4));
-        const unsigned char* fragments = x_s + g * x_pitch + b * B8_BLOCK + 64 * h + 16 * t;
-        // Four neighbouring codes of a row are one product's two pairs of k, of x as of the matrix.
-        const unsigned low[4] = {wl.x, wl.y, wl.z, wl.w}, high[4] = {wh.x, wh.y, wh.z, wh.w};
-        uint4 x[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) x[mt] = *reinterpret_cast<const uint4*>(fragments + mt * 8 * x_pitch);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          unsigned rows[4];
-          halves_of(low[i], rows[0], rows[2]);
-          halves_of(high[i], rows[1], rows[3]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            unsigned b0, b1;
-            halves_of(i == 0 ? x[mt].x : i == 1 ? x[mt].y : i == 2 ? x[mt].z : x[mt].w, b0, b1);
-            mma_f16_16816(sum[mt], rows, b0, b1);
-          }
-        }
-      }
+      stream_block<MT>(ring + slot * G9_SLOT, x_s + b * B8_BLOCK, x_pitch, own_row, sum);
       __syncwarp();                                             // the slot has been read by all lanes
       if (lane == 0) copy_next(slot);
       if (++slot == G9_DEPTH) {
         slot = 0;
         phase ^= 1;
       }
-      const float w = b8_power(__shfl_sync(0xffffffffu, w_scale, b - b_begin));
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float2 s = *reinterpret_cast<const float2*>(x_scale + b * (MT * 8) + mt * 8 + 2 * t);
-        acc[mt][0] = fmaf(sum[mt][0] * w, s.x, acc[mt][0]);
-        acc[mt][1] = fmaf(sum[mt][1] * w, s.y, acc[mt][1]);
-        acc[mt][2] = fmaf(sum[mt][2] * w, s.x, acc[mt][2]);
-        acc[mt][3] = fmaf(sum[mt][3] * w, s.y, acc[mt][3]);
-      }
+      add_scaled<MT>(acc, sum, b8_power(__shfl_sync(0xffffffffu, w_scale, b - b_begin)), x_scale + b * (MT * 8));
     }
     w_scale = next_scale;
     // (A buffer is written again two rounds on: everybody has read it by the meeting in between.)

@@ -86,7 +86,7 @@ _SIGNATURES = {
     "zb_route_align_runs": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "zb_pack_matrix": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p],
     "zb_matrix_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
-    "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int], "zb_block8_feed_forward_kernels": [c_int, c_int, c_int, c_int],
+    "zb_block8_product": [c_char_p], "zb_block8_feed_forward": [c_char_p], "zb_block8_experts": [c_char_p], "zb_block8_product_kernels": [c_int, c_int, c_int], "zb_block8_experts_kernels": [c_int, c_int, c_int, c_int, c_int], "zb_block8_feed_forward_kernels": [c_int, c_int, c_int, c_int],
     "zb_gather_places": [c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "zb_gemm_tc_experts_run": [c_int, c_int],
     "zb_gemm_tc_experts": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int,
@@ -2719,8 +2719,9 @@ def _block8_feed_forward_plan(M: int, K: int, ff: int, N: int, x_code: int, y_co
 
 
 @functools.lru_cache(maxsize=4096)
-def _block8_experts_work(T: int, top: int, E: int, width: int, ff: int, code: int, weigh_inputs: bool) -> int:
-    return library().zb_block8_experts_work(T, top, E, width, ff, code, int(weigh_inputs))
+def _block8_experts_plan(T: int, top: int, E: int, width: int, ff: int, code: int, weigh_inputs: bool) -> tuple[int, int]:
+    lib = library()
+    return lib.zb_block8_experts_work(T, top, E, width, ff, code, int(weigh_inputs)), lib.zb_block8_experts_kernels(T, top, E, width, ff)
 
 
 def _block8_gate(rows: int, act: str, bounded: BoundedGate | None) -> tuple[int, int, float, float, float]:
@@ -2813,10 +2814,11 @@ def _routed_blocks(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, ga
     if T * top >= 2 ** 31 - 512:
         raise InvalidArgumentError("choices that 32 bits can count")
     code = DTYPE_CODE[x.dtype]
-    work = torch.empty(_block8_experts_work(T, top, E, width, ff, code, weigh_inputs), dtype=torch.uint8, device=x.device)
+    bytes_, kernels = _block8_experts_plan(T, top, E, width, ff, code, weigh_inputs)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=x.device)
     _check(library().zb_block8_experts(_BLOCK8_EXPERTS(
         out.data_ptr(), x_at, pitch, code, ids_at, weights_at, gate_up.codes_at, gate_up.scales_at, down.codes_at, down.scales_at, T, top, E, width, ff, kind,
-        weigh_inputs, *bounds, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "routed_blocks", 5)
+        weigh_inputs, *bounds, work.data_ptr(), _device_status_pointer(x.device) or 0, _stream())), "routed_blocks", kernels)
     return out
 
 
