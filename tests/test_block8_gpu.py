@@ -90,7 +90,7 @@ def test_products(m, n, k, x_dtype, y_dtype):
 # Few rows of long matrices; then rows and columns for runs of 64, 128 and 256 rows, tiles of whole and shared K, result rows that are and are not
 # multiples of 16 bytes.
 @pytest.mark.parametrize("m,n,k", [(3, 5120, 25600), (16, 512, 25600), (12, 4096, 12288), (8, 30000, 256), (100, 640, 9000),
-                                   (130, 2500, 14336), (100, 6400, 14336), (1000, 4864, 10240), (300, 8200, 640), (600, 4105, 260), (1030, 4110, 384), (333, 1030, 9100)])
+                                   (130, 2500, 14336), (100, 6400, 14336), (1000, 4864, 10240), (1500, 3840, 11520), (300, 8200, 640), (600, 4105, 260), (1030, 4110, 384), (333, 1030, 9100)])
 def test_products_of_long_rows_and_of_many(m, n, k):
     x = _random((m, k), 8, dtype=torch.bfloat16)
     packed, w = _matrix((n, k), 9)
@@ -168,7 +168,7 @@ def _feed_forward(x, up, down, act, limits=LIMITS, bias=None):
 
 @pytest.mark.parametrize("m,width,ff,act", [(1, 256, 128, "silu"), (16, 1024, 904, "relu"), (17, 130, 8, "silu"), (64, 300, 1000, "bounded"),
                                             (200, 1024, 512, "silu"), (600, 640, 1544, "bounded"), (600, 4100, 4104, "silu"),
-                                            (40, 12288, 640, "silu"), (40, 1000, 9000, "relu"), (100, 14336, 3200, "silu"), (1024, 10240, 2432, "bounded")])
+                                            (40, 12288, 640, "silu"), (40, 1000, 9000, "relu"), (100, 14336, 3200, "silu"), (1024, 10240, 2432, "bounded"), (1500, 11520, 1920, "relu")])
 def test_feed_forwards(m, width, ff, act):
     x = _random((m, width), 20, dtype=torch.bfloat16)
     (up, up_values), (down, down_values) = _matrix((2 * ff, width), 21, 0.1), _matrix((width, ff), 22, 0.1)
