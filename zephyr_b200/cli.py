@@ -64,7 +64,7 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--max-prefill-chunk-tokens", type=_positive_int)
     gen.add_argument("--kv-block-size", type=_positive_int, default=16)
     gen.add_argument("--kv-bits", type=int, choices=(4,), help="hold keys and values in 4 bits: 3.2 times as many positions, slower prompts (default: in the model's type)")
-    gen.add_argument("--weight-bits", type=int, choices=(8,), help="hold the layers' matrices in 8-bit floating point with a scale for each block of 128 x 128: half the memory, faster products (default: in the model's type)")
+    gen.add_argument("--weight-bits", type=int, choices=(8,), help="hold the layers' matrices in 8-bit floating point with a scale for each block of 128 x 128: half the memory, faster steps at large widths (default: in the model's type)")
     gen.add_argument("--num-kv-blocks", type=_positive_int, help="fix the number of cache pages")
     gen.add_argument("--json", action="store_true", help="print one JSON object per request")
     gen.add_argument("--log-level", choices=("critical", "error", "warning", "info", "debug", "trace"), default="warning")
