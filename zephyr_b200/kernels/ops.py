@@ -2653,8 +2653,11 @@ class BlockMatrix:
 
     def exponents(self) -> torch.Tensor:
         """The blocks' bytes, exponent + 127: uint8 [N / 128 up, K / 128 up], with ``matrices`` ahead where there are several."""
+        rows, columns = self.blocks
         at = self._total[0] + self._total[1]
-        return self.data[at : at + self.matrices * self.blocks[0] * self.blocks[1]].view(*self.shape[:-2], *self.blocks)
+        if len(self.shape) == 2:
+            return self.data.as_strided((rows, columns), (columns, 1), at)
+        return self.data.as_strided((self.matrices, rows, columns), (rows * columns, columns, 1), at)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the codes stand for (exact in bfloat16 but below its normal numbers)."""
