@@ -81,7 +81,7 @@ struct Block8Args {
 };
 
 struct Block8Shared {
-  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], acc_edge, merged, peaks[4];
+  unsigned long long full[G8_MAX_STAGES], empty[G8_MAX_STAGES], acc_full[2], acc_empty[2], acc_edge, merged, peaks[2][4];
   unsigned tmem_base;
   volatile int failed;
   int plan[3 * G8_PLAN_RUNS];                     // the plan's runs, as many as there is room for
@@ -168,6 +168,10 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 template <int N> __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
+// One word into the other CTA's shared memory, its bytes counted on a barrier there.
+__device__ __forceinline__ void store_counted(unsigned cluster_address, unsigned value, unsigned bar_cluster_address) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];\n" ::"r"(cluster_address), "r"(value), "r"(bar_cluster_address) : "memory");
+}
 // One scaled product of 256 x N x 32: D (+)= A B, each operand's sums times the powers of two in tensor memory at `a_scales` and `b_scales`.
 __device__ __forceinline__ void tc_mma_scaled_pair(unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc,
                                                    unsigned a_scales, unsigned b_scales, unsigned accumulate) {
@@ -217,7 +221,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
       mbar_init(&sh.acc_full[b], 1);
       mbar_init(&sh.acc_empty[b], 2 * EPILOGUE_WARPS);      // of both CTAs
     }
-    for (int g = 0; g < GROUPS; ++g) mbar_init(&sh.peaks[g], 8);     // four warps of each CTA
+    for (int g = 0; g < 2 * 4; ++g) mbar_init(&sh.peaks[0][0] + g, 4);     // four warps, and the bytes of the other CTA's four
     mbar_init(&sh.acc_edge, 2 * EPILOGUE_WARPS);
     mbar_init(&sh.merged, EPILOGUE_WARPS);
     sh.failed = 0;
@@ -365,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
     const bool holds_gate = (lane & 8) == 0;
     unsigned char* staging = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * G8_STAGING;
     int acc = 0, stores = 0;
-    unsigned acc_phase = 0, merged_phase = 0, peaks_phase = 0;
+    unsigned acc_phase = 0, merged_phase = 0, turn = 0;
     while (share.next(a, item, k_first, k_end)) {
       const Run8 run = run_of(a, sh, item % runs);
       const int row = item / runs * 256 + 128 * rank + 32 * quarter + lane, column0 = (row - lane) / (GATED ? 2 : 1);
@@ -392,12 +396,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           }
         }
       };
+      // What is given back is tensor memory whose loads were waited for: these arrivals order nothing else (a release across the cluster waited for
+      // the codes' way to memory, 2000 cycles a tile).
       // The columns that the two accumulators of 256 share have been read: the last 64 of the first one, the first 64 of the second.
       auto free_edge = [&]() {
         if (RUN == 256) {
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_edge), 0));
+          if (lane == 0) mbar_arrive_at(in_cta_of_rank(smem_u32(&sh.acc_edge), 0));
         }
       };
       // A warp's chunks of 32 columns, the one that may lie on the edge first.
@@ -406,7 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
       auto free_accumulator = [&]() {
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
+        if (lane == 0) mbar_arrive_at(in_cta_of_rank(smem_u32(&sh.acc_empty[acc]), 0));
         if (++acc == accumulators) {
           acc = 0;
           acc_phase ^= 1;
@@ -528,9 +534,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           }
         } else {
           // A block of 128 hidden values of a row of x is the pair's tile: 16 of them are a warp's, and the largest of all eight warps' (four in each
-          // CTA) gives the scale.  [turn][CTA][quarter][row of x], in both CTAs; lane l finds and hands over row `mine` of 32.
+          // CTA) gives the scale.  [turn][CTA][quarter][row of x], in both CTAs; lane l finds and hands over row `mine` of 32.  A store that counts its bytes on the
+          // other CTA's barrier, one of two that take turns: a warp there may be a tile ahead of its neighbours, and never two.
           unsigned char* bytes = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * 512;
-          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + peaks_phase * 8 * RUN;
+          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + (turn & 1) * 8 * RUN;
+          unsigned long long* met = &sh.peaks[turn & 1][group];
+          const unsigned their_met = in_cta_of_rank(smem_u32(met), rank ^ 1);
+          unsigned handed = 0;
           const int mine = (lane & 8) << 1 | (lane & 16) >> 1 | (lane & 7);
 #pragma unroll
           for (int s = 0; s < CHUNKS; ++s) {
@@ -553,19 +563,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
               meet(1, 1);
               unsigned* at = peaks + (rank * 4 + quarter) * RUN + c + mine;
               *at = m[0];
-              asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(in_cta_of_rank(smem_u32(at), rank ^ 1)), "r"(m[0]) : "memory");
+              store_counted(in_cta_of_rank(smem_u32(at), rank ^ 1), m[0], their_met);
+              handed += 32 * 4;
             }
           }
           __syncwarp();
-          if (lane < 2) mbar_arrive_in_cluster(in_cta_of_rank(smem_u32(&sh.peaks[group]), lane));
+          if (lane == 0) mbar_arrive_expect_tx(met, handed);       // (as many come from the other CTA)
           bool ok = false;
-          for (int i = 0; i < G8_WAIT_LIMIT && !ok && !((i & 255) == 255 && sh.failed); ++i) ok = mbar_try_wait_cluster(&sh.peaks[group], peaks_phase);
+          for (int i = 0; i < G8_WAIT_LIMIT && !ok && !((i & 255) == 255 && sh.failed); ++i) ok = mbar_try_wait_cluster(met, turn >> 1 & 1);
           if (!__all_sync(0xffffffffu, ok)) {
             if (lane == 0 && !sh.failed) report(a.status, STATUS_BARRIER_TIMEOUT, item, -6);
             sh.failed = 1;
             break;
           }
-          peaks_phase ^= 1;
+          ++turn;
           const int block = item / runs, pitch = b8_pitch(width), hidden_pieces = b8_pieces(width);
           unsigned char* codes_at = static_cast<unsigned char*>(a.y) + static_cast<size_t>(run.place) * pitch + block * 128 + rank * 64 + quarter * 16;
 #pragma unroll
