@@ -50,8 +50,8 @@ template <int RUN> struct Block8Shape {
   static constexpr int SECOND = RUN == 256 ? 192 : RUN;
   static constexpr int SCALE_COLUMN = RUN == 256 ? 448 : 256;
   static constexpr int RING_BYTES = STAGES * (STAGE_BYTES + G8_SCALES);
-  // Behind the ring what results pass through: staging, or where they are coded 512 bytes a warp and the largest magnitudes of eight warps' rows, twice.
-  static constexpr int smem_bytes(bool coded) { return RING_BYTES + (coded ? g8_epilogue_warps(true) * 512 + 2 * 8 * RUN * 4 : g8_epilogue_warps(false) * G8_STAGING) + 1024; }
+  // Behind the ring what results pass through: staging, or where they are coded 512 bytes a warp, 32 factors a warp, and the largest magnitudes of eight warps' rows, twice.
+  static constexpr int smem_bytes(bool coded) { return RING_BYTES + (coded ? g8_epilogue_warps(true) * (512 + 128) + 2 * 8 * RUN * 4 : g8_epilogue_warps(false) * G8_STAGING) + 1024; }
   static_assert(STAGES <= G8_MAX_STAGES && smem_bytes(true) <= 227 * 1024 - 512 && smem_bytes(false) <= 227 * 1024 - 512, "shared memory");
   static_assert(SECOND + RUN <= SCALE_COLUMN && SCALE_COLUMN + 12 * STAGES <= 512, "tensor memory");
 };
@@ -537,7 +537,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           // CTA) gives the scale.  [turn][CTA][quarter][row of x], in both CTAs; lane l finds and hands over row `mine` of 32.  A store that counts its bytes on the
           // other CTA's barrier, one of two that take turns: a warp there may be a tile ahead of its neighbours, and never two.
           unsigned char* bytes = scale_ring + Shape::STAGES * G8_SCALES + (warp - 2) * 512;
-          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + (turn & 1) * 8 * RUN;
+          float* factors = reinterpret_cast<float*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * 512) + (warp - 2) * 32;
+          unsigned* peaks = reinterpret_cast<unsigned*>(scale_ring + Shape::STAGES * G8_SCALES + EPILOGUE_WARPS * (512 + 128)) + (turn & 1) * 8 * RUN;
           unsigned long long* met = &sh.peaks[turn & 1][group];
           const unsigned their_met = in_cta_of_rank(smem_u32(met), rank ^ 1);
           unsigned handed = 0;
@@ -587,12 +588,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
 #pragma unroll
               for (int q = 0; q < 8; ++q) largest = max(largest, peaks[q * RUN + c + mine]);
               const unsigned byte = b8_scale_byte(largest);
-              const float inverse = b8_inverse(byte);
+              factors[mine] = b8_inverse(byte);
+              __syncwarp();
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
-                const int from = (lane & 8) | (i & 8) << 1 | (i & 7);
-                const float one = __shfl_sync(0xffffffffu, inverse, from), two = __shfl_sync(0xffffffffu, inverse, from + 1);
-                const unsigned codes = b8_two_codes(hidden[s][i], one, hidden[s][i + 1], two);
+                const float2 own = *reinterpret_cast<const float2*>(factors + own_row + i);
+                const unsigned codes = b8_two_codes(hidden[s][i], own.x, hidden[s][i + 1], own.y);
                 unsigned char* to = bytes + (own_row + i) * 16 + own_column;
                 to[0] = static_cast<unsigned char>(codes);
                 to[16] = static_cast<unsigned char>(codes >> 8);
