@@ -1,10 +1,11 @@
 // A routed layer's two products on matrices in 8-bit floating point (block8.cuh) for the few tokens of a decode step: weight streamers that find their
 // runs themselves.  A product is one launch; for the tensor cores a step is a chain of a plan, the coding of rows and products that wait for whole
 // tiles, each of a few microseconds (one token's four experts of 2048 x 1536, 38 MB: 26.6 us, here 18.5, with the weighted sum behind them).  Fifteen of
-// those experts, 142 MB, take 43.6 us: bound by memory latency and by each kernel's start, the first product streams at 4.5 TB/s.
+// those experts, 142 MB, take 43.6 us, 5 of them the weighted sum: bound by memory latency and by each kernel's start.
 //
 // Every CTA numbers the choices ("slots") by expert, in their order, so that all CTAs agree: at most 512, one a thread, counters per warp and expert in
-// shared memory, a scan over the experts.  Up to eight slots of an expert are a run: the tensor cores' eight columns (mma.sync m16n8k16 on codes as half-precision numbers, as in gemm_block8_small.cu).
+// shared memory, a scan over the experts.  Up to eight slots of an expert are a run: the tensor cores' eight columns (mma.sync m16n8k16 on codes as
+// half-precision numbers, as in gemm_block8_small.cu).
 // All runs' tiles of 16 rows, one run behind the other, are cut into equal contiguous shares, a CTA's share passes through a run or two.  For each the CTA
 // codes the run's rows into shared memory, the tokens' for the first product, the slots' hidden values in float32 for the second one, while the copies of
 // matrices go on.  A team of TEAM of the 16 warps shares a tile, each a slice of K.  Hidden values and outputs lie by slot; results do not depend
