@@ -429,8 +429,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
 #pragma unroll
           for (int i = 0; i < 32; ++i) __stcg(part + (c + i) * 128, __uint_as_float(v[i]));
         }
+        __syncwarp();                                  // all lanes' stores are ahead of the fence that the flag follows
         __threadfence();
-        __syncwarp();
         if (lane == 0) atomicExch(flag_of(pair, group), 1);
         free_edge();
         free_accumulator();
@@ -452,6 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           sh.failed = 1;
           break;
         }
+        __syncwarp();                                 // a lane reads parts whose flags other lanes have seen: a vote orders no memory
         // The others' parts, in the order of K's blocks, are added where the sums are: 16 columns of some pairs on their way at a time.
         constexpr int PARTS = CODED ? 2 : 4;
         for (int c = 16 * group; c < run.rows; c += 16 * GROUPS) {
