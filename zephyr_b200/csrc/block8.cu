@@ -108,6 +108,14 @@ pack_matrix_kernel(unsigned char* codes, unsigned char* scales, unsigned char* e
   }
 }
 
+// Stands behind a kernel that writes a matrix.  The products for few rows read codes and scales ahead of their wait for earlier kernels, and a kernel that does
+// not say when its dependents may start lets them start when its CTAs have ended, which is before all that they wrote has to be visible.  This one
+// waits for that, and whatever is launched as its dependent starts no earlier.
+__global__ void matrix_ready_kernel() {
+  wait_for_prior_grids();
+  let_dependents_launch();
+}
+
 // 16 codes a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -307,7 +315,8 @@ ZB_API int zb_pack_matrix(void* codes, void* scales, void* exponents, const void
   else
     pack_matrix_kernel<<<grid, B8_PACK_THREADS, 0, s>>>(static_cast<unsigned char*>(codes), static_cast<unsigned char*>(scales), static_cast<unsigned char*>(exponents),
                                                         static_cast<const __nv_bfloat16*>(w), matrix_stride, ldw, N, K, wide);
-  return launch_result();
+  const int rc = launch_result();
+  return rc != OK ? rc : launch_dependent(matrix_ready_kernel, dim3(1), dim3(32), 0, s, false);
 }
 
 // out [matrices][N][K] = what a matrix's codes stand for (exact in bfloat16 but below its normal numbers).

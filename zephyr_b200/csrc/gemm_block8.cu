@@ -236,7 +236,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
   cluster_sync_all();                               // both CTAs' barriers and tensor memory are there
   tc_fence_after_sync();
   const unsigned tmem_base = sh.tmem_base;
-  // While the kernel ahead still runs: the first stages' blocks of w, which nothing ahead writes.  (Where runs come from a plan, a kernel ahead writes it.)
+  // While the kernel ahead still runs: the first stages' blocks of w, which no kernel that may still run writes (the rows were
+  // coded by one that waited for all others).  (Where runs come from a plan, a kernel ahead writes it.)
   int ahead = 0;
   if (warp == 0 && a.plan == nullptr && elect_one()) {
     Share first_share(a, runs_of(a), pair, pairs);

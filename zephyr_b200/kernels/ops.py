@@ -2643,6 +2643,7 @@ class BlockMatrix:
         pieces = torch.ones((made.matrices, rows, -(-columns // 4) * 4), dtype=torch.uint8, device=codes.device)
         pieces[:, :, :columns] = exponents.view(made.matrices, rows, columns)
         made.scales.copy_(pieces.view(made.matrices, rows, -1, 1, 4).expand(-1, -1, -1, 128, -1).reshape(made.scales.shape))
+        # (Last: products may read codes and scales ahead of their wait for earlier kernels, and whatever is copied here starts behind the copies above.)
         made.data[sum(made._total) :] = exponents.reshape(-1)
         return made
 
@@ -2683,7 +2684,7 @@ def pack_matrix(w: torch.Tensor) -> BlockMatrix:
     _check_place(place)
     made = BlockMatrix._empty(shape, w.device)
     _check(library().zb_pack_matrix(made.codes_at, made.scales_at, made.scales_at + made._total[1], w_at, made.matrices, w.stride(0) if len(shape) == 3 else 0,
-                                    w.stride(-2), made.N, made.K, DTYPE_CODE[w.dtype], _stream()), "pack_matrix")
+                                    w.stride(-2), made.N, made.K, DTYPE_CODE[w.dtype], _stream()), "pack_matrix", 2)
     return made
 
 
