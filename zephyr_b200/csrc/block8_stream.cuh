@@ -74,7 +74,7 @@ __device__ __forceinline__ void add_scaled(float (&acc)[MT][4], const float (&su
 // act(gate) * up (without a bias).
 __device__ __forceinline__ float stream_gate(float gate, float up, const GateForm& form) {
   if (form.kind == GATE_BOUNDED) return bounded_gate<false>(gate, up, form);
-  return (form.kind == GATE_RELU ? fmaxf(gate, 0.0f) : gate / (1.0f + expf(-gate))) * up;
+  return (form.kind == GATE_RELU ? relu(gate) : gate / (1.0f + expf(-gate))) * up;
 }
 
 }  // namespace zb

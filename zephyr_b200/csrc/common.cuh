@@ -52,6 +52,20 @@ __device__ __forceinline__ float load_scale(const void* w, int w_dtype, int i) {
                               : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
+// The smaller and the larger of two numbers, NaN if one of them is: fminf and fmaxf give the other one, and a NaN sum would leave an
+// activation as one of its bounds.
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float v;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float relu(float z) { return max_or_nan(z, 0.0f); }
+
 // What a gated feed-forward does with a gate sum G and its up sum U where a product's epilogue applies
 // it, in float32.  GATE_SILU: silu(G) * U.  GATE_RELU: max(G, 0) * U.  GATE_BOUNDED: with g = min(G + b_g,
 // limit) and u = clamp(U + b_u, -limit, limit), g * sigmoid(alpha * g) * (u + shift); `bias` holds one
@@ -74,8 +88,8 @@ inline GateForm plain_gate(int kind) { return GateForm{kind, nullptr, 0.0f, 1.0f
 // The bounded gate from sums that already carry their biases.
 template <bool FAST>
 __device__ __forceinline__ float bounded_gate(float g, float u, const GateForm& f) {
-  g = fminf(g, f.limit);
-  u = fminf(fmaxf(u, -f.limit), f.limit);
+  g = min_or_nan(g, f.limit);
+  u = min_or_nan(max_or_nan(u, -f.limit), f.limit);
   float s;
   if (FAST) {   // the special-function unit's exp2 and reciprocal: about 2^-21, far inside a bfloat16 rounding
     float e;
@@ -93,7 +107,7 @@ constexpr int ACT_GELU = 1;
 constexpr int ACT_RELU2 = 2;        // max(z, 0)^2
 
 __device__ __forceinline__ float relu_squared(float z) {
-  z = fmaxf(z, 0.0f);
+  z = relu(z);
   return z * z;
 }
 

@@ -228,7 +228,7 @@ rmsnorm_warp_rows_kernel(__nv_bfloat16* __restrict__ out, __nv_bfloat16* x, cons
 constexpr int ACT_SILU = 0;
 constexpr int ACT_RELU = 1;
 __device__ __forceinline__ float gate_act(float g, int act) {
-  return act == ACT_RELU ? fmaxf(g, 0.0f) : g / (1.0f + expf(-g));
+  return act == ACT_RELU ? relu(g) : g / (1.0f + expf(-g));
 }
 
 // gu is [T, 2I]: columns [0, I) hold the gate, [I, 2I) the up projection.

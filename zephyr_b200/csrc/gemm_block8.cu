@@ -522,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g8_threads(sizeof(TO
           }
         };
         if (a.gate.kind == GATE_SILU) gate_pairs([](float gate, float up) { return silu_fast(gate) * up; });
-        else if (a.gate.kind == GATE_RELU) gate_pairs([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
+        else if (a.gate.kind == GATE_RELU) gate_pairs([](float gate, float up) { return relu(gate) * up; });
         else gate_pairs([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
         free_accumulator();
         if constexpr (!CODED) {

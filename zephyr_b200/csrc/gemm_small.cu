@@ -87,7 +87,7 @@ __device__ __forceinline__ void small_gemm_finish(const SmallGemmArgs& a, int n0
         }
         v = bounded_gate<false>(gate, up, a.gate);
       } else {
-        v = (a.gate.kind == GATE_RELU ? fmaxf(gate, 0.0f) : gate / (1.0f + expf(-gate))) * up;
+        v = (a.gate.kind == GATE_RELU ? relu(gate) : gate / (1.0f + expf(-gate))) * up;
       }
       store_out<TOut>(y + static_cast<size_t>(token) * a.ldy + n0 / 2 + r, v);
     } else {

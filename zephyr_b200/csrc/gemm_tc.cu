@@ -150,7 +150,7 @@ __device__ __forceinline__ void write_out_rows(const CUtensorMap& y_map, unsigne
             for (int i = 0; i < 8; ++i) {
               if (GATED) {
                 const float gate = __uint_as_float(v[16 * j + i]), up = __uint_as_float(v[16 * j + 8 + i]);
-                o[i] = (form.kind == GATE_RELU ? fmaxf(gate, 0.0f) : silu_fast(gate)) * up;
+                o[i] = (form.kind == GATE_RELU ? relu(gate) : silu_fast(gate)) * up;
               } else if (EPI == GT_EPI_GELU) {
                 o[i] = gelu_tanh_fast(__uint_as_float(v[8 * j + i]));
               } else if (EPI == GT_EPI_RELU2) {

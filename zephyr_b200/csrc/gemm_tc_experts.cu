@@ -216,7 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GX_THREADS, 1) gemm_
             }
           };
           if (a.gate.kind == GATE_SILU) finish([](float gate, float up) { return silu_fast(gate) * up; });
-          else if (a.gate.kind == GATE_RELU) finish([](float gate, float up) { return fmaxf(gate, 0.0f) * up; });
+          else if (a.gate.kind == GATE_RELU) finish([](float gate, float up) { return relu(gate) * up; });
           else finish([&](float gate, float up) { return bounded_gate<true>(gate, up, a.gate); });
         } else {
 #pragma unroll

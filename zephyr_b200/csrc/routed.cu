@@ -345,7 +345,7 @@ __device__ __forceinline__ void gate_up_rows(const ExpertProductArgs& a, int exp
 }
 
 __device__ __forceinline__ float expert_act(float g, int act) {
-  return act == 1 ? fmaxf(g, 0.0f) : g / (1.0f + expf(-g));
+  return act == 1 ? relu(g) : g / (1.0f + expf(-g));
 }
 
 // What a gate sum and its up sum become.  Without weights on the inputs both are rounded to the model's type

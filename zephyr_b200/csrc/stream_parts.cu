@@ -279,8 +279,8 @@ clamped_gate_kernel(OUT* out, const IN* gu, const float* bias, long long total, 
       g += bias[gi];
       u += bias[ui];
     }
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = min_or_nan(g, limit);
+    u = min_or_nan(max_or_nan(u, -limit), limit);
     out[at] = from_float<OUT>(g / (1.0f + expf(-alpha * g)) * (u + shift));
   }
 }
