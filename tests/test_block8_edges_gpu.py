@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from test_block8_gpu import _random
+import plain_block8 as plain
+from test_block8_gpu import F64, HALF_STEP, _close, _feed_forward, _random
 from zephyr_b200.kernels import ops
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,51 @@ def test_a_product_directly_behind_copied_codes():
     torch.cuda.synchronize()
     for i in range(12):
         assert torch.equal(ops.block_linear(x, ops.BlockMatrix.from_codes(codes[i % 3], made[i % 3].exponents())), want[i % 3])
+
+
+# ------------------------------------------------------------------------------------------------- the ends of the range
+def _coded_matrix(shape, exponents, seed):
+    """A matrix of random codes with these bytes for its blocks, and what it stands for in 64 bits (which may be beyond float32)."""
+    codes = _random(shape, seed, 100.0).clamp(-448, 448).to(torch.float8_e4m3fn)
+    blocks = exponents.repeat_interleave(128, -2)[..., : shape[-2], :].repeat_interleave(128, -1)[..., : shape[-1]]
+    return ops.BlockMatrix.from_codes(codes, exponents), codes.to(F64) * torch.exp2(blocks.to(F64) - 127)
+
+
+def _bytes(shape, value):
+    return torch.full((*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128)), value, dtype=torch.uint8, device="cuda")
+
+
+# Powers of two of a matrix's scales (2^w) and of the rows' values (2^x): at each end, the result an ordinary number, or one close to an end of float32.
+ENDS = [(127, -126), (127, -120), (110, -110), (64, -60), (65, -60), (-126, 118), (-126, 60), (-110, 110), (60, 50), (-70, -40)]
+
+
+@pytest.mark.parametrize("m", [1, 8, 16, 17, 300])
+@pytest.mark.parametrize("n,k", [(200, 640), (48, 2300)])
+def test_products_where_scales_are_at_the_ends(m, n, k):
+    for i, (w_power, x_power) in enumerate(ENDS):
+        matrix, values = _coded_matrix((n, k), _bytes((n, k), w_power + 127), 20 + i)
+        x = (_random((m, k), 40 + i).double() * 2.0 ** x_power).float()
+        want, magnitude = plain.product(x, values)
+        assert bool((want.abs() < 2.0 ** 127).all())
+        _close(ops.block_linear(x, matrix), want, plain.sum_error(k) * magnitude, torch.float32)
+        zero = ops.block_linear(torch.zeros_like(x), matrix)
+        assert bool((zero == 0).all())
+
+
+@pytest.mark.parametrize("m", [2, 16, 40, 300])
+def test_feed_forwards_and_experts_where_scales_are_at_the_ends(m):
+    width, ff = 384, 264
+    # Sums of 2^11 times the powers, hidden values of their square; also hidden values far from one, with matrices that bring them back.
+    for i, (up_power, x_power, down_power) in enumerate([(127, -126, -10), (-126, 118, 3), (115, -120, 90), (-126, 102, 127), (127, -82, -126)]):
+        shapes = (2 * ff, width), (width, ff)
+        (up, up_values), (down, down_values) = (_coded_matrix(s, _bytes(s, p + 127), 60 + 2 * i + j) for j, (s, p) in enumerate(zip(shapes, (up_power, down_power))))
+        x = (_random((m, width), 80 + i).double() * 2.0 ** x_power).float()
+        want, error = _feed_forward(x, up_values, down_values, "relu")
+        assert bool((want.abs() < 2.0 ** 127).all()) and bool((want != 0).any())
+        _close(ops.block_feed_forward(x, up, down, act="relu"), want, error, torch.float32)
+        experts = 3
+        several = [ops.BlockMatrix.from_codes(w.codes.transpose(2, 3).flatten(3, 4).flatten(1, 2)[:, : w.N, : w.K].expand(experts, -1, -1),
+                                              w.exponents().expand(experts, -1, -1).contiguous()) for w in (up, down)]
+        ids = (torch.arange(m, device="cuda") % experts).int()[:, None].contiguous()
+        got = ops.routed_experts(x, ids, torch.ones((m, 1), device="cuda"), several[0], None, several[1], act="relu")
+        _close(got, want, error + HALF_STEP[torch.float32] * (want.abs() + error), torch.float32)

@@ -57,17 +57,23 @@ __device__ __forceinline__ void stream_block(const unsigned char* rows, const un
   }
 }
 
-// acc += a block's sums times its scales; `x_scale`: the block's, a column each.
+// acc += a block's sums times its scales; `x_scale`: the block's, a column each.  Sums are zero or of 2^-18 to 2^25, and multiples of 2^-18, so that either scale
+// leaves them exact (below float32's normal numbers too), but one of the two may leave its range where both together do not.  So the matrix's comes first where it is
+// not large, and else the row's: what is infinite then is so with both.
 template <int MT>
 __device__ __forceinline__ void add_scaled(float (&acc)[MT][4], const float (&sum)[MT][4], float w, const float* x_scale) {
   const int t = threadIdx.x & 3;
+  float2 s[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) s[mt] = *reinterpret_cast<const float2*>(x_scale + mt * 8 + 2 * t);
+  const bool large = w > __uint_as_float((127u + 64u) << 23);
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const float2 s = *reinterpret_cast<const float2*>(x_scale + mt * 8 + 2 * t);
-    acc[mt][0] = fmaf(sum[mt][0] * w, s.x, acc[mt][0]);
-    acc[mt][1] = fmaf(sum[mt][1] * w, s.y, acc[mt][1]);
-    acc[mt][2] = fmaf(sum[mt][2] * w, s.x, acc[mt][2]);
-    acc[mt][3] = fmaf(sum[mt][3] * w, s.y, acc[mt][3]);
+    const float fx = large ? s[mt].x : w, lx = large ? w : s[mt].x, fy = large ? s[mt].y : w, ly = large ? w : s[mt].y;
+    acc[mt][0] = fmaf(sum[mt][0] * fx, lx, acc[mt][0]);
+    acc[mt][1] = fmaf(sum[mt][1] * fy, ly, acc[mt][1]);
+    acc[mt][2] = fmaf(sum[mt][2] * fx, lx, acc[mt][2]);
+    acc[mt][3] = fmaf(sum[mt][3] * fy, ly, acc[mt][3]);
   }
 }
 
