@@ -93,3 +93,44 @@ def test_feed_forwards_and_experts_where_scales_are_at_the_ends(m):
         ids = (torch.arange(m, device="cuda") % experts).int()[:, None].contiguous()
         got = ops.routed_experts(x, ids, torch.ones((m, 1), device="cuda"), several[0], None, several[1], act="relu")
         _close(got, want, error + HALF_STEP[torch.float32] * (want.abs() + error), torch.float32)
+
+
+# ------------------------------------------------------------------------------------------------- long sums of one sign
+def _positive(shape, seed):
+    """Numbers that e4m3 holds beside one another in a block: eight fractions at nine sizes, none of them zero or negative."""
+    generator = torch.Generator(device="cuda")
+    generator.manual_seed(seed)
+    integers = lambda high: torch.randint(0, high, shape, generator=generator, device="cuda", dtype=torch.int32)
+    return (1 + integers(8) / 8) * torch.exp2(-integers(9).float())
+
+
+def _lost(got, want):
+    """How much of itself a sum loses on average: the tensor cores cut what a sum of 24 bits does not hold, always towards zero."""
+    return ((want - got.double()) / want).mean().item()
+
+
+def test_long_sums_to_float32_are_taken_in_two_accumulators():
+    """Of K > 8192 values: each half has lost what a sum of half as many terms loses, not twice that.  Sizes whose tiles go to one pair of SMs whole; 1.3
+    leaves room for the draws."""
+    k, n, m = 9216, 2304, 256
+    x, w = _positive((m, k), 1), _positive((n, k), 2)
+    half = _lost(ops.block_linear(x[:, : k // 2], ops.pack_matrix(w[:, : k // 2].contiguous()), torch.float32), x[:, : k // 2].double() @ w[:, : k // 2].double().t())
+    assert half > 0
+    assert _lost(ops.block_linear(x, ops.pack_matrix(w), torch.float32), x.double() @ w.double().t()) < 1.3 * half
+    # A feed-forward and experts whose hidden values are exact: gates of a power of two (relu), ups that e4m3 holds.
+    for tokens, width, experts in ((256, 2304, 1), (256, 2048, 2), (80, 4352, 2)):
+        up, values, down = torch.zeros((experts, 2 * k, 128), device="cuda"), _positive((experts, k), 3), _positive((experts, width, k), 4)
+        up.view(experts, -1, 2, 8, 128)[:, :, 0, :, 0] = 1
+        up.view(experts, -1, 2, 8, 128)[:, :, 1, :, 0] = values.view(experts, -1, 8)
+        x = torch.zeros((tokens, 128), device="cuda")
+        x[:, 0] = torch.exp2((torch.arange(tokens, device="cuda") % 5).float())
+        ids = torch.arange(tokens, device="cuda") % experts
+        if experts == 1:
+            got = ops.block_feed_forward(x, ops.pack_matrix(up[0]), ops.pack_matrix(down[0]), act="relu")
+        else:           # (the experts' rows are as wide as their outputs)
+            wide = torch.zeros((experts, 2 * k, width), device="cuda")
+            wide[:, :, :128] = up
+            x = torch.nn.functional.pad(x, (0, width - 128))
+            got = ops.routed_experts(x, ids.int()[:, None].contiguous(), torch.ones((tokens, 1), device="cuda"), ops.pack_matrix(wide), None, ops.pack_matrix(down), act="relu")
+        sums = torch.einsum("ewk,ek->ew", down.double(), values.double())
+        assert _lost(got, x[:, :1].double() ** 2 * sums[ids]) < 1.3 * half

@@ -47,8 +47,9 @@ static Rows rows_of(int M, int N, int most) {
   const int runs = (M + most - 1) / most, run = ((M + runs - 1) / runs + 15) / 16 * 16;
   return {run, run <= 64 ? 64 : run <= 128 ? 128 : 256, runs};
 }
-// Float32 results of long rows are summed in two accumulators: the tensor cores cut what a sum's 24 bits do not hold, always towards zero, so a
-// sum is off by 7e-8 of itself for every 1024 values of K (14336: 1e-6).
+// Float32 results of long rows are summed in two accumulators, each over half of K: the tensor cores cut what a sum's 24 bits do not hold, always towards zero, and
+// terms of one sign lose 4e-6 of their sum over K = 4096, 1e-5 over 8192, 5e-5 over 28672 in one accumulator (of mixed signs far less).  Halves lose what half of K
+// does.  Hidden values are coded next, to 2^-4 of themselves, and a bfloat16 result rounds to 2^-8: those keep one.
 static bool sums_in_halves(int K, int y_dtype) { return y_dtype == DTYPE_F32 && K > 8192; }
 
 struct ProductWork {
@@ -175,7 +176,8 @@ static int few_experts(Pieces& memory, const Experts& e, const Operand& up, cons
 // type before it is weighted.
 static int experts(Pieces& memory, const Experts& e, const Operand& up, const Operand& down, const Gate& g, int* status, cudaStream_t stream) {
   if (few(e.T, e.top, e.E, e.width, e.ff)) return few_experts(memory, e, up, down, g, status, stream);
-  const int num_slots = e.T * e.top, cap = zb_gemm_tc_experts_run(num_slots, e.E), runs = num_slots / cap + e.E;
+  const bool halves = sums_in_halves(e.ff, e.dtype);               // (two accumulators of up to 128 columns)
+  const int num_slots = e.T * e.top, longest = zb_gemm_tc_experts_run(num_slots, e.E), cap = halves && longest > 128 ? 128 : longest, runs = num_slots / cap + e.E;
   const long long places = static_cast<long long>(runs) * cap;
   const int groups = (cap + 127) / 128;
   int* plan = memory.take<int>(1 + 3LL * runs);
@@ -199,7 +201,7 @@ static int experts(Pieces& memory, const Experts& e, const Operand& up, const Op
                        g.alpha, g.shift, false, parts, flags, LEAST_BLOCKS, status}, stream);
   if (rc != OK) return rc;
   rc = block8_product({out, e.width, e.dtype, nullptr, hidden_codes, hidden_scales, down.codes, down.scales, plan, runs, e.E, 0, cap, cap, down.N, down.K, 0, nullptr, nullptr,
-                       0.0f, 1.0f, 0.0f, false, parts, flags + FLAGS, LEAST_BLOCKS, status}, stream);
+                       0.0f, 1.0f, 0.0f, halves, parts, flags + FLAGS, LEAST_BLOCKS, status}, stream);
   if (rc != OK) return rc;
   return zb_route_combine(e.y, out, e.width, e.dtype, e.x, e.ldx, e.ids, e.weigh_inputs ? nullptr : e.weights, place_of_slot, e.T, e.width, e.top, e.dtype, stream);
 }
