@@ -7,6 +7,7 @@ final norm with the vocabulary projection (reference forward: src/model/causal_l
 from __future__ import annotations
 
 import dataclasses
+from collections import Counter
 from typing import Mapping
 
 import torch
@@ -15,7 +16,7 @@ from ..cache import PagedCacheSpec, StateCacheSpec
 from ..config.errors import ConfigError
 from ..config.spec import LayerSpec, MixerSpec, ModelSpec
 from ..kernels import ops
-from ..weights.loader import WeightDecl, WeightStore, load_weights
+from ..weights.loader import WeightDecl, WeightsOnDemand, WeightStore, load_weights
 from .base import (BLOCKS, FEED_FORWARDS, INPUTS, MIXERS, NORMS, OUTPUTS, SIDES, ResidualStream, StepContext, lookup)
 from .fused import DecodeChains
 
@@ -36,6 +37,18 @@ def _layer_classes(layer: LayerSpec):
             {name: lookup(NORMS, "norm", norm.kind) for name, norm in layer.norms.items()})
 
 
+def _layer_weights(layer: LayerSpec) -> list[dict[str, WeightDecl]]:
+    """What the parts of a layer read, part by part."""
+    _, mixer, ffn, norms = _layer_classes(layer)
+    decls = [mixer.weight_decls(layer.mixer)]
+    if ffn is not None:
+        decls.append(ffn.weight_decls(layer.feed_forward))
+    decls += [norm.weight_decls(layer.norms[name]) for name, norm in norms.items()]
+    if layer.side is not None:
+        decls.append(lookup(SIDES, "side part", layer.side.kind).weight_decls(layer.side))
+    return decls
+
+
 def expected_weights(spec: ModelSpec) -> dict[str, WeightDecl]:
     """Every tensor the model reads, by full name.  A name declared by two parts (a head tied to the
     embedding) must have one shape; it keeps the role of its first declaration."""
@@ -51,14 +64,8 @@ def expected_weights(spec: ModelSpec) -> dict[str, WeightDecl]:
 
     merge(lookup(INPUTS, "input part", spec.input.kind).weight_decls(spec.input))
     for layer in spec.layers:
-        _, mixer, ffn, norms = _layer_classes(layer)
-        merge(mixer.weight_decls(layer.mixer))
-        if ffn is not None:
-            merge(ffn.weight_decls(layer.feed_forward))
-        for name, norm in norms.items():
-            merge(norm.weight_decls(layer.norms[name]))
-        if layer.side is not None:
-            merge(lookup(SIDES, "side part", layer.side.kind).weight_decls(layer.side))
+        for part in _layer_weights(layer):
+            merge(part)
     merge(lookup(OUTPUTS, "output part", spec.output.kind).weight_decls(spec.output))
     return decls
 
@@ -152,7 +159,13 @@ class Model:
         self.input = lookup(INPUTS, "input part", spec.input.kind)(spec.input, weights, dtype)
         self.output = lookup(OUTPUTS, "output part", spec.output.kind)(spec.output, weights, dtype)
         self.layers = []
-        for layer in spec.layers:
+        if spec.weight_bits and (spec.weight_bits != 8 or dtype != torch.bfloat16):
+            raise ConfigError("matrices in fewer bits are built for 8 bits and bfloat16 models")
+        # Matrices that go into 8 bits are packed as soon as their layer is there, and weights that come on demand are let go behind the last layer
+        # that reads them: beside what the model keeps, one layer at a time is held in the model's type.
+        names = [{name for part in _layer_weights(layer) for name in part} for layer in spec.layers]
+        to_come, any_in_8_bits = Counter(name for layer in names for name in layer), False
+        for own, layer in zip(names, spec.layers):
             block, mixer, ffn, norms = _layer_classes(layer)
             extra = {"params": layer.block_params} if layer.block_params else {}
             if layer.side is not None:
@@ -161,8 +174,16 @@ class Model:
                                      ffn(layer.feed_forward, weights, dtype) if ffn is not None else None,
                                      {name: cls(layer.norms[name], weights, dtype) for name, cls in norms.items()},
                                      **extra))
-        if spec.weight_bits:
-            self._hold_in_8_bits()
+            to_come.subtract(own)
+            if spec.weight_bits:
+                made = self.layers[-1]
+                for part in (made.mixer, made.feed_forward):
+                    if part is not None and part.hold_in_8_bits():
+                        any_in_8_bits = True
+            if isinstance(weights, WeightsOnDemand):
+                weights.let_go(name for name in own if to_come[name] == 0)
+        if spec.weight_bits and not any_in_8_bits:
+            raise ConfigError("this model has no matrices that could be held in 8 bits")
         self.cache_specs = cache_specs(spec)
         if len(self.cache_specs) > spec.num_caches:
             self.input.cache_id = spec.num_caches
@@ -188,17 +209,10 @@ class Model:
         self._layer_bytes = None
         self._side_stream = None
 
-    def _hold_in_8_bits(self) -> None:
-        if self.spec.weight_bits != 8 or self.dtype != torch.bfloat16:
-            raise ConfigError("matrices in fewer bits are built for 8 bits and bfloat16 models")
-        found = [part.hold_in_8_bits() for block in self.layers for part in (block.mixer, block.feed_forward) if part is not None]
-        if not any(found):
-            raise ConfigError("this model has no matrices that could be held in 8 bits")
-
     @classmethod
     def load(cls, spec: ModelSpec, store: WeightStore, dtype: torch.dtype, device: torch.device | str) -> "Model":
-        weights = load_weights(store, expected_weights(spec), dtype, device, spec.ignorable_weights)
-        return cls(spec, weights, dtype, device)
+        bring = WeightsOnDemand if spec.weight_bits else load_weights
+        return cls(spec, bring(store, expected_weights(spec), dtype, device, spec.ignorable_weights), dtype, device)
 
     def weight_bytes_read_per_step(self) -> int:
         """Bytes of weights one step reads when every matrix is used once (an embedding table is only

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import hashlib
 from dataclasses import dataclass
-from typing import Mapping, Protocol
+from typing import Iterable, Mapping, Protocol
 
 import torch
 
@@ -98,15 +98,42 @@ def device_dtype(stored: torch.dtype, rank: int, engine_dtype: torch.dtype) -> t
 def load_weights(store: WeightStore, expected: Mapping[str, WeightDecl], dtype: torch.dtype,
                  device: torch.device | str, ignorable: tuple[str, ...] = ()) -> dict[str, torch.Tensor]:
     """Check the store, then bring every expected tensor to ``device`` in its storage type."""
-    if dtype not in (torch.float32, torch.bfloat16):
-        raise WeightError(f"engine dtype must be float32 or bfloat16, not {dtype}")
-    check_store(store, expected, ignorable)
-    out: dict[str, torch.Tensor] = {}
-    for name, decl in expected.items():
-        tensor = store.read(name)
-        target = device_dtype(tensor.dtype, len(decl.shape), dtype)
-        out[name] = tensor.to(device=device, dtype=target).contiguous()
-    return out
+    weights = WeightsOnDemand(store, expected, dtype, device, ignorable)
+    return {name: weights[name] for name in expected}
+
+
+class WeightsOnDemand(Mapping):
+    """The expected tensors on ``device`` in their storage type, the store checked at once, each tensor read when it is first asked for and kept
+    until it is let go: who makes something smaller of a layer's tensors need not hold the others' meanwhile."""
+
+    def __init__(self, store: WeightStore, expected: Mapping[str, WeightDecl], dtype: torch.dtype, device: torch.device | str,
+                 ignorable: tuple[str, ...] = ()):
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise WeightError(f"engine dtype must be float32 or bfloat16, not {dtype}")
+        check_store(store, expected, ignorable)
+        self._store, self._expected, self._dtype, self._device = store, expected, dtype, device
+        self._read: dict[str, torch.Tensor] = {}
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        if name not in self._read:
+            decl = self._expected[name]
+            tensor = self._store.read(name)
+            target = device_dtype(tensor.dtype, len(decl.shape), self._dtype)
+            self._read[name] = tensor.to(device=self._device, dtype=target).contiguous()
+        return self._read[name]
+
+    def __contains__(self, name: object) -> bool:          # (without reading it)
+        return name in self._expected
+
+    def __iter__(self):
+        return iter(self._expected)
+
+    def __len__(self) -> int:
+        return len(self._expected)
+
+    def let_go(self, names: Iterable[str]) -> None:
+        for name in names:
+            self._read.pop(name, None)
 
 
 # ------------------------------------------------------------------ random weights
