@@ -5,6 +5,8 @@ import dataclasses
 import pytest
 import torch
 
+import plain_block8 as plain
+from test_block8_gpu import _close
 from tiny_configs import tiny_config
 from zephyr_b200.config import WeightError
 from zephyr_b200.kernels import ops
@@ -71,3 +73,21 @@ def test_a_model_in_8_bits_is_loaded_a_layer_at_a_time(cuda_device):
             a, b = getattr(getattr(mine, part), name), getattr(getattr(theirs, part), name)
             assert isinstance(a, ops.BlockMatrix) and a.shape == b.shape and torch.equal(a.data, b.data)
     assert torch.equal(model.output.weights_read()[0], other.output.weights_read()[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["A", "B", "D"])
+def test_the_queries_rows_take_no_memory_of_their_own(cuda_device, name):
+    """64, 192 and 512 rows of queries: within a block of 128, with a part of one, whole blocks."""
+    spec = with_weight_bits(tiny_config(name).to_model_spec(), 8)
+    model = Model.load(spec, RandomWeights(expected_weights(spec), 5, device=cuda_device), torch.bfloat16, cuda_device)
+    for layer in model.layers:
+        mixer = layer.mixer
+        queries = mixer.nh * mixer.hd
+        assert mixer.w_q.data is mixer.w_qkv.data and mixer.w_q.shape == (queries, mixer.hidden)
+        assert torch.equal(mixer.w_q.values(), mixer.w_qkv.values()[:queries])
+        values = mixer.w_q.values(torch.float32).double()
+        for m in (1, 12, 50, 300):
+            x = torch.randn((m, mixer.hidden), device=cuda_device, generator=torch.Generator(device="cuda").manual_seed(m))
+            want, magnitude = plain.product(x, values)
+            _close(ops.block_linear(x, mixer.w_q), want, plain.sum_error(mixer.hidden) * magnitude, torch.float32)

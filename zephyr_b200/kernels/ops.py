@@ -2650,6 +2650,11 @@ class BlockMatrix:
     def first_rows(self, rows: int) -> "BlockMatrix":
         """The first rows of one matrix, a multiple of 128 of them, over the same memory."""
         _require(len(self.shape) == 2 and 0 < rows <= self.N and (rows % BLOCK8 == 0 or rows == self.N), "whole blocks of a matrix's rows")
+        return self._leading_rows(rows)
+
+    def _leading_rows(self, rows: int) -> "BlockMatrix":
+        """The first rows of one matrix, any number of them, over the same memory: in their last block other rows' codes lie behind them where the layout
+        has zeros, which the kernels bring along and drop, as they do with zeros."""
         return BlockMatrix(self.data, (rows, self.K), self._total)
 
     def exponents(self) -> torch.Tensor:

@@ -308,8 +308,7 @@ class Attention(Mixer):
     def hold_in_8_bits(self) -> bool:
         queries = self.w_q.shape[0]
         super().hold_in_8_bits()
-        # The queries' rows alone, for a layer that reads another layer's cache: a view where they end with a block.
-        self.w_q = self.w_qkv.first_rows(queries) if queries % ops.BLOCK8 == 0 else ops.pack_matrix(self.w_q)
+        self.w_q = self.w_qkv._leading_rows(queries)     # (for a layer that reads another layer's cache, over the same memory)
         if self.w_gate is not None:          # (its rows are the last ones of w_qkv: how many there are is all that is asked of it)
             self.w_gate = self.w_gate.new_empty((self.w_gate.shape[0], 0))
         return True
