@@ -737,11 +737,11 @@ int block8_launch(const Block8Args& a, long long max_runs, cudaStream_t stream) 
 }
 template <int RUN, typename TOut>
 int block8_form(const Block8Args& a, bool gated, long long max_runs, cudaStream_t stream) {
-  if constexpr (sizeof(TOut) > 1) {
-    if (!gated) return block8_launch<RUN, TOut, false, false>(a, max_runs, stream);
-  }
-  return a.gate.row_scale != nullptr ? block8_launch<RUN, TOut, true, true>(a, max_runs, stream)
-                                     : block8_launch<RUN, TOut, true, false>(a, max_runs, stream);
+  if constexpr (sizeof(TOut) > 1)
+    return gated ? block8_launch<RUN, TOut, true, false>(a, max_runs, stream) : block8_launch<RUN, TOut, false, false>(a, max_runs, stream);
+  else        // (only a routed layer's hidden values take their places' weights)
+    return a.gate.row_scale != nullptr ? block8_launch<RUN, TOut, true, true>(a, max_runs, stream)
+                                       : block8_launch<RUN, TOut, true, false>(a, max_runs, stream);
 }
 template <typename TOut>
 int block8_run(const Block8Args& a, bool gated, long long max_runs, cudaStream_t stream) {
@@ -764,6 +764,7 @@ static bool result_map(CUtensorMap* out, void* y, long long rows, int N, long lo
 // (block8_plan) `max_runs` runs at most of `matrices`, y by place.
 int block8_product(const Block8Product& p, cudaStream_t stream) {
   const bool gated = p.kind >= 1 && p.kind <= 3;
+  if (p.y_scales != nullptr ? !gated : p.row_scale != nullptr) return ERR_BAD_ARGUMENT;
   Block8Args a = {};
   const long long runs = p.plan != nullptr ? p.max_runs : (p.M + p.run - 1) / p.run;
   a.y = p.y; a.y_scales = static_cast<unsigned char*>(p.y_scales); a.ldy = p.ldy; a.N = p.N; a.row_blocks = (p.N + 255) / 256; a.scale_groups = b8_blocks(p.N); a.k_blocks = b8_blocks(p.K); a.pieces = b8_pieces(p.K);
@@ -782,7 +783,7 @@ int block8_product(const Block8Product& p, cudaStream_t stream) {
   const int element = p.y_dtype == DTYPE_F32 ? 4 : 2;
   a.tiled = !gated && p.ldy * element % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
   if (a.tiled && !result_map(&a.y_map, p.y, p.plan != nullptr ? runs * p.cap : p.M, p.N, p.ldy, element)) return ERR_CUDA;
-  if (p.y_scales != nullptr) return gated ? block8_run<unsigned char>(a, gated, runs, stream) : ERR_BAD_ARGUMENT;
+  if (p.y_scales != nullptr) return block8_run<unsigned char>(a, gated, runs, stream);
   return p.y_dtype == DTYPE_F32 ? block8_run<float>(a, gated, runs, stream) : block8_run<__nv_bfloat16>(a, gated, runs, stream);
 }
 
