@@ -134,3 +134,32 @@ def test_long_sums_to_float32_are_taken_in_two_accumulators():
             got = ops.routed_experts(x, ids.int()[:, None].contiguous(), torch.ones((tokens, 1), device="cuda"), ops.pack_matrix(wide), None, ops.pack_matrix(down), act="relu")
         sums = torch.einsum("ewk,ek->ew", down.double(), values.double())
         assert _lost(got, x[:, :1].double() ** 2 * sums[ids]) < 1.3 * half
+
+
+# ------------------------------------------------------------------------------------------------- choices that other tests do not make
+@pytest.mark.parametrize("tokens,experts,top", [(5, 64, 40), (50, 64, 40), (3, 5, 3), (30, 5, 3)])
+@pytest.mark.parametrize("chosen", ["any", "none", "one"])
+def test_many_choices_a_token_and_tokens_without_an_expert(tokens, experts, top, chosen):
+    """More choices than a warp has lanes; ids outside the experts on either side, which stand for the token itself; no expert at all; all on the last one."""
+    width, ff = 136, 72
+    x = _random((tokens, width), 70, dtype=torch.bfloat16)
+    raw_up, raw_down = _random((experts, 2 * ff, width), 71, 0.1), _random((experts, width, ff), 72, 0.1)
+    up, down = ops.pack_matrix(raw_up), ops.pack_matrix(raw_down)
+    ids = torch.stack([torch.randperm(experts + 4, generator=torch.Generator().manual_seed(t))[:top] for t in range(tokens)]).cuda() - 2      # from -2 to experts + 1
+    if chosen == "none":
+        ids = torch.where(ids % 2 == 0, -1, experts + 7)
+    elif chosen == "one":
+        ids = torch.full_like(ids, experts - 1)
+    ids, weights = ids.int().contiguous(), (_random((tokens, top), 73).abs() / top).contiguous()
+    got = ops.routed_experts(x, ids, weights, up, None, down)
+    want, error = torch.zeros((tokens, width), dtype=F64, device="cuda"), torch.zeros((tokens, width), dtype=F64, device="cuda")
+    for e in ids.unique().tolist():
+        token, choice = torch.nonzero(ids == e, as_tuple=True)
+        weight = weights[token, choice].double()[:, None]
+        y, off = x[token].double(), torch.zeros((len(token), width), dtype=F64, device="cuda")
+        if 0 <= e < experts:
+            y, off = _feed_forward(x[token], plain.code_blocks(raw_up[e], 128)[0], plain.code_blocks(raw_down[e], 128)[0], "silu")
+            off = off + HALF_STEP[torch.bfloat16] * (y.abs() + off)
+        want.index_add_(0, token, weight * y)
+        error.index_add_(0, token, weight * off + (top + 2) * 2.0 ** -24 * (weight * y).abs())
+    _close(got, want, error * (1 + 2.0 ** -20) + top * 2.0 ** -24 * want.abs(), torch.bfloat16)
