@@ -108,9 +108,9 @@ pack_matrix_kernel(unsigned char* codes, unsigned char* scales, unsigned char* e
   }
 }
 
-// Stands behind a kernel that writes a matrix.  The products for few rows read codes and scales ahead of their wait for earlier kernels, and a kernel that does
-// not say when its dependents may start lets them start when its CTAs have ended, which is before all that they wrote has to be visible.  This one
-// waits for that, and whatever is launched as its dependent starts no earlier.
+// Stands behind a kernel that writes a matrix.  The products for few rows read codes and scales ahead of their wait for earlier kernels, and a kernel
+// that does not say when its dependents may start lets them start when its CTAs have ended, which is before all that they wrote has to be visible.  This one waits
+// for that, and whatever is launched as its dependent starts no earlier.  (It costs a call 2 us on the host and 0.5 on the device.)
 __global__ void matrix_ready_kernel() {
   wait_for_prior_grids();
   let_dependents_launch();

@@ -33,8 +33,8 @@ __host__ __device__ inline int b8_pitch(int k) { return b8_blocks(k) * B8_BLOCK;
 constexpr int G8_PAIRS = 74;           // of SMs: the most that the product for many rows takes
 
 // Whether the pairs share all tiles' blocks of K evenly instead of taking whole tiles: where the rounds of whole tiles leave more of the pairs
-// without work than the parts cost to be handed over (7 to 10 us; 1024 rows, 5120 x 25600 219 -> 119 us, 17 rows, 4096 x 12288
-// 26.0 -> 18.4).  In blocks of K on a pair, which take longer the more columns a tile has.
+// without work than the parts cost to be handed over (7 to 10 us; 1024 rows, 5120 x 25600 152 -> 119 us, 17 rows, 4096 x 12288
+// 34 -> 20 to 23).  In blocks of K on a pair, which take longer the more columns a tile has.
 __host__ __device__ inline bool b8_in_parts(long long items, int k_blocks, int cap) {
   const long long rounds = (items + G8_PAIRS - 1) / G8_PAIRS;
   const long long whole = rounds * k_blocks, even = (items * k_blocks + G8_PAIRS - 1) / G8_PAIRS;

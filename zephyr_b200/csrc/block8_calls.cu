@@ -48,7 +48,7 @@ static Rows rows_of(int M, int N, int most) {
   return {run, run <= 64 ? 64 : run <= 128 ? 128 : 256, runs};
 }
 // Float32 results of long rows are summed in two accumulators, each over half of K: the tensor cores cut what a sum's 24 bits do not hold, always towards zero, and
-// terms of one sign lose 4e-6 of their sum over K = 4096, 1e-5 over 8192, 5e-5 over 28672 in one accumulator (of mixed signs far less).  Halves lose what half of K
+// terms of one sign lose 4e-6 of their sum over K = 4096, 1e-5 over 8192, 5e-5 over 28672 in one accumulator (normal draws 5e-7 of the result over 8192).  Halves lose what half of K
 // does.  Hidden values are coded next, to 2^-4 of themselves, and a bfloat16 result rounds to 2^-8: those keep one.
 static bool sums_in_halves(int K, int y_dtype) { return y_dtype == DTYPE_F32 && K > 8192; }
 

@@ -57,9 +57,10 @@ __device__ __forceinline__ void stream_block(const unsigned char* rows, const un
   }
 }
 
-// acc += a block's sums times its scales; `x_scale`: the block's, a column each.  Sums are zero or of 2^-18 to 2^25, and multiples of 2^-18, so that either scale
-// leaves them exact (below float32's normal numbers too), but one of the two may leave its range where both together do not.  So the matrix's comes first where it is
-// not large, and else the row's: what is infinite then is so with both.
+// acc += a block's sums times its scales; `x_scale`: the block's, a column each.  Sums are zero or of 2^-18 to 2^25, and multiples of 2^-18, so that
+// either scale leaves them exact (below float32's normal numbers too), but one of the two may leave its range where both together do not.  So the matrix's comes
+// first where it is not large, and else the row's: what is infinite then is so with both.  (8 x 4096 x 4096 6.5 -> 6.6 us against the
+// matrix's always first, experts of 8 tokens 43.3 -> 43.8; with a branch in the selection's place 16 rows of 10240 x 5120 16.4, here 16.3.)
 template <int MT>
 __device__ __forceinline__ void add_scaled(float (&acc)[MT][4], const float (&sum)[MT][4], float w, const float* x_scale) {
   const int t = threadIdx.x & 3;

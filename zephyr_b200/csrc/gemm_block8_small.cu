@@ -9,8 +9,8 @@
 //
 // One CTA an SM walks tiles of 16 rows; a team of TEAM of its 16 warps shares a tile, each a slice of the blocks of K.  x lies in shared memory as
 // codes; the matrix passes through a ring of two blocks of 16 x 128 a warp, each one tiled copy (128-byte swizzle) that the warp's first lane asks
-// for, the first ones before the kernel ahead has finished: no kernel that may still run writes a matrix (matrix_ready_kernel).  64 registers a thread and less than half of shared
-// memory let the next kernel's CTA lie beside this one's with its first copies on their way.  Partial sums meet in shared memory, in two buffers that
+// for, the first ones before the kernel ahead has finished: no kernel that may still run writes a matrix (matrix_ready_kernel).  64 registers a
+// thread and less than half of shared memory let the next kernel's CTA lie beside this one's with its first copies on their way.  Partial sums meet in shared memory, in two buffers that
 // take turns, and are added in a fixed order.
 #include <algorithm>
 #include <atomic>

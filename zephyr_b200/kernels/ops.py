@@ -2681,7 +2681,7 @@ class BlockMatrix:
 
 def pack_matrix(w: torch.Tensor) -> BlockMatrix:
     """``w`` [N, K] or [matrices, N, K], bfloat16 or float32 with contiguous rows, in 8-bit floating point with a scale for each block of
-    128 x 128 (``BlockMatrix``)."""
+    128 x 128 (``BlockMatrix``).  Calls that follow on the stream may take it at once: a second small kernel lets none of them start before it is complete."""
     shape = w.shape
     if len(shape) not in (2, 3) or w.numel() == 0 or w.dtype not in DTYPE_CODE or (w.stride(-1) != 1 and shape[-1] != 1):
         raise InvalidArgumentError("w [N, K] or [matrices, N, K], not empty, bfloat16 or float32 with unit inner stride")
